@@ -106,16 +106,15 @@ def draw(rng):
         pages = slots * -(-longest // page) + _log(rng, 64, 4096)
         return {"kind": kind, "dtype": dtype, "slots": slots, "longest": longest, **pool, "pages": pages}
     layers = rng.randint(1, 30)
-    row = layers * kv_heads * dim * BYTES[dtype]
+    row = kv_heads * dim * BYTES[dtype]
+    most = 400_000_000 // (page * row)  # pages of one layer that a pool of 400 MB holds
     if kind == "fork":
         parents, branches, longest = _log(rng, 1, 16), _log(rng, 1, 16), _log(rng, 2, 1500)
-        room = max(1, 400_000_000 // (page * row) // parents - branches - 1)
-        longest = min(longest, max(2, room * page - 1))
         pages = parents * (-(-longest // page) + branches) + 8
         return {"kind": kind, "dtype": dtype, "parents": parents, "branches": branches, "longest": longest,
-                "layers": layers, **pool, "pages": pages}
-    pages = min(_log(rng, 32, 4096), max(32, 400_000_000 // (page * row)))
-    layers = max(1, min(layers, 400_000_000 // (page * pages * (row // layers))))
+                "layers": max(1, min(layers, most // pages)), **pool, "pages": pages}
+    pages = min(_log(rng, 32, 4096), max(32, most // layers))
+    layers = max(1, min(layers, most // pages))
     if kind == "copy":
         return {"kind": kind, "dtype": dtype, "pages": pages, "copies": _log(rng, 1, pages // 2), "layers": layers, **pool}
     if kind == "compact":
