@@ -98,8 +98,9 @@ def draw(rng):
         keys = min(keys, most // queries)
         if queries > 1 and dim > 128:
             dim = 128
+        widest = 4 * 32 * 4096 * 700 * 128 // (batch * query_heads * queries * dim)
         return {"kind": kind, "dtype": dtype, "batch": batch, "query_heads": query_heads, "kv_heads": kv_heads,
-                "dim": dim, "queries": queries, "keys": keys, "window": _log(rng, 16, 2048),
+                "dim": dim, "queries": queries, "keys": keys, "window": min(_log(rng, 16, 2048), widest),
                 "sinks": rng.choice((0, 1, 4, 64)), "padded": queries == keys}
     if kind == "admit":
         slots, longest = _log(rng, 1, 64), _log(rng, 4, 2000)
