@@ -98,7 +98,7 @@ def draw(rng):
         keys = min(keys, most // queries)
         if queries > 1 and dim > 128:
             dim = 128
-        widest = 4 * 32 * 4096 * 700 * 128 // (batch * query_heads * queries * dim)
+        widest = 4 * 32 * 4096 * 500 * 128 // (batch * query_heads * queries * dim)
         return {"kind": kind, "dtype": dtype, "batch": batch, "query_heads": query_heads, "kv_heads": kv_heads,
                 "dim": dim, "queries": queries, "keys": keys, "window": min(_log(rng, 16, 2048), widest),
                 "sinks": rng.choice((0, 1, 4, 64)), "padded": queries == keys}
