@@ -357,7 +357,7 @@ def _admit(s, case):
         from flux_amd import ops
 
         ops.paged_cache_free_native(*state, s["slots"])
-        positions, status = ops.paged_cache_reserve_native(*state, s["slots"], s["counts"])
+        positions, status = ops.paged_cache_reserve_native(*state, case["page"], s["slots"], s["counts"])
         ops.paged_cache_write_native(s["key"], s["value"], *pools, s["table"], s["slots"], positions, s["counts"])
         return [*pools, *state, positions, status]
     _release(*state, s["slots"])
