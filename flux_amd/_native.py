@@ -106,6 +106,22 @@ class LayerDecodeBuffers(ctypes.Structure):
     ]
 
 
+class PageBooks(ctypes.Structure):
+    _fields_ = [("page_table", _vp), ("table_stride", ctypes.c_int64), ("slots", ctypes.c_int64),
+                ("columns", ctypes.c_int64), ("lengths", _vp), ("refcounts", _vp), ("pages", ctypes.c_int64),
+                ("page_size", ctypes.c_int64)]
+
+
+class PagePool(ctypes.Structure):
+    _fields_ = [("key", _vp), ("value", _vp), ("layers", ctypes.c_int64), ("pages", ctypes.c_int64),
+                ("heads", ctypes.c_int64), ("page_size", ctypes.c_int64), ("head_dim", ctypes.c_int64),
+                ("key_strides", ctypes.c_int64 * 4), ("value_strides", ctypes.c_int64 * 4), ("dtype", ctypes.c_int64)]
+
+
+_books = ctypes.POINTER(PageBooks)
+_pool = ctypes.POINTER(PagePool)
+_n = ctypes.c_int64
+
 # (name, restype, argtypes) for every exported symbol.
 _PROTOTYPES: list[tuple[str, Any, list[Any]]] = [
     ("flux_last_error", ctypes.c_char_p, []),
@@ -193,6 +209,25 @@ _PROTOTYPES: list[tuple[str, Any, list[Any]]] = [
     ("flux_gqa_decode_attention_strided_f32", ctypes.c_int,
      [_vp, _vp, _vp, _vp, _vp, _vp, _vp, ctypes.c_int64, ctypes.c_float, ctypes.c_int64, ctypes.c_int64,
       ctypes.c_int64, ctypes.c_int64, _i64, _i64, _i64, _i64, _i64, _stream]),
+    ("flux_paged_decode_attention_workspace_bytes", ctypes.c_int, [_n] * 7 + [_i64]),
+    ("flux_paged_decode_attention", ctypes.c_int,
+     [ctypes.c_int] + [_vp] * 8 + [_n, ctypes.c_float] + [_n] * 11 + [_i64, _i64, _i64, _stream]),
+    ("flux_window_attention_workspace_bytes", ctypes.c_int, [_n] * 8 + [_i64]),
+    ("flux_window_attention", ctypes.c_int,
+     [ctypes.c_int] + [_vp] * 7 + [_n, ctypes.c_float] + [_n] * 8 + [_i64, _i64, _i64, _stream]),
+    ("flux_page_reserve_workspace_words", ctypes.c_int, [_n, _n, _n, _i64]),
+    ("flux_page_reserve", ctypes.c_int, [_books, _vp, _vp, _n, _vp, _vp, _vp, _n, _stream]),
+    ("flux_page_write", ctypes.c_int,
+     [_pool, _vp, _vp, _i64, _i64, _n, _n, _vp, _n, _n, _n, _vp, _vp, _vp, _stream]),
+    ("flux_page_copy", ctypes.c_int, [_pool, _vp, _vp, _n, _vp, _stream]),
+    ("flux_page_free", ctypes.c_int, [_books, _vp, _n, _vp, _stream]),
+    ("flux_page_fork_workspace_words", ctypes.c_int, [_n, _n, _n, _i64]),
+    ("flux_page_fork", ctypes.c_int, [_pool, _books, _vp, _vp, _n, _vp, _vp, _n, _stream]),
+    ("flux_page_compact_workspace_words", ctypes.c_int, [_n, _i64]),
+    ("flux_page_compact", ctypes.c_int, [_pool, _books, _vp, _vp, _vp, _n, _stream]),
+    ("flux_logits_process_workspace_bytes", ctypes.c_int, [_n, _n, _i64]),
+    ("flux_logits_process", ctypes.c_int,
+     [ctypes.c_int, _vp, _n, _vp, _vp, _n, _n, _vp, _n, _n, _vp, _vp, _vp, _vp, _vp, _n, _vp, _n, _vp, _n, _stream]),
 ]
 
 EXPORTED_SYMBOLS = tuple(name for name, _, _ in _PROTOTYPES)

@@ -4,6 +4,7 @@
 
 #include "flux_kernels.h"
 #include "runtime.h"
+#include "serving.h"
 
 #include <cmath>
 #include <cstdint>
@@ -666,6 +667,354 @@ int flux_gqa_decode_attention_strided_f32(const float* query, const float* key_c
                (key_strides[2] & 3) == 0 && (value_strides[1] & 3) == 0 && (value_strides[2] & 3) == 0 &&
                aligned16(key_cache) && aligned16(value_cache);
     return from_hip(flux::launch_gqa_strided(args, stream), "flux_gqa_decode_attention_strided_f32");
+}
+
+// ---------------------------------------------------------------------------
+// Serving operators.
+
+namespace {
+
+bool known_type(int64_t dtype) { return dtype >= FLUX_FLOAT32 && dtype <= FLUX_BFLOAT16; }
+
+// Whether every row starts at 16 bytes and fills whole 16-byte quads.
+bool wide_rows(const void* base, const int64_t* strides, int count, int64_t dim, int element) {
+    if (!aligned16(base) || dim * element % 16) return false;
+    for (int i = 0; i < count; ++i)
+        if (strides[i] * element % 16) return false;
+    return true;
+}
+
+// What both attention operators share; null when the arguments are in order.
+const char* attention_arguments(flux::AttentionArgs& args, int dtype, const void* query, const void* key,
+                                const void* value, void* output, float scale, int64_t batch, int64_t query_heads,
+                                int64_t kv_heads, int64_t queries, int64_t keys, int64_t head_dim, int64_t window,
+                                int64_t sinks, const int64_t* query_strides, const int64_t* key_strides,
+                                const int64_t* value_strides) {
+    if (!query || !key || !value || !output || !query_strides || !key_strides || !value_strides) return "null argument";
+    if (!known_type(dtype)) return "unknown dtype";
+    if (batch <= 0 || query_heads <= 0 || kv_heads <= 0 || query_heads % kv_heads || batch > 65535 ||
+        query_heads > 65535 || batch * query_heads > (int64_t{1} << 23) || head_dim <= 0 ||
+        head_dim > flux::kServingMaxDim || keys <= 0 || keys > FLUX_MAX_SERVING_KEYS || queries <= 0 ||
+        queries > FLUX_MAX_SERVING_KEYS || queries * (query_heads / kv_heads) > (int64_t{1} << 27))
+        return "invalid shape";
+    if (window < 0 || sinks < 0 || window > FLUX_MAX_SERVING_KEYS || sinks > FLUX_MAX_SERVING_KEYS)
+        return "window and sinks must be within [0, FLUX_MAX_SERVING_KEYS]";
+    if (!std::isfinite(scale)) return "scale must be finite";
+    if (!nonnegative(query_strides, 4) || !nonnegative(key_strides, 3) || !nonnegative(value_strides, 3))
+        return "negative strides are unsupported";
+    const auto type = static_cast<flux::Type>(dtype);
+    args.query = query;
+    args.key = key;
+    args.value = value;
+    args.out = output;
+    args.scale = scale;
+    args.batch = static_cast<int>(batch);
+    args.query_heads = static_cast<int>(query_heads);
+    args.kv_heads = static_cast<int>(kv_heads);
+    args.group = static_cast<int>(query_heads / kv_heads);
+    args.dim = static_cast<int>(head_dim);
+    args.queries = static_cast<int>(queries);
+    args.keys = keys;
+    args.window = static_cast<int>(window);
+    args.sinks = static_cast<int>(sinks);
+    for (int i = 0; i < 4; ++i) args.query_strides[i] = query_strides[i];
+    for (int i = 0; i < 3; ++i) {
+        args.key_strides[i] = key_strides[i];
+        args.value_strides[i] = value_strides[i];
+    }
+    args.wide = wide_rows(key, key_strides, 3, head_dim, flux::type_bytes(type)) &&
+                wide_rows(value, value_strides, 3, head_dim, flux::type_bytes(type));
+    args.blocks = flux::decode_attention_blocks(args.batch, keys, args.kv_heads, args.group, args.window, args.sinks);
+    return nullptr;
+}
+
+const char* pool_arguments(flux::PagePool& out, const flux_page_pool* pool) {
+    if (!pool || !pool->key || !pool->value) return "null cache";
+    if (!known_type(pool->dtype)) return "unknown dtype";
+    if (pool->layers <= 0 || pool->layers > 32000 || pool->pages <= 0 || pool->pages > (1 << 28) || pool->heads <= 0 ||
+        pool->page_size <= 0 || pool->page_size > FLUX_MAX_SERVING_KEYS || pool->head_dim <= 0 ||
+        pool->head_dim > (1 << 20) || pool->heads > (1 << 20) ||
+        pool->heads * pool->page_size > (int64_t{1} << 28) / pool->head_dim)
+        return "invalid cache shape";
+    if (!nonnegative(pool->key_strides, 4) || !nonnegative(pool->value_strides, 4))
+        return "negative strides are unsupported";
+    out.key = static_cast<char*>(pool->key);
+    out.value = static_cast<char*>(pool->value);
+    out.layers = pool->layers;
+    out.pages = pool->pages;
+    out.heads = pool->heads;
+    out.page = pool->page_size;
+    out.dim = pool->head_dim;
+    out.element = flux::type_bytes(static_cast<flux::Type>(pool->dtype));
+    for (int i = 0; i < 4; ++i) {
+        out.key_strides[i] = pool->key_strides[i];
+        out.value_strides[i] = pool->value_strides[i];
+    }
+    return nullptr;
+}
+
+const char* books_arguments(flux::PageBooks& out, const flux_page_books* books, int64_t requests) {
+    if (!books || !books->page_table || !books->lengths || !books->refcounts) return "null books";
+    if (books->slots <= 0 || books->slots > (1 << 28) || books->columns <= 0 || books->table_stride < 0 ||
+        books->pages <= 0 || books->pages > (1 << 28) || books->page_size <= 0 ||
+        books->page_size > FLUX_MAX_SERVING_KEYS || books->columns > FLUX_MAX_SERVING_KEYS / books->page_size)
+        return "invalid books (columns * page_size is at most FLUX_MAX_SERVING_KEYS)";
+    if (requests <= 0 || requests > (1 << 20) || requests * books->columns >= (int64_t{1} << 31))
+        return "invalid number of requests";
+    out.table = books->page_table;
+    out.table_stride = books->table_stride;
+    out.slots = books->slots;
+    out.columns = books->columns;
+    out.lengths = books->lengths;
+    out.refcounts = books->refcounts;
+    out.pages = books->pages;
+    out.page = books->page_size;
+    return nullptr;
+}
+
+}  // namespace
+
+int flux_paged_decode_attention_workspace_bytes(int64_t batch, int64_t query_heads, int64_t kv_heads, int64_t head_dim,
+                                                int64_t keys, int64_t window, int64_t sinks, int64_t* bytes) {
+    flux::AttentionArgs args{};
+    const int64_t strides[4] = {};
+    void* const some = &args;
+    if (!bytes || attention_arguments(args, FLUX_FLOAT32, some, some, some, some, 1.0f, batch, query_heads, kv_heads, 1,
+                                      keys, head_dim, window, sinks, strides, strides, strides))
+        return invalid("flux_paged_decode_attention_workspace_bytes: invalid argument");
+    *bytes = static_cast<int64_t>(flux::decode_attention_workspace_floats(args) * sizeof(float));
+    return FLUX_OK;
+}
+
+int flux_paged_decode_attention(int dtype, const void* query, const void* key_pages, const void* value_pages,
+                                const int32_t* page_table, const int64_t* lengths, const int64_t* slots, void* output,
+                                void* workspace, int64_t workspace_bytes, float scale, int64_t batch,
+                                int64_t query_heads, int64_t kv_heads, int64_t head_dim, int64_t pages,
+                                int64_t page_size, int64_t slot_count, int64_t columns, int64_t table_stride,
+                                int64_t window, int64_t sinks, const int64_t* query_strides,
+                                const int64_t* key_strides, const int64_t* value_strides, hipStream_t stream) {
+    if (!page_table || !workspace) return invalid("flux_paged_decode_attention: null argument");
+    if (pages <= 0 || pages > (1 << 28) || page_size <= 0 || page_size > FLUX_MAX_SERVING_KEYS || slot_count <= 0 ||
+        columns <= 0 || columns > FLUX_MAX_SERVING_KEYS / page_size || table_stride < 0)
+        return invalid("flux_paged_decode_attention: invalid pages (columns * page_size is at most "
+                       "FLUX_MAX_SERVING_KEYS)");
+    flux::AttentionArgs args{};
+    if (const char* wrong = attention_arguments(args, dtype, query, key_pages, value_pages, output, scale, batch,
+                                                query_heads, kv_heads, 1, columns * page_size, head_dim, window, sinks,
+                                                query_strides, key_strides, value_strides))
+        return invalid(std::string("flux_paged_decode_attention: ") + wrong);
+    if (!slots && slot_count < batch) return invalid("flux_paged_decode_attention: fewer table rows than sequences");
+    if (workspace_bytes < static_cast<int64_t>(flux::decode_attention_workspace_floats(args) * sizeof(float)))
+        return invalid("flux_paged_decode_attention: workspace too small (flux_paged_decode_attention_workspace_bytes)");
+    args.workspace = static_cast<float*>(workspace);
+    args.table = page_table;
+    args.lengths = lengths;
+    args.slots = slots;
+    args.slot_count = slot_count;
+    args.pages = pages;
+    args.page = flux::make_divider(static_cast<uint32_t>(page_size));
+    args.table_stride = table_stride;
+    return from_hip(flux::launch_decode_attention(args, static_cast<flux::Type>(dtype), stream),
+                    "flux_paged_decode_attention");
+}
+
+int flux_window_attention_workspace_bytes(int64_t batch, int64_t query_heads, int64_t kv_heads, int64_t queries,
+                                          int64_t head_dim, int64_t keys, int64_t window, int64_t sinks,
+                                          int64_t* bytes) {
+    flux::AttentionArgs args{};
+    const int64_t strides[4] = {};
+    void* const some = &args;
+    if (!bytes || attention_arguments(args, FLUX_FLOAT32, some, some, some, some, 1.0f, batch, query_heads, kv_heads,
+                                      queries, keys, head_dim, window, sinks, strides, strides, strides))
+        return invalid("flux_window_attention_workspace_bytes: invalid argument");
+    *bytes = queries > 1 ? 0 : static_cast<int64_t>(flux::decode_attention_workspace_floats(args) * sizeof(float));
+    return FLUX_OK;
+}
+
+int flux_window_attention(int dtype, const void* query, const void* key, const void* value, const int64_t* lengths,
+                          const int64_t* starts, void* output, void* workspace, int64_t workspace_bytes, float scale,
+                          int64_t batch, int64_t query_heads, int64_t kv_heads, int64_t queries, int64_t keys,
+                          int64_t head_dim, int64_t window, int64_t sinks, const int64_t* query_strides,
+                          const int64_t* key_strides, const int64_t* value_strides, hipStream_t stream) {
+    flux::AttentionArgs args{};
+    if (const char* wrong = attention_arguments(args, dtype, query, key, value, output, scale, batch, query_heads,
+                                                kv_heads, queries, keys, head_dim, window, sinks, query_strides,
+                                                key_strides, value_strides))
+        return invalid(std::string("flux_window_attention: ") + wrong);
+    args.lengths = lengths;
+    args.starts = starts;
+    args.slot_count = batch;
+    const auto type = static_cast<flux::Type>(dtype);
+    if (queries > 1) return from_hip(flux::launch_window_attention(args, type, stream), "flux_window_attention");
+    if (!workspace ||
+        workspace_bytes < static_cast<int64_t>(flux::decode_attention_workspace_floats(args) * sizeof(float)))
+        return invalid("flux_window_attention: workspace missing or too small (flux_window_attention_workspace_bytes)");
+    args.workspace = static_cast<float*>(workspace);
+    return from_hip(flux::launch_decode_attention(args, type, stream), "flux_window_attention");
+}
+
+int flux_page_reserve_workspace_words(int64_t requests, int64_t slots, int64_t pages, int64_t* words) {
+    if (!words || requests <= 0 || slots <= 0 || pages <= 0)
+        return invalid("flux_page_reserve_workspace_words: invalid argument");
+    *words = static_cast<int64_t>(flux::page_reserve_workspace(requests, slots, pages));
+    return FLUX_OK;
+}
+
+int flux_page_reserve(const flux_page_books* books, const int64_t* slots, const int64_t* counts, int64_t requests,
+                      int64_t* positions, int32_t* status, int32_t* workspace, int64_t workspace_words,
+                      hipStream_t stream) {
+    flux::PageBooks b{};
+    if (const char* wrong = books_arguments(b, books, requests))
+        return invalid(std::string("flux_page_reserve: ") + wrong);
+    if (!slots || !positions || !status || !workspace) return invalid("flux_page_reserve: null argument");
+    if (workspace_words < static_cast<int64_t>(flux::page_reserve_workspace(requests, b.slots, b.pages)))
+        return invalid("flux_page_reserve: workspace too small (flux_page_reserve_workspace_words)");
+    return from_hip(flux::launch_page_reserve(b, slots, counts, requests, positions, status, workspace, stream),
+                    "flux_page_reserve");
+}
+
+int flux_page_write(const flux_page_pool* pool, const void* key, const void* value, const int64_t* key_strides,
+                    const int64_t* value_strides, int64_t requests, int64_t tokens, const int32_t* page_table,
+                    int64_t table_stride, int64_t slots, int64_t columns, const int64_t* slot_list,
+                    const int64_t* positions, const int64_t* counts, hipStream_t stream) {
+    flux::PagePool p{};
+    if (const char* wrong = pool_arguments(p, pool)) return invalid(std::string("flux_page_write: ") + wrong);
+    if (!key || !value || !key_strides || !value_strides || !page_table || !slot_list || !positions)
+        return invalid("flux_page_write: null argument");
+    if (p.layers != 1) return invalid("flux_page_write: one layer is written at a time");
+    if (requests <= 0 || requests > 65535 || tokens <= 0 || tokens > FLUX_MAX_SERVING_KEYS || slots <= 0 ||
+        columns <= 0 || columns > FLUX_MAX_SERVING_KEYS / p.page || table_stride < 0 ||
+        p.heads > (int64_t{1} << 24) / p.dim)
+        return invalid("flux_page_write: invalid shape");
+    if (!nonnegative(key_strides, 3) || !nonnegative(value_strides, 3))
+        return invalid("flux_page_write: negative strides are unsupported");
+    flux::PageWriteArgs args{};
+    args.key = static_cast<const char*>(key);
+    args.value = static_cast<const char*>(value);
+    for (int i = 0; i < 3; ++i) {
+        args.key_strides[i] = key_strides[i];
+        args.value_strides[i] = value_strides[i];
+    }
+    args.requests = requests;
+    args.tokens = tokens;
+    args.table = page_table;
+    args.table_stride = table_stride;
+    args.slots = slots;
+    args.columns = columns;
+    args.slot_list = slot_list;
+    args.positions = positions;
+    args.counts = counts;
+    return from_hip(flux::launch_page_write(p, args, stream), "flux_page_write");
+}
+
+int flux_page_copy(const flux_page_pool* pool, const int64_t* source, const int64_t* target, int64_t requests,
+                   int32_t* status, hipStream_t stream) {
+    flux::PagePool p{};
+    if (const char* wrong = pool_arguments(p, pool)) return invalid(std::string("flux_page_copy: ") + wrong);
+    if (!source || !target || !status || requests <= 0 || requests > (1 << 20))
+        return invalid("flux_page_copy: invalid argument");
+    return from_hip(flux::launch_page_copy(p, source, target, requests, status, stream), "flux_page_copy");
+}
+
+int flux_page_free(const flux_page_books* books, const int64_t* slots, int64_t requests, int32_t* status,
+                   hipStream_t stream) {
+    flux::PageBooks b{};
+    if (const char* wrong = books_arguments(b, books, requests)) return invalid(std::string("flux_page_free: ") + wrong);
+    if (!slots || !status) return invalid("flux_page_free: null argument");
+    return from_hip(flux::launch_page_free(b, slots, requests, status, stream), "flux_page_free");
+}
+
+int flux_page_fork_workspace_words(int64_t requests, int64_t slots, int64_t pages, int64_t* words) {
+    if (!words || requests <= 0 || slots <= 0 || pages <= 0)
+        return invalid("flux_page_fork_workspace_words: invalid argument");
+    *words = static_cast<int64_t>(flux::page_fork_workspace(requests, slots, pages));
+    return FLUX_OK;
+}
+
+int flux_page_fork(const flux_page_pool* pool, const flux_page_books* books, const int64_t* parents,
+                   const int64_t* children, int64_t requests, int32_t* status, int32_t* workspace,
+                   int64_t workspace_words, hipStream_t stream) {
+    flux::PagePool p{};
+    flux::PageBooks b{};
+    if (const char* wrong = pool_arguments(p, pool)) return invalid(std::string("flux_page_fork: ") + wrong);
+    if (const char* wrong = books_arguments(b, books, requests)) return invalid(std::string("flux_page_fork: ") + wrong);
+    if (b.pages != p.pages || b.page != p.page) return invalid("flux_page_fork: books and cache differ in their pages");
+    if (!parents || !children || !status || !workspace) return invalid("flux_page_fork: null argument");
+    if (workspace_words < static_cast<int64_t>(flux::page_fork_workspace(requests, b.slots, b.pages)))
+        return invalid("flux_page_fork: workspace too small (flux_page_fork_workspace_words)");
+    return from_hip(flux::launch_page_fork(p, b, parents, children, requests, status, workspace, stream),
+                    "flux_page_fork");
+}
+
+int flux_page_compact_workspace_words(int64_t pages, int64_t* words) {
+    if (!words || pages <= 0) return invalid("flux_page_compact_workspace_words: invalid argument");
+    *words = static_cast<int64_t>(flux::page_compact_workspace(pages));
+    return FLUX_OK;
+}
+
+int flux_page_compact(const flux_page_pool* pool, const flux_page_books* books, int32_t* page_map, int64_t* used,
+                      int32_t* workspace, int64_t workspace_words, hipStream_t stream) {
+    flux::PagePool p{};
+    if (const char* wrong = pool_arguments(p, pool)) return invalid(std::string("flux_page_compact: ") + wrong);
+    if (!books || !books->page_table || !books->refcounts || !page_map || !used || !workspace)
+        return invalid("flux_page_compact: null argument");
+    if (books->pages != p.pages || books->slots <= 0 || books->columns <= 0 || books->table_stride < 0 ||
+        books->columns > (int64_t{1} << 40) / books->slots)
+        return invalid("flux_page_compact: invalid books");
+    if (workspace_words < static_cast<int64_t>(flux::page_compact_workspace(p.pages)))
+        return invalid("flux_page_compact: workspace too small (flux_page_compact_workspace_words)");
+    flux::PageBooks b{};
+    b.table = books->page_table;
+    b.table_stride = books->table_stride;
+    b.slots = books->slots;
+    b.columns = books->columns;
+    b.refcounts = books->refcounts;
+    b.pages = p.pages;
+    b.page = p.page;
+    return from_hip(flux::launch_page_compact(p, b, page_map, used, workspace, stream), "flux_page_compact");
+}
+
+int flux_logits_process_workspace_bytes(int64_t rows, int64_t vocab, int64_t* bytes) {
+    if (!bytes || rows <= 0 || vocab <= 0) return invalid("flux_logits_process_workspace_bytes: invalid argument");
+    *bytes = static_cast<int64_t>(flux::logits_workspace_bytes(rows, vocab));
+    return FLUX_OK;
+}
+
+int flux_logits_process(int dtype, const void* logits, int64_t logits_stride, void* output, int64_t* tokens,
+                        int64_t rows, int64_t vocab, const int64_t* history, int64_t history_width,
+                        int64_t history_stride, const int64_t* history_lengths, const float* repetition,
+                        const float* frequency, const float* presence, const float* bias, int64_t bias_stride,
+                        const int32_t* allowed, int64_t allowed_stride, void* workspace, int64_t workspace_bytes,
+                        hipStream_t stream) {
+    if (!logits || !output || !tokens) return invalid("flux_logits_process: null argument");
+    if (!known_type(dtype)) return invalid("flux_logits_process: unknown dtype");
+    if (rows <= 0 || rows > (1 << 20) || vocab <= 0 || vocab > (1 << 24) || logits_stride < 0 || bias_stride < 0 ||
+        allowed_stride < 0 || history_stride < 0 || history_width < 0 || history_width > 0x7fffffff)
+        return invalid("flux_logits_process: invalid shape");
+    const int64_t needed = static_cast<int64_t>(flux::logits_workspace_bytes(rows, vocab));
+    if (needed > 0 && (!workspace || workspace_bytes < needed))
+        return invalid("flux_logits_process: workspace missing or too small (flux_logits_process_workspace_bytes)");
+    if (rows > (int64_t{1} << 32) / (vocab + 1023)) return invalid("flux_logits_process: invalid shape");
+    flux::LogitsArgs args{};
+    args.logits = logits;
+    args.out = output;
+    args.tokens = tokens;
+    args.rows = rows;
+    args.vocab = vocab;
+    args.logits_stride = logits_stride;
+    args.history = history_width > 0 ? history : nullptr;
+    args.history_width = history_width;
+    args.history_stride = history_stride;
+    args.history_lengths = history_lengths;
+    args.repetition = repetition;
+    args.frequency = frequency;
+    args.presence = presence;
+    args.bias = bias;
+    args.bias_stride = bias_stride;
+    args.allowed = allowed;
+    args.allowed_stride = allowed_stride;
+    args.workspace = workspace;
+    return from_hip(flux::launch_logits_process(args, static_cast<flux::Type>(dtype), stream), "flux_logits_process");
 }
 
 }  // extern "C"

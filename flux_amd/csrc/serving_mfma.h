@@ -1,0 +1,251 @@
+// Register layouts of the 16 x 16 matrix instructions that the serving attention kernels share, by element type.
+//
+// Scores are S^T = K Q^T: the left operand holds 16 keys (lane % 16), the right one 16 query rows (lane % 16), and a
+// dot product may take its terms in any order as long as both operands use the same one; so each lane loads 16
+// consecutive bytes of its row and group g = lane / 16 covers dims [step * f + per * g, + per) in fragment f.
+// The result leaves lane (n, g) with the scores of keys 4 g .. 4 g + 3 for query row n, which is the right operand of
+// O^T = V^T P over those keys.  V^T's left operand needs, in lane (m, g), one dim of the same keys: the lane loads
+// consecutive dims of the four rows and each component (or byte permute of 16-bit components) is a block of 16 dims.
+#pragma once
+
+#include "flux_common.h"
+
+namespace flux {
+
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef _Float16 f16x4 __attribute__((ext_vector_type(4)));
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+
+__device__ __forceinline__ int wave_scan_int(int v) {
+    const int lane = threadIdx.x & 63;
+#pragma unroll
+    for (int step = 1; step < 64; step *= 2) {
+        const int below = __shfl_up(v, step, kWave);
+        if (lane >= step) v += below;
+    }
+    return v;
+}
+
+__device__ __forceinline__ int wave_sum_int(int v) {
+#pragma unroll
+    for (int step = 1; step < 64; step *= 2) v += __shfl_xor(v, step, kWave);
+    return v;
+}
+
+template <class T>
+struct Mfma;
+
+template <>
+struct Mfma<float> {
+    using Fragment = f32x4;
+    static constexpr int kKeyStep = 16;
+    static constexpr int kPer = 4;
+    static constexpr float kWeightShift = 0.0f;
+    template <int kDim>
+    using ValueChunk = f32x4;
+    template <int kDim>
+    static constexpr int key_fragments() { return kDim / 16; }
+    template <int kDim>
+    static constexpr int value_chunks() { return kDim / 64; }
+
+    static __device__ __forceinline__ Fragment load_query(const float* q, int64_t stride, int d, int dim, bool ok) {
+        Fragment f;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) f[j] = ok && d + j < dim ? q[(d + j) * stride] : 0.0f;
+        return f;
+    }
+    template <bool kWide>
+    static __device__ __forceinline__ Fragment load_row(const float* row, int d, int dim, bool ok) {
+        Fragment f = {0, 0, 0, 0};
+        if constexpr (kWide) {
+            if (ok && d < dim) f = *reinterpret_cast<const f32x4*>(row + d);
+        } else {
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+                if (ok && d + j < dim) f[j] = row[d + j];
+        }
+        return f;
+    }
+    template <int kDim, bool kWide>
+    static __device__ __forceinline__ f32x4 load_value(const float* row, int chunk, int m, int dim, bool ok) {
+        return load_row<kWide>(row, 64 * chunk + 4 * m, dim, ok);
+    }
+    static __device__ __forceinline__ void multiply_key(const Fragment& key, const Fragment& query, f32x4& score) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) score = __builtin_amdgcn_mfma_f32_16x16x4f32(key[j], query[j], score, 0, 0, 0);
+    }
+    template <int kDim, int kSubs>
+    static __device__ __forceinline__ void multiply_value(const f32x4 (&value)[kSubs][4][kDim / 64],
+                                                          const float (&p)[kSubs][4], f32x4* out) {
+#pragma unroll
+        for (int s = 0; s < kSubs; ++s)
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+#pragma unroll
+                for (int c = 0; c < kDim / 64; ++c)
+#pragma unroll
+                    for (int b = 0; b < 4; ++b)
+                        out[4 * c + b] = __builtin_amdgcn_mfma_f32_16x16x4f32(value[s][i][c][b], p[s][i],
+                                                                              out[4 * c + b], 0, 0, 0);
+    }
+    // Row m = 4 g + r of block i is dim 64 (i / 4) + 4 m + i % 4.
+    template <int kDim, class F>
+    static __device__ __forceinline__ void each_dim(int g, int dim, F&& f) {
+#pragma unroll
+        for (int i = 0; i < kDim / 16; ++i)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                const int d = 64 * (i / 4) + 16 * g + 4 * r + i % 4;
+                if (d < dim) f(i, r, d);
+            }
+    }
+};
+
+// What the two 16-bit types share.  The weights are split in two terms of 16 bits, so that their rounding (2^-16
+// of a weight and less) does not show beside that of the result; the matrix units wait for memory here.
+template <class T, class Derived>
+struct Mfma16 {
+    using Fragment = u32x4;
+    static constexpr int kKeyStep = 32;
+    static constexpr int kPer = 8;
+    template <int kDim>
+    static constexpr int words() { return kDim == 64 ? 2 : 4; }  // of a value chunk
+    template <int kDim>
+    using ValueChunk = u32x4;
+    template <int kDim>
+    static constexpr int key_fragments() { return kDim / 32; }
+    template <int kDim>
+    static constexpr int value_chunks() { return kDim == 64 ? 1 : kDim / 128; }
+
+    static __device__ __forceinline__ uint32_t bits(T v) { return __builtin_bit_cast(uint16_t, v); }
+
+    static __device__ __forceinline__ Fragment load_query(const T* q, int64_t stride, int d, int dim, bool ok) {
+        Fragment f;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const uint32_t low = ok && d + 2 * j < dim ? bits(q[(d + 2 * j) * stride]) : 0;
+            const uint32_t high = ok && d + 2 * j + 1 < dim ? bits(q[(d + 2 * j + 1) * stride]) : 0;
+            f[j] = low | high << 16;
+        }
+        return f;
+    }
+    template <bool kWide>
+    static __device__ __forceinline__ Fragment load_row(const T* row, int d, int dim, bool ok) {
+        Fragment f = {0, 0, 0, 0};
+        if constexpr (kWide) {
+            if (ok && d < dim) f = *reinterpret_cast<const u32x4*>(row + d);
+        } else {
+            if (ok) f = load_query(row, 1, d, dim, true);
+        }
+        return f;
+    }
+    template <int kDim, bool kWide>
+    static __device__ __forceinline__ u32x4 load_value(const T* row, int chunk, int m, int dim, bool ok) {
+        if constexpr (kDim == 64) {
+            u32x4 f = {0, 0, 0, 0};
+            if constexpr (kWide) {
+                if (ok && 4 * m < dim) {
+                    const u32x2 half = *reinterpret_cast<const u32x2*>(row + 4 * m);
+                    f[0] = half[0];
+                    f[1] = half[1];
+                }
+            } else {
+#pragma unroll
+                for (int j = 0; j < 2; ++j) {
+                    const uint32_t low = ok && 4 * m + 2 * j < dim ? bits(row[4 * m + 2 * j]) : 0;
+                    const uint32_t high = ok && 4 * m + 2 * j + 1 < dim ? bits(row[4 * m + 2 * j + 1]) : 0;
+                    f[j] = low | high << 16;
+                }
+            }
+            return f;
+        } else {
+            return load_row<kWide>(row, 128 * chunk + 8 * m, dim, ok);
+        }
+    }
+    static __device__ __forceinline__ void multiply_key(const Fragment& key, const Fragment& query, f32x4& score) {
+        score = Derived::multiply32(key, query, score);
+    }
+    // The 16-bit components `odd` of two dwords, side by side.
+    static __device__ __forceinline__ uint32_t pair(uint32_t first, uint32_t second, bool odd) {
+        return __builtin_amdgcn_perm(second, first, odd ? 0x07060302u : 0x05040100u);
+    }
+    template <int kDim, int kSubs>
+    static __device__ __forceinline__ void multiply_value(const u32x4 (&value)[kSubs][4][value_chunks<kDim>()],
+                                                          const float (&p)[kSubs][4], f32x4* out) {
+        u32x4 high = {0, 0, 0, 0}, low = {0, 0, 0, 0};
+#pragma unroll
+        for (int s = 0; s < kSubs; ++s)
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+                const T h0 = static_cast<T>(p[s][2 * j]), h1 = static_cast<T>(p[s][2 * j + 1]);
+                high[2 * s + j] = bits(h0) | bits(h1) << 16;
+                const T l0 = static_cast<T>(p[s][2 * j] - static_cast<float>(h0));
+                const T l1 = static_cast<T>(p[s][2 * j + 1] - static_cast<float>(h1));
+                low[2 * s + j] = bits(l0) | bits(l1) << 16;
+            }
+#pragma unroll
+        for (int c = 0; c < value_chunks<kDim>(); ++c)
+#pragma unroll
+            for (int b = 0; b < 2 * words<kDim>(); ++b) {
+                u32x4 left = {0, 0, 0, 0};
+#pragma unroll
+                for (int s = 0; s < kSubs; ++s) {
+                    left[2 * s] = pair(value[s][0][c][b / 2], value[s][1][c][b / 2], b & 1);
+                    left[2 * s + 1] = pair(value[s][2][c][b / 2], value[s][3][c][b / 2], b & 1);
+                }
+                f32x4& o = out[2 * words<kDim>() * c + b];
+                if constexpr (kSubs == 2) {
+                    o = Derived::multiply32(left, high, o);
+                    o = Derived::multiply32(left, low, o);
+                } else {
+                    o = Derived::multiply16(left, high, o);
+                    o = Derived::multiply16(left, low, o);
+                }
+            }
+    }
+    // Row m = 4 g + r of block i: dim 4 m + i for heads up to 64, else 128 (i / 8) + 8 m + i % 8.
+    template <int kDim, class F>
+    static __device__ __forceinline__ void each_dim(int g, int dim, F&& f) {
+#pragma unroll
+        for (int i = 0; i < kDim / 16; ++i)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                const int d = kDim == 64 ? 16 * g + 4 * r + i : 128 * (i / 8) + 8 * (4 * g + r) + i % 8;
+                if (d < dim) f(i, r, d);
+            }
+    }
+};
+
+template <>
+struct Mfma<__bf16> : Mfma16<__bf16, Mfma<__bf16>> {
+    static constexpr float kWeightShift = 0.0f;
+    static __device__ __forceinline__ f32x4 multiply32(u32x4 a, u32x4 b, f32x4 c) {
+        return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c,
+                                                       0, 0, 0);
+    }
+    static __device__ __forceinline__ f32x4 multiply16(u32x4 a, u32x4 b, f32x4 c) {
+        return __builtin_amdgcn_mfma_f32_16x16x16bf16_1k(__builtin_bit_cast(s16x4, u32x2{a[0], a[1]}),
+                                                         __builtin_bit_cast(s16x4, u32x2{b[0], b[1]}), c, 0, 0, 0);
+    }
+};
+
+// float16's smallest step is 2^-24: weights are held 2^12 times as large (at most 4096), sums of weights with them, so
+// that what a split weight loses is below 2^-36 of the largest one.
+template <>
+struct Mfma<_Float16> : Mfma16<_Float16, Mfma<_Float16>> {
+    static constexpr float kWeightShift = 12.0f;
+    static __device__ __forceinline__ f32x4 multiply32(u32x4 a, u32x4 b, f32x4 c) {
+        return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0,
+                                                      0, 0);
+    }
+    static __device__ __forceinline__ f32x4 multiply16(u32x4 a, u32x4 b, f32x4 c) {
+        return __builtin_amdgcn_mfma_f32_16x16x16f16(__builtin_bit_cast(f16x4, u32x2{a[0], a[1]}),
+                                                     __builtin_bit_cast(f16x4, u32x2{b[0], b[1]}), c, 0, 0, 0);
+    }
+};
+
+}  // namespace flux

@@ -1,0 +1,727 @@
+"""``torch.ops.flux.*`` for serving several sequences: attention over a paged K/V cache, windowed attention, the pages
+themselves, and logits on their way to the next token.
+
+They stand next to the one-sequence operators of ``flux_amd.ops.native`` and follow their manner: arguments are
+checked on the host, each ROCm kernel is a call through the C ABI of ``libflux_amd.so`` on the tensors' current stream,
+CPU tensors are checked and then refused, FakeTensor contracts are registered, and everything is inference-only.
+Nothing here synchronises with the GPU: lengths, tables and lists stay on the device, and what a request of a page
+operator came to is in the status it returns.
+
+A cache in pages is ``key_pages`` and ``value_pages`` ``[pages, kv_heads, page_size, head_dim]`` of one layer, or with
+a leading layer dimension for the operators that move pages, and the books that all layers share: ``page_table`` int32
+``[slots, columns]`` (-1: no page), ``lengths`` int64 ``[slots]`` and ``refcounts`` int32 ``[pages]`` (0: free).
+"""
+
+from __future__ import annotations
+
+import ctypes
+
+import torch
+
+from flux_amd import _native
+from flux_amd.ops.native import (_LIBRARY, _aliases, _availability, _call, _check, _cpu_kernel, _finite_fp32, _grad_free,
+                                 _on, _require_gpu, _require_library, _stream)
+
+PAGE_DONE, PAGE_OUT_OF_RANGE, PAGE_REPEATED, PAGE_NO_ROOM, PAGE_OCCUPIED = range(5)
+
+_TYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
+_MAX_DIM = 256
+_MAX_KEYS = 1 << 24  # positions of one sequence
+_MAX_VOCAB = 1 << 24
+
+SERVING_SCHEMAS = {
+    "paged_decode_attention": ("paged_decode_attention(Tensor query, Tensor key_pages, Tensor value_pages, "
+                               "Tensor page_table, Tensor lengths, float scale, int window=0, int sinks=0, "
+                               "Tensor? slots=None) -> Tensor"),
+    "paged_decode_attention_out": ("paged_decode_attention_out(Tensor query, Tensor key_pages, Tensor value_pages, "
+                                   "Tensor page_table, Tensor lengths, float scale, int window, int sinks, "
+                                   "Tensor? slots, Tensor(a!) output, Tensor(b!) workspace) -> Tensor(a!)"),
+    "window_attention": ("window_attention(Tensor query, Tensor key, Tensor value, float scale, int window, "
+                         "int sinks=0, Tensor? lengths=None, Tensor? starts=None) -> Tensor"),
+    "paged_cache_reserve": ("paged_cache_reserve(Tensor(a!) page_table, Tensor(b!) lengths, Tensor(c!) refcounts, "
+                            "int page_size, Tensor slots, Tensor? counts=None) -> (Tensor positions, Tensor status)"),
+    "paged_cache_write": ("paged_cache_write(Tensor key, Tensor value, Tensor(a!) key_pages, Tensor(b!) value_pages, "
+                          "Tensor page_table, Tensor slots, Tensor positions, Tensor? counts=None) -> ()"),
+    "paged_cache_copy": ("paged_cache_copy(Tensor(a!) key_pages, Tensor(b!) value_pages, Tensor source, "
+                         "Tensor target) -> Tensor"),
+    "paged_cache_fork": ("paged_cache_fork(Tensor(a!) key_pages, Tensor(b!) value_pages, Tensor(c!) page_table, "
+                         "Tensor(d!) lengths, Tensor(e!) refcounts, Tensor parents, Tensor children) -> Tensor"),
+    "paged_cache_free": ("paged_cache_free(Tensor(a!) page_table, Tensor(b!) lengths, Tensor(c!) refcounts, "
+                         "Tensor slots) -> Tensor"),
+    "paged_cache_compact": ("paged_cache_compact(Tensor(a!) key_pages, Tensor(b!) value_pages, Tensor(c!) page_table, "
+                            "Tensor(d!) refcounts) -> (Tensor page_map, Tensor used)"),
+    "logits_process": ("logits_process(Tensor logits, Tensor? history=None, Tensor? history_lengths=None, "
+                       "Tensor? repetition=None, Tensor? frequency=None, Tensor? presence=None, Tensor? bias=None, "
+                       "Tensor? allowed=None) -> (Tensor processed, Tensor tokens)"),
+}
+
+for _schema in SERVING_SCHEMAS.values():
+    _LIBRARY.define(_schema)
+
+_FOUR = ctypes.c_int64 * 4
+_THREE = ctypes.c_int64 * 3
+
+
+def _address(tensor):
+    return None if tensor is None else tensor.data_ptr()
+
+
+def _check_list(tensor, dtype, like, message: str) -> None:
+    """A contiguous vector of ``dtype`` on the device of ``like``."""
+    _check(tensor.dim() == 1 and tensor.dtype == dtype and tensor.device == like.device and tensor.is_contiguous(),
+           message)
+
+
+def _check_window(window, sinks, message: str) -> None:
+    _check(0 <= window <= _MAX_KEYS and 0 <= sinks <= _MAX_KEYS, message)
+
+
+# ---------------------------------------------------------------------------
+# paged_decode_attention
+
+def _validate_paged(query, key_pages, value_pages, page_table, lengths, scale, window=0, sinks=0, slots=None) -> None:
+    _check(query.dim() == 4 and key_pages.dim() == 4 and value_pages.dim() == 4,
+           "flux::paged_decode_attention: query and pages must be rank four")
+    _check(query.dtype in _TYPES and key_pages.dtype == query.dtype and value_pages.dtype == query.dtype,
+           "flux::paged_decode_attention: query and pages must share dtype float32, float16 or bfloat16")
+    _check(query.shape[2] == 1, "flux::paged_decode_attention: query length must be one")
+    _check(key_pages.shape == value_pages.shape, "flux::paged_decode_attention: key and value page shapes must match")
+    _check(all(s > 0 for s in query.shape) and all(s > 0 for s in key_pages.shape),
+           "flux::paged_decode_attention: tensor dimensions must be non-empty")
+    _check(query.shape[3] == key_pages.shape[3] and query.shape[3] <= _MAX_DIM,
+           "flux::paged_decode_attention: head dimensions must match and be at most 256")
+    _check(query.shape[1] % key_pages.shape[1] == 0,
+           "flux::paged_decode_attention: query heads must be divisible by KV heads")
+    _check(page_table.dim() == 2 and page_table.dtype == torch.int32 and page_table.shape[1] > 0,
+           "flux::paged_decode_attention: page_table must be int32 [slots, columns]")
+    _check(page_table.stride(1) == 1 or page_table.shape[1] == 1,
+           "flux::paged_decode_attention: page_table rows must be contiguous")
+    _check(page_table.shape[1] * key_pages.shape[2] <= _MAX_KEYS,
+           "flux::paged_decode_attention: page_table holds more than 16777216 positions a row")
+    _check_list(lengths, torch.int64, query,
+                "flux::paged_decode_attention: lengths must be a contiguous int64 vector on the query device")
+    _check(lengths.shape[0] == page_table.shape[0],
+           "flux::paged_decode_attention: lengths must have one entry per page_table row")
+    if slots is None:
+        _check(page_table.shape[0] == query.shape[0],
+               "flux::paged_decode_attention: without slots page_table must have one row per sequence")
+    else:
+        _check_list(slots, torch.int64, query,
+                    "flux::paged_decode_attention: slots must be a contiguous int64 vector on the query device")
+        _check(slots.shape[0] == query.shape[0], "flux::paged_decode_attention: slots must have one entry per sequence")
+    _check(key_pages.device == query.device and value_pages.device == query.device and
+           page_table.device == query.device, "flux::paged_decode_attention: tensor devices must match")
+    _check(key_pages.stride(3) == 1 and value_pages.stride(3) == 1 or key_pages.shape[3] == 1,
+           "flux::paged_decode_attention: pages must have unit stride along the head dimension")
+    _check_window(window, sinks, "flux::paged_decode_attention: window and sinks must be within [0, 16777216]")
+    _check(_finite_fp32(scale), "flux::paged_decode_attention: scale must be a finite FP32 value")
+    _grad_free("flux::paged_decode_attention", query, key_pages, value_pages)
+
+
+def paged_decode_workspace_bytes(query: torch.Tensor, key_pages: torch.Tensor, page_table: torch.Tensor, window: int = 0,
+                                 sinks: int = 0) -> int:
+    """Device workspace (bytes) that flux::paged_decode_attention needs for these shapes."""
+    value = ctypes.c_int64(0)
+    _call("flux_paged_decode_attention_workspace_bytes", query.shape[0], query.shape[1], key_pages.shape[1],
+          query.shape[3], page_table.shape[1] * key_pages.shape[2], window, sinks, ctypes.byref(value))
+    return value.value
+
+
+def _launch_paged(query, key_pages, value_pages, page_table, lengths, scale, window, sinks, slots, output, workspace):
+    batch, heads, _, dim = query.shape
+    pages, kv_heads, page_size, _ = key_pages.shape
+    with _on(query.device):
+        _call("flux_paged_decode_attention", _TYPES[query.dtype], query.data_ptr(), key_pages.data_ptr(),
+              value_pages.data_ptr(), page_table.data_ptr(), lengths.data_ptr(), _address(slots), output.data_ptr(),
+              workspace.data_ptr(), workspace.numel() * 4, scale, batch, heads, kv_heads, dim, pages, page_size,
+              page_table.shape[0], page_table.shape[1], page_table.stride(0), window, sinks, _FOUR(*query.stride()),
+              _THREE(*key_pages.stride()[:3]), _THREE(*value_pages.stride()[:3]), _stream(query))
+
+
+def _paged_cuda(query, key_pages, value_pages, page_table, lengths, scale, window=0, sinks=0, slots=None):
+    _validate_paged(query, key_pages, value_pages, page_table, lengths, scale, window, sinks, slots)
+    _require_gpu("flux::paged_decode_attention", query)
+    output = torch.empty(query.shape, dtype=query.dtype, device=query.device)
+    needed = paged_decode_workspace_bytes(query, key_pages, page_table, window, sinks)
+    workspace = torch.empty(needed // 4, dtype=torch.float32, device=query.device)
+    _launch_paged(query, key_pages, value_pages, page_table, lengths, scale, window, sinks, slots, output, workspace)
+    return output
+
+
+def _validate_paged_out(query, key_pages, value_pages, page_table, lengths, scale, window, sinks, slots, output,
+                        workspace) -> None:
+    _validate_paged(query, key_pages, value_pages, page_table, lengths, scale, window, sinks, slots)
+    op = "flux::paged_decode_attention_out"
+    _check(output.shape == query.shape and output.dtype == query.dtype and output.device == query.device and
+           output.is_contiguous(), f"{op}: output must be contiguous, of the query's shape, dtype and device")
+    _check(workspace.dtype == torch.float32 and workspace.device == query.device and workspace.is_contiguous(),
+           f"{op}: workspace must be contiguous float32 on the query device")
+    _check(not _aliases(output, workspace), f"{op}: output and workspace must not alias")
+    for tensor in (query, key_pages, value_pages, page_table, lengths, slots):
+        _check(tensor is None or not (_aliases(output, tensor) or _aliases(workspace, tensor)),
+               f"{op}: output and workspace must not alias an input")
+
+
+def _paged_out_cuda(query, key_pages, value_pages, page_table, lengths, scale, window, sinks, slots, output, workspace):
+    _validate_paged_out(query, key_pages, value_pages, page_table, lengths, scale, window, sinks, slots, output,
+                        workspace)
+    _require_gpu("flux::paged_decode_attention_out", query)
+    _check(workspace.numel() * 4 >= paged_decode_workspace_bytes(query, key_pages, page_table, window, sinks),
+           "flux::paged_decode_attention_out: workspace is too small (paged_decode_workspace_bytes)")
+    _launch_paged(query, key_pages, value_pages, page_table, lengths, scale, window, sinks, slots, output, workspace)
+    return output
+
+
+# ---------------------------------------------------------------------------
+# window_attention
+
+def _validate_window(query, key, value, scale, window, sinks=0, lengths=None, starts=None) -> None:
+    _check(query.dim() == 4 and key.dim() == 4 and value.dim() == 4,
+           "flux::window_attention: query, key and value must be rank four")
+    _check(query.dtype in _TYPES and key.dtype == query.dtype and value.dtype == query.dtype,
+           "flux::window_attention: query, key and value must share dtype float32, float16 or bfloat16")
+    _check(key.shape == value.shape, "flux::window_attention: key and value shapes must match")
+    _check(all(s > 0 for s in query.shape) and all(s > 0 for s in key.shape),
+           "flux::window_attention: tensor dimensions must be non-empty")
+    _check(query.shape[0] == key.shape[0], "flux::window_attention: batch sizes must match")
+    _check(query.shape[3] == key.shape[3] and query.shape[3] <= _MAX_DIM,
+           "flux::window_attention: head dimensions must match and be at most 256")
+    _check(query.shape[1] % key.shape[1] == 0, "flux::window_attention: query heads must be divisible by KV heads")
+    _check(key.shape[2] <= _MAX_KEYS, "flux::window_attention: more than 16777216 keys")
+    _check(key.device == query.device and value.device == query.device,
+           "flux::window_attention: tensor devices must match")
+    _check(key.stride(3) == 1 and value.stride(3) == 1 or key.shape[3] == 1,
+           "flux::window_attention: key and value must have unit stride along the head dimension")
+    if lengths is not None:
+        _check_list(lengths, torch.int64, query,
+                    "flux::window_attention: lengths must be a contiguous int64 vector on the query device")
+        _check(lengths.shape[0] == query.shape[0], "flux::window_attention: lengths must have one entry per sequence")
+    if starts is not None:
+        _check_list(starts, torch.int64, query,
+                    "flux::window_attention: starts must be a contiguous int64 vector on the query device")
+        _check(starts.shape[0] == query.shape[0], "flux::window_attention: starts must have one entry per sequence")
+    _check_window(window, sinks, "flux::window_attention: window and sinks must be within [0, 16777216]")
+    _check(_finite_fp32(scale), "flux::window_attention: scale must be a finite FP32 value")
+    _grad_free("flux::window_attention", query, key, value)
+
+
+def _window_cuda(query, key, value, scale, window, sinks=0, lengths=None, starts=None):
+    _validate_window(query, key, value, scale, window, sinks, lengths, starts)
+    _require_gpu("flux::window_attention", query)
+    batch, heads, queries, dim = query.shape
+    kv_heads, keys = key.shape[1], key.shape[2]
+    output = torch.empty(query.shape, dtype=query.dtype, device=query.device)
+    needed = ctypes.c_int64(0)
+    if queries == 1:
+        _call("flux_window_attention_workspace_bytes", batch, heads, kv_heads, queries, dim, keys, window, sinks,
+              ctypes.byref(needed))
+    workspace = torch.empty(needed.value // 4, dtype=torch.float32, device=query.device) if needed.value else None
+    with _on(query.device):
+        _call("flux_window_attention", _TYPES[query.dtype], query.data_ptr(), key.data_ptr(), value.data_ptr(),
+              _address(lengths), _address(starts), output.data_ptr(), _address(workspace), needed.value, scale, batch,
+              heads, kv_heads, queries, keys, dim, window, sinks, _FOUR(*query.stride()), _THREE(*key.stride()[:3]),
+              _THREE(*value.stride()[:3]), _stream(query))
+    return output
+
+
+# ---------------------------------------------------------------------------
+# Pages.
+
+def _check_written(tensor, message: str) -> None:
+    """A tensor that is written: no two of its elements share memory by a stride of zero."""
+    _check(all(stride > 0 or size == 1 for size, stride in zip(tensor.shape, tensor.stride())), message)
+
+
+def _validate_pools(op, key_pages, value_pages, ranks=(4, 5)) -> None:
+    _check(key_pages.dim() in ranks and value_pages.dim() == key_pages.dim(),
+           f"{op}: key_pages and value_pages must be [pages, kv_heads, page_size, head_dim]" +
+           (", or that behind a layer dimension" if 5 in ranks else ""))
+    _check(key_pages.dtype in _TYPES and value_pages.dtype == key_pages.dtype,
+           f"{op}: pages must share dtype float32, float16 or bfloat16")
+    _check(key_pages.shape == value_pages.shape, f"{op}: key and value page shapes must match")
+    _check(all(s > 0 for s in key_pages.shape), f"{op}: pages must be non-empty")
+    _check(key_pages.device == value_pages.device, f"{op}: tensor devices must match")
+    _check(key_pages.stride(-1) == 1 and value_pages.stride(-1) == 1 or key_pages.shape[-1] == 1,
+           f"{op}: pages must have unit stride along the head dimension")
+    _check_written(key_pages, f"{op}: key_pages must not overlap itself")
+    _check_written(value_pages, f"{op}: value_pages must not overlap itself")
+    _grad_free(op, key_pages, value_pages)
+
+
+def _validate_table(op, page_table) -> None:
+    _check(page_table.dim() == 2 and page_table.dtype == torch.int32 and page_table.shape[0] > 0 and
+           page_table.shape[1] > 0, f"{op}: page_table must be int32 [slots, columns]")
+    _check(page_table.stride(1) == 1 or page_table.shape[1] == 1, f"{op}: page_table rows must be contiguous")
+
+
+def _validate_books(op, page_table, lengths, refcounts) -> None:
+    _validate_table(op, page_table)
+    _check(page_table.stride(0) >= page_table.shape[1] or page_table.shape[0] == 1,
+           f"{op}: page_table rows must not overlap")
+    if lengths is not None:
+        _check_list(lengths, torch.int64, page_table,
+                    f"{op}: lengths must be a contiguous int64 vector on the page_table device")
+        _check(lengths.shape[0] == page_table.shape[0], f"{op}: lengths must have one entry per page_table row")
+    _check_list(refcounts, torch.int32, page_table,
+                f"{op}: refcounts must be a contiguous int32 vector on the page_table device")
+    _check(refcounts.shape[0] > 0, f"{op}: refcounts must have one entry per page")
+
+
+def _validate_requests(op, name, requests, like) -> None:
+    _check_list(requests, torch.int64, like, f"{op}: {name} must be a contiguous int64 vector on the cache's device")
+
+
+def _pool(key_pages, value_pages) -> _native.PagePool:
+    key_strides, value_strides = key_pages.stride(), value_pages.stride()
+    if key_pages.dim() == 4:
+        layers, shape = 1, key_pages.shape
+        key_strides, value_strides = (0, *key_strides), (0, *value_strides)
+    else:
+        layers, shape = key_pages.shape[0], key_pages.shape[1:]
+    return _native.PagePool(key_pages.data_ptr(), value_pages.data_ptr(), layers, *shape, _FOUR(*key_strides[:4]),
+                            _FOUR(*value_strides[:4]), _TYPES[key_pages.dtype])
+
+
+def _books(page_table, lengths, refcounts, page_size) -> _native.PageBooks:
+    return _native.PageBooks(page_table.data_ptr(), page_table.stride(0), page_table.shape[0], page_table.shape[1],
+                             _address(lengths), refcounts.data_ptr(), refcounts.shape[0], page_size)
+
+
+def _page_size_of(key_pages) -> int:
+    return key_pages.shape[-2]
+
+
+def _validate_reserve(page_table, lengths, refcounts, page_size, slots, counts=None) -> None:
+    op = "flux::paged_cache_reserve"
+    _validate_books(op, page_table, lengths, refcounts)
+    _check(page_size > 0 and page_table.shape[1] * page_size <= _MAX_KEYS,
+           f"{op}: page_size must be positive and a page_table row hold at most 16777216 positions")
+    _validate_requests(op, "slots", slots, page_table)
+    if counts is not None:
+        _validate_requests(op, "counts", counts, page_table)
+        _check(counts.shape == slots.shape, f"{op}: counts must have one entry per slot")
+
+
+def _reserve_cuda(page_table, lengths, refcounts, page_size, slots, counts=None):
+    _validate_reserve(page_table, lengths, refcounts, page_size, slots, counts)
+    _require_gpu("flux::paged_cache_reserve", page_table)
+    requests = slots.shape[0]
+    positions = torch.empty(requests, dtype=torch.int64, device=slots.device)
+    status = torch.empty(requests, dtype=torch.int32, device=slots.device)
+    if requests == 0:
+        return positions, status
+    words = ctypes.c_int64(0)
+    _call("flux_page_reserve_workspace_words", requests, page_table.shape[0], refcounts.shape[0], ctypes.byref(words))
+    workspace = torch.empty(words.value, dtype=torch.int32, device=slots.device)
+    with _on(slots.device):
+        _call("flux_page_reserve", ctypes.byref(_books(page_table, lengths, refcounts, page_size)), slots.data_ptr(),
+              _address(counts), requests, positions.data_ptr(), status.data_ptr(), workspace.data_ptr(), words.value,
+              _stream(slots))
+    return positions, status
+
+
+def _validate_write(key, value, key_pages, value_pages, page_table, slots, positions, counts=None) -> None:
+    op = "flux::paged_cache_write"
+    _validate_pools(op, key_pages, value_pages, ranks=(4,))
+    _validate_table(op, page_table)
+    _check(page_table.device == key_pages.device, f"{op}: tensor devices must match")
+    _check(page_table.shape[1] * key_pages.shape[2] <= _MAX_KEYS,
+           f"{op}: page_table holds more than 16777216 positions a row")
+    _check(key.dim() == 4 and value.shape == key.shape, f"{op}: key and value must be rank four and of one shape")
+    _check(key.dtype == key_pages.dtype and value.dtype == key_pages.dtype and key.device == key_pages.device and
+           value.device == key_pages.device, f"{op}: key and value must have the pages' dtype and device")
+    _check(key.shape[1] == key_pages.shape[1] and key.shape[3] == key_pages.shape[3],
+           f"{op}: key heads and head dimension must be the pages'")
+    _check(key.stride(3) == 1 and value.stride(3) == 1 or key.shape[3] == 1,
+           f"{op}: key and value must have unit stride along the head dimension")
+    for source in (key, value):
+        for pages in (key_pages, value_pages):
+            _check(not _aliases(source, pages), f"{op}: the pages must not alias key or value")
+    for name, tensor in (("slots", slots), ("positions", positions), ("counts", counts)):
+        if tensor is not None:
+            _validate_requests(op, name, tensor, key_pages)
+            _check(tensor.shape[0] == key.shape[0], f"{op}: {name} must have one entry per request")
+    _check(key.shape[0] <= 65535, f"{op}: more than 65535 requests")
+    _grad_free(op, key, value)
+
+
+def _write_cuda(key, value, key_pages, value_pages, page_table, slots, positions, counts=None):
+    _validate_write(key, value, key_pages, value_pages, page_table, slots, positions, counts)
+    _require_gpu("flux::paged_cache_write", key_pages)
+    if key.shape[0] == 0 or key.shape[2] == 0:
+        return
+    with _on(key_pages.device):
+        _call("flux_page_write", ctypes.byref(_pool(key_pages, value_pages)), key.data_ptr(), value.data_ptr(),
+              _THREE(*key.stride()[:3]), _THREE(*value.stride()[:3]), key.shape[0], key.shape[2],
+              page_table.data_ptr(), page_table.stride(0), page_table.shape[0], page_table.shape[1], slots.data_ptr(),
+              positions.data_ptr(), _address(counts), _stream(key_pages))
+
+
+def _validate_copy(key_pages, value_pages, source, target) -> None:
+    op = "flux::paged_cache_copy"
+    _validate_pools(op, key_pages, value_pages)
+    _validate_requests(op, "source", source, key_pages)
+    _validate_requests(op, "target", target, key_pages)
+    _check(source.shape == target.shape, f"{op}: source and target must have one length")
+
+
+def _copy_cuda(key_pages, value_pages, source, target):
+    _validate_copy(key_pages, value_pages, source, target)
+    _require_gpu("flux::paged_cache_copy", key_pages)
+    status = torch.empty(source.shape[0], dtype=torch.int32, device=source.device)
+    if source.shape[0]:
+        with _on(source.device):
+            _call("flux_page_copy", ctypes.byref(_pool(key_pages, value_pages)), source.data_ptr(), target.data_ptr(),
+                  source.shape[0], status.data_ptr(), _stream(source))
+    return status
+
+
+def _validate_free(page_table, lengths, refcounts, slots) -> None:
+    op = "flux::paged_cache_free"
+    _validate_books(op, page_table, lengths, refcounts)
+    _validate_requests(op, "slots", slots, page_table)
+
+
+def _free_cuda(page_table, lengths, refcounts, slots):
+    _validate_free(page_table, lengths, refcounts, slots)
+    _require_gpu("flux::paged_cache_free", page_table)
+    status = torch.empty(slots.shape[0], dtype=torch.int32, device=slots.device)
+    if slots.shape[0]:
+        with _on(slots.device):
+            _call("flux_page_free", ctypes.byref(_books(page_table, lengths, refcounts, 1)), slots.data_ptr(),
+                  slots.shape[0], status.data_ptr(), _stream(slots))
+    return status
+
+
+def _validate_fork(key_pages, value_pages, page_table, lengths, refcounts, parents, children) -> None:
+    op = "flux::paged_cache_fork"
+    _validate_pools(op, key_pages, value_pages)
+    _validate_books(op, page_table, lengths, refcounts)
+    _check(page_table.device == key_pages.device, f"{op}: tensor devices must match")
+    _check(refcounts.shape[0] == key_pages.shape[-4], f"{op}: refcounts must have one entry per page")
+    _check(page_table.shape[1] * key_pages.shape[-2] <= _MAX_KEYS,
+           f"{op}: page_table holds more than 16777216 positions a row")
+    _validate_requests(op, "parents", parents, key_pages)
+    _validate_requests(op, "children", children, key_pages)
+    _check(parents.shape == children.shape, f"{op}: parents and children must have one length")
+
+
+def _fork_cuda(key_pages, value_pages, page_table, lengths, refcounts, parents, children):
+    _validate_fork(key_pages, value_pages, page_table, lengths, refcounts, parents, children)
+    _require_gpu("flux::paged_cache_fork", key_pages)
+    requests = parents.shape[0]
+    status = torch.empty(requests, dtype=torch.int32, device=parents.device)
+    if requests == 0:
+        return status
+    words = ctypes.c_int64(0)
+    _call("flux_page_fork_workspace_words", requests, page_table.shape[0], refcounts.shape[0], ctypes.byref(words))
+    workspace = torch.empty(words.value, dtype=torch.int32, device=parents.device)
+    with _on(parents.device):
+        _call("flux_page_fork", ctypes.byref(_pool(key_pages, value_pages)),
+              ctypes.byref(_books(page_table, lengths, refcounts, _page_size_of(key_pages))), parents.data_ptr(),
+              children.data_ptr(), requests, status.data_ptr(), workspace.data_ptr(), words.value, _stream(parents))
+    return status
+
+
+def _validate_compact(key_pages, value_pages, page_table, refcounts) -> None:
+    op = "flux::paged_cache_compact"
+    _validate_pools(op, key_pages, value_pages)
+    _validate_books(op, page_table, None, refcounts)
+    _check(page_table.device == key_pages.device, f"{op}: tensor devices must match")
+    _check(refcounts.shape[0] == key_pages.shape[-4], f"{op}: refcounts must have one entry per page")
+
+
+def _compact_cuda(key_pages, value_pages, page_table, refcounts):
+    _validate_compact(key_pages, value_pages, page_table, refcounts)
+    _require_gpu("flux::paged_cache_compact", key_pages)
+    pages = refcounts.shape[0]
+    page_map = torch.empty(pages, dtype=torch.int32, device=refcounts.device)
+    used = torch.empty((), dtype=torch.int64, device=refcounts.device)
+    words = ctypes.c_int64(0)
+    _call("flux_page_compact_workspace_words", pages, ctypes.byref(words))
+    workspace = torch.empty(words.value, dtype=torch.int32, device=refcounts.device)
+    with _on(refcounts.device):
+        _call("flux_page_compact", ctypes.byref(_pool(key_pages, value_pages)),
+              ctypes.byref(_books(page_table, None, refcounts, _page_size_of(key_pages))), page_map.data_ptr(),
+              used.data_ptr(), workspace.data_ptr(), words.value, _stream(refcounts))
+    return page_map, used
+
+
+# ---------------------------------------------------------------------------
+# logits_process
+
+def _validate_logits(logits, history=None, history_lengths=None, repetition=None, frequency=None, presence=None,
+                     bias=None, allowed=None) -> None:
+    op = "flux::logits_process"
+    _check(logits.dim() == 2 and logits.shape[0] > 0 and 0 < logits.shape[1] <= _MAX_VOCAB,
+           "flux::logits_process: logits must be [rows, vocab], non-empty, vocab at most 16777216")
+    _check(logits.dtype in _TYPES, "flux::logits_process: logits must have dtype float32, float16 or bfloat16")
+    _check(logits.stride(1) == 1 or logits.shape[1] == 1, "flux::logits_process: logits rows must be contiguous")
+    rows, vocab = logits.shape
+    if history is not None:
+        _check(history.dim() == 2 and history.shape[0] == rows and history.dtype == torch.int64,
+               "flux::logits_process: history must be int64 [rows, width]")
+        _check(history.stride(1) == 1 or history.shape[1] <= 1, "flux::logits_process: history rows must be contiguous")
+        _check(history.device == logits.device, "flux::logits_process: tensor devices must match")
+    _check(history is not None or history_lengths is None, "flux::logits_process: history_lengths needs a history")
+    if history_lengths is not None:
+        _check_list(history_lengths, torch.int64, logits,
+                    "flux::logits_process: history_lengths must be a contiguous int64 vector on the logits device")
+        _check(history_lengths.shape[0] == rows, "flux::logits_process: history_lengths must have one entry per row")
+    for name, penalty in (("repetition", repetition), ("frequency", frequency), ("presence", presence)):
+        if penalty is not None:
+            _check_list(penalty, torch.float32, logits,
+                        f"{op}: {name} must be a contiguous float32 vector on the logits device")
+            _check(penalty.shape[0] == rows, f"{op}: {name} must have one entry per row")
+            _check(history is not None, f"{op}: {name} needs a history")
+    if bias is not None:
+        _check(bias.dim() == 2 and bias.shape[0] in (1, rows) and bias.shape[1] == vocab and
+               bias.dtype == torch.float32 and bias.device == logits.device,
+               "flux::logits_process: bias must be float32 [1 or rows, vocab] on the logits device")
+        _check(bias.stride(1) == 1 or vocab == 1, "flux::logits_process: bias rows must be contiguous")
+    if allowed is not None:
+        _check(allowed.dim() == 2 and allowed.shape[0] in (1, rows) and allowed.shape[1] == (vocab + 31) // 32 and
+               allowed.dtype == torch.int32 and allowed.device == logits.device,
+               "flux::logits_process: allowed must be int32 [1 or rows, ceil(vocab / 32)] on the logits device")
+        _check(allowed.stride(1) == 1 or allowed.shape[1] == 1,
+               "flux::logits_process: allowed rows must be contiguous")
+    _grad_free(op, logits, bias, repetition, frequency, presence)
+
+
+def _row_stride(tensor) -> int:
+    return 0 if tensor is None or tensor.shape[0] == 1 else tensor.stride(0)
+
+
+def _logits_cuda(logits, history=None, history_lengths=None, repetition=None, frequency=None, presence=None, bias=None,
+                 allowed=None):
+    _validate_logits(logits, history, history_lengths, repetition, frequency, presence, bias, allowed)
+    _require_gpu("flux::logits_process", logits)
+    rows, vocab = logits.shape
+    processed = torch.empty((rows, vocab), dtype=logits.dtype, device=logits.device)
+    tokens = torch.empty(rows, dtype=torch.int64, device=logits.device)
+    needed = ctypes.c_int64(0)
+    _call("flux_logits_process_workspace_bytes", rows, vocab, ctypes.byref(needed))
+    workspace = torch.empty(needed.value, dtype=torch.uint8, device=logits.device) if needed.value else None
+    with _on(logits.device):
+        _call("flux_logits_process", _TYPES[logits.dtype], logits.data_ptr(), logits.stride(0), processed.data_ptr(),
+              tokens.data_ptr(), rows, vocab, _address(history), 0 if history is None else history.shape[1],
+              0 if history is None else history.stride(0), _address(history_lengths), _address(repetition),
+              _address(frequency), _address(presence), _address(bias), _row_stride(bias), _address(allowed),
+              _row_stride(allowed), _address(workspace), needed.value, _stream(logits))
+    return processed, tokens
+
+
+# ---------------------------------------------------------------------------
+# Dispatcher registration.
+
+_KERNELS = {
+    "paged_decode_attention": (_paged_cuda, _validate_paged),
+    "paged_decode_attention_out": (_paged_out_cuda, _validate_paged_out),
+    "window_attention": (_window_cuda, _validate_window),
+    "paged_cache_reserve": (_reserve_cuda, _validate_reserve),
+    "paged_cache_write": (_write_cuda, _validate_write),
+    "paged_cache_copy": (_copy_cuda, _validate_copy),
+    "paged_cache_fork": (_fork_cuda, _validate_fork),
+    "paged_cache_free": (_free_cuda, _validate_free),
+    "paged_cache_compact": (_compact_cuda, _validate_compact),
+    "logits_process": (_logits_cuda, _validate_logits),
+}
+
+for _name, (_cuda, _validate) in _KERNELS.items():
+    _LIBRARY.impl(_name, _cuda, "CUDA")
+    _LIBRARY.impl(_name, _cpu_kernel(_name, _validate), "CPU")
+
+
+@torch.library.register_fake("flux::paged_decode_attention")
+def _paged_fake(query, key_pages, value_pages, page_table, lengths, scale, window=0, sinks=0, slots=None):
+    _validate_paged(query, key_pages, value_pages, page_table, lengths, scale, window, sinks, slots)
+    return query.new_empty(query.shape)
+
+
+@torch.library.register_fake("flux::paged_decode_attention_out")
+def _paged_out_fake(query, key_pages, value_pages, page_table, lengths, scale, window, sinks, slots, output, workspace):
+    _validate_paged(query, key_pages, value_pages, page_table, lengths, scale, window, sinks, slots)
+    return output
+
+
+@torch.library.register_fake("flux::window_attention")
+def _window_fake(query, key, value, scale, window, sinks=0, lengths=None, starts=None):
+    _validate_window(query, key, value, scale, window, sinks, lengths, starts)
+    return query.new_empty(query.shape)
+
+
+@torch.library.register_fake("flux::paged_cache_reserve")
+def _reserve_fake(page_table, lengths, refcounts, page_size, slots, counts=None):
+    _validate_reserve(page_table, lengths, refcounts, page_size, slots, counts)
+    return slots.new_empty(slots.shape), slots.new_empty(slots.shape, dtype=torch.int32)
+
+
+@torch.library.register_fake("flux::paged_cache_write")
+def _write_fake(key, value, key_pages, value_pages, page_table, slots, positions, counts=None):
+    return None
+
+
+@torch.library.register_fake("flux::paged_cache_copy")
+def _copy_fake(key_pages, value_pages, source, target):
+    return source.new_empty(source.shape, dtype=torch.int32)
+
+
+@torch.library.register_fake("flux::paged_cache_fork")
+def _fork_fake(key_pages, value_pages, page_table, lengths, refcounts, parents, children):
+    return parents.new_empty(parents.shape, dtype=torch.int32)
+
+
+@torch.library.register_fake("flux::paged_cache_free")
+def _free_fake(page_table, lengths, refcounts, slots):
+    _validate_free(page_table, lengths, refcounts, slots)
+    return slots.new_empty(slots.shape, dtype=torch.int32)
+
+
+@torch.library.register_fake("flux::paged_cache_compact")
+def _compact_fake(key_pages, value_pages, page_table, refcounts):
+    return refcounts.new_empty(refcounts.shape), refcounts.new_empty((), dtype=torch.int64)
+
+
+@torch.library.register_fake("flux::logits_process")
+def _logits_fake(logits, history=None, history_lengths=None, repetition=None, frequency=None, presence=None, bias=None,
+                 allowed=None):
+    _validate_logits(logits, history, history_lengths, repetition, frequency, presence, bias, allowed)
+    return logits.new_empty(logits.shape), logits.new_empty((logits.shape[0],), dtype=torch.int64)
+
+
+# ---------------------------------------------------------------------------
+# Python entry points.
+
+def native_paged_decode_attention_is_available() -> bool:
+    return _availability("paged_decode_attention", "paged_decode_attention_out")
+
+
+def native_window_attention_is_available() -> bool:
+    return _availability("window_attention")
+
+
+def native_paged_cache_is_available() -> bool:
+    return _availability(*(name for name in SERVING_SCHEMAS if name.startswith("paged_cache_")))
+
+
+def native_logits_process_is_available() -> bool:
+    return _availability("logits_process")
+
+
+def paged_decode_attention_native(query: torch.Tensor, key_pages: torch.Tensor, value_pages: torch.Tensor,
+                                  page_table: torch.Tensor, lengths: torch.Tensor, scale: float, window: int = 0,
+                                  sinks: int = 0, slots: torch.Tensor | None = None) -> torch.Tensor:
+    """One-token GQA attention of a batch over its cache pages; the new token's rows are already in them.
+
+    ``query`` [B, Hq, 1, D], pages [P, Hkv, page_size, D] (any strides, D contiguous); sequence b uses row ``slots[b]``
+    (b without slots) of ``page_table`` and ``lengths``.  ``window`` > 0 leaves the last ``window`` keys and the first
+    ``sinks`` visible.  Keys on an entry outside [0, P) are left out; a sequence that sees nothing gives zeros.
+    """
+    _require_library("paged decode attention")
+    return torch.ops.flux.paged_decode_attention(query, key_pages, value_pages, page_table, lengths, scale, window,
+                                                 sinks, slots)
+
+
+def paged_decode_attention_native_out(query: torch.Tensor, key_pages: torch.Tensor, value_pages: torch.Tensor,
+                                      page_table: torch.Tensor, lengths: torch.Tensor, scale: float, window: int,
+                                      sinks: int, slots: torch.Tensor | None, output: torch.Tensor,
+                                      workspace: torch.Tensor) -> torch.Tensor:
+    """The same into stable buffers (float32 workspace of at least ``paged_decode_workspace_bytes``); returns ``output``.
+
+    Calls that may overlap need workspaces of their own.
+    """
+    _require_library("paged decode attention out variant")
+    return torch.ops.flux.paged_decode_attention_out(query, key_pages, value_pages, page_table, lengths, scale, window,
+                                                     sinks, slots, output, workspace)
+
+
+def window_attention_native(query: torch.Tensor, key: torch.Tensor, value: torch.Tensor, scale: float, window: int,
+                            sinks: int = 0, lengths: torch.Tensor | None = None,
+                            starts: torch.Tensor | None = None) -> torch.Tensor:
+    """Causal GQA attention with a sliding window and sinks: prompts, chunks of them, single tokens.
+
+    ``query`` [B, Hq, S, D] over ``key``, ``value`` [B, Hkv, L, D].  Query i of sequence b is at position
+    ``starts[b] + i`` (default ``lengths[b] - S + i``, lengths by default L) and sees the keys j up to its own with
+    ``j > position - window`` or ``j < sinks``; window 0 leaves all of them visible.  Rows whose position is not a
+    key's give zeros: a padded batch of prompts passes ``starts`` of zeros and its lengths.
+    """
+    _require_library("window attention")
+    return torch.ops.flux.window_attention(query, key, value, scale, window, sinks, lengths, starts)
+
+
+def paged_cache_reserve_native(page_table: torch.Tensor, lengths: torch.Tensor, refcounts: torch.Tensor, page_size: int,
+                               slots: torch.Tensor, counts: torch.Tensor | None = None
+                               ) -> tuple[torch.Tensor, torch.Tensor]:
+    """Pages for the next ``counts`` (default one) tokens of ``slots``; returns (first positions, status).
+
+    Columns without a page get the lowest free ones, in the order of the requests, and ``lengths`` grow.  A request that
+    cannot be served changes nothing and has position -1.
+    """
+    _require_library("paged cache")
+    return torch.ops.flux.paged_cache_reserve(page_table, lengths, refcounts, page_size, slots, counts)
+
+
+def paged_cache_write_native(key: torch.Tensor, value: torch.Tensor, key_pages: torch.Tensor, value_pages: torch.Tensor,
+                             page_table: torch.Tensor, slots: torch.Tensor, positions: torch.Tensor,
+                             counts: torch.Tensor | None = None) -> None:
+    """Rows of new tokens ``key``, ``value`` [N, Hkv, S, D] of one layer to ``positions`` (and on) of ``slots``.
+
+    Only the first ``counts[i]`` tokens of request i are written.  Negative positions (refused reservations) and rows on
+    no page are skipped; two requests must not name the same rows.
+    """
+    _require_library("paged cache")
+    torch.ops.flux.paged_cache_write(key, value, key_pages, value_pages, page_table, slots, positions, counts)
+
+
+def paged_cache_copy_native(key_pages: torch.Tensor, value_pages: torch.Tensor, source: torch.Tensor,
+                            target: torch.Tensor) -> torch.Tensor:
+    """Pages ``source`` to pages ``target`` in all layers; returns the status of each pair."""
+    _require_library("paged cache")
+    return torch.ops.flux.paged_cache_copy(key_pages, value_pages, source, target)
+
+
+def paged_cache_fork_native(key_pages: torch.Tensor, value_pages: torch.Tensor, page_table: torch.Tensor,
+                            lengths: torch.Tensor, refcounts: torch.Tensor, parents: torch.Tensor,
+                            children: torch.Tensor) -> torch.Tensor:
+    """The empty slots ``children`` become branches of ``parents``; returns the status of each.
+
+    Full pages are shared, the rows of a partial last page are copied to a new page, so both may write on.
+    """
+    _require_library("paged cache")
+    return torch.ops.flux.paged_cache_fork(key_pages, value_pages, page_table, lengths, refcounts, parents, children)
+
+
+def paged_cache_free_native(page_table: torch.Tensor, lengths: torch.Tensor, refcounts: torch.Tensor,
+                            slots: torch.Tensor) -> torch.Tensor:
+    """Empties ``slots``: their pages lose a holder each, and those without one are free; returns the status of each."""
+    _require_library("paged cache")
+    return torch.ops.flux.paged_cache_free(page_table, lengths, refcounts, slots)
+
+
+def paged_cache_compact_native(key_pages: torch.Tensor, value_pages: torch.Tensor, page_table: torch.Tensor,
+                               refcounts: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
+    """Moves the pages in use to the front of the pool; returns (page_map int32 [P], pages in use).
+
+    ``page_table`` and ``refcounts`` follow; ``page_map`` gives each page's new place (-1: free) for what else names one.
+    """
+    _require_library("paged cache")
+    return torch.ops.flux.paged_cache_compact(key_pages, value_pages, page_table, refcounts)
+
+
+def logits_process_native(logits: torch.Tensor, history: torch.Tensor | None = None,
+                          history_lengths: torch.Tensor | None = None, repetition: torch.Tensor | None = None,
+                          frequency: torch.Tensor | None = None, presence: torch.Tensor | None = None,
+                          bias: torch.Tensor | None = None, allowed: torch.Tensor | None = None
+                          ) -> tuple[torch.Tensor, torch.Tensor]:
+    """Penalties, bias and grammar mask on ``logits`` [rows, vocab]; returns (processed logits, greedy tokens).
+
+    A token that occurs c > 0 times in the first ``history_lengths`` ids of the row's ``history`` becomes ``x /
+    repetition`` (``x * repetition`` when not positive), minus ``frequency * c``, minus ``presence``; then ``bias`` is
+    added and tokens whose bit of ``allowed`` (bit v % 32 of word v // 32) is clear become -inf.  The greedy token is the
+    lowest index of the largest processed logit (NaN above all numbers).
+    """
+    _require_library("logits process")
+    return torch.ops.flux.logits_process(logits, history, history_lengths, repetition, frequency, presence, bias, allowed)
+
+
+SERVING_OPERATOR_NAMES = tuple(SERVING_SCHEMAS)

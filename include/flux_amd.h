@@ -454,6 +454,125 @@ int flux_gqa_decode_attention_strided_f32(const float* query, const float* key_c
                                           const int64_t* value_strides, const int64_t* mask_sizes,
                                           const int64_t* mask_strides, hipStream_t stream);
 
+/* ---- Serving: a paged K/V cache, windowed attention, logits ----
+ * Element type of query, key, value, cache pages and logits.  Strides are in elements and non-negative; the head
+ * dimension of keys, values and pages has stride 1.  Softmax statistics and sums are float32 (integers for counts). */
+enum flux_dtype { FLUX_FLOAT32 = 0, FLUX_FLOAT16 = 1, FLUX_BFLOAT16 = 2 };
+
+/* One new token per sequence over a paged cache.  Sequence b uses row r = slots[b] (b when slots is NULL) of
+ * page_table [slot_count, columns] (int32) and of lengths [slot_count] (NULL: columns * page_size); its key j lies in
+ * row j % page_size of page page_table[r][j / page_size] of key_pages [pages, kv_heads, page_size, head_dim].  It sees
+ * the keys j < lengths[r] (clamped to columns * page_size) and, with window > 0, of those j >= lengths[r] - window and
+ * j < sinks.  Keys on a page outside [0, pages) are left out and never read; a sequence that sees nothing, or whose
+ * row is outside the table, gives zeros.  query [batch, query_heads, 1, head_dim], output contiguous.
+ * head_dim <= 256, columns * page_size <= FLUX_MAX_SERVING_KEYS. */
+#define FLUX_MAX_SERVING_KEYS (1 << 24)
+int flux_paged_decode_attention_workspace_bytes(int64_t batch, int64_t query_heads, int64_t kv_heads, int64_t head_dim,
+                                                int64_t keys, int64_t window, int64_t sinks, int64_t* bytes);
+int flux_paged_decode_attention(int dtype, const void* query, const void* key_pages, const void* value_pages,
+                                const int32_t* page_table, const int64_t* lengths, const int64_t* slots, void* output,
+                                void* workspace, int64_t workspace_bytes, float scale, int64_t batch,
+                                int64_t query_heads, int64_t kv_heads, int64_t head_dim, int64_t pages,
+                                int64_t page_size, int64_t slot_count, int64_t columns, int64_t table_stride,
+                                int64_t window, int64_t sinks, const int64_t* query_strides,
+                                const int64_t* key_strides, const int64_t* value_strides, hipStream_t stream);
+
+/* Causal attention with a sliding window and sinks over key, value [batch, kv_heads, keys, head_dim].  The query i of
+ * sequence b has position p = starts[b] + i (NULL: lengths[b] - queries + i) and sees the keys j <= p, j < lengths[b]
+ * (NULL: keys; clamped to keys) with j > p - window or j < sinks (window 0: all); a row that sees nothing or with
+ * p outside [0, lengths[b]) gives zeros.  query [batch, query_heads, queries, head_dim], output contiguous.  The
+ * workspace is needed for single queries only. */
+int flux_window_attention_workspace_bytes(int64_t batch, int64_t query_heads, int64_t kv_heads, int64_t queries,
+                                          int64_t head_dim, int64_t keys, int64_t window, int64_t sinks,
+                                          int64_t* bytes);
+int flux_window_attention(int dtype, const void* query, const void* key, const void* value, const int64_t* lengths,
+                          const int64_t* starts, void* output, void* workspace, int64_t workspace_bytes, float scale,
+                          int64_t batch, int64_t query_heads, int64_t kv_heads, int64_t queries, int64_t keys,
+                          int64_t head_dim, int64_t window, int64_t sinks, const int64_t* query_strides,
+                          const int64_t* key_strides, const int64_t* value_strides, hipStream_t stream);
+
+/* Pages of a cache.  The books: page_table int32 [slots, columns] (-1: no page), lengths int64 [slots], refcounts
+ * int32 [pages] (sequences that hold a page; 0: free).  Requests are served in their order, a needed page is the
+ * lowest free one, and what became of each request is its flux_page_status; a refused request changes nothing. */
+enum flux_page_status {
+    FLUX_PAGE_DONE = 0,
+    FLUX_PAGE_OUT_OF_RANGE = 1, /* a slot, page, count or length outside its range */
+    FLUX_PAGE_REPEATED = 2,     /* an earlier request of the call names it, or (copy) the target is also a source */
+    FLUX_PAGE_NO_ROOM = 3,      /* not enough free pages, or the slot's row is too short */
+    FLUX_PAGE_OCCUPIED = 4      /* the child of a fork holds tokens or pages */
+};
+typedef struct {
+    int32_t* page_table;
+    int64_t table_stride;
+    int64_t slots;
+    int64_t columns;
+    int64_t* lengths;
+    int32_t* refcounts;
+    int64_t pages;
+    int64_t page_size;
+} flux_page_books;
+/* key, value [layers, pages, heads, page_size, head_dim]; strides of the first four dimensions. */
+typedef struct {
+    void* key;
+    void* value;
+    int64_t layers;
+    int64_t pages;
+    int64_t heads;
+    int64_t page_size;
+    int64_t head_dim;
+    int64_t key_strides[4];
+    int64_t value_strides[4];
+    int64_t dtype;
+} flux_page_pool;
+
+/* Pages for the next counts[i] (NULL: 1) tokens of slots[i]: columns without one get the lowest free pages, lengths
+ * grow, positions[i] is the first new token's position, -1 when refused.  Requests are served until pages run out:
+ * one is refused when it and all before it need more pages than are free.  workspace: int32 words from
+ * flux_page_reserve_workspace_words. */
+int flux_page_reserve_workspace_words(int64_t requests, int64_t slots, int64_t pages, int64_t* words);
+int flux_page_reserve(const flux_page_books* books, const int64_t* slots, const int64_t* counts, int64_t requests,
+                      int64_t* positions, int32_t* status, int32_t* workspace, int64_t workspace_words,
+                      hipStream_t stream);
+/* Rows of new tokens into one layer's pages (layers 1): key, value [requests, heads, tokens, head_dim], token t < counts[i]
+ * (NULL: tokens) of request i to position positions[i] + t of slots[i].  Requests with a negative position or a slot
+ * outside the table, tokens beyond the table's columns and tokens on no page are left out. */
+int flux_page_write(const flux_page_pool* pool, const void* key, const void* value, const int64_t* key_strides,
+                    const int64_t* value_strides, int64_t requests, int64_t tokens, const int32_t* page_table,
+                    int64_t table_stride, int64_t slots, int64_t columns, const int64_t* slot_list,
+                    const int64_t* positions, const int64_t* counts, hipStream_t stream);
+/* Page source[i] to page target[i], all layers. */
+int flux_page_copy(const flux_page_pool* pool, const int64_t* source, const int64_t* target, int64_t requests,
+                   int32_t* status, hipStream_t stream);
+/* Gives the pages of slots[i] back (refcounts stay at or above 0); its row becomes -1 and its length 0. */
+int flux_page_free(const flux_page_books* books, const int64_t* slots, int64_t requests, int32_t* status,
+                   hipStream_t stream);
+/* The empty slot children[i] becomes a branch of parents[i], as the books were before the call: full pages are
+ * shared, the rows of a partial last page are copied to a new one. */
+int flux_page_fork_workspace_words(int64_t requests, int64_t slots, int64_t pages, int64_t* words);
+int flux_page_fork(const flux_page_pool* pool, const flux_page_books* books, const int64_t* parents,
+                   const int64_t* children, int64_t requests, int32_t* status, int32_t* workspace,
+                   int64_t workspace_words, hipStream_t stream);
+/* Moves the U pages in use to [0, U): the k-th one at or above U to the k-th free one below it; page_table and
+ * refcounts follow.  page_map [pages]: the new place of each page, -1 for free ones; *used = U (device). */
+int flux_page_compact_workspace_words(int64_t pages, int64_t* words);
+int flux_page_compact(const flux_page_pool* pool, const flux_page_books* books, int32_t* page_map, int64_t* used,
+                      int32_t* workspace, int64_t workspace_words, hipStream_t stream);
+
+/* logits [rows, vocab] (row stride logits_stride) on their way to the next token:
+ *   c = occurrences of v among the first history_lengths[row] (NULL: history_width) ids of history [rows, history_width]
+ *       (ids outside the vocabulary count for nothing)
+ *   c > 0: x = x > 0 ? x / repetition : x * repetition; x -= frequency * c; x -= presence    (float32 [rows], NULL: none)
+ *   x += bias (float32, row stride bias_stride, 0: one row for all); not allowed: -inf (bit v % 32 of word v / 32)
+ * output contiguous in the logits' type, rounded once; tokens[row] = lowest index of the largest output, NaN above
+ * all numbers. */
+int flux_logits_process_workspace_bytes(int64_t rows, int64_t vocab, int64_t* bytes);
+int flux_logits_process(int dtype, const void* logits, int64_t logits_stride, void* output, int64_t* tokens,
+                        int64_t rows, int64_t vocab, const int64_t* history, int64_t history_width,
+                        int64_t history_stride, const int64_t* history_lengths, const float* repetition,
+                        const float* frequency, const float* presence, const float* bias, int64_t bias_stride,
+                        const int32_t* allowed, int64_t allowed_stride, void* workspace, int64_t workspace_bytes,
+                        hipStream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -1,0 +1,741 @@
+"""GPU parity of the serving operators against plain float64 forms (``oracle/serving.py``) and Python page books.
+
+Tolerances of the attention operators are computed from the inputs (``oracle.serving.attention_bound``); everything that
+moves values or counts is exact, and processed logits are the float32 operations of the definition rounded once.
+"""
+
+from __future__ import annotations
+
+import math
+import random
+
+import pytest
+import torch
+
+from flux_amd import ops
+from oracle import serving as ref
+
+pytestmark = pytest.mark.gpu
+
+TYPES = (torch.float32, torch.float16, torch.bfloat16)
+
+
+def _close(actual, expected, bound):
+    error = (actual.cpu().double() - expected).abs()
+    beyond = float((error - bound).nan_to_num(nan=math.inf).max())
+    assert beyond <= 0, f"off by {beyond:.3g} beyond the bound, at most {float(error.max()):.3g}"
+
+
+def _randn(g, shape, dtype):
+    return torch.randn(shape, generator=g).to(dtype)
+
+
+def _paged_case(seed, dtype, heads, kv_heads, dim, page_size, lengths, spare=3, scale=None):
+    """CPU tensors of a batch whose pages lie scattered in the pool."""
+    g = torch.Generator().manual_seed(seed)
+    columns = max(1, -(-max(max(lengths), 1) // page_size))
+    needed = [-(-n // page_size) for n in lengths]
+    pages = sum(needed) + spare
+    order = torch.randperm(pages, generator=g).tolist()
+    table = torch.full((len(lengths), columns), -1, dtype=torch.int32)
+    for b, count in enumerate(needed):
+        for c in range(count):
+            table[b, c] = order.pop()
+    return {"query": _randn(g, (len(lengths), heads, 1, dim), dtype),
+            "key_pages": _randn(g, (pages, kv_heads, page_size, dim), dtype),
+            "value_pages": _randn(g, (pages, kv_heads, page_size, dim), dtype),
+            "page_table": table, "lengths": torch.tensor(lengths), "scale": scale or dim ** -0.5}
+
+
+def _to(case, device):
+    return {k: v.to(device) if isinstance(v, torch.Tensor) else v for k, v in case.items()}
+
+
+def _check_paged(case, device, actual=None, **options):
+    expected = ref.paged_decode(**case, **{k: v.cpu() if isinstance(v, torch.Tensor) else v for k, v in options.items()})
+    if actual is None:
+        options = {k: v.to(device) if isinstance(v, torch.Tensor) else v for k, v in options.items()}
+        actual = ops.paged_decode_attention_native(**_to(case, device), **options)
+    assert actual.dtype == case["query"].dtype and actual.is_contiguous() and actual.shape == expected.shape
+    terms = int(min(case["lengths"].max(), case["page_table"].shape[1] * case["key_pages"].shape[2]))
+    _close(actual, expected, ref.attention_bound(case["query"], case["key_pages"].nan_to_num(), case["value_pages"].nan_to_num(),
+                                                 case["scale"], max(terms, 1), case["query"].dtype, expected))
+    return actual
+
+
+# --------------------------------------------------------------------------- paged decode
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("dim,page_size", [(64, 16), (128, 64), (256, 16), (80, 48), (72, 7), (40, 1), (100, 5), (5, 3),
+                                           (1, 4), (192, 100), (33, 16)])
+def test_paged_decode_heads_and_pages(gpu_device, dtype, dim, page_size):
+    lengths = [1, 0, 15, 16, 17, 31, 33, 64, 127, 200, 301]
+    for heads, kv_heads in ((9, 3), (4, 4), (20, 1)):
+        case = _paged_case(dim + page_size, dtype, heads, kv_heads, dim, page_size, lengths)
+        out = _check_paged(case, gpu_device)
+        assert not out[1].any()
+
+
+@pytest.mark.parametrize("window,sinks", [(0, 0), (0, 9), (1, 0), (1, 1), (16, 0), (31, 4), (32, 33), (100, 1), (150, 64),
+                                          (1000, 5), (1 << 24, 1 << 24)])
+@pytest.mark.parametrize("dtype,dim,page_size", [(torch.float32, 64, 16), (torch.bfloat16, 128, 24),
+                                                 (torch.float16, 256, 33)])
+def test_paged_decode_windows(gpu_device, dtype, dim, page_size, window, sinks):
+    case = _paged_case(7, dtype, 6, 2, dim, page_size, [1, 0, 2, 16, 32, 33, 101, 130, 257, 400])
+    _check_paged(case, gpu_device, window=window, sinks=sinks)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_paged_decode_long_and_large_batches(gpu_device, dtype):
+    """Sequences that are cut over many workgroups next to short ones, and more sequences than one round's threads."""
+    _check_paged(_paged_case(1, dtype, 3, 1, 64, 16, [9000, 3, 700, 0, 5000]), gpu_device)
+    rng = random.Random(2)
+    lengths = [rng.choice((0, 1, 5, 40, 90)) for _ in range(601)]
+    lengths[0] = lengths[300] = 0
+    _check_paged(_paged_case(3, dtype, 2, 2, 32, 8, lengths), gpu_device)
+
+
+def test_paged_decode_one_sequence_at_every_length(gpu_device):
+    case = _paged_case(11, torch.float32, 9, 3, 64, 16, [300])
+    device = _to(case, gpu_device)
+    for n in [*range(0, 70), 127, 128, 129, 255, 256, 257, 299, 300]:
+        case["lengths"] = torch.tensor([n])
+        device["lengths"] = case["lengths"].to(gpu_device)
+        _check_paged(case, gpu_device, ops.paged_decode_attention_native(**device))
+
+
+def test_paged_decode_slots_lengths_and_bad_pages(gpu_device):
+    case = _paged_case(13, torch.float32, 6, 2, 64, 16, [50, 200, 33, 120])
+    # Rows in another order, twice, and outside the table; lengths beyond the columns and negative ones.
+    case["query"] = torch.randn(7, 6, 1, 64, generator=torch.Generator().manual_seed(1))
+    slots = torch.tensor([2, 0, 4, -1, 1, 1, 3])
+    out = _check_paged(case, gpu_device, slots=slots)
+    assert not out[2].any() and not out[3].any()
+    case["lengths"] = torch.tensor([1 << 40, -5, 33, 120])
+    _check_paged(case, gpu_device, slots=slots)
+    # Entries outside the pool are left out: the sequence attends over the others.
+    case["lengths"] = torch.tensor([50, 200, 33, 120])
+    case["page_table"][0, 1] = -1
+    case["page_table"][1, 3] = case["key_pages"].shape[0]
+    case["page_table"][1, 4] = 2 ** 31 - 1
+    case["page_table"][2] = -7
+    out = _check_paged(case, gpu_device, slots=slots)
+    assert not out[0].any()
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_paged_decode_strides_and_alignment(gpu_device, dtype):
+    case = _paged_case(17, dtype, 6, 2, 64, 16, [50, 200, 33, 120])
+    expected = ops.paged_decode_attention_native(**_to(case, gpu_device))
+    device = _to(case, gpu_device)
+    # [P, page, heads, D] pages, a table inside a wider one, a query inside a packed projection, another dim stride.
+    moved = dict(device)
+    for name in ("key_pages", "value_pages"):
+        moved[name] = device[name].transpose(1, 2).contiguous().transpose(1, 2)
+    wide = torch.full((4, 40), 99, dtype=torch.int32, device=gpu_device)
+    wide[:, 3:3 + device["page_table"].shape[1]] = device["page_table"]
+    moved["page_table"] = wide[:, 3:3 + device["page_table"].shape[1]]
+    packed = torch.randn(4, 3, 6, 64, device=gpu_device).to(dtype)
+    packed[:, 1] = device["query"][:, :, 0]
+    moved["query"] = packed[:, 1].unsqueeze(2)
+    assert torch.equal(ops.paged_decode_attention_native(**moved), expected)
+    moved["query"] = device["query"].transpose(1, 3).contiguous().transpose(1, 3)
+    assert torch.equal(ops.paged_decode_attention_native(**moved), expected)
+    # Rows that start at no 16 bytes.
+    for name in ("key_pages", "value_pages"):
+        shape = device[name].shape
+        store = torch.randn(shape[0], shape[1], shape[2], 67, device=gpu_device).to(dtype)
+        store[..., 1:65] = device[name]
+        moved[name] = store[..., 1:65]
+    torch.testing.assert_close(ops.paged_decode_attention_native(**moved), expected, rtol=0, atol=0)
+
+
+def test_paged_decode_ignores_what_lies_behind(gpu_device):
+    """NaN and infinity in rows behind the length, before the window and on other pages."""
+    case = _paged_case(19, torch.bfloat16, 8, 2, 128, 16, [50, 200, 33, 120])
+    window, sinks = 20, 3
+    clean = ops.paged_decode_attention_native(**_to(case, gpu_device), window=window, sinks=sinks)
+    seen = torch.zeros(case["key_pages"].shape[0], 16, dtype=torch.bool)
+    for b, n in enumerate(case["lengths"].tolist()):
+        for j in ref.visible_keys(n - 1, n, window, sinks):
+            seen[int(case["page_table"][b, j // 16]), j % 16] = True
+    for bad in (math.nan, math.inf, -math.inf):
+        for name in ("key_pages", "value_pages"):
+            case[name] = torch.where(seen[:, None, :, None], case[name], torch.tensor(bad, dtype=torch.bfloat16))
+        assert torch.equal(ops.paged_decode_attention_native(**_to(case, gpu_device), window=window, sinks=sinks), clean)
+
+
+def test_paged_decode_nan_and_large_scores(gpu_device):
+    case = _paged_case(23, torch.float32, 2, 1, 64, 16, [40, 40])
+    page = int(case["page_table"][1, 1])
+    case["value_pages"][page, 0, 3, 7] = math.nan
+    out = ops.paged_decode_attention_native(**_to(case, gpu_device)).cpu()
+    assert out[0].isfinite().all() and out[1, :, 0, 7].isnan().all()
+    assert out[1, :, 0].isnan().sum() == 2
+    case["key_pages"][page, 0, 3] = math.nan
+    assert ops.paged_decode_attention_native(**_to(case, gpu_device)).cpu()[1].isnan().all()
+    # Scores around 1e38 leave the largest one alone.
+    case = _paged_case(29, torch.float32, 1, 1, 64, 16, [70])
+    case["query"] = torch.full_like(case["query"], 1e18)
+    case["key_pages"] = case["key_pages"].abs() * 1e18
+    case["scale"] = 1.0
+    out = ops.paged_decode_attention_native(**_to(case, gpu_device)).cpu().double()
+    expected = ref.paged_decode(**case)
+    torch.testing.assert_close(out, expected, rtol=1e-6, atol=0)
+
+
+def test_paged_decode_many_small_weights_in_float16(gpu_device):
+    """One key far above 8000 others whose weights are below float16's smallest step together weigh a fifth."""
+    n = 8192
+    case = _paged_case(31, torch.float16, 1, 1, 64, 64, [n], scale=1.0)
+    case["query"] = torch.zeros(1, 1, 1, 64, dtype=torch.float16)
+    case["query"][..., 0] = 1.0
+    case["key_pages"] = torch.zeros_like(case["key_pages"])
+    case["key_pages"][..., 0] = -10.5
+    first = int(case["page_table"][0, 0])
+    case["key_pages"][first, 0, 0, 0] = 0.0
+    case["value_pages"] = torch.ones_like(case["value_pages"])
+    case["value_pages"][first, 0, 0] = -1.0
+    out = ops.paged_decode_attention_native(**_to(case, gpu_device)).cpu().double()
+    rest = (n - 1) * math.exp(-10.5)
+    expected = (rest - 1) / (rest + 1)
+    assert abs(float(out[0, 0, 0, 5]) - expected) <= 2.0 ** -11 * abs(expected) + 1e-5
+
+
+def test_paged_decode_out_streams_and_reuse(gpu_device):
+    case = _paged_case(37, torch.float32, 9, 3, 64, 16, [900, 30, 2000])
+    device = _to(case, gpu_device)
+    expected = _check_paged(case, gpu_device)
+    needed = ops.paged_decode_workspace_bytes(device["query"], device["key_pages"], device["page_table"])
+    output = torch.full_like(device["query"], 7.0)
+    workspace = torch.full((needed // 4 + 64,), math.nan, device=gpu_device)
+    call = lambda o, w: ops.paged_decode_attention_native_out(*device.values(), 0, 0, None, o, w)  # noqa: E731
+    assert call(output, workspace) is output
+    assert torch.equal(output, expected) and workspace[needed // 4:].isnan().all()
+    with pytest.raises(RuntimeError, match="workspace is too small"):
+        call(output, workspace[: needed // 4 - 1])
+    stream = torch.cuda.Stream()
+    stream.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(stream):
+        others = [ops.paged_decode_attention_native(**device) for _ in range(3)]
+    here = [ops.paged_decode_attention_native(**device) for _ in range(3)]
+    torch.cuda.synchronize()
+    assert all(torch.equal(t, expected) for t in others + here)
+
+
+def test_paged_decode_matches_the_one_sequence_operator(gpu_device):
+    g = torch.Generator().manual_seed(41)
+    cache = torch.randn(2, 1, 3, 1024, 64, generator=g).to(gpu_device)
+    query = torch.randn(1, 9, 1, 64, generator=g).to(gpu_device)
+    length = torch.tensor(777, device=gpu_device)
+    one = ops.gqa_decode_attention_native(query, cache[0], cache[1], None, 0.125, length)
+    pages = [c[0].view(3, 64, 16, 64).transpose(0, 1) for c in cache]
+    table = torch.arange(64, dtype=torch.int32, device=gpu_device)[None]
+    paged = ops.paged_decode_attention_native(query, *pages, table, length[None], 0.125)
+    whole = ops.window_attention_native(query, cache[0], cache[1], 0.125, 0, 0, length[None])
+    torch.testing.assert_close(paged, one, rtol=2e-5, atol=1e-6)
+    torch.testing.assert_close(whole, one, rtol=2e-5, atol=1e-6)
+
+
+# --------------------------------------------------------------------------- window attention
+
+def _window_case(seed, dtype, batch, heads, kv_heads, dim, queries, keys):
+    g = torch.Generator().manual_seed(seed)
+    return {"query": _randn(g, (batch, heads, queries, dim), dtype), "key": _randn(g, (batch, kv_heads, keys, dim), dtype),
+            "value": _randn(g, (batch, kv_heads, keys, dim), dtype), "scale": dim ** -0.5}
+
+
+def _check_window(case, device, window, sinks=0, lengths=None, starts=None):
+    lengths = None if lengths is None else torch.tensor(lengths)
+    starts = None if starts is None else torch.tensor(starts)
+    expected = ref.window_attention(**case, window=window, sinks=sinks, lengths=lengths, starts=starts)
+    actual = ops.window_attention_native(**_to(case, device), window=window, sinks=sinks,
+                                         lengths=None if lengths is None else lengths.to(device),
+                                         starts=None if starts is None else starts.to(device))
+    assert actual.dtype == case["query"].dtype and actual.is_contiguous()
+    terms = case["key"].shape[2] if window == 0 else min(case["key"].shape[2], window + sinks)
+    _close(actual, expected, ref.attention_bound(case["query"], case["key"], case["value"], case["scale"], max(terms, 1),
+                                                 case["query"].dtype, expected))
+    return actual
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("dim,heads,kv_heads", [(64, 9, 3), (128, 8, 2), (256, 2, 1), (80, 3, 3), (72, 5, 1), (40, 20, 1),
+                                                (100, 2, 2), (5, 4, 2), (1, 1, 1), (192, 2, 1)])
+def test_window_heads(gpu_device, dtype, dim, heads, kv_heads):
+    for queries, keys in ((2, 2), (35, 35), (17, 90), (1, 70)):
+        _check_window(_window_case(dim, dtype, 2, heads, kv_heads, dim, queries, keys), gpu_device, 20, 3)
+
+
+@pytest.mark.parametrize("dtype,dim", [(torch.float32, 64), (torch.float16, 64), (torch.bfloat16, 128), (torch.float32, 128)])
+@pytest.mark.parametrize("window,sinks", [(0, 0), (0, 3), (1, 0), (1, 1), (2, 0), (16, 0), (31, 4), (33, 40), (64, 1),
+                                          (150, 0), (1 << 24, 1 << 24)])
+def test_window_sizes(gpu_device, dtype, dim, window, sinks):
+    _check_window(_window_case(3, dtype, 1, 3, 1, dim, 150, 150), gpu_device, window, sinks)
+    _check_window(_window_case(5, dtype, 1, 2, 2, dim, 40, 170), gpu_device, window, sinks)
+    _check_window(_window_case(6, dtype, 1, 2, 2, dim, 1, 170), gpu_device, window, sinks)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_window_padded_batches_and_chunks(gpu_device, dtype):
+    case = _window_case(9, dtype, 5, 6, 2, 64, 70, 70)
+    out = _check_window(case, gpu_device, 16, 2, lengths=[70, 1, 0, 33, 64], starts=[0] * 5)
+    assert not out[2].any() and not out[3, :, 33:].any()
+    # Chunks of longer prompts; positions before the first and behind the last key see nothing.
+    case = _window_case(10, dtype, 5, 6, 2, 64, 20, 100)
+    _check_window(case, gpu_device, 16, 2, lengths=[100, 37, 20, 90, 500], starts=[80, 17, 0, 85, -5])
+    _check_window(case, gpu_device, 16, 2, lengths=[100, 12, 0, 90, -3])
+    _check_window(case, gpu_device, 0, 0, lengths=[100] * 5, starts=[-(2 ** 62), 2 ** 62, 99, -19, -20])
+    case = _window_case(12, dtype, 5, 6, 2, 64, 1, 100)
+    _check_window(case, gpu_device, 16, 2, lengths=[100, 37, 0, 90, 500], starts=[50, 36, 0, 90, -1])
+
+
+@pytest.mark.parametrize("dtype,dim", [(torch.float32, 64), (torch.bfloat16, 128)])
+def test_window_longer_prompts(gpu_device, dtype, dim):
+    """Against the formula in float64 as one product on the CPU, many tiles deep."""
+    case = _window_case(21, dtype, 1, 6, 2, dim, 1500, 1500)
+    for window, sinks in ((256, 4), (0, 0)):
+        p, j = torch.arange(1500)[:, None], torch.arange(1500)
+        seen = (j <= p) & ((j > p - window) | (j < sinks) if window else j >= 0)
+        keys, values = (case[k].double().repeat_interleave(3, dim=1) for k in ("key", "value"))
+        scores = (case["query"].double() @ keys.transpose(2, 3) * case["scale"]).masked_fill(~seen, -math.inf)
+        expected = torch.softmax(scores, -1) @ values
+        actual = ops.window_attention_native(**_to(case, gpu_device), window=window, sinks=sinks)
+        _close(actual, expected, ref.attention_bound(case["query"], case["key"], case["value"], case["scale"], 1500, dtype,
+                                                     expected))
+
+
+@pytest.mark.parametrize("dtype,dim", [(torch.float32, 64), (torch.bfloat16, 64), (torch.float16, 128)])
+def test_window_strides(gpu_device, dtype, dim):
+    case = _to(_window_case(25, dtype, 2, 6, 2, dim, 70, 70), gpu_device)
+    expected = ops.window_attention_native(**case, window=30, sinks=2)
+    rows = {k: case[k].transpose(1, 2).contiguous().transpose(1, 2) for k in ("query", "key", "value")}
+    assert torch.equal(ops.window_attention_native(**rows, scale=case["scale"], window=30, sinks=2), expected)
+    odd = dict(rows)
+    for name in ("key", "value"):
+        store = torch.randn(2, 2, 70, dim + 3, device=gpu_device).to(dtype)
+        store[..., 1:dim + 1] = case[name]
+        odd[name] = store[..., 1:dim + 1]
+    odd["query"] = case["query"].transpose(1, 3).contiguous().transpose(1, 3)
+    assert torch.equal(ops.window_attention_native(**odd, scale=case["scale"], window=30, sinks=2), expected)
+    # One key row for all positions (a stride of zero) is a broadcast like any other.
+    one = {k: case[k][:, :, :1].expand(2, 2, 70, dim) for k in ("key", "value")}
+    out = ops.window_attention_native(case["query"], **one, scale=case["scale"], window=30, sinks=2)
+    torch.testing.assert_close(out, one["value"].repeat_interleave(3, 1).contiguous(), rtol=2 * torch.finfo(dtype).eps, atol=1e-6)
+
+
+@pytest.mark.parametrize("dtype,dim", [(torch.float32, 64), (torch.bfloat16, 128), (torch.float16, 64)])
+def test_window_nan_reaches_only_the_rows_that_see_it(gpu_device, dtype, dim):
+    case = _window_case(27, dtype, 1, 4, 2, dim, 120, 120)
+    window, sinks = 16, 2
+    clean = ops.window_attention_native(**_to(case, gpu_device), window=window, sinks=sinks).cpu()
+    for name in ("key", "value"):
+        for bad, at in ((math.nan, 50), (math.inf, 51), (-math.inf, 1), (math.nan, 119)):
+            dirty = {**case, name: case[name].clone()}
+            dirty[name][0, 0, at, 3] = bad
+            out = ops.window_attention_native(**_to(dirty, gpu_device), window=window, sinks=sinks).cpu()
+            expected = ref.window_attention(**dirty, window=window, sinks=sinks)
+            assert torch.equal(out[0, 2:], clean[0, 2:])
+            for i in range(120):
+                if at not in ref.visible_keys(i, 120, window, sinks):
+                    torch.testing.assert_close(out[0, :2, i], clean[0, :2, i], rtol=4 * torch.finfo(dtype).eps, atol=1e-4)
+                else:
+                    assert torch.equal(out[0, :2, i].isnan(), expected[0, :2, i].isnan()), (name, bad, at, i)
+
+
+def test_window_other_stream_and_graph(gpu_device):
+    case = _to(_window_case(33, torch.bfloat16, 2, 8, 2, 64, 90, 90), gpu_device)
+    lengths, starts = torch.tensor([90, 40], device=gpu_device), torch.zeros(2, dtype=torch.int64, device=gpu_device)
+    expected = ops.window_attention_native(**case, window=20, lengths=lengths, starts=starts)
+    stream = torch.cuda.Stream()
+    stream.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(stream):
+        other = ops.window_attention_native(**case, window=20, lengths=lengths, starts=starts)
+    torch.cuda.synchronize()
+    assert torch.equal(other, expected)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        captured = ops.window_attention_native(**case, window=20, lengths=lengths, starts=starts)
+    for n in (40, 77, 1):
+        lengths[1] = n
+        case["query"].mul_(0.5)
+        graph.replay()
+        assert torch.equal(captured, ops.window_attention_native(**case, window=20, lengths=lengths, starts=starts))
+
+
+# --------------------------------------------------------------------------- pages
+
+class _Device:
+    """The pages of ``ref.Pages`` on the GPU, next to it."""
+
+    def __init__(self, model, device):
+        self.model, self.device = model, device
+        self.key, self.value = model.key.to(device), model.value.to(device)
+        self.table = torch.tensor(model.table, dtype=torch.int32, device=device)
+        self.lengths = torch.tensor(model.lengths, device=device)
+        self.refcounts = torch.tensor(model.refcounts, dtype=torch.int32, device=device)
+
+    @property
+    def books(self):
+        return self.table, self.lengths, self.refcounts
+
+    def ids(self, values):
+        return torch.tensor(values, dtype=torch.int64, device=self.device)
+
+    def same(self):
+        assert self.table.tolist() == self.model.table
+        assert self.lengths.tolist() == self.model.lengths
+        assert self.refcounts.tolist() == self.model.refcounts
+        assert torch.equal(self.key.cpu(), self.model.key) and torch.equal(self.value.cpu(), self.model.value)
+
+    def reserve(self, slots, counts):
+        positions, status = ops.paged_cache_reserve_native(*self.books, self.model.page_size, self.ids(slots), self.ids(counts))
+        assert (positions.tolist(), status.tolist()) == self.model.reserve(slots, counts)
+        return positions
+
+    def write(self, layer, key, value, slots, positions, counts):
+        ops.paged_cache_write_native(key.to(self.device), value.to(self.device), self.key[layer], self.value[layer],
+                                     self.table, self.ids(slots), positions, self.ids(counts))
+        self.model.write(layer, key, value, slots, positions.tolist(), counts)
+
+    def copy(self, source, target):
+        status = ops.paged_cache_copy_native(self.key, self.value, self.ids(source), self.ids(target))
+        assert status.tolist() == self.model.copy(source, target)
+
+    def free(self, slots):
+        assert ops.paged_cache_free_native(*self.books, self.ids(slots)).tolist() == self.model.free(slots)
+
+    def fork(self, parents, children):
+        status = ops.paged_cache_fork_native(self.key, self.value, *self.books, self.ids(parents), self.ids(children))
+        expected = self.model.fork(parents, children)
+        assert status.tolist() == expected
+        return expected
+
+    def compact(self):
+        page_map, used = ops.paged_cache_compact_native(self.key, self.value, self.table, self.refcounts)
+        assert (page_map.tolist(), int(used)) == self.model.compact()
+
+
+@pytest.mark.parametrize("dtype,dim,page_size,layers", [(torch.float32, 64, 16, 2), (torch.bfloat16, 40, 5, 3),
+                                                        (torch.float16, 7, 3, 1), (torch.float32, 3, 1, 2)])
+def test_pages_in_random_order(gpu_device, dtype, dim, page_size, layers):
+    """Every operator against the lists, requests out of range, repeated and beyond the pool among them."""
+    rng = random.Random(dim)
+    slots, columns = 9, 6
+    model = ref.Pages(layers, 24, 2, page_size, dim, slots, columns, dtype, seed=dim)
+    pages = _Device(model, gpu_device)
+    g = torch.Generator().manual_seed(1)
+    seen = set()
+    for _ in range(120):
+        action = rng.choice(("grow", "grow", "grow", "fork", "free", "compact", "copy"))
+        count = rng.randint(1, 5)
+        some = [rng.randint(-1, slots) for _ in range(count)]
+        if action == "grow":
+            counts = [rng.choice((0, 1, 1, page_size, 2 * page_size + 1, -1)) for _ in some]
+            positions = pages.reserve(some, counts)
+            key, value = (torch.randn(count, 2, 2 * page_size + 1, dim, generator=g).to(dtype) for _ in range(2))
+            for layer in range(layers):
+                pages.write(layer, key, value, some, positions, counts)
+        elif action == "fork":
+            seen |= set(pages.fork(some, [rng.randint(-1, slots) for _ in some]))
+        elif action == "free":
+            pages.free(some)
+        elif action == "compact":
+            pages.compact()
+        else:
+            pages.copy([rng.randint(-1, 24) for _ in some], [rng.randint(0, 24) for _ in some])
+        pages.same()
+    assert {ref.DONE, ref.OUT_OF_RANGE, ref.OCCUPIED} <= seen
+
+
+def test_pages_of_large_pools_and_many_requests(gpu_device):
+    """Pools and lists longer than one round of the bookkeeping workgroup, with every lowest page taken in order."""
+    model = ref.Pages(1, 9001, 1, 2, 1, 2500, 4)
+    rng = random.Random(3)
+    for p in range(9001):
+        model.refcounts[p] = rng.choice((0, 0, 1))
+    pages = _Device(model, gpu_device)
+    order = list(range(2500))
+    rng.shuffle(order)
+    pages.reserve(order, [rng.randint(0, 8) for _ in order])
+    pages.same()
+    parents = [s for s in order if model.lengths[s]][:900]
+    empty = [s for s in order if not model.lengths[s]]
+    pages.free(order[-300:])
+    pages.fork(parents[: len(empty)], empty[: len(parents)])
+    pages.same()
+    pages.compact()
+    pages.same()
+    pages.free(order)
+    pages.same()
+
+
+def test_pages_run_out_in_order(gpu_device):
+    pages = _Device(ref.Pages(2, 5, 1, 4, 8, 6, 4), gpu_device)
+    pages.reserve([0, 1, 2, 3, 4], [8, 3, 9, 0, 1])  # 2 + 1 pages fit, the third asks for 3, and the last for 1 more
+    assert pages.lengths.tolist() == [8, 3, 0, 0, 0, 0]
+    pages.reserve([1, 0], [1, 9])  # a page in hand; a row that is too short
+    pages.same()
+    pages.reserve([2, 3], [4, 4])
+    assert pages.fork([1, 0, 1], [4, 5, 4]) == [ref.DONE, ref.DONE, ref.REPEATED]  # full pages only: none is needed
+    pages.free([4])
+    pages.reserve([1], [1])
+    pages.same()
+    # A chain in one call reads the books as they were: slot 4 is empty as a parent.
+    assert pages.fork([0, 4], [4, 4]) == [ref.DONE, ref.REPEATED]
+    pages.same()
+
+
+def test_page_copies_that_clash_are_refused(gpu_device):
+    pages = _Device(ref.Pages(3, 8, 2, 4, 16, 1, 1), gpu_device)
+    pages.copy([0, 1, 2, 2, 5, 7, -1, 0], [1, 3, 4, 4, 5, 8, 6, 6])
+    pages.same()
+    assert ops.paged_cache_copy_native(pages.key, pages.value, pages.ids([]), pages.ids([])).shape == (0,)
+
+
+def test_pages_with_other_strides(gpu_device):
+    """Pools as views of [layers, P, page, heads, D] and of one tensor for keys and values; rows that are not aligned."""
+    model = ref.Pages(2, 8, 3, 4, 6, 4, 3, torch.float32, seed=2)
+    pages = _Device(model, gpu_device)
+    both = torch.zeros(2, 2, 8, 4, 3, 7, device=gpu_device)
+    untouched = both[..., 6].clone().fill_(5.0)
+    both[..., 6] = untouched
+    views = both[0, ..., :6].transpose(2, 3), both[1, ..., :6].transpose(2, 3)
+    for view, source in zip(views, (pages.key, pages.value)):
+        view.copy_(source)
+    pages.key, pages.value = views
+    table = torch.full((4, 5), 77, dtype=torch.int32, device=gpu_device)
+    table[:, 1:4] = -1
+    pages.table = table[:, 1:4]
+    positions = pages.reserve([2, 0], [10, 5])
+    for layer in range(2):
+        key = torch.randn(2, 10, 3, 6).transpose(1, 2)
+        pages.write(layer, key, -key, [2, 0], positions, [10, 5])
+    pages.fork([2, 0], [1, 3])
+    pages.free([2])
+    pages.compact()
+    pages.copy([0], [7])
+    pages.same()
+    assert torch.equal(both[..., 6], untouched) and bool((table[:, [0, 4]] == 77).all())
+
+
+def test_write_skips_what_has_no_page(gpu_device):
+    pages = _Device(ref.Pages(1, 4, 1, 4, 8, 3, 2), gpu_device)
+    pages.table[0, 0] = pages.model.table[0][0] = 2
+    pages.table[1, 0] = pages.model.table[1][0] = 9  # outside the pool
+    key = torch.randn(4, 1, 9, 8)
+    pages.write(0, key, -key, [0, 1, 3, 2], pages.ids([1, 0, 0, -1]), [9, 9, 9, 9])
+    pages.same()
+    pages.write(0, key[:1], key[:1], [0], pages.ids([2 ** 62]), [9])
+    pages.same()
+
+
+# --------------------------------------------------------------------------- logits
+
+def _logits_case(seed, dtype, rows, vocab, width, bias_rows=1, allowed_rows=None):
+    g = torch.Generator().manual_seed(seed)
+    history = torch.randint(0, vocab, (rows, width), generator=g)
+    history[:, ::3] %= min(vocab, 5)
+    return {"logits": (3 * torch.randn(rows, vocab, generator=g)).to(dtype), "history": history,
+            "history_lengths": torch.randint(0, width + 1, (rows,), generator=g),
+            "repetition": 1 + torch.rand(rows, generator=g), "frequency": torch.rand(rows, generator=g),
+            "presence": torch.rand(rows, generator=g), "bias": torch.randn(bias_rows, vocab, generator=g),
+            "allowed": torch.randint(-2 ** 31, 2 ** 31, (allowed_rows or rows, -(-vocab // 32)), generator=g).to(torch.int32)}
+
+
+def _check_logits(case, device):
+    expected = ref.processed_logits(**case)
+    processed, tokens = ops.logits_process_native(**_to(case, device))
+    assert processed.dtype == case["logits"].dtype and tokens.dtype == torch.int64
+    cpu = processed.cpu()
+    assert torch.equal(cpu.isneginf(), expected.isneginf()) and torch.equal(cpu.isnan(), expected.isnan())
+    fine = expected.isfinite()
+    # Five float32 roundings of intermediate values that are at most the sum of the magnitudes, one to the type.
+    size = case["logits"].double().abs() * 2
+    for name in ("frequency", "presence"):
+        if case.get(name) is not None:
+            size = size + case[name].double()[:, None] * (case["history"].shape[1] if name == "frequency" else 1)
+    if case.get("bias") is not None:
+        size = size + case["bias"].double().abs()
+    bound = 5 * 2.0 ** -24 * size + torch.finfo(case["logits"].dtype).eps / 2 * expected.abs().nan_to_num(posinf=0)
+    error = (cpu.double() - expected).abs()
+    assert bool((error[fine] <= bound.expand_as(error)[fine] + torch.finfo(case["logits"].dtype).tiny).all())
+    assert tokens.tolist() == ref.greedy(cpu)
+    return cpu, tokens
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("vocab", [1, 31, 32, 33, 1000, 8191, 8192, 8193, 20001, 49152])
+def test_logits_sizes(gpu_device, dtype, vocab):
+    _check_logits(_logits_case(vocab, dtype, 3, vocab, 50), gpu_device)
+    _check_logits(_logits_case(vocab + 1, dtype, 1, vocab, 1, allowed_rows=1), gpu_device)
+
+
+def test_logits_options(gpu_device):
+    case = _logits_case(1, torch.float32, 4, 5000, 600, bias_rows=4, allowed_rows=1)
+    _check_logits(case, gpu_device)
+    names = ("history_lengths", "repetition", "frequency", "presence", "bias", "allowed")
+    for left_out in names:
+        _check_logits({k: v for k, v in case.items() if k != left_out}, gpu_device)
+    for alone in names:
+        _check_logits({k: v for k, v in case.items() if k in ("logits", "history", alone)}, gpu_device)
+    plain, tokens = _check_logits({"logits": case["logits"]}, gpu_device)
+    assert torch.equal(plain, case["logits"]) and tokens.tolist() == case["logits"].argmax(1).tolist()
+    _check_logits({**case, "history": torch.zeros(4, 0, dtype=torch.int64), "history_lengths": None}, gpu_device)
+
+
+def test_logits_edges(gpu_device):
+    """Padding ids, lengths outside the width, ties, rows that allow nothing, NaN and infinity, also where masked."""
+    case = _logits_case(2, torch.float32, 6, 9000, 40)
+    case["history"][0, 5:] = -1
+    case["history"][1, :] = 2 ** 40
+    case["history_lengths"] = torch.tensor([40, 40, 0, 100, -1, 7])
+    case["allowed"][2] = 0
+    case["logits"][3] = 1.5
+    case["logits"][4, 100] = math.nan
+    case["logits"][4, 8999] = math.nan
+    case["logits"][5, :50] = torch.tensor([math.nan, math.inf, -math.inf, math.nan, 3.0] * 10)
+    case["allowed"][4, 3] |= 1 << 4
+    case["allowed"][4, 8999 // 32] |= 1 << (8999 % 32)
+    _, tokens = _check_logits(case, gpu_device)
+    assert int(tokens[2]) == 0 and int(tokens[4]) == 100
+    case = {"logits": torch.zeros(2, 20000)}
+    case["logits"][1, [15000, 300, 8192]] = 1.0
+    assert _check_logits(case, gpu_device)[1].tolist() == [0, 300]
+    low = torch.full((1, 100), torch.finfo(torch.bfloat16).min, dtype=torch.bfloat16)
+    out, tokens = ops.logits_process_native(low.to(gpu_device), bias=torch.full((1, 100), -1e38, device=gpu_device))
+    assert int(tokens[0]) == 0 and bool(out.cpu().isneginf().all())
+
+
+def test_logits_strides(gpu_device):
+    case = _logits_case(3, torch.float16, 4, 4096, 64, bias_rows=4)
+    device = _to(case, gpu_device)
+    expected, tokens = ops.logits_process_native(**device)
+    for name, extra in (("logits", 8), ("logits", 3), ("history", 5), ("bias", 3), ("bias", 4), ("allowed", 1)):
+        wide = torch.zeros(4, device[name].shape[1] + extra, dtype=device[name].dtype, device=gpu_device)
+        wide[:, : device[name].shape[1]] = device[name]
+        moved = {**device, name: wide[:, : device[name].shape[1]]}
+        out, again = ops.logits_process_native(**moved)
+        assert torch.equal(out, expected) and torch.equal(again, tokens)
+        shifted = torch.zeros(4, device[name].shape[1] + 8, dtype=device[name].dtype, device=gpu_device)
+        shifted[:, 1:1 + device[name].shape[1]] = device[name]
+        out, again = ops.logits_process_native(**{**device, name: shifted[:, 1:1 + device[name].shape[1]]})
+        assert torch.equal(out, expected) and torch.equal(again, tokens)
+
+
+def test_opcheck(gpu_device):
+    case = _to(_paged_case(43, torch.float32, 6, 2, 64, 16, [50, 20]), gpu_device)
+    for op, args in ((torch.ops.flux.paged_decode_attention.default, tuple(case.values())),
+                     (torch.ops.flux.window_attention.default,
+                      tuple(_to(_window_case(1, torch.float32, 2, 4, 2, 64, 5, 9), gpu_device).values()) + (4,)),
+                     (torch.ops.flux.logits_process.default, (torch.randn(2, 100, device=gpu_device),))):
+        result = torch.library.opcheck(op, args)
+        assert all(status == "SUCCESS" for status in result.values()), result
+
+
+# --------------------------------------------------------------------------- together
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_a_served_loop(gpu_device, dtype):
+    """Prompts through the window operator and into pages, branches, decoded tokens, upkeep of the pool between them: each
+    step's attention against the whole history in float64, and the tokens against the plain logits."""
+    g = torch.Generator().manual_seed(51)
+    layers, heads, kv_heads, dim, page_size, window, sinks, vocab = 2, 6, 2, 64, 16, 24, 2, 500
+    pages = _Device(ref.Pages(layers, 40, kv_heads, page_size, dim, 6, 8, dtype), gpu_device)
+    prompts = [37, 16, 5]
+    history = {}  # slot -> per layer (keys, values), tokens
+    slots = [4, 0, 2]
+    width = max(prompts)
+    positions = pages.reserve(slots, prompts)
+    layer_rows = [[_randn(g, (3, kv_heads, width, dim), dtype) for _ in range(2)] for _ in range(layers)]
+    for layer, (key, value) in enumerate(layer_rows):
+        query = _randn(g, (3, heads, width, dim), dtype)
+        _check_window({"query": query, "key": key, "value": value, "scale": 0.125}, gpu_device, window, sinks,
+                      lengths=prompts, starts=[0, 0, 0])
+        pages.write(layer, key, value, slots, positions, prompts)
+    for i, slot in enumerate(slots):
+        history[slot] = ([(k[i, :, : prompts[i]], v[i, :, : prompts[i]]) for k, v in layer_rows], [i, i, 7])
+    assert pages.fork([4, 0], [1, 5]) == [ref.DONE, ref.DONE]
+    for parent, child in ((4, 1), (0, 5)):
+        history[child] = (list(history[parent][0]), list(history[parent][1]))
+    for step in range(20):
+        active = sorted(history)
+        ids = pages.ids(active)
+        positions = pages.reserve(active, [1] * len(active))
+        assert min(positions.tolist()) >= 0
+        for layer in range(layers):
+            key, value = (_randn(g, (len(active), kv_heads, 1, dim), dtype) for _ in range(2))
+            query = _randn(g, (len(active), heads, 1, dim), dtype)
+            pages.write(layer, key, value, active, positions, [1] * len(active))
+            out = ops.paged_decode_attention_native(query.to(gpu_device), pages.key[layer], pages.value[layer], pages.table,
+                                                    pages.lengths, 0.125, window, sinks, ids)
+            for i, slot in enumerate(active):
+                keys, values = history[slot][0][layer]
+                keys, values = torch.cat((keys, key[i]), 1), torch.cat((values, value[i]), 1)
+                history[slot][0][layer] = (keys, values)
+                expected = ref.window_attention(query[i][None], keys[None], values[None], 0.125, window, sinks)
+                _close(out[i][None], expected, ref.attention_bound(query[i], keys, values, 0.125, window + sinks, dtype, expected))
+        logits = torch.randn(len(active), vocab, generator=g).to(dtype)
+        past = torch.full((len(active), 40), -1)
+        for i, slot in enumerate(active):
+            past[i, : len(history[slot][1])] = torch.tensor(history[slot][1])
+        rate = torch.full((len(active),), 1.3)
+        _, tokens = _check_logits({"logits": logits, "history": past, "repetition": rate, "presence": rate}, gpu_device)
+        for slot, token in zip(active, tokens.tolist()):
+            history[slot][1].append(token)
+        if step == 6:
+            pages.free([0])
+            del history[0]
+            pages.compact()
+        if step == 11:
+            assert pages.fork([1], [3]) == [ref.DONE]
+            history[3] = (list(history[1][0]), list(history[1][1]))
+        pages.same()
+
+
+def test_a_decode_step_in_a_graph(gpu_device):
+    """Reserve, write, attend and pick the token as one captured graph, replayed with the program's own work between."""
+    g = torch.Generator().manual_seed(61)
+    model = ref.Pages(1, 30, 2, 4, 64, 3, 9)
+    pages = _Device(model, gpu_device)
+    positions = pages.reserve([0, 1, 2], [5, 1, 8])
+    rows = torch.randn(3, 2, 8, 64, generator=g)
+    pages.write(0, rows, -rows, [0, 1, 2], positions, [5, 1, 8])
+    slots = pages.ids([2, 0, 1])
+    key, value, query = (torch.zeros(3, h, 1, 64, device=gpu_device) for h in (2, 2, 4))
+    history = torch.full((3, 30), -1, dtype=torch.int64, device=gpu_device)
+    logits = torch.zeros(3, 9000, device=gpu_device)
+    rate = torch.full((3,), 1.2, device=gpu_device)
+
+    def step():
+        at, status = ops.paged_cache_reserve_native(*pages.books, 4, slots)
+        ops.paged_cache_write_native(key, value, pages.key[0], pages.value[0], pages.table, slots, at)
+        out = ops.paged_decode_attention_native(query, pages.key[0], pages.value[0], pages.table, pages.lengths, 0.125, 6, 1, slots)
+        processed, tokens = ops.logits_process_native(logits, history, None, rate)
+        return at, status, out, processed, tokens
+
+    books = [t.clone() for t in (*pages.books, pages.key, pages.value)]
+    stream = torch.cuda.Stream()
+    stream.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(stream):
+        step()
+    torch.cuda.current_stream().wait_stream(stream)
+    graph = torch.cuda.CUDAGraph()
+    for t, before in zip((*pages.books, pages.key, pages.value), books):
+        t.copy_(before)
+    with torch.cuda.graph(graph):
+        captured = step()
+    for t, before in zip((*pages.books, pages.key, pages.value), books):
+        t.copy_(before)
+    for i in range(9):
+        for t in (key, value, query, logits):
+            t.copy_(torch.randn(t.shape, generator=g))
+        history[:, i] = i
+        before = [t.clone() for t in (*pages.books, pages.key, pages.value)]
+        graph.replay()
+        torch.cuda.synchronize()
+        got = [t.clone() for t in captured] + [t.clone() for t in (*pages.books, pages.key, pages.value)]
+        for t, old in zip((*pages.books, pages.key, pages.value), before):
+            t.copy_(old)
+        eager = [*step(), *pages.books, pages.key, pages.value]
+        assert all(torch.equal(a, b) for a, b in zip(got, eager)), i
