@@ -13,6 +13,10 @@
 namespace flux {
 namespace {
 
+#ifndef FLUX_ROW_TILES
+#define FLUX_ROW_TILES 1
+#endif
+
 constexpr int kThreads = 256;
 constexpr int kWaves = 4;
 
@@ -276,14 +280,345 @@ __global__ void __launch_bounds__(kThreads) window_attention_kernel(AttentionArg
     }
 }
 
+
+// ---------------------------------------------------------------------------
+// 16-bit prompts.  Here matrix instructions, exponentials and LDS reads cost about the same, so that keys and values are
+// staged once for the workgroup's four waves and each operand read from LDS serves kRowTiles x 32 rows.
+//
+// A stage holds kKeys keys: K rows as they are, V transposed (the staging thread permutes the 16-bit halves of four
+// keys), its keys in the order in which a lane's scores lie.  S^T = K Q^T on 32 x 32 tiles leaves lane (n, h) with the
+// keys 8 (r / 4) + 4 h + r % 4 of row n, which rounded in pairs are the right operand of O^T = V^T P.  Rows are padded by
+// 16 bytes so that eight lanes' 16-byte reads fall on different banks.
+// The running maximum moves only when a tile exceeds it by 2^kLazy: a rescaling of the sums costs as much as the
+// exponentials, and weights up to 2^kLazy are as exact.  Weights are rounded to the values' type for the product (half
+// a step of that type, like the result's own rounding) and summed unrounded in float32.
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+
+template <class T>
+struct Wide;
+template <>
+struct Wide<__bf16> {
+    static constexpr float kShift = 0.0f;
+    static __device__ __forceinline__ f32x16 multiply(u32x4 a, u32x4 b, f32x16 c) {
+        return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c,
+                                                       0, 0, 0);
+    }
+};
+template <>
+struct Wide<_Float16> {
+    // Weights are held 2^6 times as large (at most 2^14), which keeps those down to 2^-20 of the largest in float16's
+    // normal range.
+    static constexpr float kShift = 6.0f;
+    static __device__ __forceinline__ f32x16 multiply(u32x4 a, u32x4 b, f32x16 c) {
+        return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0,
+                                                      0, 0);
+    }
+};
+
+__device__ __forceinline__ float half_max(float v) {
+    const auto both = __builtin_amdgcn_permlane32_swap(__float_as_int(v), __float_as_int(v), false, false);
+    return fmaxf(__int_as_float(both[0]), __int_as_float(both[1]));
+}
+__device__ __forceinline__ float half_sum(float v) {
+    const auto both = __builtin_amdgcn_permlane32_swap(__float_as_int(v), __float_as_int(v), false, false);
+    return __int_as_float(both[0]) + __int_as_float(both[1]);
+}
+
+template <class T, int kDim, int kRowTiles, bool kWide>
+__global__ void __launch_bounds__(kThreads, kRowTiles == 1 && kDim <= 128 ? 2 : 1)
+window_tile_kernel(AttentionArgs a, int row_tiles, int tiles_total) {
+    using W = Wide<T>;
+    constexpr int kKeys = kDim == 64 ? 128 : (kDim == 128 ? 64 : 32);
+    constexpr int kSubs = kKeys / 32;
+    constexpr int kSteps = kDim / 16;             // of a score
+    constexpr int kBlocks = kDim / 32;            // of the result
+    constexpr int kRows = kWaves * kRowTiles * 32;
+    constexpr int kKeyRow = kDim * 2 + 16;        // bytes
+    constexpr int kValueRow = kKeys * 2 + 16;
+    constexpr int kStage = kKeys * kKeyRow + kDim * kValueRow;
+    constexpr int kKeyLoads = kKeys * kDim / 8 / kThreads;        // 16 bytes per thread
+    constexpr int kValueUnits = kKeys / 4 * (kDim / 8);           // 4 keys x 8 dims
+    constexpr int kValueLoads = (kValueUnits + kThreads - 1) / kThreads;
+    constexpr float kLazy = 8.0f;
+    extern __shared__ char stages[];
+
+    // Consecutive tiles share most of their keys: each XCD (block index modulo 8) takes a run of them.
+    const int run = tiles_total / 8, rest = tiles_total % 8;
+    const int xcd = blockIdx.x % 8;
+    const int tile = xcd * run + (xcd < rest ? xcd : rest) + blockIdx.x / 8;
+    const int64_t row0 = static_cast<int64_t>(tile % row_tiles) * kRows;
+    const int kv_head = tile / row_tiles % a.kv_heads;
+    const int64_t b = tile / row_tiles / a.kv_heads;
+
+    const int lane = threadIdx.x & 63;
+    const int wave = threadIdx.x >> 6;
+    const int n32 = lane & 31;
+    const int half = lane >> 5;
+    int64_t n = a.lengths ? a.lengths[b] : a.keys;
+    n = n < 0 ? 0 : (n > a.keys ? a.keys : n);
+    int64_t start = a.starts ? a.starts[b] : n - a.queries;
+    start = start < -a.queries ? -a.queries : (start > a.keys ? a.keys : start);
+    const int all_rows = a.queries * a.group;
+
+    // Positions of a range of rows, cut to those that are a key's; first > last when there is none.
+    auto positions = [&](int64_t from, int64_t count, int& first, int& last) {
+        const int64_t to = from + count < all_rows ? from + count - 1 : all_rows - 1;
+        const int64_t p = start + from / a.group, q = start + to / a.group;
+        first = static_cast<int>(p < 0 ? 0 : p);
+        last = static_cast<int>(q >= n ? n - 1 : q);
+        if (from > to) last = first - 1;
+    };
+    int block_first, block_last, wave_first, wave_last;
+    positions(row0, kRows, block_first, block_last);
+    const int64_t wave_row = row0 + wave * kRowTiles * 32;
+    positions(wave_row, kRowTiles * 32, wave_first, wave_last);
+
+    const T* keys = static_cast<const T*>(a.key) + b * a.key_strides[0] + kv_head * a.key_strides[1];
+    const T* values = static_cast<const T*>(a.value) + b * a.value_strides[0] + kv_head * a.value_strides[1];
+
+    RowRange mine[kRowTiles];
+    int sink_end[kRowTiles];
+    u32x4 query[kRowTiles][kSteps];
+    f32x16 out[kRowTiles][kBlocks];
+    float top[kRowTiles], weight[kRowTiles];
+    const uint32_t sign = a.scale < 0.0f ? 0x80008000u : 0u;  // the scale's sign goes to the query
+    const float factor = fmaxf(fabsf(a.scale) * kLog2e, 1e-37f);  // above 0: a masked score stays -inf
+#pragma unroll
+    for (int c = 0; c < kRowTiles; ++c) {
+        const int64_t r = wave_row + 32 * c + n32;
+        const int64_t i = r / a.group, head = kv_head * static_cast<int64_t>(a.group) + r % a.group;
+        const int64_t position = start + i;
+        mine[c].position = r < all_rows && position >= 0 && position < n ? static_cast<int>(position) : -1;
+        mine[c].low = a.window > 0 && mine[c].position >= a.window ? mine[c].position - a.window + 1 : 0;
+        sink_end[c] = a.sinks < mine[c].low ? a.sinks : mine[c].low;
+        const T* q = static_cast<const T*>(a.query) + b * a.query_strides[0] + head * a.query_strides[1] + i * a.query_strides[2];
+#pragma unroll
+        for (int s = 0; s < kSteps; ++s) {
+            query[c][s] = Mfma<T>::load_query(q, a.query_strides[3], 16 * s + 8 * half, a.dim, r < all_rows);
+            query[c][s] ^= sign;
+        }
+#pragma unroll
+        for (int i = 0; i < kBlocks; ++i)
+#pragma unroll
+            for (int j = 0; j < 16; ++j) out[c][i][j] = 0.0f;
+        top[c] = -INFINITY;
+        weight[c] = 0.0f;
+    }
+
+    if (block_first <= block_last) {
+        auto low_of = [&](int p) { return a.window > 0 && p >= a.window ? p - a.window + 1 : 0; };
+        const int low = low_of(block_first);
+        const int seen = block_last + 1;
+        const int sinks = a.sinks < low ? a.sinks : low;
+        const int first_stage = low / kKeys;
+        const int of_sinks = (sinks + kKeys - 1) / kKeys;
+        const int sink_stages = of_sinks < first_stage ? of_sinks : first_stage;
+        const int count = sink_stages + (seen + kKeys - 1) / kKeys - first_stage;
+        auto stage_key = [&](int t) { return (t < sink_stages ? t : first_stage + t - sink_stages) * kKeys; };
+
+        u32x4 held_key[kKeyLoads];
+        u32x4 held_value[kValueLoads][4];
+        auto fetch = [&](int t) {
+            const int base = stage_key(t);
+#pragma unroll
+            for (int i = 0; i < kKeyLoads; ++i) {
+                const int unit = threadIdx.x + kThreads * i;
+                const int key = base + unit / (kDim / 8), d = unit % (kDim / 8) * 8;
+                held_key[i] = Mfma<T>::template load_row<kWide>(keys + key * a.key_strides[2], d, a.dim, key < seen);
+            }
+#pragma unroll
+            for (int i = 0; i < kValueLoads; ++i) {
+                const int unit = threadIdx.x + kThreads * i;
+                const int key = base + unit % (kKeys / 4) * 4, d = unit / (kKeys / 4) * 8;
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    held_value[i][j] = Mfma<T>::template load_row<kWide>(values + (key + j) * a.value_strides[2], d, a.dim,
+                                                                         unit < kValueUnits && key + j < seen);
+                }
+            }
+        };
+        auto put = [&](char* stage) {
+#pragma unroll
+            for (int i = 0; i < kKeyLoads; ++i) {
+                const int unit = threadIdx.x + kThreads * i;
+                *reinterpret_cast<u32x4*>(stage + unit / (kDim / 8) * kKeyRow + unit % (kDim / 8) * 16) = held_key[i];
+            }
+            char* turned = stage + kKeys * kKeyRow;
+#pragma unroll
+            for (int i = 0; i < kValueLoads; ++i) {
+                const int unit = threadIdx.x + kThreads * i;
+                const int quad = unit % (kKeys / 4), d = unit / (kKeys / 4) * 8;
+                // Quads 0, 1, 2, 3 of 16 keys lie as 0, 2, 1, 3: a lane's eight keys side by side.
+                const int at = (quad & ~3) | (quad & 1) << 1 | (quad >> 1 & 1);
+                if (unit < kValueUnits) {
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) {
+                        const u32x2 four = {Mfma<T>::pair(held_value[i][0][j / 2], held_value[i][1][j / 2], j & 1),
+                                            Mfma<T>::pair(held_value[i][2][j / 2], held_value[i][3][j / 2], j & 1)};
+                        *reinterpret_cast<u32x2*>(turned + (d + j) * kValueRow + at * 8) = four;
+                    }
+                }
+            }
+        };
+
+        const int wave_low = low_of(wave_first), low_of_last = low_of(wave_last);
+        fetch(0);
+        put(stages);
+        for (int t = 0; t < count; ++t) {
+            __syncthreads();
+            const char* stage = stages + (t & 1) * kStage;
+            const char* turned = stage + kKeys * kKeyRow;
+            const int base = stage_key(t);
+            if (t + 1 < count) fetch(t + 1);
+#pragma unroll
+            for (int s = 0; s < kSubs; ++s) {
+                const int first = base + 32 * s, last = first + 31;
+                // Nothing of this wave's rows sees these keys.
+                if (first > wave_last || (last < wave_low && first >= a.sinks)) continue;
+                f32x16 score[kRowTiles];
+#pragma unroll
+                for (int c = 0; c < kRowTiles; ++c)
+#pragma unroll
+                    for (int j = 0; j < 16; ++j) score[c][j] = 0.0f;
+#pragma unroll
+                for (int k = 0; k < kSteps; ++k) {
+                    const u32x4 key = *reinterpret_cast<const u32x4*>(stage + (32 * s + n32) * kKeyRow + 32 * k + 16 * half);
+#pragma unroll
+                    for (int c = 0; c < kRowTiles; ++c) score[c] = W::multiply(key, query[c][k], score[c]);
+                }
+                const bool inside = first >= low_of_last && last <= wave_first;
+                u32x4 p[kRowTiles][2];
+#pragma unroll
+                for (int c = 0; c < kRowTiles; ++c) {
+                    if (!inside) {
+#pragma unroll
+                        for (int j = 0; j < 16; ++j) {
+                            // Without branches: low <= key <= position as one unsigned comparison, or a sink.
+                            const int key = first + 8 * (j / 4) + 4 * half + j % 4;
+                            const bool visible = (static_cast<uint32_t>(key - mine[c].low) <=
+                                                  static_cast<uint32_t>(mine[c].position - mine[c].low)) |
+                                                 (key < sink_end[c]);
+                            score[c][j] = visible ? score[c][j] : -INFINITY;
+                        }
+                    }
+                    float highest = score[c][0];
+#pragma unroll
+                    for (int j = 1; j < 16; ++j) highest = fmaxf(highest, score[c][j]);
+                    highest = half_max(highest) * factor;
+                    if (__any(highest > top[c] + kLazy)) {
+                        const float now = fmaxf(top[c], highest);
+                        const float shrink = top[c] == -INFINITY ? 0.0f : fast_exp2(top[c] - now);
+                        top[c] = now;
+                        weight[c] *= shrink;
+#pragma unroll
+                        for (int i = 0; i < kBlocks; ++i)
+#pragma unroll
+                            for (int j = 0; j < 16; ++j) out[c][i][j] *= shrink;
+                    }
+                    const float reference = W::kShift - (top[c] == -INFINITY ? 0.0f : top[c]);
+#pragma unroll
+                    for (int j = 0; j < 16; j += 2) {
+                        const float p0 = fast_exp2(fmaf(score[c][j], factor, reference));
+                        const float p1 = fast_exp2(fmaf(score[c][j + 1], factor, reference));
+                        weight[c] += p0 + p1;
+                        p[c][j / 8][j % 8 / 2] = Mfma<T>::bits(static_cast<T>(p0)) | Mfma<T>::bits(static_cast<T>(p1)) << 16;
+                    }
+                }
+#pragma unroll
+                for (int i = 0; i < kBlocks; ++i)
+#pragma unroll
+                    for (int k = 0; k < 2; ++k) {
+                        const u32x4 value = *reinterpret_cast<const u32x4*>(turned + (32 * i + n32) * kValueRow +
+                                                                            (32 * s + 16 * k) * 2 + 16 * half);
+#pragma unroll
+                        for (int c = 0; c < kRowTiles; ++c) out[c][i] = W::multiply(value, p[c][k], out[c][i]);
+                    }
+            }
+            if (t + 1 < count) put(stages + ((t + 1) & 1) * kStage);
+        }
+    }
+
+#pragma unroll
+    for (int c = 0; c < kRowTiles; ++c) {
+        weight[c] = half_sum(weight[c]);
+        float worst = fabsf(weight[c]);
+#pragma unroll
+        for (int i = 0; i < kBlocks; ++i)
+#pragma unroll
+            for (int j = 0; j < 16; ++j) worst += fabsf(out[c][i][j]);  // keeps NaN, infinity
+        const uint64_t odd = __ballot(mine[c].position >= 0 && !(worst < INFINITY));
+        uint32_t rows = static_cast<uint32_t>(odd | odd >> 32);
+        const int64_t r = wave_row + 32 * c + n32;
+        const int64_t i = r / a.group, head = kv_head * static_cast<int64_t>(a.group) + r % a.group;
+        if (r < all_rows && !(rows >> n32 & 1)) {
+            T* o = static_cast<T*>(a.out) + ((b * a.query_heads + head) * a.queries + i) * a.dim;
+            const float inverse = mine[c].position < 0 ? 0.0f : 1.0f / weight[c];
+#pragma unroll
+            for (int k = 0; k < kBlocks; ++k)
+#pragma unroll
+                for (int j = 0; j < 16; j += 4) {
+                    const int d = 32 * k + 2 * j + 4 * half;  // four dims side by side
+                    T four[4];
+#pragma unroll
+                    for (int l = 0; l < 4; ++l)
+                        four[l] = static_cast<T>(mine[c].position < 0 ? 0.0f : out[c][k][j + l] * inverse);
+                    if constexpr (kWide) {
+                        if (d < a.dim)
+                            *reinterpret_cast<u32x2*>(o + d) = u32x2{Mfma<T>::bits(four[0]) | Mfma<T>::bits(four[1]) << 16,
+                                                                     Mfma<T>::bits(four[2]) | Mfma<T>::bits(four[3]) << 16};
+                    } else {
+#pragma unroll
+                        for (int l = 0; l < 4; ++l)
+                            if (d + l < a.dim) o[d + l] = four[l];
+                    }
+                }
+        }
+        while (rows) {
+            const int which = __ffs(rows) - 1;
+            rows &= rows - 1;
+            const int64_t r = wave_row + 32 * c + which;
+            const int64_t i = r / a.group, head = kv_head * static_cast<int64_t>(a.group) + r % a.group;
+            RowRange range;
+            range.position = static_cast<int>(start + i);
+            range.low = a.window > 0 && range.position >= a.window ? range.position - a.window + 1 : 0;
+            exact_row<T>(a, static_cast<const T*>(a.query) + b * a.query_strides[0] + head * a.query_strides[1] + i * a.query_strides[2],
+                         keys, values, range, static_cast<T*>(a.out) + ((b * a.query_heads + head) * a.queries + i) * a.dim);
+        }
+    }
+}
+
+template <class T, int kDim, int kRowTiles, bool kWide>
+hipError_t launch_window_tiles(const AttentionArgs& a, hipStream_t stream) {
+    constexpr int kKeys = kDim == 64 ? 128 : (kDim == 128 ? 64 : 32);
+    constexpr int kRows = kWaves * kRowTiles * 32;
+    constexpr size_t kLds = 2 * (kKeys * (kDim * 2 + 16) + kDim * (kKeys * 2 + 16));
+    const int64_t rows = static_cast<int64_t>(a.queries) * a.group;
+    const int row_tiles = static_cast<int>((rows + kRows - 1) / kRows);
+    const int64_t tiles = static_cast<int64_t>(row_tiles) * a.kv_heads * a.batch;
+    if (tiles > (int64_t{1} << 23)) return hipErrorInvalidValue;
+    static const hipError_t room = hipFuncSetAttribute(
+        reinterpret_cast<const void*>(window_tile_kernel<T, kDim, kRowTiles, kWide>), hipFuncAttributeMaxDynamicSharedMemorySize,
+        static_cast<int>(kLds));
+    if (room != hipSuccess) return room;
+    hipLaunchKernelGGL(HIP_KERNEL_NAME(window_tile_kernel<T, kDim, kRowTiles, kWide>), dim3(static_cast<uint32_t>(tiles)),
+                       dim3(kThreads), kLds, stream, a, row_tiles, static_cast<int>(tiles));
+    return hipGetLastError();
+}
+
 template <class T, int kDim>
 hipError_t launch_window(const AttentionArgs& a, hipStream_t stream) {
+    if constexpr (sizeof(T) == 2) {
+        if (a.wide && reinterpret_cast<uintptr_t>(a.out) % 8 == 0)
+            return launch_window_tiles<T, kDim, FLUX_ROW_TILES, true>(a, stream);
+        return launch_window_tiles<T, kDim, FLUX_ROW_TILES, false>(a, stream);
+    } else {
     constexpr int kRows = kDim == 256 ? 16 : 32;
     const int64_t rows = static_cast<int64_t>(a.queries) * a.group;
     const dim3 grid(static_cast<uint32_t>((rows + kRows - 1) / kRows), a.kv_heads, a.batch);
     if (a.wide) hipLaunchKernelGGL(HIP_KERNEL_NAME(window_attention_kernel<T, kDim, true>), grid, dim3(kThreads), 0, stream, a);
     else hipLaunchKernelGGL(HIP_KERNEL_NAME(window_attention_kernel<T, kDim, false>), grid, dim3(kThreads), 0, stream, a);
     return hipGetLastError();
+    }
 }
 
 template <class T>

@@ -55,7 +55,8 @@ def window_attention(query, key, value, scale, window, sinks=0, lengths=None, st
     return out
 
 
-def attention_bound(query, keys, values, scale, terms: int, dtype: torch.dtype, expected: torch.Tensor) -> torch.Tensor:
+def attention_bound(query, keys, values, scale, terms: int, dtype: torch.dtype, expected: torch.Tensor,
+                    rounded_weights: bool = False) -> torch.Tensor:
     """How far a result computed with float32 sums may be from ``expected``.
 
     A score is a sum of D products: it is off by at most (D + 2) 2^-24 times the sum of the magnitudes, itself at most
@@ -64,6 +65,10 @@ def attention_bound(query, keys, values, scale, terms: int, dtype: torch.dtype, 
     and by 2^-22 for the exponential, and a weight below 2^-40 does not count; a 16-bit weight kept in two terms by 2^-16
     more (bfloat16's two halves).  The two sums of ``terms`` weights are off by terms 2^-23.  All of it moves a weighted
     mean of the values by at most twice the weights' relative error times the largest value.  The result is rounded once.
+
+    ``rounded_weights``: 16-bit prompts round each weight p_j once to the type for its product with v_j, and sum the
+    unrounded ones: sum p_j (1 + d_j) v_j / sum p_j with |d_j| at most half a step differs by at most half a step times
+    the largest value.
     """
     dim = query.shape[-1]
     norms = query.double().norm(dim=-1).max() * keys.double().norm(dim=-1).max() * abs(scale)
@@ -74,6 +79,8 @@ def attention_bound(query, keys, values, scale, terms: int, dtype: torch.dtype, 
     largest = float(values.double().abs().max())
     half_step = torch.finfo(dtype).eps / 2
     smallest = torch.finfo(dtype).tiny
+    if rounded_weights and dtype != torch.float32:
+        weight += half_step / 2
     return 2 * weight * largest + half_step * expected.abs() + smallest
 
 

@@ -255,7 +255,7 @@ def _check_window(case, device, window, sinks=0, lengths=None, starts=None):
     assert actual.dtype == case["query"].dtype and actual.is_contiguous()
     terms = case["key"].shape[2] if window == 0 else min(case["key"].shape[2], window + sinks)
     _close(actual, expected, ref.attention_bound(case["query"], case["key"], case["value"], case["scale"], max(terms, 1),
-                                                 case["query"].dtype, expected))
+                                                 case["query"].dtype, expected, case["query"].shape[2] > 1))
     return actual
 
 
@@ -274,6 +274,15 @@ def test_window_sizes(gpu_device, dtype, dim, window, sinks):
     _check_window(_window_case(3, dtype, 1, 3, 1, dim, 150, 150), gpu_device, window, sinks)
     _check_window(_window_case(5, dtype, 1, 2, 2, dim, 40, 170), gpu_device, window, sinks)
     _check_window(_window_case(6, dtype, 1, 2, 2, dim, 1, 170), gpu_device, window, sinks)
+
+
+@pytest.mark.parametrize("dtype,dim", [(torch.float32, 64), (torch.float16, 64), (torch.bfloat16, 128)])
+@pytest.mark.parametrize("scale", [0.0, -0.2, 1.5])
+def test_window_scales(gpu_device, dtype, dim, scale):
+    for queries in (60, 1):
+        case = {**_window_case(8, dtype, 1, 3, 1, dim, queries, 90), "scale": scale}
+        _check_window(case, gpu_device, 20, 2)
+        _check_window(case, gpu_device, 0, 0)
 
 
 @pytest.mark.parametrize("dtype", TYPES)
@@ -302,7 +311,7 @@ def test_window_longer_prompts(gpu_device, dtype, dim):
         expected = torch.softmax(scores, -1) @ values
         actual = ops.window_attention_native(**_to(case, gpu_device), window=window, sinks=sinks)
         _close(actual, expected, ref.attention_bound(case["query"], case["key"], case["value"], case["scale"], 1500, dtype,
-                                                     expected))
+                                                     expected, True))
 
 
 @pytest.mark.parametrize("dtype,dim", [(torch.float32, 64), (torch.bfloat16, 64), (torch.float16, 128)])
@@ -338,7 +347,8 @@ def test_window_nan_reaches_only_the_rows_that_see_it(gpu_device, dtype, dim):
             assert torch.equal(out[0, 2:], clean[0, 2:])
             for i in range(120):
                 if at not in ref.visible_keys(i, 120, window, sinks):
-                    torch.testing.assert_close(out[0, :2, i], clean[0, :2, i], rtol=4 * torch.finfo(dtype).eps, atol=1e-4)
+                    _close(out[0, :2, i], expected[0, :2, i], ref.attention_bound(
+                        case["query"], case["key"], case["value"], case["scale"], window + sinks, dtype, expected[0, :2, i], True))
                 else:
                     assert torch.equal(out[0, :2, i].isnan(), expected[0, :2, i].isnan()), (name, bad, at, i)
 
