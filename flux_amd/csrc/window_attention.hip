@@ -293,12 +293,18 @@ __global__ void __launch_bounds__(kThreads) window_attention_kernel(AttentionArg
 // exponentials, and weights up to 2^kLazy are as exact.  Weights are rounded to the values' type for the product (half
 // a step of that type, like the result's own rounding) and summed unrounded in float32.
 typedef float f32x16 __attribute__((ext_vector_type(16)));
+typedef float f32x2 __attribute__((ext_vector_type(2)));
+constexpr int kTileRun = 16;
 
 template <class T>
 struct Wide;
 template <>
 struct Wide<__bf16> {
     static constexpr float kShift = 0.0f;
+    typedef __bf16 Pair __attribute__((ext_vector_type(2)));
+    static __device__ __forceinline__ uint32_t round(float a, float b) {
+        return __builtin_bit_cast(uint32_t, __builtin_convertvector((f32x2{a, b}), Pair));
+    }
     static __device__ __forceinline__ f32x16 multiply(u32x4 a, u32x4 b, f32x16 c) {
         return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c,
                                                        0, 0, 0);
@@ -309,6 +315,10 @@ struct Wide<_Float16> {
     // Weights are held 2^6 times as large (at most 2^14), which keeps those down to 2^-20 of the largest in float16's
     // normal range.
     static constexpr float kShift = 6.0f;
+    typedef _Float16 Pair __attribute__((ext_vector_type(2)));
+    static __device__ __forceinline__ uint32_t round(float a, float b) {
+        return __builtin_bit_cast(uint32_t, __builtin_convertvector((f32x2{a, b}), Pair));
+    }
     static __device__ __forceinline__ f32x16 multiply(u32x4 a, u32x4 b, f32x16 c) {
         return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0,
                                                       0, 0);
@@ -324,12 +334,20 @@ __device__ __forceinline__ float half_sum(float v) {
     return __int_as_float(both[0]) + __int_as_float(both[1]);
 }
 
+// Eight values at `row`, which lies `d` dims into a key's: with kWide one load, else those before the row's end.
+template <class T, bool kWide>
+__device__ __forceinline__ u32x4 load_staged(const T* row, int d, int dim) {
+    if constexpr (kWide) return *reinterpret_cast<const u32x4*>(row);
+    return Mfma<T>::load_query(row, 1, 0, d < dim ? dim - d : dim, true);
+}
+
 template <class T, int kDim, int kRowTiles, bool kWide>
 __global__ void __launch_bounds__(kThreads, kRowTiles == 1 && kDim <= 128 ? 2 : 1)
 window_tile_kernel(AttentionArgs a, int row_tiles, int tiles_total) {
     using W = Wide<T>;
     constexpr int kKeys = kDim == 64 ? 128 : (kDim == 128 ? 64 : 32);
     constexpr int kSubs = kKeys / 32;
+    constexpr int kJoint = kSubs < 2 ? kSubs : 2; // 32-key tiles that share a maximum
     constexpr int kSteps = kDim / 16;             // of a score
     constexpr int kBlocks = kDim / 32;            // of the result
     constexpr int kRows = kWaves * kRowTiles * 32;
@@ -342,10 +360,11 @@ window_tile_kernel(AttentionArgs a, int row_tiles, int tiles_total) {
     constexpr float kLazy = 8.0f;
     extern __shared__ char stages[];
 
-    // Consecutive tiles share most of their keys: each XCD (block index modulo 8) takes a run of them.
-    const int run = tiles_total / 8, rest = tiles_total % 8;
-    const int xcd = blockIdx.x % 8;
-    const int tile = xcd * run + (xcd < rest ? xcd : rest) + blockIdx.x / 8;
+    // Consecutive tiles share most of their keys, so each XCD (block index modulo 8) takes runs of kTileRun of them.  The
+    // runs are short and the XCDs change places with every eight of them: a padded batch's sequences differ in length.
+    const int eight = blockIdx.x / (8 * kTileRun);
+    const int tile = (8 * eight + (blockIdx.x + eight) % 8) * kTileRun + blockIdx.x / 8 % kTileRun;
+    if (tile >= tiles_total) return;
     const int64_t row0 = static_cast<int64_t>(tile % row_tiles) * kRows;
     const int kv_head = tile / row_tiles % a.kv_heads;
     const int64_t b = tile / row_tiles / a.kv_heads;
@@ -372,6 +391,8 @@ window_tile_kernel(AttentionArgs a, int row_tiles, int tiles_total) {
     positions(row0, kRows, block_first, block_last);
     const int64_t wave_row = row0 + wave * kRowTiles * 32;
     positions(wave_row, kRowTiles * 32, wave_first, wave_last);
+    wave_first = __builtin_amdgcn_readfirstlane(wave_first);
+    wave_last = __builtin_amdgcn_readfirstlane(wave_last);
 
     const T* keys = static_cast<const T*>(a.key) + b * a.key_strides[0] + kv_head * a.key_strides[1];
     const T* values = static_cast<const T*>(a.value) + b * a.value_strides[0] + kv_head * a.value_strides[1];
@@ -416,25 +437,27 @@ window_tile_kernel(AttentionArgs a, int row_tiles, int tiles_total) {
         const int count = sink_stages + (seen + kKeys - 1) / kKeys - first_stage;
         auto stage_key = [&](int t) { return (t < sink_stages ? t : first_stage + t - sink_stages) * kKeys; };
 
+        // Loads are never masked: keys behind the last one repeat it and dims behind the head's repeat its first; the former
+        // have weight zero, the latter meet a zero in the query or are not stored.
         u32x4 held_key[kKeyLoads];
         u32x4 held_value[kValueLoads][4];
+        const int key_row = threadIdx.x / (kDim / 8), key_d = threadIdx.x % (kDim / 8) * 8;
+        const int value_row = threadIdx.x % (kKeys / 4) * 4, value_d = threadIdx.x / (kKeys / 4) * 8;
+        constexpr int kKeyRows = kThreads / (kDim / 8);  // rows that one load of all threads covers
+        static_assert(kValueLoads == 1, "one unit of values per thread");
+        const T* key_lane = keys + (key_d < a.dim ? key_d : 0);
+        const T* value_lane = values + (value_d < a.dim ? value_d : 0);
         auto fetch = [&](int t) {
-            const int base = stage_key(t);
+            const int base = stage_key(t), end = seen - 1 - base;
 #pragma unroll
             for (int i = 0; i < kKeyLoads; ++i) {
-                const int unit = threadIdx.x + kThreads * i;
-                const int key = base + unit / (kDim / 8), d = unit % (kDim / 8) * 8;
-                held_key[i] = Mfma<T>::template load_row<kWide>(keys + key * a.key_strides[2], d, a.dim, key < seen);
+                const int row = key_row + kKeyRows * i;
+                held_key[i] = load_staged<T, kWide>(key_lane + (base + (row < end ? row : end)) * a.key_strides[2], key_d, a.dim);
             }
 #pragma unroll
-            for (int i = 0; i < kValueLoads; ++i) {
-                const int unit = threadIdx.x + kThreads * i;
-                const int key = base + unit % (kKeys / 4) * 4, d = unit / (kKeys / 4) * 8;
-#pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    held_value[i][j] = Mfma<T>::template load_row<kWide>(values + (key + j) * a.value_strides[2], d, a.dim,
-                                                                         unit < kValueUnits && key + j < seen);
-                }
+            for (int j = 0; j < 4; ++j) {
+                const int row = value_row + j;
+                held_value[0][j] = load_staged<T, kWide>(value_lane + (base + (row < end ? row : end)) * a.value_strides[2], value_d, a.dim);
             }
         };
         auto put = [&](char* stage) {
@@ -471,39 +494,46 @@ window_tile_kernel(AttentionArgs a, int row_tiles, int tiles_total) {
             const int base = stage_key(t);
             if (t + 1 < count) fetch(t + 1);
 #pragma unroll
-            for (int s = 0; s < kSubs; ++s) {
-                const int first = base + 32 * s, last = first + 31;
+            for (int s0 = 0; s0 < kSubs; s0 += kJoint) {
+                const int first = base + 32 * s0, last = first + 32 * kJoint - 1;
                 // Nothing of this wave's rows sees these keys.
                 if (first > wave_last || (last < wave_low && first >= a.sinks)) continue;
-                f32x16 score[kRowTiles];
+                f32x16 score[kJoint][kRowTiles];
 #pragma unroll
-                for (int c = 0; c < kRowTiles; ++c)
+                for (int s = 0; s < kJoint; ++s) {
 #pragma unroll
-                    for (int j = 0; j < 16; ++j) score[c][j] = 0.0f;
+                    for (int c = 0; c < kRowTiles; ++c)
 #pragma unroll
-                for (int k = 0; k < kSteps; ++k) {
-                    const u32x4 key = *reinterpret_cast<const u32x4*>(stage + (32 * s + n32) * kKeyRow + 32 * k + 16 * half);
+                        for (int j = 0; j < 16; ++j) score[s][c][j] = 0.0f;
 #pragma unroll
-                    for (int c = 0; c < kRowTiles; ++c) score[c] = W::multiply(key, query[c][k], score[c]);
+                    for (int k = 0; k < kSteps; ++k) {
+                        const u32x4 key = *reinterpret_cast<const u32x4*>(stage + (32 * (s0 + s) + n32) * kKeyRow + 32 * k + 16 * half);
+#pragma unroll
+                        for (int c = 0; c < kRowTiles; ++c) score[s][c] = W::multiply(key, query[c][k], score[s][c]);
+                    }
                 }
                 const bool inside = first >= low_of_last && last <= wave_first;
-                u32x4 p[kRowTiles][2];
+                u32x4 p[kJoint][kRowTiles][2];
 #pragma unroll
                 for (int c = 0; c < kRowTiles; ++c) {
                     if (!inside) {
 #pragma unroll
-                        for (int j = 0; j < 16; ++j) {
-                            // Without branches: low <= key <= position as one unsigned comparison, or a sink.
-                            const int key = first + 8 * (j / 4) + 4 * half + j % 4;
-                            const bool visible = (static_cast<uint32_t>(key - mine[c].low) <=
-                                                  static_cast<uint32_t>(mine[c].position - mine[c].low)) |
-                                                 (key < sink_end[c]);
-                            score[c][j] = visible ? score[c][j] : -INFINITY;
-                        }
-                    }
-                    float highest = score[c][0];
+                        for (int s = 0; s < kJoint; ++s)
 #pragma unroll
-                    for (int j = 1; j < 16; ++j) highest = fmaxf(highest, score[c][j]);
+                            for (int j = 0; j < 16; ++j) {
+                                // Without branches: low <= key <= position as one unsigned comparison, or a sink.
+                                const int key = first + 32 * s + 8 * (j / 4) + 4 * half + j % 4;
+                                const bool visible = (static_cast<uint32_t>(key - mine[c].low) <=
+                                                      static_cast<uint32_t>(mine[c].position - mine[c].low)) |
+                                                     (key < sink_end[c]);
+                                score[s][c][j] = visible ? score[s][c][j] : -INFINITY;
+                            }
+                    }
+                    float highest = score[0][c][0];
+#pragma unroll
+                    for (int s = 0; s < kJoint; ++s)
+#pragma unroll
+                        for (int j = 0; j < 16; ++j) highest = fmaxf(highest, score[s][c][j]);
                     highest = half_max(highest) * factor;
                     if (__any(highest > top[c] + kLazy)) {
                         const float now = fmaxf(top[c], highest);
@@ -515,24 +545,30 @@ window_tile_kernel(AttentionArgs a, int row_tiles, int tiles_total) {
 #pragma unroll
                             for (int j = 0; j < 16; ++j) out[c][i][j] *= shrink;
                     }
-                    const float reference = W::kShift - (top[c] == -INFINITY ? 0.0f : top[c]);
-#pragma unroll
-                    for (int j = 0; j < 16; j += 2) {
-                        const float p0 = fast_exp2(fmaf(score[c][j], factor, reference));
-                        const float p1 = fast_exp2(fmaf(score[c][j + 1], factor, reference));
-                        weight[c] += p0 + p1;
-                        p[c][j / 8][j % 8 / 2] = Mfma<T>::bits(static_cast<T>(p0)) | Mfma<T>::bits(static_cast<T>(p1)) << 16;
-                    }
                 }
 #pragma unroll
-                for (int i = 0; i < kBlocks; ++i)
+                for (int s = 0; s < kJoint; ++s) {
 #pragma unroll
-                    for (int k = 0; k < 2; ++k) {
-                        const u32x4 value = *reinterpret_cast<const u32x4*>(turned + (32 * i + n32) * kValueRow +
-                                                                            (32 * s + 16 * k) * 2 + 16 * half);
+                    for (int c = 0; c < kRowTiles; ++c) {
+                        const float reference = W::kShift - (top[c] == -INFINITY ? 0.0f : top[c]);
 #pragma unroll
-                        for (int c = 0; c < kRowTiles; ++c) out[c][i] = W::multiply(value, p[c][k], out[c][i]);
+                        for (int j = 0; j < 16; j += 2) {
+                            const float p0 = fast_exp2(fmaf(score[s][c][j], factor, reference));
+                            const float p1 = fast_exp2(fmaf(score[s][c][j + 1], factor, reference));
+                            weight[c] += p0 + p1;
+                            p[s][c][j / 8][j % 8 / 2] = W::round(p0, p1);
+                        }
                     }
+#pragma unroll
+                    for (int i = 0; i < kBlocks; ++i)
+#pragma unroll
+                        for (int k = 0; k < 2; ++k) {
+                            const u32x4 value = *reinterpret_cast<const u32x4*>(turned + (32 * i + n32) * kValueRow +
+                                                                                (32 * (s0 + s) + 16 * k) * 2 + 16 * half);
+#pragma unroll
+                            for (int c = 0; c < kRowTiles; ++c) out[c][i] = W::multiply(value, p[s][c][k], out[c][i]);
+                        }
+                }
             }
             if (t + 1 < count) put(stages + ((t + 1) & 1) * kStage);
         }
@@ -600,8 +636,8 @@ hipError_t launch_window_tiles(const AttentionArgs& a, hipStream_t stream) {
         reinterpret_cast<const void*>(window_tile_kernel<T, kDim, kRowTiles, kWide>), hipFuncAttributeMaxDynamicSharedMemorySize,
         static_cast<int>(kLds));
     if (room != hipSuccess) return room;
-    hipLaunchKernelGGL(HIP_KERNEL_NAME(window_tile_kernel<T, kDim, kRowTiles, kWide>), dim3(static_cast<uint32_t>(tiles)),
-                       dim3(kThreads), kLds, stream, a, row_tiles, static_cast<int>(tiles));
+    hipLaunchKernelGGL(HIP_KERNEL_NAME(window_tile_kernel<T, kDim, kRowTiles, kWide>), 
+                       dim3(static_cast<uint32_t>((tiles + 8 * kTileRun - 1) / (8 * kTileRun) * (8 * kTileRun))), dim3(kThreads), kLds, stream, a, row_tiles, static_cast<int>(tiles));
     return hipGetLastError();
 }
 
