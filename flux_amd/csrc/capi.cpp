@@ -724,6 +724,8 @@ const char* attention_arguments(flux::AttentionArgs& args, int dtype, const void
     }
     args.wide = wide_rows(key, key_strides, 3, head_dim, flux::type_bytes(type)) &&
                 wide_rows(value, value_strides, 3, head_dim, flux::type_bytes(type));
+    args.query_wide = query_strides[3] == 1 && wide_rows(query, query_strides, 3, head_dim, flux::type_bytes(type));
+    args.group_of = flux::make_divider(static_cast<uint32_t>(args.group));
     args.blocks = flux::decode_attention_blocks(args.batch, keys, args.kv_heads, args.group, args.window, args.sinks);
     return nullptr;
 }

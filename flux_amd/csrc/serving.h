@@ -53,6 +53,7 @@ struct AttentionArgs {
     int query_heads;
     int kv_heads;
     int group;               // query heads per KV head
+    Divider group_of;        // divides by group
     int dim;
     int queries;
     int64_t keys;            // positions a sequence can hold
@@ -66,6 +67,7 @@ struct AttentionArgs {
     int64_t key_strides[3];    // batch (page when paged), head, row
     int64_t value_strides[3];
     bool wide;               // every key and value row starts at 16 bytes and dim fills whole 16-byte quads
+    bool query_wide;         // the same of query rows, with a dim stride of 1
     int blocks;              // workgroups over the keys, per KV head and column tile
 };
 

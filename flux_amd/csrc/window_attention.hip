@@ -347,7 +347,7 @@ window_tile_kernel(AttentionArgs a, int row_tiles, int tiles_total) {
     using W = Wide<T>;
     constexpr int kKeys = kDim == 64 ? 128 : (kDim == 128 ? 64 : 32);
     constexpr int kSubs = kKeys / 32;
-    constexpr int kJoint = kSubs < 2 ? kSubs : 2; // 32-key tiles that share a maximum
+    constexpr int kJoint = 1;
     constexpr int kSteps = kDim / 16;             // of a score
     constexpr int kBlocks = kDim / 32;            // of the result
     constexpr int kRows = kWaves * kRowTiles * 32;
@@ -365,7 +365,7 @@ window_tile_kernel(AttentionArgs a, int row_tiles, int tiles_total) {
     const int eight = blockIdx.x / (8 * kTileRun);
     const int tile = (8 * eight + (blockIdx.x + eight) % 8) * kTileRun + blockIdx.x / 8 % kTileRun;
     if (tile >= tiles_total) return;
-    const int64_t row0 = static_cast<int64_t>(tile % row_tiles) * kRows;
+    const int row0 = tile % row_tiles * kRows;
     const int kv_head = tile / row_tiles % a.kv_heads;
     const int64_t b = tile / row_tiles / a.kv_heads;
 
@@ -380,16 +380,16 @@ window_tile_kernel(AttentionArgs a, int row_tiles, int tiles_total) {
     const int all_rows = a.queries * a.group;
 
     // Positions of a range of rows, cut to those that are a key's; first > last when there is none.
-    auto positions = [&](int64_t from, int64_t count, int& first, int& last) {
-        const int64_t to = from + count < all_rows ? from + count - 1 : all_rows - 1;
-        const int64_t p = start + from / a.group, q = start + to / a.group;
+    auto positions = [&](int from, int count, int& first, int& last) {
+        const int to = from + count < all_rows ? from + count - 1 : all_rows - 1;
+        const int64_t p = start + divide(from, a.group_of), q = start + divide(to, a.group_of);
         first = static_cast<int>(p < 0 ? 0 : p);
         last = static_cast<int>(q >= n ? n - 1 : q);
         if (from > to) last = first - 1;
     };
     int block_first, block_last, wave_first, wave_last;
     positions(row0, kRows, block_first, block_last);
-    const int64_t wave_row = row0 + wave * kRowTiles * 32;
+    const int wave_row = row0 + wave * kRowTiles * 32;
     positions(wave_row, kRowTiles * 32, wave_first, wave_last);
     wave_first = __builtin_amdgcn_readfirstlane(wave_first);
     wave_last = __builtin_amdgcn_readfirstlane(wave_last);
@@ -406,8 +406,8 @@ window_tile_kernel(AttentionArgs a, int row_tiles, int tiles_total) {
     const float factor = fmaxf(fabsf(a.scale) * kLog2e, 1e-37f);  // above 0: a masked score stays -inf
 #pragma unroll
     for (int c = 0; c < kRowTiles; ++c) {
-        const int64_t r = wave_row + 32 * c + n32;
-        const int64_t i = r / a.group, head = kv_head * static_cast<int64_t>(a.group) + r % a.group;
+        const int r = wave_row + 32 * c + n32;
+        const int64_t i = divide(r, a.group_of), head = kv_head * a.group + r - i * a.group;
         const int64_t position = start + i;
         mine[c].position = r < all_rows && position >= 0 && position < n ? static_cast<int>(position) : -1;
         mine[c].low = a.window > 0 && mine[c].position >= a.window ? mine[c].position - a.window + 1 : 0;
@@ -415,7 +415,9 @@ window_tile_kernel(AttentionArgs a, int row_tiles, int tiles_total) {
         const T* q = static_cast<const T*>(a.query) + b * a.query_strides[0] + head * a.query_strides[1] + i * a.query_strides[2];
 #pragma unroll
         for (int s = 0; s < kSteps; ++s) {
-            query[c][s] = Mfma<T>::load_query(q, a.query_strides[3], 16 * s + 8 * half, a.dim, r < all_rows);
+            const int d = 16 * s + 8 * half;
+            if (a.query_wide) query[c][s] = Mfma<T>::template load_row<true>(q, d, a.dim, r < all_rows);
+            else query[c][s] = Mfma<T>::load_query(q, a.query_strides[3], d, a.dim, r < all_rows);
             query[c][s] ^= sign;
         }
 #pragma unroll
@@ -447,25 +449,30 @@ window_tile_kernel(AttentionArgs a, int row_tiles, int tiles_total) {
         static_assert(kValueLoads == 1, "one unit of values per thread");
         const T* key_lane = keys + (key_d < a.dim ? key_d : 0);
         const T* value_lane = values + (value_d < a.dim ? value_d : 0);
-        auto fetch = [&](int t) {
+        auto fetch_keys = [&](int t) {
             const int base = stage_key(t), end = seen - 1 - base;
 #pragma unroll
             for (int i = 0; i < kKeyLoads; ++i) {
                 const int row = key_row + kKeyRows * i;
                 held_key[i] = load_staged<T, kWide>(key_lane + (base + (row < end ? row : end)) * a.key_strides[2], key_d, a.dim);
             }
+        };
+        auto fetch_values = [&](int t) {
+            const int base = stage_key(t), end = seen - 1 - base;
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
                 const int row = value_row + j;
                 held_value[0][j] = load_staged<T, kWide>(value_lane + (base + (row < end ? row : end)) * a.value_strides[2], value_d, a.dim);
             }
         };
-        auto put = [&](char* stage) {
+        auto put_keys = [&](char* stage) {
 #pragma unroll
             for (int i = 0; i < kKeyLoads; ++i) {
                 const int unit = threadIdx.x + kThreads * i;
                 *reinterpret_cast<u32x4*>(stage + unit / (kDim / 8) * kKeyRow + unit % (kDim / 8) * 16) = held_key[i];
             }
+        };
+        auto put_values = [&](char* stage) {
             char* turned = stage + kKeys * kKeyRow;
 #pragma unroll
             for (int i = 0; i < kValueLoads; ++i) {
@@ -485,18 +492,25 @@ window_tile_kernel(AttentionArgs a, int row_tiles, int tiles_total) {
         };
 
         const int wave_low = low_of(wave_first), low_of_last = low_of(wave_last);
-        fetch(0);
-        put(stages);
+        fetch_keys(0);
+        fetch_values(0);
+        put_keys(stages);
+        put_values(stages);
         for (int t = 0; t < count; ++t) {
             __syncthreads();
             const char* stage = stages + (t & 1) * kStage;
             const char* turned = stage + kKeys * kKeyRow;
             const int base = stage_key(t);
-            if (t + 1 < count) fetch(t + 1);
+            char* next = stages + ((t + 1) & 1) * kStage;
+            if (t + 1 < count) fetch_keys(t + 1);
 #pragma unroll
             for (int s0 = 0; s0 < kSubs; s0 += kJoint) {
                 const int first = base + 32 * s0, last = first + 32 * kJoint - 1;
                 // Nothing of this wave's rows sees these keys.
+                if (s0 == kSubs / 2 && t + 1 < count) {
+                    put_keys(next);
+                    fetch_values(t + 1);
+                }
                 if (first > wave_last || (last < wave_low && first >= a.sinks)) continue;
                 f32x16 score[kJoint][kRowTiles];
 #pragma unroll
@@ -505,12 +519,15 @@ window_tile_kernel(AttentionArgs a, int row_tiles, int tiles_total) {
                     for (int c = 0; c < kRowTiles; ++c)
 #pragma unroll
                         for (int j = 0; j < 16; ++j) score[s][c][j] = 0.0f;
+                    u32x4 key[kSteps];
 #pragma unroll
-                    for (int k = 0; k < kSteps; ++k) {
-                        const u32x4 key = *reinterpret_cast<const u32x4*>(stage + (32 * (s0 + s) + n32) * kKeyRow + 32 * k + 16 * half);
+                    for (int k = 0; k < kSteps; ++k)
+                        key[k] = *reinterpret_cast<const u32x4*>(stage + (32 * (s0 + s) + n32) * kKeyRow + 32 * k + 16 * half);
+                    __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-                        for (int c = 0; c < kRowTiles; ++c) score[s][c] = W::multiply(key, query[c][k], score[s][c]);
-                    }
+                    for (int k = 0; k < kSteps; ++k)
+#pragma unroll
+                        for (int c = 0; c < kRowTiles; ++c) score[s][c] = W::multiply(key[k], query[c][k], score[s][c]);
                 }
                 const bool inside = first >= low_of_last && last <= wave_first;
                 u32x4 p[kJoint][kRowTiles][2];
@@ -548,6 +565,14 @@ window_tile_kernel(AttentionArgs a, int row_tiles, int tiles_total) {
                 }
 #pragma unroll
                 for (int s = 0; s < kJoint; ++s) {
+                    u32x4 value[kBlocks][2];
+#pragma unroll
+                    for (int i = 0; i < kBlocks; ++i)
+#pragma unroll
+                        for (int k = 0; k < 2; ++k)
+                            value[i][k] = *reinterpret_cast<const u32x4*>(turned + (32 * i + n32) * kValueRow +
+                                                                          (32 * (s0 + s) + 16 * k) * 2 + 16 * half);
+                    __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
                     for (int c = 0; c < kRowTiles; ++c) {
                         const float reference = W::kShift - (top[c] == -INFINITY ? 0.0f : top[c]);
@@ -562,15 +587,12 @@ window_tile_kernel(AttentionArgs a, int row_tiles, int tiles_total) {
 #pragma unroll
                     for (int i = 0; i < kBlocks; ++i)
 #pragma unroll
-                        for (int k = 0; k < 2; ++k) {
-                            const u32x4 value = *reinterpret_cast<const u32x4*>(turned + (32 * i + n32) * kValueRow +
-                                                                                (32 * (s0 + s) + 16 * k) * 2 + 16 * half);
+                        for (int k = 0; k < 2; ++k)
 #pragma unroll
-                            for (int c = 0; c < kRowTiles; ++c) out[c][i] = W::multiply(value, p[s][c][k], out[c][i]);
-                        }
+                            for (int c = 0; c < kRowTiles; ++c) out[c][i] = W::multiply(value[i][k], p[s][c][k], out[c][i]);
                 }
             }
-            if (t + 1 < count) put(stages + ((t + 1) & 1) * kStage);
+            if (t + 1 < count) put_values(next);
         }
     }
 
@@ -584,8 +606,8 @@ window_tile_kernel(AttentionArgs a, int row_tiles, int tiles_total) {
             for (int j = 0; j < 16; ++j) worst += fabsf(out[c][i][j]);  // keeps NaN, infinity
         const uint64_t odd = __ballot(mine[c].position >= 0 && !(worst < INFINITY));
         uint32_t rows = static_cast<uint32_t>(odd | odd >> 32);
-        const int64_t r = wave_row + 32 * c + n32;
-        const int64_t i = r / a.group, head = kv_head * static_cast<int64_t>(a.group) + r % a.group;
+        const int r = wave_row + 32 * c + n32;
+        const int64_t i = divide(r, a.group_of), head = kv_head * a.group + r - i * a.group;
         if (r < all_rows && !(rows >> n32 & 1)) {
             T* o = static_cast<T*>(a.out) + ((b * a.query_heads + head) * a.queries + i) * a.dim;
             const float inverse = mine[c].position < 0 ? 0.0f : 1.0f / weight[c];
@@ -612,8 +634,8 @@ window_tile_kernel(AttentionArgs a, int row_tiles, int tiles_total) {
         while (rows) {
             const int which = __ffs(rows) - 1;
             rows &= rows - 1;
-            const int64_t r = wave_row + 32 * c + which;
-            const int64_t i = r / a.group, head = kv_head * static_cast<int64_t>(a.group) + r % a.group;
+            const int r = wave_row + 32 * c + which;
+            const int64_t i = divide(r, a.group_of), head = kv_head * a.group + r - i * a.group;
             RowRange range;
             range.position = static_cast<int>(start + i);
             range.low = a.window > 0 && range.position >= a.window ? range.position - a.window + 1 : 0;
