@@ -295,6 +295,7 @@ __global__ void __launch_bounds__(kThreads) window_attention_kernel(AttentionArg
 typedef float f32x16 __attribute__((ext_vector_type(16)));
 typedef float f32x2 __attribute__((ext_vector_type(2)));
 constexpr int kTileRun = 16;
+constexpr int64_t kStagedStride = 1 << 22;
 
 template <class T>
 struct Wide;
@@ -334,12 +335,21 @@ __device__ __forceinline__ float half_sum(float v) {
     return __int_as_float(both[0]) + __int_as_float(both[1]);
 }
 
-// Eight values at `row`, which lies `d` dims into a key's: with kWide one load, else those before the row's end.
+// Rows of one stage.  With kWide 16 bytes at a byte offset through a buffer that ends with the last row (kStagedStride
+// keeps offsets in 31 bits); else eight elements by comparisons.
 template <class T, bool kWide>
-__device__ __forceinline__ u32x4 load_staged(const T* row, int d, int dim) {
-    if constexpr (kWide) return *reinterpret_cast<const u32x4*>(row);
-    return Mfma<T>::load_query(row, 1, 0, d < dim ? dim - d : dim, true);
-}
+struct StagedRows {
+    const T* base;
+    __amdgpu_buffer_rsrc_t buffer;
+    __device__ __forceinline__ StagedRows(const T* from, int64_t bytes) : base(from) {
+        if constexpr (kWide)
+            buffer = __builtin_amdgcn_make_buffer_rsrc(const_cast<T*>(from), 0, static_cast<int>(bytes), 0x00020000);
+    }
+    __device__ __forceinline__ u32x4 load(int at, int row, int d, int rows, int64_t stride, int dim) const {
+        if constexpr (kWide) return __builtin_amdgcn_raw_buffer_load_b128(buffer, at, 0, 0);
+        return Mfma<T>::load_query(base + row * stride, 1, d, dim, row < rows);
+    }
+};
 
 template <class T, int kDim, int kRowTiles, bool kWide>
 __global__ void __launch_bounds__(kThreads, kRowTiles == 1 && kDim <= 128 ? 2 : 1)
@@ -439,31 +449,32 @@ window_tile_kernel(AttentionArgs a, int row_tiles, int tiles_total) {
         const int count = sink_stages + (seen + kKeys - 1) / kKeys - first_stage;
         auto stage_key = [&](int t) { return (t < sink_stages ? t : first_stage + t - sink_stages) * kKeys; };
 
-        // Loads are never masked: keys behind the last one repeat it and dims behind the head's repeat its first; the former
-        // have weight zero, the latter meet a zero in the query or are not stored.
+        // Rows behind the last key give zeros (a buffer's range check, or a comparison), dims behind the head's repeat its
+        // first: they meet a zero in the query or are not stored.
         u32x4 held_key[kKeyLoads];
         u32x4 held_value[kValueLoads][4];
         const int key_row = threadIdx.x / (kDim / 8), key_d = threadIdx.x % (kDim / 8) * 8;
         const int value_row = threadIdx.x % (kKeys / 4) * 4, value_d = threadIdx.x / (kKeys / 4) * 8;
         constexpr int kKeyRows = kThreads / (kDim / 8);  // rows that one load of all threads covers
         static_assert(kValueLoads == 1, "one unit of values per thread");
-        const T* key_lane = keys + (key_d < a.dim ? key_d : 0);
-        const T* value_lane = values + (value_d < a.dim ? value_d : 0);
+        const int key_stride = static_cast<int>(a.key_strides[2]), value_stride = static_cast<int>(a.value_strides[2]);
+        const int key_at = (key_row * key_stride + (key_d < a.dim ? key_d : 0)) * 2;
+        const int value_at = (value_row * value_stride + (value_d < a.dim ? value_d : 0)) * 2;
         auto fetch_keys = [&](int t) {
-            const int base = stage_key(t), end = seen - 1 - base;
+            const int base = stage_key(t), rows = seen - base < kKeys ? seen - base : kKeys;
+            const T* from = keys + base * a.key_strides[2];
+            const StagedRows<T, kWide> staged(from, ((rows - 1) * a.key_strides[2] + a.dim) * 2);
 #pragma unroll
-            for (int i = 0; i < kKeyLoads; ++i) {
-                const int row = key_row + kKeyRows * i;
-                held_key[i] = load_staged<T, kWide>(key_lane + (base + (row < end ? row : end)) * a.key_strides[2], key_d, a.dim);
-            }
+            for (int i = 0; i < kKeyLoads; ++i)
+                held_key[i] = staged.load(key_at + kKeyRows * i * key_stride * 2, key_row + kKeyRows * i, key_d, rows, a.key_strides[2], a.dim);
         };
         auto fetch_values = [&](int t) {
-            const int base = stage_key(t), end = seen - 1 - base;
+            const int base = stage_key(t), rows = seen - base < kKeys ? seen - base : kKeys;
+            const T* from = values + base * a.value_strides[2];
+            const StagedRows<T, kWide> staged(from, ((rows - 1) * a.value_strides[2] + a.dim) * 2);
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                const int row = value_row + j;
-                held_value[0][j] = load_staged<T, kWide>(value_lane + (base + (row < end ? row : end)) * a.value_strides[2], value_d, a.dim);
-            }
+            for (int j = 0; j < 4; ++j)
+                held_value[0][j] = staged.load(value_at + j * value_stride * 2, value_row + j, value_d, rows, a.value_strides[2], a.dim);
         };
         auto put_keys = [&](char* stage) {
 #pragma unroll
@@ -616,18 +627,17 @@ window_tile_kernel(AttentionArgs a, int row_tiles, int tiles_total) {
 #pragma unroll
                 for (int j = 0; j < 16; j += 4) {
                     const int d = 32 * k + 2 * j + 4 * half;  // four dims side by side
-                    T four[4];
+                    float four[4];
 #pragma unroll
-                    for (int l = 0; l < 4; ++l)
-                        four[l] = static_cast<T>(mine[c].position < 0 ? 0.0f : out[c][k][j + l] * inverse);
+                    for (int l = 0; l < 4; ++l) four[l] = mine[c].position < 0 ? 0.0f : out[c][k][j + l] * inverse;
+                    const u32x2 rounded = {W::round(four[0], four[1]), W::round(four[2], four[3])};
                     if constexpr (kWide) {
-                        if (d < a.dim)
-                            *reinterpret_cast<u32x2*>(o + d) = u32x2{Mfma<T>::bits(four[0]) | Mfma<T>::bits(four[1]) << 16,
-                                                                     Mfma<T>::bits(four[2]) | Mfma<T>::bits(four[3]) << 16};
+                        if (d < a.dim) *reinterpret_cast<u32x2*>(o + d) = rounded;
                     } else {
 #pragma unroll
                         for (int l = 0; l < 4; ++l)
-                            if (d + l < a.dim) o[d + l] = four[l];
+                            if (d + l < a.dim)
+                                o[d + l] = __builtin_bit_cast(T, static_cast<uint16_t>(rounded[l / 2] >> 16 * (l % 2)));
                     }
                 }
         }
@@ -666,7 +676,8 @@ hipError_t launch_window_tiles(const AttentionArgs& a, hipStream_t stream) {
 template <class T, int kDim>
 hipError_t launch_window(const AttentionArgs& a, hipStream_t stream) {
     if constexpr (sizeof(T) == 2) {
-        if (a.wide && reinterpret_cast<uintptr_t>(a.out) % 8 == 0)
+        if (a.wide && reinterpret_cast<uintptr_t>(a.out) % 8 == 0 && a.key_strides[2] <= kStagedStride &&
+            a.value_strides[2] <= kStagedStride)
             return launch_window_tiles<T, kDim, FLUX_ROW_TILES, true>(a, stream);
         return launch_window_tiles<T, kDim, FLUX_ROW_TILES, false>(a, stream);
     } else {
