@@ -4,14 +4,15 @@
 //   s_j = scale * <q, k_j>,  m = max s_j,  p_j = exp(s_j - m),  o = sum p_j v_j / sum p_j   over the visible keys j;
 //   a sequence of n keys sees j < n with j >= n - window or j < sinks (window 0: all); nothing visible gives zeros.
 //
-// Every key and value row is read once for all query heads of its KV head, and HBM bounds the whole.  The tiles of all
-// sequences form one line that is cut into equal parts, one per workgroup, so that ragged lengths load the card
-// evenly; a part that begins or ends inside a sequence leaves (o, m, l) in the workspace and a second launch joins
-// them: o = sum o_c exp(m_c - M) / sum l_c exp(m_c - M).
+// Every key and value row is read once for all query heads of its KV head, and HBM bounds the whole.  A sequence is cut
+// into parts of about the same number of tiles as every other part of the batch, one per workgroup, so that ragged
+// lengths load the card evenly; the parts of a sequence that was cut leave (o, m, l) in the workspace and a second launch
+// joins them: o = sum o_c exp(m_c - M) / sum l_c exp(m_c - M).
 //
-// A wave takes 16 or 32 keys at a time straight into registers, laid out as the matrix instruction wants them.  Scores
-// come as S^T = K Q^T (rows: keys, columns: query heads), so the lane that holds scores of four keys holds what
-// O^T = V^T P needs as its right operand; V's left operand is transposed inside the lane by byte permutes.
+// A wave takes 16 or 32 keys at a time straight into registers, laid out as the matrix instruction wants them, while the
+// tile before is worked on.  Scores come as S^T = K Q^T (rows: keys, columns: query heads), so the lane that holds
+// scores of four keys holds what O^T = V^T P needs as its right operand; V's left operand is transposed inside the
+// lane by byte permutes.
 #include "serving.h"
 #include "serving_mfma.h"
 
@@ -33,56 +34,59 @@ struct Span {
     int sinks;
 };
 
-template <int kTile>
-__device__ __forceinline__ Span span_of(const AttentionArgs& a, int64_t b) {
-    Span s{0, 0, 0, 0, 0, 0};
+// Keys up to the query's own, 0 for a sequence that sees nothing.
+__device__ __forceinline__ int seen_of(const AttentionArgs& a, int64_t b) {
     const int64_t slot = a.slots ? a.slots[b] : b;
-    if (slot < 0 || slot >= a.slot_count) return s;
+    if (slot < 0 || slot >= a.slot_count) return 0;
     int64_t n = a.lengths ? a.lengths[slot] : a.keys;
     n = n < 0 ? 0 : (n > a.keys ? a.keys : n);
     const int64_t position = a.starts ? a.starts[b] : n - 1;
-    if (position < 0 || position >= n) return s;
-    s.seen = static_cast<int>(position) + 1;
-    s.low = a.window > 0 && s.seen > a.window ? s.seen - a.window : 0;
+    return position < 0 || position >= n ? 0 : static_cast<int>(position) + 1;
+}
+
+template <int kTile>
+__device__ __forceinline__ Span span_of(const AttentionArgs& a, int seen) {
+    Span s;
+    s.seen = seen;
+    s.low = a.window > 0 && seen > a.window ? seen - a.window : 0;
     s.sinks = a.sinks < s.low ? a.sinks : s.low;
     s.first_tile = s.low / kTile;
     const int of_sinks = (s.sinks + kTile - 1) / kTile;
     s.sink_tiles = of_sinks < s.first_tile ? of_sinks : s.first_tile;
-    s.tiles = s.sink_tiles + (s.seen + kTile - 1) / kTile - s.first_tile;
+    s.tiles = s.sink_tiles + (seen + kTile - 1) / kTile - s.first_tile;
     return s;
 }
 
-// Parts in use and the tiles [lo, hi) of one of them, of `total` tiles.
-__device__ __forceinline__ int parts_of(int64_t total, int blocks) {
-    const int64_t most = (total + kLeastTiles - 1) / kLeastTiles;
-    return static_cast<int>(most < blocks ? most : blocks);
+// Tiles of a part and the parts of a sequence; one that sees nothing has one part, which writes its zeros.
+__device__ __forceinline__ int part_tiles(int64_t total, int target) {
+    const int64_t even = (total + target - 1) / target;
+    return even < kLeastTiles ? kLeastTiles : static_cast<int>(even);
 }
-__device__ __forceinline__ int64_t part_begin(int64_t total, int parts, int64_t part) { return total * part / parts; }
-// The part that holds a tile: the largest one that begins at or before it.
-__device__ __forceinline__ int part_of(int64_t total, int parts, int64_t tile) {
-    int64_t part = (tile * parts) / total;
-    while (part + 1 < parts && part_begin(total, parts, part + 1) <= tile) ++part;
-    return static_cast<int>(part);
+__device__ __forceinline__ int parts_of(int tiles, int each) { return tiles > each ? (tiles + each - 1) / each : 1; }
+__device__ __forceinline__ int part_begin(int tiles, int parts, int part) {
+    return static_cast<int>(static_cast<int64_t>(tiles) * part / parts);
 }
 
-__device__ __forceinline__ int64_t partial_offset(const AttentionArgs& a, int64_t head_tile, int part, int which,
-                                                  int column) {
+__device__ __forceinline__ int64_t partial_offset(const AttentionArgs& a, int64_t head_tile, int64_t block, int column) {
     const int columns = a.group < kColumns ? a.group : kColumns;
-    return (((head_tile * a.blocks + part) * 2 + which) * columns + column) * (a.dim + 2);
+    return ((head_tile * (a.blocks + a.batch) + block) * columns + column) * (a.dim + 2);
 }
 
+// Sum over the workgroup, the same in every thread.
 __device__ __forceinline__ int64_t block_sum(int v, int* sums) {
-    const int inclusive = static_cast<int>(wave_sum_int(v));
+    const int sum = wave_sum_int(v);
     __syncthreads();
-    if ((threadIdx.x & 63) == 0) sums[threadIdx.x >> 6] = inclusive;
+    if ((threadIdx.x & 63) == 0) sums[threadIdx.x >> 6] = sum;
     __syncthreads();
     return static_cast<int64_t>(sums[0]) + sums[1] + sums[2] + sums[3];
 }
 
+constexpr int tile_of(int dim, int bytes) { return dim * bytes <= 256 ? 32 : 16; }
+
 template <class T, int kDim, bool kPaged, bool kWide>
-__global__ void __launch_bounds__(kDecodeThreads) decode_attention_kernel(AttentionArgs a) {
+__global__ void __launch_bounds__(kDecodeThreads, kDim * sizeof(T) <= 512 ? 2 : 1) decode_attention_kernel(AttentionArgs a) {
     using M = Mfma<T>;
-    constexpr int kTile = kDim * static_cast<int>(sizeof(T)) <= 256 ? 32 : 16;
+    constexpr int kTile = tile_of(kDim, sizeof(T));
     constexpr int kSubs = kTile / 16;
     constexpr int kFragments = M::template key_fragments<kDim>();  // of 16 bytes per lane
     constexpr int kChunks = M::template value_chunks<kDim>();
@@ -90,8 +94,7 @@ __global__ void __launch_bounds__(kDecodeThreads) decode_attention_kernel(Attent
     using Value = typename M::template ValueChunk<kDim>;
 
     __shared__ int sums[kDecodeWaves];
-    __shared__ int prefix[kDecodeThreads + 1];
-    __shared__ int first_index;
+    __shared__ int chosen[4];  // sequence, keys it sees, part, parts
     __shared__ float merge[2][kBlocks * 4 + 2][kWave];
 
     const int lane = threadIdx.x & 63;
@@ -103,231 +106,302 @@ __global__ void __launch_bounds__(kDecodeThreads) decode_attention_kernel(Attent
     const int column0 = blockIdx.y % column_tiles * kColumns;
     const int columns = a.group - column0 < kColumns ? a.group - column0 : kColumns;
 
+    // The part of this workgroup: the blockIdx.x-th of all sequences' parts.
     int64_t total = 0;
+    int seen = 0;
     for (int base = 0; base < a.batch; base += kDecodeThreads) {
-        const int b = base + threadIdx.x;
-        total += block_sum(b < a.batch ? span_of<kTile>(a, b).tiles : 0, sums);
+        const int b = base + static_cast<int>(threadIdx.x);
+        seen = b < a.batch ? seen_of(a, b) : 0;
+        total += block_sum(span_of<kTile>(a, seen).tiles, sums);
     }
-    if (total == 0) return;
-    const int parts = parts_of(total, a.blocks);
-    const int part = blockIdx.x;
-    if (part >= parts) return;
-    const int64_t lo = part_begin(total, parts, part), hi = part_begin(total, parts, part + 1);
-
+    const int each = part_tiles(total, a.blocks);
     int64_t running = 0;
-    for (int base = 0; base < a.batch && running < hi; base += kDecodeThreads) {
-        // Where this round's sequences begin on the line.
-        const int mine = base + static_cast<int>(threadIdx.x) < a.batch ? span_of<kTile>(a, base + threadIdx.x).tiles : 0;
-        const int inclusive = wave_scan_int(mine);
+    for (int base = 0; base < a.batch; base += kDecodeThreads) {
+        const int b = base + static_cast<int>(threadIdx.x);
+        if (a.batch > kDecodeThreads) seen = b < a.batch ? seen_of(a, b) : 0;
+        const int parts = b < a.batch ? parts_of(span_of<kTile>(a, seen).tiles, each) : 0;
+        const int inclusive = wave_scan_int(parts);
         __syncthreads();
         if (lane == 63) sums[wave] = inclusive;
-        if (threadIdx.x == 0) first_index = kDecodeThreads;
         __syncthreads();
-        int before = 0;
-        for (int w = 0; w < wave; ++w) before += sums[w];
-        const int begin = before + inclusive - mine;
-        prefix[threadIdx.x] = begin;
-        if (threadIdx.x == kDecodeThreads - 1) prefix[kDecodeThreads] = begin + mine;
-        if (mine > 0 && running + begin + mine > lo && running + begin <= lo) first_index = threadIdx.x;
-        if (mine > 0 && begin == 0 && running > lo) first_index = threadIdx.x;
-        __syncthreads();
-        const int round_total = prefix[kDecodeThreads];
+        int64_t begin = running + inclusive - parts;
+        for (int w = 0; w < wave; ++w) begin += sums[w];
+        running += static_cast<int64_t>(sums[0]) + sums[1] + sums[2] + sums[3];
+        if (blockIdx.x >= begin && blockIdx.x < begin + parts) {
+            chosen[0] = b;
+            chosen[1] = seen;
+            chosen[2] = static_cast<int>(blockIdx.x - begin);
+            chosen[3] = parts;
+        }
+        if (running > blockIdx.x) break;
+    }
+    if (running <= blockIdx.x) return;
+    __syncthreads();
+    const int b = chosen[0], part = chosen[2], parts = chosen[3];
+    const Span span = span_of<kTile>(a, chosen[1]);
+    const int from = part_begin(span.tiles, parts, part), to = part_begin(span.tiles, parts, part + 1);
+    const int64_t slot = kPaged && a.slots ? a.slots[b] : b;
+    const int32_t* row = kPaged ? a.table + (span.tiles > 0 ? slot : 0) * a.table_stride : nullptr;
+    const T* keys = static_cast<const T*>(a.key) + kv_head * a.key_strides[1] + (kPaged ? 0 : b * a.key_strides[0]);
+    const T* values = static_cast<const T*>(a.value) + kv_head * a.value_strides[1] + (kPaged ? 0 : b * a.value_strides[0]);
 
-        for (int j = first_index; j < kDecodeThreads && running + prefix[j] < hi; ++j) {
-            const int tiles = prefix[j + 1] - prefix[j];
-            if (tiles == 0) continue;
-            const int b = base + j;
-            const int64_t begins = running + prefix[j];
-            const int from = static_cast<int>(lo > begins ? lo - begins : 0);
-            const int to = static_cast<int>(hi - begins < tiles ? hi - begins : tiles);
-            const Span span = span_of<kTile>(a, b);
-            const int64_t slot = a.slots ? a.slots[b] : b;
-            const int32_t* row = kPaged ? a.table + slot * a.table_stride : nullptr;
-            const T* keys = static_cast<const T*>(a.key) + kv_head * a.key_strides[1] + (kPaged ? 0 : b * a.key_strides[0]);
-            const T* values = static_cast<const T*>(a.value) + kv_head * a.value_strides[1] +
-                              (kPaged ? 0 : b * a.value_strides[0]);
-
-            // Right operand of S^T: this lane's query head, zero behind the last one.
-            typename M::Fragment query[kFragments];
-            {
-                const int64_t head = kv_head * static_cast<int64_t>(a.group) + column0 + n16;
-                const T* q = static_cast<const T*>(a.query) + b * a.query_strides[0] + head * a.query_strides[1];
+    // A tile's positions, and the page of this lane's key in it (-1: not attended).
+    auto tile_key = [&](int t) { return (t < span.sink_tiles ? t : span.first_tile + t - span.sink_tiles) * kTile; };
+    struct Pages {
+        int page[kSubs];
+    };
+    auto look_up = [&](int t, Pages& p) {
+        const int base = tile_key(t);
 #pragma unroll
-                for (int f = 0; f < kFragments; ++f)
-                    query[f] = M::load_query(q, a.query_strides[3], M::kKeyStep * f + M::kPer * g, a.dim, n16 < columns);
-            }
-
-            f32x4 out[kBlocks];
-#pragma unroll
-            for (int i = 0; i < kBlocks; ++i) out[i] = f32x4{0, 0, 0, 0};
-            float top = -INFINITY, weight = 0.0f;
-
-            for (int t = from + wave; t < to; t += kDecodeWaves) {
-                const int base_key = (t < span.sink_tiles ? t : span.first_tile + t - span.sink_tiles) * kTile;
-                typename M::Fragment key[kSubs][kFragments];
-                Value value[kSubs][4][kChunks];
-                int held[kSubs][4];  // page of this lane's value rows, -1: not attended
-#pragma unroll
-                for (int s = 0; s < kSubs; ++s) {
-                    const int position = base_key + 16 * s + n16;
-                    int page = position < span.seen && (position >= span.low || position < span.sinks) ? 0 : -1;
-                    uint32_t in_page = position;
-                    if constexpr (kPaged) {
-                        const uint32_t column = divide(position, a.page);
-                        in_page = position - column * a.page.divisor;
-                        if (page == 0) {
-                            page = row[column];
-                            if (page >= a.pages) page = -1;
-                        }
-                    }
-                    const T* k = keys + (kPaged ? page * a.key_strides[0] : 0) + in_page * a.key_strides[2];
-#pragma unroll
-                    for (int f = 0; f < kFragments; ++f)
-                        key[s][f] = M::template load_row<kWide>(k, M::kKeyStep * f + M::kPer * g, a.dim, page >= 0);
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        held[s][i] = __shfl(page, 4 * g + i, kWave);
-                        const uint32_t value_position = base_key + 16 * s + 4 * g + i;
-                        uint32_t value_row = value_position;
-                        if constexpr (kPaged) value_row -= divide(value_position, a.page) * a.page.divisor;
-                        const T* v = values + (kPaged ? held[s][i] * a.value_strides[0] : 0) + value_row * a.value_strides[2];
-#pragma unroll
-                        for (int c = 0; c < kChunks; ++c)
-                            value[s][i][c] = M::template load_value<kDim, kWide>(v, c, n16, a.dim, held[s][i] >= 0);
-                    }
-                }
-
-                f32x4 score[kSubs];
-                float highest = -INFINITY;
-#pragma unroll
-                for (int s = 0; s < kSubs; ++s) {
-                    score[s] = f32x4{0, 0, 0, 0};
-#pragma unroll
-                    for (int f = 0; f < kFragments; ++f) M::multiply_key(key[s][f], query[f], score[s]);
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        score[s][i] = held[s][i] >= 0 ? score[s][i] * a.scale : -INFINITY;
-                        highest = fmaxf(highest, score[s][i]);
-                    }
-                }
-                highest = fmaxf(highest, __shfl_xor(highest, 16, kWave));
-                highest = fmaxf(highest, __shfl_xor(highest, 32, kWave));
-                if (__any(highest > top)) {
-                    const float now = fmaxf(top, highest);
-                    const float shrink = top == -INFINITY ? 0.0f : fast_exp2((top - now) * kLog2e);
-                    top = now;
-                    weight *= shrink;
-#pragma unroll
-                    for (int i = 0; i < kBlocks; ++i) out[i] *= shrink;
-                }
-                const float reference = top == -INFINITY ? 0.0f : top;
-                float p[kSubs][4];
-#pragma unroll
-                for (int s = 0; s < kSubs; ++s)
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        p[s][i] = fast_exp2((score[s][i] - reference) * kLog2e + M::kWeightShift);
-                        weight += p[s][i];
-                    }
-                M::template multiply_value<kDim, kSubs>(value, p, out);
-            }
-            weight += __shfl_xor(weight, 16, kWave);
-            weight += __shfl_xor(weight, 32, kWave);
-
-            // Join the four waves in registers: 2 and 3 into 0 and 1, then 1 into 0.
-#pragma unroll
-            for (int half = kDecodeWaves / 2; half >= 1; half /= 2) {
-                __syncthreads();
-                if (wave >= half && wave < 2 * half) {
-                    float(*to_merge)[kWave] = merge[wave - half];
-#pragma unroll
-                    for (int i = 0; i < kBlocks * 4; ++i) to_merge[i][lane] = out[i / 4][i % 4];
-                    to_merge[kBlocks * 4][lane] = top;
-                    to_merge[kBlocks * 4 + 1][lane] = weight;
-                }
-                __syncthreads();
-                if (wave < half) {
-                    const float(*other)[kWave] = merge[wave];
-                    const float other_top = other[kBlocks * 4][lane];
-                    const float now = fmaxf(top, other_top);
-                    const float mine_scale = top == -INFINITY ? 0.0f : fast_exp2((top - now) * kLog2e);
-                    const float other_scale = other_top == -INFINITY ? 0.0f : fast_exp2((other_top - now) * kLog2e);
-                    top = now;
-                    weight = weight * mine_scale + other[kBlocks * 4 + 1][lane] * other_scale;
-#pragma unroll
-                    for (int i = 0; i < kBlocks * 4; ++i)
-                        out[i / 4][i % 4] = out[i / 4][i % 4] * mine_scale + other[i][lane] * other_scale;
-                }
-            }
-
-            if (wave == 0 && n16 < columns) {
-                const bool whole = from == 0 && to == tiles;
-                const int64_t head = kv_head * static_cast<int64_t>(a.group) + column0 + n16;
-                if (whole) {
-                    T* o = static_cast<T*>(a.out) + (b * static_cast<int64_t>(a.query_heads) + head) * a.dim;
-                    M::template each_dim<kDim>(g, a.dim, [&](int i, int r, int d) {
-                        o[d] = static_cast<T>(weight == 0.0f ? 0.0f : out[i][r] / weight);
-                    });
-                } else {
-                    float* o = a.workspace + partial_offset(a, blockIdx.y, part, from == 0 ? 1 : 0, n16);
-                    M::template each_dim<kDim>(g, a.dim, [&](int i, int r, int d) { o[d] = out[i][r]; });
-                    if (g == 0) {
-                        o[a.dim] = top;
-                        o[a.dim + 1] = weight;
-                    }
-                }
+        for (int s = 0; s < kSubs; ++s) {
+            const int position = base + 16 * s + n16;
+            p.page[s] = t < to && position < span.seen && (position >= span.low || position < span.sinks) ? 0 : -1;
+            if constexpr (kPaged) {
+                if (p.page[s] == 0) p.page[s] = row[divide(position, a.page)];
             }
         }
-        running += round_total;
+    };
+    struct Tile {
+        typename M::Fragment key[kSubs][kFragments];
+        Value value[kSubs][4][kChunks];
+        int held[kSubs][4];
+    };
+    auto load = [&](int t, const Pages& p, Tile& tile) {
+        const int base = tile_key(t);
+#pragma unroll
+        for (int s = 0; s < kSubs; ++s) {
+            int page = p.page[s];
+            if constexpr (kPaged) page = page < a.pages ? page : -1;
+            const int position = base + 16 * s + n16;
+            const uint32_t in_page = kPaged ? position - divide(position, a.page) * a.page.divisor : position;
+            const T* k = keys + (kPaged ? page * a.key_strides[0] : 0) + in_page * a.key_strides[2];
+#pragma unroll
+            for (int f = 0; f < kFragments; ++f)
+                tile.key[s][f] = M::template load_row<kWide>(k, M::kKeyStep * f + M::kPer * g, a.dim, page >= 0);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const int of = __shfl(page, 4 * g + i, kWave);
+                tile.held[s][i] = of;
+                const uint32_t value_position = base + 16 * s + 4 * g + i;
+                const uint32_t value_row = kPaged ? value_position - divide(value_position, a.page) * a.page.divisor : value_position;
+                const T* v = values + (kPaged ? of * a.value_strides[0] : 0) + value_row * a.value_strides[2];
+#pragma unroll
+                for (int c = 0; c < kChunks; ++c)
+                    tile.value[s][i][c] = M::template load_value<kDim, kWide>(v, c, n16, a.dim, of >= 0);
+            }
+        }
+    };
+
+    f32x4 out[kBlocks];
+#pragma unroll
+    for (int i = 0; i < kBlocks; ++i) out[i] = f32x4{0, 0, 0, 0};
+    float top = -INFINITY, weight = 0.0f;
+    typename M::Fragment query[kFragments];  // right operand of S^T: this lane's query head, zero behind the last one
+
+    auto work = [&](const Tile& tile) {
+        f32x4 score[kSubs];
+        float highest = -INFINITY;
+#pragma unroll
+        for (int s = 0; s < kSubs; ++s) {
+            score[s] = f32x4{0, 0, 0, 0};
+#pragma unroll
+            for (int f = 0; f < kFragments; ++f) M::multiply_key(tile.key[s][f], query[f], score[s]);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                score[s][i] = tile.held[s][i] >= 0 ? score[s][i] * a.scale : -INFINITY;
+                highest = fmaxf(highest, score[s][i]);
+            }
+        }
+        highest = fmaxf(highest, __shfl_xor(highest, 16, kWave));
+        highest = fmaxf(highest, __shfl_xor(highest, 32, kWave));
+        if (__any(highest > top)) {
+            const float now = fmaxf(top, highest);
+            const float shrink = top == -INFINITY ? 0.0f : fast_exp2((top - now) * kLog2e);
+            top = now;
+            weight *= shrink;
+#pragma unroll
+            for (int i = 0; i < kBlocks; ++i) out[i] *= shrink;
+        }
+        const float reference = top == -INFINITY ? 0.0f : top;
+        float p[kSubs][4];
+#pragma unroll
+        for (int s = 0; s < kSubs; ++s)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                p[s][i] = fast_exp2((score[s][i] - reference) * kLog2e + M::kWeightShift);
+                weight += p[s][i];
+            }
+        M::template multiply_value<kDim, kSubs>(tile.value, p, out);
+    };
+
+    // Two tiles in registers where two waves per SIMD still fit: the next one's rows arrive while one is worked on (48
+    // sequences of 2 to 16k keys, 8 KV heads of 128 in bfloat16: 406 us; one tile: 417; two tiles and one wave: 511).
+    constexpr bool kAhead = kDim * static_cast<int>(sizeof(T)) <= 256;
+    Pages pages;
+    Tile even;
+    look_up(from + wave, pages);
+    {
+        const int64_t head = kv_head * static_cast<int64_t>(a.group) + column0 + n16;
+        const T* q = static_cast<const T*>(a.query) + b * a.query_strides[0] + head * a.query_strides[1];
+#pragma unroll
+        for (int f = 0; f < kFragments; ++f) {
+            const int d = M::kKeyStep * f + M::kPer * g;
+            if (a.query_wide) query[f] = M::template load_row<true>(q, d, a.dim, n16 < columns);
+            else query[f] = M::load_query(q, a.query_strides[3], d, a.dim, n16 < columns);
+        }
+    }
+    if constexpr (kAhead) {
+        Tile odd;
+        load(from + wave, pages, even);
+        look_up(from + wave + kDecodeWaves, pages);
+        for (int t = from + wave; t < to; t += 2 * kDecodeWaves) {
+            load(t + kDecodeWaves, pages, odd);
+            look_up(t + 2 * kDecodeWaves, pages);
+            work(even);
+            if (t + kDecodeWaves >= to) break;
+            load(t + 2 * kDecodeWaves, pages, even);
+            look_up(t + 3 * kDecodeWaves, pages);
+            work(odd);
+        }
+    } else {
+        for (int t = from + wave; t < to; t += kDecodeWaves) {
+            load(t, pages, even);
+            look_up(t + kDecodeWaves, pages);
+            work(even);
+        }
+    }
+    weight += __shfl_xor(weight, 16, kWave);
+    weight += __shfl_xor(weight, 32, kWave);
+
+    // Join the four waves in registers: 2 and 3 into 0 and 1, then 1 into 0.
+#pragma unroll
+    for (int half = kDecodeWaves / 2; half >= 1; half /= 2) {
+        if (half == 1) __syncthreads();
+        if (wave >= half && wave < 2 * half) {
+            float(*to_merge)[kWave] = merge[wave - half];
+#pragma unroll
+            for (int i = 0; i < kBlocks * 4; ++i) to_merge[i][lane] = out[i / 4][i % 4];
+            to_merge[kBlocks * 4][lane] = top;
+            to_merge[kBlocks * 4 + 1][lane] = weight;
+        }
+        __syncthreads();
+        if (wave < half) {
+            const float(*other)[kWave] = merge[wave];
+            const float other_top = other[kBlocks * 4][lane];
+            const float now = fmaxf(top, other_top);
+            const float mine_scale = top == -INFINITY ? 0.0f : fast_exp2((top - now) * kLog2e);
+            const float other_scale = other_top == -INFINITY ? 0.0f : fast_exp2((other_top - now) * kLog2e);
+            top = now;
+            weight = weight * mine_scale + other[kBlocks * 4 + 1][lane] * other_scale;
+#pragma unroll
+            for (int i = 0; i < kBlocks * 4; ++i)
+                out[i / 4][i % 4] = out[i / 4][i % 4] * mine_scale + other[i][lane] * other_scale;
+        }
+    }
+    if (wave != 0 || n16 >= columns) return;
+    if (parts == 1) {
+        const int64_t head = kv_head * static_cast<int64_t>(a.group) + column0 + n16;
+        T* o = static_cast<T*>(a.out) + (b * static_cast<int64_t>(a.query_heads) + head) * a.dim;
+        M::template each_dim<kDim>(g, a.dim, [&](int i, int r, int d) {
+            o[d] = static_cast<T>(weight == 0.0f ? 0.0f : out[i][r] / weight);
+        });
+    } else {
+        float* o = a.workspace + partial_offset(a, blockIdx.y, blockIdx.x, n16);
+        M::template each_dim<kDim>(g, a.dim, [&](int i, int r, int d) { o[d] = out[i][r]; });
+        if (g == 0) {
+            o[a.dim] = top;
+            o[a.dim + 1] = weight;
+        }
     }
 }
 
-// Joins the parts of a sequence that was cut, or writes zeros for one that sees nothing.  Workgroup (sequence, head).
+// Joins the parts of a sequence that was cut.  Workgroup (sequence, column tile of a KV head): the parts' weights once,
+// then the threads go over the tile's heads and dims.
+constexpr int kJoinParts = 128;  // parts whose shares are kept
+
 template <class T, int kTile>
 __global__ void __launch_bounds__(kDecodeThreads) decode_join_kernel(AttentionArgs a) {
     __shared__ int sums[kDecodeWaves];
-    const int64_t b = blockIdx.x / a.query_heads;
-    const int head = blockIdx.x % a.query_heads;
-    int64_t total = 0, begins = 0;
+    __shared__ int mine_seen;
+    __shared__ float share[kJoinParts][kColumns];
+    __shared__ float tops[kColumns], weights[kColumns];
+    const int b = blockIdx.x;
+    int64_t total = 0;
+    int seen = 0;
     for (int base = 0; base < a.batch; base += kDecodeThreads) {
-        const int i = base + threadIdx.x;
-        const int tiles = i < a.batch ? span_of<kTile>(a, i).tiles : 0;
-        total += block_sum(tiles, sums);
-        begins += block_sum(i < b ? tiles : 0, sums);
+        const int i = base + static_cast<int>(threadIdx.x);
+        seen = i < a.batch ? seen_of(a, i) : 0;
+        if (i == b) mine_seen = seen;
+        total += block_sum(span_of<kTile>(a, seen).tiles, sums);
     }
-    const int tiles = span_of<kTile>(a, b).tiles;
-    T* out = static_cast<T*>(a.out) + (b * a.query_heads + head) * a.dim;
-    const int d = threadIdx.x;
-    if (tiles == 0) {
-        if (d < a.dim) out[d] = static_cast<T>(0.0f);
-        return;
+    const int each = part_tiles(total, a.blocks);
+    const int parts = parts_of(span_of<kTile>(a, mine_seen).tiles, each);
+    if (parts == 1) return;
+    int64_t first = 0;
+    for (int base = 0; base < b; base += kDecodeThreads) {
+        const int i = base + static_cast<int>(threadIdx.x);
+        if (a.batch > kDecodeThreads) seen = i < a.batch ? seen_of(a, i) : 0;
+        first += block_sum(i < b ? parts_of(span_of<kTile>(a, seen).tiles, each) : 0, sums);
     }
-    const int parts = parts_of(total, a.blocks);
-    const int first = part_of(total, parts, begins), last = part_of(total, parts, begins + tiles - 1);
-    if (first == last) return;
-    const int kv_head = head / a.group, in_group = head % a.group;
-    const int64_t head_tile = static_cast<int64_t>(kv_head) * ((a.group + kColumns - 1) / kColumns) + in_group / kColumns;
-    const int column = in_group % kColumns;
-    float top = -INFINITY;
-    for (int part = first; part <= last; ++part)
-        top = fmaxf(top, a.workspace[partial_offset(a, head_tile, part, part == first ? 1 : 0, column) + a.dim]);
-    float weight = 0.0f, sum = 0.0f;
-    for (int part = first; part <= last; ++part) {
-        const float* o = a.workspace + partial_offset(a, head_tile, part, part == first ? 1 : 0, column);
-        const float share = o[a.dim] == -INFINITY ? 0.0f : fast_exp2((o[a.dim] - top) * kLog2e);
-        weight += o[a.dim + 1] * share;
-        if (d < a.dim) sum += o[d] * share;
+    const int column_tiles = (a.group + kColumns - 1) / kColumns;
+    const int column0 = blockIdx.y % column_tiles * kColumns;
+    const int columns = a.group - column0 < kColumns ? a.group - column0 : kColumns;
+    const int64_t stride = partial_offset(a, 0, 1, 0);
+    const float* o = a.workspace + partial_offset(a, blockIdx.y, first, 0);
+    const int width = a.dim + 2;
+
+    // Sixteen lanes go over the parts of one head: its maximum, the parts' shares (kept where there is room), their sum.
+    {
+        const int column = threadIdx.x / 16, lane = threadIdx.x % 16;
+        const float* mine = o + column * width + a.dim;
+        float top = -INFINITY, weight = 0.0f;
+        if (column < columns) {
+#pragma unroll 4
+            for (int p = lane; p < parts; p += 16) {
+                const float part_top = mine[p * stride], part_weight = mine[p * stride + 1];
+                if (p < kJoinParts) share[p][column] = part_top;
+                const float now = fmaxf(top, part_top);
+                const float kept = top == -INFINITY ? 0.0f : fast_exp2((top - now) * kLog2e);
+                const float added = part_top == -INFINITY ? 0.0f : fast_exp2((part_top - now) * kLog2e);
+                weight = weight * kept + part_weight * added;
+                top = now;
+            }
+        }
+        const float all = row16_max(top);
+        weight = row16_sum(weight * (top == -INFINITY ? 0.0f : fast_exp2((top - all) * kLog2e)));
+        if (column < columns)
+            for (int p = lane; p < parts && p < kJoinParts; p += 16)
+                share[p][column] = share[p][column] == -INFINITY ? 0.0f : fast_exp2((share[p][column] - all) * kLog2e);
+        if (lane == 0) {
+            tops[column] = all;
+            weights[column] = weight;
+        }
     }
-    if (d < a.dim) out[d] = static_cast<T>(weight == 0.0f ? 0.0f : sum / weight);
+    const int64_t head = static_cast<int64_t>(blockIdx.y / column_tiles) * a.group + column0;
+    T* out = static_cast<T*>(a.out) + (b * static_cast<int64_t>(a.query_heads) + head) * a.dim;
+    const int items = columns * a.dim;
+    __syncthreads();
+    for (int item = threadIdx.x; item < items; item += kDecodeThreads) {
+        const int column = item / a.dim, d = item - column * a.dim;
+        const float* from = o + column * width + d;
+        float sum = 0.0f;
+        const int kept = parts < kJoinParts ? parts : kJoinParts;
+#pragma unroll 8
+        for (int p = 0; p < kept; ++p) sum += from[p * stride] * share[p][column];
+        for (int p = kept; p < parts; ++p) {
+            const float part_top = from[p * stride + a.dim - d];
+            sum += from[p * stride] * (part_top == -INFINITY ? 0.0f : fast_exp2((part_top - tops[column]) * kLog2e));
+        }
+        out[item] = static_cast<T>(weights[column] == 0.0f ? 0.0f : sum / weights[column]);
+    }
 }
 
-constexpr int tile_of(int dim, int bytes) { return dim * bytes <= 256 ? 32 : 16; }
 constexpr int padded_dim(int dim) { return dim <= 64 ? 64 : (dim <= 128 ? 128 : 256); }
 
 template <class T, int kDim>
 hipError_t launch_decode(const AttentionArgs& a, hipStream_t stream) {
     const int column_tiles = (a.group + kColumns - 1) / kColumns;
-    const dim3 grid(a.blocks, a.kv_heads * column_tiles);
+    const dim3 grid(a.blocks + a.batch, a.kv_heads * column_tiles);
     if (a.pages > 0) {
         if (a.wide) hipLaunchKernelGGL(HIP_KERNEL_NAME(decode_attention_kernel<T, kDim, true, true>), grid, dim3(kDecodeThreads), 0, stream, a);
         else hipLaunchKernelGGL(HIP_KERNEL_NAME(decode_attention_kernel<T, kDim, true, false>), grid, dim3(kDecodeThreads), 0, stream, a);
@@ -337,7 +411,8 @@ hipError_t launch_decode(const AttentionArgs& a, hipStream_t stream) {
     }
     const hipError_t launched = hipGetLastError();
     if (launched != hipSuccess) return launched;
-    hipLaunchKernelGGL(HIP_KERNEL_NAME(decode_join_kernel<T, tile_of(kDim, sizeof(T))>), dim3(a.batch * a.query_heads),
+    if (a.keys <= kLeastTiles * tile_of(kDim, sizeof(T))) return hipSuccess;  // no sequence is cut
+    hipLaunchKernelGGL(HIP_KERNEL_NAME(decode_join_kernel<T, tile_of(kDim, sizeof(T))>), dim3(a.batch, a.kv_heads * column_tiles),
                        dim3(kDecodeThreads), 0, stream, a);
     return hipGetLastError();
 }
@@ -353,13 +428,15 @@ hipError_t launch_decode_dim(const AttentionArgs& a, hipStream_t stream) {
 
 }  // namespace
 
-// Two workgroups per CU of the 256, and none without kLeastTiles tiles of 16 keys.
+// Parts that the batch is cut into: two workgroups on each of 256 CUs, less one per sequence, whose last part may be short;
+// none without kLeastTiles tiles of 16 keys.
 int decode_attention_blocks(int batch, int64_t keys, int kv_heads, int group, int window, int sinks) {
     int64_t seen = keys;
     if (window > 0 && static_cast<int64_t>(window) + sinks + 32 < keys) seen = static_cast<int64_t>(window) + sinks + 32;
     const int64_t most = (batch * ((seen + 15) / 16 + 2) + kLeastTiles - 1) / kLeastTiles;
     const int64_t heads = static_cast<int64_t>(kv_heads) * ((group + kColumns - 1) / kColumns);
     int64_t blocks = (512 + heads - 1) / heads;
+    blocks = blocks - batch > blocks / 2 ? blocks - batch : (blocks + 1) / 2;
     if (blocks > most) blocks = most;
     return static_cast<int>(blocks < 1 ? 1 : blocks);
 }
@@ -367,7 +444,7 @@ int decode_attention_blocks(int batch, int64_t keys, int kv_heads, int group, in
 size_t decode_attention_workspace_floats(const AttentionArgs& a) {
     const size_t columns = a.group < kColumns ? a.group : kColumns;
     const size_t heads = static_cast<size_t>(a.kv_heads) * ((a.group + kColumns - 1) / kColumns);
-    return heads * a.blocks * 2 * columns * (a.dim + 2);
+    return heads * (a.blocks + a.batch) * columns * (a.dim + 2);
 }
 
 hipError_t launch_decode_attention(const AttentionArgs& args, Type type, hipStream_t stream) {

@@ -15,12 +15,13 @@ a leading layer dimension for the operators that move pages, and the books that 
 from __future__ import annotations
 
 import ctypes
+import functools
 
 import torch
 
 from flux_amd import _native
-from flux_amd.ops.native import (_LIBRARY, _aliases, _availability, _call, _check, _cpu_kernel, _finite_fp32, _grad_free,
-                                 _on, _require_gpu, _require_library, _stream)
+from flux_amd.ops.native import (_LIBRARY, _aliases, _availability, _check, _cpu_kernel, _finite_fp32, _grad_free, _on,
+                                 _require_gpu, _require_library, _stream)
 
 PAGE_DONE, PAGE_OUT_OF_RANGE, PAGE_REPEATED, PAGE_NO_ROOM, PAGE_OCCUPIED = range(5)
 
@@ -59,91 +60,110 @@ for _schema in SERVING_SCHEMAS.values():
     _LIBRARY.define(_schema)
 
 _FOUR = ctypes.c_int64 * 4
-_THREE = ctypes.c_int64 * 3
 
+
+# Checks are a large part of a small call's time: shapes are read once, messages are whole literals, sizes that only
+# depend on shapes come from small caches.
 
 def _address(tensor):
     return None if tensor is None else tensor.data_ptr()
 
 
-def _check_list(tensor, dtype, like, message: str) -> None:
-    """A contiguous vector of ``dtype`` on the device of ``like``."""
-    _check(tensor.dim() == 1 and tensor.dtype == dtype and tensor.device == like.device and tensor.is_contiguous(),
-           message)
+def _check_list(tensor, dtype, device, message: str, length=None, length_message: str = "") -> None:
+    """A contiguous vector of ``dtype`` (and ``length``) on ``device``."""
+    shape = tensor.shape
+    _check(len(shape) == 1 and tensor.dtype is dtype and tensor.device == device and tensor.is_contiguous(), message)
+    if length is not None:
+        _check(shape[0] == length, length_message)
 
 
-def _check_window(window, sinks, message: str) -> None:
-    _check(0 <= window <= _MAX_KEYS and 0 <= sinks <= _MAX_KEYS, message)
+def _call(function: str, *args) -> None:
+    status = getattr(_native._lib or _native.load(), function)(*args)
+    if status:
+        _native.check(status)
+
+
+def _ready(what: str) -> None:
+    if _native._lib is None:
+        _require_library(what)
+
+
+@functools.lru_cache(maxsize=1024)
+def _size_from(function: str, *sizes) -> int:
+    """A workspace size of the C ABI, a function of shapes alone."""
+    value = ctypes.c_int64(0)
+    _call(function, *sizes, ctypes.byref(value))
+    return value.value
 
 
 # ---------------------------------------------------------------------------
 # paged_decode_attention
 
 def _validate_paged(query, key_pages, value_pages, page_table, lengths, scale, window=0, sinks=0, slots=None) -> None:
-    _check(query.dim() == 4 and key_pages.dim() == 4 and value_pages.dim() == 4,
+    shape, pages, table, dtype, device = query.shape, key_pages.shape, page_table.shape, query.dtype, query.device
+    _check(len(shape) == 4 and len(pages) == 4 and value_pages.dim() == 4,
            "flux::paged_decode_attention: query and pages must be rank four")
-    _check(query.dtype in _TYPES and key_pages.dtype == query.dtype and value_pages.dtype == query.dtype,
+    _check(dtype in _TYPES and key_pages.dtype is dtype and value_pages.dtype is dtype,
            "flux::paged_decode_attention: query and pages must share dtype float32, float16 or bfloat16")
-    _check(query.shape[2] == 1, "flux::paged_decode_attention: query length must be one")
-    _check(key_pages.shape == value_pages.shape, "flux::paged_decode_attention: key and value page shapes must match")
-    _check(all(s > 0 for s in query.shape) and all(s > 0 for s in key_pages.shape),
-           "flux::paged_decode_attention: tensor dimensions must be non-empty")
-    _check(query.shape[3] == key_pages.shape[3] and query.shape[3] <= _MAX_DIM,
+    _check(shape[2] == 1, "flux::paged_decode_attention: query length must be one")
+    _check(pages == value_pages.shape, "flux::paged_decode_attention: key and value page shapes must match")
+    _check(0 not in shape and 0 not in pages, "flux::paged_decode_attention: tensor dimensions must be non-empty")
+    _check(shape[3] == pages[3] and shape[3] <= _MAX_DIM,
            "flux::paged_decode_attention: head dimensions must match and be at most 256")
-    _check(query.shape[1] % key_pages.shape[1] == 0,
-           "flux::paged_decode_attention: query heads must be divisible by KV heads")
-    _check(page_table.dim() == 2 and page_table.dtype == torch.int32 and page_table.shape[1] > 0,
+    _check(shape[1] % pages[1] == 0, "flux::paged_decode_attention: query heads must be divisible by KV heads")
+    _check(len(table) == 2 and page_table.dtype is torch.int32 and table[1] > 0,
            "flux::paged_decode_attention: page_table must be int32 [slots, columns]")
-    _check(page_table.stride(1) == 1 or page_table.shape[1] == 1,
+    _check(page_table.stride(1) == 1 or table[1] == 1,
            "flux::paged_decode_attention: page_table rows must be contiguous")
-    _check(page_table.shape[1] * key_pages.shape[2] <= _MAX_KEYS,
+    _check(table[1] * pages[2] <= _MAX_KEYS,
            "flux::paged_decode_attention: page_table holds more than 16777216 positions a row")
-    _check_list(lengths, torch.int64, query,
-                "flux::paged_decode_attention: lengths must be a contiguous int64 vector on the query device")
-    _check(lengths.shape[0] == page_table.shape[0],
-           "flux::paged_decode_attention: lengths must have one entry per page_table row")
+    _check_list(lengths, torch.int64, device,
+                "flux::paged_decode_attention: lengths must be a contiguous int64 vector on the query device",
+                table[0], "flux::paged_decode_attention: lengths must have one entry per page_table row")
     if slots is None:
-        _check(page_table.shape[0] == query.shape[0],
+        _check(table[0] == shape[0],
                "flux::paged_decode_attention: without slots page_table must have one row per sequence")
     else:
-        _check_list(slots, torch.int64, query,
-                    "flux::paged_decode_attention: slots must be a contiguous int64 vector on the query device")
-        _check(slots.shape[0] == query.shape[0], "flux::paged_decode_attention: slots must have one entry per sequence")
-    _check(key_pages.device == query.device and value_pages.device == query.device and
-           page_table.device == query.device, "flux::paged_decode_attention: tensor devices must match")
-    _check(key_pages.stride(3) == 1 and value_pages.stride(3) == 1 or key_pages.shape[3] == 1,
+        _check_list(slots, torch.int64, device,
+                    "flux::paged_decode_attention: slots must be a contiguous int64 vector on the query device",
+                    shape[0], "flux::paged_decode_attention: slots must have one entry per sequence")
+    _check(key_pages.device == device and value_pages.device == device and page_table.device == device,
+           "flux::paged_decode_attention: tensor devices must match")
+    _check(key_pages.stride(3) == 1 and value_pages.stride(3) == 1 or pages[3] == 1,
            "flux::paged_decode_attention: pages must have unit stride along the head dimension")
-    _check_window(window, sinks, "flux::paged_decode_attention: window and sinks must be within [0, 16777216]")
+    _check(0 <= window <= _MAX_KEYS and 0 <= sinks <= _MAX_KEYS,
+           "flux::paged_decode_attention: window and sinks must be within [0, 16777216]")
     _check(_finite_fp32(scale), "flux::paged_decode_attention: scale must be a finite FP32 value")
-    _grad_free("flux::paged_decode_attention", query, key_pages, value_pages)
+    if torch.is_grad_enabled():
+        _grad_free("flux::paged_decode_attention", query, key_pages, value_pages)
 
 
 def paged_decode_workspace_bytes(query: torch.Tensor, key_pages: torch.Tensor, page_table: torch.Tensor, window: int = 0,
                                  sinks: int = 0) -> int:
     """Device workspace (bytes) that flux::paged_decode_attention needs for these shapes."""
-    value = ctypes.c_int64(0)
-    _call("flux_paged_decode_attention_workspace_bytes", query.shape[0], query.shape[1], key_pages.shape[1],
-          query.shape[3], page_table.shape[1] * key_pages.shape[2], window, sinks, ctypes.byref(value))
-    return value.value
+    shape, pages = query.shape, key_pages.shape
+    return _size_from("flux_paged_decode_attention_workspace_bytes", shape[0], shape[1], pages[1], shape[3],
+                      page_table.shape[1] * pages[2], window, sinks)
 
 
 def _launch_paged(query, key_pages, value_pages, page_table, lengths, scale, window, sinks, slots, output, workspace):
     batch, heads, _, dim = query.shape
     pages, kv_heads, page_size, _ = key_pages.shape
+    slot_count, columns = page_table.shape
     with _on(query.device):
         _call("flux_paged_decode_attention", _TYPES[query.dtype], query.data_ptr(), key_pages.data_ptr(),
               value_pages.data_ptr(), page_table.data_ptr(), lengths.data_ptr(), _address(slots), output.data_ptr(),
               workspace.data_ptr(), workspace.numel() * 4, scale, batch, heads, kv_heads, dim, pages, page_size,
-              page_table.shape[0], page_table.shape[1], page_table.stride(0), window, sinks, _FOUR(*query.stride()),
-              _THREE(*key_pages.stride()[:3]), _THREE(*value_pages.stride()[:3]), _stream(query))
+              slot_count, columns, page_table.stride(0), window, sinks, _FOUR(*query.stride()),
+              _FOUR(*key_pages.stride()), _FOUR(*value_pages.stride()), _stream(query))
 
 
 def _paged_cuda(query, key_pages, value_pages, page_table, lengths, scale, window=0, sinks=0, slots=None):
     _validate_paged(query, key_pages, value_pages, page_table, lengths, scale, window, sinks, slots)
-    _require_gpu("flux::paged_decode_attention", query)
-    output = torch.empty(query.shape, dtype=query.dtype, device=query.device)
-    needed = paged_decode_workspace_bytes(query, key_pages, page_table, window, sinks)
-    workspace = torch.empty(needed // 4, dtype=torch.float32, device=query.device)
+    _check(query.is_cuda, "flux::paged_decode_attention: CUDA dispatch requires CUDA tensors")
+    output = query.new_empty(query.shape)
+    workspace = torch.empty(paged_decode_workspace_bytes(query, key_pages, page_table, window, sinks) // 4,
+                            dtype=torch.float32, device=query.device)
     _launch_paged(query, key_pages, value_pages, page_table, lengths, scale, window, sinks, slots, output, workspace)
     return output
 
@@ -176,99 +196,116 @@ def _paged_out_cuda(query, key_pages, value_pages, page_table, lengths, scale, w
 # window_attention
 
 def _validate_window(query, key, value, scale, window, sinks=0, lengths=None, starts=None) -> None:
-    _check(query.dim() == 4 and key.dim() == 4 and value.dim() == 4,
+    shape, keys, dtype, device = query.shape, key.shape, query.dtype, query.device
+    _check(len(shape) == 4 and len(keys) == 4 and value.dim() == 4,
            "flux::window_attention: query, key and value must be rank four")
-    _check(query.dtype in _TYPES and key.dtype == query.dtype and value.dtype == query.dtype,
+    _check(dtype in _TYPES and key.dtype is dtype and value.dtype is dtype,
            "flux::window_attention: query, key and value must share dtype float32, float16 or bfloat16")
-    _check(key.shape == value.shape, "flux::window_attention: key and value shapes must match")
-    _check(all(s > 0 for s in query.shape) and all(s > 0 for s in key.shape),
-           "flux::window_attention: tensor dimensions must be non-empty")
-    _check(query.shape[0] == key.shape[0], "flux::window_attention: batch sizes must match")
-    _check(query.shape[3] == key.shape[3] and query.shape[3] <= _MAX_DIM,
+    _check(keys == value.shape, "flux::window_attention: key and value shapes must match")
+    _check(0 not in shape and 0 not in keys, "flux::window_attention: tensor dimensions must be non-empty")
+    _check(shape[0] == keys[0], "flux::window_attention: batch sizes must match")
+    _check(shape[3] == keys[3] and shape[3] <= _MAX_DIM,
            "flux::window_attention: head dimensions must match and be at most 256")
-    _check(query.shape[1] % key.shape[1] == 0, "flux::window_attention: query heads must be divisible by KV heads")
-    _check(key.shape[2] <= _MAX_KEYS, "flux::window_attention: more than 16777216 keys")
-    _check(key.device == query.device and value.device == query.device,
-           "flux::window_attention: tensor devices must match")
-    _check(key.stride(3) == 1 and value.stride(3) == 1 or key.shape[3] == 1,
+    _check(shape[1] % keys[1] == 0, "flux::window_attention: query heads must be divisible by KV heads")
+    _check(keys[2] <= _MAX_KEYS, "flux::window_attention: more than 16777216 keys")
+    _check(key.device == device and value.device == device, "flux::window_attention: tensor devices must match")
+    _check(key.stride(3) == 1 and value.stride(3) == 1 or keys[3] == 1,
            "flux::window_attention: key and value must have unit stride along the head dimension")
     if lengths is not None:
-        _check_list(lengths, torch.int64, query,
-                    "flux::window_attention: lengths must be a contiguous int64 vector on the query device")
-        _check(lengths.shape[0] == query.shape[0], "flux::window_attention: lengths must have one entry per sequence")
+        _check_list(lengths, torch.int64, device,
+                    "flux::window_attention: lengths must be a contiguous int64 vector on the query device",
+                    shape[0], "flux::window_attention: lengths must have one entry per sequence")
     if starts is not None:
-        _check_list(starts, torch.int64, query,
-                    "flux::window_attention: starts must be a contiguous int64 vector on the query device")
-        _check(starts.shape[0] == query.shape[0], "flux::window_attention: starts must have one entry per sequence")
-    _check_window(window, sinks, "flux::window_attention: window and sinks must be within [0, 16777216]")
+        _check_list(starts, torch.int64, device,
+                    "flux::window_attention: starts must be a contiguous int64 vector on the query device",
+                    shape[0], "flux::window_attention: starts must have one entry per sequence")
+    _check(0 <= window <= _MAX_KEYS and 0 <= sinks <= _MAX_KEYS,
+           "flux::window_attention: window and sinks must be within [0, 16777216]")
     _check(_finite_fp32(scale), "flux::window_attention: scale must be a finite FP32 value")
-    _grad_free("flux::window_attention", query, key, value)
+    if torch.is_grad_enabled():
+        _grad_free("flux::window_attention", query, key, value)
 
 
 def _window_cuda(query, key, value, scale, window, sinks=0, lengths=None, starts=None):
     _validate_window(query, key, value, scale, window, sinks, lengths, starts)
-    _require_gpu("flux::window_attention", query)
+    _check(query.is_cuda, "flux::window_attention: CUDA dispatch requires CUDA tensors")
     batch, heads, queries, dim = query.shape
     kv_heads, keys = key.shape[1], key.shape[2]
     output = torch.empty(query.shape, dtype=query.dtype, device=query.device)
-    needed = ctypes.c_int64(0)
+    needed, workspace = 0, None
     if queries == 1:
-        _call("flux_window_attention_workspace_bytes", batch, heads, kv_heads, queries, dim, keys, window, sinks,
-              ctypes.byref(needed))
-    workspace = torch.empty(needed.value // 4, dtype=torch.float32, device=query.device) if needed.value else None
+        needed = _size_from("flux_window_attention_workspace_bytes", batch, heads, kv_heads, 1, dim, keys, window, sinks)
+        workspace = torch.empty(needed // 4, dtype=torch.float32, device=query.device)
     with _on(query.device):
         _call("flux_window_attention", _TYPES[query.dtype], query.data_ptr(), key.data_ptr(), value.data_ptr(),
-              _address(lengths), _address(starts), output.data_ptr(), _address(workspace), needed.value, scale, batch,
-              heads, kv_heads, queries, keys, dim, window, sinks, _FOUR(*query.stride()), _THREE(*key.stride()[:3]),
-              _THREE(*value.stride()[:3]), _stream(query))
+              _address(lengths), _address(starts), output.data_ptr(), _address(workspace), needed, scale, batch,
+              heads, kv_heads, queries, keys, dim, window, sinks, _FOUR(*query.stride()), _FOUR(*key.stride()),
+              _FOUR(*value.stride()), _stream(query))
     return output
 
 
 # ---------------------------------------------------------------------------
 # Pages.
 
-def _check_written(tensor, message: str) -> None:
-    """A tensor that is written: no two of its elements share memory by a stride of zero."""
-    _check(all(stride > 0 or size == 1 for size, stride in zip(tensor.shape, tensor.stride())), message)
+def _written_once(shape, stride) -> bool:
+    """No two elements of a tensor that is written share memory by a stride of zero."""
+    if 0 not in stride:
+        return True
+    return all(step > 0 or size == 1 for size, step in zip(shape, stride))
 
 
 def _validate_pools(op, key_pages, value_pages, ranks=(4, 5)) -> None:
-    _check(key_pages.dim() in ranks and value_pages.dim() == key_pages.dim(),
-           f"{op}: key_pages and value_pages must be [pages, kv_heads, page_size, head_dim]" +
-           (", or that behind a layer dimension" if 5 in ranks else ""))
-    _check(key_pages.dtype in _TYPES and value_pages.dtype == key_pages.dtype,
-           f"{op}: pages must share dtype float32, float16 or bfloat16")
-    _check(key_pages.shape == value_pages.shape, f"{op}: key and value page shapes must match")
-    _check(all(s > 0 for s in key_pages.shape), f"{op}: pages must be non-empty")
-    _check(key_pages.device == value_pages.device, f"{op}: tensor devices must match")
-    _check(key_pages.stride(-1) == 1 and value_pages.stride(-1) == 1 or key_pages.shape[-1] == 1,
-           f"{op}: pages must have unit stride along the head dimension")
-    _check_written(key_pages, f"{op}: key_pages must not overlap itself")
-    _check_written(value_pages, f"{op}: value_pages must not overlap itself")
-    _grad_free(op, key_pages, value_pages)
+    shape, dtype, key_stride, value_stride = key_pages.shape, key_pages.dtype, key_pages.stride(), value_pages.stride()
+    if len(shape) not in ranks or len(value_stride) != len(shape):
+        _check(False, f"{op}: key_pages and value_pages must be [pages, kv_heads, page_size, head_dim]" +
+               (", or that behind a layer dimension" if 5 in ranks else ""))
+    if dtype not in _TYPES or value_pages.dtype is not dtype:
+        _check(False, f"{op}: pages must share dtype float32, float16 or bfloat16")
+    if shape != value_pages.shape:
+        _check(False, f"{op}: key and value page shapes must match")
+    if 0 in shape:
+        _check(False, f"{op}: pages must be non-empty")
+    if key_pages.device != value_pages.device:
+        _check(False, f"{op}: tensor devices must match")
+    if (key_stride[-1] != 1 or value_stride[-1] != 1) and shape[-1] != 1:
+        _check(False, f"{op}: pages must have unit stride along the head dimension")
+    if not _written_once(shape, key_stride):
+        _check(False, f"{op}: key_pages must not overlap itself")
+    if not _written_once(shape, value_stride):
+        _check(False, f"{op}: value_pages must not overlap itself")
+    if torch.is_grad_enabled():
+        _grad_free(op, key_pages, value_pages)
 
 
 def _validate_table(op, page_table) -> None:
-    _check(page_table.dim() == 2 and page_table.dtype == torch.int32 and page_table.shape[0] > 0 and
-           page_table.shape[1] > 0, f"{op}: page_table must be int32 [slots, columns]")
-    _check(page_table.stride(1) == 1 or page_table.shape[1] == 1, f"{op}: page_table rows must be contiguous")
+    shape = page_table.shape
+    if len(shape) != 2 or page_table.dtype is not torch.int32 or 0 in shape:
+        _check(False, f"{op}: page_table must be int32 [slots, columns]")
+    if page_table.stride(1) != 1 and shape[1] != 1:
+        _check(False, f"{op}: page_table rows must be contiguous")
 
 
 def _validate_books(op, page_table, lengths, refcounts) -> None:
     _validate_table(op, page_table)
-    _check(page_table.stride(0) >= page_table.shape[1] or page_table.shape[0] == 1,
-           f"{op}: page_table rows must not overlap")
+    slots, columns = page_table.shape
+    if page_table.stride(0) < columns and slots != 1:
+        _check(False, f"{op}: page_table rows must not overlap")
+    device = page_table.device
     if lengths is not None:
-        _check_list(lengths, torch.int64, page_table,
-                    f"{op}: lengths must be a contiguous int64 vector on the page_table device")
-        _check(lengths.shape[0] == page_table.shape[0], f"{op}: lengths must have one entry per page_table row")
-    _check_list(refcounts, torch.int32, page_table,
-                f"{op}: refcounts must be a contiguous int32 vector on the page_table device")
-    _check(refcounts.shape[0] > 0, f"{op}: refcounts must have one entry per page")
+        if lengths.dim() != 1 or lengths.dtype is not torch.int64 or lengths.device != device or not lengths.is_contiguous():
+            _check(False, f"{op}: lengths must be a contiguous int64 vector on the page_table device")
+        if lengths.shape[0] != slots:
+            _check(False, f"{op}: lengths must have one entry per page_table row")
+    if refcounts.dim() != 1 or refcounts.dtype is not torch.int32 or refcounts.device != device or not refcounts.is_contiguous():
+        _check(False, f"{op}: refcounts must be a contiguous int32 vector on the page_table device")
+    if refcounts.shape[0] == 0:
+        _check(False, f"{op}: refcounts must have one entry per page")
 
 
 def _validate_requests(op, name, requests, like) -> None:
-    _check_list(requests, torch.int64, like, f"{op}: {name} must be a contiguous int64 vector on the cache's device")
+    if (requests.dim() != 1 or requests.dtype is not torch.int64 or requests.device != like.device or
+            not requests.is_contiguous()):
+        _check(False, f"{op}: {name} must be a contiguous int64 vector on the cache's device")
 
 
 def _pool(key_pages, value_pages) -> _native.PagePool:
@@ -310,12 +347,11 @@ def _reserve_cuda(page_table, lengths, refcounts, page_size, slots, counts=None)
     status = torch.empty(requests, dtype=torch.int32, device=slots.device)
     if requests == 0:
         return positions, status
-    words = ctypes.c_int64(0)
-    _call("flux_page_reserve_workspace_words", requests, page_table.shape[0], refcounts.shape[0], ctypes.byref(words))
-    workspace = torch.empty(words.value, dtype=torch.int32, device=slots.device)
+    words = _size_from("flux_page_reserve_workspace_words", requests, page_table.shape[0], refcounts.shape[0])
+    workspace = torch.empty(words, dtype=torch.int32, device=slots.device)
     with _on(slots.device):
         _call("flux_page_reserve", ctypes.byref(_books(page_table, lengths, refcounts, page_size)), slots.data_ptr(),
-              _address(counts), requests, positions.data_ptr(), status.data_ptr(), workspace.data_ptr(), words.value,
+              _address(counts), requests, positions.data_ptr(), status.data_ptr(), workspace.data_ptr(), words,
               _stream(slots))
     return positions, status
 
@@ -352,7 +388,7 @@ def _write_cuda(key, value, key_pages, value_pages, page_table, slots, positions
         return
     with _on(key_pages.device):
         _call("flux_page_write", ctypes.byref(_pool(key_pages, value_pages)), key.data_ptr(), value.data_ptr(),
-              _THREE(*key.stride()[:3]), _THREE(*value.stride()[:3]), key.shape[0], key.shape[2],
+              _FOUR(*key.stride()), _FOUR(*value.stride()), key.shape[0], key.shape[2],
               page_table.data_ptr(), page_table.stride(0), page_table.shape[0], page_table.shape[1], slots.data_ptr(),
               positions.data_ptr(), _address(counts), _stream(key_pages))
 
@@ -413,13 +449,12 @@ def _fork_cuda(key_pages, value_pages, page_table, lengths, refcounts, parents, 
     status = torch.empty(requests, dtype=torch.int32, device=parents.device)
     if requests == 0:
         return status
-    words = ctypes.c_int64(0)
-    _call("flux_page_fork_workspace_words", requests, page_table.shape[0], refcounts.shape[0], ctypes.byref(words))
-    workspace = torch.empty(words.value, dtype=torch.int32, device=parents.device)
+    words = _size_from("flux_page_fork_workspace_words", requests, page_table.shape[0], refcounts.shape[0])
+    workspace = torch.empty(words, dtype=torch.int32, device=parents.device)
     with _on(parents.device):
         _call("flux_page_fork", ctypes.byref(_pool(key_pages, value_pages)),
               ctypes.byref(_books(page_table, lengths, refcounts, _page_size_of(key_pages))), parents.data_ptr(),
-              children.data_ptr(), requests, status.data_ptr(), workspace.data_ptr(), words.value, _stream(parents))
+              children.data_ptr(), requests, status.data_ptr(), workspace.data_ptr(), words, _stream(parents))
     return status
 
 
@@ -437,55 +472,66 @@ def _compact_cuda(key_pages, value_pages, page_table, refcounts):
     pages = refcounts.shape[0]
     page_map = torch.empty(pages, dtype=torch.int32, device=refcounts.device)
     used = torch.empty((), dtype=torch.int64, device=refcounts.device)
-    words = ctypes.c_int64(0)
-    _call("flux_page_compact_workspace_words", pages, ctypes.byref(words))
-    workspace = torch.empty(words.value, dtype=torch.int32, device=refcounts.device)
+    words = _size_from("flux_page_compact_workspace_words", pages)
+    workspace = torch.empty(words, dtype=torch.int32, device=refcounts.device)
     with _on(refcounts.device):
         _call("flux_page_compact", ctypes.byref(_pool(key_pages, value_pages)),
               ctypes.byref(_books(page_table, None, refcounts, _page_size_of(key_pages))), page_map.data_ptr(),
-              used.data_ptr(), workspace.data_ptr(), words.value, _stream(refcounts))
+              used.data_ptr(), workspace.data_ptr(), words, _stream(refcounts))
     return page_map, used
 
 
 # ---------------------------------------------------------------------------
 # logits_process
 
+def _validate_penalty(name, penalty, device, rows, history) -> None:
+    if (penalty.dim() != 1 or penalty.dtype is not torch.float32 or penalty.device != device or
+            not penalty.is_contiguous()):
+        _check(False, f"flux::logits_process: {name} must be a contiguous float32 vector on the logits device")
+    if penalty.shape[0] != rows:
+        _check(False, f"flux::logits_process: {name} must have one entry per row")
+    if history is None:
+        _check(False, f"flux::logits_process: {name} needs a history")
+
+
 def _validate_logits(logits, history=None, history_lengths=None, repetition=None, frequency=None, presence=None,
                      bias=None, allowed=None) -> None:
-    op = "flux::logits_process"
-    _check(logits.dim() == 2 and logits.shape[0] > 0 and 0 < logits.shape[1] <= _MAX_VOCAB,
+    shape, device = logits.shape, logits.device
+    _check(len(shape) == 2 and shape[0] > 0 and 0 < shape[1] <= _MAX_VOCAB,
            "flux::logits_process: logits must be [rows, vocab], non-empty, vocab at most 16777216")
     _check(logits.dtype in _TYPES, "flux::logits_process: logits must have dtype float32, float16 or bfloat16")
-    _check(logits.stride(1) == 1 or logits.shape[1] == 1, "flux::logits_process: logits rows must be contiguous")
-    rows, vocab = logits.shape
+    rows, vocab = shape
+    _check(logits.stride(1) == 1 or vocab == 1, "flux::logits_process: logits rows must be contiguous")
     if history is not None:
-        _check(history.dim() == 2 and history.shape[0] == rows and history.dtype == torch.int64,
+        width = history.shape
+        _check(len(width) == 2 and width[0] == rows and history.dtype is torch.int64,
                "flux::logits_process: history must be int64 [rows, width]")
-        _check(history.stride(1) == 1 or history.shape[1] <= 1, "flux::logits_process: history rows must be contiguous")
-        _check(history.device == logits.device, "flux::logits_process: tensor devices must match")
+        _check(history.stride(1) == 1 or width[1] <= 1, "flux::logits_process: history rows must be contiguous")
+        _check(history.device == device, "flux::logits_process: tensor devices must match")
     _check(history is not None or history_lengths is None, "flux::logits_process: history_lengths needs a history")
     if history_lengths is not None:
-        _check_list(history_lengths, torch.int64, logits,
-                    "flux::logits_process: history_lengths must be a contiguous int64 vector on the logits device")
-        _check(history_lengths.shape[0] == rows, "flux::logits_process: history_lengths must have one entry per row")
-    for name, penalty in (("repetition", repetition), ("frequency", frequency), ("presence", presence)):
-        if penalty is not None:
-            _check_list(penalty, torch.float32, logits,
-                        f"{op}: {name} must be a contiguous float32 vector on the logits device")
-            _check(penalty.shape[0] == rows, f"{op}: {name} must have one entry per row")
-            _check(history is not None, f"{op}: {name} needs a history")
+        _check_list(history_lengths, torch.int64, device,
+                    "flux::logits_process: history_lengths must be a contiguous int64 vector on the logits device",
+                    rows, "flux::logits_process: history_lengths must have one entry per row")
+    if repetition is not None:
+        _validate_penalty("repetition", repetition, device, rows, history)
+    if frequency is not None:
+        _validate_penalty("frequency", frequency, device, rows, history)
+    if presence is not None:
+        _validate_penalty("presence", presence, device, rows, history)
     if bias is not None:
-        _check(bias.dim() == 2 and bias.shape[0] in (1, rows) and bias.shape[1] == vocab and
-               bias.dtype == torch.float32 and bias.device == logits.device,
-               "flux::logits_process: bias must be float32 [1 or rows, vocab] on the logits device")
+        width = bias.shape
+        _check(len(width) == 2 and width[0] in (1, rows) and width[1] == vocab and bias.dtype is torch.float32 and
+               bias.device == device, "flux::logits_process: bias must be float32 [1 or rows, vocab] on the logits device")
         _check(bias.stride(1) == 1 or vocab == 1, "flux::logits_process: bias rows must be contiguous")
     if allowed is not None:
-        _check(allowed.dim() == 2 and allowed.shape[0] in (1, rows) and allowed.shape[1] == (vocab + 31) // 32 and
-               allowed.dtype == torch.int32 and allowed.device == logits.device,
+        width = allowed.shape
+        _check(len(width) == 2 and width[0] in (1, rows) and width[1] == (vocab + 31) // 32 and
+               allowed.dtype is torch.int32 and allowed.device == device,
                "flux::logits_process: allowed must be int32 [1 or rows, ceil(vocab / 32)] on the logits device")
-        _check(allowed.stride(1) == 1 or allowed.shape[1] == 1,
-               "flux::logits_process: allowed rows must be contiguous")
-    _grad_free(op, logits, bias, repetition, frequency, presence)
+        _check(allowed.stride(1) == 1 or width[1] == 1, "flux::logits_process: allowed rows must be contiguous")
+    if torch.is_grad_enabled():
+        _grad_free("flux::logits_process", logits, bias, repetition, frequency, presence)
 
 
 def _row_stride(tensor) -> int:
@@ -499,15 +545,14 @@ def _logits_cuda(logits, history=None, history_lengths=None, repetition=None, fr
     rows, vocab = logits.shape
     processed = torch.empty((rows, vocab), dtype=logits.dtype, device=logits.device)
     tokens = torch.empty(rows, dtype=torch.int64, device=logits.device)
-    needed = ctypes.c_int64(0)
-    _call("flux_logits_process_workspace_bytes", rows, vocab, ctypes.byref(needed))
-    workspace = torch.empty(needed.value, dtype=torch.uint8, device=logits.device) if needed.value else None
+    needed = _size_from("flux_logits_process_workspace_bytes", rows, vocab)
+    workspace = torch.empty(needed, dtype=torch.uint8, device=logits.device) if needed else None
     with _on(logits.device):
         _call("flux_logits_process", _TYPES[logits.dtype], logits.data_ptr(), logits.stride(0), processed.data_ptr(),
               tokens.data_ptr(), rows, vocab, _address(history), 0 if history is None else history.shape[1],
               0 if history is None else history.stride(0), _address(history_lengths), _address(repetition),
               _address(frequency), _address(presence), _address(bias), _row_stride(bias), _address(allowed),
-              _row_stride(allowed), _address(workspace), needed.value, _stream(logits))
+              _row_stride(allowed), _address(workspace), needed, _stream(logits))
     return processed, tokens
 
 
@@ -617,7 +662,7 @@ def paged_decode_attention_native(query: torch.Tensor, key_pages: torch.Tensor, 
     (b without slots) of ``page_table`` and ``lengths``.  ``window`` > 0 leaves the last ``window`` keys and the first
     ``sinks`` visible.  Keys on an entry outside [0, P) are left out; a sequence that sees nothing gives zeros.
     """
-    _require_library("paged decode attention")
+    _ready("paged decode attention")
     return torch.ops.flux.paged_decode_attention(query, key_pages, value_pages, page_table, lengths, scale, window,
                                                  sinks, slots)
 
@@ -630,7 +675,7 @@ def paged_decode_attention_native_out(query: torch.Tensor, key_pages: torch.Tens
 
     Calls that may overlap need workspaces of their own.
     """
-    _require_library("paged decode attention out variant")
+    _ready("paged decode attention out variant")
     return torch.ops.flux.paged_decode_attention_out(query, key_pages, value_pages, page_table, lengths, scale, window,
                                                      sinks, slots, output, workspace)
 
@@ -645,7 +690,7 @@ def window_attention_native(query: torch.Tensor, key: torch.Tensor, value: torch
     ``j > position - window`` or ``j < sinks``; window 0 leaves all of them visible.  Rows whose position is not a
     key's give zeros: a padded batch of prompts passes ``starts`` of zeros and its lengths.
     """
-    _require_library("window attention")
+    _ready("window attention")
     return torch.ops.flux.window_attention(query, key, value, scale, window, sinks, lengths, starts)
 
 
@@ -657,7 +702,7 @@ def paged_cache_reserve_native(page_table: torch.Tensor, lengths: torch.Tensor, 
     Columns without a page get the lowest free ones, in the order of the requests, and ``lengths`` grow.  A request that
     cannot be served changes nothing and has position -1.
     """
-    _require_library("paged cache")
+    _ready("paged cache")
     return torch.ops.flux.paged_cache_reserve(page_table, lengths, refcounts, page_size, slots, counts)
 
 
@@ -669,14 +714,14 @@ def paged_cache_write_native(key: torch.Tensor, value: torch.Tensor, key_pages: 
     Only the first ``counts[i]`` tokens of request i are written.  Negative positions (refused reservations) and rows on
     no page are skipped; two requests must not name the same rows.
     """
-    _require_library("paged cache")
+    _ready("paged cache")
     torch.ops.flux.paged_cache_write(key, value, key_pages, value_pages, page_table, slots, positions, counts)
 
 
 def paged_cache_copy_native(key_pages: torch.Tensor, value_pages: torch.Tensor, source: torch.Tensor,
                             target: torch.Tensor) -> torch.Tensor:
     """Pages ``source`` to pages ``target`` in all layers; returns the status of each pair."""
-    _require_library("paged cache")
+    _ready("paged cache")
     return torch.ops.flux.paged_cache_copy(key_pages, value_pages, source, target)
 
 
@@ -687,14 +732,14 @@ def paged_cache_fork_native(key_pages: torch.Tensor, value_pages: torch.Tensor, 
 
     Full pages are shared, the rows of a partial last page are copied to a new page, so both may write on.
     """
-    _require_library("paged cache")
+    _ready("paged cache")
     return torch.ops.flux.paged_cache_fork(key_pages, value_pages, page_table, lengths, refcounts, parents, children)
 
 
 def paged_cache_free_native(page_table: torch.Tensor, lengths: torch.Tensor, refcounts: torch.Tensor,
                             slots: torch.Tensor) -> torch.Tensor:
     """Empties ``slots``: their pages lose a holder each, and those without one are free; returns the status of each."""
-    _require_library("paged cache")
+    _ready("paged cache")
     return torch.ops.flux.paged_cache_free(page_table, lengths, refcounts, slots)
 
 
@@ -704,7 +749,7 @@ def paged_cache_compact_native(key_pages: torch.Tensor, value_pages: torch.Tenso
 
     ``page_table`` and ``refcounts`` follow; ``page_map`` gives each page's new place (-1: free) for what else names one.
     """
-    _require_library("paged cache")
+    _ready("paged cache")
     return torch.ops.flux.paged_cache_compact(key_pages, value_pages, page_table, refcounts)
 
 
@@ -720,7 +765,7 @@ def logits_process_native(logits: torch.Tensor, history: torch.Tensor | None = N
     added and tokens whose bit of ``allowed`` (bit v % 32 of word v // 32) is clear become -inf.  The greedy token is the
     lowest index of the largest processed logit (NaN above all numbers).
     """
-    _require_library("logits process")
+    _ready("logits process")
     return torch.ops.flux.logits_process(logits, history, history_lengths, repetition, frequency, presence, bias, allowed)
 
 
