@@ -12,17 +12,12 @@ namespace {
 constexpr int kPlanThreads = 1024;
 constexpr int kPlanWaves = kPlanThreads / kWave;
 
-// Values that other threads of this workgroup wrote: past the L1.
+// Values that other threads of this workgroup wrote: past the L1, because some of them come from atomics.
 __device__ __forceinline__ int32_t load_shared_word(const int32_t* p) {
     return __hip_atomic_load(p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
 }
 __device__ __forceinline__ void store_shared_word(int32_t* p, int32_t v) {
     __hip_atomic_store(p, v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-}
-
-__device__ __forceinline__ void plan_barrier() {
-    __threadfence();
-    __syncthreads();
 }
 
 __device__ __forceinline__ int wave_inclusive_scan(int v) {
@@ -74,7 +69,7 @@ __device__ int find_free_pages(const int32_t* refcounts, int64_t pages, int want
         }
         found += total;
     }
-    plan_barrier();
+    __syncthreads();
     return found < wanted ? found : wanted;
 }
 
@@ -84,12 +79,12 @@ __device__ void mark_first(const int64_t* list, int64_t requests, int64_t slots,
         const int64_t slot = list[i];
         if (slot >= 0 && slot < slots) store_shared_word(first + slot, 0x7fffffff);
     }
-    plan_barrier();
+    __syncthreads();
     for (int64_t i = threadIdx.x; i < requests; i += kPlanThreads) {
         const int64_t slot = list[i];
         if (slot >= 0 && slot < slots) atomicMin(first + slot, static_cast<int32_t>(i));
     }
-    plan_barrier();
+    __syncthreads();
 }
 
 // In place: need[i] -> sum of need[0..i]; returns the total.  A request without pages to get has need 0.
@@ -103,7 +98,7 @@ __device__ int prefix_in_place(int32_t* need, int64_t requests, int* sums) {
         if (i < requests) store_shared_word(need + i, running + before + mine);
         running += total;
     }
-    plan_barrier();
+    __syncthreads();
     return running;
 }
 
@@ -164,7 +159,7 @@ __global__ void __launch_bounds__(kPlanThreads) page_reserve_kernel(PageBooks b,
         for (int step = 1; step < kReserveLanes; step *= 2) count += __shfl_xor(count, step, kWave);
         if (i < requests && lane == 0) store_shared_word(need + i, count);
     }
-    plan_barrier();
+    __syncthreads();
     const int total = prefix_in_place(need, requests, sums);
     const int64_t most = total < b.pages ? total : b.pages;
     const int found = total > 0 ? find_free_pages(b.refcounts, b.pages, static_cast<int>(most), list, sums) : 0;
@@ -229,63 +224,97 @@ __global__ void __launch_bounds__(256) page_free_kernel(PageBooks b, const int64
 }
 
 // ---------------------------------------------------------------------------
-// Rows of one page of one layer's keys or values, `rows` of each head.  kUnit: 16 bytes where rows allow it.
+// `rows` rows of each head of one page of one layer, keys and values.  Unit: 16 bytes where every row allows it.  Units
+// are numbered by row, head and place in the row, or by their address where a whole page lies in one run; every thread
+// requests kAhead of them before it writes any.
+constexpr int kAhead = 4;
+
 template <class Unit>
-__device__ __forceinline__ void copy_page_rows(char* base, const int64_t* strides, int64_t heads, int rows, int width,
-                                               int element, int64_t layer, int64_t from, int64_t to) {
-    const Unit* src = reinterpret_cast<const Unit*>(base + (layer * strides[0] + from * strides[1]) * element);
-    Unit* dst = reinterpret_cast<Unit*>(base + (layer * strides[0] + to * strides[1]) * element);
-    const int64_t head_stride = strides[2] * element / static_cast<int>(sizeof(Unit));
-    const int64_t row_stride = strides[3] * element / static_cast<int>(sizeof(Unit));
-    const int per_head = rows * width;
-    const int items = static_cast<int>(heads) * per_head;
-    constexpr int kAhead = 4;
-    for (int base_item = threadIdx.x; base_item < items; base_item += kAhead * 256) {
-        Unit held[kAhead];
-        int64_t at[kAhead];
+struct PageRows {
+    const PagePool& p;
+    const char* from[2];  // key, value
+    char* to[2];
+    int units;
+    bool run;
+
+    __device__ __forceinline__ PageRows(const PagePool& pool, int64_t layer, int64_t source, int64_t target, int rows) : p(pool) {
+        units = rows * static_cast<int>(p.row_units.divisor * p.of_heads.divisor);
+        run = rows == p.page;
+        char* base[2] = {p.key, p.value};
+#pragma unroll
+        for (int s = 0; s < 2; ++s) {
+            const int64_t* strides = s ? p.value_strides : p.key_strides;
+            from[s] = base[s] + (layer * strides[0] + source * strides[1]) * p.element;
+            to[s] = base[s] + (layer * strides[0] + target * strides[1]) * p.element;
+            run = run && strides[3] == p.dim && strides[2] == p.page * p.dim;
+        }
+    }
+    __device__ __forceinline__ int64_t offset(int unit, int s) const {
+        if (run) return static_cast<int64_t>(unit) * sizeof(Unit);
+        const uint32_t line = divide(unit, p.row_units), row = divide(line, p.of_heads);
+        const int64_t* strides = s ? p.value_strides : p.key_strides;
+        return ((line - row * p.of_heads.divisor) * strides[2] + row * strides[3]) * p.element +
+               (unit - line * p.row_units.divisor) * static_cast<int>(sizeof(Unit));
+    }
+    // Units first, first + 256, ... of one side.
+    __device__ __forceinline__ void load(int s, int first, Unit (&held)[kAhead], int64_t (&at)[kAhead]) const {
 #pragma unroll
         for (int j = 0; j < kAhead; ++j) {
-            const int item = base_item + 256 * j;
-            if (item < items) {
-                const int head = item / per_head, rest = item % per_head;
-                at[j] = head * head_stride + (rest / width) * row_stride + rest % width;
-                held[j] = src[at[j]];
-            }
+            at[j] = offset(first + 256 * j, s);
+            if (first + 256 * j < units) held[j] = *reinterpret_cast<const Unit*>(from[s] + at[j]);
         }
+    }
+    __device__ __forceinline__ void store(int s, int first, const Unit (&held)[kAhead], const int64_t (&at)[kAhead]) const {
 #pragma unroll
         for (int j = 0; j < kAhead; ++j)
-            if (base_item + 256 * j < items) dst[at[j]] = held[j];
+            if (first + 256 * j < units) *reinterpret_cast<Unit*>(to[s] + at[j]) = held[j];
     }
-}
+    __device__ __forceinline__ void copy_side(int s, int first) const {
+        for (; first < units; first += kAhead * 256) {
+            Unit held[kAhead];
+            int64_t at[kAhead];
+            load(s, first, held, at);
+            store(s, first, held, at);
+        }
+    }
+    __device__ __forceinline__ void copy_from(int first) const {
+        for (; first < units; first += kAhead * 256) {
+            Unit key[kAhead], value[kAhead];
+            int64_t key_at[kAhead], value_at[kAhead];
+            load(0, first, key, key_at);
+            load(1, first, value, value_at);
+            store(0, first, key, key_at);
+            store(1, first, value, value_at);
+        }
+    }
+};
 
-template <class Unit>
-__device__ __forceinline__ void copy_rows(const PagePool& p, int64_t layer, int side, int64_t from, int64_t to,
-                                          int64_t rows) {
-    copy_page_rows<Unit>(side ? p.value : p.key, side ? p.value_strides : p.key_strides, p.heads,
-                         static_cast<int>(rows), static_cast<int>(p.dim * p.element / static_cast<int>(sizeof(Unit))),
-                         p.element, layer, from, to);
-}
-
-// Copy.  Workgroup (request, 2 * layer + side).  Every workgroup of a request looks through the lists for the
-// conflicts that would make its result depend on the order: a few loads against a page's rows.
+// Copy.  Workgroup (request, layer).  Every workgroup of a request looks through the lists for the conflicts that would make
+// its result depend on the order, while the first rows are on their way.
 template <class Unit>
 __global__ void __launch_bounds__(256) page_copy_kernel(PagePool p, const int64_t* __restrict__ source,
                                                         const int64_t* __restrict__ target, int64_t requests,
                                                         int32_t* status) {
     const int64_t i = blockIdx.x;
     const int64_t from = source[i], to = target[i];
-    int result = kPageDone;
     if (from < 0 || from >= p.pages || to < 0 || to >= p.pages) {
-        result = kPageOutOfRange;
-    } else {
-        int clash = 0;
-        for (int64_t j = threadIdx.x; j < requests; j += 256)
-            clash |= (j < i && target[j] == to) || (j != i && source[j] == to);
-        if (__syncthreads_or(clash)) result = kPageRepeated;
+        if (blockIdx.y == 0 && threadIdx.x == 0) status[i] = kPageOutOfRange;
+        return;
     }
-    if (blockIdx.y == 0 && threadIdx.x == 0) status[i] = result;
-    if (result != kPageDone || from == to) return;
-    copy_rows<Unit>(p, blockIdx.y >> 1, blockIdx.y & 1, from, to, p.page);
+    const PageRows<Unit> rows(p, blockIdx.y, from, to, static_cast<int>(p.page));
+    Unit key[kAhead], value[kAhead];
+    int64_t key_at[kAhead], value_at[kAhead];
+    rows.load(0, threadIdx.x, key, key_at);
+    rows.load(1, threadIdx.x, value, value_at);
+    int clash = 0;
+    for (int64_t j = threadIdx.x; j < requests; j += 256)
+        clash |= (j < i && target[j] == to) || (j != i && source[j] == to);
+    clash = __syncthreads_or(clash);
+    if (blockIdx.y == 0 && threadIdx.x == 0) status[i] = clash ? kPageRepeated : kPageDone;
+    if (clash || from == to) return;
+    rows.store(0, threadIdx.x, key, key_at);
+    rows.store(1, threadIdx.x, value, value_at);
+    rows.copy_from(threadIdx.x + kAhead * 256);
 }
 
 // ---------------------------------------------------------------------------
@@ -296,6 +325,7 @@ struct ForkPlan {
     int32_t* list;           // [pages]
     int32_t* length;         // [requests]: tokens of the parent, -1: refused
     int32_t* fresh;          // [requests]: new page of the partial rows
+    int32_t* last;           // [requests]: the parent's page that holds them
 };
 
 __device__ __host__ ForkPlan fork_plan(int32_t* workspace, int64_t requests, int64_t slots, int64_t pages) {
@@ -305,6 +335,7 @@ __device__ __host__ ForkPlan fork_plan(int32_t* workspace, int64_t requests, int
     f.list = f.need + requests;
     f.length = f.list + pages;
     f.fresh = f.length + requests;
+    f.last = f.fresh + requests;
     return f;
 }
 
@@ -354,7 +385,7 @@ __global__ void __launch_bounds__(kPlanThreads) page_fork_plan_kernel(PageBooks 
             store_shared_word(f.length + i, result == kPageDone ? static_cast<int32_t>(length) : -1 - result);
         }
     }
-    plan_barrier();
+    __syncthreads();
     const int total = prefix_in_place(f.need, requests, sums);
     const int64_t most = total < b.pages ? total : b.pages;
     const int found = total > 0 ? find_free_pages(b.refcounts, b.pages, static_cast<int>(most), f.list, sums) : 0;
@@ -374,11 +405,12 @@ __global__ void __launch_bounds__(kPlanThreads) page_fork_plan_kernel(PageBooks 
         }
         if (result != kPageDone) f.length[i] = -1;
         f.fresh[i] = fresh;
+        if (fresh >= 0) f.last[i] = b.table[parents[i] * b.table_stride + length / b.page];
         status[i] = result;
     }
 }
 
-// Workgroup (request, part): part 0 writes the child's books, part 1 + 2 * layer + side copies partial rows.
+// Workgroup (request, part): part 0 writes the child's books, part 1 + layer copies partial rows.
 template <class Unit>
 __global__ void __launch_bounds__(256) page_fork_kernel(PagePool p, PageBooks b, const int64_t* __restrict__ parents,
                                                         const int64_t* __restrict__ children, int64_t requests,
@@ -386,11 +418,12 @@ __global__ void __launch_bounds__(256) page_fork_kernel(PagePool p, PageBooks b,
     const ForkPlan f = fork_plan(workspace, requests, b.slots, b.pages);
     const int64_t i = blockIdx.x;
     const int64_t length = f.length[i];
+    const int32_t fresh = f.fresh[i], last = f.last[i];  // together: last holds nothing where fresh is -1
     if (length < 0) return;
-    const int64_t full = length / b.page, rest = length % b.page;
-    // A parent that is itself a child of this call was empty: none of its columns is read.
-    const int32_t* from = b.table + parents[i] * b.table_stride;
     if (blockIdx.y == 0) {
+        const int64_t full = length / b.page;
+        // A parent that is itself a child of this call was empty: none of its columns is read.
+        const int32_t* from = b.table + parents[i] * b.table_stride;
         int32_t* to = b.table + children[i] * b.table_stride;
         for (int64_t c = threadIdx.x; c < full; c += 256) {
             const int32_t page = from[c];
@@ -398,12 +431,11 @@ __global__ void __launch_bounds__(256) page_fork_kernel(PagePool p, PageBooks b,
             atomicAdd(b.refcounts + page, 1);
         }
         if (threadIdx.x == 0) {
-            if (rest) to[full] = f.fresh[i];
+            if (fresh >= 0) to[full] = fresh;
             b.lengths[children[i]] = length;
         }
-    } else if (rest) {
-        const int part = blockIdx.y - 1;
-        copy_rows<Unit>(p, part >> 1, part & 1, from[full], f.fresh[i], rest);
+    } else if (fresh >= 0) {
+        PageRows<Unit>(p, blockIdx.y - 1, last, fresh, static_cast<int>(length % b.page)).copy_from(threadIdx.x);
     }
 }
 
@@ -454,7 +486,7 @@ __global__ void __launch_bounds__(kPlanThreads) page_compact_plan_kernel(int32_t
         holes += total_holes;
         movers += total_movers;
     }
-    plan_barrier();
+    __syncthreads();
     for (int k = threadIdx.x; k < movers; k += kPlanThreads) {  // holes == movers
         const int32_t from = load_shared_word(plan.source + k), to = load_shared_word(plan.target + k);
         page_map[from] = to;
@@ -479,20 +511,22 @@ __global__ void __launch_bounds__(256) page_compact_kernel(PagePool p, PageBooks
         const int32_t page = *entry;
         if (page >= 0) *entry = page < p.pages ? page_map[page] : -1;
     }
-    const int64_t units = static_cast<int64_t>(*plan.moves) * p.layers * 2;
+    const int64_t parts = 2 * p.layers, units = *plan.moves * parts;
     for (int64_t unit = blockIdx.x; unit < units; unit += gridDim.x) {
-        const int64_t k = unit / (2 * p.layers), part = unit % (2 * p.layers);
-        copy_rows<Unit>(p, part >> 1, part & 1, plan.source[k], plan.target[k], p.page);
+        const int64_t k = unit / parts, part = unit % parts;
+        PageRows<Unit>(p, part >> 1, plan.source[k], plan.target[k], static_cast<int>(p.page)).copy_side(part & 1, threadIdx.x);
     }
 }
 
 // ---------------------------------------------------------------------------
-// Write.  Workgroup (tokens, request): rows of new tokens, all heads, keys then values.
+// Write.  Workgroup (tokens, request): rows of kWriteTokens new tokens, all heads, keys then values.  The tokens' places are
+// looked up once; every thread requests kAhead units before it writes any.
 constexpr int kWriteTokens = 16;
 
 template <class Unit>
 __global__ void __launch_bounds__(256) page_write_kernel(PagePool p, PageWriteArgs a) {
     constexpr int kBytes = sizeof(Unit);
+    __shared__ int64_t place[2][kWriteTokens];  // bytes from the pool's start, -1: no page
     const int64_t i = blockIdx.y;
     const int64_t slot = a.slot_list[i], start = a.positions[i];
     if (slot < 0 || slot >= a.slots || start < 0) return;
@@ -502,25 +536,41 @@ __global__ void __launch_bounds__(256) page_write_kernel(PagePool p, PageWriteAr
     if (start >= capacity) return;
     if (count > capacity - start) count = capacity - start;
     const int64_t t0 = static_cast<int64_t>(blockIdx.x) * kWriteTokens;
+    if (t0 >= count) return;
     const int tokens = static_cast<int>(count - t0 < kWriteTokens ? count - t0 : kWriteTokens);
-    const int width = static_cast<int>(p.dim * p.element / kBytes);
-    const int heads = static_cast<int>(p.heads);
-    const int side_items = tokens * heads * width;
-    const int32_t* row = a.table + slot * a.table_stride;
-    for (int item = threadIdx.x; item < 2 * side_items; item += 256) {
-        const int side = item >= side_items;
-        const int at = side ? item - side_items : item;
-        const int unit = at % width, head = at / width % heads;
-        const int64_t t = t0 + at / width / heads;
-        const int64_t position = start + t;
-        const int32_t page = row[position / p.page];
-        if (page < 0 || page >= p.pages) continue;
-        const int64_t* from = side ? a.value_strides : a.key_strides;
-        const int64_t* to = side ? p.value_strides : p.key_strides;
-        const char* src = (side ? a.value : a.key) + (i * from[0] + head * from[1] + t * from[2]) * p.element;
-        char* dst = (side ? p.value : p.key) +
-                    (page * to[1] + head * to[2] + position % p.page * to[3]) * p.element;
-        reinterpret_cast<Unit*>(dst)[unit] = reinterpret_cast<const Unit*>(src)[unit];
+    if (static_cast<int>(threadIdx.x) < tokens) {
+        const uint32_t position = static_cast<uint32_t>(start + t0 + threadIdx.x), rows = static_cast<uint32_t>(p.page);
+        const int64_t page = a.table[slot * a.table_stride + position / rows], row = position % rows;
+        const bool held = page >= 0 && page < p.pages;
+        place[0][threadIdx.x] = held ? (page * p.key_strides[1] + row * p.key_strides[3]) * p.element : -1;
+        place[1][threadIdx.x] = held ? (page * p.value_strides[1] + row * p.value_strides[3]) * p.element : -1;
+    }
+    __syncthreads();
+    const uint32_t width = p.row_units.divisor, heads = p.of_heads.divisor;
+    const int side = static_cast<int>(tokens * heads * width);
+    const char* sources[2] = {a.key + (i * a.key_strides[0] + t0 * a.key_strides[2]) * p.element,
+                              a.value + (i * a.value_strides[0] + t0 * a.value_strides[2]) * p.element};
+    constexpr int kEach = 2 * kAhead;
+    for (int first = threadIdx.x; first < 2 * side; first += kEach * 256) {
+        Unit held[kEach];
+        char* to[kEach];
+#pragma unroll
+        for (int j = 0; j < kEach; ++j) {
+            const int unit = first + 256 * j, s = unit >= side;
+            to[j] = nullptr;
+            if (unit >= 2 * side) continue;
+            const uint32_t at = unit - s * side, row = divide(at, p.row_units), u = at - row * width;
+            const uint32_t t = divide(row, p.of_heads), head = row - t * heads;
+            const int64_t where = place[s][t];
+            if (where < 0) continue;
+            to[j] = (s ? p.value : p.key) + where + head * (s ? p.value_strides : p.key_strides)[2] * p.element + u * kBytes;
+            held[j] = *reinterpret_cast<const Unit*>((s ? sources[1] : sources[0]) +
+                                                     (head * (s ? a.value_strides : a.key_strides)[1] +
+                                                      t * (s ? a.value_strides : a.key_strides)[2]) * p.element + u * kBytes);
+        }
+#pragma unroll
+        for (int j = 0; j < kEach; ++j)
+            if (to[j]) *reinterpret_cast<Unit*>(to[j]) = held[j];
     }
 }
 
@@ -542,7 +592,7 @@ bool rows_of(const PageWriteArgs& a, int element, int64_t bytes) {
 }  // namespace
 
 size_t page_reserve_workspace(int64_t requests, int64_t slots, int64_t pages) { return requests + slots + pages; }
-size_t page_fork_workspace(int64_t requests, int64_t slots, int64_t pages) { return 3 * requests + slots + pages; }
+size_t page_fork_workspace(int64_t requests, int64_t slots, int64_t pages) { return 4 * requests + slots + pages; }
 size_t page_compact_workspace(int64_t pages) { return 4 + 2 * pages; }
 
 hipError_t launch_page_reserve(const PageBooks& books, const int64_t* slots, const int64_t* counts, int64_t requests,
@@ -560,46 +610,58 @@ hipError_t launch_page_free(const PageBooks& books, const int64_t* slots, int64_
 }
 
 // The widest unit that every row's start and length is a multiple of: 16 bytes, else one element.
-#define FLUX_BY_UNIT(wide, element, kernel, grid, ...)                                                              \
-    if (wide) hipLaunchKernelGGL(HIP_KERNEL_NAME(kernel<uint4>), grid, dim3(256), 0, stream, __VA_ARGS__);          \
-    else if ((element) == 4) hipLaunchKernelGGL(HIP_KERNEL_NAME(kernel<uint32_t>), grid, dim3(256), 0, stream,      \
-                                                __VA_ARGS__);                                                       \
-    else hipLaunchKernelGGL(HIP_KERNEL_NAME(kernel<uint16_t>), grid, dim3(256), 0, stream, __VA_ARGS__);            \
-    return hipGetLastError()
-
-hipError_t launch_page_copy(const PagePool& pool, const int64_t* source, const int64_t* target, int64_t requests,
-                            int32_t* status, hipStream_t stream) {
-    const dim3 grid(static_cast<uint32_t>(requests), static_cast<uint32_t>(2 * pool.layers));
-    FLUX_BY_UNIT(rows_of(pool, 16), pool.element, page_copy_kernel, grid, pool, source, target, requests, status);
+PagePool with_units(PagePool pool, bool wide) {
+    pool.unit = wide ? 16 : pool.element;
+    pool.row_units = make_divider(static_cast<uint32_t>(pool.dim * pool.element / pool.unit));
+    pool.of_heads = make_divider(static_cast<uint32_t>(pool.heads));
+    return pool;
 }
 
-hipError_t launch_page_fork(const PagePool& pool, const PageBooks& books, const int64_t* parents,
+#define FLUX_BY_UNIT(pool, kernel, grid, ...)                                                                       \
+    if ((pool).unit == 16)                                                                                          \
+        hipLaunchKernelGGL(HIP_KERNEL_NAME(kernel<uint4>), grid, dim3(256), 0, stream, pool, __VA_ARGS__);          \
+    else if ((pool).unit == 4)                                                                                      \
+        hipLaunchKernelGGL(HIP_KERNEL_NAME(kernel<uint32_t>), grid, dim3(256), 0, stream, pool, __VA_ARGS__);       \
+    else                                                                                                            \
+        hipLaunchKernelGGL(HIP_KERNEL_NAME(kernel<uint16_t>), grid, dim3(256), 0, stream, pool, __VA_ARGS__);       \
+    return hipGetLastError()
+
+hipError_t launch_page_copy(const PagePool& plain, const int64_t* source, const int64_t* target, int64_t requests,
+                            int32_t* status, hipStream_t stream) {
+    const PagePool pool = with_units(plain, rows_of(plain, 16));
+    const dim3 grid(static_cast<uint32_t>(requests), static_cast<uint32_t>(pool.layers));
+    FLUX_BY_UNIT(pool, page_copy_kernel, grid, source, target, requests, status);
+}
+
+hipError_t launch_page_fork(const PagePool& plain, const PageBooks& books, const int64_t* parents,
                             const int64_t* children, int64_t requests, int32_t* status, int32_t* workspace,
                             hipStream_t stream) {
     hipLaunchKernelGGL(page_fork_plan_kernel, dim3(1), dim3(kPlanThreads), 0, stream, books, parents, children,
                        requests, status, workspace);
     const hipError_t launched = hipGetLastError();
     if (launched != hipSuccess) return launched;
-    const dim3 grid(static_cast<uint32_t>(requests), static_cast<uint32_t>(1 + 2 * pool.layers));
-    FLUX_BY_UNIT(rows_of(pool, 16), pool.element, page_fork_kernel, grid, pool, books, parents, children, requests,
+    const PagePool pool = with_units(plain, rows_of(plain, 16));
+    const dim3 grid(static_cast<uint32_t>(requests), static_cast<uint32_t>(1 + pool.layers));
+    FLUX_BY_UNIT(pool, page_fork_kernel, grid, books, parents, children, requests,
                  workspace);
 }
 
-hipError_t launch_page_compact(const PagePool& pool, const PageBooks& books, int32_t* page_map, int64_t* used,
+hipError_t launch_page_compact(const PagePool& plain, const PageBooks& books, int32_t* page_map, int64_t* used,
                                int32_t* workspace, hipStream_t stream) {
-    hipLaunchKernelGGL(page_compact_plan_kernel, dim3(1), dim3(kPlanThreads), 0, stream, books.refcounts, pool.pages,
+    hipLaunchKernelGGL(page_compact_plan_kernel, dim3(1), dim3(kPlanThreads), 0, stream, books.refcounts, plain.pages,
                        page_map, used, workspace);
     const hipError_t launched = hipGetLastError();
     if (launched != hipSuccess) return launched;
-    const dim3 grid(2048);
-    FLUX_BY_UNIT(rows_of(pool, 16), pool.element, page_compact_kernel, grid, pool, books, page_map, workspace);
+    const PagePool pool = with_units(plain, rows_of(plain, 16));
+    const dim3 grid(8192);
+    FLUX_BY_UNIT(pool, page_compact_kernel, grid, books, page_map, workspace);
 }
 
-hipError_t launch_page_write(const PagePool& pool, const PageWriteArgs& args, hipStream_t stream) {
+hipError_t launch_page_write(const PagePool& plain, const PageWriteArgs& args, hipStream_t stream) {
     const dim3 grid(static_cast<uint32_t>((args.tokens + kWriteTokens - 1) / kWriteTokens),
                     static_cast<uint32_t>(args.requests));
-    FLUX_BY_UNIT(rows_of(pool, 16) && rows_of(args, pool.element, 16), pool.element, page_write_kernel, grid, pool,
-                 args);
+    const PagePool pool = with_units(plain, rows_of(plain, 16) && rows_of(args, plain.element, 16));
+    FLUX_BY_UNIT(pool, page_write_kernel, grid, args);
 }
 
 #undef FLUX_BY_UNIT

@@ -315,8 +315,8 @@ __global__ void __launch_bounds__(kDecodeThreads, kDim * sizeof(T) <= 512 ? 2 : 
     }
 }
 
-// Joins the parts of a sequence that was cut.  Workgroup (sequence, column tile of a KV head): the parts' weights once,
-// then the threads go over the tile's heads and dims.
+// Joins the parts of a sequence that was cut.  Workgroup (sequence, column tile of a KV head, 256 of the
+// tile's heads and dims): the parts' shares first.
 constexpr int kJoinParts = 128;  // parts whose shares are kept
 
 template <class T, int kTile>
@@ -381,7 +381,8 @@ __global__ void __launch_bounds__(kDecodeThreads) decode_join_kernel(AttentionAr
     T* out = static_cast<T*>(a.out) + (b * static_cast<int64_t>(a.query_heads) + head) * a.dim;
     const int items = columns * a.dim;
     __syncthreads();
-    for (int item = threadIdx.x; item < items; item += kDecodeThreads) {
+    const int item = blockIdx.z * kDecodeThreads + threadIdx.x;
+    if (item < items) {
         const int column = item / a.dim, d = item - column * a.dim;
         const float* from = o + column * width + d;
         float sum = 0.0f;
@@ -412,7 +413,8 @@ hipError_t launch_decode(const AttentionArgs& a, hipStream_t stream) {
     const hipError_t launched = hipGetLastError();
     if (launched != hipSuccess) return launched;
     if (a.keys <= kLeastTiles * tile_of(kDim, sizeof(T))) return hipSuccess;  // no sequence is cut
-    hipLaunchKernelGGL(HIP_KERNEL_NAME(decode_join_kernel<T, tile_of(kDim, sizeof(T))>), dim3(a.batch, a.kv_heads * column_tiles),
+    const int items = ((a.group < kColumns ? a.group : kColumns) * a.dim + kDecodeThreads - 1) / kDecodeThreads;
+    hipLaunchKernelGGL(HIP_KERNEL_NAME(decode_join_kernel<T, tile_of(kDim, sizeof(T))>), dim3(a.batch, a.kv_heads * column_tiles, items),
                        dim3(kDecodeThreads), 0, stream, a);
     return hipGetLastError();
 }

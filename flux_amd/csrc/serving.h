@@ -90,6 +90,10 @@ struct PagePool {
     int64_t key_strides[4];  // layer, page, head, row
     int64_t value_strides[4];
     int element;  // bytes
+    // Set by the launchers: the unit that rows are moved in, and divisions by a row's units and by the heads.
+    int unit;
+    Divider row_units;
+    Divider of_heads;
 };
 
 // What an operator did with one request (flux_page_status in the C ABI).

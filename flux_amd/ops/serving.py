@@ -56,6 +56,8 @@ SERVING_SCHEMAS = {
                        "Tensor? allowed=None) -> (Tensor processed, Tensor tokens)"),
 }
 
+SERVING_OPERATOR_NAMES = tuple(SERVING_SCHEMAS)
+
 for _schema in SERVING_SCHEMAS.values():
     _LIBRARY.define(_schema)
 
@@ -343,7 +345,7 @@ def _reserve_cuda(page_table, lengths, refcounts, page_size, slots, counts=None)
     _validate_reserve(page_table, lengths, refcounts, page_size, slots, counts)
     _require_gpu("flux::paged_cache_reserve", page_table)
     requests = slots.shape[0]
-    positions = torch.empty(requests, dtype=torch.int64, device=slots.device)
+    positions = torch.empty_like(slots)
     status = torch.empty(requests, dtype=torch.int32, device=slots.device)
     if requests == 0:
         return positions, status
@@ -635,7 +637,18 @@ def _logits_fake(logits, history=None, history_lengths=None, repetition=None, fr
 
 
 # ---------------------------------------------------------------------------
-# Python entry points.
+# Python entry points.  They call the overloads themselves: looking one up by its packet costs 2 us a call.
+
+class _Overloads:
+    __slots__ = SERVING_OPERATOR_NAMES
+
+    def __init__(self) -> None:
+        for name in SERVING_OPERATOR_NAMES:
+            setattr(self, name, getattr(torch.ops.flux, name).default)
+
+
+_OPS = _Overloads()
+
 
 def native_paged_decode_attention_is_available() -> bool:
     return _availability("paged_decode_attention", "paged_decode_attention_out")
@@ -663,7 +676,7 @@ def paged_decode_attention_native(query: torch.Tensor, key_pages: torch.Tensor, 
     ``sinks`` visible.  Keys on an entry outside [0, P) are left out; a sequence that sees nothing gives zeros.
     """
     _ready("paged decode attention")
-    return torch.ops.flux.paged_decode_attention(query, key_pages, value_pages, page_table, lengths, scale, window,
+    return _OPS.paged_decode_attention(query, key_pages, value_pages, page_table, lengths, scale, window,
                                                  sinks, slots)
 
 
@@ -676,7 +689,7 @@ def paged_decode_attention_native_out(query: torch.Tensor, key_pages: torch.Tens
     Calls that may overlap need workspaces of their own.
     """
     _ready("paged decode attention out variant")
-    return torch.ops.flux.paged_decode_attention_out(query, key_pages, value_pages, page_table, lengths, scale, window,
+    return _OPS.paged_decode_attention_out(query, key_pages, value_pages, page_table, lengths, scale, window,
                                                      sinks, slots, output, workspace)
 
 
@@ -691,7 +704,7 @@ def window_attention_native(query: torch.Tensor, key: torch.Tensor, value: torch
     key's give zeros: a padded batch of prompts passes ``starts`` of zeros and its lengths.
     """
     _ready("window attention")
-    return torch.ops.flux.window_attention(query, key, value, scale, window, sinks, lengths, starts)
+    return _OPS.window_attention(query, key, value, scale, window, sinks, lengths, starts)
 
 
 def paged_cache_reserve_native(page_table: torch.Tensor, lengths: torch.Tensor, refcounts: torch.Tensor, page_size: int,
@@ -703,7 +716,7 @@ def paged_cache_reserve_native(page_table: torch.Tensor, lengths: torch.Tensor, 
     cannot be served changes nothing and has position -1.
     """
     _ready("paged cache")
-    return torch.ops.flux.paged_cache_reserve(page_table, lengths, refcounts, page_size, slots, counts)
+    return _OPS.paged_cache_reserve(page_table, lengths, refcounts, page_size, slots, counts)
 
 
 def paged_cache_write_native(key: torch.Tensor, value: torch.Tensor, key_pages: torch.Tensor, value_pages: torch.Tensor,
@@ -715,14 +728,14 @@ def paged_cache_write_native(key: torch.Tensor, value: torch.Tensor, key_pages: 
     no page are skipped; two requests must not name the same rows.
     """
     _ready("paged cache")
-    torch.ops.flux.paged_cache_write(key, value, key_pages, value_pages, page_table, slots, positions, counts)
+    _OPS.paged_cache_write(key, value, key_pages, value_pages, page_table, slots, positions, counts)
 
 
 def paged_cache_copy_native(key_pages: torch.Tensor, value_pages: torch.Tensor, source: torch.Tensor,
                             target: torch.Tensor) -> torch.Tensor:
     """Pages ``source`` to pages ``target`` in all layers; returns the status of each pair."""
     _ready("paged cache")
-    return torch.ops.flux.paged_cache_copy(key_pages, value_pages, source, target)
+    return _OPS.paged_cache_copy(key_pages, value_pages, source, target)
 
 
 def paged_cache_fork_native(key_pages: torch.Tensor, value_pages: torch.Tensor, page_table: torch.Tensor,
@@ -733,14 +746,14 @@ def paged_cache_fork_native(key_pages: torch.Tensor, value_pages: torch.Tensor, 
     Full pages are shared, the rows of a partial last page are copied to a new page, so both may write on.
     """
     _ready("paged cache")
-    return torch.ops.flux.paged_cache_fork(key_pages, value_pages, page_table, lengths, refcounts, parents, children)
+    return _OPS.paged_cache_fork(key_pages, value_pages, page_table, lengths, refcounts, parents, children)
 
 
 def paged_cache_free_native(page_table: torch.Tensor, lengths: torch.Tensor, refcounts: torch.Tensor,
                             slots: torch.Tensor) -> torch.Tensor:
     """Empties ``slots``: their pages lose a holder each, and those without one are free; returns the status of each."""
     _ready("paged cache")
-    return torch.ops.flux.paged_cache_free(page_table, lengths, refcounts, slots)
+    return _OPS.paged_cache_free(page_table, lengths, refcounts, slots)
 
 
 def paged_cache_compact_native(key_pages: torch.Tensor, value_pages: torch.Tensor, page_table: torch.Tensor,
@@ -750,7 +763,7 @@ def paged_cache_compact_native(key_pages: torch.Tensor, value_pages: torch.Tenso
     ``page_table`` and ``refcounts`` follow; ``page_map`` gives each page's new place (-1: free) for what else names one.
     """
     _ready("paged cache")
-    return torch.ops.flux.paged_cache_compact(key_pages, value_pages, page_table, refcounts)
+    return _OPS.paged_cache_compact(key_pages, value_pages, page_table, refcounts)
 
 
 def logits_process_native(logits: torch.Tensor, history: torch.Tensor | None = None,
@@ -766,7 +779,5 @@ def logits_process_native(logits: torch.Tensor, history: torch.Tensor | None = N
     lowest index of the largest processed logit (NaN above all numbers).
     """
     _ready("logits process")
-    return torch.ops.flux.logits_process(logits, history, history_lengths, repetition, frequency, presence, bias, allowed)
+    return _OPS.logits_process(logits, history, history_lengths, repetition, frequency, presence, bias, allowed)
 
-
-SERVING_OPERATOR_NAMES = tuple(SERVING_SCHEMAS)
