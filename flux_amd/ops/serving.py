@@ -360,27 +360,37 @@ def _reserve_cuda(page_table, lengths, refcounts, page_size, slots, counts=None)
 
 def _validate_write(key, value, key_pages, value_pages, page_table, slots, positions, counts=None) -> None:
     op = "flux::paged_cache_write"
-    _validate_pools(op, key_pages, value_pages, ranks=(4,))
+    _validate_pools(op, key_pages, value_pages, (4,))
     _validate_table(op, page_table)
-    _check(page_table.device == key_pages.device, f"{op}: tensor devices must match")
-    _check(page_table.shape[1] * key_pages.shape[2] <= _MAX_KEYS,
-           f"{op}: page_table holds more than 16777216 positions a row")
-    _check(key.dim() == 4 and value.shape == key.shape, f"{op}: key and value must be rank four and of one shape")
-    _check(key.dtype == key_pages.dtype and value.dtype == key_pages.dtype and key.device == key_pages.device and
-           value.device == key_pages.device, f"{op}: key and value must have the pages' dtype and device")
-    _check(key.shape[1] == key_pages.shape[1] and key.shape[3] == key_pages.shape[3],
-           f"{op}: key heads and head dimension must be the pages'")
-    _check(key.stride(3) == 1 and value.stride(3) == 1 or key.shape[3] == 1,
-           f"{op}: key and value must have unit stride along the head dimension")
-    for source in (key, value):
-        for pages in (key_pages, value_pages):
-            _check(not _aliases(source, pages), f"{op}: the pages must not alias key or value")
-    for name, tensor in (("slots", slots), ("positions", positions), ("counts", counts)):
-        if tensor is not None:
-            _validate_requests(op, name, tensor, key_pages)
-            _check(tensor.shape[0] == key.shape[0], f"{op}: {name} must have one entry per request")
-    _check(key.shape[0] <= 65535, f"{op}: more than 65535 requests")
-    _grad_free(op, key, value)
+    shape, pages, dtype, device = key.shape, key_pages.shape, key_pages.dtype, key_pages.device
+    _check(page_table.device == device, "flux::paged_cache_write: tensor devices must match")
+    _check(page_table.shape[1] * pages[2] <= _MAX_KEYS,
+           "flux::paged_cache_write: page_table holds more than 16777216 positions a row")
+    _check(len(shape) == 4 and value.shape == shape,
+           "flux::paged_cache_write: key and value must be rank four and of one shape")
+    _check(key.dtype is dtype and value.dtype is dtype and key.device == device and value.device == device,
+           "flux::paged_cache_write: key and value must have the pages' dtype and device")
+    _check(shape[1] == pages[1] and shape[3] == pages[3],
+           "flux::paged_cache_write: key heads and head dimension must be the pages'")
+    _check(key.stride(3) == 1 and value.stride(3) == 1 or shape[3] == 1,
+           "flux::paged_cache_write: key and value must have unit stride along the head dimension")
+    stores = key_pages.untyped_storage().data_ptr(), value_pages.untyped_storage().data_ptr()
+    _check(key.untyped_storage().data_ptr() not in stores and value.untyped_storage().data_ptr() not in stores,
+           "flux::paged_cache_write: the pages must not alias key or value")
+    requests = shape[0]
+    _check_list(slots, torch.int64, device,
+                "flux::paged_cache_write: slots must be a contiguous int64 vector on the cache's device",
+                requests, "flux::paged_cache_write: slots must have one entry per request")
+    _check_list(positions, torch.int64, device,
+                "flux::paged_cache_write: positions must be a contiguous int64 vector on the cache's device",
+                requests, "flux::paged_cache_write: positions must have one entry per request")
+    if counts is not None:
+        _check_list(counts, torch.int64, device,
+                    "flux::paged_cache_write: counts must be a contiguous int64 vector on the cache's device",
+                    requests, "flux::paged_cache_write: counts must have one entry per request")
+    _check(requests <= 65535, "flux::paged_cache_write: more than 65535 requests")
+    if torch.is_grad_enabled():
+        _grad_free(op, key, value)
 
 
 def _write_cuda(key, value, key_pages, value_pages, page_table, slots, positions, counts=None):
