@@ -13,10 +13,6 @@
 namespace flux {
 namespace {
 
-#ifndef FLUX_ROW_TILES
-#define FLUX_ROW_TILES 1
-#endif
-
 constexpr int kThreads = 256;
 constexpr int kWaves = 4;
 
@@ -71,148 +67,213 @@ __device__ void exact_row(const AttentionArgs& a, const T* query, const T* keys,
         if (kWave * c + lane < a.dim) out[kWave * c + lane] = static_cast<T>(sum[c] / weight);
 }
 
-template <class T, int kDim, bool kWide>
-__global__ void __launch_bounds__(kThreads) window_attention_kernel(AttentionArgs a) {
-    using M = Mfma<T>;
+// Blocks that an XCD (block index modulo 8) takes one after the other: consecutive tiles share most of their keys.  The
+// runs are short and the XCDs change places with every eight of them, because a padded batch's sequences differ in length.
+constexpr int kTileRun = 16;
+__device__ __forceinline__ int tile_of_block() {
+    const int eight = blockIdx.x / (8 * kTileRun);
+    return (8 * eight + (blockIdx.x + eight) % 8) * kTileRun + blockIdx.x / 8 % kTileRun;
+}
+int64_t blocks_of_tiles(int64_t tiles) { return (tiles + 8 * kTileRun - 1) / (8 * kTileRun) * (8 * kTileRun); }
+
+// One tile's place and the rows' common quantities.
+struct TileRows {
+    int row0, all_rows, kv_head;
+    int64_t b, n, start;
+
+    __device__ __forceinline__ TileRows(const AttentionArgs& a, int tile, int row_tiles, int rows) {
+        row0 = tile % row_tiles * rows;
+        kv_head = tile / row_tiles % a.kv_heads;
+        b = tile / row_tiles / a.kv_heads;
+        all_rows = a.queries * a.group;
+        n = a.lengths ? a.lengths[b] : a.keys;
+        n = n < 0 ? 0 : (n > a.keys ? a.keys : n);
+        start = a.starts ? a.starts[b] : n - a.queries;
+        start = start < -a.queries ? -a.queries : (start > a.keys ? a.keys : start);  // no row beyond these sees a key
+    }
+    // Query index and head of a row.
+    __device__ __forceinline__ void place(const AttentionArgs& a, int r, int64_t& i, int64_t& head) const {
+        i = divide(r, a.group_of);
+        head = kv_head * a.group + r - i * a.group;
+    }
+    __device__ __forceinline__ RowRange range(const AttentionArgs& a, int r, int64_t i) const {
+        const int64_t position = start + i;
+        RowRange range;
+        range.position = r < all_rows && position >= 0 && position < n ? static_cast<int>(position) : -1;
+        range.low = a.window > 0 && range.position >= a.window ? range.position - a.window + 1 : 0;
+        return range;
+    }
+    // Positions of the rows [from, from + count), cut to those that are a key's; first > last when there is none.
+    __device__ __forceinline__ void positions(const AttentionArgs& a, int from, int count, int& first, int& last) const {
+        const int to = from + count < all_rows ? from + count - 1 : all_rows - 1;
+        const int64_t p = start + divide(from, a.group_of), q = start + divide(to, a.group_of);
+        first = static_cast<int>(p < 0 ? 0 : p);
+        last = static_cast<int>(q >= n ? n - 1 : q);
+        if (from > to) last = first - 1;
+    }
+    // The row again over the keys it sees alone.
+    template <class T>
+    __device__ __forceinline__ void again(const AttentionArgs& a, int r, const T* keys, const T* values) const {
+        int64_t i, head;
+        place(a, r, i, head);
+        exact_row<T>(a, static_cast<const T*>(a.query) + b * a.query_strides[0] + head * a.query_strides[1] + i * a.query_strides[2],
+                     keys, values, range(a, r, i), static_cast<T*>(a.out) + ((b * a.query_heads + head) * a.queries + i) * a.dim);
+    }
+};
+
+// The keys that any of a tile's rows sees, as tiles of kTile: the sinks', then the window's.
+template <int kTile>
+struct KeyTiles {
+    int seen, sink_tiles, first_tile, count;
+    __device__ __forceinline__ KeyTiles(const AttentionArgs& a, int first, int last) {
+        const int low = a.window > 0 && first >= a.window ? first - a.window + 1 : 0;
+        const int sinks = a.sinks < low ? a.sinks : low;
+        const int of_sinks = (sinks + kTile - 1) / kTile;
+        seen = last + 1;
+        first_tile = low / kTile;
+        sink_tiles = of_sinks < first_tile ? of_sinks : first_tile;
+        count = first > last ? 0 : sink_tiles + (seen + kTile - 1) / kTile - first_tile;
+    }
+    __device__ __forceinline__ int base(int t) const { return (t < sink_tiles ? t : first_tile + t - sink_tiles) * kTile; }
+};
+
+template <int kDim, bool kWide>
+__global__ void __launch_bounds__(kThreads, kDim <= 64 ? 2 : 1) window_attention_kernel(AttentionArgs a, int row_tiles, int tiles_total) {
+    using M = Mfma<float>;
     constexpr int kCols = kDim == 256 ? 1 : 2;  // tiles of 16 rows
     constexpr int kRows = 16 * kCols;
-    constexpr int kTile = kDim * static_cast<int>(sizeof(T)) <= 256 ? 32 : 16;
+    constexpr int kTile = kDim <= 64 ? 32 : 16;
     constexpr int kSubs = kTile / 16;
     constexpr int kFragments = M::template key_fragments<kDim>();
     constexpr int kChunks = M::template value_chunks<kDim>();
     constexpr int kBlocks = kDim / 16;
     constexpr int kWords = kBlocks * 4 + 2;
-    using Value = typename M::template ValueChunk<kDim>;
     __shared__ float merge[2][kCols * kWords][kWave];
 
+    const int tile = tile_of_block();
+    if (tile >= tiles_total) return;
+    const TileRows rows(a, tile, row_tiles, kRows);
     const int lane = threadIdx.x & 63;
     const int wave = threadIdx.x >> 6;
     const int n16 = lane & 15;
     const int g = lane >> 4;
-    const int kv_head = blockIdx.y;
-    const int64_t b = blockIdx.z;
-    int64_t n = a.lengths ? a.lengths[b] : a.keys;
-    n = n < 0 ? 0 : (n > a.keys ? a.keys : n);
-    int64_t start = a.starts ? a.starts[b] : n - a.queries;
-    start = start < -a.queries ? -a.queries : (start > a.keys ? a.keys : start);  // no row beyond these sees a key
-    const int64_t row0 = static_cast<int64_t>(blockIdx.x) * kRows;
-    const int64_t all_rows = static_cast<int64_t>(a.queries) * a.group;
+    const float* keys = static_cast<const float*>(a.key) + rows.b * a.key_strides[0] + rows.kv_head * a.key_strides[1];
+    const float* values = static_cast<const float*>(a.value) + rows.b * a.value_strides[0] + rows.kv_head * a.value_strides[1];
 
-    // This lane's rows, one per column tile.
     RowRange mine[kCols];
-    const T* query_row[kCols];
-    int64_t out_row[kCols];
-    bool real[kCols];
-#pragma unroll
-    for (int c = 0; c < kCols; ++c) {
-        const int64_t r = row0 + 16 * c + n16;
-        const int64_t i = r / a.group, head = kv_head * static_cast<int64_t>(a.group) + r % a.group;
-        real[c] = r < all_rows;
-        const int64_t position = start + i;
-        mine[c].position = real[c] && position >= 0 && position < n ? static_cast<int>(position) : -1;
-        mine[c].low = a.window > 0 && mine[c].position >= a.window ? mine[c].position - a.window + 1 : 0;
-        query_row[c] = static_cast<const T*>(a.query) + b * a.query_strides[0] + head * a.query_strides[1] +
-                       i * a.query_strides[2];
-        out_row[c] = (b * a.query_heads + head) * a.queries + i;
-    }
-    // The tile's first and last position that is a key's; all of its rows lie between.
-    const int64_t last_row = row0 + kRows < all_rows ? row0 + kRows - 1 : all_rows - 1;
-    int64_t first_position = start + row0 / a.group, last_position = start + last_row / a.group;
-    if (first_position < 0) first_position = 0;
-    if (last_position >= n) last_position = n - 1;
-    const bool any = first_position <= last_position;
-
-    const T* keys = static_cast<const T*>(a.key) + b * a.key_strides[0] + kv_head * a.key_strides[1];
-    const T* values = static_cast<const T*>(a.value) + b * a.value_strides[0] + kv_head * a.value_strides[1];
-
-    typename M::Fragment query[kCols][kFragments];
-#pragma unroll
-    for (int c = 0; c < kCols; ++c)
-#pragma unroll
-        for (int f = 0; f < kFragments; ++f)
-            query[c][f] = M::load_query(query_row[c], a.query_strides[3], M::kKeyStep * f + M::kPer * g, a.dim, real[c]);
-
+    int sink_end[kCols];
+    f32x4 query[kCols][kFragments];
     f32x4 out[kCols][kBlocks];
     float top[kCols], weight[kCols];
 #pragma unroll
     for (int c = 0; c < kCols; ++c) {
+        const int r = rows.row0 + 16 * c + n16;
+        int64_t i, head;
+        rows.place(a, r, i, head);
+        mine[c] = rows.range(a, r, i);
+        sink_end[c] = a.sinks < mine[c].low ? a.sinks : mine[c].low;
+        const float* q = static_cast<const float*>(a.query) + rows.b * a.query_strides[0] + head * a.query_strides[1] + i * a.query_strides[2];
+#pragma unroll
+        for (int f = 0; f < kFragments; ++f) {
+            const int d = M::kKeyStep * f + M::kPer * g;
+            if (a.query_wide) query[c][f] = M::template load_row<true>(q, d, a.dim, r < rows.all_rows);
+            else query[c][f] = M::load_query(q, a.query_strides[3], d, a.dim, r < rows.all_rows);
+        }
+#pragma unroll
+        for (int k = 0; k < kBlocks; ++k) out[c][k] = f32x4{0, 0, 0, 0};
         top[c] = -INFINITY;
         weight[c] = 0.0f;
-#pragma unroll
-        for (int i = 0; i < kBlocks; ++i) out[c][i] = f32x4{0, 0, 0, 0};
     }
+    int first_p, last_p;
+    rows.positions(a, rows.row0, kRows, first_p, last_p);
+    const KeyTiles<kTile> tiles(a, first_p, last_p);
+    const int low_of_last = a.window > 0 && last_p >= a.window ? last_p - a.window + 1 : 0;
 
-    if (any) {
-        const int first_p = static_cast<int>(first_position), last_p = static_cast<int>(last_position);
-        const int seen = last_p + 1;
-        const int low = a.window > 0 && first_p >= a.window ? first_p - a.window + 1 : 0;
-        const int low_of_last = a.window > 0 && last_p >= a.window ? last_p - a.window + 1 : 0;
-        const int sinks = a.sinks < low ? a.sinks : low;
-        const int first_tile = low / kTile;
-        const int of_sinks = (sinks + kTile - 1) / kTile;
-        const int sink_tiles = of_sinks < first_tile ? of_sinks : first_tile;
-        const int tiles = sink_tiles + (seen + kTile - 1) / kTile - first_tile;
-
-        for (int t = wave; t < tiles; t += kWaves) {
-            const int base_key = (t < sink_tiles ? t : first_tile + t - sink_tiles) * kTile;
-            typename M::Fragment key[kSubs][kFragments];
-            Value value[kSubs][4][kChunks];
+    struct Tile {
+        f32x4 key[kSubs][kFragments];
+        f32x4 value[kSubs][4][kChunks];
+    };
+    auto load = [&](int t, Tile& into) {
+        const int base = tiles.base(t), end = t < tiles.count ? tiles.seen : 0;
+#pragma unroll
+        for (int s = 0; s < kSubs; ++s) {
+            const int position = base + 16 * s + n16;
+            const float* k = keys + position * a.key_strides[2];
+#pragma unroll
+            for (int f = 0; f < kFragments; ++f)
+                into.key[s][f] = M::template load_row<kWide>(k, M::kKeyStep * f + M::kPer * g, a.dim, position < end);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const int value_position = base + 16 * s + 4 * g + i;
+                const float* v = values + value_position * a.value_strides[2];
+#pragma unroll
+                for (int c = 0; c < kChunks; ++c)
+                    into.value[s][i][c] = M::template load_value<kDim, kWide>(v, c, n16, a.dim, value_position < end);
+            }
+        }
+    };
+    auto work = [&](int t, const Tile& of) {
+        const int base = tiles.base(t);
+        // Every key of the tile is seen by every row that sees any (the others are zeroed at the end).
+        const bool inside = base >= low_of_last && base + kTile - 1 <= first_p;
+#pragma unroll
+        for (int c = 0; c < kCols; ++c) {
+            f32x4 score[kSubs];
+            float highest = -INFINITY;
 #pragma unroll
             for (int s = 0; s < kSubs; ++s) {
-                const int position = base_key + 16 * s + n16;
-                const T* k = keys + position * a.key_strides[2];
+                score[s] = f32x4{0, 0, 0, 0};
 #pragma unroll
-                for (int f = 0; f < kFragments; ++f)
-                    key[s][f] = M::template load_row<kWide>(k, M::kKeyStep * f + M::kPer * g, a.dim, position < seen);
+                for (int f = 0; f < kFragments; ++f) M::multiply_key(of.key[s][f], query[c][f], score[s]);
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
-                    const int value_position = base_key + 16 * s + 4 * g + i;
-                    const T* v = values + value_position * a.value_strides[2];
-#pragma unroll
-                    for (int c = 0; c < kChunks; ++c)
-                        value[s][i][c] = M::template load_value<kDim, kWide>(v, c, n16, a.dim, value_position < seen);
+                    const int j = base + 16 * s + 4 * g + i;
+                    // Without branches: low <= key <= position as one unsigned comparison, or a sink.
+                    const bool visible = inside | (static_cast<uint32_t>(j - mine[c].low) <=
+                                                   static_cast<uint32_t>(mine[c].position - mine[c].low)) | (j < sink_end[c]);
+                    score[s][i] = visible ? score[s][i] * a.scale : -INFINITY;
+                    highest = fmaxf(highest, score[s][i]);
                 }
             }
-            // Every key of the tile is seen by every row that sees any (the others are zeroed at the end).
-            const bool inside = base_key >= low_of_last && base_key + kTile - 1 <= first_p;
+            highest = fmaxf(highest, __shfl_xor(highest, 16, kWave));
+            highest = fmaxf(highest, __shfl_xor(highest, 32, kWave));
+            if (__any(highest > top[c])) {
+                const float now = fmaxf(top[c], highest);
+                const float shrink = top[c] == -INFINITY ? 0.0f : fast_exp2((top[c] - now) * kLog2e);
+                top[c] = now;
+                weight[c] *= shrink;
 #pragma unroll
-            for (int c = 0; c < kCols; ++c) {
-                f32x4 score[kSubs];
-                float highest = -INFINITY;
-#pragma unroll
-                for (int s = 0; s < kSubs; ++s) {
-                    score[s] = f32x4{0, 0, 0, 0};
-#pragma unroll
-                    for (int f = 0; f < kFragments; ++f) M::multiply_key(key[s][f], query[c][f], score[s]);
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        const int j = base_key + 16 * s + 4 * g + i;
-                        const bool visible = inside || (j <= mine[c].position && (j >= mine[c].low || j < a.sinks));
-                        score[s][i] = visible ? score[s][i] * a.scale : -INFINITY;
-                        highest = fmaxf(highest, score[s][i]);
-                    }
-                }
-                highest = fmaxf(highest, __shfl_xor(highest, 16, kWave));
-                highest = fmaxf(highest, __shfl_xor(highest, 32, kWave));
-                if (__any(highest > top[c])) {
-                    const float now = fmaxf(top[c], highest);
-                    const float shrink = top[c] == -INFINITY ? 0.0f : fast_exp2((top[c] - now) * kLog2e);
-                    top[c] = now;
-                    weight[c] *= shrink;
-#pragma unroll
-                    for (int i = 0; i < kBlocks; ++i) out[c][i] *= shrink;
-                }
-                const float reference = top[c] == -INFINITY ? 0.0f : top[c];
-                float p[kSubs][4];
-#pragma unroll
-                for (int s = 0; s < kSubs; ++s)
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        p[s][i] = fast_exp2((score[s][i] - reference) * kLog2e + M::kWeightShift);
-                        weight[c] += p[s][i];
-                    }
-                M::template multiply_value<kDim, kSubs>(value, p, out[c]);
+                for (int i = 0; i < kBlocks; ++i) out[c][i] *= shrink;
             }
+            const float reference = top[c] == -INFINITY ? 0.0f : top[c];
+            float p[kSubs][4];
+#pragma unroll
+            for (int s = 0; s < kSubs; ++s)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    p[s][i] = fast_exp2((score[s][i] - reference) * kLog2e);
+                    weight[c] += p[s][i];
+                }
+            M::template multiply_value<kDim, kSubs>(of.value, p, out[c]);
+        }
+    };
+
+    // Two tiles in registers where two waves per SIMD still fit.
+    Tile even;
+    if constexpr (kDim <= 64) {
+        Tile odd;
+        load(wave, even);
+        for (int t = wave; t < tiles.count; t += 2 * kWaves) {
+            load(t + kWaves, odd);
+            work(t, even);
+            if (t + kWaves >= tiles.count) break;
+            load(t + 2 * kWaves, even);
+            work(t + kWaves, odd);
+        }
+    } else {
+        for (int t = wave; t < tiles.count; t += kWaves) {
+            load(t, even);
+            work(t, even);
         }
     }
 
@@ -224,7 +285,7 @@ __global__ void __launch_bounds__(kThreads) window_attention_kernel(AttentionArg
     // Join the four waves: 2 and 3 into 0 and 1, then 1 into 0.
 #pragma unroll
     for (int half = kWaves / 2; half >= 1; half /= 2) {
-        __syncthreads();
+        if (half == 1) __syncthreads();
         if (wave >= half && wave < 2 * half) {
 #pragma unroll
             for (int c = 0; c < kCols; ++c) {
@@ -258,28 +319,23 @@ __global__ void __launch_bounds__(kThreads) window_attention_kernel(AttentionArg
         float worst = fabsf(weight[c]);
         M::template each_dim<kDim>(g, a.dim, [&](int i, int r, int) { worst += fabsf(out[c][i][r]); });  // keeps NaN, infinity
         const uint64_t odd = __ballot(mine[c].position >= 0 && !(worst < INFINITY));
-        uint32_t rows = static_cast<uint32_t>((odd | odd >> 16 | odd >> 32 | odd >> 48) & 0xffff);
-        if (real[c] && !(rows >> n16 & 1)) {
-            T* o = static_cast<T*>(a.out) + out_row[c] * a.dim;
-            M::template each_dim<kDim>(g, a.dim, [&](int i, int r, int d) {
-                o[d] = static_cast<T>(mine[c].position < 0 ? 0.0f : out[c][i][r] / weight[c]);
+        uint32_t again = static_cast<uint32_t>((odd | odd >> 16 | odd >> 32 | odd >> 48) & 0xffff);
+        const int r = rows.row0 + 16 * c + n16;
+        if (r < rows.all_rows && !(again >> n16 & 1)) {
+            int64_t i, head;
+            rows.place(a, r, i, head);
+            float* o = static_cast<float*>(a.out) + ((rows.b * a.query_heads + head) * a.queries + i) * a.dim;
+            M::template each_dim<kDim>(g, a.dim, [&](int k, int j, int d) {
+                o[d] = mine[c].position < 0 ? 0.0f : out[c][k][j] / weight[c];
             });
         }
-        while (rows) {
-            const int which = __ffs(rows) - 1;
-            rows &= rows - 1;
-            const int64_t r = row0 + 16 * c + which;
-            const int64_t i = r / a.group, head = kv_head * static_cast<int64_t>(a.group) + r % a.group;
-            RowRange range;
-            range.position = static_cast<int>(start + i);
-            range.low = a.window > 0 && range.position >= a.window ? range.position - a.window + 1 : 0;
-            exact_row<T>(a, static_cast<const T*>(a.query) + b * a.query_strides[0] + head * a.query_strides[1] +
-                                i * a.query_strides[2],
-                         keys, values, range, static_cast<T*>(a.out) + ((b * a.query_heads + head) * a.queries + i) * a.dim);
+        while (again) {
+            const int which = __ffs(again) - 1;
+            again &= again - 1;
+            rows.template again<float>(a, rows.row0 + 16 * c + which, keys, values);
         }
     }
 }
-
 
 // ---------------------------------------------------------------------------
 // 16-bit prompts.  Here matrix instructions, exponentials and LDS reads cost about the same, so that keys and values are
@@ -294,7 +350,6 @@ __global__ void __launch_bounds__(kThreads) window_attention_kernel(AttentionArg
 // a step of that type, like the result's own rounding) and summed unrounded in float32.
 typedef float f32x16 __attribute__((ext_vector_type(16)));
 typedef float f32x2 __attribute__((ext_vector_type(2)));
-constexpr int kTileRun = 16;
 constexpr int64_t kStagedStride = 1 << 22;
 
 template <class T>
@@ -370,42 +425,22 @@ window_tile_kernel(AttentionArgs a, int row_tiles, int tiles_total) {
     constexpr float kLazy = 8.0f;
     extern __shared__ char stages[];
 
-    // Consecutive tiles share most of their keys, so each XCD (block index modulo 8) takes runs of kTileRun of them.  The
-    // runs are short and the XCDs change places with every eight of them: a padded batch's sequences differ in length.
-    const int eight = blockIdx.x / (8 * kTileRun);
-    const int tile = (8 * eight + (blockIdx.x + eight) % 8) * kTileRun + blockIdx.x / 8 % kTileRun;
+    const int tile = tile_of_block();
     if (tile >= tiles_total) return;
-    const int row0 = tile % row_tiles * kRows;
-    const int kv_head = tile / row_tiles % a.kv_heads;
-    const int64_t b = tile / row_tiles / a.kv_heads;
-
+    const TileRows rows(a, tile, row_tiles, kRows);
     const int lane = threadIdx.x & 63;
     const int wave = threadIdx.x >> 6;
     const int n32 = lane & 31;
     const int half = lane >> 5;
-    int64_t n = a.lengths ? a.lengths[b] : a.keys;
-    n = n < 0 ? 0 : (n > a.keys ? a.keys : n);
-    int64_t start = a.starts ? a.starts[b] : n - a.queries;
-    start = start < -a.queries ? -a.queries : (start > a.keys ? a.keys : start);
-    const int all_rows = a.queries * a.group;
-
-    // Positions of a range of rows, cut to those that are a key's; first > last when there is none.
-    auto positions = [&](int from, int count, int& first, int& last) {
-        const int to = from + count < all_rows ? from + count - 1 : all_rows - 1;
-        const int64_t p = start + divide(from, a.group_of), q = start + divide(to, a.group_of);
-        first = static_cast<int>(p < 0 ? 0 : p);
-        last = static_cast<int>(q >= n ? n - 1 : q);
-        if (from > to) last = first - 1;
-    };
     int block_first, block_last, wave_first, wave_last;
-    positions(row0, kRows, block_first, block_last);
-    const int wave_row = row0 + wave * kRowTiles * 32;
-    positions(wave_row, kRowTiles * 32, wave_first, wave_last);
+    rows.positions(a, rows.row0, kRows, block_first, block_last);
+    const int wave_row = rows.row0 + wave * kRowTiles * 32;
+    rows.positions(a, wave_row, kRowTiles * 32, wave_first, wave_last);
     wave_first = __builtin_amdgcn_readfirstlane(wave_first);
     wave_last = __builtin_amdgcn_readfirstlane(wave_last);
 
-    const T* keys = static_cast<const T*>(a.key) + b * a.key_strides[0] + kv_head * a.key_strides[1];
-    const T* values = static_cast<const T*>(a.value) + b * a.value_strides[0] + kv_head * a.value_strides[1];
+    const T* keys = static_cast<const T*>(a.key) + rows.b * a.key_strides[0] + rows.kv_head * a.key_strides[1];
+    const T* values = static_cast<const T*>(a.value) + rows.b * a.value_strides[0] + rows.kv_head * a.value_strides[1];
 
     RowRange mine[kRowTiles];
     int sink_end[kRowTiles];
@@ -417,17 +452,16 @@ window_tile_kernel(AttentionArgs a, int row_tiles, int tiles_total) {
 #pragma unroll
     for (int c = 0; c < kRowTiles; ++c) {
         const int r = wave_row + 32 * c + n32;
-        const int64_t i = divide(r, a.group_of), head = kv_head * a.group + r - i * a.group;
-        const int64_t position = start + i;
-        mine[c].position = r < all_rows && position >= 0 && position < n ? static_cast<int>(position) : -1;
-        mine[c].low = a.window > 0 && mine[c].position >= a.window ? mine[c].position - a.window + 1 : 0;
+        int64_t i, head;
+        rows.place(a, r, i, head);
+        mine[c] = rows.range(a, r, i);
         sink_end[c] = a.sinks < mine[c].low ? a.sinks : mine[c].low;
-        const T* q = static_cast<const T*>(a.query) + b * a.query_strides[0] + head * a.query_strides[1] + i * a.query_strides[2];
+        const T* q = static_cast<const T*>(a.query) + rows.b * a.query_strides[0] + head * a.query_strides[1] + i * a.query_strides[2];
 #pragma unroll
         for (int s = 0; s < kSteps; ++s) {
             const int d = 16 * s + 8 * half;
-            if (a.query_wide) query[c][s] = Mfma<T>::template load_row<true>(q, d, a.dim, r < all_rows);
-            else query[c][s] = Mfma<T>::load_query(q, a.query_strides[3], d, a.dim, r < all_rows);
+            if (a.query_wide) query[c][s] = Mfma<T>::template load_row<true>(q, d, a.dim, r < rows.all_rows);
+            else query[c][s] = Mfma<T>::load_query(q, a.query_strides[3], d, a.dim, r < rows.all_rows);
             query[c][s] ^= sign;
         }
 #pragma unroll
@@ -439,15 +473,9 @@ window_tile_kernel(AttentionArgs a, int row_tiles, int tiles_total) {
     }
 
     if (block_first <= block_last) {
+        const KeyTiles<kKeys> tiles(a, block_first, block_last);
+        const int seen = tiles.seen, count = tiles.count;
         auto low_of = [&](int p) { return a.window > 0 && p >= a.window ? p - a.window + 1 : 0; };
-        const int low = low_of(block_first);
-        const int seen = block_last + 1;
-        const int sinks = a.sinks < low ? a.sinks : low;
-        const int first_stage = low / kKeys;
-        const int of_sinks = (sinks + kKeys - 1) / kKeys;
-        const int sink_stages = of_sinks < first_stage ? of_sinks : first_stage;
-        const int count = sink_stages + (seen + kKeys - 1) / kKeys - first_stage;
-        auto stage_key = [&](int t) { return (t < sink_stages ? t : first_stage + t - sink_stages) * kKeys; };
 
         // Rows behind the last key give zeros (a buffer's range check, or a comparison), dims behind the head's repeat its
         // first: they meet a zero in the query or are not stored.
@@ -461,7 +489,7 @@ window_tile_kernel(AttentionArgs a, int row_tiles, int tiles_total) {
         const int key_at = (key_row * key_stride + (key_d < a.dim ? key_d : 0)) * 2;
         const int value_at = (value_row * value_stride + (value_d < a.dim ? value_d : 0)) * 2;
         auto fetch_keys = [&](int t) {
-            const int base = stage_key(t), rows = seen - base < kKeys ? seen - base : kKeys;
+            const int base = tiles.base(t), rows = seen - base < kKeys ? seen - base : kKeys;
             const T* from = keys + base * a.key_strides[2];
             const StagedRows<T, kWide> staged(from, ((rows - 1) * a.key_strides[2] + a.dim) * 2);
 #pragma unroll
@@ -469,7 +497,7 @@ window_tile_kernel(AttentionArgs a, int row_tiles, int tiles_total) {
                 held_key[i] = staged.load(key_at + kKeyRows * i * key_stride * 2, key_row + kKeyRows * i, key_d, rows, a.key_strides[2], a.dim);
         };
         auto fetch_values = [&](int t) {
-            const int base = stage_key(t), rows = seen - base < kKeys ? seen - base : kKeys;
+            const int base = tiles.base(t), rows = seen - base < kKeys ? seen - base : kKeys;
             const T* from = values + base * a.value_strides[2];
             const StagedRows<T, kWide> staged(from, ((rows - 1) * a.value_strides[2] + a.dim) * 2);
 #pragma unroll
@@ -511,7 +539,7 @@ window_tile_kernel(AttentionArgs a, int row_tiles, int tiles_total) {
             __syncthreads();
             const char* stage = stages + (t & 1) * kStage;
             const char* turned = stage + kKeys * kKeyRow;
-            const int base = stage_key(t);
+            const int base = tiles.base(t);
             char* next = stages + ((t + 1) & 1) * kStage;
             if (t + 1 < count) fetch_keys(t + 1);
 #pragma unroll
@@ -616,11 +644,12 @@ window_tile_kernel(AttentionArgs a, int row_tiles, int tiles_total) {
 #pragma unroll
             for (int j = 0; j < 16; ++j) worst += fabsf(out[c][i][j]);  // keeps NaN, infinity
         const uint64_t odd = __ballot(mine[c].position >= 0 && !(worst < INFINITY));
-        uint32_t rows = static_cast<uint32_t>(odd | odd >> 32);
+        uint32_t again = static_cast<uint32_t>(odd | odd >> 32);
         const int r = wave_row + 32 * c + n32;
-        const int64_t i = divide(r, a.group_of), head = kv_head * a.group + r - i * a.group;
-        if (r < all_rows && !(rows >> n32 & 1)) {
-            T* o = static_cast<T*>(a.out) + ((b * a.query_heads + head) * a.queries + i) * a.dim;
+        if (r < rows.all_rows && !(again >> n32 & 1)) {
+            int64_t i, head;
+            rows.place(a, r, i, head);
+            T* o = static_cast<T*>(a.out) + ((rows.b * a.query_heads + head) * a.queries + i) * a.dim;
             const float inverse = mine[c].position < 0 ? 0.0f : 1.0f / weight[c];
 #pragma unroll
             for (int k = 0; k < kBlocks; ++k)
@@ -641,16 +670,10 @@ window_tile_kernel(AttentionArgs a, int row_tiles, int tiles_total) {
                     }
                 }
         }
-        while (rows) {
-            const int which = __ffs(rows) - 1;
-            rows &= rows - 1;
-            const int r = wave_row + 32 * c + which;
-            const int64_t i = divide(r, a.group_of), head = kv_head * a.group + r - i * a.group;
-            RowRange range;
-            range.position = static_cast<int>(start + i);
-            range.low = a.window > 0 && range.position >= a.window ? range.position - a.window + 1 : 0;
-            exact_row<T>(a, static_cast<const T*>(a.query) + b * a.query_strides[0] + head * a.query_strides[1] + i * a.query_strides[2],
-                         keys, values, range, static_cast<T*>(a.out) + ((b * a.query_heads + head) * a.queries + i) * a.dim);
+        while (again) {
+            const int which = __ffs(again) - 1;
+            again &= again - 1;
+            rows.template again<T>(a, wave_row + 32 * c + which, keys, values);
         }
     }
 }
@@ -663,13 +686,14 @@ hipError_t launch_window_tiles(const AttentionArgs& a, hipStream_t stream) {
     const int64_t rows = static_cast<int64_t>(a.queries) * a.group;
     const int row_tiles = static_cast<int>((rows + kRows - 1) / kRows);
     const int64_t tiles = static_cast<int64_t>(row_tiles) * a.kv_heads * a.batch;
-    if (tiles > (int64_t{1} << 23)) return hipErrorInvalidValue;
+    if (tiles >= (int64_t{1} << 24) - 256) return hipErrorInvalidValue;  // a grid has below 2^32 threads
     static const hipError_t room = hipFuncSetAttribute(
         reinterpret_cast<const void*>(window_tile_kernel<T, kDim, kRowTiles, kWide>), hipFuncAttributeMaxDynamicSharedMemorySize,
         static_cast<int>(kLds));
     if (room != hipSuccess) return room;
-    hipLaunchKernelGGL(HIP_KERNEL_NAME(window_tile_kernel<T, kDim, kRowTiles, kWide>), 
-                       dim3(static_cast<uint32_t>((tiles + 8 * kTileRun - 1) / (8 * kTileRun) * (8 * kTileRun))), dim3(kThreads), kLds, stream, a, row_tiles, static_cast<int>(tiles));
+    hipLaunchKernelGGL(HIP_KERNEL_NAME(window_tile_kernel<T, kDim, kRowTiles, kWide>),
+                       dim3(static_cast<uint32_t>(blocks_of_tiles(tiles))), dim3(kThreads), kLds, stream, a, row_tiles,
+                       static_cast<int>(tiles));
     return hipGetLastError();
 }
 
@@ -678,15 +702,17 @@ hipError_t launch_window(const AttentionArgs& a, hipStream_t stream) {
     if constexpr (sizeof(T) == 2) {
         if (a.wide && reinterpret_cast<uintptr_t>(a.out) % 8 == 0 && a.key_strides[2] <= kStagedStride &&
             a.value_strides[2] <= kStagedStride)
-            return launch_window_tiles<T, kDim, FLUX_ROW_TILES, true>(a, stream);
-        return launch_window_tiles<T, kDim, FLUX_ROW_TILES, false>(a, stream);
+            return launch_window_tiles<T, kDim, 1, true>(a, stream);
+        return launch_window_tiles<T, kDim, 1, false>(a, stream);
     } else {
-    constexpr int kRows = kDim == 256 ? 16 : 32;
-    const int64_t rows = static_cast<int64_t>(a.queries) * a.group;
-    const dim3 grid(static_cast<uint32_t>((rows + kRows - 1) / kRows), a.kv_heads, a.batch);
-    if (a.wide) hipLaunchKernelGGL(HIP_KERNEL_NAME(window_attention_kernel<T, kDim, true>), grid, dim3(kThreads), 0, stream, a);
-    else hipLaunchKernelGGL(HIP_KERNEL_NAME(window_attention_kernel<T, kDim, false>), grid, dim3(kThreads), 0, stream, a);
-    return hipGetLastError();
+        constexpr int kRows = kDim == 256 ? 16 : 32;
+        const int64_t row_tiles = (static_cast<int64_t>(a.queries) * a.group + kRows - 1) / kRows;
+        const int64_t tiles = row_tiles * a.kv_heads * a.batch;
+        if (tiles >= (int64_t{1} << 24) - 256) return hipErrorInvalidValue;  // a grid has below 2^32 threads
+        const dim3 grid(static_cast<uint32_t>(blocks_of_tiles(tiles)));
+        if (a.wide) hipLaunchKernelGGL(HIP_KERNEL_NAME(window_attention_kernel<kDim, true>), grid, dim3(kThreads), 0, stream, a, static_cast<int>(row_tiles), static_cast<int>(tiles));
+        else hipLaunchKernelGGL(HIP_KERNEL_NAME(window_attention_kernel<kDim, false>), grid, dim3(kThreads), 0, stream, a, static_cast<int>(row_tiles), static_cast<int>(tiles));
+        return hipGetLastError();
     }
 }
 
