@@ -83,7 +83,7 @@ __device__ __forceinline__ int64_t block_sum(int v, int* sums) {
 
 constexpr int tile_of(int dim, int bytes) { return dim * bytes <= 256 ? 32 : 16; }
 
-template <class T, int kDim, bool kPaged, bool kWide>
+template <class T, int kDim, bool kPaged, Rows kRows>
 __global__ void __launch_bounds__(kDecodeThreads, kDim * sizeof(T) <= 512 ? 2 : 1) decode_attention_kernel(AttentionArgs a) {
     using M = Mfma<T>;
     constexpr int kTile = tile_of(kDim, sizeof(T));
@@ -164,32 +164,35 @@ __global__ void __launch_bounds__(kDecodeThreads, kDim * sizeof(T) <= 512 ? 2 : 
     struct Tile {
         typename M::Fragment key[kSubs][kFragments];
         Value value[kSubs][4][kChunks];
-        int held[kSubs][4];
+        int held[kSubs][4];  // page of each value row, -1: not attended
+        bool partial;        // some key of the tile is not attended; its rows are the pool's first
     };
     auto load = [&](int t, const Pages& p, Tile& tile) {
         const int base = tile_key(t);
+        bool whole = true;
 #pragma unroll
         for (int s = 0; s < kSubs; ++s) {
             int page = p.page[s];
             if constexpr (kPaged) page = page < a.pages ? page : -1;
+            whole = whole && page >= 0;
             const int position = base + 16 * s + n16;
-            const uint32_t in_page = kPaged ? position - divide(position, a.page) * a.page.divisor : position;
-            const T* k = keys + (kPaged ? page * a.key_strides[0] : 0) + in_page * a.key_strides[2];
+            const uint32_t in_page = kPaged ? position - divide(position, a.page) * a.page.divisor : (page >= 0 ? position : 0);
+            const T* k = keys + (kPaged && page > 0 ? page * a.key_strides[0] : 0) + in_page * a.key_strides[2];
 #pragma unroll
             for (int f = 0; f < kFragments; ++f)
-                tile.key[s][f] = M::template load_row<kWide>(k, M::kKeyStep * f + M::kPer * g, a.dim, page >= 0);
+                tile.key[s][f] = M::template load_row<kRows>(k, M::kKeyStep * f + M::kPer * g, a.dim);
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
                 const int of = __shfl(page, 4 * g + i, kWave);
                 tile.held[s][i] = of;
                 const uint32_t value_position = base + 16 * s + 4 * g + i;
-                const uint32_t value_row = kPaged ? value_position - divide(value_position, a.page) * a.page.divisor : value_position;
-                const T* v = values + (kPaged ? of * a.value_strides[0] : 0) + value_row * a.value_strides[2];
+                const uint32_t value_row = kPaged ? value_position - divide(value_position, a.page) * a.page.divisor : (of >= 0 ? value_position : 0);
+                const T* v = values + (kPaged && of > 0 ? of * a.value_strides[0] : 0) + value_row * a.value_strides[2];
 #pragma unroll
-                for (int c = 0; c < kChunks; ++c)
-                    tile.value[s][i][c] = M::template load_value<kDim, kWide>(v, c, n16, a.dim, of >= 0);
+                for (int c = 0; c < kChunks; ++c) tile.value[s][i][c] = M::template load_value<kDim, kRows>(v, c, n16, a.dim);
             }
         }
+        tile.partial = !__all(whole);
     };
 
     f32x4 out[kBlocks];
@@ -198,7 +201,15 @@ __global__ void __launch_bounds__(kDecodeThreads, kDim * sizeof(T) <= 512 ? 2 : 
     float top = -INFINITY, weight = 0.0f;
     typename M::Fragment query[kFragments];  // right operand of S^T: this lane's query head, zero behind the last one
 
-    auto work = [&](const Tile& tile) {
+    auto work = [&](Tile& tile) {
+        if (tile.partial) {  // a weight of zero does not undo a NaN
+#pragma unroll
+            for (int s = 0; s < kSubs; ++s)
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+#pragma unroll
+                    for (int c = 0; c < kChunks; ++c) tile.value[s][i][c] = tile.held[s][i] >= 0 ? tile.value[s][i][c] : Value{};
+        }
         f32x4 score[kSubs];
         float highest = -INFINITY;
 #pragma unroll
@@ -241,30 +252,28 @@ __global__ void __launch_bounds__(kDecodeThreads, kDim * sizeof(T) <= 512 ? 2 : 
     Tile even;
     look_up(from + wave, pages);
     {
-        const int64_t head = kv_head * static_cast<int64_t>(a.group) + column0 + n16;
+        const int64_t head = kv_head * static_cast<int64_t>(a.group) + column0 + (n16 < columns ? n16 : 0);
         const T* q = static_cast<const T*>(a.query) + b * a.query_strides[0] + head * a.query_strides[1];
-#pragma unroll
-        for (int f = 0; f < kFragments; ++f) {
-            const int d = M::kKeyStep * f + M::kPer * g;
-            if (a.query_wide) query[f] = M::template load_row<true>(q, d, a.dim, n16 < columns);
-            else query[f] = M::load_query(q, a.query_strides[3], d, a.dim, n16 < columns);
-        }
+        load_query<T, kFragments, M::kKeyStep>(query, q, a.query_strides[3], a.query_wide, M::kPer * g, a.dim, n16 < columns);
     }
+    // A wave's tile numbers are the same in all its lanes, and said to be: the branches on them are scalar.
+    const int first_tile = __builtin_amdgcn_readfirstlane(from + wave);
     if constexpr (kAhead) {
         Tile odd;
-        load(from + wave, pages, even);
-        look_up(from + wave + kDecodeWaves, pages);
-        for (int t = from + wave; t < to; t += 2 * kDecodeWaves) {
-            load(t + kDecodeWaves, pages, odd);
+        if (first_tile < to) load(first_tile, pages, even);
+        look_up(first_tile + kDecodeWaves, pages);
+        for (int t = first_tile; t < to; t += 2 * kDecodeWaves) {
+            const bool second = t + kDecodeWaves < to;
+            if (second) load(t + kDecodeWaves, pages, odd);
             look_up(t + 2 * kDecodeWaves, pages);
             work(even);
-            if (t + kDecodeWaves >= to) break;
-            load(t + 2 * kDecodeWaves, pages, even);
+            if (!second) break;
+            if (t + 2 * kDecodeWaves < to) load(t + 2 * kDecodeWaves, pages, even);
             look_up(t + 3 * kDecodeWaves, pages);
             work(odd);
         }
     } else {
-        for (int t = from + wave; t < to; t += kDecodeWaves) {
+        for (int t = first_tile; t < to; t += kDecodeWaves) {
             load(t, pages, even);
             look_up(t + kDecodeWaves, pages);
             work(even);
@@ -404,11 +413,13 @@ hipError_t launch_decode(const AttentionArgs& a, hipStream_t stream) {
     const int column_tiles = (a.group + kColumns - 1) / kColumns;
     const dim3 grid(a.blocks + a.batch, a.kv_heads * column_tiles);
     if (a.pages > 0) {
-        if (a.wide) hipLaunchKernelGGL(HIP_KERNEL_NAME(decode_attention_kernel<T, kDim, true, true>), grid, dim3(kDecodeThreads), 0, stream, a);
-        else hipLaunchKernelGGL(HIP_KERNEL_NAME(decode_attention_kernel<T, kDim, true, false>), grid, dim3(kDecodeThreads), 0, stream, a);
+        if (a.wide && a.dim == kDim) hipLaunchKernelGGL(HIP_KERNEL_NAME(decode_attention_kernel<T, kDim, true, kFullRows>), grid, dim3(kDecodeThreads), 0, stream, a);
+        else if (a.wide) hipLaunchKernelGGL(HIP_KERNEL_NAME(decode_attention_kernel<T, kDim, true, kWideRows>), grid, dim3(kDecodeThreads), 0, stream, a);
+        else hipLaunchKernelGGL(HIP_KERNEL_NAME(decode_attention_kernel<T, kDim, true, kNarrow>), grid, dim3(kDecodeThreads), 0, stream, a);
     } else {
-        if (a.wide) hipLaunchKernelGGL(HIP_KERNEL_NAME(decode_attention_kernel<T, kDim, false, true>), grid, dim3(kDecodeThreads), 0, stream, a);
-        else hipLaunchKernelGGL(HIP_KERNEL_NAME(decode_attention_kernel<T, kDim, false, false>), grid, dim3(kDecodeThreads), 0, stream, a);
+        if (a.wide && a.dim == kDim) hipLaunchKernelGGL(HIP_KERNEL_NAME(decode_attention_kernel<T, kDim, false, kFullRows>), grid, dim3(kDecodeThreads), 0, stream, a);
+        else if (a.wide) hipLaunchKernelGGL(HIP_KERNEL_NAME(decode_attention_kernel<T, kDim, false, kWideRows>), grid, dim3(kDecodeThreads), 0, stream, a);
+        else hipLaunchKernelGGL(HIP_KERNEL_NAME(decode_attention_kernel<T, kDim, false, kNarrow>), grid, dim3(kDecodeThreads), 0, stream, a);
     }
     const hipError_t launched = hipGetLastError();
     if (launched != hipSuccess) return launched;

@@ -36,6 +36,11 @@ __device__ __forceinline__ int wave_sum_int(int v) {
     return v;
 }
 
+// How rows are read: element by element, in 16-byte loads, or those where the head fills the padded dims.  Loads are not
+// masked (masks put each one in a block of its own, behind a wait for the register's last value): in 16-byte loads dims
+// behind the head's repeat its first ones, which meet zeros of the query or results that are not stored.
+enum Rows : int { kNarrow = 0, kWideRows = 1, kFullRows = 2 };
+
 template <class T>
 struct Mfma;
 
@@ -52,27 +57,26 @@ struct Mfma<float> {
     template <int kDim>
     static constexpr int value_chunks() { return kDim / 64; }
 
-    static __device__ __forceinline__ Fragment load_query(const float* q, int64_t stride, int d, int dim, bool ok) {
+    static __device__ __forceinline__ Fragment load_strided(const float* row, int64_t stride, int d, int dim) {
         Fragment f;
 #pragma unroll
-        for (int j = 0; j < 4; ++j) f[j] = ok && d + j < dim ? q[(d + j) * stride] : 0.0f;
+        for (int j = 0; j < 4; ++j) f[j] = row[(d + j < dim ? d + j : 0) * stride];
         return f;
     }
-    template <bool kWide>
-    static __device__ __forceinline__ Fragment load_row(const float* row, int d, int dim, bool ok) {
-        Fragment f = {0, 0, 0, 0};
-        if constexpr (kWide) {
-            if (ok && d < dim) f = *reinterpret_cast<const f32x4*>(row + d);
-        } else {
+    static __device__ __forceinline__ Fragment zero_behind(Fragment f, int d, int dim) {
 #pragma unroll
-            for (int j = 0; j < 4; ++j)
-                if (ok && d + j < dim) f[j] = row[d + j];
-        }
+        for (int j = 0; j < 4; ++j) f[j] = d + j < dim ? f[j] : 0.0f;
         return f;
     }
-    template <int kDim, bool kWide>
-    static __device__ __forceinline__ f32x4 load_value(const float* row, int chunk, int m, int dim, bool ok) {
-        return load_row<kWide>(row, 64 * chunk + 4 * m, dim, ok);
+    template <Rows kRows>
+    static __device__ __forceinline__ Fragment load_row(const float* row, int d, int dim) {
+        if constexpr (kRows == kNarrow) return load_strided(row, 1, d, dim);
+        if constexpr (kRows == kWideRows) d = d < dim ? d : 0;
+        return *reinterpret_cast<const f32x4*>(row + d);
+    }
+    template <int kDim, Rows kRows>
+    static __device__ __forceinline__ f32x4 load_value(const float* row, int chunk, int m, int dim) {
+        return load_row<kRows>(row, 64 * chunk + 4 * m, dim);
     }
     static __device__ __forceinline__ void multiply_key(const Fragment& key, const Fragment& query, f32x4& score) {
 #pragma unroll
@@ -123,47 +127,37 @@ struct Mfma16 {
 
     static __device__ __forceinline__ uint32_t bits(T v) { return __builtin_bit_cast(uint16_t, v); }
 
-    static __device__ __forceinline__ Fragment load_query(const T* q, int64_t stride, int d, int dim, bool ok) {
+    static __device__ __forceinline__ Fragment load_strided(const T* row, int64_t stride, int d, int dim) {
         Fragment f;
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-            const uint32_t low = ok && d + 2 * j < dim ? bits(q[(d + 2 * j) * stride]) : 0;
-            const uint32_t high = ok && d + 2 * j + 1 < dim ? bits(q[(d + 2 * j + 1) * stride]) : 0;
+            const uint32_t low = bits(row[(d + 2 * j < dim ? d + 2 * j : 0) * stride]);
+            const uint32_t high = bits(row[(d + 2 * j + 1 < dim ? d + 2 * j + 1 : 0) * stride]);
             f[j] = low | high << 16;
         }
         return f;
     }
-    template <bool kWide>
-    static __device__ __forceinline__ Fragment load_row(const T* row, int d, int dim, bool ok) {
-        Fragment f = {0, 0, 0, 0};
-        if constexpr (kWide) {
-            if (ok && d < dim) f = *reinterpret_cast<const u32x4*>(row + d);
-        } else {
-            if (ok) f = load_query(row, 1, d, dim, true);
-        }
+    static __device__ __forceinline__ Fragment zero_behind(Fragment f, int d, int dim) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) f[j] &= (d + 2 * j < dim ? 0xffffu : 0u) | (d + 2 * j + 1 < dim ? 0xffff0000u : 0u);
         return f;
     }
-    template <int kDim, bool kWide>
-    static __device__ __forceinline__ u32x4 load_value(const T* row, int chunk, int m, int dim, bool ok) {
+    template <Rows kRows>
+    static __device__ __forceinline__ Fragment load_row(const T* row, int d, int dim) {
+        if constexpr (kRows == kNarrow) return load_strided(row, 1, d, dim);
+        if constexpr (kRows == kWideRows) d = d < dim ? d : 0;
+        return *reinterpret_cast<const u32x4*>(row + d);
+    }
+    template <int kDim, Rows kRows>
+    static __device__ __forceinline__ u32x4 load_value(const T* row, int chunk, int m, int dim) {
         if constexpr (kDim == 64) {
-            u32x4 f = {0, 0, 0, 0};
-            if constexpr (kWide) {
-                if (ok && 4 * m < dim) {
-                    const u32x2 half = *reinterpret_cast<const u32x2*>(row + 4 * m);
-                    f[0] = half[0];
-                    f[1] = half[1];
-                }
-            } else {
-#pragma unroll
-                for (int j = 0; j < 2; ++j) {
-                    const uint32_t low = ok && 4 * m + 2 * j < dim ? bits(row[4 * m + 2 * j]) : 0;
-                    const uint32_t high = ok && 4 * m + 2 * j + 1 < dim ? bits(row[4 * m + 2 * j + 1]) : 0;
-                    f[j] = low | high << 16;
-                }
-            }
-            return f;
+            int d = 4 * m;
+            if constexpr (kRows == kNarrow) return load_strided(row, 1, d, dim);
+            if constexpr (kRows == kWideRows) d = d < dim ? d : 0;
+            const u32x2 half = *reinterpret_cast<const u32x2*>(row + d);
+            return u32x4{half[0], half[1], 0, 0};
         } else {
-            return load_row<kWide>(row, 128 * chunk + 8 * m, dim, ok);
+            return load_row<kRows>(row, 128 * chunk + 8 * m, dim);
         }
     }
     static __device__ __forceinline__ void multiply_key(const Fragment& key, const Fragment& query, f32x4& score) {
@@ -247,5 +241,21 @@ struct Mfma<_Float16> : Mfma16<_Float16, Mfma<_Float16>> {
                                                      __builtin_bit_cast(f16x4, u32x2{b[0], b[1]}), c, 0, 0, 0);
     }
 };
+
+// The fragments of one query row, zero behind its dims, all zero unless `real` (the row's memory is valid either way).
+template <class T, int kFragments, int kStep>
+__device__ __forceinline__ void load_query(typename Mfma<T>::Fragment (&query)[kFragments], const T* row, int64_t stride,
+                                           bool wide, int first, int dim, bool real) {
+    using M = Mfma<T>;
+    if (wide) {
+#pragma unroll
+        for (int f = 0; f < kFragments; ++f) query[f] = M::template load_row<kWideRows>(row, kStep * f + first, dim);
+    } else {
+#pragma unroll
+        for (int f = 0; f < kFragments; ++f) query[f] = M::load_strided(row, stride, kStep * f + first, dim);
+    }
+#pragma unroll
+    for (int f = 0; f < kFragments; ++f) query[f] = M::zero_behind(query[f], kStep * f + first, real ? dim : 0);
+}
 
 }  // namespace flux

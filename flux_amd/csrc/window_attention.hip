@@ -137,7 +137,7 @@ struct KeyTiles {
     __device__ __forceinline__ int base(int t) const { return (t < sink_tiles ? t : first_tile + t - sink_tiles) * kTile; }
 };
 
-template <int kDim, bool kWide>
+template <int kDim, Rows kRowsRead>
 __global__ void __launch_bounds__(kThreads, kDim <= 64 ? 2 : 1) window_attention_kernel(AttentionArgs a, int row_tiles, int tiles_total) {
     using M = Mfma<float>;
     constexpr int kCols = kDim == 256 ? 1 : 2;  // tiles of 16 rows
@@ -168,17 +168,13 @@ __global__ void __launch_bounds__(kThreads, kDim <= 64 ? 2 : 1) window_attention
 #pragma unroll
     for (int c = 0; c < kCols; ++c) {
         const int r = rows.row0 + 16 * c + n16;
+        const bool real = r < rows.all_rows;
         int64_t i, head;
-        rows.place(a, r, i, head);
+        rows.place(a, real ? r : rows.row0, i, head);
         mine[c] = rows.range(a, r, i);
         sink_end[c] = a.sinks < mine[c].low ? a.sinks : mine[c].low;
         const float* q = static_cast<const float*>(a.query) + rows.b * a.query_strides[0] + head * a.query_strides[1] + i * a.query_strides[2];
-#pragma unroll
-        for (int f = 0; f < kFragments; ++f) {
-            const int d = M::kKeyStep * f + M::kPer * g;
-            if (a.query_wide) query[c][f] = M::template load_row<true>(q, d, a.dim, r < rows.all_rows);
-            else query[c][f] = M::load_query(q, a.query_strides[3], d, a.dim, r < rows.all_rows);
-        }
+        load_query<float, kFragments, M::kKeyStep>(query[c], q, a.query_strides[3], a.query_wide, M::kPer * g, a.dim, real);
 #pragma unroll
         for (int k = 0; k < kBlocks; ++k) out[c][k] = f32x4{0, 0, 0, 0};
         top[c] = -INFINITY;
@@ -193,22 +189,23 @@ __global__ void __launch_bounds__(kThreads, kDim <= 64 ? 2 : 1) window_attention
         f32x4 key[kSubs][kFragments];
         f32x4 value[kSubs][4][kChunks];
     };
+    // Rows behind the last key repeat it: their weights are zero.
     auto load = [&](int t, Tile& into) {
-        const int base = tiles.base(t), end = t < tiles.count ? tiles.seen : 0;
+        const int base = tiles.base(t), end = tiles.seen - 1;
 #pragma unroll
         for (int s = 0; s < kSubs; ++s) {
             const int position = base + 16 * s + n16;
-            const float* k = keys + position * a.key_strides[2];
+            const float* k = keys + (position < end ? position : end) * a.key_strides[2];
 #pragma unroll
             for (int f = 0; f < kFragments; ++f)
-                into.key[s][f] = M::template load_row<kWide>(k, M::kKeyStep * f + M::kPer * g, a.dim, position < end);
+                into.key[s][f] = M::template load_row<kRowsRead>(k, M::kKeyStep * f + M::kPer * g, a.dim);
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
                 const int value_position = base + 16 * s + 4 * g + i;
-                const float* v = values + value_position * a.value_strides[2];
+                const float* v = values + (value_position < end ? value_position : end) * a.value_strides[2];
 #pragma unroll
                 for (int c = 0; c < kChunks; ++c)
-                    into.value[s][i][c] = M::template load_value<kDim, kWide>(v, c, n16, a.dim, value_position < end);
+                    into.value[s][i][c] = M::template load_value<kDim, kRowsRead>(v, c, n16, a.dim);
             }
         }
     };
@@ -258,20 +255,22 @@ __global__ void __launch_bounds__(kThreads, kDim <= 64 ? 2 : 1) window_attention
         }
     };
 
-    // Two tiles in registers where two waves per SIMD still fit.
+    // Two tiles in registers where two waves per SIMD still fit.  A wave's tile numbers are the same in all its lanes.
+    const int first_tile = __builtin_amdgcn_readfirstlane(wave);
     Tile even;
     if constexpr (kDim <= 64) {
         Tile odd;
-        load(wave, even);
-        for (int t = wave; t < tiles.count; t += 2 * kWaves) {
-            load(t + kWaves, odd);
+        if (first_tile < tiles.count) load(first_tile, even);
+        for (int t = first_tile; t < tiles.count; t += 2 * kWaves) {
+            const bool second = t + kWaves < tiles.count;
+            if (second) load(t + kWaves, odd);
             work(t, even);
-            if (t + kWaves >= tiles.count) break;
-            load(t + 2 * kWaves, even);
+            if (!second) break;
+            if (t + 2 * kWaves < tiles.count) load(t + 2 * kWaves, even);
             work(t + kWaves, odd);
         }
     } else {
-        for (int t = wave; t < tiles.count; t += kWaves) {
+        for (int t = first_tile; t < tiles.count; t += kWaves) {
             load(t, even);
             work(t, even);
         }
@@ -391,7 +390,7 @@ __device__ __forceinline__ float half_sum(float v) {
 }
 
 // Rows of one stage.  With kWide 16 bytes at a byte offset through a buffer that ends with the last row (kStagedStride
-// keeps offsets in 31 bits); else eight elements by comparisons.
+// keeps offsets in 31 bits); else eight elements, of the last row where there is none.
 template <class T, bool kWide>
 struct StagedRows {
     const T* base;
@@ -402,7 +401,7 @@ struct StagedRows {
     }
     __device__ __forceinline__ u32x4 load(int at, int row, int d, int rows, int64_t stride, int dim) const {
         if constexpr (kWide) return __builtin_amdgcn_raw_buffer_load_b128(buffer, at, 0, 0);
-        return Mfma<T>::load_query(base + row * stride, 1, d, dim, row < rows);
+        return Mfma<T>::load_strided(base + (row < rows ? row : rows - 1) * stride, 1, d, dim);
     }
 };
 
@@ -452,18 +451,15 @@ window_tile_kernel(AttentionArgs a, int row_tiles, int tiles_total) {
 #pragma unroll
     for (int c = 0; c < kRowTiles; ++c) {
         const int r = wave_row + 32 * c + n32;
+        const bool real = r < rows.all_rows;
         int64_t i, head;
-        rows.place(a, r, i, head);
+        rows.place(a, real ? r : rows.row0, i, head);
         mine[c] = rows.range(a, r, i);
         sink_end[c] = a.sinks < mine[c].low ? a.sinks : mine[c].low;
         const T* q = static_cast<const T*>(a.query) + rows.b * a.query_strides[0] + head * a.query_strides[1] + i * a.query_strides[2];
+        load_query<T, kSteps, 16>(query[c], q, a.query_strides[3], a.query_wide, 8 * half, a.dim, real);
 #pragma unroll
-        for (int s = 0; s < kSteps; ++s) {
-            const int d = 16 * s + 8 * half;
-            if (a.query_wide) query[c][s] = Mfma<T>::template load_row<true>(q, d, a.dim, r < rows.all_rows);
-            else query[c][s] = Mfma<T>::load_query(q, a.query_strides[3], d, a.dim, r < rows.all_rows);
-            query[c][s] ^= sign;
-        }
+        for (int s = 0; s < kSteps; ++s) query[c][s] ^= sign;
 #pragma unroll
         for (int i = 0; i < kBlocks; ++i)
 #pragma unroll
@@ -477,8 +473,8 @@ window_tile_kernel(AttentionArgs a, int row_tiles, int tiles_total) {
         const int seen = tiles.seen, count = tiles.count;
         auto low_of = [&](int p) { return a.window > 0 && p >= a.window ? p - a.window + 1 : 0; };
 
-        // Rows behind the last key give zeros (a buffer's range check, or a comparison), dims behind the head's repeat its
-        // first: they meet a zero in the query or are not stored.
+        // Rows behind the last key are zeros (a buffer's range check) or repeat it, and weigh nothing; dims behind the head's
+        // repeat its first ones, which meet a zero in the query or are not stored.
         u32x4 held_key[kKeyLoads];
         u32x4 held_value[kValueLoads][4];
         const int key_row = threadIdx.x / (kDim / 8), key_d = threadIdx.x % (kDim / 8) * 8;
@@ -710,8 +706,10 @@ hipError_t launch_window(const AttentionArgs& a, hipStream_t stream) {
         const int64_t tiles = row_tiles * a.kv_heads * a.batch;
         if (tiles >= (int64_t{1} << 24) - 256) return hipErrorInvalidValue;  // a grid has below 2^32 threads
         const dim3 grid(static_cast<uint32_t>(blocks_of_tiles(tiles)));
-        if (a.wide) hipLaunchKernelGGL(HIP_KERNEL_NAME(window_attention_kernel<kDim, true>), grid, dim3(kThreads), 0, stream, a, static_cast<int>(row_tiles), static_cast<int>(tiles));
-        else hipLaunchKernelGGL(HIP_KERNEL_NAME(window_attention_kernel<kDim, false>), grid, dim3(kThreads), 0, stream, a, static_cast<int>(row_tiles), static_cast<int>(tiles));
+        const int in_row = static_cast<int>(row_tiles), all = static_cast<int>(tiles);
+        if (a.wide && a.dim == kDim) hipLaunchKernelGGL(HIP_KERNEL_NAME(window_attention_kernel<kDim, kFullRows>), grid, dim3(kThreads), 0, stream, a, in_row, all);
+        else if (a.wide) hipLaunchKernelGGL(HIP_KERNEL_NAME(window_attention_kernel<kDim, kWideRows>), grid, dim3(kThreads), 0, stream, a, in_row, all);
+        else hipLaunchKernelGGL(HIP_KERNEL_NAME(window_attention_kernel<kDim, kNarrow>), grid, dim3(kThreads), 0, stream, a, in_row, all);
         return hipGetLastError();
     }
 }
