@@ -138,11 +138,11 @@ struct KeyTiles {
 };
 
 template <int kDim, Rows kRowsRead>
-__global__ void __launch_bounds__(kThreads, kDim <= 64 ? 2 : 1) window_attention_kernel(AttentionArgs a, int row_tiles, int tiles_total) {
+__global__ void __launch_bounds__(kThreads, kDim <= 64 ? 4 : (kDim <= 128 ? 2 : 1)) window_attention_kernel(AttentionArgs a, int row_tiles, int tiles_total) {
     using M = Mfma<float>;
     constexpr int kCols = kDim == 256 ? 1 : 2;  // tiles of 16 rows
     constexpr int kRows = 16 * kCols;
-    constexpr int kTile = kDim <= 64 ? 32 : 16;
+    constexpr int kTile = 16;
     constexpr int kSubs = kTile / 16;
     constexpr int kFragments = M::template key_fragments<kDim>();
     constexpr int kChunks = M::template value_chunks<kDim>();
@@ -255,25 +255,13 @@ __global__ void __launch_bounds__(kThreads, kDim <= 64 ? 2 : 1) window_attention
         }
     };
 
-    // Two tiles in registers where two waves per SIMD still fit.  A wave's tile numbers are the same in all its lanes.
-    const int first_tile = __builtin_amdgcn_readfirstlane(wave);
-    Tile even;
-    if constexpr (kDim <= 64) {
-        Tile odd;
-        if (first_tile < tiles.count) load(first_tile, even);
-        for (int t = first_tile; t < tiles.count; t += 2 * kWaves) {
-            const bool second = t + kWaves < tiles.count;
-            if (second) load(t + kWaves, odd);
-            work(t, even);
-            if (!second) break;
-            if (t + 2 * kWaves < tiles.count) load(t + 2 * kWaves, even);
-            work(t + kWaves, odd);
-        }
-    } else {
-        for (int t = first_tile; t < tiles.count; t += kWaves) {
-            load(t, even);
-            work(t, even);
-        }
+    // Many waves with one small tile each do better than few with two larger ones in flight (4096 tokens, 9 / 3 heads of 64,
+    // window 1024: 16 keys and four waves per SIMD 110 us, three 115; 32 keys, one more in flight, two waves 132).  A wave's
+    // tile numbers are the same in all its lanes.
+    Tile held;
+    for (int t = __builtin_amdgcn_readfirstlane(wave); t < tiles.count; t += kWaves) {
+        load(t, held);
+        work(t, held);
     }
 
 #pragma unroll
