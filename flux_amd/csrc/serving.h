@@ -69,6 +69,7 @@ struct AttentionArgs {
     bool wide;               // every key and value row starts at 16 bytes and dim fills whole 16-byte quads
     bool query_wide;         // the same of query rows, with a dim stride of 1
     int blocks;              // workgroups over the keys, per KV head and column tile
+    int least;               // tiles below which a sequence is not cut
 };
 
 int decode_attention_blocks(int batch, int64_t keys, int kv_heads, int group, int window, int sinks);
