@@ -61,6 +61,11 @@ __device__ void exact_row(const AttentionArgs& a, const T* query, const T* keys,
             for (int c = 0; c < kServingMaxDim / kWave; ++c)
                 if (kWave * c + lane < a.dim) sum[c] = fmaf(pj, static_cast<float>(value[kWave * c + lane]), sum[c]);
         }
+        // What is NaN stays NaN: a row whose sums all are is done.
+        bool lost = true;
+#pragma unroll
+        for (int c = 0; c < kServingMaxDim / kWave; ++c) lost = lost && (kWave * c + lane >= a.dim || sum[c] != sum[c]);
+        if (__all(weight != weight || lost)) break;
     }
 #pragma unroll
     for (int c = 0; c < kServingMaxDim / kWave; ++c)
@@ -671,9 +676,9 @@ hipError_t launch_window_tiles(const AttentionArgs& a, hipStream_t stream) {
     const int row_tiles = static_cast<int>((rows + kRows - 1) / kRows);
     const int64_t tiles = static_cast<int64_t>(row_tiles) * a.kv_heads * a.batch;
     if (tiles >= (int64_t{1} << 24) - 256) return hipErrorInvalidValue;  // a grid has below 2^32 threads
-    static const hipError_t room = hipFuncSetAttribute(
-        reinterpret_cast<const void*>(window_tile_kernel<T, kDim, kRowTiles, kWide>), hipFuncAttributeMaxDynamicSharedMemorySize,
-        static_cast<int>(kLds));
+    const hipError_t room = hipFuncSetAttribute(
+        reinterpret_cast<const void*>(window_tile_kernel<T, kDim, kRowTiles, kWide>),
+        hipFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(kLds));
     if (room != hipSuccess) return room;
     hipLaunchKernelGGL(HIP_KERNEL_NAME(window_tile_kernel<T, kDim, kRowTiles, kWide>),
                        dim3(static_cast<uint32_t>(blocks_of_tiles(tiles))), dim3(kThreads), kLds, stream, a, row_tiles,

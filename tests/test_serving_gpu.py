@@ -353,6 +353,17 @@ def test_window_nan_reaches_only_the_rows_that_see_it(gpu_device, dtype, dim):
                     assert torch.equal(out[0, :2, i].isnan(), expected[0, :2, i].isnan()), (name, bad, at, i)
 
 
+def test_window_rows_that_are_all_nan(gpu_device):
+    case = _to(_window_case(29, torch.bfloat16, 1, 4, 2, 64, 700, 700), gpu_device)
+    for name in ("key", "value"):
+        dirty = {**case, name: torch.full_like(case[name], math.nan)}
+        assert bool(ops.window_attention_native(**dirty, window=300, sinks=2).isnan().all())
+    half = {**case, "value": case["value"].clone()}
+    half["value"][..., ::2] = math.inf  # every dim of every row sees one; the others stay finite
+    out = ops.window_attention_native(**half, window=300, sinks=2)
+    assert bool(out[..., 1::2].isfinite().all()) and not bool(out[..., ::2].isfinite().any())
+
+
 def test_window_other_stream_and_graph(gpu_device):
     case = _to(_window_case(33, torch.bfloat16, 2, 8, 2, 64, 90, 90), gpu_device)
     lengths, starts = torch.tensor([90, 40], device=gpu_device), torch.zeros(2, dtype=torch.int64, device=gpu_device)
@@ -640,6 +651,17 @@ def test_opcheck(gpu_device):
                       tuple(_to(_window_case(1, torch.float32, 2, 4, 2, 64, 5, 9), gpu_device).values()) + (4,)),
                      (torch.ops.flux.logits_process.default, (torch.randn(2, 100, device=gpu_device),))):
         result = torch.library.opcheck(op, args)
+        assert all(status == "SUCCESS" for status in result.values()), result
+    pages = _Device(ref.Pages(2, 9, 2, 4, 8, 3, 4), gpu_device)
+    pools, ids = (pages.key, pages.value), pages.ids([0, 2])
+    rows = torch.randn(2, 2, 3, 8, device=gpu_device)
+    for op, args in ((torch.ops.flux.paged_cache_reserve, (*pages.books, 4, ids, pages.ids([3, 5]))),
+                     (torch.ops.flux.paged_cache_write, (rows, -rows, pages.key[0], pages.value[0], pages.table, ids, ids)),
+                     (torch.ops.flux.paged_cache_copy, (*pools, ids, ids + 1)),
+                     (torch.ops.flux.paged_cache_fork, (*pools, *pages.books, ids[:1], ids[:1] + 1)),
+                     (torch.ops.flux.paged_cache_free, (*pages.books, ids)),
+                     (torch.ops.flux.paged_cache_compact, (*pools, pages.table, pages.refcounts))):
+        result = torch.library.opcheck(op.default, args, test_utils=("test_schema", "test_faketensor"))
         assert all(status == "SUCCESS" for status in result.values()), result
 
 
