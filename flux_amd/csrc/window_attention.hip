@@ -331,7 +331,10 @@ __global__ void __launch_bounds__(kThreads, kDim <= 64 ? 4 : (kDim <= 128 ? 2 : 
 
 // ---------------------------------------------------------------------------
 // 16-bit prompts.  Here matrix instructions, exponentials and LDS reads cost about the same, so that keys and values are
-// staged once for the workgroup's four waves and each operand read from LDS serves kRowTiles x 32 rows.
+// staged once for the workgroup's four waves, 32 rows each.  4 x 4096 tokens (padded), 32 / 8 heads of 128, window 1024 in
+// bfloat16: 240 us, 700 TFLOP/s.  A 32 x 32 tile costs a SIMD 512 cycles of matrix instructions and as many of vector
+// instructions (half of them exponentials), and the two waves of a SIMD overlap them in part: 64 rows a wave (one wave
+// per SIMD) took 640 us, a workgroup of eight waves 236, two tiles per maximum 244.
 //
 // A stage holds kKeys keys: K rows as they are, V transposed (the staging thread permutes the 16-bit halves of four
 // keys), its keys in the order in which a lane's scores lie.  S^T = K Q^T on 32 x 32 tiles leaves lane (n, h) with the
@@ -398,22 +401,20 @@ struct StagedRows {
     }
 };
 
-template <class T, int kDim, int kRowTiles, bool kWide>
-__global__ void __launch_bounds__(kThreads, kRowTiles == 1 && kDim <= 128 ? 2 : 1)
+template <class T, int kDim, bool kWide>
+__global__ void __launch_bounds__(kThreads, kDim <= 128 ? 2 : 1)
 window_tile_kernel(AttentionArgs a, int row_tiles, int tiles_total) {
     using W = Wide<T>;
     constexpr int kKeys = kDim == 64 ? 128 : (kDim == 128 ? 64 : 32);
     constexpr int kSubs = kKeys / 32;
-    constexpr int kJoint = 1;
     constexpr int kSteps = kDim / 16;             // of a score
     constexpr int kBlocks = kDim / 32;            // of the result
-    constexpr int kRows = kWaves * kRowTiles * 32;
+    constexpr int kRows = kWaves * 32;
     constexpr int kKeyRow = kDim * 2 + 16;        // bytes
     constexpr int kValueRow = kKeys * 2 + 16;
     constexpr int kStage = kKeys * kKeyRow + kDim * kValueRow;
     constexpr int kKeyLoads = kKeys * kDim / 8 / kThreads;        // 16 bytes per thread
-    constexpr int kValueUnits = kKeys / 4 * (kDim / 8);           // 4 keys x 8 dims
-    constexpr int kValueLoads = (kValueUnits + kThreads - 1) / kThreads;
+    static_assert(kKeys / 4 * (kDim / 8) == kThreads, "every thread stages four keys by eight dims of the values");
     constexpr float kLazy = 8.0f;
     extern __shared__ char stages[];
 
@@ -426,40 +427,34 @@ window_tile_kernel(AttentionArgs a, int row_tiles, int tiles_total) {
     const int half = lane >> 5;
     int block_first, block_last, wave_first, wave_last;
     rows.positions(a, rows.row0, kRows, block_first, block_last);
-    const int wave_row = rows.row0 + wave * kRowTiles * 32;
-    rows.positions(a, wave_row, kRowTiles * 32, wave_first, wave_last);
+    const int wave_row = rows.row0 + wave * 32;
+    rows.positions(a, wave_row, 32, wave_first, wave_last);
     wave_first = __builtin_amdgcn_readfirstlane(wave_first);
     wave_last = __builtin_amdgcn_readfirstlane(wave_last);
 
     const T* keys = static_cast<const T*>(a.key) + rows.b * a.key_strides[0] + rows.kv_head * a.key_strides[1];
     const T* values = static_cast<const T*>(a.value) + rows.b * a.value_strides[0] + rows.kv_head * a.value_strides[1];
 
-    RowRange mine[kRowTiles];
-    int sink_end[kRowTiles];
-    u32x4 query[kRowTiles][kSteps];
-    f32x16 out[kRowTiles][kBlocks];
-    float top[kRowTiles], weight[kRowTiles];
+    const int r = wave_row + n32;  // this lane's row
+    const bool real = r < rows.all_rows;
+    int64_t query_index, head;
+    rows.place(a, real ? r : rows.row0, query_index, head);
+    const RowRange mine = rows.range(a, r, query_index);
+    const int sink_end = a.sinks < mine.low ? a.sinks : mine.low;
     const uint32_t sign = a.scale < 0.0f ? 0x80008000u : 0u;  // the scale's sign goes to the query
     const float factor = fmaxf(fabsf(a.scale) * kLog2e, 1e-37f);  // above 0: a masked score stays -inf
+    u32x4 query[kSteps];
+    load_query<T, kSteps, 16>(query, static_cast<const T*>(a.query) + rows.b * a.query_strides[0] + head * a.query_strides[1] +
+                                         query_index * a.query_strides[2],
+                              a.query_strides[3], a.query_wide, 8 * half, a.dim, real);
 #pragma unroll
-    for (int c = 0; c < kRowTiles; ++c) {
-        const int r = wave_row + 32 * c + n32;
-        const bool real = r < rows.all_rows;
-        int64_t i, head;
-        rows.place(a, real ? r : rows.row0, i, head);
-        mine[c] = rows.range(a, r, i);
-        sink_end[c] = a.sinks < mine[c].low ? a.sinks : mine[c].low;
-        const T* q = static_cast<const T*>(a.query) + rows.b * a.query_strides[0] + head * a.query_strides[1] + i * a.query_strides[2];
-        load_query<T, kSteps, 16>(query[c], q, a.query_strides[3], a.query_wide, 8 * half, a.dim, real);
+    for (int s = 0; s < kSteps; ++s) query[s] ^= sign;
+    f32x16 out[kBlocks];
 #pragma unroll
-        for (int s = 0; s < kSteps; ++s) query[c][s] ^= sign;
+    for (int i = 0; i < kBlocks; ++i)
 #pragma unroll
-        for (int i = 0; i < kBlocks; ++i)
-#pragma unroll
-            for (int j = 0; j < 16; ++j) out[c][i][j] = 0.0f;
-        top[c] = -INFINITY;
-        weight[c] = 0.0f;
-    }
+        for (int j = 0; j < 16; ++j) out[i][j] = 0.0f;
+    float top = -INFINITY, weight = 0.0f;
 
     if (block_first <= block_last) {
         const KeyTiles<kKeys> tiles(a, block_first, block_last);
@@ -469,11 +464,10 @@ window_tile_kernel(AttentionArgs a, int row_tiles, int tiles_total) {
         // Rows behind the last key are zeros (a buffer's range check) or repeat it, and weigh nothing; dims behind the head's
         // repeat its first ones, which meet a zero in the query or are not stored.
         u32x4 held_key[kKeyLoads];
-        u32x4 held_value[kValueLoads][4];
+        u32x4 held_value[4];
         const int key_row = threadIdx.x / (kDim / 8), key_d = threadIdx.x % (kDim / 8) * 8;
         const int value_row = threadIdx.x % (kKeys / 4) * 4, value_d = threadIdx.x / (kKeys / 4) * 8;
         constexpr int kKeyRows = kThreads / (kDim / 8);  // rows that one load of all threads covers
-        static_assert(kValueLoads == 1, "one unit of values per thread");
         const int key_stride = static_cast<int>(a.key_strides[2]), value_stride = static_cast<int>(a.value_strides[2]);
         const int key_at = (key_row * key_stride + (key_d < a.dim ? key_d : 0)) * 2;
         const int value_at = (value_row * value_stride + (value_d < a.dim ? value_d : 0)) * 2;
@@ -491,7 +485,7 @@ window_tile_kernel(AttentionArgs a, int row_tiles, int tiles_total) {
             const StagedRows<T, kWide> staged(from, ((rows - 1) * a.value_strides[2] + a.dim) * 2);
 #pragma unroll
             for (int j = 0; j < 4; ++j)
-                held_value[0][j] = staged.load(value_at + j * value_stride * 2, value_row + j, value_d, rows, a.value_strides[2], a.dim);
+                held_value[j] = staged.load(value_at + j * value_stride * 2, value_row + j, value_d, rows, a.value_strides[2], a.dim);
         };
         auto put_keys = [&](char* stage) {
 #pragma unroll
@@ -502,21 +496,13 @@ window_tile_kernel(AttentionArgs a, int row_tiles, int tiles_total) {
         };
         auto put_values = [&](char* stage) {
             char* turned = stage + kKeys * kKeyRow;
+            // Quads 0, 1, 2, 3 of 16 keys lie as 0, 2, 1, 3: a lane's eight keys side by side.
+            const int quad = value_row / 4, at = (quad & ~3) | (quad & 1) << 1 | (quad >> 1 & 1);
 #pragma unroll
-            for (int i = 0; i < kValueLoads; ++i) {
-                const int unit = threadIdx.x + kThreads * i;
-                const int quad = unit % (kKeys / 4), d = unit / (kKeys / 4) * 8;
-                // Quads 0, 1, 2, 3 of 16 keys lie as 0, 2, 1, 3: a lane's eight keys side by side.
-                const int at = (quad & ~3) | (quad & 1) << 1 | (quad >> 1 & 1);
-                if (unit < kValueUnits) {
-#pragma unroll
-                    for (int j = 0; j < 8; ++j) {
-                        const u32x2 four = {Mfma<T>::pair(held_value[i][0][j / 2], held_value[i][1][j / 2], j & 1),
-                                            Mfma<T>::pair(held_value[i][2][j / 2], held_value[i][3][j / 2], j & 1)};
-                        *reinterpret_cast<u32x2*>(turned + (d + j) * kValueRow + at * 8) = four;
-                    }
-                }
-            }
+            for (int j = 0; j < 8; ++j)
+                *reinterpret_cast<u32x2*>(turned + (value_d + j) * kValueRow + at * 8) =
+                    u32x2{Mfma<T>::pair(held_value[0][j / 2], held_value[1][j / 2], j & 1),
+                          Mfma<T>::pair(held_value[2][j / 2], held_value[3][j / 2], j & 1)};
         };
 
         const int wave_low = low_of(wave_first), low_of_last = low_of(wave_last);
@@ -532,155 +518,123 @@ window_tile_kernel(AttentionArgs a, int row_tiles, int tiles_total) {
             char* next = stages + ((t + 1) & 1) * kStage;
             if (t + 1 < count) fetch_keys(t + 1);
 #pragma unroll
-            for (int s0 = 0; s0 < kSubs; s0 += kJoint) {
-                const int first = base + 32 * s0, last = first + 32 * kJoint - 1;
-                // Nothing of this wave's rows sees these keys.
-                if (s0 == kSubs / 2 && t + 1 < count) {
+            for (int s = 0; s < kSubs; ++s) {
+                if (s == kSubs / 2 && t + 1 < count) {  // K and V take the same registers on their way
                     put_keys(next);
                     fetch_values(t + 1);
                 }
+                const int first = base + 32 * s, last = first + 31;
+                // Nothing of this wave's rows sees these keys.
                 if (first > wave_last || (last < wave_low && first >= a.sinks)) continue;
-                f32x16 score[kJoint][kRowTiles];
+                u32x4 key[kSteps];
 #pragma unroll
-                for (int s = 0; s < kJoint; ++s) {
+                for (int k = 0; k < kSteps; ++k)
+                    key[k] = *reinterpret_cast<const u32x4*>(stage + (32 * s + n32) * kKeyRow + 32 * k + 16 * half);
+                __builtin_amdgcn_sched_barrier(0);  // all reads first: one wait
+                f32x16 score;
 #pragma unroll
-                    for (int c = 0; c < kRowTiles; ++c)
+                for (int j = 0; j < 16; ++j) score[j] = 0.0f;
 #pragma unroll
-                        for (int j = 0; j < 16; ++j) score[s][c][j] = 0.0f;
-                    u32x4 key[kSteps];
+                for (int k = 0; k < kSteps; ++k) score = W::multiply(key[k], query[k], score);
+                if (first < low_of_last || last > wave_first) {
 #pragma unroll
-                    for (int k = 0; k < kSteps; ++k)
-                        key[k] = *reinterpret_cast<const u32x4*>(stage + (32 * (s0 + s) + n32) * kKeyRow + 32 * k + 16 * half);
-                    __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-                    for (int k = 0; k < kSteps; ++k)
-#pragma unroll
-                        for (int c = 0; c < kRowTiles; ++c) score[s][c] = W::multiply(key[k], query[c][k], score[s][c]);
-                }
-                const bool inside = first >= low_of_last && last <= wave_first;
-                u32x4 p[kJoint][kRowTiles][2];
-#pragma unroll
-                for (int c = 0; c < kRowTiles; ++c) {
-                    if (!inside) {
-#pragma unroll
-                        for (int s = 0; s < kJoint; ++s)
-#pragma unroll
-                            for (int j = 0; j < 16; ++j) {
-                                // Without branches: low <= key <= position as one unsigned comparison, or a sink.
-                                const int key = first + 32 * s + 8 * (j / 4) + 4 * half + j % 4;
-                                const bool visible = (static_cast<uint32_t>(key - mine[c].low) <=
-                                                      static_cast<uint32_t>(mine[c].position - mine[c].low)) |
-                                                     (key < sink_end[c]);
-                                score[s][c][j] = visible ? score[s][c][j] : -INFINITY;
-                            }
-                    }
-                    float highest = score[0][c][0];
-#pragma unroll
-                    for (int s = 0; s < kJoint; ++s)
-#pragma unroll
-                        for (int j = 0; j < 16; ++j) highest = fmaxf(highest, score[s][c][j]);
-                    highest = half_max(highest) * factor;
-                    if (__any(highest > top[c] + kLazy)) {
-                        const float now = fmaxf(top[c], highest);
-                        const float shrink = top[c] == -INFINITY ? 0.0f : fast_exp2(top[c] - now);
-                        top[c] = now;
-                        weight[c] *= shrink;
-#pragma unroll
-                        for (int i = 0; i < kBlocks; ++i)
-#pragma unroll
-                            for (int j = 0; j < 16; ++j) out[c][i][j] *= shrink;
+                    for (int j = 0; j < 16; ++j) {
+                        // Without branches: low <= key <= position as one unsigned comparison, or a sink.
+                        const int of = first + 8 * (j / 4) + 4 * half + j % 4;
+                        const bool visible = (static_cast<uint32_t>(of - mine.low) <= static_cast<uint32_t>(mine.position - mine.low)) |
+                                             (of < sink_end);
+                        score[j] = visible ? score[j] : -INFINITY;
                     }
                 }
+                float highest = score[0];
 #pragma unroll
-                for (int s = 0; s < kJoint; ++s) {
-                    u32x4 value[kBlocks][2];
+                for (int j = 1; j < 16; ++j) highest = fmaxf(highest, score[j]);
+                highest = half_max(highest) * factor;
+                if (__any(highest > top + kLazy)) {
+                    const float now = fmaxf(top, highest);
+                    const float shrink = top == -INFINITY ? 0.0f : fast_exp2(top - now);
+                    top = now;
+                    weight *= shrink;
 #pragma unroll
                     for (int i = 0; i < kBlocks; ++i)
 #pragma unroll
-                        for (int k = 0; k < 2; ++k)
-                            value[i][k] = *reinterpret_cast<const u32x4*>(turned + (32 * i + n32) * kValueRow +
-                                                                          (32 * (s0 + s) + 16 * k) * 2 + 16 * half);
-                    __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-                    for (int c = 0; c < kRowTiles; ++c) {
-                        const float reference = W::kShift - (top[c] == -INFINITY ? 0.0f : top[c]);
-#pragma unroll
-                        for (int j = 0; j < 16; j += 2) {
-                            const float p0 = fast_exp2(fmaf(score[s][c][j], factor, reference));
-                            const float p1 = fast_exp2(fmaf(score[s][c][j + 1], factor, reference));
-                            weight[c] += p0 + p1;
-                            p[s][c][j / 8][j % 8 / 2] = W::round(p0, p1);
-                        }
-                    }
-#pragma unroll
-                    for (int i = 0; i < kBlocks; ++i)
-#pragma unroll
-                        for (int k = 0; k < 2; ++k)
-#pragma unroll
-                            for (int c = 0; c < kRowTiles; ++c) out[c][i] = W::multiply(value[i][k], p[s][c][k], out[c][i]);
+                        for (int j = 0; j < 16; ++j) out[i][j] *= shrink;
                 }
+                u32x4 value[kBlocks][2];
+#pragma unroll
+                for (int i = 0; i < kBlocks; ++i)
+#pragma unroll
+                    for (int k = 0; k < 2; ++k)
+                        value[i][k] = *reinterpret_cast<const u32x4*>(turned + (32 * i + n32) * kValueRow + (32 * s + 16 * k) * 2 + 16 * half);
+                __builtin_amdgcn_sched_barrier(0);
+                const float reference = W::kShift - (top == -INFINITY ? 0.0f : top);
+                u32x4 p[2];
+#pragma unroll
+                for (int j = 0; j < 16; j += 2) {
+                    const float p0 = fast_exp2(fmaf(score[j], factor, reference));
+                    const float p1 = fast_exp2(fmaf(score[j + 1], factor, reference));
+                    weight += p0 + p1;
+                    p[j / 8][j % 8 / 2] = W::round(p0, p1);
+                }
+#pragma unroll
+                for (int i = 0; i < kBlocks; ++i)
+#pragma unroll
+                    for (int k = 0; k < 2; ++k) out[i] = W::multiply(value[i][k], p[k], out[i]);
             }
             if (t + 1 < count) put_values(next);
         }
     }
 
+    weight = half_sum(weight);
+    float worst = fabsf(weight);
 #pragma unroll
-    for (int c = 0; c < kRowTiles; ++c) {
-        weight[c] = half_sum(weight[c]);
-        float worst = fabsf(weight[c]);
+    for (int i = 0; i < kBlocks; ++i)
+#pragma unroll
+        for (int j = 0; j < 16; ++j) worst += fabsf(out[i][j]);  // keeps NaN, infinity
+    const uint64_t odd = __ballot(mine.position >= 0 && !(worst < INFINITY));
+    uint32_t again = static_cast<uint32_t>(odd | odd >> 32);
+    if (real && !(again >> n32 & 1)) {
+        T* o = static_cast<T*>(a.out) + ((rows.b * a.query_heads + head) * a.queries + query_index) * a.dim;
+        const float inverse = 1.0f / weight;
 #pragma unroll
         for (int i = 0; i < kBlocks; ++i)
 #pragma unroll
-            for (int j = 0; j < 16; ++j) worst += fabsf(out[c][i][j]);  // keeps NaN, infinity
-        const uint64_t odd = __ballot(mine[c].position >= 0 && !(worst < INFINITY));
-        uint32_t again = static_cast<uint32_t>(odd | odd >> 32);
-        const int r = wave_row + 32 * c + n32;
-        if (r < rows.all_rows && !(again >> n32 & 1)) {
-            int64_t i, head;
-            rows.place(a, r, i, head);
-            T* o = static_cast<T*>(a.out) + ((rows.b * a.query_heads + head) * a.queries + i) * a.dim;
-            const float inverse = mine[c].position < 0 ? 0.0f : 1.0f / weight[c];
+            for (int j = 0; j < 16; j += 4) {
+                const int d = 32 * i + 2 * j + 4 * half;  // four dims side by side
+                float four[4];
 #pragma unroll
-            for (int k = 0; k < kBlocks; ++k)
+                for (int l = 0; l < 4; ++l) four[l] = mine.position < 0 ? 0.0f : out[i][j + l] * inverse;
+                const u32x2 rounded = {W::round(four[0], four[1]), W::round(four[2], four[3])};
+                if constexpr (kWide) {
+                    if (d < a.dim) *reinterpret_cast<u32x2*>(o + d) = rounded;
+                } else {
 #pragma unroll
-                for (int j = 0; j < 16; j += 4) {
-                    const int d = 32 * k + 2 * j + 4 * half;  // four dims side by side
-                    float four[4];
-#pragma unroll
-                    for (int l = 0; l < 4; ++l) four[l] = mine[c].position < 0 ? 0.0f : out[c][k][j + l] * inverse;
-                    const u32x2 rounded = {W::round(four[0], four[1]), W::round(four[2], four[3])};
-                    if constexpr (kWide) {
-                        if (d < a.dim) *reinterpret_cast<u32x2*>(o + d) = rounded;
-                    } else {
-#pragma unroll
-                        for (int l = 0; l < 4; ++l)
-                            if (d + l < a.dim)
-                                o[d + l] = __builtin_bit_cast(T, static_cast<uint16_t>(rounded[l / 2] >> 16 * (l % 2)));
-                    }
+                    for (int l = 0; l < 4; ++l)
+                        if (d + l < a.dim) o[d + l] = __builtin_bit_cast(T, static_cast<uint16_t>(rounded[l / 2] >> 16 * (l % 2)));
                 }
-        }
-        while (again) {
-            const int which = __ffs(again) - 1;
-            again &= again - 1;
-            rows.template again<T>(a, wave_row + 32 * c + which, keys, values);
-        }
+            }
+    }
+    while (again) {
+        const int which = __ffs(again) - 1;
+        again &= again - 1;
+        rows.template again<T>(a, wave_row + which, keys, values);
     }
 }
 
-template <class T, int kDim, int kRowTiles, bool kWide>
+template <class T, int kDim, bool kWide>
 hipError_t launch_window_tiles(const AttentionArgs& a, hipStream_t stream) {
     constexpr int kKeys = kDim == 64 ? 128 : (kDim == 128 ? 64 : 32);
-    constexpr int kRows = kWaves * kRowTiles * 32;
+    constexpr int kRows = kWaves * 32;
     constexpr size_t kLds = 2 * (kKeys * (kDim * 2 + 16) + kDim * (kKeys * 2 + 16));
     const int64_t rows = static_cast<int64_t>(a.queries) * a.group;
     const int row_tiles = static_cast<int>((rows + kRows - 1) / kRows);
     const int64_t tiles = static_cast<int64_t>(row_tiles) * a.kv_heads * a.batch;
     if (tiles >= (int64_t{1} << 24) - 256) return hipErrorInvalidValue;  // a grid has below 2^32 threads
     const hipError_t room = hipFuncSetAttribute(
-        reinterpret_cast<const void*>(window_tile_kernel<T, kDim, kRowTiles, kWide>),
+        reinterpret_cast<const void*>(window_tile_kernel<T, kDim, kWide>),
         hipFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(kLds));
     if (room != hipSuccess) return room;
-    hipLaunchKernelGGL(HIP_KERNEL_NAME(window_tile_kernel<T, kDim, kRowTiles, kWide>),
+    hipLaunchKernelGGL(HIP_KERNEL_NAME(window_tile_kernel<T, kDim, kWide>),
                        dim3(static_cast<uint32_t>(blocks_of_tiles(tiles))), dim3(kThreads), kLds, stream, a, row_tiles,
                        static_cast<int>(tiles));
     return hipGetLastError();
@@ -691,8 +645,8 @@ hipError_t launch_window(const AttentionArgs& a, hipStream_t stream) {
     if constexpr (sizeof(T) == 2) {
         if (a.wide && reinterpret_cast<uintptr_t>(a.out) % 8 == 0 && a.key_strides[2] <= kStagedStride &&
             a.value_strides[2] <= kStagedStride)
-            return launch_window_tiles<T, kDim, 1, true>(a, stream);
-        return launch_window_tiles<T, kDim, 1, false>(a, stream);
+            return launch_window_tiles<T, kDim, true>(a, stream);
+        return launch_window_tiles<T, kDim, false>(a, stream);
     } else {
         constexpr int kRows = kDim == 256 ? 16 : 32;
         const int64_t row_tiles = (static_cast<int64_t>(a.queries) * a.group + kRows - 1) / kRows;
