@@ -19,7 +19,6 @@ namespace {
 struct Candidate {
     int64_t index;
     float value;
-    float pad;
 };
 
 template <class T>
@@ -157,12 +156,12 @@ __global__ void __launch_bounds__(kThreads) logits_kernel(LogitsArgs a, int chun
     }
     int64_t index = at < size ? c0 + at : INT64_MAX;
     wave_best(value, index);
-    if ((threadIdx.x & 63) == 0) best[threadIdx.x >> 6] = Candidate{index, value, 0.0f};
+    if ((threadIdx.x & 63) == 0) best[threadIdx.x >> 6] = Candidate{index, value};
     __syncthreads();
     if (threadIdx.x == 0) {
         for (int w = 1; w < kThreads / kWave; ++w) keep_better(value, index, best[w].value, best[w].index);
         if (chunks == 1) a.tokens[row] = index;
-        else static_cast<Candidate*>(a.workspace)[blockIdx.x] = Candidate{index, value, 0.0f};
+        else static_cast<Candidate*>(a.workspace)[blockIdx.x] = Candidate{index, value};
     }
 }
 

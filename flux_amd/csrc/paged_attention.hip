@@ -2,7 +2,8 @@
 // sliding window and sink tokens:
 //
 //   s_j = scale * <q, k_j>,  m = max s_j,  p_j = exp(s_j - m),  o = sum p_j v_j / sum p_j   over the visible keys j;
-//   a sequence of n keys sees j < n with j >= n - window or j < sinks (window 0: all); nothing visible gives zeros.
+//   a sequence of n keys sees j < n with j >= n - window or j < sinks (window 0: all); nothing visible, or nothing whose
+//   score is above -inf, gives zeros.
 //
 // Every key and value row is read once for all query heads of its KV head, and HBM bounds the whole.  A sequence is cut
 // into parts of about the same number of tiles as every other part of the batch, one per workgroup, so that ragged
@@ -220,7 +221,8 @@ __global__ void __launch_bounds__(kDecodeThreads, kDim * sizeof(T) <= 512 ? 2 : 
         for (int s = 0; s < kSubs; ++s) {
             score[s] = f32x4{0, 0, 0, 0};
 #pragma unroll
-            for (int f = 0; f < kFragments; ++f) M::multiply_key(tile.key[s][f], query[f], score[s]);
+            for (int f = 0; f < kFragments; ++f)
+                M::multiply_key(key_dims<M, kRows>(tile.key[s][f], M::kKeyStep * f + M::kPer * g, a.dim), query[f], score[s]);
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
                 score[s][i] = tile.held[s][i] >= 0 ? score[s][i] * a.scale : -INFINITY;

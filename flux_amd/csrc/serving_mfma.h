@@ -37,9 +37,18 @@ __device__ __forceinline__ int wave_sum_int(int v) {
 }
 
 // How rows are read: element by element, in 16-byte loads, or those where the head fills the padded dims.  Loads are not
-// masked (masks put each one in a block of its own, behind a wait for the register's last value): in 16-byte loads dims
-// behind the head's repeat its first ones, which meet zeros of the query or results that are not stored.
+// masked (masks put each one in a block of its own, behind a wait for the register's last value): dims behind the head's
+// repeat its first ones, which meet zeros of the query (and are cleared themselves where an infinity in them must not
+// show, by key_dims) or results that are not stored.
 enum Rows : int { kNarrow = 0, kWideRows = 1, kFullRows = 2 };
+
+// A fragment of a key row as loaded by load_row, zero behind the head's dims.
+template <class M, Rows kRows>
+__device__ __forceinline__ typename M::Fragment key_dims(const typename M::Fragment& f, int d, int dim) {
+    if constexpr (kRows == kFullRows) return f;
+    if constexpr (kRows == kWideRows) return d < dim ? f : typename M::Fragment{};
+    return M::zero_behind(f, d, dim);
+}
 
 template <class T>
 struct Mfma;

@@ -2,7 +2,7 @@
 // and single tokens (which take the split kernel of paged_attention.hip).
 //
 // The query at position p of a sequence of n keys sees j <= p, j < n, with j > p - window or j < sinks (window 0: all);
-// a row that sees nothing, or whose position is no key's, gives zeros.
+// a row that sees nothing, nothing whose score is above -inf, or whose position is no key's, gives zeros.
 //
 // A workgroup takes kRows rows of one KV head, a row being a query position and one of the head's query heads, so that a
 // group of heads shares each key and value row.  Its four waves split the keys, hold the running maximum and sum per
@@ -69,7 +69,7 @@ __device__ void exact_row(const AttentionArgs& a, const T* query, const T* keys,
     }
 #pragma unroll
     for (int c = 0; c < kServingMaxDim / kWave; ++c)
-        if (kWave * c + lane < a.dim) out[kWave * c + lane] = static_cast<T>(sum[c] / weight);
+        if (kWave * c + lane < a.dim) out[kWave * c + lane] = static_cast<T>(weight == 0.0f ? 0.0f : sum[c] / weight);
 }
 
 // Blocks that an XCD (block index modulo 8) takes one after the other: consecutive tiles share most of their keys.  The
@@ -318,7 +318,7 @@ __global__ void __launch_bounds__(kThreads, kDim <= 64 ? 4 : (kDim <= 128 ? 2 : 
             rows.place(a, r, i, head);
             float* o = static_cast<float*>(a.out) + ((rows.b * a.query_heads + head) * a.queries + i) * a.dim;
             M::template each_dim<kDim>(g, a.dim, [&](int k, int j, int d) {
-                o[d] = mine[c].position < 0 ? 0.0f : out[c][k][j] / weight[c];
+                o[d] = mine[c].position < 0 || weight[c] == 0.0f ? 0.0f : out[c][k][j] / weight[c];
             });
         }
         while (again) {
@@ -595,7 +595,7 @@ window_tile_kernel(AttentionArgs a, int row_tiles, int tiles_total) {
     uint32_t again = static_cast<uint32_t>(odd | odd >> 32);
     if (real && !(again >> n32 & 1)) {
         T* o = static_cast<T*>(a.out) + ((rows.b * a.query_heads + head) * a.queries + query_index) * a.dim;
-        const float inverse = 1.0f / weight;
+        const float inverse = weight == 0.0f ? 0.0f : 1.0f / weight;
 #pragma unroll
         for (int i = 0; i < kBlocks; ++i)
 #pragma unroll

@@ -463,8 +463,8 @@ enum flux_dtype { FLUX_FLOAT32 = 0, FLUX_FLOAT16 = 1, FLUX_BFLOAT16 = 2 };
  * page_table [slot_count, columns] (int32) and of lengths [slot_count] (NULL: columns * page_size); its key j lies in
  * row j % page_size of page page_table[r][j / page_size] of key_pages [pages, kv_heads, page_size, head_dim].  It sees
  * the keys j < lengths[r] (clamped to columns * page_size) and, with window > 0, of those j >= lengths[r] - window and
- * j < sinks.  Keys on a page outside [0, pages) are left out and never read; a sequence that sees nothing, or whose
- * row is outside the table, gives zeros.  query [batch, query_heads, 1, head_dim], output contiguous.
+ * j < sinks.  Keys on a page outside [0, pages) are left out and never read; a sequence that sees nothing, nothing
+ * whose score is above -inf, or whose row is outside the table, gives zeros.  query [batch, query_heads, 1, head_dim], output contiguous.
  * head_dim <= 256, columns * page_size <= FLUX_MAX_SERVING_KEYS. */
 #define FLUX_MAX_SERVING_KEYS (1 << 24)
 int flux_paged_decode_attention_workspace_bytes(int64_t batch, int64_t query_heads, int64_t kv_heads, int64_t head_dim,
@@ -479,8 +479,8 @@ int flux_paged_decode_attention(int dtype, const void* query, const void* key_pa
 
 /* Causal attention with a sliding window and sinks over key, value [batch, kv_heads, keys, head_dim].  The query i of
  * sequence b has position p = starts[b] + i (NULL: lengths[b] - queries + i) and sees the keys j <= p, j < lengths[b]
- * (NULL: keys; clamped to keys) with j > p - window or j < sinks (window 0: all); a row that sees nothing or with
- * p outside [0, lengths[b]) gives zeros.  query [batch, query_heads, queries, head_dim], output contiguous.  The
+ * (NULL: keys; clamped to keys) with j > p - window or j < sinks (window 0: all); a row that sees nothing,
+ * nothing whose score is above -inf, or with p outside [0, lengths[b]) gives zeros.  query [batch, query_heads, queries, head_dim], output contiguous.  The
  * workspace is needed for single queries only. */
 int flux_window_attention_workspace_bytes(int64_t batch, int64_t query_heads, int64_t kv_heads, int64_t queries,
                                           int64_t head_dim, int64_t keys, int64_t window, int64_t sinks,
@@ -493,7 +493,8 @@ int flux_window_attention(int dtype, const void* query, const void* key, const v
 
 /* Pages of a cache.  The books: page_table int32 [slots, columns] (-1: no page), lengths int64 [slots], refcounts
  * int32 [pages] (sequences that hold a page; 0: free).  Requests are served in their order, a needed page is the
- * lowest free one, and what became of each request is its flux_page_status; a refused request changes nothing. */
+ * lowest free one, and what became of each request is its flux_page_status; a refused request changes nothing.  Lists of
+ * requests must not lie in the books (refused), nor may outputs and workspaces. */
 enum flux_page_status {
     FLUX_PAGE_DONE = 0,
     FLUX_PAGE_OUT_OF_RANGE = 1, /* a slot, page, count or length outside its range */

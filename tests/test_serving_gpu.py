@@ -184,6 +184,44 @@ def test_paged_decode_nan_and_large_scores(gpu_device):
     torch.testing.assert_close(out, expected, rtol=1e-6, atol=0)
 
 
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("dim", [64, 80, 100, 5, 136, 129])
+def test_a_key_of_infinities_has_no_weight(gpu_device, dtype, dim):
+    """A key whose score is -inf is as good as masked, also where the head does not fill the registers' dims."""
+    case = _paged_case(37, dtype, 4, 2, dim, 16, [50, 33])
+    case["query"][..., 0] = case["query"][..., 0].abs() + 0.5
+    finite = {**case, "key_pages": case["key_pages"].clone()}
+    for b, position in ((0, 3), (0, 49), (1, 20)):
+        case["key_pages"][int(case["page_table"][b, position // 16]), :, position % 16, 0] = -math.inf
+    expected = ref.paged_decode(**case)
+    assert bool(expected.isfinite().all())
+    bound = ref.attention_bound(finite["query"], finite["key_pages"], finite["value_pages"], finite["scale"], 50, dtype, expected)
+    _close(ops.paged_decode_attention_native(**_to(case, gpu_device)), expected, bound)
+
+    case = _window_case(41, dtype, 1, 4, 2, dim, 40, 40)
+    case["query"][..., 0] = case["query"][..., 0].abs() + 0.5
+    finite = {**case, "key": case["key"].clone()}
+    case["key"][:, :, [5, 22], 0] = -math.inf
+    expected = ref.window_attention(**case, window=0)
+    assert bool(expected.isfinite().all())
+    bound = ref.attention_bound(finite["query"], finite["key"], finite["value"], finite["scale"], 40, dtype, expected, True)
+    _close(ops.window_attention_native(**_to(case, gpu_device), window=0), expected, bound)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("dim", [64, 80])
+def test_scores_that_are_all_minus_infinity_give_zeros(gpu_device, dtype, dim):
+    case = _to(_window_case(43, dtype, 1, 4, 2, dim, 40, 40), gpu_device)
+    case["query"][..., 0] = case["query"][..., 0].abs() + 0.5
+    case["key"][:, :, :20, 0] = -math.inf
+    out = ops.window_attention_native(**case, window=8, sinks=2)
+    assert not bool(out[:, :, :20].any()) and bool(out[:, :, 20:].isfinite().all()) and bool(out[:, :, 20:].any())
+    for n in (1, 20, 21):
+        one = ops.window_attention_native(**{**case, "query": case["query"][:, :, n - 1 : n]}, window=8, sinks=2,
+                                          lengths=torch.tensor([n], device=gpu_device))
+        assert bool(one.isfinite().all()) and bool(one.any()) == (n > 20)
+
+
 def test_paged_decode_many_small_weights_in_float16(gpu_device):
     """One key far above 8000 others whose weights are below float16's smallest step together weigh a fifth."""
     n = 8192
@@ -771,3 +809,99 @@ def test_a_decode_step_in_a_graph(gpu_device):
             t.copy_(old)
         eager = [*step(), *pages.books, pages.key, pages.value]
         assert all(torch.equal(a, b) for a, b in zip(got, eager)), i
+
+
+def test_two_graphs_replayed_in_turn(gpu_device):
+    """Captured calls keep workspaces of their own: cut sequences, single windowed tokens, logits and pages in two graphs."""
+    cases = [_to(_paged_case(67 + i, torch.float32, 6, 2, 64, 16, [3000 - 900 * i, 700, 40]), gpu_device) for i in range(2)]
+    rows = [_to(_window_case(71 + i, torch.bfloat16, 2, 4, 2, 64, 1, 2500), gpu_device) for i in range(2)]
+    logits = [torch.randn(2, 20000, generator=torch.Generator().manual_seed(73 + i)).to(gpu_device) for i in range(2)]
+    books = [(torch.full((3, 4), -1, dtype=torch.int32, device=gpu_device), torch.zeros(3, dtype=torch.int64, device=gpu_device),
+              torch.zeros(9 + i, dtype=torch.int32, device=gpu_device)) for i in range(2)]
+    slots = torch.tensor([2, 0], device=gpu_device)
+
+    def step(i):
+        at, status = ops.paged_cache_reserve_native(*books[i], 4, slots)
+        return (ops.paged_decode_attention_native(**cases[i], window=0), ops.window_attention_native(**rows[i], window=2000, sinks=3),
+                *ops.logits_process_native(logits[i]), at, status)
+
+    graphs, outputs = [], []
+    for i in range(2):
+        stream = torch.cuda.Stream()
+        stream.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(stream):
+            step(i)
+        torch.cuda.current_stream().wait_stream(stream)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            outputs.append(step(i))
+        graphs.append(graph)
+    for turn in range(6):
+        for case, row, logit in zip(cases, rows, logits):
+            case["query"].normal_()
+            row["query"].normal_()
+            logit.normal_()
+        for table, lengths, refcounts in books:
+            table.fill_(-1)
+            lengths.fill_(turn)
+            refcounts.zero_()
+        for i in ((0, 1), (1, 0))[turn % 2]:
+            graphs[i].replay()
+        torch.cuda.synchronize()
+        got = [[t.clone() for t in (*outputs[i], *books[i])] for i in range(2)]
+        for i in range(2):
+            table, lengths, refcounts = books[i]
+            table.fill_(-1)
+            lengths.fill_(turn)
+            refcounts.zero_()
+            eager = [*step(i), *books[i]]
+            assert all(torch.equal(a, b) for a, b in zip(got[i], eager)), (turn, i)
+
+
+def test_offsets_beyond_32_bits(gpu_device):
+    """A pool of more than 2^32 elements gives what a small one gives, and so do rows far apart."""
+    dim, page_size, far = 128, 64, 2 ** 32 // (128 * 64)
+    small = [torch.zeros(12, 1, page_size, dim, dtype=torch.bfloat16, device=gpu_device) for _ in range(2)]
+    large = [torch.empty(far + 12, 1, page_size, dim, dtype=torch.bfloat16, device=gpu_device) for _ in range(2)]
+    for pool in large:
+        pool[far:] = 0
+    key, value = (torch.randn(2, 1, 150, dim, device=gpu_device).bfloat16() for _ in range(2))
+    query = torch.randn(3, 4, 1, dim, device=gpu_device).bfloat16()
+    slots, counts = torch.tensor([0, 1], device=gpu_device), torch.tensor([150, 70], device=gpu_device)
+    source, target = torch.tensor([0, 3], device=gpu_device), torch.tensor([9, 10], device=gpu_device)
+    results = []
+    for (key_pages, value_pages), start in ((small, 0), (large, far)):
+        table = torch.full((3, 4), -1, dtype=torch.int32, device=gpu_device)
+        lengths = torch.zeros(3, dtype=torch.int64, device=gpu_device)
+        refcounts = torch.zeros(start + 12, dtype=torch.int32, device=gpu_device)
+        refcounts[:start] = 1
+        positions, status = ops.paged_cache_reserve_native(table, lengths, refcounts, page_size, slots, counts)
+        ops.paged_cache_write_native(key, value, key_pages, value_pages, table, slots, positions, counts)
+        forked = ops.paged_cache_fork_native(key_pages, value_pages, table, lengths, refcounts, slots[:1], slots[:1] + 2)
+        copied = ops.paged_cache_copy_native(key_pages, value_pages, source + start, target + start)
+        out = ops.paged_decode_attention_native(query, key_pages, value_pages, table, lengths, dim ** -0.5)
+        results.append([status, positions, forked, copied, out, lengths, torch.where(table >= 0, table - start, table),
+                        refcounts[start:], key_pages[start:], value_pages[start:]])
+    for a, b in zip(*results):
+        assert torch.equal(a, b)
+    assert bool(results[0][4].any()) and results[0][0].tolist() == [0, 0]
+    # A page from behind 2^32 elements to the front.
+    held = large[0][far + 1].clone()
+    free = torch.ones(far + 12, dtype=torch.int32, device=gpu_device)
+    free[far + 2 :] = 0
+    free[5] = free[6] = 0
+    table = torch.tensor([[far, far + 1]], dtype=torch.int32, device=gpu_device)
+    page_map, used = ops.paged_cache_compact_native(*large, table, free)
+    assert int(used) == far and table.tolist() == [[5, 6]] and page_map[far:].tolist() == [5, 6] + [-1] * 10
+    assert torch.equal(large[0][6], held)
+    # Rows 2^23 elements apart, and sequences 2^31: keys and values side by side.
+    flat, apart, sequence = large[0].view(-1), 2 ** 23, 2 ** 31 + 64
+    case = _to(_window_case(79, torch.bfloat16, 2, 4, 1, dim, 200, 250), gpu_device)
+    spread = {"key": flat.as_strided((2, 1, 250, dim), (sequence, dim, apart, 1)),
+              "value": flat.as_strided((2, 1, 250, dim), (sequence, dim, apart, 1), dim)}
+    for name, view in spread.items():
+        view.copy_(case[name])
+    for queries in (1, 200):
+        q = case["query"][:, :, :queries]
+        expected = ops.window_attention_native(**{**case, "query": q}, window=90, sinks=5)
+        assert torch.equal(ops.window_attention_native(q, **spread, scale=case["scale"], window=90, sinks=5), expected)
