@@ -774,6 +774,19 @@ const char* books_arguments(flux::PageBooks& out, const flux_page_books* books, 
     return nullptr;
 }
 
+bool overlap(const void* a, int64_t a_bytes, const void* b, int64_t b_bytes) {
+    const auto from_a = reinterpret_cast<uintptr_t>(a), from_b = reinterpret_cast<uintptr_t>(b);
+    return from_a < from_b + static_cast<uintptr_t>(b_bytes) && from_b < from_a + static_cast<uintptr_t>(a_bytes);
+}
+
+// Whether a list of requests lies in the books that its kernel changes while it reads the list again.
+bool list_in_books(const int64_t* list, int64_t requests, const flux::PageBooks& b) {
+    if (!list) return false;
+    const int64_t bytes = requests * 8;
+    return overlap(list, bytes, b.table, ((b.slots - 1) * b.table_stride + b.columns) * 4) ||
+           overlap(list, bytes, b.lengths, b.slots * 8) || overlap(list, bytes, b.refcounts, b.pages * 4);
+}
+
 }  // namespace
 
 int flux_paged_decode_attention_workspace_bytes(int64_t batch, int64_t query_heads, int64_t kv_heads, int64_t head_dim,
@@ -871,6 +884,8 @@ int flux_page_reserve(const flux_page_books* books, const int64_t* slots, const 
     if (!slots || !positions || !status || !workspace) return invalid("flux_page_reserve: null argument");
     if (workspace_words < static_cast<int64_t>(flux::page_reserve_workspace(requests, b.slots, b.pages)))
         return invalid("flux_page_reserve: workspace too small (flux_page_reserve_workspace_words)");
+    if (list_in_books(slots, requests, b) || list_in_books(counts, requests, b))
+        return invalid("flux_page_reserve: slots and counts must not lie in the books");
     return from_hip(flux::launch_page_reserve(b, slots, counts, requests, positions, status, workspace, stream),
                     "flux_page_reserve");
 }
@@ -923,6 +938,7 @@ int flux_page_free(const flux_page_books* books, const int64_t* slots, int64_t r
     flux::PageBooks b{};
     if (const char* wrong = books_arguments(b, books, requests)) return invalid(std::string("flux_page_free: ") + wrong);
     if (!slots || !status) return invalid("flux_page_free: null argument");
+    if (list_in_books(slots, requests, b)) return invalid("flux_page_free: slots must not lie in the books");
     return from_hip(flux::launch_page_free(b, slots, requests, status, stream), "flux_page_free");
 }
 
@@ -944,6 +960,8 @@ int flux_page_fork(const flux_page_pool* pool, const flux_page_books* books, con
     if (!parents || !children || !status || !workspace) return invalid("flux_page_fork: null argument");
     if (workspace_words < static_cast<int64_t>(flux::page_fork_workspace(requests, b.slots, b.pages)))
         return invalid("flux_page_fork: workspace too small (flux_page_fork_workspace_words)");
+    if (list_in_books(parents, requests, b) || list_in_books(children, requests, b))
+        return invalid("flux_page_fork: parents and children must not lie in the books");
     return from_hip(flux::launch_page_fork(p, b, parents, children, requests, status, workspace, stream),
                     "flux_page_fork");
 }

@@ -178,6 +178,13 @@ def _validate_paged_out(query, key_pages, value_pages, page_table, lengths, scal
            output.is_contiguous(), f"{op}: output must be contiguous, of the query's shape, dtype and device")
     _check(workspace.dtype == torch.float32 and workspace.device == query.device and workspace.is_contiguous(),
            f"{op}: workspace must be contiguous float32 on the query device")
+
+
+def _validate_paged_out_memory(query, key_pages, value_pages, page_table, lengths, scale, window, sinks, slots, output,
+                               workspace) -> None:
+    _validate_paged_out(query, key_pages, value_pages, page_table, lengths, scale, window, sinks, slots, output,
+                        workspace)
+    op = "flux::paged_decode_attention_out"
     _check(not _aliases(output, workspace), f"{op}: output and workspace must not alias")
     for tensor in (query, key_pages, value_pages, page_table, lengths, slots):
         _check(tensor is None or not (_aliases(output, tensor) or _aliases(workspace, tensor)),
@@ -185,8 +192,8 @@ def _validate_paged_out(query, key_pages, value_pages, page_table, lengths, scal
 
 
 def _paged_out_cuda(query, key_pages, value_pages, page_table, lengths, scale, window, sinks, slots, output, workspace):
-    _validate_paged_out(query, key_pages, value_pages, page_table, lengths, scale, window, sinks, slots, output,
-                        workspace)
+    _validate_paged_out_memory(query, key_pages, value_pages, page_table, lengths, scale, window, sinks, slots, output,
+                               workspace)
     _require_gpu("flux::paged_decode_attention_out", query)
     _check(workspace.numel() * 4 >= paged_decode_workspace_bytes(query, key_pages, page_table, window, sinks),
            "flux::paged_decode_attention_out: workspace is too small (paged_decode_workspace_bytes)")
@@ -249,11 +256,16 @@ def _window_cuda(query, key, value, scale, window, sinks=0, lengths=None, starts
 # ---------------------------------------------------------------------------
 # Pages.
 
-def _written_once(shape, stride) -> bool:
-    """No two elements of a tensor that is written share memory by a stride of zero."""
-    if 0 not in stride:
+def _written_once(tensor) -> bool:
+    """No two elements of a tensor that is written share memory: each dimension steps over all smaller ones."""
+    if tensor.is_contiguous():
         return True
-    return all(step > 0 or size == 1 for size, step in zip(shape, stride))
+    reach = 0
+    for step, size in sorted((step, size) for step, size in zip(tensor.stride(), tensor.shape) if size > 1):
+        if step <= reach:
+            return False
+        reach += step * (size - 1)
+    return True
 
 
 def _validate_pools(op, key_pages, value_pages, ranks=(4, 5)) -> None:
@@ -271,10 +283,12 @@ def _validate_pools(op, key_pages, value_pages, ranks=(4, 5)) -> None:
         _check(False, f"{op}: tensor devices must match")
     if (key_stride[-1] != 1 or value_stride[-1] != 1) and shape[-1] != 1:
         _check(False, f"{op}: pages must have unit stride along the head dimension")
-    if not _written_once(shape, key_stride):
+    if not _written_once(key_pages):
         _check(False, f"{op}: key_pages must not overlap itself")
-    if not _written_once(shape, value_stride):
+    if not _written_once(value_pages):
         _check(False, f"{op}: value_pages must not overlap itself")
+    if key_pages.is_set_to(value_pages):
+        _check(False, f"{op}: key_pages and value_pages must not be the same memory")
     if torch.is_grad_enabled():
         _grad_free(op, key_pages, value_pages)
 
@@ -374,9 +388,6 @@ def _validate_write(key, value, key_pages, value_pages, page_table, slots, posit
            "flux::paged_cache_write: key heads and head dimension must be the pages'")
     _check(key.stride(3) == 1 and value.stride(3) == 1 or shape[3] == 1,
            "flux::paged_cache_write: key and value must have unit stride along the head dimension")
-    stores = key_pages.untyped_storage().data_ptr(), value_pages.untyped_storage().data_ptr()
-    _check(key.untyped_storage().data_ptr() not in stores and value.untyped_storage().data_ptr() not in stores,
-           "flux::paged_cache_write: the pages must not alias key or value")
     requests = shape[0]
     _check_list(slots, torch.int64, device,
                 "flux::paged_cache_write: slots must be a contiguous int64 vector on the cache's device",
@@ -393,8 +404,15 @@ def _validate_write(key, value, key_pages, value_pages, page_table, slots, posit
         _grad_free(op, key, value)
 
 
-def _write_cuda(key, value, key_pages, value_pages, page_table, slots, positions, counts=None):
+def _validate_write_memory(key, value, key_pages, value_pages, page_table, slots, positions, counts=None) -> None:
     _validate_write(key, value, key_pages, value_pages, page_table, slots, positions, counts)
+    stores = key_pages.untyped_storage().data_ptr(), value_pages.untyped_storage().data_ptr()
+    _check(key.untyped_storage().data_ptr() not in stores and value.untyped_storage().data_ptr() not in stores,
+           "flux::paged_cache_write: the pages must not alias key or value")
+
+
+def _write_cuda(key, value, key_pages, value_pages, page_table, slots, positions, counts=None):
+    _validate_write_memory(key, value, key_pages, value_pages, page_table, slots, positions, counts)
     _require_gpu("flux::paged_cache_write", key_pages)
     if key.shape[0] == 0 or key.shape[2] == 0:
         return
@@ -573,10 +591,10 @@ def _logits_cuda(logits, history=None, history_lengths=None, repetition=None, fr
 
 _KERNELS = {
     "paged_decode_attention": (_paged_cuda, _validate_paged),
-    "paged_decode_attention_out": (_paged_out_cuda, _validate_paged_out),
+    "paged_decode_attention_out": (_paged_out_cuda, _validate_paged_out_memory),
     "window_attention": (_window_cuda, _validate_window),
     "paged_cache_reserve": (_reserve_cuda, _validate_reserve),
-    "paged_cache_write": (_write_cuda, _validate_write),
+    "paged_cache_write": (_write_cuda, _validate_write_memory),
     "paged_cache_copy": (_copy_cuda, _validate_copy),
     "paged_cache_fork": (_fork_cuda, _validate_fork),
     "paged_cache_free": (_free_cuda, _validate_free),
@@ -597,7 +615,8 @@ def _paged_fake(query, key_pages, value_pages, page_table, lengths, scale, windo
 
 @torch.library.register_fake("flux::paged_decode_attention_out")
 def _paged_out_fake(query, key_pages, value_pages, page_table, lengths, scale, window, sinks, slots, output, workspace):
-    _validate_paged(query, key_pages, value_pages, page_table, lengths, scale, window, sinks, slots)
+    _validate_paged_out(query, key_pages, value_pages, page_table, lengths, scale, window, sinks, slots, output,
+                        workspace)
     return output
 
 
@@ -615,16 +634,18 @@ def _reserve_fake(page_table, lengths, refcounts, page_size, slots, counts=None)
 
 @torch.library.register_fake("flux::paged_cache_write")
 def _write_fake(key, value, key_pages, value_pages, page_table, slots, positions, counts=None):
-    return None
+    _validate_write(key, value, key_pages, value_pages, page_table, slots, positions, counts)
 
 
 @torch.library.register_fake("flux::paged_cache_copy")
 def _copy_fake(key_pages, value_pages, source, target):
+    _validate_copy(key_pages, value_pages, source, target)
     return source.new_empty(source.shape, dtype=torch.int32)
 
 
 @torch.library.register_fake("flux::paged_cache_fork")
 def _fork_fake(key_pages, value_pages, page_table, lengths, refcounts, parents, children):
+    _validate_fork(key_pages, value_pages, page_table, lengths, refcounts, parents, children)
     return parents.new_empty(parents.shape, dtype=torch.int32)
 
 
@@ -636,6 +657,7 @@ def _free_fake(page_table, lengths, refcounts, slots):
 
 @torch.library.register_fake("flux::paged_cache_compact")
 def _compact_fake(key_pages, value_pages, page_table, refcounts):
+    _validate_compact(key_pages, value_pages, page_table, refcounts)
     return refcounts.new_empty(refcounts.shape), refcounts.new_empty((), dtype=torch.int64)
 
 

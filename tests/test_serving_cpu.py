@@ -179,6 +179,35 @@ def test_write_refuses_a_source_inside_the_pages():
         torch.ops.flux.paged_cache_write(**args)
 
 
+PAGES_CALLS = ("paged_cache_write", "paged_cache_copy", "paged_cache_fork", "paged_cache_compact")
+
+
+@pytest.mark.parametrize("name", PAGES_CALLS)
+def test_pages_that_are_written_lie_apart(name):
+    args = CALLS[name]()
+    with pytest.raises(RuntimeError, match="must not be the same memory"):
+        getattr(torch.ops.flux, name)(**{**args, "value_pages": args["key_pages"]})
+    shape = args["key_pages"].shape
+    strides = torch.empty(shape).stride()
+    for dimension in range(len(shape) - 1):  # a step that ends inside what lies below it
+        short = [step - (i == dimension) for i, step in enumerate(strides)]
+        if shape[dimension] > 1:
+            with pytest.raises(RuntimeError, match="value_pages must not overlap itself"):
+                getattr(torch.ops.flux, name)(**{**args, "value_pages": torch.zeros(4000).as_strided(shape, short)})
+    padded = {n: torch.zeros(*shape[:-1], shape[-1] + 3)[..., :-3].transpose(-2, -3).contiguous().transpose(-2, -3)
+              for n in ("key_pages", "value_pages")}
+    with pytest.raises(RuntimeError, match="no CPU kernel"):
+        getattr(torch.ops.flux, name)(**{**args, **padded})
+
+
+@pytest.mark.parametrize("name,change,message", [r for r in REFUSED if "requires_grad" not in str(r[1])][::4])
+def test_fake_tensors_are_refused_alike(name, change, message):
+    mode = FakeTensorMode()
+    args = {k: mode.from_tensor(v) if isinstance(v, torch.Tensor) else v for k, v in {**CALLS[name](), **change}.items()}
+    with mode, pytest.raises(RuntimeError, match=message):
+        getattr(torch.ops.flux, name)(**args)
+
+
 def test_fake_shapes():
     with FakeTensorMode(allow_non_fake_inputs=True) as mode:
         def fake(values):
@@ -257,6 +286,25 @@ def test_c_entries_refuse_before_any_launch():
                                    None, 0, None) == bad
     assert lib.flux_logits_process(0, some, 100000, some, some, 2, 100000, None, 0, 0, None, None, None, None, None, 0,
                                    None, 0, None, 0, None) == bad and "workspace" in _native.last_error()
+
+
+def test_c_entries_refuse_lists_inside_the_books():
+    """Each kernel reads its lists again after it has changed the books."""
+    lib, bad = _native.load(), _native.FLUX_ERROR_INVALID_VALUE
+    at = {"page_table": 0x10000, "lengths": 0x20000, "refcounts": 0x30000}
+    books, some, apart = _books_struct(**at), ctypes.c_void_p(16), ctypes.c_void_p(0x40000)
+    sizes = {"page_table": 2 * 4 * 4, "lengths": 2 * 8, "refcounts": 4 * 4}
+    for name, start in at.items():
+        for inside in (start - 8, start, start + sizes[name] - 1):  # two requests: 16 bytes
+            where = ctypes.c_void_p(inside)
+            for slots, counts in ((where, None), (where, apart), (apart, where)):
+                assert lib.flux_page_reserve(books, slots, counts, 2, some, some, some, 100, None) == bad
+                assert "must not lie in the books" in _native.last_error()
+            assert lib.flux_page_free(books, where, 2, some, None) == bad
+            assert "must not lie in the books" in _native.last_error()
+            for parents, children in ((where, apart), (apart, where)):
+                assert lib.flux_page_fork(_pool_struct(), books, parents, children, 2, some, some, 100, None) == bad
+                assert "must not lie in the books" in _native.last_error()
 
 
 # --------------------------------------------------------------------------- the plain page model
