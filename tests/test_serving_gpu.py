@@ -666,6 +666,27 @@ def test_logits_edges(gpu_device):
     assert int(tokens[0]) == 0 and bool(out.cpu().isneginf().all())
 
 
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("rows,vocab", [(1, 20000), (300, 8200), (300, 8203)])
+def test_logits_ties_go_to_the_lowest_index(gpu_device, dtype, rows, vocab):
+    """Zeros of both signs are equal, what a rounding makes equal is equal, and the first NaN is above all."""
+    low = torch.full((rows, vocab), -3.0, dtype=dtype)
+    for places in ([0, 1], [7, 8], [5, 4100], [2047, 2048], [4093, 8199], [vocab - 2, vocab - 1]):
+        for first, second in ((0.0, -0.0), (-0.0, 0.0), (math.inf, math.inf), (math.nan, math.nan), (math.nan, math.inf)):
+            logits = low.clone()
+            logits[:, places[0]], logits[:, places[1]] = first, second
+            processed, tokens = ops.logits_process_native(logits.to(gpu_device))
+            assert tokens.tolist() == [places[0]] * rows, (places, first, second)
+            assert torch.equal(processed.cpu().nan_to_num(nan=9.0), logits.nan_to_num(nan=9.0))
+        # The second is larger by less than half a step of the type before the rounding.
+        logits = low.clone()
+        logits[:, places] = 1.0
+        bias = torch.zeros(1, vocab)
+        bias[0, places[1]] = torch.finfo(dtype).eps / 4
+        _, tokens = ops.logits_process_native(logits.to(gpu_device), bias=bias.to(gpu_device))
+        assert tokens.tolist() == [places[0]] * rows
+
+
 def test_logits_strides(gpu_device):
     case = _logits_case(3, torch.float16, 4, 4096, 64, bias_rows=4)
     device = _to(case, gpu_device)
