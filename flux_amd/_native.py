@@ -118,8 +118,7 @@ class PagePool(ctypes.Structure):
                 ("key_strides", ctypes.c_int64 * 4), ("value_strides", ctypes.c_int64 * 4), ("dtype", ctypes.c_int64)]
 
 
-_books = ctypes.POINTER(PageBooks)
-_pool = ctypes.POINTER(PagePool)
+_books = _pool = _strides = ctypes.c_void_p  # by reference, or their fields packed into bytes
 _n = ctypes.c_int64
 
 # (name, restype, argtypes) for every exported symbol.
@@ -211,14 +210,14 @@ _PROTOTYPES: list[tuple[str, Any, list[Any]]] = [
       ctypes.c_int64, ctypes.c_int64, _i64, _i64, _i64, _i64, _i64, _stream]),
     ("flux_paged_decode_attention_workspace_bytes", ctypes.c_int, [_n] * 7 + [_i64]),
     ("flux_paged_decode_attention", ctypes.c_int,
-     [ctypes.c_int] + [_vp] * 8 + [_n, ctypes.c_float] + [_n] * 11 + [_i64, _i64, _i64, _stream]),
+     [ctypes.c_int] + [_vp] * 8 + [_n, ctypes.c_float] + [_n] * 11 + [_strides] * 3 + [_stream]),
     ("flux_window_attention_workspace_bytes", ctypes.c_int, [_n] * 8 + [_i64]),
     ("flux_window_attention", ctypes.c_int,
-     [ctypes.c_int] + [_vp] * 7 + [_n, ctypes.c_float] + [_n] * 8 + [_i64, _i64, _i64, _stream]),
+     [ctypes.c_int] + [_vp] * 7 + [_n, ctypes.c_float] + [_n] * 8 + [_strides] * 3 + [_stream]),
     ("flux_page_reserve_workspace_words", ctypes.c_int, [_n, _n, _n, _i64]),
     ("flux_page_reserve", ctypes.c_int, [_books, _vp, _vp, _n, _vp, _vp, _vp, _n, _stream]),
     ("flux_page_write", ctypes.c_int,
-     [_pool, _vp, _vp, _i64, _i64, _n, _n, _vp, _n, _n, _n, _vp, _vp, _vp, _stream]),
+     [_pool, _vp, _vp, _strides, _strides, _n, _n, _vp, _n, _n, _n, _vp, _vp, _vp, _stream]),
     ("flux_page_copy", ctypes.c_int, [_pool, _vp, _vp, _n, _vp, _stream]),
     ("flux_page_free", ctypes.c_int, [_books, _vp, _n, _vp, _stream]),
     ("flux_page_fork_workspace_words", ctypes.c_int, [_n, _n, _n, _i64]),

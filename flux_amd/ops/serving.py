@@ -16,12 +16,13 @@ from __future__ import annotations
 
 import ctypes
 import functools
+import struct
 
 import torch
 
 from flux_amd import _native
-from flux_amd.ops.native import (_LIBRARY, _aliases, _availability, _check, _cpu_kernel, _finite_fp32, _grad_free, _on,
-                                 _require_gpu, _require_library, _stream)
+from flux_amd.ops.native import (_LIBRARY, _aliases, _availability, _check, _cpu_kernel, _finite_fp32, _grad_free,
+                                 _require_gpu, _require_library)
 
 PAGE_DONE, PAGE_OUT_OF_RANGE, PAGE_REPEATED, PAGE_NO_ROOM, PAGE_OCCUPIED = range(5)
 
@@ -61,11 +62,12 @@ SERVING_OPERATOR_NAMES = tuple(SERVING_SCHEMAS)
 for _schema in SERVING_SCHEMAS.values():
     _LIBRARY.define(_schema)
 
-_FOUR = ctypes.c_int64 * 4
-
-
-# Checks are a large part of a small call's time: shapes are read once, messages are whole literals, sizes that only
-# depend on shapes come from small caches.
+# Checks and arguments are a large part of a small call's time (one sequence of 900 keys: 20 us, on the GPU 15): shapes are
+# read once, conditions are tested in place, messages are whole literals, sizes that only depend on shapes come from small
+# caches, and structures and strides are packed into bytes (a ctypes array of four costs 0.5 us, its bytes 0.2).
+_four = struct.Struct("4q").pack
+_page_books = struct.Struct("8q").pack   # flux_page_books
+_page_pool = struct.Struct("16q").pack   # flux_page_pool
 
 def _address(tensor):
     return None if tensor is None else tensor.data_ptr()
@@ -74,7 +76,8 @@ def _address(tensor):
 def _check_list(tensor, dtype, device, message: str, length=None, length_message: str = "") -> None:
     """A contiguous vector of ``dtype`` (and ``length``) on ``device``."""
     shape = tensor.shape
-    _check(len(shape) == 1 and tensor.dtype is dtype and tensor.device == device and tensor.is_contiguous(), message)
+    if not (len(shape) == 1 and tensor.dtype is dtype and tensor.device == device and tensor.is_contiguous()):
+        _check(False, message)
     if length is not None:
         _check(shape[0] == length, length_message)
 
@@ -83,6 +86,15 @@ def _call(function: str, *args) -> None:
     status = getattr(_native._lib or _native.load(), function)(*args)
     if status:
         _native.check(status)
+
+
+def _launch(function: str, device: torch.device, *args) -> None:
+    """A C entry on the device's current stream."""
+    if device.index == torch.cuda.current_device():
+        _call(function, *args, _native.current_stream(device))
+    else:
+        with torch.cuda.device(device):
+            _call(function, *args, _native.current_stream(device))
 
 
 def _ready(what: str) -> None:
@@ -103,22 +115,26 @@ def _size_from(function: str, *sizes) -> int:
 
 def _validate_paged(query, key_pages, value_pages, page_table, lengths, scale, window=0, sinks=0, slots=None) -> None:
     shape, pages, table, dtype, device = query.shape, key_pages.shape, page_table.shape, query.dtype, query.device
-    _check(len(shape) == 4 and len(pages) == 4 and value_pages.dim() == 4,
-           "flux::paged_decode_attention: query and pages must be rank four")
-    _check(dtype in _TYPES and key_pages.dtype is dtype and value_pages.dtype is dtype,
-           "flux::paged_decode_attention: query and pages must share dtype float32, float16 or bfloat16")
-    _check(shape[2] == 1, "flux::paged_decode_attention: query length must be one")
-    _check(pages == value_pages.shape, "flux::paged_decode_attention: key and value page shapes must match")
-    _check(0 not in shape and 0 not in pages, "flux::paged_decode_attention: tensor dimensions must be non-empty")
-    _check(shape[3] == pages[3] and shape[3] <= _MAX_DIM,
-           "flux::paged_decode_attention: head dimensions must match and be at most 256")
-    _check(shape[1] % pages[1] == 0, "flux::paged_decode_attention: query heads must be divisible by KV heads")
-    _check(len(table) == 2 and page_table.dtype is torch.int32 and table[1] > 0,
-           "flux::paged_decode_attention: page_table must be int32 [slots, columns]")
-    _check(page_table.stride(1) == 1 or table[1] == 1,
-           "flux::paged_decode_attention: page_table rows must be contiguous")
-    _check(table[1] * pages[2] <= _MAX_KEYS,
-           "flux::paged_decode_attention: page_table holds more than 16777216 positions a row")
+    if not (len(shape) == 4 and len(pages) == 4 and value_pages.dim() == 4):
+        _check(False, "flux::paged_decode_attention: query and pages must be rank four")
+    if not (dtype in _TYPES and key_pages.dtype is dtype and value_pages.dtype is dtype):
+        _check(False, "flux::paged_decode_attention: query and pages must share dtype float32, float16 or bfloat16")
+    if not (shape[2] == 1):
+        _check(False, "flux::paged_decode_attention: query length must be one")
+    if not (pages == value_pages.shape):
+        _check(False, "flux::paged_decode_attention: key and value page shapes must match")
+    if not (0 not in shape and 0 not in pages):
+        _check(False, "flux::paged_decode_attention: tensor dimensions must be non-empty")
+    if not (shape[3] == pages[3] and shape[3] <= _MAX_DIM):
+        _check(False, "flux::paged_decode_attention: head dimensions must match and be at most 256")
+    if not (shape[1] % pages[1] == 0):
+        _check(False, "flux::paged_decode_attention: query heads must be divisible by KV heads")
+    if not (len(table) == 2 and page_table.dtype is torch.int32 and table[1] > 0):
+        _check(False, "flux::paged_decode_attention: page_table must be int32 [slots, columns]")
+    if not (page_table.stride(1) == 1 or table[1] == 1):
+        _check(False, "flux::paged_decode_attention: page_table rows must be contiguous")
+    if not (table[1] * pages[2] <= _MAX_KEYS):
+        _check(False, "flux::paged_decode_attention: page_table holds more than 16777216 positions a row")
     _check_list(lengths, torch.int64, device,
                 "flux::paged_decode_attention: lengths must be a contiguous int64 vector on the query device",
                 table[0], "flux::paged_decode_attention: lengths must have one entry per page_table row")
@@ -129,13 +145,14 @@ def _validate_paged(query, key_pages, value_pages, page_table, lengths, scale, w
         _check_list(slots, torch.int64, device,
                     "flux::paged_decode_attention: slots must be a contiguous int64 vector on the query device",
                     shape[0], "flux::paged_decode_attention: slots must have one entry per sequence")
-    _check(key_pages.device == device and value_pages.device == device and page_table.device == device,
-           "flux::paged_decode_attention: tensor devices must match")
-    _check(key_pages.stride(3) == 1 and value_pages.stride(3) == 1 or pages[3] == 1,
-           "flux::paged_decode_attention: pages must have unit stride along the head dimension")
-    _check(0 <= window <= _MAX_KEYS and 0 <= sinks <= _MAX_KEYS,
-           "flux::paged_decode_attention: window and sinks must be within [0, 16777216]")
-    _check(_finite_fp32(scale), "flux::paged_decode_attention: scale must be a finite FP32 value")
+    if not (key_pages.device == device and value_pages.device == device and page_table.device == device):
+        _check(False, "flux::paged_decode_attention: tensor devices must match")
+    if not (key_pages.stride(3) == 1 and value_pages.stride(3) == 1 or pages[3] == 1):
+        _check(False, "flux::paged_decode_attention: pages must have unit stride along the head dimension")
+    if not (0 <= window <= _MAX_KEYS and 0 <= sinks <= _MAX_KEYS):
+        _check(False, "flux::paged_decode_attention: window and sinks must be within [0, 16777216]")
+    if not (_finite_fp32(scale)):
+        _check(False, "flux::paged_decode_attention: scale must be a finite FP32 value")
     if torch.is_grad_enabled():
         _grad_free("flux::paged_decode_attention", query, key_pages, value_pages)
 
@@ -152,20 +169,19 @@ def _launch_paged(query, key_pages, value_pages, page_table, lengths, scale, win
     batch, heads, _, dim = query.shape
     pages, kv_heads, page_size, _ = key_pages.shape
     slot_count, columns = page_table.shape
-    with _on(query.device):
-        _call("flux_paged_decode_attention", _TYPES[query.dtype], query.data_ptr(), key_pages.data_ptr(),
-              value_pages.data_ptr(), page_table.data_ptr(), lengths.data_ptr(), _address(slots), output.data_ptr(),
-              workspace.data_ptr(), workspace.numel() * 4, scale, batch, heads, kv_heads, dim, pages, page_size,
-              slot_count, columns, page_table.stride(0), window, sinks, _FOUR(*query.stride()),
-              _FOUR(*key_pages.stride()), _FOUR(*value_pages.stride()), _stream(query))
+    _launch("flux_paged_decode_attention", query.device, _TYPES[query.dtype], query.data_ptr(), key_pages.data_ptr(),
+            value_pages.data_ptr(), page_table.data_ptr(), lengths.data_ptr(), _address(slots), output.data_ptr(),
+            workspace.data_ptr(), workspace.numel() * 4, scale, batch, heads, kv_heads, dim, pages, page_size, slot_count,
+            columns, page_table.stride(0), window, sinks, _four(*query.stride()), _four(*key_pages.stride()),
+            _four(*value_pages.stride()))
 
 
 def _paged_cuda(query, key_pages, value_pages, page_table, lengths, scale, window=0, sinks=0, slots=None):
     _validate_paged(query, key_pages, value_pages, page_table, lengths, scale, window, sinks, slots)
     _check(query.is_cuda, "flux::paged_decode_attention: CUDA dispatch requires CUDA tensors")
     output = query.new_empty(query.shape)
-    workspace = torch.empty(paged_decode_workspace_bytes(query, key_pages, page_table, window, sinks) // 4,
-                            dtype=torch.float32, device=query.device)
+    workspace = lengths.new_empty(paged_decode_workspace_bytes(query, key_pages, page_table, window, sinks) // 4,
+                                  dtype=torch.float32)
     _launch_paged(query, key_pages, value_pages, page_table, lengths, scale, window, sinks, slots, output, workspace)
     return output
 
@@ -206,20 +222,26 @@ def _paged_out_cuda(query, key_pages, value_pages, page_table, lengths, scale, w
 
 def _validate_window(query, key, value, scale, window, sinks=0, lengths=None, starts=None) -> None:
     shape, keys, dtype, device = query.shape, key.shape, query.dtype, query.device
-    _check(len(shape) == 4 and len(keys) == 4 and value.dim() == 4,
-           "flux::window_attention: query, key and value must be rank four")
-    _check(dtype in _TYPES and key.dtype is dtype and value.dtype is dtype,
-           "flux::window_attention: query, key and value must share dtype float32, float16 or bfloat16")
-    _check(keys == value.shape, "flux::window_attention: key and value shapes must match")
-    _check(0 not in shape and 0 not in keys, "flux::window_attention: tensor dimensions must be non-empty")
-    _check(shape[0] == keys[0], "flux::window_attention: batch sizes must match")
-    _check(shape[3] == keys[3] and shape[3] <= _MAX_DIM,
-           "flux::window_attention: head dimensions must match and be at most 256")
-    _check(shape[1] % keys[1] == 0, "flux::window_attention: query heads must be divisible by KV heads")
-    _check(keys[2] <= _MAX_KEYS, "flux::window_attention: more than 16777216 keys")
-    _check(key.device == device and value.device == device, "flux::window_attention: tensor devices must match")
-    _check(key.stride(3) == 1 and value.stride(3) == 1 or keys[3] == 1,
-           "flux::window_attention: key and value must have unit stride along the head dimension")
+    if not (len(shape) == 4 and len(keys) == 4 and value.dim() == 4):
+        _check(False, "flux::window_attention: query, key and value must be rank four")
+    if not (dtype in _TYPES and key.dtype is dtype and value.dtype is dtype):
+        _check(False, "flux::window_attention: query, key and value must share dtype float32, float16 or bfloat16")
+    if not (keys == value.shape):
+        _check(False, "flux::window_attention: key and value shapes must match")
+    if not (0 not in shape and 0 not in keys):
+        _check(False, "flux::window_attention: tensor dimensions must be non-empty")
+    if not (shape[0] == keys[0]):
+        _check(False, "flux::window_attention: batch sizes must match")
+    if not (shape[3] == keys[3] and shape[3] <= _MAX_DIM):
+        _check(False, "flux::window_attention: head dimensions must match and be at most 256")
+    if not (shape[1] % keys[1] == 0):
+        _check(False, "flux::window_attention: query heads must be divisible by KV heads")
+    if not (keys[2] <= _MAX_KEYS):
+        _check(False, "flux::window_attention: more than 16777216 keys")
+    if not (key.device == device and value.device == device):
+        _check(False, "flux::window_attention: tensor devices must match")
+    if not (key.stride(3) == 1 and value.stride(3) == 1 or keys[3] == 1):
+        _check(False, "flux::window_attention: key and value must have unit stride along the head dimension")
     if lengths is not None:
         _check_list(lengths, torch.int64, device,
                     "flux::window_attention: lengths must be a contiguous int64 vector on the query device",
@@ -228,9 +250,10 @@ def _validate_window(query, key, value, scale, window, sinks=0, lengths=None, st
         _check_list(starts, torch.int64, device,
                     "flux::window_attention: starts must be a contiguous int64 vector on the query device",
                     shape[0], "flux::window_attention: starts must have one entry per sequence")
-    _check(0 <= window <= _MAX_KEYS and 0 <= sinks <= _MAX_KEYS,
-           "flux::window_attention: window and sinks must be within [0, 16777216]")
-    _check(_finite_fp32(scale), "flux::window_attention: scale must be a finite FP32 value")
+    if not (0 <= window <= _MAX_KEYS and 0 <= sinks <= _MAX_KEYS):
+        _check(False, "flux::window_attention: window and sinks must be within [0, 16777216]")
+    if not (_finite_fp32(scale)):
+        _check(False, "flux::window_attention: scale must be a finite FP32 value")
     if torch.is_grad_enabled():
         _grad_free("flux::window_attention", query, key, value)
 
@@ -240,16 +263,15 @@ def _window_cuda(query, key, value, scale, window, sinks=0, lengths=None, starts
     _check(query.is_cuda, "flux::window_attention: CUDA dispatch requires CUDA tensors")
     batch, heads, queries, dim = query.shape
     kv_heads, keys = key.shape[1], key.shape[2]
-    output = torch.empty(query.shape, dtype=query.dtype, device=query.device)
+    output = query.new_empty(query.shape)
     needed, workspace = 0, None
     if queries == 1:
         needed = _size_from("flux_window_attention_workspace_bytes", batch, heads, kv_heads, 1, dim, keys, window, sinks)
-        workspace = torch.empty(needed // 4, dtype=torch.float32, device=query.device)
-    with _on(query.device):
-        _call("flux_window_attention", _TYPES[query.dtype], query.data_ptr(), key.data_ptr(), value.data_ptr(),
-              _address(lengths), _address(starts), output.data_ptr(), _address(workspace), needed, scale, batch,
-              heads, kv_heads, queries, keys, dim, window, sinks, _FOUR(*query.stride()), _FOUR(*key.stride()),
-              _FOUR(*value.stride()), _stream(query))
+        workspace = query.new_empty(needed // 4, dtype=torch.float32)
+    _launch("flux_window_attention", query.device, _TYPES[query.dtype], query.data_ptr(), key.data_ptr(), value.data_ptr(),
+            _address(lengths), _address(starts), output.data_ptr(), _address(workspace), needed, scale, batch, heads,
+            kv_heads, queries, keys, dim, window, sinks, _four(*query.stride()), _four(*key.stride()),
+            _four(*value.stride()))
     return output
 
 
@@ -308,11 +330,13 @@ def _validate_books(op, page_table, lengths, refcounts) -> None:
         _check(False, f"{op}: page_table rows must not overlap")
     device = page_table.device
     if lengths is not None:
-        if lengths.dim() != 1 or lengths.dtype is not torch.int64 or lengths.device != device or not lengths.is_contiguous():
+        if (lengths.dim() != 1 or lengths.dtype is not torch.int64 or lengths.device != device or
+                not lengths.is_contiguous()):
             _check(False, f"{op}: lengths must be a contiguous int64 vector on the page_table device")
         if lengths.shape[0] != slots:
             _check(False, f"{op}: lengths must have one entry per page_table row")
-    if refcounts.dim() != 1 or refcounts.dtype is not torch.int32 or refcounts.device != device or not refcounts.is_contiguous():
+    if (refcounts.dim() != 1 or refcounts.dtype is not torch.int32 or refcounts.device != device or
+            not refcounts.is_contiguous()):
         _check(False, f"{op}: refcounts must be a contiguous int32 vector on the page_table device")
     if refcounts.shape[0] == 0:
         _check(False, f"{op}: refcounts must have one entry per page")
@@ -324,20 +348,18 @@ def _validate_requests(op, name, requests, like) -> None:
         _check(False, f"{op}: {name} must be a contiguous int64 vector on the cache's device")
 
 
-def _pool(key_pages, value_pages) -> _native.PagePool:
+def _pool(key_pages, value_pages) -> bytes:
+    layers, *shape = key_pages.shape if key_pages.dim() == 5 else (1, *key_pages.shape)
     key_strides, value_strides = key_pages.stride(), value_pages.stride()
-    if key_pages.dim() == 4:
-        layers, shape = 1, key_pages.shape
+    if len(key_strides) == 4:
         key_strides, value_strides = (0, *key_strides), (0, *value_strides)
-    else:
-        layers, shape = key_pages.shape[0], key_pages.shape[1:]
-    return _native.PagePool(key_pages.data_ptr(), value_pages.data_ptr(), layers, *shape, _FOUR(*key_strides[:4]),
-                            _FOUR(*value_strides[:4]), _TYPES[key_pages.dtype])
+    return _page_pool(key_pages.data_ptr(), value_pages.data_ptr(), layers, *shape, *key_strides[:4], *value_strides[:4],
+                      _TYPES[key_pages.dtype])
 
 
-def _books(page_table, lengths, refcounts, page_size) -> _native.PageBooks:
-    return _native.PageBooks(page_table.data_ptr(), page_table.stride(0), page_table.shape[0], page_table.shape[1],
-                             _address(lengths), refcounts.data_ptr(), refcounts.shape[0], page_size)
+def _books(page_table, lengths, refcounts, page_size) -> bytes:
+    return _page_books(page_table.data_ptr(), page_table.stride(0), *page_table.shape,
+                       0 if lengths is None else lengths.data_ptr(), refcounts.data_ptr(), refcounts.shape[0], page_size)
 
 
 def _page_size_of(key_pages) -> int:
@@ -347,8 +369,8 @@ def _page_size_of(key_pages) -> int:
 def _validate_reserve(page_table, lengths, refcounts, page_size, slots, counts=None) -> None:
     op = "flux::paged_cache_reserve"
     _validate_books(op, page_table, lengths, refcounts)
-    _check(page_size > 0 and page_table.shape[1] * page_size <= _MAX_KEYS,
-           f"{op}: page_size must be positive and a page_table row hold at most 16777216 positions")
+    if not (page_size > 0 and page_table.shape[1] * page_size <= _MAX_KEYS):
+        _check(False, f"{op}: page_size must be positive and a page_table row hold at most 16777216 positions")
     _validate_requests(op, "slots", slots, page_table)
     if counts is not None:
         _validate_requests(op, "counts", counts, page_table)
@@ -360,15 +382,13 @@ def _reserve_cuda(page_table, lengths, refcounts, page_size, slots, counts=None)
     _require_gpu("flux::paged_cache_reserve", page_table)
     requests = slots.shape[0]
     positions = torch.empty_like(slots)
-    status = torch.empty(requests, dtype=torch.int32, device=slots.device)
+    status = page_table.new_empty(requests)
     if requests == 0:
         return positions, status
     words = _size_from("flux_page_reserve_workspace_words", requests, page_table.shape[0], refcounts.shape[0])
-    workspace = torch.empty(words, dtype=torch.int32, device=slots.device)
-    with _on(slots.device):
-        _call("flux_page_reserve", ctypes.byref(_books(page_table, lengths, refcounts, page_size)), slots.data_ptr(),
-              _address(counts), requests, positions.data_ptr(), status.data_ptr(), workspace.data_ptr(), words,
-              _stream(slots))
+    workspace = page_table.new_empty(words)
+    _launch("flux_page_reserve", slots.device, _books(page_table, lengths, refcounts, page_size), slots.data_ptr(),
+            _address(counts), requests, positions.data_ptr(), status.data_ptr(), workspace.data_ptr(), words)
     return positions, status
 
 
@@ -377,17 +397,18 @@ def _validate_write(key, value, key_pages, value_pages, page_table, slots, posit
     _validate_pools(op, key_pages, value_pages, (4,))
     _validate_table(op, page_table)
     shape, pages, dtype, device = key.shape, key_pages.shape, key_pages.dtype, key_pages.device
-    _check(page_table.device == device, "flux::paged_cache_write: tensor devices must match")
-    _check(page_table.shape[1] * pages[2] <= _MAX_KEYS,
-           "flux::paged_cache_write: page_table holds more than 16777216 positions a row")
-    _check(len(shape) == 4 and value.shape == shape,
-           "flux::paged_cache_write: key and value must be rank four and of one shape")
-    _check(key.dtype is dtype and value.dtype is dtype and key.device == device and value.device == device,
-           "flux::paged_cache_write: key and value must have the pages' dtype and device")
-    _check(shape[1] == pages[1] and shape[3] == pages[3],
-           "flux::paged_cache_write: key heads and head dimension must be the pages'")
-    _check(key.stride(3) == 1 and value.stride(3) == 1 or shape[3] == 1,
-           "flux::paged_cache_write: key and value must have unit stride along the head dimension")
+    if not (page_table.device == device):
+        _check(False, "flux::paged_cache_write: tensor devices must match")
+    if not (page_table.shape[1] * pages[2] <= _MAX_KEYS):
+        _check(False, "flux::paged_cache_write: page_table holds more than 16777216 positions a row")
+    if not (len(shape) == 4 and value.shape == shape):
+        _check(False, "flux::paged_cache_write: key and value must be rank four and of one shape")
+    if not (key.dtype is dtype and value.dtype is dtype and key.device == device and value.device == device):
+        _check(False, "flux::paged_cache_write: key and value must have the pages' dtype and device")
+    if not (shape[1] == pages[1] and shape[3] == pages[3]):
+        _check(False, "flux::paged_cache_write: key heads and head dimension must be the pages'")
+    if not (key.stride(3) == 1 and value.stride(3) == 1 or shape[3] == 1):
+        _check(False, "flux::paged_cache_write: key and value must have unit stride along the head dimension")
     requests = shape[0]
     _check_list(slots, torch.int64, device,
                 "flux::paged_cache_write: slots must be a contiguous int64 vector on the cache's device",
@@ -399,7 +420,8 @@ def _validate_write(key, value, key_pages, value_pages, page_table, slots, posit
         _check_list(counts, torch.int64, device,
                     "flux::paged_cache_write: counts must be a contiguous int64 vector on the cache's device",
                     requests, "flux::paged_cache_write: counts must have one entry per request")
-    _check(requests <= 65535, "flux::paged_cache_write: more than 65535 requests")
+    if not (requests <= 65535):
+        _check(False, "flux::paged_cache_write: more than 65535 requests")
     if torch.is_grad_enabled():
         _grad_free(op, key, value)
 
@@ -416,11 +438,9 @@ def _write_cuda(key, value, key_pages, value_pages, page_table, slots, positions
     _require_gpu("flux::paged_cache_write", key_pages)
     if key.shape[0] == 0 or key.shape[2] == 0:
         return
-    with _on(key_pages.device):
-        _call("flux_page_write", ctypes.byref(_pool(key_pages, value_pages)), key.data_ptr(), value.data_ptr(),
-              _FOUR(*key.stride()), _FOUR(*value.stride()), key.shape[0], key.shape[2],
-              page_table.data_ptr(), page_table.stride(0), page_table.shape[0], page_table.shape[1], slots.data_ptr(),
-              positions.data_ptr(), _address(counts), _stream(key_pages))
+    _launch("flux_page_write", key_pages.device, _pool(key_pages, value_pages), key.data_ptr(), value.data_ptr(),
+            _four(*key.stride()), _four(*value.stride()), key.shape[0], key.shape[2], page_table.data_ptr(),
+            page_table.stride(0), *page_table.shape, slots.data_ptr(), positions.data_ptr(), _address(counts))
 
 
 def _validate_copy(key_pages, value_pages, source, target) -> None:
@@ -428,17 +448,17 @@ def _validate_copy(key_pages, value_pages, source, target) -> None:
     _validate_pools(op, key_pages, value_pages)
     _validate_requests(op, "source", source, key_pages)
     _validate_requests(op, "target", target, key_pages)
-    _check(source.shape == target.shape, f"{op}: source and target must have one length")
+    if not (source.shape == target.shape):
+        _check(False, f"{op}: source and target must have one length")
 
 
 def _copy_cuda(key_pages, value_pages, source, target):
     _validate_copy(key_pages, value_pages, source, target)
     _require_gpu("flux::paged_cache_copy", key_pages)
-    status = torch.empty(source.shape[0], dtype=torch.int32, device=source.device)
+    status = source.new_empty(source.shape[0], dtype=torch.int32)
     if source.shape[0]:
-        with _on(source.device):
-            _call("flux_page_copy", ctypes.byref(_pool(key_pages, value_pages)), source.data_ptr(), target.data_ptr(),
-                  source.shape[0], status.data_ptr(), _stream(source))
+        _launch("flux_page_copy", source.device, _pool(key_pages, value_pages), source.data_ptr(), target.data_ptr(),
+                source.shape[0], status.data_ptr())
     return status
 
 
@@ -451,11 +471,10 @@ def _validate_free(page_table, lengths, refcounts, slots) -> None:
 def _free_cuda(page_table, lengths, refcounts, slots):
     _validate_free(page_table, lengths, refcounts, slots)
     _require_gpu("flux::paged_cache_free", page_table)
-    status = torch.empty(slots.shape[0], dtype=torch.int32, device=slots.device)
+    status = page_table.new_empty(slots.shape[0])
     if slots.shape[0]:
-        with _on(slots.device):
-            _call("flux_page_free", ctypes.byref(_books(page_table, lengths, refcounts, 1)), slots.data_ptr(),
-                  slots.shape[0], status.data_ptr(), _stream(slots))
+        _launch("flux_page_free", slots.device, _books(page_table, lengths, refcounts, 1), slots.data_ptr(),
+                slots.shape[0], status.data_ptr())
     return status
 
 
@@ -463,28 +482,30 @@ def _validate_fork(key_pages, value_pages, page_table, lengths, refcounts, paren
     op = "flux::paged_cache_fork"
     _validate_pools(op, key_pages, value_pages)
     _validate_books(op, page_table, lengths, refcounts)
-    _check(page_table.device == key_pages.device, f"{op}: tensor devices must match")
-    _check(refcounts.shape[0] == key_pages.shape[-4], f"{op}: refcounts must have one entry per page")
-    _check(page_table.shape[1] * key_pages.shape[-2] <= _MAX_KEYS,
-           f"{op}: page_table holds more than 16777216 positions a row")
+    if not (page_table.device == key_pages.device):
+        _check(False, f"{op}: tensor devices must match")
+    if not (refcounts.shape[0] == key_pages.shape[-4]):
+        _check(False, f"{op}: refcounts must have one entry per page")
+    if not (page_table.shape[1] * key_pages.shape[-2] <= _MAX_KEYS):
+        _check(False, f"{op}: page_table holds more than 16777216 positions a row")
     _validate_requests(op, "parents", parents, key_pages)
     _validate_requests(op, "children", children, key_pages)
-    _check(parents.shape == children.shape, f"{op}: parents and children must have one length")
+    if not (parents.shape == children.shape):
+        _check(False, f"{op}: parents and children must have one length")
 
 
 def _fork_cuda(key_pages, value_pages, page_table, lengths, refcounts, parents, children):
     _validate_fork(key_pages, value_pages, page_table, lengths, refcounts, parents, children)
     _require_gpu("flux::paged_cache_fork", key_pages)
     requests = parents.shape[0]
-    status = torch.empty(requests, dtype=torch.int32, device=parents.device)
+    status = page_table.new_empty(requests)
     if requests == 0:
         return status
     words = _size_from("flux_page_fork_workspace_words", requests, page_table.shape[0], refcounts.shape[0])
-    workspace = torch.empty(words, dtype=torch.int32, device=parents.device)
-    with _on(parents.device):
-        _call("flux_page_fork", ctypes.byref(_pool(key_pages, value_pages)),
-              ctypes.byref(_books(page_table, lengths, refcounts, _page_size_of(key_pages))), parents.data_ptr(),
-              children.data_ptr(), requests, status.data_ptr(), workspace.data_ptr(), words, _stream(parents))
+    workspace = page_table.new_empty(words)
+    _launch("flux_page_fork", parents.device, _pool(key_pages, value_pages),
+            _books(page_table, lengths, refcounts, _page_size_of(key_pages)), parents.data_ptr(), children.data_ptr(),
+            requests, status.data_ptr(), workspace.data_ptr(), words)
     return status
 
 
@@ -492,22 +513,23 @@ def _validate_compact(key_pages, value_pages, page_table, refcounts) -> None:
     op = "flux::paged_cache_compact"
     _validate_pools(op, key_pages, value_pages)
     _validate_books(op, page_table, None, refcounts)
-    _check(page_table.device == key_pages.device, f"{op}: tensor devices must match")
-    _check(refcounts.shape[0] == key_pages.shape[-4], f"{op}: refcounts must have one entry per page")
+    if not (page_table.device == key_pages.device):
+        _check(False, f"{op}: tensor devices must match")
+    if not (refcounts.shape[0] == key_pages.shape[-4]):
+        _check(False, f"{op}: refcounts must have one entry per page")
 
 
 def _compact_cuda(key_pages, value_pages, page_table, refcounts):
     _validate_compact(key_pages, value_pages, page_table, refcounts)
     _require_gpu("flux::paged_cache_compact", key_pages)
     pages = refcounts.shape[0]
-    page_map = torch.empty(pages, dtype=torch.int32, device=refcounts.device)
-    used = torch.empty((), dtype=torch.int64, device=refcounts.device)
+    page_map = refcounts.new_empty(pages)
+    used = refcounts.new_empty((), dtype=torch.int64)
     words = _size_from("flux_page_compact_workspace_words", pages)
-    workspace = torch.empty(words, dtype=torch.int32, device=refcounts.device)
-    with _on(refcounts.device):
-        _call("flux_page_compact", ctypes.byref(_pool(key_pages, value_pages)),
-              ctypes.byref(_books(page_table, None, refcounts, _page_size_of(key_pages))), page_map.data_ptr(),
-              used.data_ptr(), workspace.data_ptr(), words, _stream(refcounts))
+    workspace = refcounts.new_empty(words)
+    _launch("flux_page_compact", refcounts.device, _pool(key_pages, value_pages),
+            _books(page_table, None, refcounts, _page_size_of(key_pages)), page_map.data_ptr(), used.data_ptr(),
+            workspace.data_ptr(), words)
     return page_map, used
 
 
@@ -527,18 +549,21 @@ def _validate_penalty(name, penalty, device, rows, history) -> None:
 def _validate_logits(logits, history=None, history_lengths=None, repetition=None, frequency=None, presence=None,
                      bias=None, allowed=None) -> None:
     shape, device = logits.shape, logits.device
-    _check(len(shape) == 2 and shape[0] > 0 and 0 < shape[1] <= _MAX_VOCAB,
-           "flux::logits_process: logits must be [rows, vocab], non-empty, vocab at most 16777216")
-    _check(logits.dtype in _TYPES, "flux::logits_process: logits must have dtype float32, float16 or bfloat16")
+    if not (len(shape) == 2 and shape[0] > 0 and 0 < shape[1] <= _MAX_VOCAB):
+        _check(False, "flux::logits_process: logits must be [rows, vocab], non-empty, vocab at most 16777216")
+    if not (logits.dtype in _TYPES):
+        _check(False, "flux::logits_process: logits must have dtype float32, float16 or bfloat16")
     rows, vocab = shape
-    _check(logits.stride(1) == 1 or vocab == 1, "flux::logits_process: logits rows must be contiguous")
+    if not (logits.stride(1) == 1 or vocab == 1):
+        _check(False, "flux::logits_process: logits rows must be contiguous")
     if history is not None:
         width = history.shape
         _check(len(width) == 2 and width[0] == rows and history.dtype is torch.int64,
                "flux::logits_process: history must be int64 [rows, width]")
         _check(history.stride(1) == 1 or width[1] <= 1, "flux::logits_process: history rows must be contiguous")
         _check(history.device == device, "flux::logits_process: tensor devices must match")
-    _check(history is not None or history_lengths is None, "flux::logits_process: history_lengths needs a history")
+    if not (history is not None or history_lengths is None):
+        _check(False, "flux::logits_process: history_lengths needs a history")
     if history_lengths is not None:
         _check_list(history_lengths, torch.int64, device,
                     "flux::logits_process: history_lengths must be a contiguous int64 vector on the logits device",
@@ -573,16 +598,15 @@ def _logits_cuda(logits, history=None, history_lengths=None, repetition=None, fr
     _validate_logits(logits, history, history_lengths, repetition, frequency, presence, bias, allowed)
     _require_gpu("flux::logits_process", logits)
     rows, vocab = logits.shape
-    processed = torch.empty((rows, vocab), dtype=logits.dtype, device=logits.device)
-    tokens = torch.empty(rows, dtype=torch.int64, device=logits.device)
+    processed = logits.new_empty((rows, vocab))
+    tokens = logits.new_empty(rows, dtype=torch.int64)
     needed = _size_from("flux_logits_process_workspace_bytes", rows, vocab)
-    workspace = torch.empty(needed, dtype=torch.uint8, device=logits.device) if needed else None
-    with _on(logits.device):
-        _call("flux_logits_process", _TYPES[logits.dtype], logits.data_ptr(), logits.stride(0), processed.data_ptr(),
-              tokens.data_ptr(), rows, vocab, _address(history), 0 if history is None else history.shape[1],
-              0 if history is None else history.stride(0), _address(history_lengths), _address(repetition),
-              _address(frequency), _address(presence), _address(bias), _row_stride(bias), _address(allowed),
-              _row_stride(allowed), _address(workspace), needed, _stream(logits))
+    workspace = tokens.new_empty(needed // 8) if needed else None
+    _launch("flux_logits_process", logits.device, _TYPES[logits.dtype], logits.data_ptr(), logits.stride(0),
+            processed.data_ptr(), tokens.data_ptr(), rows, vocab, _address(history),
+            0 if history is None else history.shape[1], 0 if history is None else history.stride(0),
+            _address(history_lengths), _address(repetition), _address(frequency), _address(presence), _address(bias),
+            _row_stride(bias), _address(allowed), _row_stride(allowed), _address(workspace), needed)
     return processed, tokens
 
 
