@@ -9,8 +9,8 @@
 // (integers, so the order of the additions does not show), then writes.  Few tokens are in a history: a bit per token
 // says which, and only those take the penalties' path, whose results replace the counts.  The best token is looked for by
 // unit: a unit's largest value first (maximum keeps a NaN), its place in the unit once for the workgroup's best.
-// HBM and the latency of its phases bound a batch (128 rows of 128000 in bfloat16, 65.5 MB: 24 us with histories of 4096,
-// a bias and a mask, 2.7 TB/s; 14 us without, where a copy takes 10.5), launches one row.
+// HBM and the latency of its phases bound a batch (128 rows of 128000 in bfloat16, 65.5 MB: 22 us with histories of 4096,
+// a bias and a mask, 24 if stored through the caches; 13.4 us without them, where a copy takes 10.5), launches one row.
 #include "serving.h"
 
 namespace flux {
@@ -73,7 +73,7 @@ struct Unit {
         }
     }
     __device__ __forceinline__ void store(T* to) const {
-        if constexpr (kWide) *reinterpret_cast<uint4*>(to) = make_uint4(word[0], word[1], word[2], word[3]);
+        if constexpr (kWide) store_past_caches(to, Quad{word[0], word[1], word[2], word[3]});
         else *to = static_cast<T>(value(word[0], 0));
     }
     __device__ __forceinline__ void round(const float (&y)[kWidth]) {
@@ -270,8 +270,8 @@ __global__ void __launch_bounds__(64) logits_token_kernel(const uint64_t* __rest
     if (threadIdx.x == 0) tokens[row] = ~static_cast<uint32_t>(rank);
 }
 
-// Tokens of a workgroup: 8192 with 512 threads (the batch above: 24 us; 4096 with 256, which read the history twice as
-// often, 27), unless that leaves CUs without one.
+// Tokens of a workgroup: 8192 with 512 threads (the batch above; 4096 with 256, which read the history twice as
+// often, take 3 us more), unless that leaves CUs without one.
 constexpr int kLargeChunk = 8192, kSmallChunk = 2048;
 int logits_chunk(int64_t rows, int64_t vocab) {
     return rows * ((vocab + kLargeChunk - 1) / kLargeChunk) >= 256 ? kLargeChunk : kSmallChunk;

@@ -34,6 +34,13 @@ __device__ __forceinline__ uint32_t divide(uint32_t n, const Divider& d) {
     return (__umulhi(n, d.magic) + n) >> d.shift;  // n < 2^31 and the high product is below n: the sum fits
 }
 
+// Sixteen bytes past the caches, for what is written in bulk and not read soon: dirty lines that wait for the kernel's end
+// are written back all at once then.
+typedef uint32_t Quad __attribute__((ext_vector_type(4)));
+__device__ __forceinline__ void store_past_caches(void* to, Quad value) {
+    __builtin_nontemporal_store(value, static_cast<Quad*>(to));
+}
+
 // ---- attention ----
 
 // Keys and values: pages behind a table (pages > 0), or one contiguous run per sequence (pages == 0).
