@@ -229,7 +229,7 @@ __global__ void __launch_bounds__(256) page_free_kernel(PageBooks b, const int64
 // requests kAhead of them before it writes any.
 constexpr int kAhead = 4;
 
-// Past the caches in units of 16 bytes (512 of 2048 pages of 8 layers, 268 MB moved: 120 us through the caches, 98 past
+// Past the caches in units of 16 bytes (40 pages of 30 layers, 29 MB: 22.0 us a call through the caches, 12.9 past
 // them; 12 MB of new rows: 13.8 and 8.8; 1920 partial pages, 12 MB: 23.3 and 8.6).
 template <class Unit>
 __device__ __forceinline__ void store_unit(char* to, const Unit& held) {
