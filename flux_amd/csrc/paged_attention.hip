@@ -204,7 +204,7 @@ __global__ void __launch_bounds__(kDecodeThreads, kDim * sizeof(T) <= 512 ? 2 : 
 #pragma unroll
     for (int i = 0; i < kBlocks; ++i) out[i] = f32x4{0, 0, 0, 0};
     float top = -INFINITY, weight = 0.0f;
-    typename M::Fragment query[kFragments];  // right operand of S^T: this lane's query head, zero behind the last one
+    typename M::Fragment query[kFragments];  // right operand of S^T: this lane's query head, behind the last one the first
 
     auto work = [&](Tile& tile) {
         if (tile.partial) {  // a weight of zero does not undo a NaN
@@ -260,7 +260,7 @@ __global__ void __launch_bounds__(kDecodeThreads, kDim * sizeof(T) <= 512 ? 2 : 
     {
         const int64_t head = kv_head * static_cast<int64_t>(a.group) + column0 + (n16 < columns ? n16 : 0);
         const T* q = static_cast<const T*>(a.query) + b * a.query_strides[0] + head * a.query_strides[1];
-        load_query<T, kFragments, M::kKeyStep>(query, q, a.query_strides[3], a.query_wide, M::kPer * g, a.dim, n16 < columns);
+        load_query<T, kFragments, M::kKeyStep>(query, q, a.query_strides[3], a.query_wide, M::kPer * g, a.dim);
     }
     // A wave's tile numbers are the same in all its lanes, and said to be: the branches on them are scalar.
     const int first_tile = __builtin_amdgcn_readfirstlane(from + wave);

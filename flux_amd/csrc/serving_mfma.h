@@ -251,10 +251,11 @@ struct Mfma<_Float16> : Mfma16<_Float16, Mfma<_Float16>> {
     }
 };
 
-// The fragments of one query row, zero behind its dims, all zero unless `real` (the row's memory is valid either way).
+// The fragments of one query row, zero behind its dims.  Columns without a row of their own take another's: results of
+// one column depend on no other, and theirs are not stored.
 template <class T, int kFragments, int kStep>
 __device__ __forceinline__ void load_query(typename Mfma<T>::Fragment (&query)[kFragments], const T* row, int64_t stride,
-                                           bool wide, int first, int dim, bool real) {
+                                           bool wide, int first, int dim) {
     using M = Mfma<T>;
     if (wide) {
 #pragma unroll
@@ -263,8 +264,10 @@ __device__ __forceinline__ void load_query(typename Mfma<T>::Fragment (&query)[k
 #pragma unroll
         for (int f = 0; f < kFragments; ++f) query[f] = M::load_strided(row, stride, kStep * f + first, dim);
     }
+    if (dim < kFragments * kStep) {
 #pragma unroll
-    for (int f = 0; f < kFragments; ++f) query[f] = M::zero_behind(query[f], kStep * f + first, real ? dim : 0);
+        for (int f = 0; f < kFragments; ++f) query[f] = M::zero_behind(query[f], kStep * f + first, dim);
+    }
 }
 
 }  // namespace flux

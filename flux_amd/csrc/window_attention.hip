@@ -165,6 +165,9 @@ __global__ void __launch_bounds__(kThreads, kDim <= 64 ? 4 : (kDim <= 128 ? 2 : 
     const float* keys = static_cast<const float*>(a.key) + rows.b * a.key_strides[0] + rows.kv_head * a.key_strides[1];
     const float* values = static_cast<const float*>(a.value) + rows.b * a.value_strides[0] + rows.kv_head * a.value_strides[1];
 
+    int first_p, last_p;
+    rows.positions(a, rows.row0, kRows, first_p, last_p);
+    const KeyTiles<kTile> tiles(a, first_p, last_p);
     RowRange mine[kCols];
     int sink_end[kCols];
     f32x4 query[kCols][kFragments];
@@ -179,15 +182,13 @@ __global__ void __launch_bounds__(kThreads, kDim <= 64 ? 4 : (kDim <= 128 ? 2 : 
         mine[c] = rows.range(a, r, i);
         sink_end[c] = a.sinks < mine[c].low ? a.sinks : mine[c].low;
         const float* q = static_cast<const float*>(a.query) + rows.b * a.query_strides[0] + head * a.query_strides[1] + i * a.query_strides[2];
-        load_query<float, kFragments, M::kKeyStep>(query[c], q, a.query_strides[3], a.query_wide, M::kPer * g, a.dim, real);
+        if (tiles.count > 0)  // a padded batch has many tiles of rows that are no key's
+            load_query<float, kFragments, M::kKeyStep>(query[c], q, a.query_strides[3], a.query_wide, M::kPer * g, a.dim);
 #pragma unroll
         for (int k = 0; k < kBlocks; ++k) out[c][k] = f32x4{0, 0, 0, 0};
         top[c] = -INFINITY;
         weight[c] = 0.0f;
     }
-    int first_p, last_p;
-    rows.positions(a, rows.row0, kRows, first_p, last_p);
-    const KeyTiles<kTile> tiles(a, first_p, last_p);
     const int low_of_last = a.window > 0 && last_p >= a.window ? last_p - a.window + 1 : 0;
 
     struct Tile {
@@ -443,12 +444,6 @@ window_tile_kernel(AttentionArgs a, int row_tiles, int tiles_total) {
     const int sink_end = a.sinks < mine.low ? a.sinks : mine.low;
     const uint32_t sign = a.scale < 0.0f ? 0x80008000u : 0u;  // the scale's sign goes to the query
     const float factor = fmaxf(fabsf(a.scale) * kLog2e, 1e-37f);  // above 0: a masked score stays -inf
-    u32x4 query[kSteps];
-    load_query<T, kSteps, 16>(query, static_cast<const T*>(a.query) + rows.b * a.query_strides[0] + head * a.query_strides[1] +
-                                         query_index * a.query_strides[2],
-                              a.query_strides[3], a.query_wide, 8 * half, a.dim, real);
-#pragma unroll
-    for (int s = 0; s < kSteps; ++s) query[s] ^= sign;
     f32x16 out[kBlocks];
 #pragma unroll
     for (int i = 0; i < kBlocks; ++i)
@@ -456,7 +451,13 @@ window_tile_kernel(AttentionArgs a, int row_tiles, int tiles_total) {
         for (int j = 0; j < 16; ++j) out[i][j] = 0.0f;
     float top = -INFINITY, weight = 0.0f;
 
-    if (block_first <= block_last) {
+    if (block_first <= block_last) {  // a padded batch has many tiles of rows that are no key's
+        u32x4 query[kSteps];
+        load_query<T, kSteps, 16>(query, static_cast<const T*>(a.query) + rows.b * a.query_strides[0] + head * a.query_strides[1] +
+                                             query_index * a.query_strides[2],
+                                  a.query_strides[3], a.query_wide, 8 * half, a.dim);
+#pragma unroll
+        for (int s = 0; s < kSteps; ++s) query[s] ^= sign;
         const KeyTiles<kKeys> tiles(a, block_first, block_last);
         const int seen = tiles.seen, count = tiles.count;
         auto low_of = [&](int p) { return a.window > 0 && p >= a.window ? p - a.window + 1 : 0; };
