@@ -39,16 +39,8 @@ __device__ __forceinline__ int wave_sum_int(int v) {
 // How rows are read: element by element, in 16-byte loads, or those where the head fills the padded dims.  Loads are not
 // masked (masks put each one in a block of its own, behind a wait for the register's last value): dims behind the head's
 // repeat its first ones, which meet zeros of the query (and are cleared themselves where an infinity in them must not
-// show, by key_dims) or results that are not stored.
+// show, by multiply_keys) or results that are not stored.
 enum Rows : int { kNarrow = 0, kWideRows = 1, kFullRows = 2 };
-
-// A fragment of a key row as loaded by load_row, zero behind the head's dims.
-template <class M, Rows kRows>
-__device__ __forceinline__ typename M::Fragment key_dims(const typename M::Fragment& f, int d, int dim) {
-    if constexpr (kRows == kFullRows) return f;
-    if constexpr (kRows == kWideRows) return d < dim ? f : typename M::Fragment{};
-    return M::zero_behind(f, d, dim);
-}
 
 template <class T>
 struct Mfma;
@@ -251,11 +243,22 @@ struct Mfma<_Float16> : Mfma16<_Float16, Mfma<_Float16>> {
     }
 };
 
-// The fragments of one query row, zero behind its dims.  Columns without a row of their own take another's: results of
-// one column depend on no other, and theirs are not stored.
+// The scores of 16 keys, whose rows were loaded by load_row; kClear clears the dims behind the head's.
+template <class M, bool kClear, int kFragments>
+__device__ __forceinline__ f32x4 multiply_keys(const typename M::Fragment (&key)[kFragments],
+                                               const typename M::Fragment (&query)[kFragments], int group, int dim) {
+    f32x4 score = {0, 0, 0, 0};
+#pragma unroll
+    for (int f = 0; f < kFragments; ++f)
+        M::multiply_key(kClear ? M::zero_behind(key[f], M::kKeyStep * f + M::kPer * group, dim) : key[f], query[f], score);
+    return score;
+}
+
+// The fragments of one query row, zero behind its dims, all zero unless `real` (the row's memory is valid either way:
+// products with zeros draw less power).
 template <class T, int kFragments, int kStep>
 __device__ __forceinline__ void load_query(typename Mfma<T>::Fragment (&query)[kFragments], const T* row, int64_t stride,
-                                           bool wide, int first, int dim) {
+                                           bool wide, int first, int dim, bool real) {
     using M = Mfma<T>;
     if (wide) {
 #pragma unroll
@@ -264,9 +267,9 @@ __device__ __forceinline__ void load_query(typename Mfma<T>::Fragment (&query)[k
 #pragma unroll
         for (int f = 0; f < kFragments; ++f) query[f] = M::load_strided(row, stride, kStep * f + first, dim);
     }
-    if (dim < kFragments * kStep) {
+    if (dim < kFragments * kStep || !__all(real)) {
 #pragma unroll
-        for (int f = 0; f < kFragments; ++f) query[f] = M::zero_behind(query[f], kStep * f + first, dim);
+        for (int f = 0; f < kFragments; ++f) query[f] = M::zero_behind(query[f], kStep * f + first, real ? dim : 0);
     }
 }
 

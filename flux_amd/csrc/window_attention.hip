@@ -183,7 +183,7 @@ __global__ void __launch_bounds__(kThreads, kDim <= 64 ? 4 : (kDim <= 128 ? 2 : 
         sink_end[c] = a.sinks < mine[c].low ? a.sinks : mine[c].low;
         const float* q = static_cast<const float*>(a.query) + rows.b * a.query_strides[0] + head * a.query_strides[1] + i * a.query_strides[2];
         if (tiles.count > 0)  // a padded batch has many tiles of rows that are no key's
-            load_query<float, kFragments, M::kKeyStep>(query[c], q, a.query_strides[3], a.query_wide, M::kPer * g, a.dim);
+            load_query<float, kFragments, M::kKeyStep>(query[c], q, a.query_strides[3], a.query_wide, M::kPer * g, a.dim, real);
 #pragma unroll
         for (int k = 0; k < kBlocks; ++k) out[c][k] = f32x4{0, 0, 0, 0};
         top[c] = -INFINITY;
@@ -333,7 +333,7 @@ __global__ void __launch_bounds__(kThreads, kDim <= 64 ? 4 : (kDim <= 128 ? 2 : 
 // ---------------------------------------------------------------------------
 // 16-bit prompts.  Here matrix instructions, exponentials and LDS reads cost about the same, so that keys and values are
 // staged once for the workgroup's four waves, 32 rows each.  4 x 4096 tokens (padded), 32 / 8 heads of 128, window 1024 in
-// bfloat16: 240 us, 700 TFLOP/s.  A 32 x 32 tile costs a SIMD 512 cycles of matrix instructions and as many of vector
+// bfloat16: 230 us, 720 TFLOP/s.  A 32 x 32 tile costs a SIMD 512 cycles of matrix instructions and as many of vector
 // instructions (half of them exponentials), and the two waves of a SIMD overlap them in part: 64 rows a wave (one wave
 // per SIMD) took 640 us, a workgroup of eight waves 236, two tiles per maximum 244.
 //
@@ -455,7 +455,7 @@ window_tile_kernel(AttentionArgs a, int row_tiles, int tiles_total) {
         u32x4 query[kSteps];
         load_query<T, kSteps, 16>(query, static_cast<const T*>(a.query) + rows.b * a.query_strides[0] + head * a.query_strides[1] +
                                              query_index * a.query_strides[2],
-                                  a.query_strides[3], a.query_wide, 8 * half, a.dim);
+                                  a.query_strides[3], a.query_wide, 8 * half, a.dim, real);
 #pragma unroll
         for (int s = 0; s < kSteps; ++s) query[s] ^= sign;
         const KeyTiles<kKeys> tiles(a, block_first, block_last);

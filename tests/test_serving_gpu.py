@@ -687,6 +687,22 @@ def test_logits_ties_go_to_the_lowest_index(gpu_device, dtype, rows, vocab):
         assert tokens.tolist() == [places[0]] * rows
 
 
+@pytest.mark.parametrize("rows,vocab", [(1, 2 ** 24), (2, 2 ** 24 - 5), (70001, 5)])
+def test_logits_of_the_largest_shapes(gpu_device, rows, vocab):
+    g = torch.Generator().manual_seed(rows)
+    logits = torch.randn(rows, vocab, generator=g).half()
+    at = torch.randint(0, vocab, (rows,), generator=g)
+    logits[torch.arange(rows), at] = 100.0
+    history = torch.stack([at, (at + 1) % vocab], 1)
+    processed, tokens = ops.logits_process_native(logits.to(gpu_device), history.to(gpu_device),
+                                                  presence=torch.full((rows,), 0.5, device=gpu_device))
+    assert torch.equal(tokens.cpu(), at)
+    expected = logits.float()
+    for column in range(2):
+        expected[torch.arange(rows), history[:, column]] -= 0.5
+    assert torch.equal(processed.cpu(), expected.half())
+
+
 def test_logits_strides(gpu_device):
     case = _logits_case(3, torch.float16, 4, 4096, 64, bias_rows=4)
     device = _to(case, gpu_device)
