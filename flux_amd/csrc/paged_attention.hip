@@ -9,7 +9,7 @@
 // into parts of about the same number of tiles as every other part of the batch, one per workgroup, so that ragged
 // lengths load the card evenly; the parts of a sequence that was cut leave (o, m, l) in the workspace and a second launch
 // joins them: o = sum o_c exp(m_c - M) / sum l_c exp(m_c - M).  (48 sequences to 16384, 32 / 8 heads of 128 in bfloat16:
-// 400 us, 4.5 TB/s; 24 to 8192, 9 / 3 heads of 64 in float32: 46 us, the join 6.6 of them.)
+// 400 us, 4.5 TB/s; 24 to 8192, 9 / 3 heads of 64 in float32: 44 us, the join 4.6 of them.)
 //
 // A wave takes 16 or 32 keys at a time straight into registers, laid out as the matrix instruction wants them, while the
 // tile before is worked on.  Scores come as S^T = K Q^T (rows: keys, columns: query heads), so the lane that holds
@@ -76,6 +76,14 @@ __device__ __forceinline__ int part_begin(int tiles, int parts, int part) {
 __device__ __forceinline__ int64_t partial_offset(const AttentionArgs& a, int64_t head_tile, int64_t block, int column) {
     const int columns = a.group < kColumns ? a.group : kColumns;
     return ((head_tile * (a.blocks + a.batch) + block) * columns + column) * (a.dim + 2);
+}
+
+// The parts' place of each sequence, behind the partials: its first workgroup and their number.  The sequence's first part
+// leaves it for the launch that joins them (derived from the lengths again, a join takes 1.2 us longer).
+__device__ __host__ __forceinline__ int64_t plan_offset(const AttentionArgs& a) {
+    const int64_t columns = a.group < kColumns ? a.group : kColumns;
+    const int64_t heads = static_cast<int64_t>(a.kv_heads) * ((a.group + kColumns - 1) / kColumns);
+    return heads * (a.blocks + a.batch) * columns * (a.dim + 2);
 }
 
 // Sum over the workgroup, the same in every thread.
@@ -145,6 +153,11 @@ __global__ void __launch_bounds__(kDecodeThreads, kDim * sizeof(T) <= 512 ? 2 : 
     __syncthreads();
     const int b = chosen[0], part = chosen[2], parts = chosen[3];
     const Span span = span_of<kTile>(a, chosen[1]);
+    if (blockIdx.y == 0 && part == 0 && threadIdx.x == 0) {
+        int* plan = reinterpret_cast<int*>(a.workspace + plan_offset(a)) + 2 * b;
+        plan[0] = blockIdx.x;
+        plan[1] = parts;
+    }
     const int from = part_begin(span.tiles, parts, part), to = part_begin(span.tiles, parts, part + 1);
     const int64_t slot = kPaged && a.slots ? a.slots[b] : b;
     const int32_t* row = kPaged ? a.table + (span.tiles > 0 ? slot : 0) * a.table_stride : nullptr;
@@ -344,30 +357,14 @@ __global__ void __launch_bounds__(kDecodeThreads, kDim * sizeof(T) <= 512 ? 2 : 
 // tile's heads and dims): the parts' shares first.
 constexpr int kJoinParts = 128;  // parts whose shares are kept
 
-template <class T, int kTile>
+template <class T>
 __global__ void __launch_bounds__(kDecodeThreads) decode_join_kernel(AttentionArgs a) {
-    __shared__ int sums[kDecodeWaves];
-    __shared__ int mine_seen;
     __shared__ float share[kJoinParts][kColumns];
     __shared__ float tops[kColumns], weights[kColumns];
     const int b = blockIdx.x;
-    int64_t total = 0;
-    int seen = 0;
-    for (int base = 0; base < a.batch; base += kDecodeThreads) {
-        const int i = base + static_cast<int>(threadIdx.x);
-        seen = i < a.batch ? seen_of(a, i) : 0;
-        if (i == b) mine_seen = seen;
-        total += block_sum(span_of<kTile>(a, seen).tiles, sums);
-    }
-    const int each = part_tiles(total, a.blocks, a.least);
-    const int parts = parts_of(span_of<kTile>(a, mine_seen).tiles, each);
+    const int* plan = reinterpret_cast<const int*>(a.workspace + plan_offset(a)) + 2 * b;
+    const int first = plan[0], parts = plan[1];
     if (parts == 1) return;
-    int64_t first = 0;
-    for (int base = 0; base < b; base += kDecodeThreads) {
-        const int i = base + static_cast<int>(threadIdx.x);
-        if (a.batch > kDecodeThreads) seen = i < a.batch ? seen_of(a, i) : 0;
-        first += block_sum(i < b ? parts_of(span_of<kTile>(a, seen).tiles, each) : 0, sums);
-    }
     const int column_tiles = (a.group + kColumns - 1) / kColumns;
     const int column0 = blockIdx.y % column_tiles * kColumns;
     const int columns = a.group - column0 < kColumns ? a.group - column0 : kColumns;
@@ -452,7 +449,7 @@ hipError_t launch_decode(AttentionArgs a, hipStream_t stream) {
     if (launched != hipSuccess) return launched;
     if (whole) return hipSuccess;
     const int items = ((a.group < kColumns ? a.group : kColumns) * a.dim + kDecodeThreads - 1) / kDecodeThreads;
-    hipLaunchKernelGGL(HIP_KERNEL_NAME(decode_join_kernel<T, tile_of(kDim, sizeof(T))>), dim3(a.batch, a.kv_heads * column_tiles, items),
+    hipLaunchKernelGGL(HIP_KERNEL_NAME(decode_join_kernel<T>), dim3(a.batch, a.kv_heads * column_tiles, items),
                        dim3(kDecodeThreads), 0, stream, a);
     return hipGetLastError();
 }
@@ -482,9 +479,7 @@ int decode_attention_blocks(int batch, int64_t keys, int kv_heads, int group, in
 }
 
 size_t decode_attention_workspace_floats(const AttentionArgs& a) {
-    const size_t columns = a.group < kColumns ? a.group : kColumns;
-    const size_t heads = static_cast<size_t>(a.kv_heads) * ((a.group + kColumns - 1) / kColumns);
-    return heads * (a.blocks + a.batch) * columns * (a.dim + 2);
+    return static_cast<size_t>(plan_offset(a) + 2 * static_cast<int64_t>(a.batch));
 }
 
 hipError_t launch_decode_attention(const AttentionArgs& args, Type type, hipStream_t stream) {
