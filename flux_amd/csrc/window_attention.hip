@@ -443,7 +443,11 @@ window_tile_kernel(AttentionArgs a, int row_tiles, int tiles_total) {
     const RowRange mine = rows.range(a, r, query_index);
     const int sink_end = a.sinks < mine.low ? a.sinks : mine.low;
     const uint32_t sign = a.scale < 0.0f ? 0x80008000u : 0u;  // the scale's sign goes to the query
-    const float factor = fmaxf(fabsf(a.scale) * kLog2e, 1e-37f);  // above 0: a masked score stays -inf
+    // Its size goes into the exponent's argument, unless it is 0 (which makes a masked score's -inf NaN, and has to make an
+    // infinite score NaN) or next to what float32 holds: then it multiplies the scores before they are masked.
+    const float size = fabsf(a.scale);
+    const bool ordinary = size >= 1e-30f && size <= 1e30f;
+    const float factor = ordinary ? size * kLog2e : kLog2e;
     f32x16 out[kBlocks];
 #pragma unroll
     for (int i = 0; i < kBlocks; ++i)
@@ -537,6 +541,10 @@ window_tile_kernel(AttentionArgs a, int row_tiles, int tiles_total) {
                 for (int j = 0; j < 16; ++j) score[j] = 0.0f;
 #pragma unroll
                 for (int k = 0; k < kSteps; ++k) score = W::multiply(key[k], query[k], score);
+                if (!ordinary) {
+#pragma unroll
+                    for (int j = 0; j < 16; ++j) score[j] *= size;
+                }
                 if (first < low_of_last || last > wave_first) {
 #pragma unroll
                     for (int j = 0; j < 16; ++j) {

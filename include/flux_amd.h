@@ -456,7 +456,8 @@ int flux_gqa_decode_attention_strided_f32(const float* query, const float* key_c
 
 /* ---- Serving: a paged K/V cache, windowed attention, logits ----
  * Element type of query, key, value, cache pages and logits.  Strides are in elements and non-negative; the head
- * dimension of keys, values and pages has stride 1.  Softmax statistics and sums are float32 (integers for counts). */
+ * dimension of keys, values and pages has stride 1.  Softmax statistics and sums are float32 (integers for counts); a
+ * product <q, k> is such a sum before the scale multiplies it. */
 enum flux_dtype { FLUX_FLOAT32 = 0, FLUX_FLOAT16 = 1, FLUX_BFLOAT16 = 2 };
 
 /* One new token per sequence over a paged cache.  Sequence b uses row r = slots[b] (b when slots is NULL) of

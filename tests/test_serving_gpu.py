@@ -324,6 +324,54 @@ def test_window_scales(gpu_device, dtype, dim, scale):
 
 
 @pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("dim", [64, 128, 40])
+def test_window_scale_of_zero_makes_infinite_scores_nan(gpu_device, dtype, dim):
+    """0 * inf is NaN, for one query as for many; rows that do not see the key are means of their values."""
+    case = {**_window_case(47, dtype, 1, 3, 1, dim, 40, 40), "scale": 0.0}
+    case["query"][..., 0] = case["query"][..., 0].abs() + 0.5
+    finite = {**case, "key": case["key"].clone()}
+    case["key"][0, 0, 25, 0] = -math.inf
+    expected = ref.window_attention(**case, window=10)
+    lost = expected.isnan().all(-1)[0, 0]
+    assert lost.nonzero().flatten().tolist() == list(range(25, 35))
+    out = ops.window_attention_native(**_to(case, gpu_device), window=10).cpu()
+    assert out[:, :, lost].isnan().all()
+    bound = ref.attention_bound(finite["query"], finite["key"], finite["value"], 0.0, 10, dtype, expected, True)
+    _close(out[:, :, ~lost], expected[:, :, ~lost], bound[:, :, ~lost])
+    for n in (25, 26, 35, 36):
+        one = ops.window_attention_native(**_to({**case, "query": case["query"][:, :, :1]}, gpu_device), window=10,
+                                          lengths=torch.tensor([n], device=gpu_device))
+        assert bool(one.isnan().all()) == bool(lost[n - 1])
+
+
+@pytest.mark.parametrize("scale", [2.0 ** -126, -(2.0 ** -126), 2.0 ** -103, 2.0 ** 103, 2.0 ** 120, 3e38])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_window_scales_next_to_what_float32_holds(gpu_device, dtype, scale):
+    """Queries and keys that bring the scores back to ordinary ones, exactly: powers of two.  <q, k> is a float32 sum before
+    the scale: from key 16 on it is j 2^124 >= 2^128 at the smallest scales, an infinite score."""
+    case = {**_window_case(53, dtype, 1, 2, 1, 64, 40, 40), "scale": scale}
+    each = 2.0 ** math.floor(-math.log2(abs(scale)) / 2)
+    case["query"] = torch.full_like(case["query"], each)
+    case["key"] = torch.zeros_like(case["key"])
+    case["key"][0, 0, :, 3] = torch.arange(40.0) * each / 4
+    raw = case["key"][0, 0, :, 3].double() * each
+    bounded = {**case, "key": torch.where(raw.float().isinf()[:, None], 0.0, case["key"].double()).to(dtype)}
+    scores = raw.float().double() * float(torch.tensor(scale))
+    for window, sinks in ((0, 0), (9, 2)):
+        expected = torch.zeros(1, 2, 40, 64, dtype=torch.float64)
+        for i in range(40):
+            seen = ref.visible_keys(i, 40, window, sinks)
+            weights = torch.exp(scores[seen] - scores[seen].max())
+            expected[0, :, i] = weights @ case["value"][0, 0, seen].double() / weights.sum()
+        lost = expected.isnan()
+        assert bool(lost.any()) == (scale == 2.0 ** -126)
+        out = ops.window_attention_native(**_to(case, gpu_device), window=window, sinks=sinks).cpu()
+        assert torch.equal(out.isnan(), lost)
+        bound = ref.attention_bound(bounded["query"], bounded["key"], bounded["value"], scale, 40, dtype, expected, True)
+        _close(out.nan_to_num(), expected.nan_to_num(), bound.nan_to_num())
+
+
+@pytest.mark.parametrize("dtype", TYPES)
 def test_window_padded_batches_and_chunks(gpu_device, dtype):
     case = _window_case(9, dtype, 5, 6, 2, 64, 70, 70)
     out = _check_window(case, gpu_device, 16, 2, lengths=[70, 1, 0, 33, 64], starts=[0] * 5)
