@@ -779,6 +779,64 @@ bool overlap(const void* a, int64_t a_bytes, const void* b, int64_t b_bytes) {
     return from_a < from_b + static_cast<uintptr_t>(b_bytes) && from_b < from_a + static_cast<uintptr_t>(a_bytes);
 }
 
+// The dimensions of a side that have more than one element, by rising step.
+struct SideSteps {
+    int count = 0;
+    int64_t step[5], size[5];
+
+    SideSteps(const flux::PagePool& p, const int64_t* strides) {
+        const int64_t sizes[5] = {p.layers, p.pages, p.heads, p.page, p.dim};
+        for (int i = 0; i < 5; ++i) {
+            if (sizes[i] == 1) continue;
+            const int64_t by = i < 4 ? strides[i] : 1;
+            int at = count++;
+            for (; at > 0 && step[at - 1] > by; --at) step[at] = step[at - 1], size[at] = size[at - 1];
+            step[at] = by, size[at] = sizes[i];
+        }
+    }
+    // The last element that the dimensions of steps below `period` reach.
+    __int128 reach(int64_t period) const {
+        __int128 sum = 0;
+        for (int i = 0; i < count && step[i] < period; ++i) sum += static_cast<__int128>(step[i]) * (size[i] - 1);
+        return sum;
+    }
+    // No two elements share memory: each dimension steps over all smaller ones.
+    bool written_once() const {
+        for (int i = 0; i < count; ++i)
+            if (step[i] == 0 || (i > 0 && (step[i] == step[i - 1] || step[i] <= reach(step[i])))) return false;
+        return true;
+    }
+    bool whole_periods(int64_t period) const {
+        for (int i = 0; i < count; ++i)
+            if (step[i] >= period && step[i] % period) return false;
+        return true;
+    }
+};
+
+// Whether the sides share no memory: one ends before the other starts, or, where they are interleaved, every step is below
+// a period or a multiple of it, and the parts below it lie apart in it.
+bool sides_apart(const flux::PagePool& p, const SideSteps& key, const SideSteps& value) {
+    const __int128 bytes = static_cast<__int128>(reinterpret_cast<uintptr_t>(p.value)) - reinterpret_cast<uintptr_t>(p.key);
+    if (bytes >= (key.reach(INT64_MAX) + 1) * p.element || -bytes >= (value.reach(INT64_MAX) + 1) * p.element) return true;
+    if (bytes % p.element) return false;
+    for (int i = 0; i < key.count; ++i) {
+        const int64_t period = key.step[i];
+        const __int128 offset = (bytes / p.element % period + period) % period;
+        if (key.reach(period) < offset && offset + value.reach(period) < period && key.whole_periods(period) &&
+            value.whole_periods(period))
+            return true;
+    }
+    return false;
+}
+
+// What the operators that write pages ask of the pool's memory; null when it is in order.
+const char* pool_memory(const flux::PagePool& p) {
+    const SideSteps key(p, p.key_strides), value(p, p.value_strides);
+    if (!key.written_once() || !value.written_once()) return "key and value pages must not overlap themselves";
+    if (!sides_apart(p, key, value)) return "key and value pages must not overlap";
+    return nullptr;
+}
+
 // Whether a list of requests lies in the books that its kernel changes while it reads the list again.
 bool list_in_books(const int64_t* list, int64_t requests, const flux::PageBooks& b) {
     if (!list) return false;
@@ -905,6 +963,7 @@ int flux_page_write(const flux_page_pool* pool, const void* key, const void* val
         return invalid("flux_page_write: invalid shape");
     if (!nonnegative(key_strides, 3) || !nonnegative(value_strides, 3))
         return invalid("flux_page_write: negative strides are unsupported");
+    if (const char* wrong = pool_memory(p)) return invalid(std::string("flux_page_write: ") + wrong);
     flux::PageWriteArgs args{};
     args.key = static_cast<const char*>(key);
     args.value = static_cast<const char*>(value);
@@ -930,6 +989,7 @@ int flux_page_copy(const flux_page_pool* pool, const int64_t* source, const int6
     if (const char* wrong = pool_arguments(p, pool)) return invalid(std::string("flux_page_copy: ") + wrong);
     if (!source || !target || !status || requests <= 0 || requests > (1 << 20))
         return invalid("flux_page_copy: invalid argument");
+    if (const char* wrong = pool_memory(p)) return invalid(std::string("flux_page_copy: ") + wrong);
     return from_hip(flux::launch_page_copy(p, source, target, requests, status, stream), "flux_page_copy");
 }
 
@@ -962,6 +1022,7 @@ int flux_page_fork(const flux_page_pool* pool, const flux_page_books* books, con
         return invalid("flux_page_fork: workspace too small (flux_page_fork_workspace_words)");
     if (list_in_books(parents, requests, b) || list_in_books(children, requests, b))
         return invalid("flux_page_fork: parents and children must not lie in the books");
+    if (const char* wrong = pool_memory(p)) return invalid(std::string("flux_page_fork: ") + wrong);
     return from_hip(flux::launch_page_fork(p, b, parents, children, requests, status, workspace, stream),
                     "flux_page_fork");
 }
@@ -983,6 +1044,7 @@ int flux_page_compact(const flux_page_pool* pool, const flux_page_books* books, 
         return invalid("flux_page_compact: invalid books");
     if (workspace_words < static_cast<int64_t>(flux::page_compact_workspace(p.pages)))
         return invalid("flux_page_compact: workspace too small (flux_page_compact_workspace_words)");
+    if (const char* wrong = pool_memory(p)) return invalid(std::string("flux_page_compact: ") + wrong);
     flux::PageBooks b{};
     b.table = books->page_table;
     b.table_stride = books->table_stride;

@@ -16,6 +16,7 @@ from __future__ import annotations
 
 import ctypes
 import functools
+import math
 import struct
 
 import torch
@@ -290,6 +291,36 @@ def _written_once(tensor) -> bool:
     return True
 
 
+def _pools_apart(key_pages, value_pages) -> bool:
+    """No element of one lies in the other: one ends before the other starts, or, where they are interleaved, every step is
+    below a period or a multiple of it, and the parts below it lie apart in it."""
+    size = key_pages.element_size()
+    between = value_pages.data_ptr() - key_pages.data_ptr()
+    if key_pages.is_contiguous() and value_pages.is_contiguous():
+        return abs(between) >= key_pages.numel() * size
+    key, value = ([(step, count) for step, count in zip(pages.stride(), pages.shape) if count > 1]
+                  for pages in (key_pages, value_pages))
+
+    def reach(steps, below):
+        return sum(step * (count - 1) for step, count in steps if step < below)
+
+    if between >= (reach(key, math.inf) + 1) * size or -between >= (reach(value, math.inf) + 1) * size:
+        return True
+    if between % size:
+        return False
+    for period, _ in key:
+        offset = between // size % period
+        if (reach(key, period) < offset and offset + reach(value, period) < period and
+                not any(step % period for step, _ in key + value if step >= period)):
+            return True
+    return False
+
+
+def _validate_pool_memory(op, key_pages, value_pages) -> None:
+    if not _pools_apart(key_pages, value_pages):
+        _check(False, f"{op}: key_pages and value_pages must not overlap")
+
+
 def _validate_pools(op, key_pages, value_pages, ranks=(4, 5)) -> None:
     shape, dtype, key_stride, value_stride = key_pages.shape, key_pages.dtype, key_pages.stride(), value_pages.stride()
     if len(shape) not in ranks or len(value_stride) != len(shape):
@@ -431,6 +462,7 @@ def _validate_write_memory(key, value, key_pages, value_pages, page_table, slots
     stores = key_pages.untyped_storage().data_ptr(), value_pages.untyped_storage().data_ptr()
     _check(key.untyped_storage().data_ptr() not in stores and value.untyped_storage().data_ptr() not in stores,
            "flux::paged_cache_write: the pages must not alias key or value")
+    _validate_pool_memory("flux::paged_cache_write", key_pages, value_pages)
 
 
 def _write_cuda(key, value, key_pages, value_pages, page_table, slots, positions, counts=None):
@@ -452,8 +484,13 @@ def _validate_copy(key_pages, value_pages, source, target) -> None:
         _check(False, f"{op}: source and target must have one length")
 
 
-def _copy_cuda(key_pages, value_pages, source, target):
+def _validate_copy_memory(key_pages, value_pages, source, target) -> None:
     _validate_copy(key_pages, value_pages, source, target)
+    _validate_pool_memory("flux::paged_cache_copy", key_pages, value_pages)
+
+
+def _copy_cuda(key_pages, value_pages, source, target):
+    _validate_copy_memory(key_pages, value_pages, source, target)
     _require_gpu("flux::paged_cache_copy", key_pages)
     status = source.new_empty(source.shape[0], dtype=torch.int32)
     if source.shape[0]:
@@ -494,8 +531,13 @@ def _validate_fork(key_pages, value_pages, page_table, lengths, refcounts, paren
         _check(False, f"{op}: parents and children must have one length")
 
 
-def _fork_cuda(key_pages, value_pages, page_table, lengths, refcounts, parents, children):
+def _validate_fork_memory(key_pages, value_pages, page_table, lengths, refcounts, parents, children) -> None:
     _validate_fork(key_pages, value_pages, page_table, lengths, refcounts, parents, children)
+    _validate_pool_memory("flux::paged_cache_fork", key_pages, value_pages)
+
+
+def _fork_cuda(key_pages, value_pages, page_table, lengths, refcounts, parents, children):
+    _validate_fork_memory(key_pages, value_pages, page_table, lengths, refcounts, parents, children)
     _require_gpu("flux::paged_cache_fork", key_pages)
     requests = parents.shape[0]
     status = page_table.new_empty(requests)
@@ -519,8 +561,13 @@ def _validate_compact(key_pages, value_pages, page_table, refcounts) -> None:
         _check(False, f"{op}: refcounts must have one entry per page")
 
 
-def _compact_cuda(key_pages, value_pages, page_table, refcounts):
+def _validate_compact_memory(key_pages, value_pages, page_table, refcounts) -> None:
     _validate_compact(key_pages, value_pages, page_table, refcounts)
+    _validate_pool_memory("flux::paged_cache_compact", key_pages, value_pages)
+
+
+def _compact_cuda(key_pages, value_pages, page_table, refcounts):
+    _validate_compact_memory(key_pages, value_pages, page_table, refcounts)
     _require_gpu("flux::paged_cache_compact", key_pages)
     pages = refcounts.shape[0]
     page_map = refcounts.new_empty(pages)
@@ -619,10 +666,10 @@ _KERNELS = {
     "window_attention": (_window_cuda, _validate_window),
     "paged_cache_reserve": (_reserve_cuda, _validate_reserve),
     "paged_cache_write": (_write_cuda, _validate_write_memory),
-    "paged_cache_copy": (_copy_cuda, _validate_copy),
-    "paged_cache_fork": (_fork_cuda, _validate_fork),
+    "paged_cache_copy": (_copy_cuda, _validate_copy_memory),
+    "paged_cache_fork": (_fork_cuda, _validate_fork_memory),
     "paged_cache_free": (_free_cuda, _validate_free),
-    "paged_cache_compact": (_compact_cuda, _validate_compact),
+    "paged_cache_compact": (_compact_cuda, _validate_compact_memory),
     "logits_process": (_logits_cuda, _validate_logits),
 }
 

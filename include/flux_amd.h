@@ -513,7 +513,9 @@ typedef struct {
     int64_t pages;
     int64_t page_size;
 } flux_page_books;
-/* key, value [layers, pages, heads, page_size, head_dim]; strides of the first four dimensions. */
+/* key, value [layers, pages, heads, page_size, head_dim]; strides of the first four dimensions.  No two elements that a call
+ * may write share memory: a side whose rows overlap, and sides that overlap, are refused (interleaved ones are fine where
+ * every stride is below a common period or a multiple of it and the sides lie apart within the period). */
 typedef struct {
     void* key;
     void* value;

@@ -200,6 +200,56 @@ def test_pages_that_are_written_lie_apart(name):
         getattr(torch.ops.flux, name)(**{**args, **padded})
 
 
+def _side_views(shape):
+    """(name, key, value, whether they share memory) of one storage, over the layouts that pools come in."""
+    *outer, heads, rows, dim = shape
+    count = torch.empty(shape).numel()
+    page = heads * rows * dim
+    flat = torch.zeros(8 * count + 64)
+    halves = flat[: 2 * count].view(2, *shape)
+    yield "one after the other", halves[0], halves[1], False
+    yield "the other after one", halves[1], halves[0], False
+    by_page = flat[: 2 * count].view(*outer, 2, heads, rows, dim)
+    yield "interleaved by page", by_page[..., 0, :, :, :], by_page[..., 1, :, :, :], False
+    by_row = flat[: 2 * count].view(*outer, heads, rows, 2, dim)
+    yield "interleaved by row", by_row[..., 1, :], by_row[..., 0, :], False
+    turned = flat[: 2 * count].view(*outer, 2, page)
+    yield ("interleaved by page, rows before heads", turned[..., 0, :].unflatten(-1, (heads, rows, dim)),
+           turned[..., 1, :].unflatten(-1, (rows, heads, dim)).transpose(-2, -3), False)
+    padded = flat[: count // dim * (2 * dim + 5)].view(*outer, heads, rows, 2 * dim + 5)
+    yield "interleaved in wider rows", padded[..., :dim], padded[..., dim + 3 : 2 * dim + 3], False
+    yield "wider rows that meet", padded[..., : dim], padded[..., dim - 1 : 2 * dim - 1], True
+    yield "a page on", flat[:count].view(shape), flat[page : page + count].view(shape), True
+    yield "an element on", flat[1 : count + 1].view(shape), flat[:count].view(shape), True
+    yield "the last element", flat[:count].view(shape), flat[count - 1 : 2 * count - 1].view(shape), True
+    yield "the next element", flat[:count].view(shape), flat[count : 2 * count].view(shape), False
+    yield "other strides", flat[:count].view(shape), flat[:count].view(*outer, rows, heads, dim).transpose(-2, -3), True
+    by_page = flat[: 2 * count].view(*outer, 2, page)
+    yield ("interleaved and half a page on", by_page[..., 0, :].unflatten(-1, (heads, rows, dim)),
+           flat[page // 2 : 2 * count + page // 2].view(*outer, 2, page)[..., 1, :].unflatten(-1, (heads, rows, dim)), True)
+
+
+def _shares_memory(key, value):
+    def places(t):
+        at = torch.zeros(t.shape, dtype=torch.int64)
+        for d, step in enumerate(t.stride()):
+            at += (torch.arange(t.shape[d]) * step).view([-1 if i == d else 1 for i in range(t.dim())])
+        return set((at + t.storage_offset()).flatten().tolist())
+
+    return bool(places(key) & places(value))
+
+
+@pytest.mark.parametrize("name", PAGES_CALLS)
+def test_pools_that_share_memory_are_refused(name):
+    """Interleaved pools stay allowed; two views of one storage that meet in an element are not."""
+    args = CALLS[name]()
+    for what, key, value, shared in _side_views(tuple(args["key_pages"].shape)):
+        assert _shares_memory(key, value) == shared, what
+        message = "key_pages and value_pages must not overlap" if shared else "no CPU kernel"
+        with pytest.raises(RuntimeError, match=message):
+            getattr(torch.ops.flux, name)(**{**args, "key_pages": key, "value_pages": value})
+
+
 @pytest.mark.parametrize("name,change,message", [r for r in REFUSED if "requires_grad" not in str(r[1])][::4])
 def test_fake_tensors_are_refused_alike(name, change, message):
     mode = FakeTensorMode()
@@ -305,6 +355,44 @@ def test_c_entries_refuse_lists_inside_the_books():
             for parents, children in ((where, apart), (apart, where)):
                 assert lib.flux_page_fork(_pool_struct(), books, parents, children, 2, some, some, 100, None) == bad
                 assert "must not lie in the books" in _native.last_error()
+
+
+def test_c_entries_refuse_pages_that_share_memory():
+    """Every entry that writes pages, on addresses that nothing reads: the sides are in order in none of the calls."""
+    lib, bad, some = _native.load(), _native.FLUX_ERROR_INVALID_VALUE, ctypes.c_void_p(16)
+
+    def pool(key, value):
+        layers, pages, heads, rows, dim = key.shape
+        out = _native.PagePool(key=0x100000 + 4 * key.storage_offset(), value=0x100000 + 4 * value.storage_offset(),
+                               layers=layers, pages=pages, heads=heads, page_size=rows, head_dim=dim, dtype=0)
+        out.key_strides[:], out.value_strides[:] = key.stride()[:4], value.stride()[:4]
+        return ctypes.byref(out)
+
+    three = (ctypes.c_int64 * 3)(64, 32, 8)
+
+    def message_of(key, value):
+        p, found = pool(key, value), set()
+        books = _books_struct(pages=key.shape[1], page_size=key.shape[3], page_table=0x10000, lengths=0x20000, refcounts=0x30000)
+        calls = [lambda: lib.flux_page_copy(p, some, some, 1, some, None),
+                 lambda: lib.flux_page_fork(p, books, some, some, 1, some, some, 1000, None),
+                 lambda: lib.flux_page_compact(p, books, some, some, some, 1000, None)]
+        if key.shape[0] == 1:
+            calls.append(lambda: lib.flux_page_write(p, some, some, three, three, 1, 1, some, 4, 2, 4, some, some, None, None))
+        for call in calls:
+            assert call() == bad
+            found.add(_native.last_error().split(": ")[1])
+        assert len(found) == 1
+        return found.pop()
+
+    for shape in ((2, 7, 2, 4, 8), (1, 7, 2, 4, 8), (1, 1, 3, 5, 1), (2, 3, 1, 1, 4)):
+        for what, key, value, _ in _side_views(shape):
+            if key.stride(4) != 1 or value.stride(4) != 1 or not _shares_memory(key, value):
+                continue
+            assert message_of(key, value) == "key and value pages must not overlap", (shape, what)
+    key = torch.zeros(4000)[:448].view(1, 7, 2, 4, 8)
+    for strides in ((448, 63, 32, 8, 1), (448, 64, 31, 8, 1), (448, 64, 32, 7, 1), (448, 0, 32, 8, 1)):
+        assert message_of(key, torch.zeros(4000).as_strided(key.shape, strides, 1000)) == \
+            "key and value pages must not overlap themselves"
 
 
 # --------------------------------------------------------------------------- the plain page model
