@@ -761,6 +761,7 @@ const char* books_arguments(flux::PageBooks& out, const flux_page_books* books, 
         books->pages <= 0 || books->pages > (1 << 28) || books->page_size <= 0 ||
         books->page_size > FLUX_MAX_SERVING_KEYS || books->columns > FLUX_MAX_SERVING_KEYS / books->page_size)
         return "invalid books (columns * page_size is at most FLUX_MAX_SERVING_KEYS)";
+    if (books->slots > 1 && books->table_stride < books->columns) return "page_table rows must not overlap";
     if (requests <= 0 || requests > (1 << 20) || requests * books->columns >= (int64_t{1} << 31))
         return "invalid number of requests";
     out.table = books->page_table;
@@ -1042,6 +1043,8 @@ int flux_page_compact(const flux_page_pool* pool, const flux_page_books* books, 
     if (books->pages != p.pages || books->slots <= 0 || books->columns <= 0 || books->table_stride < 0 ||
         books->columns > (int64_t{1} << 40) / books->slots)
         return invalid("flux_page_compact: invalid books");
+    if (books->slots > 1 && books->table_stride < books->columns)
+        return invalid("flux_page_compact: page_table rows must not overlap");
     if (workspace_words < static_cast<int64_t>(flux::page_compact_workspace(p.pages)))
         return invalid("flux_page_compact: workspace too small (flux_page_compact_workspace_words)");
     if (const char* wrong = pool_memory(p)) return invalid(std::string("flux_page_compact: ") + wrong);

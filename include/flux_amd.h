@@ -495,7 +495,8 @@ int flux_window_attention(int dtype, const void* query, const void* key, const v
 /* Pages of a cache.  The books: page_table int32 [slots, columns] (-1: no page), lengths int64 [slots], refcounts
  * int32 [pages] (sequences that hold a page; 0: free).  Requests are served in their order, a needed page is the
  * lowest free one, and what became of each request is its flux_page_status; a refused request changes nothing.  Lists of
- * requests must not lie in the books (refused), nor may outputs and workspaces. */
+ * requests must not lie in the books (refused), nor may outputs and workspaces; rows of a page_table that is written must
+ * not overlap (table_stride below columns is refused). */
 enum flux_page_status {
     FLUX_PAGE_DONE = 0,
     FLUX_PAGE_OUT_OF_RANGE = 1, /* a slot, page, count or length outside its range */
@@ -539,7 +540,8 @@ int flux_page_reserve(const flux_page_books* books, const int64_t* slots, const 
                       hipStream_t stream);
 /* Rows of new tokens into one layer's pages (layers 1): key, value [requests, heads, tokens, head_dim], token t < counts[i]
  * (NULL: tokens) of request i to position positions[i] + t of slots[i].  Requests with a negative position or a slot
- * outside the table, tokens beyond the table's columns and tokens on no page are left out. */
+ * outside the table, tokens beyond the table's columns and tokens on no page are left out.  Two requests must not name the
+ * same rows, and key and value must not share memory with the rows that are written. */
 int flux_page_write(const flux_page_pool* pool, const void* key, const void* value, const int64_t* key_strides,
                     const int64_t* value_strides, int64_t requests, int64_t tokens, const int32_t* page_table,
                     int64_t table_stride, int64_t slots, int64_t columns, const int64_t* slot_list,

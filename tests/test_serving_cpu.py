@@ -395,6 +395,24 @@ def test_c_entries_refuse_pages_that_share_memory():
             "key and value pages must not overlap themselves"
 
 
+def test_c_entries_refuse_table_rows_that_overlap():
+    """Requests of different slots write their rows at the same time."""
+    lib, bad, some = _native.load(), _native.FLUX_ERROR_INVALID_VALUE, ctypes.c_void_p(16)
+    pool = _pool_struct(key=0x100000, value=0x200000)
+    for stride in (0, 1, 3):
+        books = _books_struct(table_stride=stride, page_table=0x10000, lengths=0x20000, refcounts=0x30000)
+        for call in (lambda: lib.flux_page_reserve(books, some, None, 2, some, some, some, 100, None),
+                     lambda: lib.flux_page_free(books, some, 2, some, None),
+                     lambda: lib.flux_page_fork(pool, books, some, some, 1, some, some, 100, None),
+                     lambda: lib.flux_page_compact(pool, books, some, some, some, 100, None)):
+            assert call() == bad
+            assert "rows must not overlap" in _native.last_error()
+    # One row overlaps nothing: the next check answers.
+    books = _books_struct(slots=1, table_stride=0, page_table=0x10000, lengths=0x20000, refcounts=0x30000)
+    assert lib.flux_page_reserve(books, some, None, 2, some, some, some, 3, None) == bad
+    assert "workspace too small" in _native.last_error()
+
+
 # --------------------------------------------------------------------------- the plain page model
 
 def test_page_model_keeps_every_sequence():
