@@ -97,6 +97,83 @@ __device__ __forceinline__ int64_t block_sum(int v, int* sums) {
 
 constexpr int tile_of(int dim, int bytes) { return dim * bytes <= 256 ? 32 : 16; }
 
+// A part of one query head in float32, for 16-bit results that are not finite: the two terms of a weight are of either sign or
+// zero, and their products with an infinite value would add up to NaN.  One wave.  It derives all it needs from the
+// arguments and `chosen` again: values kept for it would cost the kernel's loop registers.
+template <class T, int kTile, bool kPaged>
+__device__ void exact_part(const AttentionArgs& a, const int* chosen, int column) {
+    const int lane = threadIdx.x & 63;
+    const int column_tiles = (a.group + kColumns - 1) / kColumns;
+    const int kv_head = blockIdx.y / column_tiles;
+    const int64_t head = kv_head * static_cast<int64_t>(a.group) + blockIdx.y % column_tiles * kColumns + column;
+    const int b = chosen[0], part = chosen[2], parts = chosen[3];
+    const Span span = span_of<kTile>(a, chosen[1]);
+    const int from = part_begin(span.tiles, parts, part), to = part_begin(span.tiles, parts, part + 1);
+    const int32_t* row = kPaged ? a.table + (a.slots ? a.slots[b] : b) * a.table_stride : nullptr;
+    const T* query = static_cast<const T*>(a.query) + b * a.query_strides[0] + head * a.query_strides[1];
+    const T* keys = static_cast<const T*>(a.key) + kv_head * a.key_strides[1] + (kPaged ? 0 : b * a.key_strides[0]);
+    const T* values = static_cast<const T*>(a.value) + kv_head * a.value_strides[1] + (kPaged ? 0 : b * a.value_strides[0]);
+
+    float top = -INFINITY, weight = 0.0f, sum[kServingMaxDim / kWave];
+#pragma unroll
+    for (int c = 0; c < kServingMaxDim / kWave; ++c) sum[c] = 0.0f;
+    for (int base = from * kTile; base < to * kTile; base += kWave) {
+        const int t = (base + lane) / kTile;
+        const int position = (t < span.sink_tiles ? t : span.first_tile + t - span.sink_tiles) * kTile + (base + lane) % kTile;
+        bool seen = t < to && position < span.seen && (position >= span.low || position < span.sinks);
+        int64_t page = 0, in_page = position;
+        if (kPaged && seen) {
+            const uint32_t column_of = divide(position, a.page);
+            page = row[column_of];
+            in_page = position - column_of * a.page.divisor;
+            seen = page >= 0 && page < a.pages;
+        }
+        float score = -INFINITY;
+        if (seen) {
+            const T* key = keys + (kPaged ? page * a.key_strides[0] : 0) + in_page * a.key_strides[2];
+            score = 0.0f;
+            for (int d = 0; d < a.dim; ++d)
+                score = fmaf(static_cast<float>(query[d * a.query_strides[3]]), static_cast<float>(key[d]), score);
+            score *= a.scale;
+        }
+        const float now = fmaxf(top, wave_max(score));
+        const float reference = now == -INFINITY ? 0.0f : now;
+        const float shrink = top == -INFINITY ? 0.0f : fast_exp2((top - reference) * kLog2e);
+        top = now;
+        const float p = seen ? fast_exp2((score - reference) * kLog2e + Mfma<T>::kWeightShift) : 0.0f;
+        weight = weight * shrink + wave_sum(p);
+#pragma unroll
+        for (int c = 0; c < kServingMaxDim / kWave; ++c) sum[c] *= shrink;
+        const int64_t mine = seen ? (kPaged ? page * a.value_strides[0] : 0) + in_page * a.value_strides[2] : -1;
+        for (int j = 0; j < kWave; ++j) {
+            const int64_t of = __shfl(mine, j, kWave);
+            const float pj = __shfl(p, j, kWave);
+            if (of < 0) continue;
+#pragma unroll
+            for (int c = 0; c < kServingMaxDim / kWave; ++c)
+                if (kWave * c + lane < a.dim) sum[c] = fmaf(pj, static_cast<float>(values[of + kWave * c + lane]), sum[c]);
+        }
+        // What is NaN stays NaN: a head whose sums all are is done.
+        bool lost = true;
+#pragma unroll
+        for (int c = 0; c < kServingMaxDim / kWave; ++c) lost = lost && (kWave * c + lane >= a.dim || sum[c] != sum[c]);
+        if (__all(weight != weight || lost)) break;
+    }
+    T* out = static_cast<T*>(a.out) + (b * static_cast<int64_t>(a.query_heads) + head) * a.dim;
+    float* partial = a.workspace + partial_offset(a, blockIdx.y, blockIdx.x, column);
+#pragma unroll
+    for (int c = 0; c < kServingMaxDim / kWave; ++c) {
+        const int d = kWave * c + lane;
+        if (d >= a.dim) continue;
+        if (parts == 1) out[d] = static_cast<T>(weight == 0.0f ? 0.0f : sum[c] / weight);
+        else partial[d] = sum[c];
+    }
+    if (parts > 1 && lane == 0) {
+        partial[a.dim] = top;
+        partial[a.dim + 1] = weight;
+    }
+}
+
 template <class T, int kDim, bool kPaged, Rows kRows>
 __global__ void __launch_bounds__(kDecodeThreads, kDim * sizeof(T) <= 512 ? 2 : 1) decode_attention_kernel(AttentionArgs a) {
     using M = Mfma<T>;
@@ -336,19 +413,38 @@ __global__ void __launch_bounds__(kDecodeThreads, kDim * sizeof(T) <= 512 ? 2 : 
                 out[i / 4][i % 4] = out[i / 4][i % 4] * mine_scale + other[i][lane] * other_scale;
         }
     }
-    if (wave != 0 || n16 >= columns) return;
-    if (parts == 1) {
-        const int64_t head = kv_head * static_cast<int64_t>(a.group) + column0 + n16;
-        T* o = static_cast<T*>(a.out) + (b * static_cast<int64_t>(a.query_heads) + head) * a.dim;
-        M::template each_dim<kDim>(g, a.dim, [&](int i, int r, int d) {
-            o[d] = static_cast<T>(weight == 0.0f ? 0.0f : out[i][r] / weight);
-        });
-    } else {
-        float* o = a.workspace + partial_offset(a, blockIdx.y, blockIdx.x, n16);
-        M::template each_dim<kDim>(g, a.dim, [&](int i, int r, int d) { o[d] = out[i][r]; });
-        if (g == 0) {
-            o[a.dim] = top;
-            o[a.dim + 1] = weight;
+    if (wave != 0) return;
+    uint32_t again = 0;  // heads whose sums are not finite
+    if constexpr (sizeof(T) == 2) {
+        f32x4 sum = out[0];  // keeps NaN and infinity; dims behind the head's repeat its first ones
+#pragma unroll
+        for (int i = 1; i < kBlocks; ++i) sum += out[i];
+        const uint64_t odd = __ballot(n16 < columns && !(fabsf((sum[0] + sum[1]) + (sum[2] + sum[3]) + weight) < INFINITY));
+        again = static_cast<uint32_t>((odd | odd >> 16 | odd >> 32 | odd >> 48) & 0xffff);
+    }
+    if (n16 < columns && !(again >> n16 & 1)) {
+        if (parts == 1) {
+            const int64_t head = kv_head * static_cast<int64_t>(a.group) + column0 + n16;
+            T* o = static_cast<T*>(a.out) + (b * static_cast<int64_t>(a.query_heads) + head) * a.dim;
+            M::template each_dim<kDim>(g, a.dim, [&](int i, int r, int d) {
+                o[d] = static_cast<T>(weight == 0.0f ? 0.0f : out[i][r] / weight);
+            });
+        } else {
+            float* o = a.workspace + partial_offset(a, blockIdx.y, blockIdx.x, n16);
+            M::template each_dim<kDim>(g, a.dim, [&](int i, int r, int d) { o[d] = out[i][r]; });
+            if (g == 0) {
+                o[a.dim] = top;
+                o[a.dim + 1] = weight;
+            }
+        }
+    }
+    if constexpr (sizeof(T) == 2) {
+        if (again) {
+            // The arguments by their address, which the compiler does not see through: read here, not held since the start.
+            uint64_t held = reinterpret_cast<uint64_t>((const void*)__builtin_amdgcn_kernarg_segment_ptr());
+            asm volatile("" : "+s"(held));
+            for (; again; again &= again - 1)
+                exact_part<T, kTile, kPaged>(*reinterpret_cast<const AttentionArgs*>(held), chosen, __ffs(again) - 1);
         }
     }
 }

@@ -209,6 +209,48 @@ def test_a_key_of_infinities_has_no_weight(gpu_device, dtype, dim):
 
 
 @pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("heads,kv_heads,dim,page_size", [(9, 3, 64, 16), (20, 1, 128, 24), (4, 2, 80, 16), (6, 2, 5, 7), (2, 1, 256, 33),
+                                                          (3, 3, 100, 48)])
+def test_infinite_values_stay_infinite(gpu_device, dtype, heads, kv_heads, dim, page_size):
+    """A visible infinity times a weight above zero is an infinity of its sign; two of both signs are NaN.  Also behind small
+    weights, in sequences that are cut over workgroups, and next to NaN."""
+    case = _paged_case(59, dtype, heads, kv_heads, dim, page_size, [40, 2500, 2500, 33])
+    finite = {**case, "value_pages": case["value_pages"].clone()}
+
+    def place(b, position):
+        return int(case["page_table"][b, position // page_size]), slice(None), position % page_size
+
+    for b, position, d, value in ((0, 5, 0, math.inf), (0, 39, 1, -math.inf), (1, 5, 2, math.inf), (1, 1700, 2, math.inf),
+                                  (1, 2499, 3, math.inf), (1, 20, 3, -math.inf), (2, 700, 4, math.nan), (2, 701, 4, math.inf)):
+        case["value_pages"][place(b, position)][..., d] = value
+    # Its score lies 40 below the others' middle: a weight that 16 bits do not hold next to the largest.
+    low = place(0, 5)
+    for h in range(kv_heads):
+        q = case["query"][0, h * (heads // kv_heads), 0].double()
+        case["key_pages"][low[0], h, low[2]] = (-40 / case["scale"] * q / q.dot(q).clamp(min=0.1)).to(dtype)
+    finite["key_pages"] = case["key_pages"]
+    expected = ref.paged_decode(**case)
+    assert bool(expected[0, ..., 0].isinf().any()) and bool(expected[1, ..., 3].isnan().all()) and bool(expected[3].isfinite().all())
+    bound = ref.attention_bound(finite["query"], finite["key_pages"], finite["value_pages"], case["scale"], 2500, dtype, expected)
+    out = ops.paged_decode_attention_native(**_to(case, gpu_device)).cpu()
+    for sign in (math.inf, -math.inf):
+        assert torch.equal(out == sign, expected == sign)
+    assert torch.equal(out.isnan(), expected.isnan())
+    kept = expected.isfinite()
+    _close(out[kept], expected[kept], bound[kept])
+
+    # One run of keys per sequence, one token and several.
+    for queries in (1, 3):
+        case = _window_case(61, dtype, 2, heads, kv_heads, dim, queries, 300)
+        case["value"][0, :, 7, 0], case["value"][0, :, 250, 1], case["value"][1, :, 299, 2] = math.inf, -math.inf, math.inf
+        expected = ref.window_attention(**case, window=100, sinks=8)
+        out = ops.window_attention_native(**_to(case, gpu_device), window=100, sinks=8).cpu()
+        for sign in (math.inf, -math.inf):
+            assert torch.equal(out == sign, expected == sign)
+        assert torch.equal(out.isnan(), expected.isnan()) and not bool(out.isnan().any())
+
+
+@pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("dim", [64, 80])
 def test_scores_that_are_all_minus_infinity_give_zeros(gpu_device, dtype, dim):
     case = _to(_window_case(43, dtype, 1, 4, 2, dim, 40, 40), gpu_device)
