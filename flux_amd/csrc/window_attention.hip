@@ -342,8 +342,10 @@ __global__ void __launch_bounds__(kThreads, kDim <= 64 ? 4 : (kDim <= 128 ? 2 : 
 // keys 8 (r / 4) + 4 h + r % 4 of row n, which rounded in pairs are the right operand of O^T = V^T P.  Rows are padded by
 // 16 bytes so that eight lanes' 16-byte reads fall on different banks.
 // The running maximum moves only when a tile exceeds it by 2^kLazy: a rescaling of the sums costs as much as the
-// exponentials, and weights up to 2^kLazy are as exact.  Weights are rounded to the values' type for the product (half
-// a step of that type, like the result's own rounding) and summed unrounded in float32.
+// exponentials, and weights up to 2^kLazy are as exact.  Weights are rounded once to the values' type for the product: by
+// at most half a step of that type relative to themselves, which moves a weighted mean of the values by at most half a step
+// of the largest of them, as the result's own rounding does.  They are summed unrounded in float32.  (Two terms a weight, as
+// in paged_attention.hip, would double the matrix instructions of the product, here where they bound the kernel.)
 typedef float f32x16 __attribute__((ext_vector_type(16)));
 typedef float f32x2 __attribute__((ext_vector_type(2)));
 constexpr int64_t kStagedStride = 1 << 22;
@@ -352,7 +354,7 @@ template <class T>
 struct Wide;
 template <>
 struct Wide<__bf16> {
-    static constexpr float kShift = 0.0f;
+    static constexpr float kShift = 0.0f, kLazy = 8.0f;
     typedef __bf16 Pair __attribute__((ext_vector_type(2)));
     static __device__ __forceinline__ uint32_t round(float a, float b) {
         return __builtin_bit_cast(uint32_t, __builtin_convertvector((f32x2{a, b}), Pair));
@@ -364,9 +366,10 @@ struct Wide<__bf16> {
 };
 template <>
 struct Wide<_Float16> {
-    // Weights are held 2^6 times as large (at most 2^14), which keeps those down to 2^-20 of the largest in float16's
-    // normal range.
-    static constexpr float kShift = 6.0f;
+    // Weights are held 2^11 times as large, at most 2^15 with kLazy.  Those from 2^-25 of the reference on are normal numbers;
+    // smaller ones are off by at most half of float16's smallest step, 2^-36 of the reference, and the 2^24 keys that a
+    // sequence can have together by 2^-12 of the largest value.
+    static constexpr float kShift = 11.0f, kLazy = 4.0f;
     typedef _Float16 Pair __attribute__((ext_vector_type(2)));
     static __device__ __forceinline__ uint32_t round(float a, float b) {
         return __builtin_bit_cast(uint32_t, __builtin_convertvector((f32x2{a, b}), Pair));
@@ -416,7 +419,6 @@ window_tile_kernel(AttentionArgs a, int row_tiles, int tiles_total) {
     constexpr int kStage = kKeys * kKeyRow + kDim * kValueRow;
     constexpr int kKeyLoads = kKeys * kDim / 8 / kThreads;        // 16 bytes per thread
     static_assert(kKeys / 4 * (kDim / 8) == kThreads, "every thread stages four keys by eight dims of the values");
-    constexpr float kLazy = 8.0f;
     extern __shared__ char stages[];
 
     const int tile = tile_of_block();
@@ -559,7 +561,7 @@ window_tile_kernel(AttentionArgs a, int row_tiles, int tiles_total) {
 #pragma unroll
                 for (int j = 1; j < 16; ++j) highest = fmaxf(highest, score[j]);
                 highest = half_max(highest) * factor;
-                if (__any(highest > top + kLazy)) {
+                if (__any(highest > top + W::kLazy)) {
                     const float now = fmaxf(top, highest);
                     const float shrink = top == -INFINITY ? 0.0f : fast_exp2(top - now);
                     top = now;

@@ -365,6 +365,33 @@ def test_window_scales(gpu_device, dtype, dim, scale):
         _check_window(case, gpu_device, 0, 0)
 
 
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("below", [20, 24, 30, 31, 33, 35])
+def test_window_many_small_weights_over_a_long_run(gpu_device, dtype, below):
+    """One key whose value is 0 far above n = 2^22 others, each 2^-below of it: what they add up to must not be lost.
+
+    The scale is ln 2, so that a weight is 2^-below (1 + d) with |d| <= below 3 2^-24 ln 2 + 2^-22 < 2^-17, which both types
+    round to 2^-below itself; its products with powers of two add up without rounding (at most 2^22 multiples of the
+    smallest).  The sum of the weights lies between that of the large one alone, in whose lane a float32 sum may lose the
+    others, and that of all, both within 2^-17; the result is rounded once, by half a step.
+    """
+    n, dim = 1 << 22, 8
+    query, key = torch.zeros(1, 1, 2, dim, dtype=dtype), torch.full((1, 1, n, dim), 0.0, dtype=dtype)
+    query[..., 0] = 1
+    key[..., 0] = -below
+    key[0, 0, 0, 0] = 0
+    each = torch.tensor([1, -2, 0.25, 4, -0.5, 1, 2, 0])
+    value = each.to(dtype).repeat(1, 1, n, 1)
+    value[0, 0, 0] = 0
+    out = ops.window_attention_native(query.to(gpu_device), key.to(gpu_device), value.to(gpu_device), math.log(2), 0).cpu().double()
+    for row, count in ((0, n - 2), (1, n - 1)):
+        rest = count * 2.0 ** -below
+        slack = torch.finfo(dtype).eps / 2 + 2.0 ** -16
+        size = out[0, 0, row] / each.double().where(each != 0, torch.tensor(1.0, dtype=torch.float64))
+        assert float(size[7]) == 0
+        assert bool((size[:7] >= rest / (1 + rest) * (1 - slack)).all()) and bool((size[:7] <= rest * (1 + slack)).all()), (size, rest)
+
+
 @pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("dim", [64, 128, 40])
 def test_window_scale_of_zero_makes_infinite_scores_nan(gpu_device, dtype, dim):
