@@ -95,6 +95,80 @@ def test_paged_decode_long_and_large_batches(gpu_device, dtype):
     _check_paged(_paged_case(3, dtype, 2, 2, 32, 8, lengths), gpu_device)
 
 
+# Inputs whose results tell every key: the score of key j is -(j // 16 % 8) times the head's factor, so that with a scale of
+# ln 2 its weight is a power of two, and its value is 1 in the dim j // 16 % D and 0 in all others.
+
+def _telling_keys(count, dim, dtype):
+    tile = torch.arange(count) // 16
+    key, value = torch.zeros(count, dim, dtype=dtype), torch.zeros(count, dim, dtype=dtype)
+    key[:, 0] = -(tile % 8).to(dtype)
+    value[torch.arange(count), tile % dim] = 1
+    return key, value
+
+
+def _telling_query(shape, dtype):
+    query = torch.zeros(shape, dtype=dtype)
+    query[..., 0] = (1 + torch.arange(shape[1]) % 2).to(dtype).view(1, -1, 1)
+    return query
+
+
+def _telling_bound(expected, dtype, additions):
+    """Relative, as all terms are positive.  The exponent of a weight, at most 32 below the running maximum's, is off by 3
+    2^-24 of itself, together with the steps that the maximum takes: 32 * 3 * 2^-24 ln 2 < 2^-17 of the weight, and 2^-22 for
+    each of at most 20 exponentials, < 2^-17.  What a power of two that is off by this leaves in 16 bits is below 2^-17 again.
+    ``additions``, one after the other, are off by 2^-24 each, in the sums of the weights and of the values; the quotient by
+    2^-23; and the result is rounded once."""
+    relative = 2.0 ** -15 + additions * 2.0 ** -23 + torch.finfo(dtype).eps / 2
+    return relative * expected + torch.finfo(dtype).tiny
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("heads,kv_heads,dim", [(3, 1, 64), (20, 1, 128), (4, 2, 80), (2, 1, 256)])
+@pytest.mark.parametrize("window,sinks", [(0, 0), (2000, 40)])
+def test_paged_decode_loses_no_key_where_sequences_are_cut(gpu_device, dtype, heads, kv_heads, dim, window, sinks):
+    lengths, page_size = [9000, 3, 700, 0, 5000, 16, 1999], 48
+    case = _paged_case(67, dtype, heads, kv_heads, dim, page_size, lengths, scale=math.log(2))
+    case["query"] = _telling_query(case["query"].shape, dtype)
+    for b, n in enumerate(lengths):
+        key, value = _telling_keys(-(-n // page_size) * page_size, dim, dtype)
+        for c in range(-(-n // page_size)):
+            page = int(case["page_table"][b, c])
+            case["key_pages"][page] = key[c * page_size : (c + 1) * page_size]
+            case["value_pages"][page] = value[c * page_size : (c + 1) * page_size]
+    expected = ref.paged_decode(**case, window=window, sinks=sinks)
+    # 2 tiles of a wave and as many additions a key as a lane makes, four waves, 71 parts.
+    bound = _telling_bound(expected, dtype, 128)
+    _close(ops.paged_decode_attention_native(**_to(case, gpu_device), window=window, sinks=sinks), expected, bound)
+    # The bound tells a lost tile of 16 keys, wherever it lies.
+    for b, n in enumerate(lengths):
+        key, value = _telling_keys(n, dim, dtype)
+        for first in {0, n // 3 // 16 * 16, (n - 1) // 16 * 16} if n > 16 else ():
+            seen = [j for j in ref.visible_keys(n - 1, n, window, sinks)]
+            kept = [j for j in seen if not first <= j < first + 16]
+            if len(kept) < len(seen):
+                lost = ref.attend(case["query"][b, 0, 0], key[kept], value[kept], case["scale"])
+                assert bool(((lost - expected[b, 0, 0]).abs() > bound[b, 0, 0]).any())
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("heads,kv_heads,dim", [(3, 1, 64), (6, 2, 128), (2, 1, 80), (2, 1, 256)])
+@pytest.mark.parametrize("window,sinks", [(0, 0), (500, 21), (37, 0)])
+def test_window_attention_loses_no_key(gpu_device, dtype, heads, kv_heads, dim, window, sinks):
+    """A chunk, a prompt and a token at the end of long keys."""
+    for queries, keys in ((40, 2000), (330, 330), (1, 9000)):
+        key, value = _telling_keys(keys, dim, dtype)
+        case = {"query": _telling_query((1, heads, queries, dim), dtype), "key": key.expand(1, kv_heads, keys, dim),
+                "value": value.expand(1, kv_heads, keys, dim), "scale": math.log(2)}
+        expected = ref.window_attention(**case, window=window, sinks=sinks)
+        bound = _telling_bound(expected, dtype, keys // 4)  # two lanes share a row and add its weights in pairs
+        _close(ops.window_attention_native(**_to(case, gpu_device), window=window, sinks=sinks), expected, bound)
+        seen = ref.visible_keys(keys - 1, keys, window, sinks)
+        for first in (seen[0], seen[len(seen) // 2], seen[-1] - 15):
+            kept = [j for j in seen if not first <= j < first + 16]
+            lost = ref.attend(case["query"][0, 0, -1], key[kept], value[kept], case["scale"])
+            assert bool(((lost - expected[0, 0, -1]).abs() > bound[0, 0, -1]).any())
+
+
 def test_paged_decode_one_sequence_at_every_length(gpu_device):
     case = _paged_case(11, torch.float32, 9, 3, 64, 16, [300])
     device = _to(case, gpu_device)
