@@ -150,6 +150,43 @@ def test_paged_decode_loses_no_key_where_sequences_are_cut(gpu_device, dtype, he
                 assert bool(((lost - expected[b, 0, 0]).abs() > bound[b, 0, 0]).any())
 
 
+@pytest.mark.parametrize("dtype,dim", [(torch.float32, 64), (torch.float32, 128), (torch.float16, 64), (torch.bfloat16, 128)])
+def test_paged_decode_joins_more_parts_than_it_keeps_shares_of(gpu_device, dtype, dim):
+    """One sequence in hundreds of parts: a far larger key behind the 128th part, parts whose keys are all left out (no page, or
+    a score of -inf) before and behind it."""
+    n, page_size = 33000, 16
+    case = _paged_case(71, dtype, 3, 1, dim, page_size, [n], scale=math.log(2))
+    case["query"] = _telling_query(case["query"].shape, dtype)
+    key, value = _telling_keys(case["page_table"].shape[1] * page_size, dim, dtype)
+    key[30000, 0] = 8
+    for gone in (6400, 27520):  # 320 keys hold a whole part of 128 or 80, wherever it starts
+        key[gone : gone + 320, 0] = -math.inf
+    table = case["page_table"][0].long()
+    case["key_pages"][table] = key.view(-1, 1, page_size, dim)
+    case["value_pages"][table] = value.view(-1, 1, page_size, dim)
+    for gone in (3200, 25600):
+        case["page_table"][0, gone // page_size : (gone + 320) // page_size] = -1
+    device = _to(case, gpu_device)
+    needed = ops.paged_decode_workspace_bytes(device["query"], device["key_pages"], device["page_table"]) // 4
+    output, workspace = torch.empty_like(device["query"]), torch.empty(needed, device=gpu_device)
+    ops.paged_decode_attention_native_out(*device.values(), 0, 0, None, output, workspace)
+    first, parts = workspace[-2:].view(torch.int32).tolist()
+    assert first == 0 and parts > 200
+    expected = ref.paged_decode(**case)
+    assert bool(expected.isfinite().all())
+    bound = _telling_bound(expected, dtype, 64 + parts)
+    _close(output, expected, bound)
+    # The bound tells a part behind the 128th, or its share taken for 1.
+    weights = torch.exp2(key[:, 0].double())
+    weights[[*range(3200, 3520), *range(25600, 25920)]] = 0
+    weights[n:] = 0
+    for changed in (0.0, 2.0 ** 8):
+        other = weights.clone()
+        other[26880:27008] *= changed
+        moved = (other @ value.double()) / other.sum()
+        assert bool(((moved - expected[0, 0, 0]).abs() > bound[0, 0, 0]).any())
+
+
 @pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("heads,kv_heads,dim", [(3, 1, 64), (6, 2, 128), (2, 1, 80), (2, 1, 256)])
 @pytest.mark.parametrize("window,sinks", [(0, 0), (500, 21), (37, 0)])
