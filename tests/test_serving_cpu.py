@@ -4,7 +4,9 @@ plain page model against a direct simulation."""
 from __future__ import annotations
 
 import ctypes
+import os
 import random
+import re
 
 import pytest
 import torch
@@ -13,6 +15,7 @@ from torch._subclasses.fake_tensor import FakeTensorMode
 from flux_amd import _native, ops
 from flux_amd.ops import serving
 from oracle import serving as ref
+from tests.conftest import ROOT
 
 
 def _paged(batch=2, heads=6, kv_heads=2, dim=16, pages=5, page_size=4, columns=3, dtype=torch.float32):
@@ -411,6 +414,41 @@ def test_c_entries_refuse_table_rows_that_overlap():
     books = _books_struct(slots=1, table_stride=0, page_table=0x10000, lengths=0x20000, refcounts=0x30000)
     assert lib.flux_page_reserve(books, some, None, 2, some, some, some, 3, None) == bad
     assert "workspace too small" in _native.last_error()
+
+
+def _header_fields(name):
+    """(field, bytes) of a structure in include/flux_amd.h, in their order."""
+    text = open(os.path.join(ROOT, "include", "flux_amd.h")).read()
+    body = re.search(r"typedef struct \{([^}]*)\} %s;" % name, text).group(1)
+    fields = []
+    for declaration in filter(None, (d.strip() for d in body.split(";"))):
+        kind, field, count = re.fullmatch(r"(int64_t|\w+\*) ?(\w+)(?:\[(\d+)\])?", declaration.replace(" *", "*")).groups()
+        fields.append((field, 8 * int(count or 1)))
+    return fields
+
+
+def test_packed_structures_are_those_of_the_header():
+    """The operators pack flux_page_books and flux_page_pool into bytes: field by field the header's and ctypes' structures."""
+    for name, struct_type in (("flux_page_books", _native.PageBooks), ("flux_page_pool", _native.PagePool)):
+        assert _header_fields(name) == [(field, ctypes.sizeof(kind)) for field, kind in struct_type._fields_]
+        assert ctypes.sizeof(struct_type) == sum(size for _, size in _header_fields(name))
+
+    table = torch.zeros(5, 9, dtype=i32)[1:4, 2:6]
+    lengths, refcounts = torch.zeros(3, dtype=i64), torch.zeros(7, dtype=i32)
+    books = _native.PageBooks(page_table=table.data_ptr(), table_stride=9, slots=3, columns=4, lengths=lengths.data_ptr(),
+                              refcounts=refcounts.data_ptr(), pages=7, page_size=16)
+    assert serving._books(table, lengths, refcounts, 16) == bytes(books)
+    books.lengths = None
+    assert serving._books(table, None, refcounts, 16) == bytes(books)
+
+    for dtype, code in ((torch.float32, 0), (torch.float16, 1), (torch.bfloat16, 2)):
+        key, value = torch.zeros(2, 7, 3, 4, 8, dtype=dtype), torch.zeros(2, 7, 4, 3, 8, dtype=dtype).transpose(2, 3)
+        for layered in (True, False):
+            pool = _native.PagePool(key=key.data_ptr(), value=value.data_ptr(), layers=2 if layered else 1, pages=7, heads=3,
+                                    page_size=4, head_dim=8, dtype=code)
+            pool.key_strides[:] = (672 if layered else 0, 96, 32, 8)
+            pool.value_strides[:] = (672 if layered else 0, 96, 8, 24)
+            assert serving._pool(*((key, value) if layered else (key[0], value[0]))) == bytes(pool)
 
 
 # --------------------------------------------------------------------------- the plain page model
