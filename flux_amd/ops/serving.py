@@ -317,8 +317,8 @@ def _pools_apart(key_pages, value_pages) -> bool:
 
 
 def _validate_pool_memory(op, key_pages, value_pages) -> None:
-    if not _pools_apart(key_pages, value_pages):
-        _check(False, f"{op}: key_pages and value_pages must not overlap")
+    """For CPU tensors; the C entries look themselves."""
+    _check(_pools_apart(key_pages, value_pages), f"{op}: key and value pages must not overlap")
 
 
 def _validate_pools(op, key_pages, value_pages, ranks=(4, 5)) -> None:
@@ -462,6 +462,10 @@ def _validate_write_memory(key, value, key_pages, value_pages, page_table, slots
     stores = key_pages.untyped_storage().data_ptr(), value_pages.untyped_storage().data_ptr()
     _check(key.untyped_storage().data_ptr() not in stores and value.untyped_storage().data_ptr() not in stores,
            "flux::paged_cache_write: the pages must not alias key or value")
+
+
+def _validate_write_pools(key, value, key_pages, value_pages, page_table, slots, positions, counts=None) -> None:
+    _validate_write_memory(key, value, key_pages, value_pages, page_table, slots, positions, counts)
     _validate_pool_memory("flux::paged_cache_write", key_pages, value_pages)
 
 
@@ -484,13 +488,13 @@ def _validate_copy(key_pages, value_pages, source, target) -> None:
         _check(False, f"{op}: source and target must have one length")
 
 
-def _validate_copy_memory(key_pages, value_pages, source, target) -> None:
+def _validate_copy_pools(key_pages, value_pages, source, target) -> None:
     _validate_copy(key_pages, value_pages, source, target)
     _validate_pool_memory("flux::paged_cache_copy", key_pages, value_pages)
 
 
 def _copy_cuda(key_pages, value_pages, source, target):
-    _validate_copy_memory(key_pages, value_pages, source, target)
+    _validate_copy(key_pages, value_pages, source, target)
     _require_gpu("flux::paged_cache_copy", key_pages)
     status = source.new_empty(source.shape[0], dtype=torch.int32)
     if source.shape[0]:
@@ -531,13 +535,13 @@ def _validate_fork(key_pages, value_pages, page_table, lengths, refcounts, paren
         _check(False, f"{op}: parents and children must have one length")
 
 
-def _validate_fork_memory(key_pages, value_pages, page_table, lengths, refcounts, parents, children) -> None:
+def _validate_fork_pools(key_pages, value_pages, page_table, lengths, refcounts, parents, children) -> None:
     _validate_fork(key_pages, value_pages, page_table, lengths, refcounts, parents, children)
     _validate_pool_memory("flux::paged_cache_fork", key_pages, value_pages)
 
 
 def _fork_cuda(key_pages, value_pages, page_table, lengths, refcounts, parents, children):
-    _validate_fork_memory(key_pages, value_pages, page_table, lengths, refcounts, parents, children)
+    _validate_fork(key_pages, value_pages, page_table, lengths, refcounts, parents, children)
     _require_gpu("flux::paged_cache_fork", key_pages)
     requests = parents.shape[0]
     status = page_table.new_empty(requests)
@@ -561,13 +565,13 @@ def _validate_compact(key_pages, value_pages, page_table, refcounts) -> None:
         _check(False, f"{op}: refcounts must have one entry per page")
 
 
-def _validate_compact_memory(key_pages, value_pages, page_table, refcounts) -> None:
+def _validate_compact_pools(key_pages, value_pages, page_table, refcounts) -> None:
     _validate_compact(key_pages, value_pages, page_table, refcounts)
     _validate_pool_memory("flux::paged_cache_compact", key_pages, value_pages)
 
 
 def _compact_cuda(key_pages, value_pages, page_table, refcounts):
-    _validate_compact_memory(key_pages, value_pages, page_table, refcounts)
+    _validate_compact(key_pages, value_pages, page_table, refcounts)
     _require_gpu("flux::paged_cache_compact", key_pages)
     pages = refcounts.shape[0]
     page_map = refcounts.new_empty(pages)
@@ -665,11 +669,11 @@ _KERNELS = {
     "paged_decode_attention_out": (_paged_out_cuda, _validate_paged_out_memory),
     "window_attention": (_window_cuda, _validate_window),
     "paged_cache_reserve": (_reserve_cuda, _validate_reserve),
-    "paged_cache_write": (_write_cuda, _validate_write_memory),
-    "paged_cache_copy": (_copy_cuda, _validate_copy_memory),
-    "paged_cache_fork": (_fork_cuda, _validate_fork_memory),
+    "paged_cache_write": (_write_cuda, _validate_write_pools),
+    "paged_cache_copy": (_copy_cuda, _validate_copy_pools),
+    "paged_cache_fork": (_fork_cuda, _validate_fork_pools),
     "paged_cache_free": (_free_cuda, _validate_free),
-    "paged_cache_compact": (_compact_cuda, _validate_compact_memory),
+    "paged_cache_compact": (_compact_cuda, _validate_compact_pools),
     "logits_process": (_logits_cuda, _validate_logits),
 }
 

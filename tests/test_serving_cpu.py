@@ -248,7 +248,7 @@ def test_pools_that_share_memory_are_refused(name):
     args = CALLS[name]()
     for what, key, value, shared in _side_views(tuple(args["key_pages"].shape)):
         assert _shares_memory(key, value) == shared, what
-        message = "key_pages and value_pages must not overlap" if shared else "no CPU kernel"
+        message = f"{name}: key and value pages must not overlap" if shared else "no CPU kernel"
         with pytest.raises(RuntimeError, match=message):
             getattr(torch.ops.flux, name)(**{**args, "key_pages": key, "value_pages": value})
 

@@ -806,6 +806,37 @@ def test_pages_with_other_strides(gpu_device):
     assert torch.equal(both[..., 6], untouched) and bool((table[:, [0, 4]] == 77).all())
 
 
+def test_pools_of_one_storage(gpu_device):
+    """Interleaved keys and values work as separate ones; views that meet are refused before any launch."""
+    shape = (3, 9, 2, 4, 8)
+    ids = torch.tensor([0, 4, 7], device=gpu_device)
+    source = torch.randn(2, *shape, generator=torch.Generator().manual_seed(3)).to(gpu_device)
+    expected = source.clone()
+    expected[:, :, ids + 1] = source[:, :, ids]
+    for layout in ((3, 9, 2, 2, 4, 8), (3, 9, 2, 4, 2, 8)):
+        at = layout.index(2, 2) if layout[3] == 2 else 4
+        store = torch.zeros(layout, device=gpu_device)
+        key, value = store.unbind(at)
+        key.copy_(source[0]), value.copy_(source[1])
+        status = ops.paged_cache_copy_native(key, value, ids, ids + 1)
+        assert status.tolist() == [ops.PAGE_DONE] * 3
+        assert torch.equal(key, expected[0]) and torch.equal(value, expected[1])
+    store = torch.randn(3 * 9 * 64 + 64, device=gpu_device)
+    key, value = store[:-64].view(shape), store[64:].view(shape)
+    books = {"page_table": torch.full((3, 4), -1, dtype=torch.int32, device=gpu_device),
+             "lengths": torch.zeros(3, dtype=torch.int64, device=gpu_device),
+             "refcounts": torch.zeros(9, dtype=torch.int32, device=gpu_device)}
+    rows = torch.zeros(1, 2, 1, 8, device=gpu_device)
+    kept = store.clone()
+    for call in (lambda: ops.paged_cache_copy_native(key, value, ids, ids + 1),
+                 lambda: ops.paged_cache_fork_native(key, value, *books.values(), ids[:1], ids[:1] + 1),
+                 lambda: ops.paged_cache_compact_native(key, value, books["page_table"], books["refcounts"]),
+                 lambda: ops.paged_cache_write_native(rows, rows.clone(), key[0], value[0], books["page_table"], ids[:1], ids[:1])):
+        with pytest.raises(RuntimeError, match="key and value pages must not overlap"):
+            call()
+    assert torch.equal(store, kept)
+
+
 def test_write_skips_what_has_no_page(gpu_device):
     pages = _Device(ref.Pages(1, 4, 1, 4, 8, 3, 2), gpu_device)
     pages.table[0, 0] = pages.model.table[0][0] = 2
