@@ -3,8 +3,8 @@
 // The books are a page table [slots, columns] (-1: no page), the slots' lengths and a count of holders per page (0:
 // free).  A page that is needed is always the lowest free one, and requests are served in their order, so that
 // results do not depend on scheduling.  Every operator is one launch of bookkeeping, or one and a copy over the whole
-// card: the bookkeeping is a few KB and bound by the latency of dependent reads (16 prompts reserved in 8.8 us, 64 forks
-// planned in 7.9), the copies by HBM (40 pages of 30 layers, 59 MB moved, in 11.1 us).
+// card: the bookkeeping is a few KB and bound by the latency of dependent reads (16 prompts reserved in 8.7 us, 64 forks
+// planned in 7.5), the copies by HBM (40 pages of 30 layers, 59 MB moved, in 11.8 us).
 #include "serving.h"
 
 namespace flux {

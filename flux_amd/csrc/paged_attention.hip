@@ -9,7 +9,7 @@
 // into parts of about the same number of tiles as every other part of the batch, one per workgroup, so that ragged
 // lengths load the card evenly; the parts of a sequence that was cut leave (o, m, l) in the workspace and a second launch
 // joins them: o = sum o_c exp(m_c - M) / sum l_c exp(m_c - M).  (48 sequences to 16384, 32 / 8 heads of 128 in bfloat16:
-// 400 us, 4.5 TB/s; 24 to 8192, 9 / 3 heads of 64 in float32: 44 us, the join 4.6 of them.)
+// 400 us, 4.5 TB/s; 24 to 8192, 9 / 3 heads of 64 in float32: 45 us, the join 4.4 of them.)
 //
 // A wave takes 16 or 32 keys at a time straight into registers, laid out as the matrix instruction wants them, while the
 // tile before is worked on.  Scores come as S^T = K Q^T (rows: keys, columns: query heads), so the lane that holds
@@ -25,8 +25,8 @@ constexpr int kDecodeThreads = 256;
 constexpr int kDecodeWaves = 4;
 constexpr int kColumns = 16;          // query heads of one workgroup
 constexpr int kLeastTiles = 4;        // tiles that are worth a workgroup: one per wave
-// A call whose sequences have no more tiles than this leaves each to one workgroup and saves the join's launch: two tiles a
-// wave, or eight where the sequences fill the card uncut.  (100 sequences to 1000 keys, 40 / 8 heads of 128 in bfloat16: 55
+// A call whose sequences have no more tiles than this, by the table's width or the window, leaves each to one workgroup and
+// saves the join's launch: two tiles a wave, or eight where the sequences fill the card uncut.  (100 sequences to 1000 keys, 40 / 8 heads of 128 in bfloat16: 55
 // against 59 us cut; one of 900 keys, 9 / 3 heads of 64 in float32: 20 us cut, 26 whole.)
 constexpr int kWholeTiles = 8, kWholeTilesFull = 32;
 

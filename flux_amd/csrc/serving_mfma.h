@@ -110,8 +110,8 @@ struct Mfma<float> {
     }
 };
 
-// What the two 16-bit types share.  The weights are split in two terms of 16 bits, so that their rounding (2^-16
-// of a weight and less) does not show beside that of the result; the matrix units wait for memory here.
+// What the two 16-bit types share.  The weights are split in two terms of 16 bits, so that their rounding (2^-16 of a weight
+// in bfloat16; float16's is below) does not show beside that of the result; the matrix units wait for memory here.
 template <class T, class Derived>
 struct Mfma16 {
     using Fragment = u32x4;
@@ -228,8 +228,9 @@ struct Mfma<__bf16> : Mfma16<__bf16, Mfma<__bf16>> {
     }
 };
 
-// float16's smallest step is 2^-24: weights are held 2^12 times as large (at most 4096), sums of weights with them, so
-// that what a split weight loses is below 2^-36 of the largest one.
+// float16's smallest step is 2^-24: weights are held 2^12 times as large (at most 4096), sums of weights with them.  Each term
+// is off by at most 2^-11 of itself, so that a split weight loses 2^-22 of itself where its lower term is a normal number, and
+// else half a smallest step, 2^-25 of 4096: 2^-37 of the largest weight.
 template <>
 struct Mfma<_Float16> : Mfma16<_Float16, Mfma<_Float16>> {
     static constexpr float kWeightShift = 12.0f;

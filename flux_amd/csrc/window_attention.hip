@@ -333,7 +333,7 @@ __global__ void __launch_bounds__(kThreads, kDim <= 64 ? 4 : (kDim <= 128 ? 2 : 
 // ---------------------------------------------------------------------------
 // 16-bit prompts.  Here matrix instructions, exponentials and LDS reads cost about the same, so that keys and values are
 // staged once for the workgroup's four waves, 32 rows each.  4 x 4096 tokens (padded), 32 / 8 heads of 128, window 1024 in
-// bfloat16: 230 us, 720 TFLOP/s.  A 32 x 32 tile costs a SIMD 512 cycles of matrix instructions and as many of vector
+// bfloat16: 239 to 250 us, 670 to 700 TFLOP/s.  A 32 x 32 tile costs a SIMD 512 cycles of matrix instructions and as many of vector
 // instructions (half of them exponentials), and the two waves of a SIMD overlap them in part: 64 rows a wave (one wave
 // per SIMD) took 640 us, a workgroup of eight waves 236, two tiles per maximum 244.
 //

@@ -63,7 +63,7 @@ SERVING_OPERATOR_NAMES = tuple(SERVING_SCHEMAS)
 for _schema in SERVING_SCHEMAS.values():
     _LIBRARY.define(_schema)
 
-# Checks and arguments are a large part of a small call's time (one sequence of 900 keys: 20 us, on the GPU 15): shapes are
+# Checks and arguments are a large part of a small call's time (one sequence of 900 keys: 18.7 us, in a graph 12.5): shapes are
 # read once, conditions are tested in place, messages are whole literals, sizes that only depend on shapes come from small
 # caches, and structures and strides are packed into bytes (a ctypes array of four costs 0.5 us, its bytes 0.2).
 _four = struct.Struct("4q").pack
