@@ -63,9 +63,10 @@ def attention_bound(query, keys, values, scale, terms: int, dtype: torch.dtype, 
     |scale| |q| |k|; a matrix instruction may round a partial sum down instead of to nearest, which doubles the step.  A
     weight exp(s - m) is off, relative to itself, by the errors of s and m, by |s - m| 2^-23 for the scaled argument
     and by 2^-22 for the exponential, and a weight below 2^-40 does not count; a 16-bit weight kept in two terms by 2^-16
-    more (bfloat16's two halves; float16's lose 2^-22 of themselves or 2^-37 of the largest weight, and its weights in one
-    term at least 2^-36 of it, which the ``terms`` 2^-23 below hold).  The two sums of ``terms`` weights are off by terms 2^-23.  All of it moves a weighted
-    mean of the values by at most twice the weights' relative error times the largest value.  The result is rounded once.
+    more (bfloat16's two halves; a float16 weight loses 2^-22 of itself or, where it is small, 2^-37 of the largest weight,
+    2^-36 where it has one term, which the step of the sums holds).  The two sums of ``terms`` weights are off by terms
+    2^-23.  All of it moves a weighted mean of the values by at most twice the weights' relative error times the largest
+    value.  The result is rounded once.
 
     ``rounded_weights``: 16-bit prompts round each weight p_j once to the type for its product with v_j, and sum the
     unrounded ones: sum p_j (1 + d_j) v_j / sum p_j with |d_j| at most half a step differs by at most half a step times
