@@ -224,6 +224,13 @@ _PROTOTYPES: list[tuple[str, Any, list[Any]]] = [
     ("flux_page_fork", ctypes.c_int, [_pool, _books, _vp, _vp, _n, _vp, _vp, _n, _stream]),
     ("flux_page_compact_workspace_words", ctypes.c_int, [_n, _i64]),
     ("flux_page_compact", ctypes.c_int, [_pool, _books, _vp, _vp, _vp, _n, _stream]),
+    ("flux_page_write_rows", ctypes.c_int, [_pool, _vp, _vp, _strides, _strides, _n, _vp, _stream]),
+    ("flux_step_layout", ctypes.c_int, [_vp] + [_n] * 4 + [_vp] * 3 + [_n] * 2 + [_vp] * 4 + [_stream]),
+    ("flux_paged_chunk_attention_workspace_bytes", ctypes.c_int, [ctypes.c_int] + [_n] * 9 + [_i64]),
+    ("flux_paged_chunk_attention", ctypes.c_int,
+     [ctypes.c_int] + [_vp] * 10 + [_n, ctypes.c_float] + [_n] * 12 + [_strides] * 3 + [_stream]),
+    ("flux_logits_sample_workspace_bytes", ctypes.c_int, [_n, _n, _i64]),
+    ("flux_logits_sample", ctypes.c_int, [ctypes.c_int, _vp, _n] + [_vp] * 7 + [_n, _n, _vp, _n, _stream]),
     ("flux_logits_process_workspace_bytes", ctypes.c_int, [_n, _n, _i64]),
     ("flux_logits_process", ctypes.c_int,
      [ctypes.c_int, _vp, _n, _vp, _vp, _n, _n, _vp, _n, _n, _vp, _vp, _vp, _vp, _vp, _n, _vp, _n, _vp, _n, _stream]),

@@ -892,6 +892,96 @@ int flux_paged_decode_attention(int dtype, const void* query, const void* key_pa
                     "flux_paged_decode_attention");
 }
 
+namespace {
+
+const char* chunk_arguments(flux::ChunkArgs& args, int dtype, float scale, int64_t tokens, int64_t requests, int64_t query_heads,
+                            int64_t kv_heads, int64_t head_dim, int64_t pages, int64_t page_size, int64_t slot_count,
+                            int64_t columns, int64_t window, int64_t sinks) {
+    if (!known_type(dtype)) return "unknown dtype";
+    if (tokens <= 0 || tokens > FLUX_MAX_SERVING_KEYS || requests <= 0 || requests > 65535 || query_heads <= 0 ||
+        kv_heads <= 0 || query_heads % kv_heads || query_heads > 65535 || tokens * (query_heads / kv_heads) > (int64_t{1} << 27) ||
+        head_dim <= 0 || head_dim > flux::kServingMaxDim)
+        return "invalid shape";
+    if (pages <= 0 || pages > (1 << 28) || page_size <= 0 || page_size > FLUX_MAX_SERVING_KEYS || slot_count <= 0 ||
+        columns <= 0 || columns > FLUX_MAX_SERVING_KEYS / page_size)
+        return "invalid pages (columns * page_size is at most FLUX_MAX_SERVING_KEYS)";
+    if (window < 0 || sinks < 0 || window > FLUX_MAX_SERVING_KEYS || sinks > FLUX_MAX_SERVING_KEYS)
+        return "window and sinks must be within [0, FLUX_MAX_SERVING_KEYS]";
+    if (!std::isfinite(scale)) return "scale must be finite";
+    args.scale = scale;
+    args.requests = static_cast<int>(requests);
+    args.tokens = tokens;
+    args.query_heads = static_cast<int>(query_heads);
+    args.kv_heads = static_cast<int>(kv_heads);
+    args.group = static_cast<int>(query_heads / kv_heads);
+    args.group_of = flux::make_divider(static_cast<uint32_t>(args.group));
+    args.dim = static_cast<int>(head_dim);
+    args.keys = columns * page_size;
+    args.slot_count = slot_count;
+    args.window = static_cast<int>(window);
+    args.sinks = static_cast<int>(sinks);
+    args.pages = pages;
+    args.page = flux::make_divider(static_cast<uint32_t>(page_size));
+    return nullptr;
+}
+
+}  // namespace
+
+int flux_paged_chunk_attention_workspace_bytes(int dtype, int64_t tokens, int64_t requests, int64_t query_heads, int64_t kv_heads,
+                                               int64_t head_dim, int64_t page_size, int64_t columns, int64_t window,
+                                               int64_t sinks, int64_t* bytes) {
+    flux::ChunkArgs args{};
+    if (!bytes || chunk_arguments(args, dtype, 1.0f, tokens, requests, query_heads, kv_heads, head_dim, 1, page_size, 1, columns,
+                                  window, sinks))
+        return invalid("flux_paged_chunk_attention_workspace_bytes: invalid argument");
+    *bytes = static_cast<int64_t>(flux::chunk_attention_workspace_floats(args, static_cast<flux::Type>(dtype)) * sizeof(float));
+    return FLUX_OK;
+}
+
+int flux_paged_chunk_attention(int dtype, const void* query, const void* key_pages, const void* value_pages,
+                               const int32_t* page_table, const int64_t* lengths, const int64_t* offsets, const int64_t* slots,
+                               const int64_t* positions, void* output, void* workspace, int64_t workspace_bytes, float scale,
+                               int64_t tokens, int64_t requests, int64_t query_heads, int64_t kv_heads, int64_t head_dim,
+                               int64_t pages, int64_t page_size, int64_t slot_count, int64_t columns, int64_t table_stride,
+                               int64_t window, int64_t sinks, const int64_t* query_strides, const int64_t* key_strides,
+                               const int64_t* value_strides, hipStream_t stream) {
+    if (!query || !key_pages || !value_pages || !page_table || !lengths || !offsets || !output || !query_strides ||
+        !key_strides || !value_strides)
+        return invalid("flux_paged_chunk_attention: null argument");
+    flux::ChunkArgs args{};
+    if (const char* wrong = chunk_arguments(args, dtype, scale, tokens, requests, query_heads, kv_heads, head_dim, pages,
+                                            page_size, slot_count, columns, window, sinks))
+        return invalid(std::string("flux_paged_chunk_attention: ") + wrong);
+    if (!nonnegative(query_strides, 3) || !nonnegative(key_strides, 3) || !nonnegative(value_strides, 3) || table_stride < 0)
+        return invalid("flux_paged_chunk_attention: negative strides are unsupported");
+    if (!slots && slot_count < requests) return invalid("flux_paged_chunk_attention: fewer table rows than requests");
+    const auto type = static_cast<flux::Type>(dtype);
+    const auto needed = static_cast<int64_t>(flux::chunk_attention_workspace_floats(args, type) * sizeof(float));
+    if (needed > 0 && (!workspace || !aligned16(workspace) || workspace_bytes < needed))
+        return invalid("flux_paged_chunk_attention: workspace missing, too small (flux_paged_chunk_attention_workspace_bytes) "
+                       "or not 16-byte aligned");
+    args.query = query;
+    args.key = key_pages;
+    args.value = value_pages;
+    args.out = output;
+    args.workspace = static_cast<float*>(workspace);
+    args.table = page_table;
+    args.lengths = lengths;
+    args.offsets = offsets;
+    args.slots = slots;
+    args.positions = positions;
+    args.table_stride = table_stride;
+    for (int i = 0; i < 3; ++i) {
+        args.query_strides[i] = query_strides[i];
+        args.key_strides[i] = key_strides[i];
+        args.value_strides[i] = value_strides[i];
+    }
+    const int element = flux::type_bytes(type);
+    args.wide = wide_rows(key_pages, key_strides, 3, head_dim, element) && wide_rows(value_pages, value_strides, 3, head_dim, element);
+    args.query_wide = query_strides[2] == 1 && wide_rows(query, query_strides, 2, head_dim, element);
+    return from_hip(flux::launch_chunk_attention(args, type, stream), "flux_paged_chunk_attention");
+}
+
 int flux_window_attention_workspace_bytes(int64_t batch, int64_t query_heads, int64_t kv_heads, int64_t queries,
                                           int64_t head_dim, int64_t keys, int64_t window, int64_t sinks,
                                           int64_t* bytes) {
@@ -982,6 +1072,57 @@ int flux_page_write(const flux_page_pool* pool, const void* key, const void* val
     args.positions = positions;
     args.counts = counts;
     return from_hip(flux::launch_page_write(p, args, stream), "flux_page_write");
+}
+
+int flux_page_write_rows(const flux_page_pool* pool, const void* key, const void* value, const int64_t* key_strides,
+                         const int64_t* value_strides, int64_t tokens, const int64_t* rows, hipStream_t stream) {
+    flux::PagePool p{};
+    if (const char* wrong = pool_arguments(p, pool)) return invalid(std::string("flux_page_write_rows: ") + wrong);
+    if (!key || !value || !key_strides || !value_strides || !rows) return invalid("flux_page_write_rows: null argument");
+    if (p.layers != 1) return invalid("flux_page_write_rows: one layer is written at a time");
+    if (tokens <= 0 || tokens > FLUX_MAX_SERVING_KEYS || p.heads > (int64_t{1} << 24) / p.dim)
+        return invalid("flux_page_write_rows: invalid shape");
+    if (!nonnegative(key_strides, 2) || !nonnegative(value_strides, 2))
+        return invalid("flux_page_write_rows: negative strides are unsupported");
+    if (const char* wrong = pool_memory(p)) return invalid(std::string("flux_page_write_rows: ") + wrong);
+    flux::PageRowsArgs args{};
+    args.key = static_cast<const char*>(key);
+    args.value = static_cast<const char*>(value);
+    for (int i = 0; i < 2; ++i) {
+        args.key_strides[i] = key_strides[i];
+        args.value_strides[i] = value_strides[i];
+    }
+    args.tokens = tokens;
+    args.rows = rows;
+    return from_hip(flux::launch_page_write_rows(p, args, stream), "flux_page_write_rows");
+}
+
+int flux_step_layout(const int32_t* page_table, int64_t table_stride, int64_t slot_count, int64_t columns, int64_t page_size,
+                     const int64_t* slots, const int64_t* positions, const int64_t* counts, int64_t requests, int64_t tokens,
+                     int64_t* offsets, int64_t* token_requests, int64_t* token_positions, int64_t* token_rows,
+                     hipStream_t stream) {
+    if (!page_table || !slots || !positions || !offsets || !token_requests || !token_positions || !token_rows)
+        return invalid("flux_step_layout: null argument");
+    if (slot_count <= 0 || page_size <= 0 || page_size > FLUX_MAX_SERVING_KEYS || columns <= 0 ||
+        columns > FLUX_MAX_SERVING_KEYS / page_size || table_stride < 0 || requests <= 0 || requests > 65535 || tokens <= 0 ||
+        tokens > FLUX_MAX_SERVING_KEYS)
+        return invalid("flux_step_layout: invalid shape");
+    flux::StepLayoutArgs args{};
+    args.table = page_table;
+    args.table_stride = table_stride;
+    args.slot_count = slot_count;
+    args.columns = columns;
+    args.page = page_size;
+    args.slots = slots;
+    args.positions = positions;
+    args.counts = counts;
+    args.requests = static_cast<int>(requests);
+    args.tokens = tokens;
+    args.offsets = offsets;
+    args.token_requests = token_requests;
+    args.token_positions = token_positions;
+    args.token_rows = token_rows;
+    return from_hip(flux::launch_step_layout(args, stream), "flux_step_layout");
 }
 
 int flux_page_copy(const flux_page_pool* pool, const int64_t* source, const int64_t* target, int64_t requests,
@@ -1103,3 +1244,37 @@ int flux_logits_process(int dtype, const void* logits, int64_t logits_stride, vo
 }
 
 }  // extern "C"
+
+int flux_logits_sample_workspace_bytes(int64_t rows, int64_t vocab, int64_t* bytes) {
+    if (!bytes || rows <= 0 || rows > (1 << 20) || vocab <= 0 || vocab > (1 << 24))
+        return invalid("flux_logits_sample_workspace_bytes: invalid argument");
+    *bytes = static_cast<int64_t>(flux::sample_workspace_bytes(rows, vocab));
+    return FLUX_OK;
+}
+
+int flux_logits_sample(int dtype, const void* logits, int64_t logits_stride, const float* uniforms, const float* temperature,
+                       const int64_t* top_k, const float* top_p, const float* min_p, int64_t* tokens, float* probabilities,
+                       int64_t rows, int64_t vocab, void* workspace, int64_t workspace_bytes, hipStream_t stream) {
+    if (!logits || !uniforms || !tokens || !probabilities) return invalid("flux_logits_sample: null argument");
+    if (!known_type(dtype)) return invalid("flux_logits_sample: unknown dtype");
+    if (rows <= 0 || rows > (1 << 20) || vocab <= 0 || vocab > (1 << 24) || logits_stride < 0 ||
+        rows > (int64_t{1} << 32) / (vocab + 1023))
+        return invalid("flux_logits_sample: invalid shape");
+    const auto needed = static_cast<int64_t>(flux::sample_workspace_bytes(rows, vocab));
+    if (needed > 0 && (!workspace || workspace_bytes < needed))
+        return invalid("flux_logits_sample: workspace missing or too small (flux_logits_sample_workspace_bytes)");
+    flux::SampleArgs args{};
+    args.logits = logits;
+    args.logits_stride = logits_stride;
+    args.rows = rows;
+    args.vocab = vocab;
+    args.uniforms = uniforms;
+    args.temperature = temperature;
+    args.top_k = top_k;
+    args.top_p = top_p;
+    args.min_p = min_p;
+    args.tokens = tokens;
+    args.probabilities = probabilities;
+    args.workspace = workspace;
+    return from_hip(flux::launch_logits_sample(args, static_cast<flux::Type>(dtype), stream), "flux_logits_sample");
+}

@@ -1,0 +1,933 @@
+// Attention of a step's packed tokens over a K/V cache in pages: chunks of prompts next to single tokens.
+//
+//   o = sum exp(s_j - m) v_j / sum exp(s_j - m),  s_j = scale <q, k_j>,  m = max s_j   over the keys j that the token sees:
+//   j <= p and j < n, with j > p - window or j < sinks (window 0: all), on a page of the pool; nothing seen gives zeros.
+//
+// A tile is kRows rows of one request and KV head, a row being a token and one of the head's query heads, so that a
+// group of heads shares each key and value row.  Tiles whose keys are many for the step's work are cut into parts of whole
+// stages (kStage keys): every workgroup derives from the lists which part of which tile is its own, so that neither the
+// host nor a launch before has to know the lengths, and a second launch joins the parts: o = sum o_c 2^(m_c - M) / sum l_c 2^(m_c - M).
+#include "serving.h"
+#include "serving_mfma.h"
+
+namespace flux {
+namespace {
+
+constexpr int kThreads = 256;
+constexpr int kWaves = 4;
+constexpr int kLeastStages = 4;  // that are worth a workgroup
+
+template <class T>
+constexpr int rows_of_tile(int dim) { return sizeof(T) == 2 ? 32 * kWaves : (dim <= 128 ? 32 : 16); }
+template <class T>
+constexpr int stage_keys(int dim) { return sizeof(T) == 2 ? (dim == 64 ? 128 : (dim == 128 ? 64 : 32)) : 64; }
+constexpr int padded_dim(int dim) { return dim <= 64 ? 64 : (dim <= 128 ? 128 : 256); }
+
+// What the launches of one call agree on.
+struct ChunkPlan {
+    int rows;          // of a tile
+    int64_t tiles;     // at most, of one KV head
+    int target;        // parts of one KV head that a step's work is cut into
+    bool whole;        // no tile is cut
+    int64_t units;     // parts and whole tiles, at most, of one KV head
+    int64_t slots;     // parts of cut tiles, at most, of one KV head
+    int64_t splits;    // cut tiles, at most
+    int slot_rows;     // rows of a slot
+    int width;         // floats of a row: the dims in fours, the maximum, the sum
+};
+
+// In the workspace: the cut tiles' number, their descriptions, the parts' rows.
+constexpr int kDescription = 8;  // ints
+__host__ __device__ __forceinline__ int64_t parts_offset(const ChunkPlan& p) { return kDescription * (p.splits + 1); }
+__device__ __forceinline__ float* part_row(const ChunkArgs& a, const ChunkPlan& p, int kv_head, int64_t slot, int row) {
+    return a.workspace + parts_offset(p) + ((kv_head * p.slots + slot) * p.slot_rows + row) * p.width;
+}
+
+struct Sequence {
+    int begin, count;  // tokens
+    int64_t slot;      // row of the table; -1: none, and no keys
+    int n;             // keys
+    int start;         // position of the first token
+};
+
+__device__ __forceinline__ Sequence sequence_of(const ChunkArgs& a, int b) {
+    Sequence s;
+    const int64_t from = a.offsets[b], to = a.offsets[b + 1];
+    const int64_t begin = from < 0 ? 0 : (from < a.tokens ? from : a.tokens);
+    const int64_t end = to < begin ? begin : (to < a.tokens ? to : a.tokens);
+    s.begin = static_cast<int>(begin);
+    s.count = static_cast<int>(end - begin);
+    s.slot = a.slots ? a.slots[b] : b;
+    if (s.slot < 0 || s.slot >= a.slot_count) s.slot = -1;
+    int64_t n = s.slot >= 0 ? a.lengths[s.slot] : 0;
+    n = n < 0 ? 0 : (n < a.keys ? n : a.keys);
+    const int64_t length = static_cast<int64_t>(static_cast<uint64_t>(to) - static_cast<uint64_t>(from));
+    int64_t start = a.positions ? a.positions[b] : n - (length < 0 ? 0 : (length < (1 << 30) ? length : (1 << 30)));
+    start = start < -s.count ? -s.count : (start < a.keys ? start : a.keys);  // no token beyond these has a key's position
+    s.n = static_cast<int>(n);
+    s.start = static_cast<int>(start);
+    return s;
+}
+
+// The keys that any token of the positions first .. last sees, as stages: first the sinks', then the window's.
+template <int kStage>
+struct KeyStages {
+    int seen, sink_stages, first_stage, count;
+    __device__ __forceinline__ KeyStages(const ChunkArgs& a, int first, int last) {
+        const int low = a.window > 0 && first >= a.window ? first - a.window + 1 : 0;
+        const int sinks = a.sinks < low ? a.sinks : low;
+        const int of_sinks = (sinks + kStage - 1) / kStage;
+        seen = last + 1;
+        first_stage = low / kStage;
+        sink_stages = of_sinks < first_stage ? of_sinks : first_stage;
+        count = first > last ? 0 : sink_stages + (seen + kStage - 1) / kStage - first_stage;
+    }
+    __device__ __forceinline__ int base(int t) const { return (t < sink_stages ? t : first_stage + t - sink_stages) * kStage; }
+};
+
+// Positions of the rows [from, from + rows) that are a key's; first > last when there is none.
+__device__ __forceinline__ void positions_of(const ChunkArgs& a, const Sequence& s, int from, int rows, int& first, int& last) {
+    const int all = s.count * a.group, to = from + rows < all ? from + rows - 1 : all - 1;
+    const int p = s.start + static_cast<int>(divide(from, a.group_of)), q = s.start + static_cast<int>(divide(to < 0 ? 0 : to, a.group_of));
+    first = p < 0 ? 0 : p;
+    last = q >= s.n ? s.n - 1 : q;
+    if (from > to) last = first - 1;
+}
+
+// Stages of a request's longest tile, at most.
+template <int kRows, int kStage>
+__device__ __forceinline__ int most_stages(const ChunkArgs& a, const Sequence& s) {
+    const int last = s.start + s.count - 1 < s.n ? s.start + s.count - 1 : s.n - 1;
+    if (last < 0 || s.count == 0) return 0;
+    const int all = last / kStage + 1;
+    if (a.window == 0) return all;
+    const int windowed = (a.sinks + kStage - 1) / kStage + (a.window + static_cast<int>(divide(kRows, a.group_of)) + 1) / kStage + 2;
+    return windowed < all ? windowed : all;
+}
+
+// The part that a workgroup works on.
+struct Part {
+    int request, tile, part, parts;
+    int slot;   // of the part, when the tile is cut
+    bool real;  // some request has it
+};
+
+struct PlanShared {
+    int sums[3][kWaves];
+    int chosen[4];
+};
+
+__device__ __forceinline__ int64_t sum_of_block(int64_t v, int64_t* sums) {
+#pragma unroll
+    for (int step = 1; step < 64; step *= 2) v += __shfl_xor(static_cast<long long>(v), step, kWave);
+    __syncthreads();
+    if ((threadIdx.x & 63) == 0) sums[threadIdx.x >> 6] = v;
+    __syncthreads();
+    return sums[0] + sums[1] + sums[2] + sums[3];
+}
+
+template <int kRows, int kStage>
+__device__ Part part_of(const ChunkArgs& a, const ChunkPlan& plan, int unit, bool describes, Sequence& sequence) {
+    __shared__ PlanShared s;
+    __shared__ int64_t work_sums[kWaves];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    Sequence mine;
+    int tiles = 0, stages = 0;
+    auto look = [&](int b) {
+        tiles = stages = 0;
+        if (b >= a.requests) return;
+        mine = sequence_of(a, b);
+        tiles = static_cast<int>((static_cast<int64_t>(mine.count) * a.group + kRows - 1) / kRows);
+        stages = most_stages<kRows, kStage>(a, mine);
+    };
+    int each = 1 << 30;
+    if (!plan.whole) {
+        int64_t work = 0;
+        for (int base = 0; base < a.requests; base += kThreads) {
+            look(base + threadIdx.x);
+            work += sum_of_block(static_cast<int64_t>(tiles) * stages, work_sums);
+        }
+        const int64_t even = (work + plan.target - 1) / plan.target;
+        each = even < kLeastStages ? kLeastStages : (even < each ? static_cast<int>(even) : each);
+    }
+    int units_before = 0, slots_before = 0, splits_before = 0;
+    bool found = false;
+    for (int base = 0; base < a.requests; base += kThreads) {
+        const int b = base + static_cast<int>(threadIdx.x);
+        if (plan.whole || a.requests > kThreads) look(b);
+        const int parts = stages > each ? (stages + each - 1) / each : 1;
+        const int units = tiles * parts;
+        const int slots = parts > 1 ? units : 0, splits = parts > 1 ? tiles : 0;
+        int units_to = wave_scan_int(units), slots_to = wave_scan_int(slots), splits_to = wave_scan_int(splits);
+        __syncthreads();
+        if (lane == 63) s.sums[0][wave] = units_to, s.sums[1][wave] = slots_to, s.sums[2][wave] = splits_to;
+        __syncthreads();
+        for (int w = 0; w < wave; ++w) units_to += s.sums[0][w], slots_to += s.sums[1][w], splits_to += s.sums[2][w];
+        units_to += units_before, slots_to += slots_before, splits_to += splits_before;
+        if (unit < units_to && unit >= units_to - units) {
+            const int local = unit - (units_to - units);
+            s.chosen[0] = b;
+            s.chosen[1] = local;
+            s.chosen[2] = parts;
+            // Offsets that decrease could name more rows than there are: what has no room is left out.
+            const int split = splits_to - splits + local / parts, slot = slots_to - slots + local;
+            const bool room = parts == 1 || (slot >= 0 && slot - local % parts + parts <= plan.slots && split >= 0 && split < plan.splits);
+            s.chosen[3] = room ? slot : -1;
+            if (describes && parts > 1 && room && local % parts == 0) {
+                int* d = reinterpret_cast<int*>(a.workspace) + kDescription * (1 + split);
+                const int row0 = (tiles - 1 - local / parts) * kRows, rows = mine.count * a.group - row0;
+                d[0] = mine.begin;
+                d[1] = row0;
+                d[2] = rows < kRows ? rows : kRows;
+                d[3] = slot;
+                d[4] = parts;
+            }
+        }
+        for (int w = 0; w < kWaves; ++w)
+            units_before += s.sums[0][w], slots_before += s.sums[1][w], splits_before += s.sums[2][w];
+        found = found || units_before > unit;
+        if (found && !(describes && unit == 0)) break;
+    }
+    if (describes && unit == 0 && threadIdx.x == 0 && !plan.whole) *reinterpret_cast<int*>(a.workspace) = splits_before < plan.splits ? splits_before : static_cast<int>(plan.splits);
+    __syncthreads();
+    Part part{0, 0, 0, 1, 0, found};
+    if (!found) return part;
+    part.request = s.chosen[0];
+    part.parts = s.chosen[2];
+    part.part = s.chosen[1] % part.parts;
+    part.slot = s.chosen[3];
+    part.real = part.slot >= 0;
+    sequence = sequence_of(a, part.request);
+    // The longest tiles first.
+    part.tile = static_cast<int>((static_cast<int64_t>(sequence.count) * a.group + kRows - 1) / kRows) - 1 - s.chosen[1] / part.parts;
+    return part;
+}
+
+// Rows before the first request and behind the last are zeros.
+template <class T>
+__device__ __forceinline__ void clear_other_rows(const ChunkArgs& a) {
+    const int64_t from = a.offsets[0], to = a.offsets[a.requests];
+    const int64_t before = from < 0 ? 0 : (from < a.tokens ? from : a.tokens), behind = to < 0 ? 0 : (to < a.tokens ? to : a.tokens);
+    const int64_t others = before + a.tokens - behind;
+    const int width = a.query_heads * a.dim;
+    T* out = static_cast<T*>(a.out);
+    for (int64_t i = blockIdx.x; i < others; i += gridDim.x) {
+        T* row = out + (i < before ? i : behind + i - before) * width;
+        for (int d = threadIdx.x; d < width; d += kThreads) row[d] = static_cast<T>(0.0f);
+    }
+}
+
+// This lane's row of the tile.
+struct Row {
+    int position;  // -1: sees nothing
+    int low;       // first key of the window
+    int sink_end;
+};
+__device__ __forceinline__ Row row_of(const ChunkArgs& a, const Sequence& s, int r) {
+    Row row;
+    const int position = s.start + static_cast<int>(divide(r, a.group_of));
+    row.position = r < s.count * a.group && position >= 0 && position < s.n ? position : -1;
+    row.low = a.window > 0 && row.position >= a.window ? row.position - a.window + 1 : 0;
+    row.sink_end = a.sinks < row.low ? a.sinks : row.low;
+    return row;
+}
+
+// Weights of 16-bit types are 2^(s log2(e) - top) by one fused product, top = m log2(e) rounded: what that moves is common to
+// all weights of a row and cancels, unless top is so large that it moves them out of float32's range.  From kFar on the
+// difference s - m is taken first.
+constexpr float kFar = 4194304.0f;
+
+// What the join needs to know of a part's row: the maximum that its weights refer to, in the exponent's unit (powers of two for
+// 16-bit types), its sum of weights, and the maximum of the scores.
+__device__ __forceinline__ void put_statistics(float* to, float top, float weight, float natural) {
+    to[0] = top;
+    to[1] = weight;
+    to[2] = natural;
+}
+
+// A row whose sums are not finite, computed again over the keys it sees alone: a matrix instruction multiplies a masked
+// key's zero weight with its value too, and a NaN or infinity there must not reach the row.  One wave.
+template <class T, int kStage>
+__device__ void exact_row(const ChunkArgs& a, const ChunkPlan& plan, const Sequence& s, const Part& part, int kv_head, int row0, int r,
+                          const KeyStages<kStage>& stages, int from, int to, float shift) {
+    const int lane = threadIdx.x & 63;
+    const Row row = row_of(a, s, r);
+    const int i = static_cast<int>(divide(r, a.group_of)), head = kv_head * a.group + r - i * a.group;
+    const int64_t token = s.begin + i;
+    const T* query = static_cast<const T*>(a.query) + token * a.query_strides[0] + head * a.query_strides[1];
+    const T* keys = static_cast<const T*>(a.key) + kv_head * a.key_strides[1];
+    const T* values = static_cast<const T*>(a.value) + kv_head * a.value_strides[1];
+    const int32_t* table = a.table + (s.slot < 0 ? 0 : s.slot) * a.table_stride;
+    float top = -INFINITY, weight = 0.0f, sum[kServingMaxDim / kWave];
+#pragma unroll
+    for (int c = 0; c < kServingMaxDim / kWave; ++c) sum[c] = 0.0f;
+    for (int at = from * kStage; at < to * kStage; at += kWave) {
+        const int t = (at + lane) / kStage, position = stages.base(t) + (at + lane) % kStage;
+        bool seen = t < to && row.position >= 0 && position <= row.position && (position >= row.low || position < row.sink_end);
+        int64_t page = 0, in_page = 0;
+        if (seen) {
+            const uint32_t column = divide(position, a.page);
+            page = table[column];
+            in_page = position - column * a.page.divisor;
+            seen = page >= 0 && page < a.pages;
+        }
+        float score = -INFINITY;
+        if (seen) {
+            const T* key = keys + page * a.key_strides[0] + in_page * a.key_strides[2];
+            score = 0.0f;
+            for (int d = 0; d < a.dim; ++d)
+                score = fmaf(static_cast<float>(query[d * a.query_strides[2]]), static_cast<float>(key[d]), score);
+            score *= a.scale;
+        }
+        const float now = fmaxf(top, wave_max(score));
+        const float reference = now == -INFINITY ? 0.0f : now, scaled = reference * kLog2e;
+        const bool near = sizeof(T) == 2 && fabsf(scaled) < kFar;
+        auto difference = [&](float x) { return near ? fmaf(x, kLog2e, -scaled) : (x - reference) * kLog2e; };
+        const float shrink = top == -INFINITY ? 0.0f : fast_exp2(near ? top * kLog2e - scaled : (top - reference) * kLog2e);
+        top = now;
+        const float p = seen ? fast_exp2(difference(score) + shift) : 0.0f;
+        weight = weight * shrink + wave_sum(p);
+#pragma unroll
+        for (int c = 0; c < kServingMaxDim / kWave; ++c) sum[c] *= shrink;
+        const int64_t place = seen ? page * a.value_strides[0] + in_page * a.value_strides[2] : -1;
+        for (int j = 0; j < kWave; ++j) {
+            const int64_t of = __shfl(static_cast<long long>(place), j, kWave);
+            const float pj = __shfl(p, j, kWave);
+            if (of < 0) continue;
+#pragma unroll
+            for (int c = 0; c < kServingMaxDim / kWave; ++c)
+                if (kWave * c + lane < a.dim) sum[c] = fmaf(pj, static_cast<float>(values[of + kWave * c + lane]), sum[c]);
+        }
+        // What is NaN stays NaN: a row whose sums all are is done.
+        bool lost = true;
+#pragma unroll
+        for (int c = 0; c < kServingMaxDim / kWave; ++c) lost = lost && (kWave * c + lane >= a.dim || sum[c] != sum[c]);
+        if (__all(weight != weight || lost)) break;
+    }
+    T* out = static_cast<T*>(a.out) + (token * a.query_heads + head) * a.dim;
+    float* partial = part.parts > 1 ? part_row(a, plan, kv_head, part.slot, r - row0) : nullptr;
+#pragma unroll
+    for (int c = 0; c < kServingMaxDim / kWave; ++c) {
+        const int d = kWave * c + lane;
+        if (d >= a.dim) continue;
+        if (partial) partial[d] = sum[c];
+        else out[d] = static_cast<T>(weight == 0.0f ? 0.0f : sum[c] / weight);
+    }
+    if (partial && lane == 0) put_statistics(partial + plan.width - 4, sizeof(T) == 2 ? top * kLog2e : top, weight, top);
+}
+
+// ---------------------------------------------------------------------------
+// float32: everything in registers; a workgroup's four waves split a tile's keys and join at the end.
+template <int kDim, Rows kRowsRead>
+__global__ void __launch_bounds__(kThreads, kDim <= 64 ? 3 : (kDim <= 128 ? 2 : 1)) chunk_register_kernel(ChunkArgs a, ChunkPlan plan) {
+    using M = Mfma<float>;
+    constexpr int kRows = rows_of_tile<float>(kDim);
+    constexpr int kCols = kRows / 16;
+    constexpr int kStage = stage_keys<float>(kDim);
+    constexpr int kTile = 16;
+    constexpr int kFragments = M::template key_fragments<kDim>();
+    constexpr int kChunks = M::template value_chunks<kDim>();
+    constexpr int kBlocks = kDim / 16;
+    constexpr int kWords = kBlocks * 4 + 2;
+    static_assert(kStage == kTile * kWaves, "a stage is one tile for each wave");
+    __shared__ float merge[2][kCols * kWords][kWave];
+
+    clear_other_rows<float>(a);
+    const int kv_head = blockIdx.x % a.kv_heads, unit = blockIdx.x / a.kv_heads;
+    Sequence s;
+    const Part part = part_of<kRows, kStage>(a, plan, unit, kv_head == 0, s);
+    if (!part.real) return;
+    const int lane = threadIdx.x & 63;
+    const int wave = threadIdx.x >> 6;
+    const int n16 = lane & 15;
+    const int g = lane >> 4;
+    const int row0 = part.tile * kRows, all_rows = s.count * a.group;
+    const float* keys = static_cast<const float*>(a.key) + kv_head * a.key_strides[1];
+    const float* values = static_cast<const float*>(a.value) + kv_head * a.value_strides[1];
+    const int32_t* table = a.table + (s.slot < 0 ? 0 : s.slot) * a.table_stride;
+
+    int first_p, last_p;
+    positions_of(a, s, row0, kRows, first_p, last_p);
+    const KeyStages<kStage> stages(a, first_p, last_p);
+    const int from = static_cast<int>(static_cast<int64_t>(stages.count) * part.part / part.parts);
+    const int to = static_cast<int>(static_cast<int64_t>(stages.count) * (part.part + 1) / part.parts);
+    Row mine[kCols];
+    f32x4 query[kCols][kFragments];
+    f32x4 out[kCols][kBlocks];
+    float top[kCols], weight[kCols];
+#pragma unroll
+    for (int c = 0; c < kCols; ++c) {
+        const int r = row0 + 16 * c + n16;
+        const bool real = r < all_rows;
+        const int i = static_cast<int>(divide(real ? r : row0, a.group_of)), head = kv_head * a.group + (real ? r : row0) - i * a.group;
+        mine[c] = row_of(a, s, r);
+        const float* q = static_cast<const float*>(a.query) + static_cast<int64_t>(s.begin + i) * a.query_strides[0] + head * a.query_strides[1];
+        load_query<float, kFragments, M::kKeyStep>(query[c], q, a.query_strides[2], a.query_wide, M::kPer * g, a.dim, real);
+#pragma unroll
+        for (int k = 0; k < kBlocks; ++k) out[c][k] = f32x4{0, 0, 0, 0};
+        top[c] = -INFINITY;
+        weight[c] = 0.0f;
+    }
+    const int low_of_last = a.window > 0 && last_p >= a.window ? last_p - a.window + 1 : 0;
+
+    // This wave's tile of stage t.  Rows behind the last key repeat it; keys on no page are the pool's first row.
+    auto position_of = [&](int t) {
+        const int position = stages.base(t) + kTile * wave + n16;
+        return position < stages.seen ? position : stages.seen - 1;
+    };
+    auto look_up = [&](int t) { return t < to ? table[divide(position_of(t), a.page)] : -1; };
+    auto work = [&](int t, int page) {
+        const int base = stages.base(t) + kTile * wave;
+        if (base >= stages.seen) return;
+        const bool held = page >= 0 && page < a.pages;
+        const bool whole = __all(held);
+        const int position = position_of(t);
+        const int in_page = held ? position - static_cast<int>(divide(position, a.page) * a.page.divisor) : 0;
+        const int64_t of_page = held ? page : 0;
+        f32x4 key[kFragments], value[4][kChunks];
+        const float* k = keys + of_page * a.key_strides[0] + in_page * a.key_strides[2];
+#pragma unroll
+        for (int f = 0; f < kFragments; ++f) key[f] = M::template load_row<kRowsRead>(k, M::kKeyStep * f + M::kPer * g, a.dim);
+        const int64_t value_at = of_page * a.value_strides[0] + in_page * a.value_strides[2];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const float* v = values + __shfl(static_cast<long long>(value_at), 4 * g + i, kWave);
+#pragma unroll
+            for (int c = 0; c < kChunks; ++c) value[i][c] = M::template load_value<kDim, kRowsRead>(v, c, n16, a.dim);
+        }
+        uint32_t missing = 0;
+        if (!whole) {
+            missing = static_cast<uint32_t>(__ballot(!held));
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                if (missing >> (4 * g + i) & 1) {
+#pragma unroll
+                    for (int c = 0; c < kChunks; ++c) value[i][c] = f32x4{0, 0, 0, 0};
+                }
+        }
+        // Every key of the tile is seen by every row that sees any (the others are zeroed at the end).
+        const bool inside = whole && base >= low_of_last && base + kTile - 1 <= first_p;
+#pragma unroll
+        for (int c = 0; c < kCols; ++c) {
+            f32x4 score = {0, 0, 0, 0};
+#pragma unroll
+            for (int f = 0; f < kFragments; ++f) M::multiply_key(key[f], query[c][f], score);
+            float highest = -INFINITY;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const int j = base + 4 * g + i;
+                // Without branches: low <= key <= position as one unsigned comparison, or a sink.
+                const bool visible = inside | (((static_cast<uint32_t>(j - mine[c].low) <=
+                                                 static_cast<uint32_t>(mine[c].position - mine[c].low)) | (j < mine[c].sink_end)) &
+                                               !(missing >> (4 * g + i) & 1));
+                score[i] = visible ? score[i] * a.scale : -INFINITY;
+                highest = fmaxf(highest, score[i]);
+            }
+            highest = fmaxf(highest, __shfl_xor(highest, 16, kWave));
+            highest = fmaxf(highest, __shfl_xor(highest, 32, kWave));
+            if (__any(highest > top[c])) {
+                const float now = fmaxf(top[c], highest);
+                const float shrink = top[c] == -INFINITY ? 0.0f : fast_exp2((top[c] - now) * kLog2e);
+                top[c] = now;
+                weight[c] *= shrink;
+#pragma unroll
+                for (int i = 0; i < kBlocks; ++i) out[c][i] *= shrink;
+            }
+            const float reference = top[c] == -INFINITY ? 0.0f : top[c];
+            float p[1][4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                p[0][i] = fast_exp2((score[i] - reference) * kLog2e);
+                weight[c] += p[0][i];
+            }
+            f32x4 turned[1][4][kChunks];
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+#pragma unroll
+                for (int k2 = 0; k2 < kChunks; ++k2) turned[0][i][k2] = value[i][k2];
+            M::template multiply_value<kDim, 1>(turned, p, out[c]);
+        }
+    };
+    int page = look_up(from);
+    for (int t = from; t < to; ++t) {
+        const int next = look_up(t + 1);
+        work(t, page);
+        page = next;
+    }
+
+#pragma unroll
+    for (int c = 0; c < kCols; ++c) {
+        weight[c] += __shfl_xor(weight[c], 16, kWave);
+        weight[c] += __shfl_xor(weight[c], 32, kWave);
+    }
+    // Join the four waves: 2 and 3 into 0 and 1, then 1 into 0.
+#pragma unroll
+    for (int half = kWaves / 2; half >= 1; half /= 2) {
+        if (half == 1) __syncthreads();
+        if (wave >= half && wave < 2 * half) {
+#pragma unroll
+            for (int c = 0; c < kCols; ++c) {
+                float(*into)[kWave] = merge[wave - half] + c * kWords;
+#pragma unroll
+                for (int i = 0; i < kBlocks * 4; ++i) into[i][lane] = out[c][i / 4][i % 4];
+                into[kBlocks * 4][lane] = top[c];
+                into[kBlocks * 4 + 1][lane] = weight[c];
+            }
+        }
+        __syncthreads();
+        if (wave < half) {
+#pragma unroll
+            for (int c = 0; c < kCols; ++c) {
+                const float(*other)[kWave] = merge[wave] + c * kWords;
+                const float other_top = other[kBlocks * 4][lane];
+                const float now = fmaxf(top[c], other_top);
+                const float mine_scale = top[c] == -INFINITY ? 0.0f : fast_exp2((top[c] - now) * kLog2e);
+                const float other_scale = other_top == -INFINITY ? 0.0f : fast_exp2((other_top - now) * kLog2e);
+                top[c] = now;
+                weight[c] = weight[c] * mine_scale + other[kBlocks * 4 + 1][lane] * other_scale;
+#pragma unroll
+                for (int i = 0; i < kBlocks * 4; ++i)
+                    out[c][i / 4][i % 4] = out[c][i / 4][i % 4] * mine_scale + other[i][lane] * other_scale;
+            }
+        }
+    }
+    if (wave != 0) return;
+#pragma unroll
+    for (int c = 0; c < kCols; ++c) {
+        float worst = fabsf(weight[c]);
+        M::template each_dim<kDim>(g, a.dim, [&](int i, int r, int) { worst += fabsf(out[c][i][r]); });  // keeps NaN, infinity
+        const uint64_t odd = __ballot(mine[c].position >= 0 && !(worst < INFINITY));
+        uint32_t again = static_cast<uint32_t>((odd | odd >> 16 | odd >> 32 | odd >> 48) & 0xffff);
+        const int r = row0 + 16 * c + n16;
+        if (r < all_rows && !(again >> n16 & 1)) {
+            const int i = static_cast<int>(divide(r, a.group_of)), head = kv_head * a.group + r - i * a.group;
+            if (part.parts == 1) {
+                float* o = static_cast<float*>(a.out) + (static_cast<int64_t>(s.begin + i) * a.query_heads + head) * a.dim;
+                M::template each_dim<kDim>(g, a.dim, [&](int k, int j, int d) {
+                    o[d] = mine[c].position < 0 || weight[c] == 0.0f ? 0.0f : out[c][k][j] / weight[c];
+                });
+            } else {
+                float* o = part_row(a, plan, kv_head, part.slot, r - row0);
+                M::template each_dim<kDim>(g, a.dim, [&](int k, int j, int d) { o[d] = out[c][k][j]; });
+                const float highest = mine[c].position < 0 ? -INFINITY : top[c];
+                if (g == 0) put_statistics(o + plan.width - 4, highest, mine[c].position < 0 ? 0.0f : weight[c], highest);
+            }
+        }
+        while (again) {
+            const int which = __ffs(again) - 1;
+            again &= again - 1;
+            exact_row<float, kStage>(a, plan, s, part, kv_head, row0, row0 + 16 * c + which, stages, from, to, 0.0f);
+        }
+    }
+}
+
+// ---------------------------------------------------------------------------
+// 16-bit types: keys and values are staged in LDS for the workgroup's four waves, 32 rows each.  A stage holds kStage
+// keys: K rows as they are, V transposed (the staging thread permutes the 16-bit halves of four keys), its keys in the
+// order in which a lane's scores lie.  S^T = K Q^T on 32 x 32 tiles leaves lane (n, h) with the keys 8 (r / 4) + 4 h + r % 4
+// of row n, which rounded in pairs are the right operand of O^T = V^T P.  Where a stage's rows lie is looked up two stages
+// ahead.  Weights are rounded once to the values' type for the product and summed unrounded; the running maximum moves
+// only when a tile exceeds it by 2^kLazy.
+template <class T, int kDim, bool kWide>
+__global__ void __launch_bounds__(kThreads, kDim <= 128 ? 2 : 1) chunk_tile_kernel(ChunkArgs a, ChunkPlan plan) {
+    using W = Wide<T>;
+    constexpr int kStage = stage_keys<T>(kDim);
+    constexpr int kSubs = kStage / 32;
+    constexpr int kSteps = kDim / 16;             // of a score
+    constexpr int kBlocks = kDim / 32;            // of the result
+    constexpr int kRows = rows_of_tile<T>(kDim);
+    constexpr int kKeyRow = kDim * 2 + 16;        // bytes
+    constexpr int kValueRow = kStage * 2 + 16;
+    constexpr int kBytes = kStage * kKeyRow + kDim * kValueRow;
+    constexpr int kKeyLoads = kStage * kDim / 8 / kThreads;        // 16 bytes per thread
+    constexpr int kKeyRows = kThreads / (kDim / 8);                // rows that one load of all threads covers
+    static_assert(kStage / 4 * (kDim / 8) == kThreads, "every thread stages four keys by eight dims of the values");
+    extern __shared__ char stages_memory[];
+    __shared__ int64_t places[2][2][kStage];   // elements from the pool's start, by stage parity
+    __shared__ uint32_t missing[2][kSubs];     // keys of a stage that are on no page
+
+    clear_other_rows<T>(a);
+    const int kv_head = blockIdx.x % a.kv_heads, unit = blockIdx.x / a.kv_heads;
+    Sequence s;
+    const Part part = part_of<kRows, kStage>(a, plan, unit, kv_head == 0, s);
+    if (!part.real) return;
+    const int lane = threadIdx.x & 63;
+    const int wave = threadIdx.x >> 6;
+    const int n32 = lane & 31;
+    const int half = lane >> 5;
+    const int row0 = part.tile * kRows, all_rows = s.count * a.group, wave_row = row0 + wave * 32;
+    int block_first, block_last, wave_first, wave_last;
+    positions_of(a, s, row0, kRows, block_first, block_last);
+    positions_of(a, s, wave_row, 32, wave_first, wave_last);
+    wave_first = __builtin_amdgcn_readfirstlane(wave_first);
+    wave_last = __builtin_amdgcn_readfirstlane(wave_last);
+    const KeyStages<kStage> stages(a, block_first, block_last);
+    const int from = static_cast<int>(static_cast<int64_t>(stages.count) * part.part / part.parts);
+    const int to = static_cast<int>(static_cast<int64_t>(stages.count) * (part.part + 1) / part.parts);
+
+    const T* keys = static_cast<const T*>(a.key) + kv_head * a.key_strides[1];
+    const T* values = static_cast<const T*>(a.value) + kv_head * a.value_strides[1];
+    const int32_t* table = a.table + (s.slot < 0 ? 0 : s.slot) * a.table_stride;
+
+    const int r = wave_row + n32;  // this lane's row
+    const bool real = r < all_rows;
+    const int index = static_cast<int>(divide(real ? r : row0, a.group_of)), head = kv_head * a.group + (real ? r : row0) - index * a.group;
+    const Row mine = row_of(a, s, r);
+    const uint32_t sign = a.scale < 0.0f ? 0x80008000u : 0u;  // the scale's sign goes to the query
+    // Its size goes into the exponent's argument, unless it is 0 (which makes a masked score's -inf NaN, and has to make an
+    // infinite score NaN) or next to what float32 holds: then it multiplies the scores before they are masked.
+    const float size = fabsf(a.scale);
+    const bool ordinary = size >= 1e-30f && size <= 1e30f;
+    const float factor = ordinary ? size * kLog2e : kLog2e;
+    f32x16 out[kBlocks];
+#pragma unroll
+    for (int i = 0; i < kBlocks; ++i)
+#pragma unroll
+        for (int j = 0; j < 16; ++j) out[i][j] = 0.0f;
+    float top = -INFINITY, weight = 0.0f;
+
+    if (from < to) {
+        u32x4 query[kSteps];
+        load_query<T, kSteps, 16>(query, static_cast<const T*>(a.query) + static_cast<int64_t>(s.begin + index) * a.query_strides[0] +
+                                             head * a.query_strides[1],
+                                  a.query_strides[2], a.query_wide, 8 * half, a.dim, real);
+#pragma unroll
+        for (int k = 0; k < kSteps; ++k) query[k] ^= sign;
+        auto low_of = [&](int p) { return a.window > 0 && p >= a.window ? p - a.window + 1 : 0; };
+
+        // Threads below kStage look up one key each.  Rows behind the last key repeat it; keys on no page are the pool's first.
+        auto position_of = [&](int t) {
+            const int position = stages.base(t) + static_cast<int>(threadIdx.x);
+            return position < stages.seen ? position : stages.seen - 1;
+        };
+        auto look_up = [&](int t) {
+            return t < to && static_cast<int>(threadIdx.x) < kStage ? table[divide(position_of(t), a.page)] : 0;
+        };
+        auto put_places = [&](int t, int page) {
+            if (t >= to || static_cast<int>(threadIdx.x) >= kStage) return;
+            const int position = position_of(t);
+            const bool held = page >= 0 && page < a.pages;
+            const int64_t of_page = held ? page : 0;
+            const int in_page = held ? position - static_cast<int>(divide(position, a.page) * a.page.divisor) : 0;
+            places[t & 1][0][threadIdx.x] = of_page * a.key_strides[0] + in_page * a.key_strides[2];
+            places[t & 1][1][threadIdx.x] = of_page * a.value_strides[0] + in_page * a.value_strides[2];
+            const uint64_t gone = __ballot(!held);
+            if (lane == 0) missing[t & 1][threadIdx.x / 32] = static_cast<uint32_t>(gone);
+            if (lane == 32) missing[t & 1][threadIdx.x / 32] = static_cast<uint32_t>(gone >> 32);
+        };
+        u32x4 held_key[kKeyLoads];
+        u32x4 held_value[4];
+        const int key_row = threadIdx.x / (kDim / 8), key_d = threadIdx.x % (kDim / 8) * 8;
+        const int value_row = threadIdx.x % (kStage / 4) * 4, value_d = threadIdx.x / (kStage / 4) * 8;
+        auto load = [&](const T* row, int d) {
+            if constexpr (kWide) return *reinterpret_cast<const u32x4*>(row + (d < a.dim ? d : 0));
+            else return Mfma<T>::load_strided(row, 1, d, a.dim);
+        };
+        auto fetch_keys = [&](int t) {
+#pragma unroll
+            for (int i = 0; i < kKeyLoads; ++i) held_key[i] = load(keys + places[t & 1][0][key_row + kKeyRows * i], key_d);
+        };
+        auto fetch_values = [&](int t) {
+#pragma unroll
+            for (int j = 0; j < 4; ++j) held_value[j] = load(values + places[t & 1][1][value_row + j], value_d);
+        };
+        auto put_keys = [&](char* stage) {
+#pragma unroll
+            for (int i = 0; i < kKeyLoads; ++i) {
+                const int at = threadIdx.x + kThreads * i;
+                *reinterpret_cast<u32x4*>(stage + at / (kDim / 8) * kKeyRow + at % (kDim / 8) * 16) = held_key[i];
+            }
+        };
+        auto put_values = [&](char* stage, int t) {
+            const uint32_t gone = missing[t & 1][value_row / 32] >> (value_row % 32) & 15u;
+            if (gone) {  // a weight of zero does not undo a NaN
+#pragma unroll
+                for (int j = 0; j < 4; ++j)
+                    if (gone >> j & 1) held_value[j] = u32x4{0, 0, 0, 0};
+            }
+            char* turned = stage + kStage * kKeyRow;
+            // Quads 0, 1, 2, 3 of 16 keys lie as 0, 2, 1, 3: a lane's eight keys side by side.
+            const int quad = value_row / 4, at = (quad & ~3) | (quad & 1) << 1 | (quad >> 1 & 1);
+#pragma unroll
+            for (int j = 0; j < 8; ++j)
+                *reinterpret_cast<u32x2*>(turned + (value_d + j) * kValueRow + at * 8) =
+                    u32x2{Mfma<T>::pair(held_value[0][j / 2], held_value[1][j / 2], j & 1),
+                          Mfma<T>::pair(held_value[2][j / 2], held_value[3][j / 2], j & 1)};
+        };
+
+        const int wave_low = low_of(wave_first), low_of_last = low_of(wave_last);
+        put_places(from, look_up(from));
+        put_places(from + 1, look_up(from + 1));
+        __syncthreads();
+        uint32_t gone_next[kSubs];
+#pragma unroll
+        for (int i = 0; i < kSubs; ++i) gone_next[i] = missing[from & 1][i];
+        fetch_keys(from);
+        fetch_values(from);
+        put_keys(stages_memory + (from & 1) * kBytes);
+        put_values(stages_memory + (from & 1) * kBytes, from);
+        for (int t = from; t < to; ++t) {
+            __syncthreads();
+            const char* stage = stages_memory + (t & 1) * kBytes;
+            const char* turned = stage + kStage * kKeyRow;
+            const int base = stages.base(t);
+            char* next = stages_memory + ((t + 1) & 1) * kBytes;
+            uint32_t gone[kSubs];  // read a stage ahead: that of this one may be another's already
+#pragma unroll
+            for (int i = 0; i < kSubs; ++i) gone[i] = gone_next[i], gone_next[i] = t + 1 < to ? missing[(t + 1) & 1][i] : 0;
+            const int page = look_up(t + 2);
+            if (t + 1 < to) fetch_keys(t + 1);
+#pragma unroll
+            for (int i = 0; i < kSubs; ++i) {
+                if (i == kSubs / 2 && t + 1 < to) {  // K and V take the same registers on their way
+                    put_keys(next);
+                    fetch_values(t + 1);
+                }
+                const int first = base + 32 * i, last = first + 31;
+                // Nothing of this wave's rows sees these keys.
+                if (first > wave_last || (last < wave_low && first >= a.sinks)) continue;
+                u32x4 key[kSteps];
+#pragma unroll
+                for (int k = 0; k < kSteps; ++k)
+                    key[k] = *reinterpret_cast<const u32x4*>(stage + (32 * i + n32) * kKeyRow + 32 * k + 16 * half);
+                __builtin_amdgcn_sched_barrier(0);  // all reads first: one wait
+                f32x16 score;
+#pragma unroll
+                for (int j = 0; j < 16; ++j) score[j] = 0.0f;
+#pragma unroll
+                for (int k = 0; k < kSteps; ++k) score = W::multiply(key[k], query[k], score);
+                if (!ordinary) {
+#pragma unroll
+                    for (int j = 0; j < 16; ++j) score[j] *= size;
+                }
+                if (first < low_of_last || last > wave_first || __builtin_amdgcn_readfirstlane(gone[i]) != 0) {
+#pragma unroll
+                    for (int j = 0; j < 16; ++j) {
+                        // Without branches: low <= key <= position as one unsigned comparison, or a sink.
+                        const int in = 8 * (j / 4) + 4 * half + j % 4, of = first + in;
+                        const bool visible = ((static_cast<uint32_t>(of - mine.low) <= static_cast<uint32_t>(mine.position - mine.low)) |
+                                              (of < mine.sink_end)) & !(gone[i] >> in & 1);
+                        score[j] = visible ? score[j] : -INFINITY;
+                    }
+                }
+                float highest = score[0];
+#pragma unroll
+                for (int j = 1; j < 16; ++j) highest = fmaxf(highest, score[j]);
+                highest = half_max(highest);
+                if (__any((highest - top) * factor > W::kLazy)) {  // NaN where both are -inf
+                    const float now = fmaxf(top, highest);
+                    const float scaled = now * factor;
+                    const float shrink = top == -INFINITY ? 0.0f : fast_exp2(fabsf(scaled) < kFar ? top * factor - scaled : (top - now) * factor);
+                    top = now;
+                    weight *= shrink;
+#pragma unroll
+                    for (int k = 0; k < kBlocks; ++k)
+#pragma unroll
+                        for (int j = 0; j < 16; ++j) out[k][j] *= shrink;
+                }
+                u32x4 value[kBlocks][2];
+#pragma unroll
+                for (int b = 0; b < kBlocks; ++b)
+#pragma unroll
+                    for (int k = 0; k < 2; ++k)
+                        value[b][k] = *reinterpret_cast<const u32x4*>(turned + (32 * b + n32) * kValueRow + (32 * i + 16 * k) * 2 + 16 * half);
+                __builtin_amdgcn_sched_barrier(0);
+                const float scaled = top == -INFINITY ? 0.0f : top * factor;
+                const bool far = !(fabsf(scaled) < kFar);
+                const float reference = W::kShift - (far ? 0.0f : scaled);
+                if (__any(far)) {
+#pragma unroll
+                    for (int j = 0; j < 16; ++j) score[j] = far ? score[j] - top : score[j];
+                }
+                u32x4 p[2];
+#pragma unroll
+                for (int j = 0; j < 16; j += 2) {
+                    const float p0 = fast_exp2(fmaf(score[j], factor, reference));
+                    const float p1 = fast_exp2(fmaf(score[j + 1], factor, reference));
+                    weight += p0 + p1;
+                    p[j / 8][j % 8 / 2] = W::round(p0, p1);
+                }
+#pragma unroll
+                for (int b = 0; b < kBlocks; ++b)
+#pragma unroll
+                    for (int k = 0; k < 2; ++k) out[b] = W::multiply(value[b][k], p[k], out[b]);
+            }
+            if (t + 1 < to) put_values(next, t + 1);
+            put_places(t + 2, page);
+        }
+    }
+
+    weight = half_sum(weight);
+    float worst = fabsf(weight);
+#pragma unroll
+    for (int i = 0; i < kBlocks; ++i)
+#pragma unroll
+        for (int j = 0; j < 16; ++j) worst += fabsf(out[i][j]);  // keeps NaN, infinity
+    const uint64_t odd = __ballot(mine.position >= 0 && !(worst < INFINITY));
+    uint32_t again = static_cast<uint32_t>(odd | odd >> 32);
+    if (real && !(again >> n32 & 1)) {
+        if (part.parts == 1) {
+            T* o = static_cast<T*>(a.out) + (static_cast<int64_t>(s.begin + index) * a.query_heads + head) * a.dim;
+            const float inverse = weight == 0.0f ? 0.0f : 1.0f / weight;
+#pragma unroll
+            for (int i = 0; i < kBlocks; ++i)
+#pragma unroll
+                for (int j = 0; j < 16; j += 4) {
+                    const int d = 32 * i + 2 * j + 4 * half;  // four dims side by side
+                    float four[4];
+#pragma unroll
+                    for (int l = 0; l < 4; ++l) four[l] = mine.position < 0 ? 0.0f : out[i][j + l] * inverse;
+                    const u32x2 rounded = {W::round(four[0], four[1]), W::round(four[2], four[3])};
+                    if constexpr (kWide) {
+                        if (d < a.dim) *reinterpret_cast<u32x2*>(o + d) = rounded;
+                    } else {
+#pragma unroll
+                        for (int l = 0; l < 4; ++l)
+                            if (d + l < a.dim) o[d + l] = __builtin_bit_cast(T, static_cast<uint16_t>(rounded[l / 2] >> 16 * (l % 2)));
+                    }
+                }
+        } else {
+            float* o = part_row(a, plan, kv_head, part.slot, r - row0);
+#pragma unroll
+            for (int i = 0; i < kBlocks; ++i)
+#pragma unroll
+                for (int j = 0; j < 16; j += 4) {
+                    const int d = 32 * i + 2 * j + 4 * half;
+                    if (d < a.dim) *reinterpret_cast<f32x4*>(o + d) = f32x4{out[i][j], out[i][j + 1], out[i][j + 2], out[i][j + 3]};
+                }
+            const float highest = mine.position < 0 ? -INFINITY : top;
+            if (half == 0)
+                put_statistics(o + plan.width - 4, highest * factor, mine.position < 0 ? 0.0f : weight, ordinary ? highest * size : highest);
+        }
+    }
+    while (again) {
+        const int which = __ffs(again) - 1;
+        again &= again - 1;
+        exact_row<T, kStage>(a, plan, s, part, kv_head, row0, wave_row + which, stages, from, to, W::kShift);
+    }
+}
+
+// Joins the parts of a tile that was cut.  Workgroup (cut tile, KV head, every gridDim.z-th 256 fours of dims).
+template <class T>
+__global__ void __launch_bounds__(kThreads) chunk_join_kernel(ChunkArgs a, ChunkPlan plan) {
+    const int* header = reinterpret_cast<const int*>(a.workspace);
+    if (static_cast<int>(blockIdx.x) >= header[0]) return;
+    const int* d = header + kDescription * (1 + blockIdx.x);
+    const int begin = d[0], row0 = d[1], rows = d[2], slot = d[3], parts = d[4];
+    const int kv_head = blockIdx.y, fours = (a.dim + 3) / 4;
+    const int64_t stride = static_cast<int64_t>(plan.slot_rows) * plan.width;
+    for (int item = blockIdx.z * kThreads + threadIdx.x; item < rows * fours; item += gridDim.z * kThreads) {
+        const int r = item / fours, four = item - r * fours;
+        const float* o = part_row(a, plan, kv_head, slot, r);
+        const float* of = o + plan.width - 4;
+        float top = -INFINITY, natural = -INFINITY;
+        for (int p = 0; p < parts; ++p) top = fmaxf(top, of[p * stride]), natural = fmaxf(natural, of[p * stride + 2]);
+        float weight = 0.0f;
+        f32x4 sum = {0, 0, 0, 0};
+        for (int p = 0; p < parts; ++p) {
+            const float part_top = of[p * stride], part_weight = of[p * stride + 1];
+            if (part_weight == 0.0f) continue;  // such a part's sums are zeros, or it saw nothing
+            const bool near = sizeof(T) == 2 && fabsf(top) < kFar && fabsf(part_top) < kFar;
+            const float share = fast_exp2(near ? part_top - top : (of[p * stride + 2] - natural) * kLog2e);
+            weight += part_weight * share;
+            sum += *reinterpret_cast<const f32x4*>(o + p * stride + 4 * four) * share;
+        }
+        const int i = static_cast<int>(divide(row0 + r, a.group_of)), head = kv_head * a.group + row0 + r - i * a.group;
+        T* out = static_cast<T*>(a.out) + (static_cast<int64_t>(begin + i) * a.query_heads + head) * a.dim + 4 * four;
+#pragma unroll
+        for (int l = 0; l < 4; ++l)
+            if (4 * four + l < a.dim) out[l] = static_cast<T>(weight == 0.0f ? 0.0f : sum[l] / weight);
+    }
+}
+
+// Parts of a step: two workgroups on each of 256 CUs.
+constexpr int kTarget = 512;
+
+template <class T>
+ChunkPlan plan_of(const ChunkArgs& a) {
+    const int dim = padded_dim(a.dim);
+    ChunkPlan p{};
+    p.rows = rows_of_tile<T>(dim);
+    const int stage = stage_keys<T>(dim);
+    const int64_t rows = a.tokens * a.group;
+    p.tiles = rows / p.rows + a.requests;
+    if (p.tiles > rows) p.tiles = rows;
+    p.target = (kTarget + a.kv_heads - 1) / a.kv_heads;
+    int64_t stages = (a.keys + stage - 1) / stage;
+    if (a.window > 0) {
+        const int64_t windowed = (static_cast<int64_t>(a.sinks) + stage - 1) / stage + (static_cast<int64_t>(a.window) + p.rows / a.group + 1) / stage + 2;
+        if (windowed < stages) stages = windowed;
+    }
+    p.whole = stages <= kLeastStages;
+    p.units = p.tiles;
+    if (!p.whole) {
+        // A tile of S > each stages has at most S / each + 1 < 2 S / each parts, and the sum of all S is at most target times
+        // each; kLeastStages bounds them as well.
+        const int64_t most = p.tiles * ((stages + kLeastStages - 1) / kLeastStages);
+        p.slots = 2 * static_cast<int64_t>(p.target) < most ? 2 * static_cast<int64_t>(p.target) : most;
+        p.splits = p.target < p.tiles ? p.target : p.tiles;
+        p.units = p.tiles + p.target < most ? p.tiles + p.target : most;
+    }
+    p.slot_rows = rows < p.rows ? static_cast<int>(rows) : p.rows;
+    p.width = (a.dim + 3) / 4 * 4 + 4;
+    return p;
+}
+
+template <class T, int kDim>
+hipError_t launch_tiles(const ChunkArgs& a, const ChunkPlan& plan, dim3 grid, hipStream_t stream) {
+    if constexpr (sizeof(T) == 2) {
+        constexpr int kStage = stage_keys<T>(kDim);
+        constexpr size_t kLds = 2 * (kStage * (kDim * 2 + 16) + kDim * (kStage * 2 + 16));
+        auto launch = [&](auto* kernel) {
+            const hipError_t room = hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize,
+                                                        static_cast<int>(kLds));
+            if (room != hipSuccess) return room;
+            hipLaunchKernelGGL(kernel, grid, dim3(kThreads), kLds, stream, a, plan);
+            return hipGetLastError();
+        };
+        if (a.wide && reinterpret_cast<uintptr_t>(a.out) % 8 == 0) return launch(chunk_tile_kernel<T, kDim, true>);
+        return launch(chunk_tile_kernel<T, kDim, false>);
+    } else {
+        if (a.wide && a.dim == kDim) hipLaunchKernelGGL(HIP_KERNEL_NAME(chunk_register_kernel<kDim, kFullRows>), grid, dim3(kThreads), 0, stream, a, plan);
+        else if (a.wide) hipLaunchKernelGGL(HIP_KERNEL_NAME(chunk_register_kernel<kDim, kWideRows>), grid, dim3(kThreads), 0, stream, a, plan);
+        else hipLaunchKernelGGL(HIP_KERNEL_NAME(chunk_register_kernel<kDim, kNarrow>), grid, dim3(kThreads), 0, stream, a, plan);
+        return hipGetLastError();
+    }
+}
+
+template <class T>
+hipError_t launch_chunks(const ChunkArgs& a, hipStream_t stream) {
+    const ChunkPlan plan = plan_of<T>(a);
+    const int64_t blocks = plan.units * a.kv_heads;
+    if (blocks >= (int64_t{1} << 24)) return hipErrorInvalidValue;  // a grid has below 2^32 threads
+    const dim3 grid(static_cast<uint32_t>(blocks));
+    hipError_t launched;
+    switch (padded_dim(a.dim)) {
+        case 64: launched = launch_tiles<T, 64>(a, plan, grid, stream); break;
+        case 128: launched = launch_tiles<T, 128>(a, plan, grid, stream); break;
+        default: launched = launch_tiles<T, 256>(a, plan, grid, stream);
+    }
+    if (launched != hipSuccess || plan.whole) return launched;
+    const int items = plan.slot_rows * ((a.dim + 3) / 4);
+    const int fold = (items + 4 * kThreads - 1) / (4 * kThreads);
+    hipLaunchKernelGGL(HIP_KERNEL_NAME(chunk_join_kernel<T>), dim3(static_cast<uint32_t>(plan.splits), a.kv_heads, fold), dim3(kThreads), 0,
+                       stream, a, plan);
+    return hipGetLastError();
+}
+
+}  // namespace
+
+size_t chunk_attention_workspace_floats(const ChunkArgs& a, Type type) {
+    const ChunkPlan p = type == Type::kFloat32 ? plan_of<float>(a) : plan_of<__bf16>(a);
+    return p.whole ? 0 : static_cast<size_t>(parts_offset(p) + a.kv_heads * p.slots * p.slot_rows * p.width);
+}
+
+hipError_t launch_chunk_attention(const ChunkArgs& args, Type type, hipStream_t stream) {
+    switch (type) {
+        case Type::kFloat32: return launch_chunks<float>(args, stream);
+        case Type::kFloat16: return launch_chunks<_Float16>(args, stream);
+        default: return launch_chunks<__bf16>(args, stream);
+    }
+}
+
+}  // namespace flux

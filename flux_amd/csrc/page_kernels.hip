@@ -532,10 +532,40 @@ __global__ void __launch_bounds__(256) page_compact_kernel(PagePool p, PageBooks
 // looked up once; every thread requests kAhead units before it writes any.
 constexpr int kWriteTokens = 16;
 
+// The rows of `tokens` tokens, from `sources` (keys, values) to their places: bytes from the pool's start, -1: nowhere.
+template <class Unit>
+__device__ __forceinline__ void move_rows(const PagePool& p, const int64_t (&place)[2][kWriteTokens], int tokens,
+                                          const char* key, const char* value, int64_t key_head, int64_t key_token,
+                                          int64_t value_head, int64_t value_token) {
+    constexpr int kBytes = sizeof(Unit);
+    const uint32_t width = p.row_units.divisor, heads = p.of_heads.divisor;
+    const int side = static_cast<int>(tokens * heads * width);
+    constexpr int kEach = 2 * kAhead;
+    for (int first = threadIdx.x; first < 2 * side; first += kEach * 256) {
+        Unit held[kEach];
+        char* to[kEach];
+#pragma unroll
+        for (int j = 0; j < kEach; ++j) {
+            const int unit = first + 256 * j, s = unit >= side;
+            to[j] = nullptr;
+            if (unit >= 2 * side) continue;
+            const uint32_t at = unit - s * side, row = divide(at, p.row_units), u = at - row * width;
+            const uint32_t t = divide(row, p.of_heads), head = row - t * heads;
+            const int64_t where = place[s][t];
+            if (where < 0) continue;
+            to[j] = (s ? p.value : p.key) + where + head * (s ? p.value_strides : p.key_strides)[2] * p.element + u * kBytes;
+            held[j] = *reinterpret_cast<const Unit*>((s ? value : key) + (head * (s ? value_head : key_head) +
+                                                                          t * (s ? value_token : key_token)) * p.element + u * kBytes);
+        }
+#pragma unroll
+        for (int j = 0; j < kEach; ++j)
+            if (to[j]) store_unit(to[j], held[j]);
+    }
+}
+
 template <class Unit>
 __global__ void __launch_bounds__(256) page_write_kernel(PagePool p, PageWriteArgs a) {
-    constexpr int kBytes = sizeof(Unit);
-    __shared__ int64_t place[2][kWriteTokens];  // bytes from the pool's start, -1: no page
+    __shared__ int64_t place[2][kWriteTokens];
     const int64_t i = blockIdx.y;
     const int64_t slot = a.slot_list[i], start = a.positions[i];
     if (slot < 0 || slot >= a.slots || start < 0) return;
@@ -555,32 +585,91 @@ __global__ void __launch_bounds__(256) page_write_kernel(PagePool p, PageWriteAr
         place[1][threadIdx.x] = held ? (page * p.value_strides[1] + row * p.value_strides[3]) * p.element : -1;
     }
     __syncthreads();
-    const uint32_t width = p.row_units.divisor, heads = p.of_heads.divisor;
-    const int side = static_cast<int>(tokens * heads * width);
-    const char* sources[2] = {a.key + (i * a.key_strides[0] + t0 * a.key_strides[2]) * p.element,
-                              a.value + (i * a.value_strides[0] + t0 * a.value_strides[2]) * p.element};
-    constexpr int kEach = 2 * kAhead;
-    for (int first = threadIdx.x; first < 2 * side; first += kEach * 256) {
-        Unit held[kEach];
-        char* to[kEach];
-#pragma unroll
-        for (int j = 0; j < kEach; ++j) {
-            const int unit = first + 256 * j, s = unit >= side;
-            to[j] = nullptr;
-            if (unit >= 2 * side) continue;
-            const uint32_t at = unit - s * side, row = divide(at, p.row_units), u = at - row * width;
-            const uint32_t t = divide(row, p.of_heads), head = row - t * heads;
-            const int64_t where = place[s][t];
-            if (where < 0) continue;
-            to[j] = (s ? p.value : p.key) + where + head * (s ? p.value_strides : p.key_strides)[2] * p.element + u * kBytes;
-            held[j] = *reinterpret_cast<const Unit*>((s ? sources[1] : sources[0]) +
-                                                     (head * (s ? a.value_strides : a.key_strides)[1] +
-                                                      t * (s ? a.value_strides : a.key_strides)[2]) * p.element + u * kBytes);
-        }
-#pragma unroll
-        for (int j = 0; j < kEach; ++j)
-            if (to[j]) store_unit(to[j], held[j]);
+    move_rows<Unit>(p, place, tokens, a.key + (i * a.key_strides[0] + t0 * a.key_strides[2]) * p.element,
+                    a.value + (i * a.value_strides[0] + t0 * a.value_strides[2]) * p.element, a.key_strides[1],
+                    a.key_strides[2], a.value_strides[1], a.value_strides[2]);
+}
+
+// The same for packed tokens whose rows of the pool are given (row r is row r % page of page r / page).
+template <class Unit>
+__global__ void __launch_bounds__(256) page_write_rows_kernel(PagePool p, PageRowsArgs a) {
+    __shared__ int64_t place[2][kWriteTokens];
+    const int64_t t0 = static_cast<int64_t>(blockIdx.x) * kWriteTokens;
+    const int tokens = static_cast<int>(a.tokens - t0 < kWriteTokens ? a.tokens - t0 : kWriteTokens);
+    if (static_cast<int>(threadIdx.x) < tokens) {
+        const int64_t of = a.rows[t0 + threadIdx.x], page = of / p.page, row = of - page * p.page;
+        const bool held = of >= 0 && page < p.pages;
+        place[0][threadIdx.x] = held ? (page * p.key_strides[1] + row * p.key_strides[3]) * p.element : -1;
+        place[1][threadIdx.x] = held ? (page * p.value_strides[1] + row * p.value_strides[3]) * p.element : -1;
     }
+    __syncthreads();
+    move_rows<Unit>(p, place, tokens, a.key + t0 * a.key_strides[0] * p.element, a.value + t0 * a.value_strides[0] * p.element,
+                    a.key_strides[1], a.key_strides[0], a.value_strides[1], a.value_strides[0]);
+}
+
+// ---------------------------------------------------------------------------
+// Layout.  The tokens of a step lie packed one request after the other, and each workgroup places kPlanThreads of them: it
+// sums the requests' counts itself (all of them up to its own last token; they are a few KB in the L2), so that one launch
+// does.  Sums stop at the number of tokens, which also keeps them in 32 bits.
+__device__ __forceinline__ int saturating_scan(int v, int most) {
+    const int lane = threadIdx.x & 63;
+#pragma unroll
+    for (int step = 1; step < 64; step *= 2) {
+        const int below = __shfl_up(v, step, kWave);
+        if (lane >= step) v = v + below < most ? v + below : most;
+    }
+    return v;
+}
+
+__global__ void __launch_bounds__(kPlanThreads) step_layout_kernel(StepLayoutArgs a) {
+    __shared__ int sums[kPlanWaves];
+    __shared__ int ends[kPlanThreads];
+    const int wave = threadIdx.x >> 6, most = static_cast<int>(a.tokens);
+    const int token = static_cast<int>(blockIdx.x) * kPlanThreads + static_cast<int>(threadIdx.x);
+    const int last = static_cast<int>(blockIdx.x) * kPlanThreads + kPlanThreads - 1;
+    int running = 0, request = -1, first = 0;
+    if (blockIdx.x == 0 && threadIdx.x == 0) a.offsets[0] = 0;
+    for (int base = 0; base < a.requests && (blockIdx.x == 0 || running <= last); base += kPlanThreads) {
+        const int i = base + static_cast<int>(threadIdx.x);
+        int64_t count = 0;
+        if (i < a.requests) {
+            count = a.counts ? a.counts[i] : 1;
+            const int64_t slot = a.slots[i];
+            if (a.positions[i] < 0 || slot < 0 || slot >= a.slot_count || count < 0) count = 0;
+        }
+        int end = saturating_scan(static_cast<int>(count < most ? count : most), most);
+        if ((threadIdx.x & 63) == 63) sums[wave] = end;
+        __syncthreads();
+        int before = running;
+        for (int w = 0; w < wave; ++w) before = before + sums[w] < most ? before + sums[w] : most;
+        end = before + end < most ? before + end : most;
+        ends[threadIdx.x] = end;
+        if (blockIdx.x == 0 && i < a.requests) a.offsets[i + 1] = end;
+        __syncthreads();
+        const int reached = ends[kPlanThreads - 1];
+        if (token >= running && token < reached) {  // the first request that ends behind the token
+            int low = 0;
+#pragma unroll
+            for (int step = kPlanThreads / 2; step >= 1; step /= 2)
+                if (ends[low + step - 1] <= token) low += step;
+            request = base + low;
+            first = low ? ends[low - 1] : running;
+        }
+        running = reached;
+    }
+    if (token >= most) return;
+    int64_t position = -1, row = -1;
+    if (request >= 0) {
+        position = static_cast<int64_t>(static_cast<uint64_t>(a.positions[request]) + static_cast<uint64_t>(token - first));
+        if (position >= 0 && position < a.columns * a.page) {
+            const uint32_t column = static_cast<uint32_t>(position) / static_cast<uint32_t>(a.page);
+            const int64_t page = a.table[a.slots[request] * a.table_stride + column];
+            if (page >= 0) row = page * a.page + (position - column * a.page);
+        }
+    }
+    a.token_requests[token] = request;
+    a.token_positions[token] = position;
+    a.token_rows[token] = row;
 }
 
 bool rows_of(const PagePool& p, int64_t bytes) {
@@ -594,6 +683,13 @@ bool rows_of(const PagePool& p, int64_t bytes) {
 bool rows_of(const PageWriteArgs& a, int element, int64_t bytes) {
     if (reinterpret_cast<uintptr_t>(a.key) % bytes || reinterpret_cast<uintptr_t>(a.value) % bytes) return false;
     for (int i = 0; i < 3; ++i)
+        if (a.key_strides[i] * element % bytes || a.value_strides[i] * element % bytes) return false;
+    return true;
+}
+
+bool rows_of(const PageRowsArgs& a, int element, int64_t bytes) {
+    if (reinterpret_cast<uintptr_t>(a.key) % bytes || reinterpret_cast<uintptr_t>(a.value) % bytes) return false;
+    for (int i = 0; i < 2; ++i)
         if (a.key_strides[i] * element % bytes || a.value_strides[i] * element % bytes) return false;
     return true;
 }
@@ -673,6 +769,18 @@ hipError_t launch_page_write(const PagePool& plain, const PageWriteArgs& args, h
     FLUX_BY_UNIT(pool, page_write_kernel, grid, args);
 }
 
+hipError_t launch_page_write_rows(const PagePool& plain, const PageRowsArgs& args, hipStream_t stream) {
+    const dim3 grid(static_cast<uint32_t>((args.tokens + kWriteTokens - 1) / kWriteTokens));
+    const PagePool pool = with_units(plain, rows_of(plain, 16) && rows_of(args, plain.element, 16));
+    FLUX_BY_UNIT(pool, page_write_rows_kernel, grid, args);
+}
+
 #undef FLUX_BY_UNIT
+
+hipError_t launch_step_layout(const StepLayoutArgs& args, hipStream_t stream) {
+    const dim3 grid(static_cast<uint32_t>((args.tokens + kPlanThreads - 1) / kPlanThreads));
+    hipLaunchKernelGGL(step_layout_kernel, grid, dim3(kPlanThreads), 0, stream, args);
+    return hipGetLastError();
+}
 
 }  // namespace flux

@@ -84,6 +84,43 @@ size_t decode_attention_workspace_floats(const AttentionArgs& args);
 hipError_t launch_decode_attention(const AttentionArgs& args, Type type, hipStream_t stream);
 hipError_t launch_window_attention(const AttentionArgs& args, Type type, hipStream_t stream);
 
+// Packed tokens of several requests over pages: request i has the tokens offsets[i] .. offsets[i + 1].
+struct ChunkArgs {
+    const void* query;  // [tokens, query_heads, dim]
+    const void* key;    // pages
+    const void* value;
+    void* out;  // contiguous [tokens, query_heads, dim]
+    float* workspace;
+    const int32_t* table;    // [slot_count, columns], row stride table_stride
+    const int64_t* lengths;  // [slot_count]
+    const int64_t* offsets;  // [requests + 1]
+    const int64_t* slots;      // [requests]; null: its own index
+    const int64_t* positions;  // of each request's first token; null: length - tokens of the request
+    float scale;
+    int requests;
+    int64_t tokens;
+    int query_heads;
+    int kv_heads;
+    int group;  // query heads per KV head
+    Divider group_of;
+    int dim;
+    int64_t keys;  // positions a table row holds
+    int64_t slot_count;
+    int window;  // 0: no window
+    int sinks;
+    int64_t pages;
+    Divider page;
+    int64_t table_stride;
+    int64_t query_strides[3];  // token, head, dim
+    int64_t key_strides[3];    // page, head, row
+    int64_t value_strides[3];
+    bool wide;        // every key and value row starts at 16 bytes and dim fills whole 16-byte quads
+    bool query_wide;  // the same of query rows, with a dim stride of 1
+};
+
+size_t chunk_attention_workspace_floats(const ChunkArgs& args, Type type);
+hipError_t launch_chunk_attention(const ChunkArgs& args, Type type, hipStream_t stream);
+
 // ---- cache pages ----
 
 // The K and V pages of one or more layers; strides in elements, the head dimension's is 1.
@@ -134,6 +171,32 @@ struct PageWriteArgs {
     const int64_t* counts;  // null: `tokens`
 };
 
+struct PageRowsArgs {
+    const char* key;
+    const char* value;
+    int64_t key_strides[2];  // token, head
+    int64_t value_strides[2];
+    int64_t tokens;
+    const int64_t* rows;  // of the pool
+};
+
+struct StepLayoutArgs {
+    const int32_t* table;
+    int64_t table_stride;
+    int64_t slot_count;
+    int64_t columns;
+    int64_t page;  // rows
+    const int64_t* slots;
+    const int64_t* positions;
+    const int64_t* counts;  // null: 1
+    int requests;
+    int64_t tokens;
+    int64_t* offsets;  // [requests + 1]
+    int64_t* token_requests;
+    int64_t* token_positions;
+    int64_t* token_rows;
+};
+
 // int32 words of scratch memory.
 size_t page_reserve_workspace(int64_t requests, int64_t slots, int64_t pages);
 size_t page_fork_workspace(int64_t requests, int64_t slots, int64_t pages);
@@ -142,6 +205,8 @@ size_t page_compact_workspace(int64_t pages);
 hipError_t launch_page_reserve(const PageBooks& books, const int64_t* slots, const int64_t* counts, int64_t requests,
                                int64_t* positions, int32_t* status, int32_t* workspace, hipStream_t stream);
 hipError_t launch_page_write(const PagePool& pool, const PageWriteArgs& args, hipStream_t stream);
+hipError_t launch_page_write_rows(const PagePool& pool, const PageRowsArgs& args, hipStream_t stream);
+hipError_t launch_step_layout(const StepLayoutArgs& args, hipStream_t stream);
 hipError_t launch_page_copy(const PagePool& pool, const int64_t* source, const int64_t* target, int64_t requests,
                             int32_t* status, hipStream_t stream);
 hipError_t launch_page_free(const PageBooks& books, const int64_t* slots, int64_t requests, int32_t* status,
@@ -174,7 +239,25 @@ struct LogitsArgs {
     void* workspace;
 };
 
+struct SampleArgs {
+    const void* logits;  // [rows, vocab], row stride logits_stride
+    int64_t logits_stride;
+    int64_t rows;
+    int64_t vocab;
+    const float* uniforms;     // [rows]
+    const float* temperature;  // [rows] or null: 1
+    const int64_t* top_k;      // [rows] or null
+    const float* top_p;
+    const float* min_p;
+    int64_t* tokens;       // [rows]
+    float* probabilities;  // [rows]
+    void* workspace;
+};
+
 size_t logits_workspace_bytes(int64_t rows, int64_t vocab);
 hipError_t launch_logits_process(const LogitsArgs& args, Type type, hipStream_t stream);
+
+size_t sample_workspace_bytes(int64_t rows, int64_t vocab);
+hipError_t launch_logits_sample(const SampleArgs& args, Type type, hipStream_t stream);
 
 }  // namespace flux

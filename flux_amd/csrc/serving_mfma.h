@@ -274,4 +274,50 @@ __device__ __forceinline__ void load_query(typename Mfma<T>::Fragment (&query)[k
     }
 }
 
+// ---- 32 x 32 tiles of the 16-bit kernels that stage keys and values ----
+
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+typedef float f32x2 __attribute__((ext_vector_type(2)));
+
+// The weights' place in the type (kShift: powers of two that they are held larger by) and how far a tile's largest score may
+// exceed the running maximum's before the sums are rescaled (kLazy).
+template <class T>
+struct Wide;
+template <>
+struct Wide<__bf16> {
+    static constexpr float kShift = 0.0f, kLazy = 8.0f;
+    typedef __bf16 Pair __attribute__((ext_vector_type(2)));
+    static __device__ __forceinline__ uint32_t round(float a, float b) {
+        return __builtin_bit_cast(uint32_t, __builtin_convertvector((f32x2{a, b}), Pair));
+    }
+    static __device__ __forceinline__ f32x16 multiply(u32x4 a, u32x4 b, f32x16 c) {
+        return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c,
+                                                       0, 0, 0);
+    }
+};
+template <>
+struct Wide<_Float16> {
+    // Weights are held 2^11 times as large, at most 2^15 with kLazy.  Those from 2^-25 of the reference on are normal numbers;
+    // smaller ones are off by at most half of float16's smallest step, 2^-36 of the reference, and the 2^24 keys that a
+    // sequence can have together by 2^-12 of the largest value.
+    static constexpr float kShift = 11.0f, kLazy = 4.0f;
+    typedef _Float16 Pair __attribute__((ext_vector_type(2)));
+    static __device__ __forceinline__ uint32_t round(float a, float b) {
+        return __builtin_bit_cast(uint32_t, __builtin_convertvector((f32x2{a, b}), Pair));
+    }
+    static __device__ __forceinline__ f32x16 multiply(u32x4 a, u32x4 b, f32x16 c) {
+        return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0,
+                                                      0, 0);
+    }
+};
+
+__device__ __forceinline__ float half_max(float v) {
+    const auto both = __builtin_amdgcn_permlane32_swap(__float_as_int(v), __float_as_int(v), false, false);
+    return fmaxf(__int_as_float(both[0]), __int_as_float(both[1]));
+}
+__device__ __forceinline__ float half_sum(float v) {
+    const auto both = __builtin_amdgcn_permlane32_swap(__float_as_int(v), __float_as_int(v), false, false);
+    return __int_as_float(both[0]) + __int_as_float(both[1]);
+}
+
 }  // namespace flux

@@ -346,48 +346,7 @@ __global__ void __launch_bounds__(kThreads, kDim <= 64 ? 4 : (kDim <= 128 ? 2 : 
 // at most half a step of that type relative to themselves, which moves a weighted mean of the values by at most half a step
 // of the largest of them, as the result's own rounding does.  They are summed unrounded in float32.  (Two terms a weight, as
 // in paged_attention.hip, would double the matrix instructions of the product, here where they bound the kernel.)
-typedef float f32x16 __attribute__((ext_vector_type(16)));
-typedef float f32x2 __attribute__((ext_vector_type(2)));
 constexpr int64_t kStagedStride = 1 << 22;
-
-template <class T>
-struct Wide;
-template <>
-struct Wide<__bf16> {
-    static constexpr float kShift = 0.0f, kLazy = 8.0f;
-    typedef __bf16 Pair __attribute__((ext_vector_type(2)));
-    static __device__ __forceinline__ uint32_t round(float a, float b) {
-        return __builtin_bit_cast(uint32_t, __builtin_convertvector((f32x2{a, b}), Pair));
-    }
-    static __device__ __forceinline__ f32x16 multiply(u32x4 a, u32x4 b, f32x16 c) {
-        return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c,
-                                                       0, 0, 0);
-    }
-};
-template <>
-struct Wide<_Float16> {
-    // Weights are held 2^11 times as large, at most 2^15 with kLazy.  Those from 2^-25 of the reference on are normal numbers;
-    // smaller ones are off by at most half of float16's smallest step, 2^-36 of the reference, and the 2^24 keys that a
-    // sequence can have together by 2^-12 of the largest value.
-    static constexpr float kShift = 11.0f, kLazy = 4.0f;
-    typedef _Float16 Pair __attribute__((ext_vector_type(2)));
-    static __device__ __forceinline__ uint32_t round(float a, float b) {
-        return __builtin_bit_cast(uint32_t, __builtin_convertvector((f32x2{a, b}), Pair));
-    }
-    static __device__ __forceinline__ f32x16 multiply(u32x4 a, u32x4 b, f32x16 c) {
-        return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0,
-                                                      0, 0);
-    }
-};
-
-__device__ __forceinline__ float half_max(float v) {
-    const auto both = __builtin_amdgcn_permlane32_swap(__float_as_int(v), __float_as_int(v), false, false);
-    return fmaxf(__int_as_float(both[0]), __int_as_float(both[1]));
-}
-__device__ __forceinline__ float half_sum(float v) {
-    const auto both = __builtin_amdgcn_permlane32_swap(__float_as_int(v), __float_as_int(v), false, false);
-    return __int_as_float(both[0]) + __int_as_float(both[1]);
-}
 
 // Rows of one stage.  With kWide 16 bytes at a byte offset through a buffer that ends with the last row (kStagedStride
 // keeps offsets in 31 bits); else eight elements, of the last row where there is none.

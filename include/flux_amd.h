@@ -478,6 +478,24 @@ int flux_paged_decode_attention(int dtype, const void* query, const void* key_pa
                                 int64_t window, int64_t sinks, const int64_t* query_strides,
                                 const int64_t* key_strides, const int64_t* value_strides, hipStream_t stream);
 
+/* The packed tokens of a step over a paged cache: chunks of prompts next to single tokens.  Request i has the rows
+ * offsets[i] .. offsets[i + 1] (offsets [requests + 1] do not decrease) of query [tokens, query_heads, head_dim] and uses
+ * row r = slots[i] (i when slots is NULL) of page_table and lengths, as above.  Its first token is at positions[i]
+ * (NULL: lengths[r] less its tokens), the others behind it; a token at p sees the keys j <= p, j < lengths[r] with
+ * j > p - window or j < sinks (window 0: all).  Keys on a page outside [0, pages) are left out and never read.  A token
+ * that sees nothing, nothing whose score is above -inf, with p outside [0, lengths[r]), or of no request gives zeros.
+ * Strides: query's token, head, dim; pages' page, head, row.  output contiguous. */
+int flux_paged_chunk_attention_workspace_bytes(int dtype, int64_t tokens, int64_t requests, int64_t query_heads, int64_t kv_heads,
+                                               int64_t head_dim, int64_t page_size, int64_t columns, int64_t window,
+                                               int64_t sinks, int64_t* bytes);
+int flux_paged_chunk_attention(int dtype, const void* query, const void* key_pages, const void* value_pages,
+                               const int32_t* page_table, const int64_t* lengths, const int64_t* offsets, const int64_t* slots,
+                               const int64_t* positions, void* output, void* workspace, int64_t workspace_bytes, float scale,
+                               int64_t tokens, int64_t requests, int64_t query_heads, int64_t kv_heads, int64_t head_dim,
+                               int64_t pages, int64_t page_size, int64_t slot_count, int64_t columns, int64_t table_stride,
+                               int64_t window, int64_t sinks, const int64_t* query_strides, const int64_t* key_strides,
+                               const int64_t* value_strides, hipStream_t stream);
+
 /* Causal attention with a sliding window and sinks over key, value [batch, kv_heads, keys, head_dim].  The query i of
  * sequence b has position p = starts[b] + i (NULL: lengths[b] - queries + i) and sees the keys j <= p, j < lengths[b]
  * (NULL: keys; clamped to keys) with j > p - window or j < sinks (window 0: all); a row that sees nothing,
@@ -546,6 +564,20 @@ int flux_page_write(const flux_page_pool* pool, const void* key, const void* val
                     const int64_t* value_strides, int64_t requests, int64_t tokens, const int32_t* page_table,
                     int64_t table_stride, int64_t slots, int64_t columns, const int64_t* slot_list,
                     const int64_t* positions, const int64_t* counts, hipStream_t stream);
+/* The same for packed tokens whose places are known: key, value [tokens, heads, head_dim] (strides of token and head) to
+ * rows[t] of the pool, row r being row r % page_size of page r / page_size; rows outside the pool are left out.  Two tokens
+ * must not name the same row, and key and value must not share memory with the rows that are written. */
+int flux_page_write_rows(const flux_page_pool* pool, const void* key, const void* value, const int64_t* key_strides,
+                         const int64_t* value_strides, int64_t tokens, const int64_t* rows, hipStream_t stream);
+/* Places of the packed tokens of a step, one request after the other.  Request i has counts[i] (NULL: 1) tokens from
+ * positions[i] on of slots[i], none where the position or count is negative (a refused reservation) or the slot outside
+ * page_table [slot_count, columns].  offsets [requests + 1]: its tokens are offsets[i] .. offsets[i + 1], cut at `tokens`.
+ * Token t: its request, its position, and its row of the pool for flux_page_write_rows (-1: beyond the columns or on no
+ * page); all three -1 behind the last one. */
+int flux_step_layout(const int32_t* page_table, int64_t table_stride, int64_t slot_count, int64_t columns, int64_t page_size,
+                     const int64_t* slots, const int64_t* positions, const int64_t* counts, int64_t requests, int64_t tokens,
+                     int64_t* offsets, int64_t* token_requests, int64_t* token_positions, int64_t* token_rows,
+                     hipStream_t stream);
 /* Page source[i] to page target[i], all layers. */
 int flux_page_copy(const flux_page_pool* pool, const int64_t* source, const int64_t* target, int64_t requests,
                    int32_t* status, hipStream_t stream);
@@ -578,6 +610,21 @@ int flux_logits_process(int dtype, const void* logits, int64_t logits_stride, vo
                         const float* frequency, const float* presence, const float* bias, int64_t bias_stride,
                         const int32_t* allowed, int64_t allowed_stride, void* workspace, int64_t workspace_bytes,
                         hipStream_t stream);
+
+/* The next token of each row of logits [rows, vocab] by uniforms [rows], u within [0, 1).  With m the row's largest logit and
+ * t its temperature, w_v = exp((x_v - m) / t), in the order (x descending, index ascending):
+ *   top_k: the first k tokens (k <= 0 or >= vocab: all);
+ *   top_p: of those, a token while the weights before it are below p times theirs, the first always (p >= 1 or NaN: all);
+ *   min_p: of those, tokens with w >= min(min_p, 1) (min_p <= 0 or NaN: all).
+ * tokens[row]: the first one kept, by index, at which the kept weights reached exceed u times all of them (u <= 0 or NaN: the
+ * first of any weight, u >= 1: the last); probabilities[row]: its share of them.  A row whose temperature is not above 0 or whose
+ * largest logit is not finite gives the lowest index of the largest logit (NaN above all numbers) and 1.  Vectors [rows];
+ * NULL: temperature 1, no filter.  Weights are held in integers of 2^-b, b = min(51, 62 - ceil(log2 vocab)): results
+ * do not depend on scheduling. */
+int flux_logits_sample_workspace_bytes(int64_t rows, int64_t vocab, int64_t* bytes);
+int flux_logits_sample(int dtype, const void* logits, int64_t logits_stride, const float* uniforms, const float* temperature,
+                       const int64_t* top_k, const float* top_p, const float* min_p, int64_t* tokens, float* probabilities,
+                       int64_t rows, int64_t vocab, void* workspace, int64_t workspace_bytes, hipStream_t stream);
 
 #ifdef __cplusplus
 }
