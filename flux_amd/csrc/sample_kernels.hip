@@ -5,17 +5,19 @@
 //   min-p: w >= min(min_p, 1).  The token is the first one, by index, at which the kept mass reached exceeds u times all of it.
 //   t not above 0, or m not finite: the lowest index of the largest logit (NaN above all numbers).
 //
-// Weights are integers, 2^kBits exp(..) rounded, so that sums do not depend on their order: a histogram's atomics and any
+// Weights are integers, 2^bits exp(..) rounded, so that sums do not depend on their order: a histogram's atomics and any
 // split of the row give the same token.  With 62 - log2(vocab) bits (45 at 128000 tokens) a sum of all of them is exact in
 // 64 bits, and each is off by half of 2^-45: borders between tokens move by less than 1e-11 of the mass.
+//
+// A row is split over workgroups and takes four launches: the largest logit; weights, their sums by workgroup and a
+// histogram of counts and masses over 1/32 steps of log2 w; the mass of all tokens in steps above those where top-k or top-p end,
+// and a list of the tokens in these; the end's place in that list, the workgroup's part in which the number lies, and the
+// token in it.  Short rows, and rows whose list is too long (thousands of equal logits at the end), are one workgroup's,
+// which finds the end digit by digit of the logits' bits.
 #include "serving.h"
 
 namespace flux {
 namespace {
-
-constexpr int kThreads = 1024;
-constexpr int kWaves = kThreads / kWave;
-constexpr int kBins = 2048;
 
 // Larger values have larger keys, NaN the largest; zeros of both signs have one.
 __device__ __forceinline__ uint32_t key_of(float value) {
@@ -25,217 +27,716 @@ __device__ __forceinline__ uint32_t key_of(float value) {
 __device__ __forceinline__ float value_of(uint32_t key) {
     return __uint_as_float(key & 0x80000000u ? key ^ 0x80000000u : ~key);
 }
+// A token's place in the order, the first ones largest; never 0.
+__device__ __forceinline__ uint64_t rank_of(float value, uint32_t index) {
+    return static_cast<uint64_t>(key_of(value)) << 32 | ~index;
+}
 
-// 2^bits exp2((x - top) rate), rounded; rate = log2(e) / temperature.  2^f for |f| <= 1/2 by its Taylor series: the first
-// term left out, (ln 2 / 2)^13 / 13!, is below 2^-52.
+// 2^(-j / 32).
+__constant__ double kRoots[32] = {
+    0x1.0000000000000p+0, 0x1.f50765b6e4540p-1, 0x1.ea4afa2a490dap-1, 0x1.dfc97337b9b5fp-1,
+    0x1.d5818dcfba487p-1, 0x1.cb720dcef9069p-1, 0x1.c199bdd85529cp-1, 0x1.b7f76f2fb5e47p-1,
+    0x1.ae89f995ad3adp-1, 0x1.a5503b23e255dp-1, 0x1.9c49182a3f090p-1, 0x1.93737b0cdc5e5p-1,
+    0x1.8ace5422aa0dbp-1, 0x1.82589994cce13p-1, 0x1.7a11473eb0187p-1, 0x1.71f75e8ec5f74p-1,
+    0x1.6a09e667f3bcdp-1, 0x1.6247eb03a5585p-1, 0x1.5ab07dd485429p-1, 0x1.5342b569d4f82p-1,
+    0x1.4bfdad5362a27p-1, 0x1.44e086061892dp-1, 0x1.3dea64c123422p-1, 0x1.371a7373aa9cbp-1,
+    0x1.306fe0a31b715p-1, 0x1.29e9df51fdee1p-1, 0x1.2387a6e756238p-1, 0x1.1d4873168b9aap-1,
+    0x1.172b83c7d517bp-1, 0x1.11301d0125b51p-1, 0x1.0b5586cf9890fp-1, 0x1.059b0d3158574p-1};
+
+// 2^bits exp((x - top) / t), rounded.  In steps of 1/32 below the largest logit, -(x - top) / t log2(e) = (step - f) / 32 with
+// |f| <= 1/2: 2^(-step / 32) from a table of 32 (one for each bank pair of the LDS: no conflicts) and 2^(f / 32) by its
+// Taylor series, whose first term left out, (ln 2 / 64)^6 / 6!, is 2^-48.7.
 struct Weigher {
-    double top, rate;
+    const double* roots;  // in LDS
+    double top, rate;     // rate: 32 log2(e) / t
     int bits;
 
-    __device__ __forceinline__ double exponent(float x) const { return (static_cast<double>(x) - top) * rate; }
-    __device__ __forceinline__ double power(double y) const {
+    // The step, and f; a step beyond those that weigh anything, also for NaN (an infinite temperature's -inf).
+    __device__ __forceinline__ int step_of(float x, double& f) const {
+        const double y = (static_cast<double>(x) - top) * rate;
+        if (!(y >= -32.0 * (bits + 1))) return 1 << 20;
         const double n = __builtin_rint(y);
-        const double f = (y - n) * 0.69314718055994530942;
-        double p = 1.0 / 479001600.0;
-        p = fma(p, f, 1.0 / 39916800.0);
-        p = fma(p, f, 1.0 / 3628800.0);
-        p = fma(p, f, 1.0 / 362880.0);
-        p = fma(p, f, 1.0 / 40320.0);
-        p = fma(p, f, 1.0 / 5040.0);
-        p = fma(p, f, 1.0 / 720.0);
-        p = fma(p, f, 1.0 / 120.0);
-        p = fma(p, f, 1.0 / 24.0);
-        p = fma(p, f, 1.0 / 6.0);
-        p = fma(p, f, 0.5);
-        p = fma(p, f, 1.0);
-        p = fma(p, f, 1.0);
-        return __builtin_amdgcn_ldexp(p, static_cast<int>(n) + bits);
+        f = y - n;
+        return -static_cast<int>(n);
     }
-    // An integer below 2^52 by the addition of 2^52; NaN (an infinite temperature's -inf) weighs nothing.
+    __device__ __forceinline__ double power(int step, double f) const {
+        double p = 0x1.5d87fe78a6731p-35;
+        p = fma(p, f, 0x1.3b2ab6fba4e77p-27);
+        p = fma(p, f, 0x1.c6b08d704a0c0p-20);
+        p = fma(p, f, 0x1.ebfbdff82c58fp-13);
+        p = fma(p, f, 0x1.62e42fefa39efp-6);
+        p = fma(p, f, 1.0);
+        return __builtin_amdgcn_ldexp(p * roots[step & 31], bits - (step >> 5));
+    }
+    // An integer below 2^52 by the addition of 2^52.
+    __device__ __forceinline__ uint64_t weight(int step, double f) const {
+        return __double_as_longlong(power(step, f) + 0x1p52) - __double_as_longlong(0x1p52);
+    }
     __device__ __forceinline__ uint64_t operator()(float x) const {
-        const double y = exponent(x);
-        if (!(y >= -(bits + 1))) return 0;
-        return __double_as_longlong(power(y) + 0x1p52) - __double_as_longlong(0x1p52);
+        double f;
+        const int step = step_of(x, f);
+        return step < 1 << 20 ? weight(step, f) : 0;
     }
 };
 
-struct Shared {
-    unsigned long long mass[kBins];
-    uint32_t count[kBins];
-    unsigned long long sums[kWaves];
-    unsigned long long word, above;
-    uint32_t index;
-};
-
-__device__ __forceinline__ uint64_t shuffle_up(uint64_t v, int by) {
-    return static_cast<uint64_t>(__shfl_up(static_cast<unsigned long long>(v), by, kWave));
+template <int kThreads>
+__device__ __forceinline__ uint64_t block_best(uint64_t v, unsigned long long* words) {
+#pragma unroll
+    for (int step = 1; step < 64; step *= 2) {
+        const uint64_t other = __shfl_xor(static_cast<unsigned long long>(v), step, kWave);
+        v = other > v ? other : v;
+    }
+    __syncthreads();
+    if ((threadIdx.x & 63) == 0) words[threadIdx.x >> 6] = v;
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < kThreads / kWave; ++w) v = words[w] > v ? words[w] : v;
+    return v;
 }
 
 // Inclusive prefix sums over the workgroup's threads, and the total.
-__device__ uint64_t block_scan(uint64_t v, unsigned long long* sums, uint64_t* total) {
+template <int kThreads>
+__device__ __forceinline__ uint64_t block_scan(uint64_t v, unsigned long long* words, uint64_t* total) {
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
 #pragma unroll
     for (int step = 1; step < 64; step *= 2) {
-        const uint64_t below = shuffle_up(v, step);
+        const uint64_t below = __shfl_up(static_cast<unsigned long long>(v), step, kWave);
         if (lane >= step) v += below;
     }
     __syncthreads();
-    if (lane == 63) sums[wave] = v;
+    if (lane == 63) words[wave] = v;
     __syncthreads();
     uint64_t all = 0;
-    for (int w = 0; w < kWaves; ++w) {
-        if (w < wave) v += sums[w];
-        all += sums[w];
+#pragma unroll
+    for (int w = 0; w < kThreads / kWave; ++w) {
+        if (w < wave) v += words[w];
+        all += words[w];
     }
     *total = all;
     return v;
 }
 
-// The end of the kept tokens in the order: those with keys above `key`, and the first `ties` of those with it.
-struct End {
-    uint32_t key;
-    uint32_t ties;
-    uint64_t mass;  // of all kept
+// What a row asks for.
+struct RowOptions {
+    uint32_t greedy;
+    bool draws;        // not greedy
+    int64_t k;         // vocab: all
+    float p;           // 1: all
+    uint64_t least;    // weight that min-p asks for
+    double rate, top;
 };
 
-// The token where the count reaches `limit` (kCount) or the mass does: eleven, eleven and ten bits of its key in turn.
-template <bool kCount, class T>
-__device__ End find_end(const T* row, int64_t vocab, const Weigher& weigh, uint64_t limit, Shared& s) {
+__device__ __forceinline__ RowOptions options_of(const SampleArgs& a, int64_t row, int bits, uint64_t best) {
+    RowOptions o;
+    o.greedy = ~static_cast<uint32_t>(best);
+    const float top = value_of(static_cast<uint32_t>(best >> 32));
+    const float temperature = a.temperature ? a.temperature[row] : 1.0f;
+    o.draws = temperature > 0.0f && fabsf(top) < INFINITY;
+    const int64_t k = a.top_k ? a.top_k[row] : 0;
+    o.k = k > 0 && k < a.vocab ? k : a.vocab;
+    const float p = a.top_p ? a.top_p[row] : 1.0f;
+    o.p = p < 1.0f ? (p > 0.0f ? p : 0.0f) : 1.0f;
+    const float least = a.min_p ? a.min_p[row] : 0.0f;
+    o.least = least > 0.0f ? static_cast<uint64_t>(ceil(ldexp(static_cast<double>(least < 1.0f ? least : 1.0f), bits))) : 0;
+    o.top = top;
+    o.rate = 32.0 * 1.44269504088896340736 / static_cast<double>(temperature);
+    return o;
+}
+
+// The mass before which a token is kept by top-p, at least 1: the first always is.
+__device__ __forceinline__ uint64_t mass_limit(float p, uint64_t all) {
+    const double mass = ceil(static_cast<double>(p) * static_cast<double>(all));
+    return mass >= 1.0 ? static_cast<uint64_t>(mass) : 1;
+}
+// The mass that the token has to exceed.
+__device__ __forceinline__ uint64_t drawn_mass(float uniform, uint64_t all) {
+    const double wanted = uniform > 0.0f ? static_cast<double>(uniform) * static_cast<double>(all) : 0.0;
+    return wanted < static_cast<double>(all - 1) ? static_cast<uint64_t>(wanted) : all - 1;
+}
+
+// Logits that a thread reads at once.
+template <class T>
+struct Unit {
+    static constexpr int kWidth = 16 / sizeof(T);
+    T value[kWidth];
+    // Those from `v` on, -inf from `end` on.
+    __device__ __forceinline__ void load(const T* row, int64_t v, int64_t end, bool wide) {
+        if (wide && v + kWidth <= end) {
+            const uint4 quad = *reinterpret_cast<const uint4*>(row + v);
+            __builtin_memcpy(value, &quad, 16);
+        } else {
+#pragma unroll
+            for (int j = 0; j < kWidth; ++j) value[j] = v + j < end ? row[v + j] : static_cast<T>(-INFINITY);
+        }
+    }
+    __device__ __forceinline__ float operator[](int j) const { return static_cast<float>(value[j]); }
+};
+
+// The token of the part [from, to) of a row at which the kept mass, `before` in front of the part, exceeds `target`; kept are
+// tokens ranked `end` or higher that weigh `least` or more.
+template <class T, int kThreads>
+__device__ void draw_in(const SampleArgs& a, int64_t row, const T* in, bool wide, int64_t from, int64_t to, const Weigher& weigh,
+                        uint64_t end, uint64_t least, uint64_t before, uint64_t target, uint64_t all, unsigned long long* words) {
+    using U = Unit<T>;
+    uint64_t running = before;
+    for (int64_t base = from; base < to; base += kThreads * U::kWidth) {
+        const int64_t v = base + U::kWidth * static_cast<int>(threadIdx.x);
+        U unit;
+        unit.load(in, v, to, wide);
+        uint64_t w[U::kWidth], sum = 0;
+#pragma unroll
+        for (int j = 0; j < U::kWidth; ++j) {
+            w[j] = v + j < to && rank_of(unit[j], static_cast<uint32_t>(v + j)) >= end ? weigh(unit[j]) : 0;
+            if (w[j] < least) w[j] = 0;
+            sum += w[j];
+        }
+        uint64_t total;
+        uint64_t reached = running + block_scan<kThreads>(sum, words, &total) - sum;
+#pragma unroll
+        for (int j = 0; j < U::kWidth; ++j) {
+            if (w[j] && reached <= target && reached + w[j] > target) {
+                double f;
+                const int step = weigh.step_of(unit[j], f);
+                a.tokens[row] = v + j;
+                a.probabilities[row] = static_cast<float>(weigh.power(step, f) / static_cast<double>(all));
+            }
+            reached += w[j];
+        }
+        running += total;
+        if (running > target) return;
+    }
+}
+
+// ---------------------------------------------------------------------------
+// One workgroup a row.
+constexpr int kRowThreads = 1024;
+constexpr int kDigitBins = 2048;
+
+struct DigitShared {
+    unsigned long long mass[kDigitBins];
+    uint32_t count[kDigitBins];
+    unsigned long long words[kRowThreads / kWave];
+    unsigned long long word, above;
+    uint32_t index;
+    double roots[32];
+};
+
+// The last token kept, where the count reaches `limit` (kCount) or the mass does: eleven, eleven and ten bits of the keys in
+// turn, then the equal logits by index.  `mass`: of all kept.
+template <bool kCount, class T, int kThreads>
+__device__ uint64_t find_end(const T* row, int64_t vocab, bool wide, const Weigher& weigh, uint64_t limit, DigitShared& s, uint64_t* mass) {
+    using U = Unit<T>;
     uint32_t prefix = 0;
-    uint64_t above_count = 0, above_mass = 0;
-    uint64_t last_count = 0, last_mass = 0;
+    uint64_t above_count = 0, above_mass = 0, last_count = 0, last_mass = 0;
     for (int digit = 0; digit < 3; ++digit) {
         const int shift = digit == 0 ? 21 : (digit == 1 ? 10 : 0), bins = digit == 2 ? 1024 : 2048;
         const int fixed = digit == 0 ? 32 : (digit == 1 ? 21 : 10);
         __syncthreads();
-        for (int b = threadIdx.x; b < kBins; b += kThreads) s.mass[b] = 0, s.count[b] = 0;
+        for (int b = threadIdx.x; b < kDigitBins; b += kThreads) s.mass[b] = 0, s.count[b] = 0;
         __syncthreads();
-        for (int64_t v = threadIdx.x; v < vocab; v += kThreads) {
-            const float x = static_cast<float>(row[v]);
-            const uint32_t key = key_of(x);
-            if (fixed < 32 && (key ^ prefix) >> fixed) continue;
-            const uint32_t bin = key >> shift & (bins - 1);
-            atomicAdd(s.count + bin, 1u);
-            const uint64_t w = weigh(x);
-            if (w) atomicAdd(s.mass + bin, static_cast<unsigned long long>(w));
+        for (int64_t v = U::kWidth * static_cast<int>(threadIdx.x); v < vocab; v += U::kWidth * kThreads) {
+            U unit;
+            unit.load(row, v, vocab, wide);
+#pragma unroll
+            for (int j = 0; j < U::kWidth; ++j) {
+                const uint32_t key = key_of(unit[j]);
+                if (v + j >= vocab || (fixed < 32 && (key ^ prefix) >> fixed)) continue;
+                const uint32_t bin = key >> shift & (bins - 1);
+                atomicAdd(s.count + bin, 1u);
+                const uint64_t w = weigh(unit[j]);
+                if (w) atomicAdd(s.mass + bin, static_cast<unsigned long long>(w));
+            }
         }
         __syncthreads();
-        // Thread t looks at the bins from the highest on: 2 t and 2 t + 1 below it.
-        const int high = bins - 1 - 2 * static_cast<int>(threadIdx.x), low = high - 1;
-        const bool mine = high >= 0;
-        const uint64_t c0 = mine ? s.count[high] : 0, c1 = mine && low >= 0 ? s.count[low] : 0;
-        const uint64_t m0 = mine ? s.mass[high] : 0, m1 = mine && low >= 0 ? s.mass[low] : 0;
+        // Each thread looks at some bins, the first one at the highest.
+        constexpr int kEach = kDigitBins / kThreads;
+        const int high = bins - 1 - kEach * static_cast<int>(threadIdx.x);
+        uint64_t counts = 0, masses = 0;
+        for (int j = 0; j < kEach && high - j >= 0; ++j) counts += s.count[high - j], masses += s.mass[high - j];
         uint64_t total;
-        const uint64_t counts = above_count + block_scan(c0 + c1, s.sums, &total);
-        const uint64_t masses = above_mass + block_scan(m0 + m1, s.sums, &total);
-        const uint64_t reached = kCount ? counts : masses, added = kCount ? c0 + c1 : m0 + m1, first = kCount ? c0 : m0;
-        if (reached >= limit && reached - added < limit) {
-            s.index = reached - added + first >= limit ? high : low;
-            s.word = masses - m0 - m1;
-            s.above = counts - c0 - c1;
+        uint64_t count_before = above_count + block_scan<kThreads>(counts, s.words, &total) - counts;
+        uint64_t mass_before = above_mass + block_scan<kThreads>(masses, s.words, &total) - masses;
+        for (int j = 0; j < kEach && high - j >= 0; ++j) {
+            const uint64_t c = s.count[high - j], m = s.mass[high - j];
+            const uint64_t reached = kCount ? count_before : mass_before, added = kCount ? c : m;
+            if (reached < limit && reached + added >= limit) {
+                s.index = high - j;
+                s.word = mass_before;
+                s.above = count_before;
+            }
+            count_before += c;
+            mass_before += m;
         }
         __syncthreads();
         const int bin = s.index;
         above_mass = s.word;
         above_count = s.above;
-        const int of = bins - 1 - bin;
-        if (of & 1) above_mass += s.mass[bin + 1], above_count += s.count[bin + 1];
         last_count = s.count[bin];
         last_mass = s.mass[bin];
         prefix |= static_cast<uint32_t>(bin) << shift;
     }
+    const uint64_t each = last_mass / last_count;  // they are equal
+    const uint64_t ties = kCount ? limit - above_count : (limit - 1 - above_mass) / each + 1;
+    *mass = above_mass + each * ties;
+    if (ties >= last_count) return static_cast<uint64_t>(prefix) << 32;
+    uint64_t found = 0;  // the index of the last of the equal ones that is kept
+    for (int64_t base = 0; base < vocab && found < ties; base += U::kWidth * kThreads) {
+        const int64_t v = base + U::kWidth * static_cast<int>(threadIdx.x);
+        U unit;
+        unit.load(row, v, vocab, wide);
+        uint64_t mine = 0;
+#pragma unroll
+        for (int j = 0; j < U::kWidth; ++j) mine += v + j < vocab && key_of(unit[j]) == prefix;
+        uint64_t total;
+        uint64_t before = found + block_scan<kThreads>(mine, s.words, &total) - mine;
+#pragma unroll
+        for (int j = 0; j < U::kWidth; ++j)
+            if (v + j < vocab && key_of(unit[j]) == prefix && ++before == ties) s.index = static_cast<uint32_t>(v + j);
+        found += total;
+    }
     __syncthreads();
-    End end;
-    end.key = prefix;
-    const uint64_t each = last_count ? last_mass / last_count : 0;  // they are equal
-    end.ties = static_cast<uint32_t>(kCount ? limit - above_count : (limit - 1 - above_mass) / each + 1);
-    end.mass = above_mass + each * end.ties;
-    return end;
+    return static_cast<uint64_t>(prefix) << 32 | ~s.index;
+}
+
+template <class T, int kThreads>
+__device__ void sample_row(const SampleArgs& a, int64_t row, const RowOptions& o, int bits, bool wide, DigitShared& s) {
+    using U = Unit<T>;
+    const T* in = static_cast<const T*>(a.logits) + row * a.logits_stride;
+    const Weigher weigh{s.roots, o.top, o.rate, bits};
+    uint64_t end = 0, mass = 0;
+    if (o.k < a.vocab) end = find_end<true, T, kThreads>(in, a.vocab, wide, weigh, o.k, s, &mass);
+    if (mass == 0) {
+        uint64_t sum = 0;
+        for (int64_t v = U::kWidth * static_cast<int>(threadIdx.x); v < a.vocab; v += U::kWidth * kThreads) {
+            U unit;
+            unit.load(in, v, a.vocab, wide);
+#pragma unroll
+            for (int j = 0; j < U::kWidth; ++j) sum += weigh(unit[j]);
+        }
+        block_scan<kThreads>(sum, s.words, &mass);
+    }
+    if (o.p < 1.0f) end = find_end<false, T, kThreads>(in, a.vocab, wide, weigh, mass_limit(o.p, mass), s, &mass);
+    if (o.least > 0) {
+        uint64_t sum = 0;
+        for (int64_t v = U::kWidth * static_cast<int>(threadIdx.x); v < a.vocab; v += U::kWidth * kThreads) {
+            U unit;
+            unit.load(in, v, a.vocab, wide);
+#pragma unroll
+            for (int j = 0; j < U::kWidth; ++j) {
+                const uint64_t w = rank_of(unit[j], static_cast<uint32_t>(v + j)) >= end && v + j < a.vocab ? weigh(unit[j]) : 0;
+                sum += w < o.least ? 0 : w;
+            }
+        }
+        block_scan<kThreads>(sum, s.words, &mass);
+    }
+    draw_in<T, kThreads>(a, row, in, wide, 0, a.vocab, weigh, end, o.least, 0, drawn_mass(a.uniforms[row], mass), mass, s.words);
 }
 
 template <class T>
-__global__ void __launch_bounds__(kThreads) sample_row_kernel(SampleArgs a, int bits) {
-    __shared__ Shared s;
+__global__ void __launch_bounds__(kRowThreads) sample_row_kernel(SampleArgs a, int bits, bool wide) {
+    using U = Unit<T>;
+    __shared__ DigitShared s;
     const int64_t row = blockIdx.x;
     const T* in = static_cast<const T*>(a.logits) + row * a.logits_stride;
-    // The largest logit and its lowest index.
+    if (threadIdx.x < 32) s.roots[threadIdx.x] = kRoots[threadIdx.x];
     uint64_t best = 0;
-    for (int64_t v = threadIdx.x; v < a.vocab; v += kThreads) {
-        const uint64_t rank = static_cast<uint64_t>(key_of(static_cast<float>(in[v]))) << 32 | ~static_cast<uint32_t>(v);
-        best = rank > best ? rank : best;
+    for (int64_t v = U::kWidth * static_cast<int>(threadIdx.x); v < a.vocab; v += U::kWidth * kRowThreads) {
+        U unit;
+        unit.load(in, v, a.vocab, wide);
+#pragma unroll
+        for (int j = 0; j < U::kWidth; ++j) {
+            const uint64_t rank = rank_of(unit[j], static_cast<uint32_t>(v + j));
+            best = v + j < a.vocab && rank > best ? rank : best;
+        }
     }
-    if (threadIdx.x == 0) s.word = 0;
-    __syncthreads();
-    atomicMax(&s.word, static_cast<unsigned long long>(best));
-    __syncthreads();
-    best = s.word;
-    const uint32_t greedy = ~static_cast<uint32_t>(best);
-    const float top = static_cast<float>(in[greedy]);
-    const float temperature = a.temperature ? a.temperature[row] : 1.0f;
-    if (!(temperature > 0.0f) || !(fabsf(top) < INFINITY)) {
-        if (threadIdx.x == 0) a.tokens[row] = greedy, a.probabilities[row] = 1.0f;
+    best = block_best<kRowThreads>(best, s.words);
+    const RowOptions o = options_of(a, row, bits, best);
+    if (!o.draws) {
+        if (threadIdx.x == 0) a.tokens[row] = o.greedy, a.probabilities[row] = 1.0f;
         return;
     }
-    const Weigher weigh{static_cast<double>(top), 1.44269504088896340736 / static_cast<double>(temperature), bits};
-    End end{0, ~0u, 0};
-    const int64_t k = a.top_k ? a.top_k[row] : 0;
-    const float p = a.top_p ? a.top_p[row] : 1.0f, least = a.min_p ? a.min_p[row] : 0.0f;
-    if (k > 0 && k < a.vocab) end = find_end<true, T>(in, a.vocab, weigh, k, s);
-    if (p < 1.0f) {
-        if (end.mass == 0) {
-            uint64_t sum = 0;
-            for (int64_t v = threadIdx.x; v < a.vocab; v += kThreads) sum += weigh(static_cast<float>(in[v]));
-            block_scan(sum, s.sums, &end.mass);
-        }
-        const double mass = ceil(static_cast<double>(p) * static_cast<double>(end.mass));
-        end = find_end<false, T>(in, a.vocab, weigh, mass >= 1.0 ? static_cast<uint64_t>(mass) : 1, s);
-    }
-    const uint64_t floor_mass =
-        least > 0.0f ? static_cast<uint64_t>(ceil(ldexp(static_cast<double>(least < 1.0f ? least : 1.0f), bits))) : 0;
+    sample_row<T, kRowThreads>(a, row, o, bits, wide, s);
+}
 
-    // Twice over the row by index: the kept mass, then the place where it is reached.
-    uint64_t target = 0, all = 0;
-    for (int pass = 0; pass < 2; ++pass) {
-        uint64_t running = 0, ties = 0;
-        for (int64_t base = 0; base < a.vocab; base += kThreads) {
-            const int64_t v = base + threadIdx.x;
-            const float x = v < a.vocab ? static_cast<float>(in[v]) : -INFINITY;
-            const uint32_t key = v < a.vocab ? key_of(x) : 0;
-            const bool tie = v < a.vocab && key == end.key;
-            uint64_t of_block;
-            const uint64_t rank = ties + block_scan(tie, s.sums, &of_block);
-            ties += of_block;
-            uint64_t w = v < a.vocab && (key > end.key || (tie && rank <= end.ties)) ? weigh(x) : 0;
-            if (w < floor_mass) w = 0;
-            const uint64_t reached = running + block_scan(w, s.sums, &of_block);
-            if (pass == 1 && w && reached > target && reached - w <= target) {
-                a.tokens[row] = v;
-                a.probabilities[row] = static_cast<float>(weigh.power(weigh.exponent(x)) / static_cast<double>(all));
-            }
-            running += of_block;
-            if (pass == 1 && running > target) return;
+// ---------------------------------------------------------------------------
+// Several workgroups a row.
+constexpr int kThreads = 512;
+constexpr int kWaves = kThreads / kWave;
+constexpr int kSteps = 1600;  // of weights that are not 0: 32 (bits + 1), at most 48 bits
+constexpr int kList = 1024;   // tokens in the steps where top-k and top-p end
+constexpr int kMostParts = 64;
+
+struct SampleSplit {
+    int parts;      // of a row
+    int64_t part;   // tokens
+    unsigned long long* best;    // [rows, parts]
+    unsigned long long* mass;    // [rows, parts]
+    unsigned long long* masses;  // [rows, kSteps]
+    unsigned long long* list;    // [rows, kList] ranks
+    uint32_t* counts;            // [rows, kSteps]
+    uint32_t* listed;            // [rows]
+};
+
+// All parts of a row on one XCD (block index modulo 8), whose L2 then holds the row and its histogram.
+__device__ __forceinline__ bool place_of(const SampleArgs& a, const SampleSplit& s, int64_t& row, int& part) {
+    const uint32_t j = blockIdx.x / 8;
+    row = static_cast<int64_t>(j / s.parts) * 8 + blockIdx.x % 8;
+    part = j % s.parts;
+    return row < a.rows;
+}
+
+template <class T>
+__global__ void __launch_bounds__(kThreads) sample_best_kernel(SampleArgs a, SampleSplit s, bool wide) {
+    using U = Unit<T>;
+    __shared__ unsigned long long words[kWaves];
+    int64_t row;
+    int part;
+    if (!place_of(a, s, row, part)) return;
+    const T* in = static_cast<const T*>(a.logits) + row * a.logits_stride;
+    const int64_t from = part * s.part, to = from + s.part < a.vocab ? from + s.part : a.vocab;
+    uint64_t best = 0;
+#pragma unroll 4
+    for (int64_t v = from + U::kWidth * static_cast<int>(threadIdx.x); v < to; v += U::kWidth * kThreads) {
+        U unit;
+        unit.load(in, v, to, wide);
+#pragma unroll
+        for (int j = 0; j < U::kWidth; ++j) {
+            const uint64_t rank = rank_of(unit[j], static_cast<uint32_t>(v + j));
+            best = v + j < to && rank > best ? rank : best;
         }
-        all = running;
-        const double u = a.uniforms[row];
-        const double wanted = u > 0.0 ? u * static_cast<double>(all) : 0.0;
-        target = wanted < static_cast<double>(all - 1) ? static_cast<uint64_t>(wanted) : all - 1;
     }
+    best = block_best<kThreads>(best, words);
+    if (threadIdx.x == 0) s.best[row * s.parts + part] = best;
+    for (int b = part * kThreads + threadIdx.x; b < kSteps; b += s.parts * kThreads)
+        s.masses[row * kSteps + b] = 0, s.counts[row * kSteps + b] = 0;
+    if (part == 0 && threadIdx.x == 0) s.listed[row] = 0;
+}
+
+__device__ __forceinline__ RowOptions row_options(const SampleArgs& a, const SampleSplit& s, int64_t row, int bits, unsigned long long* words) {
+    uint64_t best = threadIdx.x < static_cast<uint32_t>(s.parts) ? s.best[row * s.parts + threadIdx.x] : 0;  // at most kMostParts
+    return options_of(a, row, bits, block_best<kThreads>(best, words));
+}
+
+template <class T>
+__global__ void __launch_bounds__(kThreads) sample_mass_kernel(SampleArgs a, SampleSplit s, int bits, bool wide) {
+    using U = Unit<T>;
+    __shared__ unsigned long long words[kWaves];
+    __shared__ double roots[32];
+    __shared__ unsigned long long masses[kSteps];
+    __shared__ uint32_t counts[kSteps];
+    int64_t row;
+    int part;
+    if (!place_of(a, s, row, part)) return;
+    if (threadIdx.x < 32) roots[threadIdx.x] = kRoots[threadIdx.x];
+    const RowOptions o = row_options(a, s, row, bits, words);
+    if (!o.draws) {
+        if (part == 0 && threadIdx.x == 0) a.tokens[row] = o.greedy, a.probabilities[row] = 1.0f;
+        return;
+    }
+    const bool by_count = o.k < a.vocab, by_mass = o.p < 1.0f, filtered = by_count || by_mass;
+    if (filtered) {
+        for (int b = threadIdx.x; b < kSteps; b += kThreads) masses[b] = 0, counts[b] = 0;
+        __syncthreads();
+    }
+    const Weigher weigh{roots, o.top, o.rate, bits};
+    const T* in = static_cast<const T*>(a.logits) + row * a.logits_stride;
+    const int64_t from = part * s.part, to = from + s.part < a.vocab ? from + s.part : a.vocab;
+    uint64_t sum = 0;
+    for (int64_t v = from + U::kWidth * static_cast<int>(threadIdx.x); v < to; v += U::kWidth * kThreads) {
+        U unit;
+        unit.load(in, v, to, wide);
+#pragma unroll
+        for (int j = 0; j < U::kWidth; ++j) {
+            double f;
+            const int step = weigh.step_of(unit[j], f);
+            if (step >= kSteps) continue;
+            if (by_count) atomicAdd(counts + step, 1u);
+            if (by_count && !by_mass) continue;
+            const uint64_t w = weigh.weight(step, f);
+            if (by_mass) atomicAdd(masses + step, static_cast<unsigned long long>(w));
+            else sum += w < o.least ? 0 : w;
+        }
+    }
+    if (!filtered) {
+        uint64_t all;
+        block_scan<kThreads>(sum, words, &all);
+        if (threadIdx.x == 0) s.mass[row * s.parts + part] = all;
+        return;
+    }
+    __syncthreads();
+    for (int b = threadIdx.x; b < kSteps; b += kThreads) {
+        if (counts[b]) atomicAdd(s.counts + row * kSteps + b, counts[b]);
+        if (masses[b]) atomicAdd(s.masses + row * kSteps + b, masses[b]);
+    }
+}
+
+// Where the kept tokens of a row end, as far as its histogram tells: steps below `sure` are kept, the end is in the list, that
+// is the steps [sure, last] and `by_count`, in which the k-th token is.  kSteps: none.
+struct Ends {
+    int sure, last, by_count;
+    uint64_t count_before, mass_before;  // of the step by_count
+    uint64_t mass_sure;  // of the steps below `sure`
+    uint64_t mass_all;
+};
+
+struct EndsShared {
+    unsigned long long words[kWaves];
+    int step;
+    unsigned long long count, mass;
+};
+
+__device__ Ends ends_of(const SampleSplit& s, int64_t row, const RowOptions& o, int64_t vocab, EndsShared& shared) {
+    constexpr int kEach = (kSteps + kThreads - 1) / kThreads;
+    const int b0 = kEach * threadIdx.x;
+    uint64_t mass[kEach], masses = 0, count[kEach], counts = 0;
+#pragma unroll
+    for (int j = 0; j < kEach; ++j) {
+        const bool real = b0 + j < kSteps;
+        mass[j] = real ? s.masses[row * kSteps + b0 + j] : 0;
+        count[j] = real && o.k < vocab ? s.counts[row * kSteps + b0 + j] : 0;
+        masses += mass[j];
+        counts += count[j];
+    }
+    uint64_t all_mass, all_count = 0, count_before = 0;
+    const uint64_t mass_before = block_scan<kThreads>(masses, shared.words, &all_mass) - masses;
+    if (o.k < vocab) count_before = block_scan<kThreads>(counts, shared.words, &all_count) - counts;
+    // The first step at which the sum reaches the limit.
+    auto reach = [&](uint64_t limit, uint64_t before, const uint64_t (&added)[kEach]) {
+        __syncthreads();
+        if (threadIdx.x == 0) shared.step = kSteps;
+        __syncthreads();
+        uint64_t mass_at = mass_before, at = before;
+#pragma unroll
+        for (int j = 0; j < kEach; ++j) {
+            if (at < limit && at + added[j] >= limit) shared.step = b0 + j, shared.count = at, shared.mass = mass_at;
+            at += added[j];
+            mass_at += mass[j];
+        }
+        __syncthreads();
+        return shared.step;
+    };
+    Ends e{kSteps, kSteps, kSteps, 0, 0, all_mass, all_mass};
+    uint64_t low = all_mass, high = all_mass;
+    if (o.k < vocab && all_count >= static_cast<uint64_t>(o.k)) {
+        e.by_count = reach(o.k, count_before, count);
+        e.count_before = shared.count;
+        e.mass_before = e.mass_sure = shared.mass;
+        e.sure = e.last = e.by_count;
+        low = e.mass_before;
+        high = e.by_count < kSteps ? e.mass_before + s.masses[row * kSteps + e.by_count] : all_mass;
+    }
+    if (o.p < 1.0f) {
+        e.last = reach(mass_limit(o.p, high), mass_before, mass);
+        e.sure = reach(mass_limit(o.p, low), mass_before, mass);
+        e.mass_sure = shared.mass;
+    }
+    return e;
+}
+
+template <class T>
+__global__ void __launch_bounds__(kThreads) sample_list_kernel(SampleArgs a, SampleSplit s, int bits, bool wide) {
+    using U = Unit<T>;
+    __shared__ EndsShared shared;
+    __shared__ double roots[32];
+    __shared__ unsigned long long found[kList];
+    __shared__ uint32_t count, first;
+    int64_t row;
+    int part;
+    if (!place_of(a, s, row, part)) return;
+    if (threadIdx.x < 32) roots[threadIdx.x] = kRoots[threadIdx.x];
+    const RowOptions o = row_options(a, s, row, bits, shared.words);
+    if (!o.draws || (o.k >= a.vocab && o.p >= 1.0f)) return;
+    const Ends e = ends_of(s, row, o, a.vocab, shared);
+    if (threadIdx.x == 0) count = 0;
+    __syncthreads();
+    const Weigher weigh{roots, o.top, o.rate, bits};
+    const T* in = static_cast<const T*>(a.logits) + row * a.logits_stride;
+    const int64_t from = part * s.part, to = from + s.part < a.vocab ? from + s.part : a.vocab;
+    uint64_t sum = 0;
+    for (int64_t v = from + U::kWidth * static_cast<int>(threadIdx.x); v < to; v += U::kWidth * kThreads) {
+        U unit;
+        unit.load(in, v, to, wide);
+#pragma unroll
+        for (int j = 0; j < U::kWidth; ++j) {
+            double f;
+            const int step = weigh.step_of(unit[j], f);
+            if (step >= kSteps) continue;
+            if (step < e.sure) {
+                const uint64_t w = weigh.weight(step, f);
+                sum += w < o.least ? 0 : w;
+            } else if (step <= e.last || step == e.by_count) {
+                const uint32_t at = atomicAdd(&count, 1u);
+                if (at < kList) found[at] = rank_of(unit[j], static_cast<uint32_t>(v + j));
+            }
+        }
+    }
+    uint64_t all;
+    block_scan<kThreads>(sum, shared.words, &all);
+    if (threadIdx.x == 0) {
+        s.mass[row * s.parts + part] = all;
+        first = count ? atomicAdd(s.listed + row, count) : 0;
+    }
+    __syncthreads();
+    for (uint32_t i = threadIdx.x; i < count && i < kList; i += kThreads)
+        if (first + i < kList) s.list[row * kList + first + i] = found[i];
+}
+
+struct DrawShared {
+    unsigned long long list[kList], sorted[kList];
+    unsigned long long part_mass[kMostParts];
+    unsigned long long end, before;
+    int index;
+};
+
+template <class T>
+__global__ void __launch_bounds__(kThreads) sample_draw_kernel(SampleArgs a, SampleSplit s, int bits, bool wide) {
+    __shared__ union {
+        DrawShared draw;
+        DigitShared digits;
+    } u;
+    __shared__ EndsShared shared;
+    __shared__ double roots[32];
+    const int64_t row = blockIdx.x;
+    if (threadIdx.x < 32) roots[threadIdx.x] = kRoots[threadIdx.x];
+    const RowOptions o = row_options(a, s, row, bits, shared.words);
+    if (!o.draws) return;
+    const Weigher weigh{roots, o.top, o.rate, bits};
+    const T* in = static_cast<const T*>(a.logits) + row * a.logits_stride;
+    DrawShared& d = u.draw;
+    const bool mine = threadIdx.x < static_cast<uint32_t>(s.parts);
+    if (threadIdx.x < kMostParts) d.part_mass[threadIdx.x] = mine ? s.mass[row * s.parts + threadIdx.x] : 0;
+    uint64_t end = 0;
+    if (o.k < a.vocab || o.p < 1.0f) {
+        const uint32_t listed = s.listed[row];
+        if (listed > kList) {
+            __syncthreads();
+            if (threadIdx.x < 32) u.digits.roots[threadIdx.x] = kRoots[threadIdx.x];
+            __syncthreads();
+            sample_row<T, kThreads>(a, row, o, bits, wide, u.digits);
+            return;
+        }
+        const Ends e = ends_of(s, row, o, a.vocab, shared);
+        // In their order: every token counts those before it.
+        for (uint32_t i = threadIdx.x; i < listed; i += kThreads) d.list[i] = s.list[row * kList + i];
+        if (threadIdx.x == 0) d.end = ~0ull;
+        __syncthreads();
+        for (uint32_t i = threadIdx.x; i < listed; i += kThreads) {
+            uint32_t before = 0;
+            for (uint32_t j = 0; j < listed; ++j) before += d.list[j] > d.list[i];
+            d.sorted[before] = d.list[i];
+        }
+        __syncthreads();
+        constexpr int kEach = kList / kThreads;
+        const uint32_t i0 = kEach * threadIdx.x;
+        uint64_t w[kEach], sum = 0, counted = 0, below = 0;
+        bool of_count[kEach];
+#pragma unroll
+        for (int j = 0; j < kEach; ++j) {
+            w[j] = 0;
+            of_count[j] = false;
+            if (i0 + j < listed) {
+                double f;
+                const int step = weigh.step_of(value_of(static_cast<uint32_t>(d.sorted[i0 + j] >> 32)), f);
+                w[j] = weigh.weight(step, f);
+                of_count[j] = step == e.by_count;
+                below += step < e.by_count;
+            }
+            sum += w[j];
+        }
+        uint64_t first_of_count, total;
+        block_scan<kThreads>(below, shared.words, &first_of_count);
+        // The mass of the first k: the step by_count's tokens up to the k-th one.
+        const uint64_t kept_of_count = e.by_count < kSteps ? o.k - e.count_before : 0;
+#pragma unroll
+        for (int j = 0; j < kEach; ++j)
+            if (of_count[j] && i0 + j < first_of_count + kept_of_count) counted += w[j];
+        block_scan<kThreads>(counted, shared.words, &total);
+        const uint64_t first_k = e.by_count < kSteps ? e.mass_before + total : e.mass_all;
+        const uint64_t limit = o.p < 1.0f ? mass_limit(o.p, first_k) : ~uint64_t{0};
+        // Kept of the list: up to the k-th token, and while the mass before is below the limit.  Between the steps [sure, last]
+        // and by_count others are left out of the list: what follows them is beyond the limit.
+        uint64_t reached = e.mass_sure + block_scan<kThreads>(sum, shared.words, &total) - sum;
+#pragma unroll
+        for (int j = 0; j < kEach; ++j) {
+            if (i0 + j < listed && reached < limit && (!of_count[j] || i0 + j < first_of_count + kept_of_count)) {
+                atomicMin(&d.end, d.sorted[i0 + j]);
+                const uint32_t index = ~static_cast<uint32_t>(d.sorted[i0 + j]);
+                if (w[j] >= o.least) atomicAdd(d.part_mass + index / s.part, static_cast<unsigned long long>(w[j]));
+            }
+            reached += w[j];
+        }
+        __syncthreads();
+        if (listed) end = d.end;
+    }
+    __syncthreads();
+    uint64_t all;
+    const uint64_t mass = threadIdx.x < kMostParts ? d.part_mass[threadIdx.x] : 0;
+    const uint64_t reached = block_scan<kThreads>(mass, shared.words, &all);
+    const uint64_t target = drawn_mass(a.uniforms[row], all);
+    if (mass && reached > target && reached - mass <= target) d.index = threadIdx.x, d.before = reached - mass;
+    __syncthreads();
+    const int64_t from = d.index * s.part, to = from + s.part < a.vocab ? from + s.part : a.vocab;
+    draw_in<T, kThreads>(a, row, in, wide, from, to, weigh, end, o.least, d.before, target, all, shared.words);
+}
+
+// Rows up to this many tokens are one workgroup's.
+constexpr int64_t kShortRow = 8192;
+// Tokens that all threads of a workgroup read at once in 16-bit types: parts are multiples of it.
+constexpr int64_t kPartStep = 4096;
+
+// About four workgroups a CU.
+SampleSplit split_of(int64_t rows, int64_t vocab, void* workspace, size_t* bytes) {
+    SampleSplit s{};
+    int64_t parts = (1024 + rows - 1) / rows;
+    if (parts > kMostParts) parts = kMostParts;
+    s.part = ((vocab + parts - 1) / parts + kPartStep - 1) / kPartStep * kPartStep;
+    s.parts = static_cast<int>((vocab + s.part - 1) / s.part);
+    auto* at = static_cast<unsigned long long*>(workspace);
+    s.best = at;
+    s.mass = s.best + rows * s.parts;
+    s.masses = s.mass + rows * s.parts;
+    s.list = s.masses + rows * kSteps;
+    s.counts = reinterpret_cast<uint32_t*>(s.list + rows * kList);
+    s.listed = s.counts + rows * kSteps;
+    *bytes = static_cast<size_t>(rows) * (16 * s.parts + 8 * kSteps + 8 * kList + 4 * kSteps) + static_cast<size_t>(rows + rows % 2) * 4;
+    return s;
+}
+
+template <class T>
+hipError_t launch_sample(const SampleArgs& a, hipStream_t stream) {
+    int bits = 51;
+    while (bits > 0 && (a.vocab << bits) > (int64_t{1} << 62)) --bits;
+    const bool wide = reinterpret_cast<uintptr_t>(a.logits) % 16 == 0 && a.logits_stride * sizeof(T) % 16 == 0;
+    const auto rows = static_cast<uint32_t>(a.rows);
+    if (a.vocab <= kShortRow) {
+        hipLaunchKernelGGL(HIP_KERNEL_NAME(sample_row_kernel<T>), dim3(rows), dim3(kRowThreads), 0, stream, a, bits, wide);
+        return hipGetLastError();
+    }
+    size_t bytes = 0;
+    const SampleSplit s = split_of(a.rows, a.vocab, a.workspace, &bytes);
+    const dim3 grid((rows + 7) / 8 * 8 * static_cast<uint32_t>(s.parts));
+    hipLaunchKernelGGL(HIP_KERNEL_NAME(sample_best_kernel<T>), grid, dim3(kThreads), 0, stream, a, s, wide);
+    hipLaunchKernelGGL(HIP_KERNEL_NAME(sample_mass_kernel<T>), grid, dim3(kThreads), 0, stream, a, s, bits, wide);
+    if (a.top_k || a.top_p) hipLaunchKernelGGL(HIP_KERNEL_NAME(sample_list_kernel<T>), grid, dim3(kThreads), 0, stream, a, s, bits, wide);
+    hipLaunchKernelGGL(HIP_KERNEL_NAME(sample_draw_kernel<T>), dim3(rows), dim3(kThreads), 0, stream, a, s, bits, wide);
+    return hipGetLastError();
 }
 
 }  // namespace
 
-size_t sample_workspace_bytes(int64_t rows, int64_t vocab) { return 0; }
+size_t sample_workspace_bytes(int64_t rows, int64_t vocab) {
+    if (vocab <= kShortRow) return 0;
+    size_t bytes = 0;
+    split_of(rows, vocab, nullptr, &bytes);
+    return bytes;
+}
 
-hipError_t launch_logits_sample(const SampleArgs& a, Type type, hipStream_t stream) {
-    int bits = 51;
-    while (bits > 0 && (a.vocab << bits) > (int64_t{1} << 62)) --bits;
-    const dim3 grid(static_cast<uint32_t>(a.rows));
+hipError_t launch_logits_sample(const SampleArgs& args, Type type, hipStream_t stream) {
     switch (type) {
-        case Type::kFloat32: hipLaunchKernelGGL(sample_row_kernel<float>, grid, dim3(kThreads), 0, stream, a, bits); break;
-        case Type::kFloat16: hipLaunchKernelGGL(sample_row_kernel<_Float16>, grid, dim3(kThreads), 0, stream, a, bits); break;
-        default: hipLaunchKernelGGL(sample_row_kernel<__bf16>, grid, dim3(kThreads), 0, stream, a, bits);
+        case Type::kFloat32: return launch_sample<float>(args, stream);
+        case Type::kFloat16: return launch_sample<_Float16>(args, stream);
+        default: return launch_sample<__bf16>(args, stream);
     }
-    return hipGetLastError();
 }
 
 }  // namespace flux
