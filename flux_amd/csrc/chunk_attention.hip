@@ -10,6 +10,8 @@
 #include "serving.h"
 #include "serving_mfma.h"
 
+#include <type_traits>
+
 namespace flux {
 namespace {
 
@@ -20,7 +22,7 @@ constexpr int kLeastStages = 4;  // that are worth a workgroup
 template <class T>
 constexpr int rows_of_tile(int dim) { return sizeof(T) == 2 ? 32 * kWaves : (dim <= 128 ? 32 : 16); }
 template <class T>
-constexpr int stage_keys(int dim) { return sizeof(T) == 2 ? (dim == 64 ? 128 : (dim == 128 ? 64 : 32)) : 64; }
+constexpr int stage_keys(int dim) { return sizeof(T) == 2 && dim == 64 ? 128 : 64; }
 constexpr int padded_dim(int dim) { return dim <= 64 ? 64 : (dim <= 128 ? 128 : 256); }
 
 // What the launches of one call agree on.
@@ -522,12 +524,24 @@ __global__ void __launch_bounds__(kThreads, kDim <= 64 ? 3 : (kDim <= 128 ? 2 : 
 }
 
 // ---------------------------------------------------------------------------
-// 16-bit types: keys and values are staged in LDS for the workgroup's four waves, 32 rows each.  A stage holds kStage
-// keys: K rows as they are, V transposed (the staging thread permutes the 16-bit halves of four keys), its keys in the
-// order in which a lane's scores lie.  S^T = K Q^T on 32 x 32 tiles leaves lane (n, h) with the keys 8 (r / 4) + 4 h + r % 4
-// of row n, which rounded in pairs are the right operand of O^T = V^T P.  Where a stage's rows lie is looked up two stages
-// ahead.  Weights are rounded once to the values' type for the product and summed unrounded; the running maximum moves
-// only when a tile exceeds it by 2^kLazy.
+// 16-bit types: keys and values are staged in LDS, row by row as they are, for the workgroup's four waves of 32 rows each, and
+// copied there past the registers while the stage before is worked on.  S^T = K Q^T on 32 x 32 tiles leaves lane (n, h) with the
+// keys 8 (r / 4) + 4 h + r % 4 of row n, which rounded in pairs are the right operand of O^T = V^T P; V's left operand, one dim
+// of four keys, comes by reads that transpose 4 x 16 blocks.  A row's 16-byte pieces lie permuted, so that these reads meet
+// different banks: piece c of row r is at c ^ swizzle(r).  Where a stage's rows lie is looked up two stages ahead.  Weights are
+// rounded once to the values' type for the product and summed unrounded; the running maximum moves only when a tile exceeds it
+// by 2^kLazy.
+template <int kDim>
+__device__ __forceinline__ int swizzle(int r) {
+    if constexpr (kDim == 64) return (r >> 1 & 1) << 2 | (r >> 2 & 3);  // rows of half the banks
+    else return (r & 3) << 2 | (r >> 2 & 3);
+}
+
+__device__ __forceinline__ u32x2 read_transposed(const char* at) {
+    typedef __attribute__((address_space(3))) s16x4 Block;
+    return __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((Block*)(at)));
+}
+
 template <class T, int kDim, bool kWide>
 __global__ void __launch_bounds__(kThreads, kDim <= 128 ? 2 : 1) chunk_tile_kernel(ChunkArgs a, ChunkPlan plan) {
     using W = Wide<T>;
@@ -536,14 +550,13 @@ __global__ void __launch_bounds__(kThreads, kDim <= 128 ? 2 : 1) chunk_tile_kern
     constexpr int kSteps = kDim / 16;             // of a score
     constexpr int kBlocks = kDim / 32;            // of the result
     constexpr int kRows = rows_of_tile<T>(kDim);
-    constexpr int kKeyRow = kDim * 2 + 16;        // bytes
-    constexpr int kValueRow = kStage * 2 + 16;
-    constexpr int kBytes = kStage * kKeyRow + kDim * kValueRow;
-    constexpr int kKeyLoads = kStage * kDim / 8 / kThreads;        // 16 bytes per thread
-    constexpr int kKeyRows = kThreads / (kDim / 8);                // rows that one load of all threads covers
-    static_assert(kStage / 4 * (kDim / 8) == kThreads, "every thread stages four keys by eight dims of the values");
+    constexpr int kRowBytes = kDim * 2;
+    constexpr int kSide = kStage * kRowBytes;     // keys or values of a stage
+    constexpr int kPieces = kDim / 8;             // of a row, 16 bytes each
+    constexpr int kCopyRows = 64 / kPieces;       // of one copy of a wave
+    constexpr int kCopies = kStage / kCopyRows / kWaves;  // of a wave, for each side
     extern __shared__ char stages_memory[];
-    __shared__ int64_t places[2][2][kStage];   // elements from the pool's start, by stage parity
+    __shared__ int64_t places[2][2][kStage];   // bytes from the head's first, by stage parity
     __shared__ uint32_t missing[2][kSubs];     // keys of a stage that are on no page
 
     clear_other_rows<T>(a);
@@ -552,7 +565,7 @@ __global__ void __launch_bounds__(kThreads, kDim <= 128 ? 2 : 1) chunk_tile_kern
     const Part part = part_of<kRows, kStage>(a, plan, unit, kv_head == 0, s);
     if (!part.real) return;
     const int lane = threadIdx.x & 63;
-    const int wave = threadIdx.x >> 6;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int n32 = lane & 31;
     const int half = lane >> 5;
     const int row0 = part.tile * kRows, all_rows = s.count * a.group, wave_row = row0 + wave * 32;
@@ -562,11 +575,11 @@ __global__ void __launch_bounds__(kThreads, kDim <= 128 ? 2 : 1) chunk_tile_kern
     wave_first = __builtin_amdgcn_readfirstlane(wave_first);
     wave_last = __builtin_amdgcn_readfirstlane(wave_last);
     const KeyStages<kStage> stages(a, block_first, block_last);
-    const int from = static_cast<int>(static_cast<int64_t>(stages.count) * part.part / part.parts);
-    const int to = static_cast<int>(static_cast<int64_t>(stages.count) * (part.part + 1) / part.parts);
+    const int from = __builtin_amdgcn_readfirstlane(static_cast<int>(static_cast<int64_t>(stages.count) * part.part / part.parts));
+    const int to = __builtin_amdgcn_readfirstlane(static_cast<int>(static_cast<int64_t>(stages.count) * (part.part + 1) / part.parts));
 
-    const T* keys = static_cast<const T*>(a.key) + kv_head * a.key_strides[1];
-    const T* values = static_cast<const T*>(a.value) + kv_head * a.value_strides[1];
+    const char* keys = static_cast<const char*>(a.key) + 2 * kv_head * a.key_strides[1];
+    const char* values = static_cast<const char*>(a.value) + 2 * kv_head * a.value_strides[1];
     const int32_t* table = a.table + (s.slot < 0 ? 0 : s.slot) * a.table_stride;
 
     const int r = wave_row + n32;  // this lane's row
@@ -609,150 +622,164 @@ __global__ void __launch_bounds__(kThreads, kDim <= 128 ? 2 : 1) chunk_tile_kern
             const bool held = page >= 0 && page < a.pages;
             const int64_t of_page = held ? page : 0;
             const int in_page = held ? position - static_cast<int>(divide(position, a.page) * a.page.divisor) : 0;
-            places[t & 1][0][threadIdx.x] = of_page * a.key_strides[0] + in_page * a.key_strides[2];
-            places[t & 1][1][threadIdx.x] = of_page * a.value_strides[0] + in_page * a.value_strides[2];
+            places[t & 1][0][threadIdx.x] = 2 * (of_page * a.key_strides[0] + in_page * a.key_strides[2]);
+            places[t & 1][1][threadIdx.x] = 2 * (of_page * a.value_strides[0] + in_page * a.value_strides[2]);
             const uint64_t gone = __ballot(!held);
             if (lane == 0) missing[t & 1][threadIdx.x / 32] = static_cast<uint32_t>(gone);
             if (lane == 32) missing[t & 1][threadIdx.x / 32] = static_cast<uint32_t>(gone >> 32);
         };
-        u32x4 held_key[kKeyLoads];
-        u32x4 held_value[4];
-        const int key_row = threadIdx.x / (kDim / 8), key_d = threadIdx.x % (kDim / 8) * 8;
-        const int value_row = threadIdx.x % (kStage / 4) * 4, value_d = threadIdx.x / (kStage / 4) * 8;
-        auto load = [&](const T* row, int d) {
-            if constexpr (kWide) return *reinterpret_cast<const u32x4*>(row + (d < a.dim ? d : 0));
-            else return Mfma<T>::load_strided(row, 1, d, a.dim);
-        };
-        auto fetch_keys = [&](int t) {
+        // Copy j of a wave: rows kCopyRows (kWaves j + wave) and on, of which this lane brings one piece.  Dims behind the head's
+        // repeat its first ones, which meet zeros of the query or results that are not stored.
+        auto copy = [&](int t) {
+            char* stage = stages_memory + (t & 1) * 2 * kSide;
 #pragma unroll
-            for (int i = 0; i < kKeyLoads; ++i) held_key[i] = load(keys + places[t & 1][0][key_row + kKeyRows * i], key_d);
-        };
-        auto fetch_values = [&](int t) {
-#pragma unroll
-            for (int j = 0; j < 4; ++j) held_value[j] = load(values + places[t & 1][1][value_row + j], value_d);
-        };
-        auto put_keys = [&](char* stage) {
-#pragma unroll
-            for (int i = 0; i < kKeyLoads; ++i) {
-                const int at = threadIdx.x + kThreads * i;
-                *reinterpret_cast<u32x4*>(stage + at / (kDim / 8) * kKeyRow + at % (kDim / 8) * 16) = held_key[i];
+            for (int j = 0; j < kCopies; ++j) {
+                const int row = kCopyRows * (kWaves * j + wave) + lane / kPieces;
+                const int piece = (lane % kPieces) ^ swizzle<kDim>(row), d = 8 * piece < a.dim ? 8 * piece : 0;
+                char* to_key = stage + kCopyRows * (kWaves * j + wave) * kRowBytes;
+                const char* key = keys + places[t & 1][0][row];
+                const char* value = values + places[t & 1][1][row];
+                if constexpr (kWide) {
+                    __builtin_amdgcn_global_load_lds(reinterpret_cast<const uint32_t*>(key + 2 * d), (__attribute__((address_space(3))) uint32_t*)(to_key), 16, 0, 0);
+                    __builtin_amdgcn_global_load_lds(reinterpret_cast<const uint32_t*>(value + 2 * d), (__attribute__((address_space(3))) uint32_t*)(to_key + kSide), 16, 0, 0);
+                } else {
+                    *reinterpret_cast<u32x4*>(to_key + 16 * lane) = Mfma<T>::load_strided(reinterpret_cast<const T*>(key), 1, 8 * piece, a.dim);
+                    *reinterpret_cast<u32x4*>(to_key + kSide + 16 * lane) =
+                        Mfma<T>::load_strided(reinterpret_cast<const T*>(value), 1, 8 * piece, a.dim);
+                }
             }
         };
-        auto put_values = [&](char* stage, int t) {
-            const uint32_t gone = missing[t & 1][value_row / 32] >> (value_row % 32) & 15u;
-            if (gone) {  // a weight of zero does not undo a NaN
+        int key_at[kSteps], value_at[kBlocks][2];
 #pragma unroll
-                for (int j = 0; j < 4; ++j)
-                    if (gone >> j & 1) held_value[j] = u32x4{0, 0, 0, 0};
+        for (int k = 0; k < kSteps; ++k) key_at[k] = n32 * kRowBytes + (((2 * k + half) ^ swizzle<kDim>(n32)) * 16);
+#pragma unroll
+        for (int b = 0; b < kBlocks; ++b)
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+                const int row = 8 * e + 4 * half + (lane & 15) / 4, piece = 4 * b + 2 * (lane >> 4 & 1) + (lane & 3) / 2;
+                value_at[b][e] = kSide + row * kRowBytes + (piece ^ swizzle<kDim>(row)) * 16 + 8 * (lane & 1);
             }
-            char* turned = stage + kStage * kKeyRow;
-            // Quads 0, 1, 2, 3 of 16 keys lie as 0, 2, 1, 3: a lane's eight keys side by side.
-            const int quad = value_row / 4, at = (quad & ~3) | (quad & 1) << 1 | (quad >> 1 & 1);
-#pragma unroll
-            for (int j = 0; j < 8; ++j)
-                *reinterpret_cast<u32x2*>(turned + (value_d + j) * kValueRow + at * 8) =
-                    u32x2{Mfma<T>::pair(held_value[0][j / 2], held_value[1][j / 2], j & 1),
-                          Mfma<T>::pair(held_value[2][j / 2], held_value[3][j / 2], j & 1)};
-        };
 
         const int wave_low = low_of(wave_first), low_of_last = low_of(wave_last);
+        // 32 keys, `first` on, of the stage at `at`.
+        auto work = [&](const char* at, int first, uint32_t gone, auto masked) {
+            u32x4 key[kSteps];
+#pragma unroll
+            for (int k = 0; k < kSteps; ++k) key[k] = *reinterpret_cast<const u32x4*>(at + key_at[k]);
+            f32x16 score;
+#pragma unroll
+            for (int j = 0; j < 16; ++j) score[j] = 0.0f;
+#pragma unroll
+            for (int k = 0; k < kSteps; ++k) score = W::multiply(key[k], query[k], score);
+            if (!ordinary) {
+#pragma unroll
+                for (int j = 0; j < 16; ++j) {
+                    float product = score[j];
+                    asm volatile("" : "+v"(product));  // a branch stays: else all scores pay for the product
+                    score[j] = product * size;
+                }
+            }
+            if constexpr (decltype(masked)::value) {
+#pragma unroll
+                for (int j = 0; j < 16; ++j) {
+                    // Without branches: low <= key <= position as one unsigned comparison, or a sink.
+                    const int in = 8 * (j / 4) + 4 * half + j % 4, of = first + in;
+                    const bool visible = ((static_cast<uint32_t>(of - mine.low) <= static_cast<uint32_t>(mine.position - mine.low)) |
+                                          (of < mine.sink_end)) & !(gone >> in & 1);
+                    score[j] = visible ? score[j] : -INFINITY;
+                }
+            }
+            float highest = fmaxf(score[0], score[1]);
+#pragma unroll
+            for (int j = 2; j < 16; j += 2) highest = fmaxf(fmaxf(highest, score[j]), score[j + 1]);
+            highest = half_max(highest);
+            if (__any((highest - top) * factor > W::kLazy)) {  // NaN where both are -inf
+                const float now = fmaxf(top, highest);
+                const float scaled = now * factor;
+                const float shrink = top == -INFINITY ? 0.0f : fast_exp2(fabsf(scaled) < kFar ? top * factor - scaled : (top - now) * factor);
+                top = now;
+                weight *= shrink;
+#pragma unroll
+                for (int b = 0; b < kBlocks; ++b)
+#pragma unroll
+                    for (int j = 0; j < 16; ++j) out[b][j] *= shrink;
+            }
+            u32x4 value[kBlocks][2];
+#pragma unroll
+            for (int b = 0; b < kBlocks; ++b)
+#pragma unroll
+                for (int k = 0; k < 2; ++k) {
+                    const u32x2 low = read_transposed(at + value_at[b][0] + 16 * k * kRowBytes);
+                    const u32x2 high = read_transposed(at + value_at[b][1] + 16 * k * kRowBytes);
+                    value[b][k] = u32x4{low[0], low[1], high[0], high[1]};
+                }
+            const float scaled = top == -INFINITY ? 0.0f : top * factor;
+            const bool far = !(fabsf(scaled) < kFar);
+            const float reference = W::kShift - (far ? 0.0f : scaled);
+            if (__any(far)) {
+#pragma unroll
+                for (int j = 0; j < 16; ++j) {
+                    float difference = score[j];
+                    asm volatile("" : "+v"(difference));
+                    score[j] = far ? difference - top : difference;
+                }
+            }
+            u32x4 p[2];
+#pragma unroll
+            for (int j = 0; j < 16; j += 2) {
+                const float p0 = fast_exp2(fmaf(score[j], factor, reference));
+                const float p1 = fast_exp2(fmaf(score[j + 1], factor, reference));
+                weight += p0 + p1;
+                p[j / 8][j % 8 / 2] = W::round(p0, p1);
+            }
+#pragma unroll
+            for (int k = 0; k < 2; ++k)
+#pragma unroll
+                for (int b = 0; b < kBlocks; ++b) out[b] = W::multiply(value[b][k], p[k], out[b]);
+        };
+
         put_places(from, look_up(from));
         put_places(from + 1, look_up(from + 1));
         __syncthreads();
         uint32_t gone_next[kSubs];
 #pragma unroll
         for (int i = 0; i < kSubs; ++i) gone_next[i] = missing[from & 1][i];
-        fetch_keys(from);
-        fetch_values(from);
-        put_keys(stages_memory + (from & 1) * kBytes);
-        put_values(stages_memory + (from & 1) * kBytes, from);
+        copy(from);
         for (int t = from; t < to; ++t) {
+            __builtin_amdgcn_s_waitcnt(0);  // this wave's copies have landed
             __syncthreads();
-            const char* stage = stages_memory + (t & 1) * kBytes;
-            const char* turned = stage + kStage * kKeyRow;
+            char* stage = stages_memory + (t & 1) * 2 * kSide;
             const int base = stages.base(t);
-            char* next = stages_memory + ((t + 1) & 1) * kBytes;
-            uint32_t gone[kSubs];  // read a stage ahead: that of this one may be another's already
-#pragma unroll
-            for (int i = 0; i < kSubs; ++i) gone[i] = gone_next[i], gone_next[i] = t + 1 < to ? missing[(t + 1) & 1][i] : 0;
-            const int page = look_up(t + 2);
-            if (t + 1 < to) fetch_keys(t + 1);
+            uint32_t gone[kSubs], any_gone = 0;  // read a stage ahead: that of this one may be another's already
 #pragma unroll
             for (int i = 0; i < kSubs; ++i) {
-                if (i == kSubs / 2 && t + 1 < to) {  // K and V take the same registers on their way
-                    put_keys(next);
-                    fetch_values(t + 1);
-                }
-                const int first = base + 32 * i, last = first + 31;
-                // Nothing of this wave's rows sees these keys.
-                if (first > wave_last || (last < wave_low && first >= a.sinks)) continue;
-                u32x4 key[kSteps];
-#pragma unroll
-                for (int k = 0; k < kSteps; ++k)
-                    key[k] = *reinterpret_cast<const u32x4*>(stage + (32 * i + n32) * kKeyRow + 32 * k + 16 * half);
-                __builtin_amdgcn_sched_barrier(0);  // all reads first: one wait
-                f32x16 score;
-#pragma unroll
-                for (int j = 0; j < 16; ++j) score[j] = 0.0f;
-#pragma unroll
-                for (int k = 0; k < kSteps; ++k) score = W::multiply(key[k], query[k], score);
-                if (!ordinary) {
-#pragma unroll
-                    for (int j = 0; j < 16; ++j) score[j] *= size;
-                }
-                if (first < low_of_last || last > wave_first || __builtin_amdgcn_readfirstlane(gone[i]) != 0) {
-#pragma unroll
-                    for (int j = 0; j < 16; ++j) {
-                        // Without branches: low <= key <= position as one unsigned comparison, or a sink.
-                        const int in = 8 * (j / 4) + 4 * half + j % 4, of = first + in;
-                        const bool visible = ((static_cast<uint32_t>(of - mine.low) <= static_cast<uint32_t>(mine.position - mine.low)) |
-                                              (of < mine.sink_end)) & !(gone[i] >> in & 1);
-                        score[j] = visible ? score[j] : -INFINITY;
-                    }
-                }
-                float highest = score[0];
-#pragma unroll
-                for (int j = 1; j < 16; ++j) highest = fmaxf(highest, score[j]);
-                highest = half_max(highest);
-                if (__any((highest - top) * factor > W::kLazy)) {  // NaN where both are -inf
-                    const float now = fmaxf(top, highest);
-                    const float scaled = now * factor;
-                    const float shrink = top == -INFINITY ? 0.0f : fast_exp2(fabsf(scaled) < kFar ? top * factor - scaled : (top - now) * factor);
-                    top = now;
-                    weight *= shrink;
-#pragma unroll
-                    for (int k = 0; k < kBlocks; ++k)
-#pragma unroll
-                        for (int j = 0; j < 16; ++j) out[k][j] *= shrink;
-                }
-                u32x4 value[kBlocks][2];
-#pragma unroll
-                for (int b = 0; b < kBlocks; ++b)
-#pragma unroll
-                    for (int k = 0; k < 2; ++k)
-                        value[b][k] = *reinterpret_cast<const u32x4*>(turned + (32 * b + n32) * kValueRow + (32 * i + 16 * k) * 2 + 16 * half);
-                __builtin_amdgcn_sched_barrier(0);
-                const float scaled = top == -INFINITY ? 0.0f : top * factor;
-                const bool far = !(fabsf(scaled) < kFar);
-                const float reference = W::kShift - (far ? 0.0f : scaled);
-                if (__any(far)) {
-#pragma unroll
-                    for (int j = 0; j < 16; ++j) score[j] = far ? score[j] - top : score[j];
-                }
-                u32x4 p[2];
-#pragma unroll
-                for (int j = 0; j < 16; j += 2) {
-                    const float p0 = fast_exp2(fmaf(score[j], factor, reference));
-                    const float p1 = fast_exp2(fmaf(score[j + 1], factor, reference));
-                    weight += p0 + p1;
-                    p[j / 8][j % 8 / 2] = W::round(p0, p1);
-                }
-#pragma unroll
-                for (int b = 0; b < kBlocks; ++b)
-#pragma unroll
-                    for (int k = 0; k < 2; ++k) out[b] = W::multiply(value[b][k], p[k], out[b]);
+                gone[i] = gone_next[i];
+                any_gone |= gone[i];
+                gone_next[i] = t + 1 < to ? missing[(t + 1) & 1][i] : 0;
             }
-            if (t + 1 < to) put_values(next, t + 1);
+            const int page = look_up(t + 2);
+            if (t + 1 < to) copy(t + 1);
+            any_gone = __builtin_amdgcn_readfirstlane(any_gone);
+            if (any_gone) {  // a weight of zero does not undo a NaN
+                for (int piece = threadIdx.x; piece < kStage * kPieces; piece += kThreads) {
+                    const int row = piece / kPieces;
+                    if (gone[row / 32] >> (row % 32) & 1) *reinterpret_cast<u32x4*>(stage + kSide + 16 * piece) = u32x4{0, 0, 0, 0};
+                }
+                __syncthreads();
+            }
+            const int last = base + kStage - 1;
+            const bool seen = base <= wave_last && (last >= wave_low || base < a.sinks);
+            if (seen && !any_gone && base >= low_of_last && last <= wave_first) {  // all of it, by all rows
+#pragma unroll
+                for (int i = 0; i < kSubs; ++i) work(stage + 32 * i * kRowBytes, base + 32 * i, 0, std::false_type{});
+            } else if (seen) {
+#pragma unroll 1
+                for (int i = 0; i < kSubs; ++i) {
+                    const int first = base + 32 * i;
+                    if (first > wave_last || (first + 31 < wave_low && first >= a.sinks)) continue;
+                    work(stage + 32 * i * kRowBytes, first, gone[i], std::true_type{});
+                }
+            }
             put_places(t + 2, page);
         }
     }
@@ -841,7 +868,10 @@ __global__ void __launch_bounds__(kThreads) chunk_join_kernel(ChunkArgs a, Chunk
 }
 
 // Parts of a step: two workgroups on each of 256 CUs.
-constexpr int kTarget = 512;
+#ifndef TARGET
+#define TARGET 512
+#endif
+constexpr int kTarget = TARGET;
 
 template <class T>
 ChunkPlan plan_of(const ChunkArgs& a) {
@@ -877,7 +907,7 @@ template <class T, int kDim>
 hipError_t launch_tiles(const ChunkArgs& a, const ChunkPlan& plan, dim3 grid, hipStream_t stream) {
     if constexpr (sizeof(T) == 2) {
         constexpr int kStage = stage_keys<T>(kDim);
-        constexpr size_t kLds = 2 * (kStage * (kDim * 2 + 16) + kDim * (kStage * 2 + 16));
+        constexpr size_t kLds = 4 * kStage * kDim * 2;
         auto launch = [&](auto* kernel) {
             const hipError_t room = hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize,
                                                         static_cast<int>(kLds));
