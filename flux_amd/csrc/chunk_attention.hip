@@ -76,6 +76,8 @@ template <int kStage>
 struct KeyStages {
     int seen, sink_stages, first_stage, count;
     __device__ __forceinline__ KeyStages(const ChunkArgs& a, int first, int last) {
+        first = __builtin_amdgcn_readfirstlane(first);  // the same in all lanes
+        last = __builtin_amdgcn_readfirstlane(last);
         const int low = a.window > 0 && first >= a.window ? first - a.window + 1 : 0;
         const int sinks = a.sinks < low ? a.sinks : low;
         const int of_sinks = (sinks + kStage - 1) / kStage;
@@ -537,9 +539,58 @@ __device__ __forceinline__ int swizzle(int r) {
     else return (r & 3) << 2 | (r >> 2 & 3);
 }
 
+__device__ __forceinline__ uint32_t lds_address(const char* at) {
+    return static_cast<uint32_t>(reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) const char*)(at)));
+}
+// Sixteen bytes of every lane to the LDS at `to` + 16 lane.  In assembly, because the compiler waits for a copy before the next
+// read of any LDS; the kernel waits itself, before the barrier that hands a stage over.  The address register needs one state
+// between its write and its use.
+__device__ __forceinline__ void copy_to_lds(const void* from, uint32_t to) {
+    asm volatile("s_nop 0\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(from), "{m0}"(to) : "memory");
+}
+
 __device__ __forceinline__ u32x2 read_transposed(const char* at) {
     typedef __attribute__((address_space(3))) s16x4 Block;
     return __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((Block*)(at)));
+}
+
+// out *= shrink where `moves`.  In assembly, with its branch inside: behind a branch of the compiler's the sums' registers are
+// moved in the other arm, 64 moves a tile.  The waits cover the matrix instructions that wrote the sums and read them next.
+template <int kBlocks>
+__device__ __forceinline__ void scale_if(bool moves, float shrink, f32x16 (&out)[kBlocks]) {
+    if constexpr (kBlocks > 4) {  // these are in accumulation registers, which no vector instruction takes
+        if (moves) {
+#pragma unroll
+            for (int b = 0; b < kBlocks; ++b) out[b] *= shrink;
+        }
+        return;
+    }
+    const int some = __builtin_amdgcn_readfirstlane(moves);
+#pragma unroll
+    for (int b = 0; b < kBlocks; b += 2) {
+        float o[32];
+#pragma unroll
+        for (int j = 0; j < 32; ++j) o[j] = out[b + j / 16][j % 16];
+        asm volatile(
+            "s_cmp_eq_u32 %32, 0\n\ts_cbranch_scc1 .Lkept%=\n\ts_nop 15\n\ts_nop 15\n\t"
+            "v_mul_f32 %0, %33, %0\n\tv_mul_f32 %1, %33, %1\n\tv_mul_f32 %2, %33, %2\n\tv_mul_f32 %3, %33, %3\n\t"
+            "v_mul_f32 %4, %33, %4\n\tv_mul_f32 %5, %33, %5\n\tv_mul_f32 %6, %33, %6\n\tv_mul_f32 %7, %33, %7\n\t"
+            "v_mul_f32 %8, %33, %8\n\tv_mul_f32 %9, %33, %9\n\tv_mul_f32 %10, %33, %10\n\tv_mul_f32 %11, %33, %11\n\t"
+            "v_mul_f32 %12, %33, %12\n\tv_mul_f32 %13, %33, %13\n\tv_mul_f32 %14, %33, %14\n\tv_mul_f32 %15, %33, %15\n\t"
+            "v_mul_f32 %16, %33, %16\n\tv_mul_f32 %17, %33, %17\n\tv_mul_f32 %18, %33, %18\n\tv_mul_f32 %19, %33, %19\n\t"
+            "v_mul_f32 %20, %33, %20\n\tv_mul_f32 %21, %33, %21\n\tv_mul_f32 %22, %33, %22\n\tv_mul_f32 %23, %33, %23\n\t"
+            "v_mul_f32 %24, %33, %24\n\tv_mul_f32 %25, %33, %25\n\tv_mul_f32 %26, %33, %26\n\tv_mul_f32 %27, %33, %27\n\t"
+            "v_mul_f32 %28, %33, %28\n\tv_mul_f32 %29, %33, %29\n\tv_mul_f32 %30, %33, %30\n\tv_mul_f32 %31, %33, %31\n\t"
+            "s_nop 7\n.Lkept%=:"
+            : "+v"(o[0]), "+v"(o[1]), "+v"(o[2]), "+v"(o[3]), "+v"(o[4]), "+v"(o[5]), "+v"(o[6]), "+v"(o[7]),
+              "+v"(o[8]), "+v"(o[9]), "+v"(o[10]), "+v"(o[11]), "+v"(o[12]), "+v"(o[13]), "+v"(o[14]), "+v"(o[15]),
+              "+v"(o[16]), "+v"(o[17]), "+v"(o[18]), "+v"(o[19]), "+v"(o[20]), "+v"(o[21]), "+v"(o[22]), "+v"(o[23]),
+              "+v"(o[24]), "+v"(o[25]), "+v"(o[26]), "+v"(o[27]), "+v"(o[28]), "+v"(o[29]), "+v"(o[30]), "+v"(o[31])
+            : "s"(some), "v"(shrink)
+            : "scc");
+#pragma unroll
+        for (int j = 0; j < 32; ++j) out[b + j / 16][j % 16] = o[j];
+    }
 }
 
 template <class T, int kDim, bool kWide>
@@ -630,21 +681,22 @@ __global__ void __launch_bounds__(kThreads, kDim <= 128 ? 2 : 1) chunk_tile_kern
         };
         // Copy j of a wave: rows kCopyRows (kWaves j + wave) and on, of which this lane brings one piece.  Dims behind the head's
         // repeat its first ones, which meet zeros of the query or results that are not stored.
+        const uint32_t memory = lds_address(stages_memory);
         auto copy = [&](int t) {
-            char* stage = stages_memory + (t & 1) * 2 * kSide;
+            const int stage = (t & 1) * 2 * kSide;
 #pragma unroll
             for (int j = 0; j < kCopies; ++j) {
                 const int row = kCopyRows * (kWaves * j + wave) + lane / kPieces;
                 const int piece = (lane % kPieces) ^ swizzle<kDim>(row), d = 8 * piece < a.dim ? 8 * piece : 0;
-                char* to_key = stage + kCopyRows * (kWaves * j + wave) * kRowBytes;
+                const int to_key = stage + kCopyRows * (kWaves * j + wave) * kRowBytes;
                 const char* key = keys + places[t & 1][0][row];
                 const char* value = values + places[t & 1][1][row];
                 if constexpr (kWide) {
-                    __builtin_amdgcn_global_load_lds(reinterpret_cast<const uint32_t*>(key + 2 * d), (__attribute__((address_space(3))) uint32_t*)(to_key), 16, 0, 0);
-                    __builtin_amdgcn_global_load_lds(reinterpret_cast<const uint32_t*>(value + 2 * d), (__attribute__((address_space(3))) uint32_t*)(to_key + kSide), 16, 0, 0);
+                    copy_to_lds(key + 2 * d, memory + to_key);
+                    copy_to_lds(value + 2 * d, memory + to_key + kSide);
                 } else {
-                    *reinterpret_cast<u32x4*>(to_key + 16 * lane) = Mfma<T>::load_strided(reinterpret_cast<const T*>(key), 1, 8 * piece, a.dim);
-                    *reinterpret_cast<u32x4*>(to_key + kSide + 16 * lane) =
+                    *reinterpret_cast<u32x4*>(stages_memory + to_key + 16 * lane) = Mfma<T>::load_strided(reinterpret_cast<const T*>(key), 1, 8 * piece, a.dim);
+                    *reinterpret_cast<u32x4*>(stages_memory + to_key + kSide + 16 * lane) =
                         Mfma<T>::load_strided(reinterpret_cast<const T*>(value), 1, 8 * piece, a.dim);
                 }
             }
@@ -666,6 +718,7 @@ __global__ void __launch_bounds__(kThreads, kDim <= 128 ? 2 : 1) chunk_tile_kern
             u32x4 key[kSteps];
 #pragma unroll
             for (int k = 0; k < kSteps; ++k) key[k] = *reinterpret_cast<const u32x4*>(at + key_at[k]);
+            __builtin_amdgcn_sched_barrier(0);  // all reads first
             f32x16 score;
 #pragma unroll
             for (int j = 0; j < 16; ++j) score[j] = 0.0f;
@@ -693,17 +746,17 @@ __global__ void __launch_bounds__(kThreads, kDim <= 128 ? 2 : 1) chunk_tile_kern
 #pragma unroll
             for (int j = 2; j < 16; j += 2) highest = fmaxf(fmaxf(highest, score[j]), score[j + 1]);
             highest = half_max(highest);
-            if (__any((highest - top) * factor > W::kLazy)) {  // NaN where both are -inf
+            // By 2^(old maximum - new one), where a row's moved: in few tiles behind the first.
+            const bool moves = __any((highest - top) * factor > W::kLazy);  // NaN where both are -inf
+            float shrink = 1.0f;
+            if (moves) {
                 const float now = fmaxf(top, highest);
                 const float scaled = now * factor;
-                const float shrink = top == -INFINITY ? 0.0f : fast_exp2(fabsf(scaled) < kFar ? top * factor - scaled : (top - now) * factor);
+                shrink = top == -INFINITY ? 0.0f : fast_exp2(fabsf(scaled) < kFar ? top * factor - scaled : (top - now) * factor);
                 top = now;
                 weight *= shrink;
-#pragma unroll
-                for (int b = 0; b < kBlocks; ++b)
-#pragma unroll
-                    for (int j = 0; j < 16; ++j) out[b][j] *= shrink;
             }
+            scale_if<kBlocks>(moves, shrink, out);
             u32x4 value[kBlocks][2];
 #pragma unroll
             for (int b = 0; b < kBlocks; ++b)
@@ -755,16 +808,17 @@ __global__ void __launch_bounds__(kThreads, kDim <= 128 ? 2 : 1) chunk_tile_kern
             for (int i = 0; i < kSubs; ++i) {
                 gone[i] = gone_next[i];
                 any_gone |= gone[i];
-                gone_next[i] = t + 1 < to ? missing[(t + 1) & 1][i] : 0;
+                gone_next[i] = missing[(t + 1) & 1][i];  // of no stage behind the last
             }
             const int page = look_up(t + 2);
             if (t + 1 < to) copy(t + 1);
             any_gone = __builtin_amdgcn_readfirstlane(any_gone);
             if (any_gone) {  // a weight of zero does not undo a NaN
-                for (int piece = threadIdx.x; piece < kStage * kPieces; piece += kThreads) {
-                    const int row = piece / kPieces;
-                    if (gone[row / 32] >> (row % 32) & 1) *reinterpret_cast<u32x4*>(stage + kSide + 16 * piece) = u32x4{0, 0, 0, 0};
-                }
+#pragma unroll
+                for (int i = 0; i < kSubs; ++i)
+                    for (int piece = threadIdx.x; piece < 32 * kPieces; piece += kThreads)
+                        if (gone[i] >> (piece / kPieces) & 1)
+                            *reinterpret_cast<u32x4*>(stage + kSide + 32 * i * kRowBytes + 16 * piece) = u32x4{0, 0, 0, 0};
                 __syncthreads();
             }
             const int last = base + kStage - 1;
