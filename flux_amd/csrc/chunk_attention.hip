@@ -10,6 +10,8 @@
 #include "serving.h"
 #include "serving_mfma.h"
 
+#include "prefill_limb.h"
+
 #include <type_traits>
 
 namespace flux {
@@ -114,6 +116,14 @@ struct Part {
     int request, tile, part, parts;
     int slot;   // of the part, when the tile is cut
     bool real;  // some request has it
+
+    // Its stages, of a tile's `count`.
+    __device__ __forceinline__ int from(int count) const {
+        return __builtin_amdgcn_readfirstlane(static_cast<int>(static_cast<int64_t>(count) * part / parts));
+    }
+    __device__ __forceinline__ int to(int count) const {
+        return __builtin_amdgcn_readfirstlane(static_cast<int>(static_cast<int64_t>(count) * (part + 1) / parts));
+    }
 };
 
 struct PlanShared {
@@ -130,8 +140,15 @@ __device__ __forceinline__ int64_t sum_of_block(int64_t v, int64_t* sums) {
     return sums[0] + sums[1] + sums[2] + sums[3];
 }
 
+// Parts lie in kStrips strips, from which the workgroups take one each in turn: what runs at the same time is then of all
+// requests, chunks that matrix instructions bound next to single tokens that memory does.
+#ifndef STRIPS
+#define STRIPS 64
+#endif
+constexpr int kStrips = STRIPS;
+
 template <int kRows, int kStage>
-__device__ Part part_of(const ChunkArgs& a, const ChunkPlan& plan, int unit, bool describes, Sequence& sequence) {
+__device__ Part part_of(const ChunkArgs& a, const ChunkPlan& plan, int place, bool describes, Sequence& sequence) {
     __shared__ PlanShared s;
     __shared__ int64_t work_sums[kWaves];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
@@ -154,48 +171,59 @@ __device__ Part part_of(const ChunkArgs& a, const ChunkPlan& plan, int unit, boo
         const int64_t even = (work + plan.target - 1) / plan.target;
         each = even < kLeastStages ? kLeastStages : (even < each ? static_cast<int>(even) : each);
     }
-    int units_before = 0, slots_before = 0, splits_before = 0;
-    bool found = false;
-    for (int base = 0; base < a.requests; base += kThreads) {
-        const int b = base + static_cast<int>(threadIdx.x);
-        if (plan.whole || a.requests > kThreads) look(b);
-        const int parts = stages > each ? (stages + each - 1) / each : 1;
-        const int units = tiles * parts;
-        const int slots = parts > 1 ? units : 0, splits = parts > 1 ? tiles : 0;
-        int units_to = wave_scan_int(units), slots_to = wave_scan_int(slots), splits_to = wave_scan_int(splits);
-        __syncthreads();
-        if (lane == 63) s.sums[0][wave] = units_to, s.sums[1][wave] = slots_to, s.sums[2][wave] = splits_to;
-        __syncthreads();
-        for (int w = 0; w < wave; ++w) units_to += s.sums[0][w], slots_to += s.sums[1][w], splits_to += s.sums[2][w];
-        units_to += units_before, slots_to += slots_before, splits_to += splits_before;
-        if (unit < units_to && unit >= units_to - units) {
-            const int local = unit - (units_to - units);
-            s.chosen[0] = b;
-            s.chosen[1] = local;
-            s.chosen[2] = parts;
-            // Offsets that decrease could name more rows than there are: what has no room is left out.
-            const int split = splits_to - splits + local / parts, slot = slots_to - slots + local;
-            const bool room = parts == 1 || (slot >= 0 && slot - local % parts + parts <= plan.slots && split >= 0 && split < plan.splits);
-            s.chosen[3] = room ? slot : -1;
-            if (describes && parts > 1 && room && local % parts == 0) {
-                int* d = reinterpret_cast<int*>(a.workspace) + kDescription * (1 + split);
-                const int row0 = (tiles - 1 - local / parts) * kRows, rows = mine.count * a.group - row0;
-                d[0] = mine.begin;
-                d[1] = row0;
-                d[2] = rows < kRows ? rows : kRows;
-                d[3] = slot;
-                d[4] = parts;
+    const bool one_round = a.requests <= kThreads;
+    int all_units = 0, all_splits = 0, unit = -1;
+    for (int round = one_round ? 1 : 0; round < 2; ++round) {  // the first one of two counts all parts
+        int units_before = 0, slots_before = 0, splits_before = 0;
+        for (int base = 0; base < a.requests; base += kThreads) {
+            const int b = base + static_cast<int>(threadIdx.x);
+            if (plan.whole || !one_round) look(b);
+            const int parts = stages > each ? (stages + each - 1) / each : 1;
+            const int units = tiles * parts;
+            const int slots = parts > 1 ? units : 0, splits = parts > 1 ? tiles : 0;
+            int units_to = wave_scan_int(units), slots_to = wave_scan_int(slots), splits_to = wave_scan_int(splits);
+            __syncthreads();
+            if (lane == 63) s.sums[0][wave] = units_to, s.sums[1][wave] = slots_to, s.sums[2][wave] = splits_to;
+            __syncthreads();
+            int units_here = 0, slots_here = 0, splits_here = 0;
+#pragma unroll
+            for (int w = 0; w < kWaves; ++w) {
+                if (w < wave) units_to += s.sums[0][w], slots_to += s.sums[1][w], splits_to += s.sums[2][w];
+                units_here += s.sums[0][w], slots_here += s.sums[1][w], splits_here += s.sums[2][w];
+            }
+            units_to += units_before, slots_to += slots_before, splits_to += splits_before;
+            units_before += units_here, slots_before += slots_here, splits_before += splits_here;
+            if (one_round) all_units = units_before, all_splits = splits_before;
+            if (round == 0) continue;
+            const int strip = (all_units + kStrips - 1) / kStrips;
+            unit = place / kStrips < strip ? place % kStrips * strip + place / kStrips : all_units;
+            if (unit < units_to && unit >= units_to - units) {
+                const int local = unit - (units_to - units);
+                // Offsets that decrease could name more rows than there are: what has no room is left out.
+                const int split = splits_to - splits + local / parts, slot = slots_to - slots + local;
+                const bool room = parts == 1 || (slot >= 0 && slot - local % parts + parts <= plan.slots && split >= 0 && split < plan.splits);
+                s.chosen[0] = b;
+                s.chosen[1] = local;
+                s.chosen[2] = parts;
+                s.chosen[3] = room ? slot : -1;
+                if (describes && parts > 1 && room && local % parts == 0) {
+                    int* d = reinterpret_cast<int*>(a.workspace) + kDescription * (1 + split);
+                    const int row0 = (tiles - 1 - local / parts) * kRows, rows = mine.count * a.group - row0;
+                    d[0] = mine.begin;
+                    d[1] = row0;
+                    d[2] = rows < kRows ? rows : kRows;
+                    d[3] = slot;
+                    d[4] = parts;
+                }
             }
         }
-        for (int w = 0; w < kWaves; ++w)
-            units_before += s.sums[0][w], slots_before += s.sums[1][w], splits_before += s.sums[2][w];
-        found = found || units_before > unit;
-        if (found && !(describes && unit == 0)) break;
+        all_units = units_before, all_splits = splits_before;
     }
-    if (describes && unit == 0 && threadIdx.x == 0 && !plan.whole) *reinterpret_cast<int*>(a.workspace) = splits_before < plan.splits ? splits_before : static_cast<int>(plan.splits);
+    if (describes && place == 0 && threadIdx.x == 0 && !plan.whole)
+        *reinterpret_cast<int*>(a.workspace) = all_splits < plan.splits ? all_splits : static_cast<int>(plan.splits);
     __syncthreads();
-    Part part{0, 0, 0, 1, 0, found};
-    if (!found) return part;
+    Part part{0, 0, 0, 1, 0, unit >= 0 && unit < all_units};
+    if (!part.real) return part;
     part.request = s.chosen[0];
     part.parts = s.chosen[2];
     part.part = s.chosen[1] % part.parts;
@@ -236,13 +264,18 @@ __device__ __forceinline__ Row row_of(const ChunkArgs& a, const Sequence& s, int
     return row;
 }
 
-// Weights of 16-bit types are 2^(s log2(e) - top) by one fused product, top = m log2(e) rounded: what that moves is common to
+// Weights are 2^(s log2(e) - top) by one fused product, top = m log2(e) rounded: what that moves is common to
 // all weights of a row and cancels, unless top is so large that it moves them out of float32's range.  From kFar on the
 // difference s - m is taken first.
 constexpr float kFar = 4194304.0f;
+// Of a weight relative to one of another maximum.
+__device__ __forceinline__ float exponent_of(float maximum, float other) {
+    const float scaled = other * kLog2e;
+    return fabsf(scaled) < kFar ? maximum * kLog2e - scaled : (maximum - other) * kLog2e;
+}
 
-// What the join needs to know of a part's row: the maximum that its weights refer to, in the exponent's unit (powers of two for
-// 16-bit types), its sum of weights, and the maximum of the scores.
+// What the join needs to know of a part's row: the maximum that its weights refer to, in powers of two, its sum of weights, and the
+// maximum of the scores.
 __device__ __forceinline__ void put_statistics(float* to, float top, float weight, float natural) {
     to[0] = top;
     to[1] = weight;
@@ -285,7 +318,7 @@ __device__ void exact_row(const ChunkArgs& a, const ChunkPlan& plan, const Seque
         }
         const float now = fmaxf(top, wave_max(score));
         const float reference = now == -INFINITY ? 0.0f : now, scaled = reference * kLog2e;
-        const bool near = sizeof(T) == 2 && fabsf(scaled) < kFar;
+        const bool near = fabsf(scaled) < kFar;
         auto difference = [&](float x) { return near ? fmaf(x, kLog2e, -scaled) : (x - reference) * kLog2e; };
         const float shrink = top == -INFINITY ? 0.0f : fast_exp2(near ? top * kLog2e - scaled : (top - reference) * kLog2e);
         top = now;
@@ -317,13 +350,19 @@ __device__ void exact_row(const ChunkArgs& a, const ChunkPlan& plan, const Seque
         if (partial) partial[d] = sum[c];
         else out[d] = static_cast<T>(weight == 0.0f ? 0.0f : sum[c] / weight);
     }
-    if (partial && lane == 0) put_statistics(partial + plan.width - 4, sizeof(T) == 2 ? top * kLog2e : top, weight, top);
+    if (partial && lane == 0) put_statistics(partial + plan.width - 4, top * kLog2e, weight, top);
 }
 
 // ---------------------------------------------------------------------------
-// float32: everything in registers; a workgroup's four waves split a tile's keys and join at the end.
+// float32 with the float32 matrix instruction: everything in registers; a workgroup's four waves split the keys of the rows
+// [row0, row0 + kRows) of a tile that starts at tile_row0, and join at the end.  `merge` holds merge_words<kDim>() words.
+template <int kDim>
+constexpr int merge_words() { return 2 * (rows_of_tile<float>(kDim) / 16) * (kDim / 4 + 2) * kWave; }
+
 template <int kDim, Rows kRowsRead>
-__global__ void __launch_bounds__(kThreads, kDim <= 64 ? 3 : (kDim <= 128 ? 2 : 1)) chunk_register_kernel(ChunkArgs a, ChunkPlan plan) {
+__device__ __forceinline__ void register_rows(const ChunkArgs& a, const ChunkPlan& plan, const Sequence& s, const Part& part, int kv_head,
+                                              int tile_row0, int row0, const KeyStages<stage_keys<float>(kDim)>& stages, int from, int to,
+                                              float* merge_memory) {
     using M = Mfma<float>;
     constexpr int kRows = rows_of_tile<float>(kDim);
     constexpr int kCols = kRows / 16;
@@ -334,27 +373,18 @@ __global__ void __launch_bounds__(kThreads, kDim <= 64 ? 3 : (kDim <= 128 ? 2 : 
     constexpr int kBlocks = kDim / 16;
     constexpr int kWords = kBlocks * 4 + 2;
     static_assert(kStage == kTile * kWaves, "a stage is one tile for each wave");
-    __shared__ float merge[2][kCols * kWords][kWave];
-
-    clear_other_rows<float>(a);
-    const int kv_head = blockIdx.x % a.kv_heads, unit = blockIdx.x / a.kv_heads;
-    Sequence s;
-    const Part part = part_of<kRows, kStage>(a, plan, unit, kv_head == 0, s);
-    if (!part.real) return;
+    auto merge = reinterpret_cast<float(*)[kCols * kWords][kWave]>(merge_memory);
     const int lane = threadIdx.x & 63;
     const int wave = threadIdx.x >> 6;
     const int n16 = lane & 15;
     const int g = lane >> 4;
-    const int row0 = part.tile * kRows, all_rows = s.count * a.group;
+    const int all_rows = s.count * a.group;
     const float* keys = static_cast<const float*>(a.key) + kv_head * a.key_strides[1];
     const float* values = static_cast<const float*>(a.value) + kv_head * a.value_strides[1];
     const int32_t* table = a.table + (s.slot < 0 ? 0 : s.slot) * a.table_stride;
 
     int first_p, last_p;
     positions_of(a, s, row0, kRows, first_p, last_p);
-    const KeyStages<kStage> stages(a, first_p, last_p);
-    const int from = static_cast<int>(static_cast<int64_t>(stages.count) * part.part / part.parts);
-    const int to = static_cast<int>(static_cast<int64_t>(stages.count) * (part.part + 1) / part.parts);
     Row mine[kCols];
     f32x4 query[kCols][kFragments];
     f32x4 out[kCols][kBlocks];
@@ -431,17 +461,19 @@ __global__ void __launch_bounds__(kThreads, kDim <= 64 ? 3 : (kDim <= 128 ? 2 : 
             highest = fmaxf(highest, __shfl_xor(highest, 32, kWave));
             if (__any(highest > top[c])) {
                 const float now = fmaxf(top[c], highest);
-                const float shrink = top[c] == -INFINITY ? 0.0f : fast_exp2((top[c] - now) * kLog2e);
+                const float shrink = top[c] == -INFINITY ? 0.0f : fast_exp2(exponent_of(top[c], now));
                 top[c] = now;
                 weight[c] *= shrink;
 #pragma unroll
                 for (int i = 0; i < kBlocks; ++i) out[c][i] *= shrink;
             }
             const float reference = top[c] == -INFINITY ? 0.0f : top[c];
+            const float scaled = reference * kLog2e;
+            const bool near = fabsf(scaled) < kFar;
             float p[1][4];
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-                p[0][i] = fast_exp2((score[i] - reference) * kLog2e);
+                p[0][i] = fast_exp2(near ? fmaf(score[i], kLog2e, -scaled) : (score[i] - reference) * kLog2e);
                 weight[c] += p[0][i];
             }
             f32x4 turned[1][4][kChunks];
@@ -485,8 +517,8 @@ __global__ void __launch_bounds__(kThreads, kDim <= 64 ? 3 : (kDim <= 128 ? 2 : 
                 const float(*other)[kWave] = merge[wave] + c * kWords;
                 const float other_top = other[kBlocks * 4][lane];
                 const float now = fmaxf(top[c], other_top);
-                const float mine_scale = top[c] == -INFINITY ? 0.0f : fast_exp2((top[c] - now) * kLog2e);
-                const float other_scale = other_top == -INFINITY ? 0.0f : fast_exp2((other_top - now) * kLog2e);
+                const float mine_scale = top[c] == -INFINITY ? 0.0f : fast_exp2(exponent_of(top[c], now));
+                const float other_scale = other_top == -INFINITY ? 0.0f : fast_exp2(exponent_of(other_top, now));
                 top[c] = now;
                 weight[c] = weight[c] * mine_scale + other[kBlocks * 4 + 1][lane] * other_scale;
 #pragma unroll
@@ -511,18 +543,35 @@ __global__ void __launch_bounds__(kThreads, kDim <= 64 ? 3 : (kDim <= 128 ? 2 : 
                     o[d] = mine[c].position < 0 || weight[c] == 0.0f ? 0.0f : out[c][k][j] / weight[c];
                 });
             } else {
-                float* o = part_row(a, plan, kv_head, part.slot, r - row0);
+                float* o = part_row(a, plan, kv_head, part.slot, r - tile_row0);
                 M::template each_dim<kDim>(g, a.dim, [&](int k, int j, int d) { o[d] = out[c][k][j]; });
                 const float highest = mine[c].position < 0 ? -INFINITY : top[c];
-                if (g == 0) put_statistics(o + plan.width - 4, highest, mine[c].position < 0 ? 0.0f : weight[c], highest);
+                if (g == 0) put_statistics(o + plan.width - 4, highest * kLog2e, mine[c].position < 0 ? 0.0f : weight[c], highest);
             }
         }
         while (again) {
             const int which = __ffs(again) - 1;
             again &= again - 1;
-            exact_row<float, kStage>(a, plan, s, part, kv_head, row0, row0 + 16 * c + which, stages, from, to, 0.0f);
+            exact_row<float, kStage>(a, plan, s, part, kv_head, tile_row0, row0 + 16 * c + which, stages, from, to, 0.0f);
         }
     }
+}
+
+template <int kDim, Rows kRowsRead>
+__global__ void __launch_bounds__(kThreads, kDim <= 64 ? 3 : (kDim <= 128 ? 2 : 1)) chunk_register_kernel(ChunkArgs a, ChunkPlan plan) {
+    constexpr int kRows = rows_of_tile<float>(kDim);
+    constexpr int kStage = stage_keys<float>(kDim);
+    __shared__ float merge[merge_words<kDim>()];
+    clear_other_rows<float>(a);
+    const int kv_head = blockIdx.x % a.kv_heads, unit = blockIdx.x / a.kv_heads;
+    Sequence s;
+    const Part part = part_of<kRows, kStage>(a, plan, unit, kv_head == 0, s);
+    if (!part.real) return;
+    const int row0 = part.tile * kRows;
+    int first_p, last_p;
+    positions_of(a, s, row0, kRows, first_p, last_p);
+    const KeyStages<kStage> stages(a, first_p, last_p);
+    register_rows<kDim, kRowsRead>(a, plan, s, part, kv_head, row0, row0, stages, part.from(stages.count), part.to(stages.count), merge);
 }
 
 // ---------------------------------------------------------------------------
@@ -626,8 +675,7 @@ __global__ void __launch_bounds__(kThreads, kDim <= 128 ? 2 : 1) chunk_tile_kern
     wave_first = __builtin_amdgcn_readfirstlane(wave_first);
     wave_last = __builtin_amdgcn_readfirstlane(wave_last);
     const KeyStages<kStage> stages(a, block_first, block_last);
-    const int from = __builtin_amdgcn_readfirstlane(static_cast<int>(static_cast<int64_t>(stages.count) * part.part / part.parts));
-    const int to = __builtin_amdgcn_readfirstlane(static_cast<int>(static_cast<int64_t>(stages.count) * (part.part + 1) / part.parts));
+    const int from = part.from(stages.count), to = part.to(stages.count);
 
     const char* keys = static_cast<const char*>(a.key) + 2 * kv_head * a.key_strides[1];
     const char* values = static_cast<const char*>(a.value) + 2 * kv_head * a.value_strides[1];
@@ -888,6 +936,309 @@ __global__ void __launch_bounds__(kThreads, kDim <= 128 ? 2 : 1) chunk_tile_kern
     }
 }
 
+// ---------------------------------------------------------------------------
+// float32 chunks of heads up to 64: products of three bf16 limbs, six of the nine (prefill_limb.h states what they carry), whose rate
+// is 16 / 6 times that of the float32 instruction, closer to 64 bits than that one's sums.  A workgroup's four waves take 32 rows each.
+// The threads fetch a stage's rows while the stage before is worked on, and split them into limbs on the way to LDS, where
+// each limb's rows lie as a 16-bit type's do below.  Scores are in powers of two: the query is multiplied by scale * log2(e).
+// Where limbs do not do (an infinity, a NaN, magnitudes of kLimbMaxScore or kLimbMaxValue on, scores of kFar on, sums so small that
+// bits are lacking) the tile is computed again by register_rows.
+// A score that is kFar or more: its own rounding shows, and the tile is left to register_rows as well.
+constexpr float kLimbMostScore = 0x1p60f;  // of a scaled query and of a key: no sum of 64 products overflows
+constexpr float kLimbMostValue = 0x1p19f;
+constexpr float kLimbLeastSum = 0x1p-82f;  // of a row, per 64 keys: bits below 2^-134 of each factor are under 2^-26 of it
+
+__device__ __forceinline__ bool beyond(const f32x4& a, const f32x4& b, float most) {
+    float m = 0.0f;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) m = __builtin_elementwise_maximum(m, __builtin_elementwise_maximum(fabsf(a[j]), fabsf(b[j])));  // keeps NaN
+    return !(m <= most);
+}
+
+template <bool kWide>
+__global__ void __launch_bounds__(kThreads, 2) chunk_limb_kernel(ChunkArgs a, ChunkPlan plan) {
+    constexpr int kDim = 64, kStage = 64, kRows = 32 * kWaves;
+    constexpr int kSteps = kDim / 16, kBlocks = kDim / 32, kSubs = kStage / 32, kPieces = kDim / 8;
+    constexpr int kRowBytes = kDim * 2, kPlane = kStage * kRowBytes, kSide = kLimbs * kPlane;
+    constexpr int kPerThread = kStage * kPieces / kThreads;  // pieces of eight dims, for each side
+    constexpr float kLazy = 4.0f;
+    __shared__ __attribute__((aligned(16))) char planes[2 * kSide];
+    __shared__ int64_t places[2][2][kStage];  // elements from the head's first, by stage parity
+    __shared__ uint32_t missing[2][kSubs];
+    static_assert(sizeof(float) * merge_words<kDim>() <= sizeof(planes), "register_rows uses the planes");
+
+    clear_other_rows<float>(a);
+    const int kv_head = blockIdx.x % a.kv_heads, unit = blockIdx.x / a.kv_heads;
+    Sequence s;
+    const Part part = part_of<kRows, kStage>(a, plan, unit, kv_head == 0, s);
+    if (!part.real) return;
+    const int lane = threadIdx.x & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int n32 = lane & 31;
+    const int half = lane >> 5;
+    const int row0 = part.tile * kRows, all_rows = s.count * a.group, wave_row = row0 + wave * 32;
+    int block_first, block_last, wave_first, wave_last;
+    positions_of(a, s, row0, kRows, block_first, block_last);
+    positions_of(a, s, wave_row, 32, wave_first, wave_last);
+    wave_first = __builtin_amdgcn_readfirstlane(wave_first);
+    wave_last = __builtin_amdgcn_readfirstlane(wave_last);
+    const KeyStages<kStage> stages(a, block_first, block_last);
+    const int from = part.from(stages.count), to = part.to(stages.count);
+
+    const float* keys = static_cast<const float*>(a.key) + kv_head * a.key_strides[1];
+    const float* values = static_cast<const float*>(a.value) + kv_head * a.value_strides[1];
+    const int32_t* table = a.table + (s.slot < 0 ? 0 : s.slot) * a.table_stride;
+    const int r = wave_row + n32;  // this lane's row
+    const bool real = r < all_rows;
+    const int index = static_cast<int>(divide(real ? r : row0, a.group_of)), head = kv_head * a.group + (real ? r : row0) - index * a.group;
+    const Row mine = row_of(a, s, r);
+    f32x16 out[2 * kBlocks];  // then the sums of the small products
+#pragma unroll
+    for (int i = 0; i < 2 * kBlocks; ++i)
+#pragma unroll
+        for (int j = 0; j < 16; ++j) out[i][j] = 0.0f;
+    float top = -INFINITY, weight = 0.0f;
+    bool unsure = false;
+
+    if (from < to) {
+        u32x4 query[kSteps][kLimbs];
+        {
+            const float* q = static_cast<const float*>(a.query) + static_cast<int64_t>(s.begin + index) * a.query_strides[0] + head * a.query_strides[1];
+            const float factor = a.scale * kLog2e;
+#pragma unroll
+            for (int k = 0; k < kSteps; ++k) {
+                f32x4 four[2];
+#pragma unroll
+                for (int j = 0; j < 2; ++j) {
+                    const int d = 16 * k + 8 * half + 4 * j;
+                    if (a.query_wide) four[j] = *reinterpret_cast<const f32x4*>(q + (d < a.dim ? d : 0));
+                    else four[j] = Mfma<float>::load_strided(q, a.query_strides[2], d, a.dim);
+                    four[j] = Mfma<float>::zero_behind(four[j], d, real ? a.dim : 0) * factor;
+                }
+                unsure |= beyond(four[0], four[1], kLimbMostScore);
+                const Limbs8 limbs = split8(four[0], four[1]);
+#pragma unroll
+                for (int l = 0; l < kLimbs; ++l) query[k][l] = limbs.limb[l];
+            }
+        }
+        auto low_of = [&](int p) { return a.window > 0 && p >= a.window ? p - a.window + 1 : 0; };
+
+        // Threads below kStage look up one key each.  Rows behind the last key repeat it; keys on no page are the pool's first.
+        auto position_of = [&](int t) {
+            const int position = stages.base(t) + static_cast<int>(threadIdx.x);
+            return position < stages.seen ? position : stages.seen - 1;
+        };
+        auto look_up = [&](int t) {
+            return t < to && static_cast<int>(threadIdx.x) < kStage ? table[divide(position_of(t), a.page)] : 0;
+        };
+        auto put_places = [&](int t, int page) {
+            if (t >= to || static_cast<int>(threadIdx.x) >= kStage) return;
+            const int position = position_of(t);
+            const bool held = page >= 0 && page < a.pages;
+            const int64_t of_page = held ? page : 0;
+            const int in_page = held ? position - static_cast<int>(divide(position, a.page) * a.page.divisor) : 0;
+            places[t & 1][0][threadIdx.x] = of_page * a.key_strides[0] + in_page * a.key_strides[2];
+            places[t & 1][1][threadIdx.x] = of_page * a.value_strides[0] + in_page * a.value_strides[2];
+            const uint64_t gone = __ballot(!held);
+            if (lane == 0) missing[t & 1][0] = static_cast<uint32_t>(gone);
+            if (lane == 32) missing[t & 1][1] = static_cast<uint32_t>(gone >> 32);
+        };
+        f32x4 held[2][kPerThread][2];  // of this thread's pieces: row threadIdx.x / kPieces + 32 i, piece threadIdx.x % kPieces
+        const int piece = threadIdx.x % kPieces, piece_row = threadIdx.x / kPieces;
+        auto fetch = [&](int t) {
+#pragma unroll
+            for (int side = 0; side < 2; ++side)
+#pragma unroll
+                for (int i = 0; i < kPerThread; ++i) {
+                    const float* row = (side ? values : keys) + places[t & 1][side][piece_row + 32 * i];
+#pragma unroll
+                    for (int j = 0; j < 2; ++j) {
+                        const int d = 8 * piece + 4 * j;  // dims behind the head's: its first, which meet zeros or are not stored
+                        if constexpr (kWide) held[side][i][j] = *reinterpret_cast<const f32x4*>(row + (d < a.dim ? d : 0));
+                        else held[side][i][j] = Mfma<float>::load_strided(row, 1, d, a.dim);
+                    }
+                }
+        };
+        auto put = [&](const uint32_t (&gone)[kSubs]) {
+#pragma unroll
+            for (int side = 0; side < 2; ++side)
+#pragma unroll
+                for (int i = 0; i < kPerThread; ++i) {
+                    const int row = piece_row + 32 * i;
+                    if (gone[i] >> piece_row & 1) held[side][i][0] = held[side][i][1] = f32x4{0, 0, 0, 0};
+                    unsure |= beyond(held[side][i][0], held[side][i][1], side ? kLimbMostValue : kLimbMostScore);
+                    const Limbs8 limbs = split8(held[side][i][0], held[side][i][1]);
+                    char* at = planes + side * kSide + row * kRowBytes + (piece ^ swizzle<kDim>(row)) * 16;
+#pragma unroll
+                    for (int l = 0; l < kLimbs; ++l) *reinterpret_cast<u32x4*>(at + l * kPlane) = limbs.limb[l];
+                }
+        };
+        int key_at[kSteps], value_at[kBlocks][2];
+#pragma unroll
+        for (int k = 0; k < kSteps; ++k) key_at[k] = n32 * kRowBytes + (((2 * k + half) ^ swizzle<kDim>(n32)) * 16);
+#pragma unroll
+        for (int b = 0; b < kBlocks; ++b)
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+                const int row = 8 * e + 4 * half + (lane & 15) / 4, at = 4 * b + 2 * (lane >> 4 & 1) + (lane & 3) / 2;
+                value_at[b][e] = kSide + row * kRowBytes + (at ^ swizzle<kDim>(row)) * 16 + 8 * (lane & 1);
+            }
+
+        const int wave_low = low_of(wave_first), low_of_last = low_of(wave_last);
+        auto work = [&](const char* at, int first, uint32_t gone, auto masked) {
+            f32x16 score;
+#pragma unroll
+            for (int j = 0; j < 16; ++j) score[j] = 0.0f;
+            u32x4 lead[kSteps];
+#pragma unroll
+            for (int k = 0; k < kSteps; ++k) {  // the small products first
+                lead[k] = *reinterpret_cast<const u32x4*>(at + key_at[k]);
+                const u32x4 middle = *reinterpret_cast<const u32x4*>(at + key_at[k] + kPlane);
+                const u32x4 last = *reinterpret_cast<const u32x4*>(at + key_at[k] + 2 * kPlane);
+                score = mfma_bf16(last, query[k][0], score);
+                score = mfma_bf16(lead[k], query[k][2], score);
+                score = mfma_bf16(middle, query[k][1], score);
+                score = mfma_bf16(middle, query[k][0], score);
+                score = mfma_bf16(lead[k], query[k][1], score);
+            }
+#pragma unroll
+            for (int k = 0; k < kSteps; ++k) score = mfma_bf16(lead[k], query[k][0], score);
+            if constexpr (decltype(masked)::value) {
+#pragma unroll
+                for (int j = 0; j < 16; ++j) {
+                    // Without branches: low <= key <= position as one unsigned comparison, or a sink.
+                    const int in = 8 * (j / 4) + 4 * half + j % 4, of = first + in;
+                    const bool visible = ((static_cast<uint32_t>(of - mine.low) <= static_cast<uint32_t>(mine.position - mine.low)) |
+                                          (of < mine.sink_end)) & !(gone >> in & 1);
+                    score[j] = visible ? score[j] : -INFINITY;
+                }
+            }
+            float highest = fmaxf(score[0], score[1]);
+#pragma unroll
+            for (int j = 2; j < 16; j += 2) highest = fmaxf(fmaxf(highest, score[j]), score[j + 1]);
+            highest = half_max(highest);
+            const bool moves = __any(highest - top > kLazy);  // NaN where both are -inf
+            float shrink = 1.0f;
+            if (moves) {
+                const float now = fmaxf(top, highest);
+                shrink = top == -INFINITY ? 0.0f : fast_exp2(top - now);
+                top = now;
+                weight *= shrink;
+            }
+            scale_if<2 * kBlocks>(moves, shrink, out);
+            const float reference = top == -INFINITY ? 0.0f : top;
+#pragma unroll
+            for (int k = 0; k < 2; ++k) {
+                f32x4 p[2];
+#pragma unroll
+                for (int j = 0; j < 8; ++j) {
+                    p[j / 4][j % 4] = fast_exp2(score[8 * k + j] - reference);
+                    weight += p[j / 4][j % 4];
+                }
+                const Limbs8 limbs = split8(p[0], p[1]);
+                u32x4 value[kBlocks][kLimbs];
+#pragma unroll
+                for (int b = 0; b < kBlocks; ++b)
+#pragma unroll
+                    for (int l = 0; l < kLimbs; ++l) {
+                        const u32x2 low = read_transposed(at + value_at[b][0] + l * kPlane + 16 * k * kRowBytes);
+                        const u32x2 high = read_transposed(at + value_at[b][1] + l * kPlane + 16 * k * kRowBytes);
+                        value[b][l] = u32x4{low[0], low[1], high[0], high[1]};
+                    }
+#pragma unroll
+                for (int b = 0; b < kBlocks; ++b) out[kBlocks + b] = mfma_bf16(value[b][2], limbs.limb[0], out[kBlocks + b]);
+#pragma unroll
+                for (int b = 0; b < kBlocks; ++b) out[kBlocks + b] = mfma_bf16(value[b][0], limbs.limb[2], out[kBlocks + b]);
+#pragma unroll
+                for (int b = 0; b < kBlocks; ++b) out[kBlocks + b] = mfma_bf16(value[b][1], limbs.limb[1], out[kBlocks + b]);
+#pragma unroll
+                for (int b = 0; b < kBlocks; ++b) out[kBlocks + b] = mfma_bf16(value[b][1], limbs.limb[0], out[kBlocks + b]);
+#pragma unroll
+                for (int b = 0; b < kBlocks; ++b) out[kBlocks + b] = mfma_bf16(value[b][0], limbs.limb[1], out[kBlocks + b]);
+#pragma unroll
+                for (int b = 0; b < kBlocks; ++b) out[b] = mfma_bf16(value[b][0], limbs.limb[0], out[b]);
+            }
+        };
+
+        put_places(from, look_up(from));
+        put_places(from + 1, look_up(from + 1));
+        __syncthreads();
+        uint32_t gone[kSubs];
+#pragma unroll
+        for (int i = 0; i < kSubs; ++i) gone[i] = missing[from & 1][i];
+        fetch(from);
+        for (int t = from; t < to; ++t) {
+            __syncthreads();  // the stage before has been read
+            put(gone);
+            const int page = look_up(t + 2);
+            __syncthreads();
+            uint32_t next[kSubs];
+#pragma unroll
+            for (int i = 0; i < kSubs; ++i) next[i] = missing[(t + 1) & 1][i];  // of no stage behind the last
+            if (t + 1 < to) fetch(t + 1);
+            const uint32_t any_gone = __builtin_amdgcn_readfirstlane(gone[0] | gone[1]);
+            const int base = stages.base(t), last = base + kStage - 1;
+            const bool seen = base <= wave_last && (last >= wave_low || base < a.sinks);
+            if (seen && !any_gone && base >= low_of_last && last <= wave_first) {  // all of it, by all rows
+#pragma unroll
+                for (int i = 0; i < kSubs; ++i) work(planes + 32 * i * kRowBytes, base + 32 * i, 0, std::false_type{});
+            } else if (seen) {
+#pragma unroll 1
+                for (int i = 0; i < kSubs; ++i) {
+                    const int first = base + 32 * i;
+                    if (first > wave_last || (first + 31 < wave_low && first >= a.sinks)) continue;
+                    work(planes + 32 * i * kRowBytes, first, gone[i], std::true_type{});
+                }
+            }
+#pragma unroll
+            for (int i = 0; i < kSubs; ++i) gone[i] = next[i];
+            put_places(t + 2, page);
+        }
+    }
+
+    weight = half_sum(weight);
+    unsigned least = ~0u;
+#pragma unroll
+    for (int b = 0; b < kBlocks; ++b)
+#pragma unroll
+        for (int j = 0; j < 16; ++j) {
+            out[b][j] += out[kBlocks + b][j];
+            least = min(least, magnitude_key(out[b][j]));
+        }
+    unsure |= least < magnitude_key(kLimbLeastSum * static_cast<float>(to - from + 1));
+    unsure |= mine.position >= 0 && top != -INFINITY && !(fabsf(top) < kFar);
+    if (__syncthreads_or(unsure)) {
+        for (int row = row0; row < row0 + kRows && row < all_rows; row += rows_of_tile<float>(kDim)) {
+            register_rows<kDim, kWide ? kWideRows : kNarrow>(a, plan, s, part, kv_head, row0, row, stages, from, to, reinterpret_cast<float*>(planes));
+            __syncthreads();
+        }
+        return;
+    }
+    if (!real) return;
+    const bool cut = part.parts > 1;
+    float* o = cut ? part_row(a, plan, kv_head, part.slot, r - row0)
+                   : static_cast<float*>(a.out) + (static_cast<int64_t>(s.begin + index) * a.query_heads + head) * a.dim;
+    const float inverse = cut ? 1.0f : (weight == 0.0f || mine.position < 0 ? 0.0f : 1.0f / weight);
+#pragma unroll
+    for (int b = 0; b < kBlocks; ++b)
+#pragma unroll
+        for (int j = 0; j < 16; j += 4) {
+            const int d = 32 * b + 2 * j + 4 * half;  // four dims side by side
+            const f32x4 four = {out[b][j] * inverse, out[b][j + 1] * inverse, out[b][j + 2] * inverse, out[b][j + 3] * inverse};
+            if (kWide || cut) {
+                if (d < a.dim) *reinterpret_cast<f32x4*>(o + d) = four;
+            } else {
+#pragma unroll
+                for (int l = 0; l < 4; ++l)
+                    if (d + l < a.dim) o[d + l] = four[l];
+            }
+        }
+    if (cut && half == 0) {
+        const float highest = mine.position < 0 ? -INFINITY : top;
+        put_statistics(o + plan.width - 4, highest, mine.position < 0 ? 0.0f : weight, highest / kLog2e);
+    }
+}
+
 // Joins the parts of a tile that was cut.  Workgroup (cut tile, KV head, every gridDim.z-th 256 fours of dims).
 template <class T>
 __global__ void __launch_bounds__(kThreads) chunk_join_kernel(ChunkArgs a, ChunkPlan plan) {
@@ -908,7 +1259,7 @@ __global__ void __launch_bounds__(kThreads) chunk_join_kernel(ChunkArgs a, Chunk
         for (int p = 0; p < parts; ++p) {
             const float part_top = of[p * stride], part_weight = of[p * stride + 1];
             if (part_weight == 0.0f) continue;  // such a part's sums are zeros, or it saw nothing
-            const bool near = sizeof(T) == 2 && fabsf(top) < kFar && fabsf(part_top) < kFar;
+            const bool near = fabsf(top) < kFar && fabsf(part_top) < kFar;
             const float share = fast_exp2(near ? part_top - top : (of[p * stride + 2] - natural) * kLog2e);
             weight += part_weight * share;
             sum += *reinterpret_cast<const f32x4*>(o + p * stride + 4 * four) * share;
@@ -922,16 +1273,22 @@ __global__ void __launch_bounds__(kThreads) chunk_join_kernel(ChunkArgs a, Chunk
 }
 
 // Parts of a step: two workgroups on each of 256 CUs.
+#ifndef LIMB_ROWS
+#define LIMB_ROWS 64
+#endif
 #ifndef TARGET
-#define TARGET 512
+#define TARGET 1024
 #endif
 constexpr int kTarget = TARGET;
+
+// Whether float32 takes the limb kernel.
+bool by_limbs(const ChunkArgs& a) { return a.dim <= 64 && a.tokens * a.group >= LIMB_ROWS * a.requests; }
 
 template <class T>
 ChunkPlan plan_of(const ChunkArgs& a) {
     const int dim = padded_dim(a.dim);
     ChunkPlan p{};
-    p.rows = rows_of_tile<T>(dim);
+    p.rows = sizeof(T) == 4 && by_limbs(a) ? 32 * kWaves : rows_of_tile<T>(dim);
     const int stage = stage_keys<T>(dim);
     const int64_t rows = a.tokens * a.group;
     p.tiles = rows / p.rows + a.requests;
@@ -972,6 +1329,13 @@ hipError_t launch_tiles(const ChunkArgs& a, const ChunkPlan& plan, dim3 grid, hi
         if (a.wide && reinterpret_cast<uintptr_t>(a.out) % 8 == 0) return launch(chunk_tile_kernel<T, kDim, true>);
         return launch(chunk_tile_kernel<T, kDim, false>);
     } else {
+        if constexpr (kDim == 64) {
+            if (by_limbs(a)) {
+                if (a.wide && reinterpret_cast<uintptr_t>(a.out) % 16 == 0) hipLaunchKernelGGL(chunk_limb_kernel<true>, grid, dim3(kThreads), 0, stream, a, plan);
+                else hipLaunchKernelGGL(chunk_limb_kernel<false>, grid, dim3(kThreads), 0, stream, a, plan);
+                return hipGetLastError();
+            }
+        }
         if (a.wide && a.dim == kDim) hipLaunchKernelGGL(HIP_KERNEL_NAME(chunk_register_kernel<kDim, kFullRows>), grid, dim3(kThreads), 0, stream, a, plan);
         else if (a.wide) hipLaunchKernelGGL(HIP_KERNEL_NAME(chunk_register_kernel<kDim, kWideRows>), grid, dim3(kThreads), 0, stream, a, plan);
         else hipLaunchKernelGGL(HIP_KERNEL_NAME(chunk_register_kernel<kDim, kNarrow>), grid, dim3(kThreads), 0, stream, a, plan);
@@ -982,7 +1346,7 @@ hipError_t launch_tiles(const ChunkArgs& a, const ChunkPlan& plan, dim3 grid, hi
 template <class T>
 hipError_t launch_chunks(const ChunkArgs& a, hipStream_t stream) {
     const ChunkPlan plan = plan_of<T>(a);
-    const int64_t blocks = plan.units * a.kv_heads;
+    const int64_t blocks = (plan.units + kStrips - 1) * a.kv_heads;
     if (blocks >= (int64_t{1} << 24)) return hipErrorInvalidValue;  // a grid has below 2^32 threads
     const dim3 grid(static_cast<uint32_t>(blocks));
     hipError_t launched;
