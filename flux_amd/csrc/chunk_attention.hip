@@ -224,14 +224,21 @@ __device__ Part part_of(const ChunkArgs& a, const ChunkPlan& plan, int place, bo
     __syncthreads();
     Part part{0, 0, 0, 1, 0, unit >= 0 && unit < all_units};
     if (!part.real) return part;
-    part.request = s.chosen[0];
-    part.parts = s.chosen[2];
-    part.part = s.chosen[1] % part.parts;
-    part.slot = s.chosen[3];
+    auto same = [](int v) { return __builtin_amdgcn_readfirstlane(v); };  // in all lanes
+    part.request = same(s.chosen[0]);
+    part.parts = same(s.chosen[2]);
+    const int local = same(s.chosen[1]);
+    part.part = local % part.parts;
+    part.slot = same(s.chosen[3]);
     part.real = part.slot >= 0;
     sequence = sequence_of(a, part.request);
+    sequence.begin = same(sequence.begin);
+    sequence.count = same(sequence.count);
+    sequence.n = same(sequence.n);
+    sequence.start = same(sequence.start);
+    sequence.slot = static_cast<int64_t>(same(static_cast<int>(sequence.slot >> 32))) << 32 | static_cast<uint32_t>(same(static_cast<int>(sequence.slot)));
     // The longest tiles first.
-    part.tile = static_cast<int>((static_cast<int64_t>(sequence.count) * a.group + kRows - 1) / kRows) - 1 - s.chosen[1] / part.parts;
+    part.tile = static_cast<int>((static_cast<int64_t>(sequence.count) * a.group + kRows - 1) / kRows) - 1 - local / part.parts;
     return part;
 }
 
@@ -992,9 +999,9 @@ __global__ void __launch_bounds__(kThreads, 2) chunk_limb_kernel(ChunkArgs a, Ch
     const bool real = r < all_rows;
     const int index = static_cast<int>(divide(real ? r : row0, a.group_of)), head = kv_head * a.group + (real ? r : row0) - index * a.group;
     const Row mine = row_of(a, s, r);
-    f32x16 out[2 * kBlocks];  // then the sums of the small products
+    f32x16 out[kBlocks];
 #pragma unroll
-    for (int i = 0; i < 2 * kBlocks; ++i)
+    for (int i = 0; i < kBlocks; ++i)
 #pragma unroll
         for (int j = 0; j < 16; ++j) out[i][j] = 0.0f;
     float top = -INFINITY, weight = 0.0f;
@@ -1125,7 +1132,7 @@ __global__ void __launch_bounds__(kThreads, 2) chunk_limb_kernel(ChunkArgs a, Ch
                 top = now;
                 weight *= shrink;
             }
-            scale_if<2 * kBlocks>(moves, shrink, out);
+            scale_if<kBlocks>(moves, shrink, out);
             const float reference = top == -INFINITY ? 0.0f : top;
 #pragma unroll
             for (int k = 0; k < 2; ++k) {
@@ -1146,15 +1153,15 @@ __global__ void __launch_bounds__(kThreads, 2) chunk_limb_kernel(ChunkArgs a, Ch
                         value[b][l] = u32x4{low[0], low[1], high[0], high[1]};
                     }
 #pragma unroll
-                for (int b = 0; b < kBlocks; ++b) out[kBlocks + b] = mfma_bf16(value[b][2], limbs.limb[0], out[kBlocks + b]);
+                for (int b = 0; b < kBlocks; ++b) out[b] = mfma_bf16(value[b][2], limbs.limb[0], out[b]);
 #pragma unroll
-                for (int b = 0; b < kBlocks; ++b) out[kBlocks + b] = mfma_bf16(value[b][0], limbs.limb[2], out[kBlocks + b]);
+                for (int b = 0; b < kBlocks; ++b) out[b] = mfma_bf16(value[b][0], limbs.limb[2], out[b]);
 #pragma unroll
-                for (int b = 0; b < kBlocks; ++b) out[kBlocks + b] = mfma_bf16(value[b][1], limbs.limb[1], out[kBlocks + b]);
+                for (int b = 0; b < kBlocks; ++b) out[b] = mfma_bf16(value[b][1], limbs.limb[1], out[b]);
 #pragma unroll
-                for (int b = 0; b < kBlocks; ++b) out[kBlocks + b] = mfma_bf16(value[b][1], limbs.limb[0], out[kBlocks + b]);
+                for (int b = 0; b < kBlocks; ++b) out[b] = mfma_bf16(value[b][1], limbs.limb[0], out[b]);
 #pragma unroll
-                for (int b = 0; b < kBlocks; ++b) out[kBlocks + b] = mfma_bf16(value[b][0], limbs.limb[1], out[kBlocks + b]);
+                for (int b = 0; b < kBlocks; ++b) out[b] = mfma_bf16(value[b][0], limbs.limb[1], out[b]);
 #pragma unroll
                 for (int b = 0; b < kBlocks; ++b) out[b] = mfma_bf16(value[b][0], limbs.limb[0], out[b]);
             }
@@ -1202,7 +1209,6 @@ __global__ void __launch_bounds__(kThreads, 2) chunk_limb_kernel(ChunkArgs a, Ch
     for (int b = 0; b < kBlocks; ++b)
 #pragma unroll
         for (int j = 0; j < 16; ++j) {
-            out[b][j] += out[kBlocks + b][j];
             least = min(least, magnitude_key(out[b][j]));
         }
     unsure |= least < magnitude_key(kLimbLeastSum * static_cast<float>(to - from + 1));
