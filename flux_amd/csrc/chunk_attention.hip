@@ -19,7 +19,10 @@ namespace {
 
 constexpr int kThreads = 256;
 constexpr int kWaves = 4;
-constexpr int kLeastStages = 4;  // that are worth a workgroup
+// Stages that are worth a workgroup, and below which no tile is cut, which saves the join's launch.
+template <class T>
+constexpr int least_stages() { return sizeof(T) == 2 ? 4 : 1; }
+constexpr int kWholeStages = 4;
 
 template <class T>
 constexpr int rows_of_tile(int dim) { return sizeof(T) == 2 ? 32 * kWaves : (dim <= 128 ? 32 : 16); }
@@ -33,6 +36,7 @@ struct ChunkPlan {
     int64_t tiles;     // at most, of one KV head
     int target;        // parts of one KV head that a step's work is cut into
     bool whole;        // no tile is cut
+    int least;         // stages of a part, but for a tile's shorter ones
     int64_t units;     // parts and whole tiles, at most, of one KV head
     int64_t slots;     // parts of cut tiles, at most, of one KV head
     int64_t splits;    // cut tiles, at most
@@ -129,6 +133,8 @@ struct Part {
 struct PlanShared {
     int sums[3][kWaves];
     int chosen[4];
+    Sequence sequence;
+    int first_row, behind;  // of the requests' tokens
 };
 
 __device__ __forceinline__ int64_t sum_of_block(int64_t v, int64_t* sums) {
@@ -140,6 +146,18 @@ __device__ __forceinline__ int64_t sum_of_block(int64_t v, int64_t* sums) {
     return sums[0] + sums[1] + sums[2] + sums[3];
 }
 
+// Rows before the first request and behind the last are zeros.
+template <class T>
+__device__ __forceinline__ void clear_other_rows(const ChunkArgs& a, int before, int behind) {
+    const int64_t others = before + a.tokens - behind;
+    const int width = a.query_heads * a.dim;
+    T* out = static_cast<T*>(a.out);
+    for (int64_t i = blockIdx.x; i < others; i += gridDim.x) {
+        T* row = out + (i < before ? i : behind + i - before) * width;
+        for (int d = threadIdx.x; d < width; d += kThreads) row[d] = static_cast<T>(0.0f);
+    }
+}
+
 // Parts lie in kStrips strips, from which the workgroups take one each in turn: what runs at the same time is then of all
 // requests, chunks that matrix instructions bound next to single tokens that memory does.
 #ifndef STRIPS
@@ -147,7 +165,7 @@ __device__ __forceinline__ int64_t sum_of_block(int64_t v, int64_t* sums) {
 #endif
 constexpr int kStrips = STRIPS;
 
-template <int kRows, int kStage>
+template <class T, int kRows, int kStage>
 __device__ Part part_of(const ChunkArgs& a, const ChunkPlan& plan, int place, bool describes, Sequence& sequence) {
     __shared__ PlanShared s;
     __shared__ int64_t work_sums[kWaves];
@@ -160,6 +178,8 @@ __device__ Part part_of(const ChunkArgs& a, const ChunkPlan& plan, int place, bo
         mine = sequence_of(a, b);
         tiles = static_cast<int>((static_cast<int64_t>(mine.count) * a.group + kRows - 1) / kRows);
         stages = most_stages<kRows, kStage>(a, mine);
+        if (b == 0) s.first_row = mine.begin;
+        if (b == a.requests - 1) s.behind = mine.begin + mine.count;
     };
     int each = 1 << 30;
     if (!plan.whole) {
@@ -169,7 +189,7 @@ __device__ Part part_of(const ChunkArgs& a, const ChunkPlan& plan, int place, bo
             work += sum_of_block(static_cast<int64_t>(tiles) * stages, work_sums);
         }
         const int64_t even = (work + plan.target - 1) / plan.target;
-        each = even < kLeastStages ? kLeastStages : (even < each ? static_cast<int>(even) : each);
+        each = even < plan.least ? plan.least : (even < each ? static_cast<int>(even) : each);
     }
     const bool one_round = a.requests <= kThreads;
     int all_units = 0, all_splits = 0, unit = -1;
@@ -206,6 +226,7 @@ __device__ Part part_of(const ChunkArgs& a, const ChunkPlan& plan, int place, bo
                 s.chosen[1] = local;
                 s.chosen[2] = parts;
                 s.chosen[3] = room ? slot : -1;
+                s.sequence = mine;
                 if (describes && parts > 1 && room && local % parts == 0) {
                     int* d = reinterpret_cast<int*>(a.workspace) + kDescription * (1 + split);
                     const int row0 = (tiles - 1 - local / parts) * kRows, rows = mine.count * a.group - row0;
@@ -222,6 +243,7 @@ __device__ Part part_of(const ChunkArgs& a, const ChunkPlan& plan, int place, bo
     if (describes && place == 0 && threadIdx.x == 0 && !plan.whole)
         *reinterpret_cast<int*>(a.workspace) = all_splits < plan.splits ? all_splits : static_cast<int>(plan.splits);
     __syncthreads();
+    clear_other_rows<T>(a, s.first_row, s.behind);
     Part part{0, 0, 0, 1, 0, unit >= 0 && unit < all_units};
     if (!part.real) return part;
     auto same = [](int v) { return __builtin_amdgcn_readfirstlane(v); };  // in all lanes
@@ -231,7 +253,7 @@ __device__ Part part_of(const ChunkArgs& a, const ChunkPlan& plan, int place, bo
     part.part = local % part.parts;
     part.slot = same(s.chosen[3]);
     part.real = part.slot >= 0;
-    sequence = sequence_of(a, part.request);
+    sequence = s.sequence;
     sequence.begin = same(sequence.begin);
     sequence.count = same(sequence.count);
     sequence.n = same(sequence.n);
@@ -240,20 +262,6 @@ __device__ Part part_of(const ChunkArgs& a, const ChunkPlan& plan, int place, bo
     // The longest tiles first.
     part.tile = static_cast<int>((static_cast<int64_t>(sequence.count) * a.group + kRows - 1) / kRows) - 1 - local / part.parts;
     return part;
-}
-
-// Rows before the first request and behind the last are zeros.
-template <class T>
-__device__ __forceinline__ void clear_other_rows(const ChunkArgs& a) {
-    const int64_t from = a.offsets[0], to = a.offsets[a.requests];
-    const int64_t before = from < 0 ? 0 : (from < a.tokens ? from : a.tokens), behind = to < 0 ? 0 : (to < a.tokens ? to : a.tokens);
-    const int64_t others = before + a.tokens - behind;
-    const int width = a.query_heads * a.dim;
-    T* out = static_cast<T*>(a.out);
-    for (int64_t i = blockIdx.x; i < others; i += gridDim.x) {
-        T* row = out + (i < before ? i : behind + i - before) * width;
-        for (int d = threadIdx.x; d < width; d += kThreads) row[d] = static_cast<T>(0.0f);
-    }
 }
 
 // This lane's row of the tile.
@@ -569,10 +577,9 @@ __global__ void __launch_bounds__(kThreads, kDim <= 64 ? 3 : (kDim <= 128 ? 2 : 
     constexpr int kRows = rows_of_tile<float>(kDim);
     constexpr int kStage = stage_keys<float>(kDim);
     __shared__ float merge[merge_words<kDim>()];
-    clear_other_rows<float>(a);
     const int kv_head = blockIdx.x % a.kv_heads, unit = blockIdx.x / a.kv_heads;
     Sequence s;
-    const Part part = part_of<kRows, kStage>(a, plan, unit, kv_head == 0, s);
+    const Part part = part_of<float, kRows, kStage>(a, plan, unit, kv_head == 0, s);
     if (!part.real) return;
     const int row0 = part.tile * kRows;
     int first_p, last_p;
@@ -666,10 +673,9 @@ __global__ void __launch_bounds__(kThreads, kDim <= 128 ? 2 : 1) chunk_tile_kern
     __shared__ int64_t places[2][2][kStage];   // bytes from the head's first, by stage parity
     __shared__ uint32_t missing[2][kSubs];     // keys of a stage that are on no page
 
-    clear_other_rows<T>(a);
     const int kv_head = blockIdx.x % a.kv_heads, unit = blockIdx.x / a.kv_heads;
     Sequence s;
-    const Part part = part_of<kRows, kStage>(a, plan, unit, kv_head == 0, s);
+    const Part part = part_of<T, kRows, kStage>(a, plan, unit, kv_head == 0, s);
     if (!part.real) return;
     const int lane = threadIdx.x & 63;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -974,10 +980,9 @@ __global__ void __launch_bounds__(kThreads, 2) chunk_limb_kernel(ChunkArgs a, Ch
     __shared__ uint32_t missing[2][kSubs];
     static_assert(sizeof(float) * merge_words<kDim>() <= sizeof(planes), "register_rows uses the planes");
 
-    clear_other_rows<float>(a);
     const int kv_head = blockIdx.x % a.kv_heads, unit = blockIdx.x / a.kv_heads;
     Sequence s;
-    const Part part = part_of<kRows, kStage>(a, plan, unit, kv_head == 0, s);
+    const Part part = part_of<float, kRows, kStage>(a, plan, unit, kv_head == 0, s);
     if (!part.real) return;
     const int lane = threadIdx.x & 63;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -1245,40 +1250,105 @@ __global__ void __launch_bounds__(kThreads, 2) chunk_limb_kernel(ChunkArgs a, Ch
     }
 }
 
-// Joins the parts of a tile that was cut.  Workgroup (cut tile, KV head, every gridDim.z-th 256 fours of dims).
+// Joins the parts of a tile that was cut.  Workgroup (cut tile, KV head, a share of the rows).  With few parts a thread takes four
+// dims of a row.  With more a wave takes a row, its lanes the parts' shares first, then fours of dims, of which a narrow head's
+// lanes divide the parts among them (63 parts of 64 rows, 8 heads of 128: 37 us a call against 81; 4387 rows of 2 to 4
+// parts, 8 heads of 80: 12 us against 26 with a wave a row).
+constexpr int kFewParts = 8;
+constexpr int kJoinParts = 1024;  // whose shares are kept
+
+__device__ __forceinline__ float share_of(const float* statistics, float top, float natural) {
+    const bool near = fabsf(top) < kFar && fabsf(statistics[0]) < kFar;
+    const float share = fast_exp2(near ? statistics[0] - top : (statistics[2] - natural) * kLog2e);
+    return statistics[1] != 0.0f ? share : 0.0f;  // else it saw nothing, or its sums are zeros
+}
+
 template <class T>
-__global__ void __launch_bounds__(kThreads) chunk_join_kernel(ChunkArgs a, ChunkPlan plan) {
+__device__ __forceinline__ void store_joined(const ChunkArgs& a, int begin, int row, int kv_head, int four, float weight, const f32x4& sum) {
+    const int i = static_cast<int>(divide(row, a.group_of)), head = kv_head * a.group + row - i * a.group;
+    T* out = static_cast<T*>(a.out) + (static_cast<int64_t>(begin + i) * a.query_heads + head) * a.dim + 4 * four;
+#pragma unroll
+    for (int l = 0; l < 4; ++l)
+        if (4 * four + l < a.dim) out[l] = static_cast<T>(weight == 0.0f ? 0.0f : sum[l] / weight);
+}
+
+template <class T>
+__global__ void __launch_bounds__(kThreads) chunk_join_kernel(ChunkArgs a, ChunkPlan plan, int fours_bits) {
+    __shared__ float shares[kWaves][kJoinParts];
     const int* header = reinterpret_cast<const int*>(a.workspace);
     if (static_cast<int>(blockIdx.x) >= header[0]) return;
     const int* d = header + kDescription * (1 + blockIdx.x);
     const int begin = d[0], row0 = d[1], rows = d[2], slot = d[3], parts = d[4];
-    const int kv_head = blockIdx.y, fours = (a.dim + 3) / 4;
+    const int kv_head = blockIdx.y, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const int64_t stride = static_cast<int64_t>(plan.slot_rows) * plan.width;
-    for (int item = blockIdx.z * kThreads + threadIdx.x; item < rows * fours; item += gridDim.z * kThreads) {
-        const int r = item / fours, four = item - r * fours;
+    const int each = (rows + gridDim.z - 1) / gridDim.z, from = blockIdx.z * each, to = from + each < rows ? from + each : rows;
+    if (parts <= kFewParts) {
+        const int fours = (a.dim + 3) / 4;
+        for (int item = threadIdx.x; item < (to - from) * fours; item += kThreads) {
+            const int r = from + item / fours, four = item % fours;
+            const float* o = part_row(a, plan, kv_head, slot, r);
+            const float* of = o + plan.width - 4;
+            float top = -INFINITY, natural = -INFINITY, weight = 0.0f;
+            f32x4 statistics[kFewParts], sums[kFewParts], sum = {0, 0, 0, 0};
+#pragma unroll
+            for (int p = 0; p < kFewParts; ++p) {  // all loads ahead, of the first part where there is none
+                const int64_t at = p < parts ? p * stride : 0;
+                statistics[p] = *reinterpret_cast<const f32x4*>(of + at);
+                sums[p] = *reinterpret_cast<const f32x4*>(o + at + 4 * four);
+            }
+#pragma unroll
+            for (int p = 0; p < kFewParts; ++p) top = fmaxf(top, statistics[p][0]), natural = fmaxf(natural, statistics[p][2]);
+#pragma unroll
+            for (int p = 0; p < kFewParts; ++p) {
+                const float own[3] = {statistics[p][0], statistics[p][1], statistics[p][2]};
+                const float share = p < parts ? share_of(own, top, natural) : 0.0f;
+                weight += share != 0.0f ? own[1] * share : 0.0f;
+#pragma unroll
+                for (int l = 0; l < 4; ++l) sum[l] += share != 0.0f ? sums[p][l] * share : 0.0f;
+            }
+            store_joined<T>(a, begin, row0 + r, kv_head, four, weight, sum);
+        }
+        return;
+    }
+    const int four = lane & ((1 << fours_bits) - 1), turn = lane >> fours_bits, turns = kWave >> fours_bits;
+    for (int r = from + wave; r < to; r += kWaves) {
         const float* o = part_row(a, plan, kv_head, slot, r);
         const float* of = o + plan.width - 4;
         float top = -INFINITY, natural = -INFINITY;
-        for (int p = 0; p < parts; ++p) top = fmaxf(top, of[p * stride]), natural = fmaxf(natural, of[p * stride + 2]);
+#pragma unroll 2
+        for (int p = lane; p < parts; p += kWave) top = fmaxf(top, of[p * stride]), natural = fmaxf(natural, of[p * stride + 2]);
+        top = wave_max(top);
+        natural = wave_max(natural);
         float weight = 0.0f;
-        f32x4 sum = {0, 0, 0, 0};
-        for (int p = 0; p < parts; ++p) {
-            const float part_top = of[p * stride], part_weight = of[p * stride + 1];
-            if (part_weight == 0.0f) continue;  // such a part's sums are zeros, or it saw nothing
-            const bool near = fabsf(top) < kFar && fabsf(part_top) < kFar;
-            const float share = fast_exp2(near ? part_top - top : (of[p * stride + 2] - natural) * kLog2e);
-            weight += part_weight * share;
-            sum += *reinterpret_cast<const f32x4*>(o + p * stride + 4 * four) * share;
+        for (int p = lane; p < parts; p += kWave) {
+            const float share = share_of(of + p * stride, top, natural);
+            weight += share != 0.0f ? of[p * stride + 1] * share : 0.0f;
+            if (p < kJoinParts) shares[wave][p] = share;
         }
-        const int i = static_cast<int>(divide(row0 + r, a.group_of)), head = kv_head * a.group + row0 + r - i * a.group;
-        T* out = static_cast<T*>(a.out) + (static_cast<int64_t>(begin + i) * a.query_heads + head) * a.dim + 4 * four;
+        weight = wave_sum(weight);
+        f32x4 sum = {0, 0, 0, 0};
+        if (4 * four < a.dim) {
+#pragma unroll 8
+            for (int p = turn; p < parts; p += turns) {
+                const f32x4 part_sum = *reinterpret_cast<const f32x4*>(o + p * stride + 4 * four);
+                const float share = p < kJoinParts ? shares[wave][p] : share_of(of + p * stride, top, natural);
 #pragma unroll
-        for (int l = 0; l < 4; ++l)
-            if (4 * four + l < a.dim) out[l] = static_cast<T>(weight == 0.0f ? 0.0f : sum[l] / weight);
+                for (int l = 0; l < 4; ++l) sum[l] += share != 0.0f ? part_sum[l] * share : 0.0f;
+            }
+        }
+        for (int step = 1 << fours_bits; step < kWave; step *= 2)
+#pragma unroll
+            for (int l = 0; l < 4; ++l) sum[l] += __shfl_xor(sum[l], step, kWave);
+        if (turn == 0) store_joined<T>(a, begin, row0 + r, kv_head, four, weight, sum);
     }
 }
 
+constexpr int64_t kJoinBlocks = 4096;  // about, most of which find no cut tile
+
 // Parts of a step: two workgroups on each of 256 CUs.
+#ifndef LIMB_ALL
+#define LIMB_ALL 2048
+#endif
 #ifndef LIMB_ROWS
 #define LIMB_ROWS 64
 #endif
@@ -1288,7 +1358,7 @@ __global__ void __launch_bounds__(kThreads) chunk_join_kernel(ChunkArgs a, Chunk
 constexpr int kTarget = TARGET;
 
 // Whether float32 takes the limb kernel.
-bool by_limbs(const ChunkArgs& a) { return a.dim <= 64 && a.tokens * a.group >= LIMB_ROWS * a.requests; }
+bool by_limbs(const ChunkArgs& a) { return a.dim <= 64 && a.tokens * a.group >= LIMB_ROWS * a.requests && a.tokens * a.group >= LIMB_ALL; }
 
 template <class T>
 ChunkPlan plan_of(const ChunkArgs& a) {
@@ -1305,12 +1375,13 @@ ChunkPlan plan_of(const ChunkArgs& a) {
         const int64_t windowed = (static_cast<int64_t>(a.sinks) + stage - 1) / stage + (static_cast<int64_t>(a.window) + p.rows / a.group + 1) / stage + 2;
         if (windowed < stages) stages = windowed;
     }
-    p.whole = stages <= kLeastStages;
+    p.whole = stages <= kWholeStages;
+    p.least = sizeof(T) == 4 && by_limbs(a) ? 4 : least_stages<T>();
     p.units = p.tiles;
     if (!p.whole) {
         // A tile of S > each stages has at most S / each + 1 < 2 S / each parts, and the sum of all S is at most target times
-        // each; kLeastStages bounds them as well.
-        const int64_t most = p.tiles * ((stages + kLeastStages - 1) / kLeastStages);
+        // each; the least number of stages bounds them as well.
+        const int64_t most = p.tiles * ((stages + p.least - 1) / p.least);
         p.slots = 2 * static_cast<int64_t>(p.target) < most ? 2 * static_cast<int64_t>(p.target) : most;
         p.splits = p.target < p.tiles ? p.target : p.tiles;
         p.units = p.tiles + p.target < most ? p.tiles + p.target : most;
@@ -1362,10 +1433,13 @@ hipError_t launch_chunks(const ChunkArgs& a, hipStream_t stream) {
         default: launched = launch_tiles<T, 256>(a, plan, grid, stream);
     }
     if (launched != hipSuccess || plan.whole) return launched;
-    const int items = plan.slot_rows * ((a.dim + 3) / 4);
-    const int fold = (items + 4 * kThreads - 1) / (4 * kThreads);
-    hipLaunchKernelGGL(HIP_KERNEL_NAME(chunk_join_kernel<T>), dim3(static_cast<uint32_t>(plan.splits), a.kv_heads, fold), dim3(kThreads), 0,
-                       stream, a, plan);
+    int fours_bits = 0;
+    while (4 << fours_bits < a.dim) ++fours_bits;
+    const int64_t tiles = plan.splits * a.kv_heads, most = (plan.slot_rows + kWaves - 1) / kWaves;
+    int64_t folds = (kJoinBlocks + tiles - 1) / tiles;
+    if (folds > most) folds = most;
+    hipLaunchKernelGGL(HIP_KERNEL_NAME(chunk_join_kernel<T>), dim3(static_cast<uint32_t>(plan.splits), a.kv_heads, static_cast<uint32_t>(folds)),
+                       dim3(kThreads), 0, stream, a, plan, fours_bits);
     return hipGetLastError();
 }
 
