@@ -19,10 +19,11 @@ namespace {
 
 constexpr int kThreads = 256;
 constexpr int kWaves = 4;
-// Stages that are worth a workgroup, and below which no tile is cut, which saves the join's launch.
+// Stages that are worth a workgroup.  16-bit, with 1, 2, 3, 4 and 6 of them: 512 tokens over 512 keys 51, 42, 39, 36 and 36
+// us.  float32's stages of 64 keys are four times as long for 32 rows: 16 tokens over 900 keys 21 us with 1, 24 with 4.
 template <class T>
 constexpr int least_stages() { return sizeof(T) == 2 ? 4 : 1; }
-constexpr int kWholeStages = 4;
+constexpr int kWholeStages = 4;  // up to which no tile is cut, which saves the join's launch
 
 template <class T>
 constexpr int rows_of_tile(int dim) { return sizeof(T) == 2 ? 32 * kWaves : (dim <= 128 ? 32 : 16); }
@@ -159,11 +160,9 @@ __device__ __forceinline__ void clear_other_rows(const ChunkArgs& a, int before,
 }
 
 // Parts lie in kStrips strips, from which the workgroups take one each in turn: what runs at the same time is then of all
-// requests, chunks that matrix instructions bound next to single tokens that memory does.
-#ifndef STRIPS
-#define STRIPS 64
-#endif
-constexpr int kStrips = STRIPS;
+// requests, chunks that matrix instructions bound next to single tokens that memory does.  A step of both in bfloat16 (2
+// chunks of some 1000 tokens, 48 single tokens, 15000 keys and fewer) took 765, 762, 788 and 729 us with 1, 4, 16 and 64.
+constexpr int kStrips = 64;
 
 template <class T, int kRows, int kStage>
 __device__ Part part_of(const ChunkArgs& a, const ChunkPlan& plan, int place, bool describes, Sequence& sequence) {
@@ -252,7 +251,6 @@ __device__ Part part_of(const ChunkArgs& a, const ChunkPlan& plan, int place, bo
     const int local = same(s.chosen[1]);
     part.part = local % part.parts;
     part.slot = same(s.chosen[3]);
-    part.real = part.slot >= 0;
     sequence = s.sequence;
     sequence.begin = same(sequence.begin);
     sequence.count = same(sequence.count);
@@ -261,6 +259,7 @@ __device__ Part part_of(const ChunkArgs& a, const ChunkPlan& plan, int place, bo
     sequence.slot = static_cast<int64_t>(same(static_cast<int>(sequence.slot >> 32))) << 32 | static_cast<uint32_t>(same(static_cast<int>(sequence.slot)));
     // The longest tiles first.
     part.tile = static_cast<int>((static_cast<int64_t>(sequence.count) * a.group + kRows - 1) / kRows) - 1 - local / part.parts;
+    part.real = part.slot >= 0 && part.tile >= 0;
     return part;
 }
 
@@ -630,7 +629,7 @@ __device__ __forceinline__ void scale_if(bool moves, float shrink, f32x16 (&out)
     }
     const int some = __builtin_amdgcn_readfirstlane(moves);
 #pragma unroll
-    for (int b = 0; b < kBlocks; b += 2) {
+    for (int b = 0; b + 1 < kBlocks; b += 2) {
         float o[32];
 #pragma unroll
         for (int j = 0; j < 32; ++j) o[j] = out[b + j / 16][j % 16];
@@ -654,15 +653,34 @@ __device__ __forceinline__ void scale_if(bool moves, float shrink, f32x16 (&out)
 #pragma unroll
         for (int j = 0; j < 32; ++j) out[b + j / 16][j % 16] = o[j];
     }
+    if constexpr (kBlocks % 2) {
+        float o[16];
+#pragma unroll
+        for (int j = 0; j < 16; ++j) o[j] = out[kBlocks - 1][j];
+        asm volatile(
+            "s_cmp_eq_u32 %16, 0\n\ts_cbranch_scc1 .Lkept%=\n\ts_nop 15\n\ts_nop 15\n\t"
+            "v_mul_f32 %0, %17, %0\n\tv_mul_f32 %1, %17, %1\n\tv_mul_f32 %2, %17, %2\n\tv_mul_f32 %3, %17, %3\n\t"
+            "v_mul_f32 %4, %17, %4\n\tv_mul_f32 %5, %17, %5\n\tv_mul_f32 %6, %17, %6\n\tv_mul_f32 %7, %17, %7\n\t"
+            "v_mul_f32 %8, %17, %8\n\tv_mul_f32 %9, %17, %9\n\tv_mul_f32 %10, %17, %10\n\tv_mul_f32 %11, %17, %11\n\t"
+            "v_mul_f32 %12, %17, %12\n\tv_mul_f32 %13, %17, %13\n\tv_mul_f32 %14, %17, %14\n\tv_mul_f32 %15, %17, %15\n\t"
+            "s_nop 7\n.Lkept%=:"
+            : "+v"(o[0]), "+v"(o[1]), "+v"(o[2]), "+v"(o[3]), "+v"(o[4]), "+v"(o[5]), "+v"(o[6]), "+v"(o[7]),
+              "+v"(o[8]), "+v"(o[9]), "+v"(o[10]), "+v"(o[11]), "+v"(o[12]), "+v"(o[13]), "+v"(o[14]), "+v"(o[15])
+            : "s"(some), "v"(shrink)
+            : "scc");
+#pragma unroll
+        for (int j = 0; j < 16; ++j) out[kBlocks - 1][j] = o[j];
+    }
 }
 
-template <class T, int kDim, bool kWide>
+// kUsed: dims that are worked on, of the kDim that a row in LDS has.
+template <class T, int kDim, int kUsed, bool kWide>
 __global__ void __launch_bounds__(kThreads, kDim <= 128 ? 2 : 1) chunk_tile_kernel(ChunkArgs a, ChunkPlan plan) {
     using W = Wide<T>;
     constexpr int kStage = stage_keys<T>(kDim);
     constexpr int kSubs = kStage / 32;
-    constexpr int kSteps = kDim / 16;             // of a score
-    constexpr int kBlocks = kDim / 32;            // of the result
+    constexpr int kSteps = kUsed / 16;            // of a score
+    constexpr int kBlocks = kUsed / 32;           // of the result
     constexpr int kRows = rows_of_tile<T>(kDim);
     constexpr int kRowBytes = kDim * 2;
     constexpr int kSide = kStage * kRowBytes;     // keys or values of a stage
@@ -956,7 +974,6 @@ __global__ void __launch_bounds__(kThreads, kDim <= 128 ? 2 : 1) chunk_tile_kern
 // each limb's rows lie as a 16-bit type's do below.  Scores are in powers of two: the query is multiplied by scale * log2(e).
 // Where limbs do not do (an infinity, a NaN, magnitudes of kLimbMaxScore or kLimbMaxValue on, scores of kFar on, sums so small that
 // bits are lacking) the tile is computed again by register_rows.
-// A score that is kFar or more: its own rounding shows, and the tile is left to register_rows as well.
 constexpr float kLimbMostScore = 0x1p60f;  // of a scaled query and of a key: no sum of 64 products overflows
 constexpr float kLimbMostValue = 0x1p19f;
 constexpr float kLimbLeastSum = 0x1p-82f;  // of a row, per 64 keys: bits below 2^-134 of each factor are under 2^-26 of it
@@ -1272,6 +1289,37 @@ __device__ __forceinline__ void store_joined(const ChunkArgs& a, int begin, int 
         if (4 * four + l < a.dim) out[l] = static_cast<T>(weight == 0.0f ? 0.0f : sum[l] / weight);
 }
 
+// kMost parts or fewer: a thread takes four dims of a row, all of its loads ahead of their use.
+template <class T, int kMost>
+__device__ __forceinline__ void join_few(const ChunkArgs& a, const ChunkPlan& plan, int begin, int row0, int slot, int parts, int from, int to) {
+    const int kv_head = blockIdx.y, fours = (a.dim + 3) / 4;
+    const int64_t stride = static_cast<int64_t>(plan.slot_rows) * plan.width;
+    for (int item = threadIdx.x; item < (to - from) * fours; item += kThreads) {
+        const int r = from + item / fours, four = item % fours;
+        const float* o = part_row(a, plan, kv_head, slot, r);
+        const float* of = o + plan.width - 4;
+        float top = -INFINITY, natural = -INFINITY, weight = 0.0f;
+        f32x4 statistics[kMost], sums[kMost], sum = {0, 0, 0, 0};
+#pragma unroll
+        for (int p = 0; p < kMost; ++p) {  // of the first part where there is none
+            const int64_t at = p < parts ? p * stride : 0;
+            statistics[p] = *reinterpret_cast<const f32x4*>(of + at);
+            sums[p] = *reinterpret_cast<const f32x4*>(o + at + 4 * four);
+        }
+#pragma unroll
+        for (int p = 0; p < kMost; ++p) top = fmaxf(top, statistics[p][0]), natural = fmaxf(natural, statistics[p][2]);
+#pragma unroll
+        for (int p = 0; p < kMost; ++p) {
+            const float own[3] = {statistics[p][0], statistics[p][1], statistics[p][2]};
+            const float share = p < parts ? share_of(own, top, natural) : 0.0f;
+            weight += share != 0.0f ? own[1] * share : 0.0f;
+#pragma unroll
+            for (int l = 0; l < 4; ++l) sum[l] += share != 0.0f ? sums[p][l] * share : 0.0f;
+        }
+        store_joined<T>(a, begin, row0 + r, kv_head, four, weight, sum);
+    }
+}
+
 template <class T>
 __global__ void __launch_bounds__(kThreads) chunk_join_kernel(ChunkArgs a, ChunkPlan plan, int fours_bits) {
     __shared__ float shares[kWaves][kJoinParts];
@@ -1282,34 +1330,9 @@ __global__ void __launch_bounds__(kThreads) chunk_join_kernel(ChunkArgs a, Chunk
     const int kv_head = blockIdx.y, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const int64_t stride = static_cast<int64_t>(plan.slot_rows) * plan.width;
     const int each = (rows + gridDim.z - 1) / gridDim.z, from = blockIdx.z * each, to = from + each < rows ? from + each : rows;
-    if (parts <= kFewParts) {
-        const int fours = (a.dim + 3) / 4;
-        for (int item = threadIdx.x; item < (to - from) * fours; item += kThreads) {
-            const int r = from + item / fours, four = item % fours;
-            const float* o = part_row(a, plan, kv_head, slot, r);
-            const float* of = o + plan.width - 4;
-            float top = -INFINITY, natural = -INFINITY, weight = 0.0f;
-            f32x4 statistics[kFewParts], sums[kFewParts], sum = {0, 0, 0, 0};
-#pragma unroll
-            for (int p = 0; p < kFewParts; ++p) {  // all loads ahead, of the first part where there is none
-                const int64_t at = p < parts ? p * stride : 0;
-                statistics[p] = *reinterpret_cast<const f32x4*>(of + at);
-                sums[p] = *reinterpret_cast<const f32x4*>(o + at + 4 * four);
-            }
-#pragma unroll
-            for (int p = 0; p < kFewParts; ++p) top = fmaxf(top, statistics[p][0]), natural = fmaxf(natural, statistics[p][2]);
-#pragma unroll
-            for (int p = 0; p < kFewParts; ++p) {
-                const float own[3] = {statistics[p][0], statistics[p][1], statistics[p][2]};
-                const float share = p < parts ? share_of(own, top, natural) : 0.0f;
-                weight += share != 0.0f ? own[1] * share : 0.0f;
-#pragma unroll
-                for (int l = 0; l < 4; ++l) sum[l] += share != 0.0f ? sums[p][l] * share : 0.0f;
-            }
-            store_joined<T>(a, begin, row0 + r, kv_head, four, weight, sum);
-        }
-        return;
-    }
+    if (parts <= 2) return join_few<T, 2>(a, plan, begin, row0, slot, parts, from, to);
+    if (parts <= 4) return join_few<T, 4>(a, plan, begin, row0, slot, parts, from, to);
+    if (parts <= kFewParts) return join_few<T, kFewParts>(a, plan, begin, row0, slot, parts, from, to);
     const int four = lane & ((1 << fours_bits) - 1), turn = lane >> fours_bits, turns = kWave >> fours_bits;
     for (int r = from + wave; r < to; r += kWaves) {
         const float* o = part_row(a, plan, kv_head, slot, r);
@@ -1343,22 +1366,21 @@ __global__ void __launch_bounds__(kThreads) chunk_join_kernel(ChunkArgs a, Chunk
     }
 }
 
-constexpr int64_t kJoinBlocks = 4096;  // about, most of which find no cut tile
+constexpr int64_t kJoinBlocks = 1024;  // about, many of which find no cut tile (4096: 89 us for 88 of a call, 16384: 93)
 
-// Parts of a step: two workgroups on each of 256 CUs.
-#ifndef LIMB_ALL
-#define LIMB_ALL 2048
-#endif
-#ifndef LIMB_ROWS
-#define LIMB_ROWS 64
-#endif
-#ifndef TARGET
-#define TARGET 1024
-#endif
-constexpr int kTarget = TARGET;
+// Parts that a step's work is cut into: two rounds of two workgroups on each of 256 CUs, so that a CU whose parts end early
+// takes others.  The step of chunks and single tokens took 860, 809, 787 and 778 us with 512, 768, 1024 and 1536, where more
+// parts write and join more sums: 16 chunks in a window of 2048 keys took 102 us with 1024 and 104 with 2048.
+constexpr int kTarget = 1024;
 
-// Whether float32 takes the limb kernel.
-bool by_limbs(const ChunkArgs& a) { return a.dim <= 64 && a.tokens * a.group >= LIMB_ROWS * a.requests && a.tokens * a.group >= LIMB_ALL; }
+// Whether float32 takes the limb kernel: its tiles have 128 rows, which single tokens leave empty, and few of them leave CUs
+// idle.  Limbs and float32 products: 4 x 512 tokens over 512 keys each 161 and 238 us, 2048 tokens over 8192 253 and 443;
+// but 512 tokens over 512 keys in 4 heads 38 and 28, 64 over 2000 55 and 27, 32 single tokens over 4000 89 and 51.
+constexpr int64_t kLimbRows = 64, kLimbAll = 2048;
+bool by_limbs(const ChunkArgs& a) {
+    const int64_t rows = a.tokens * a.group;
+    return a.dim <= 64 && rows >= kLimbRows * a.requests && rows >= kLimbAll;
+}
 
 template <class T>
 ChunkPlan plan_of(const ChunkArgs& a) {
@@ -1391,7 +1413,7 @@ ChunkPlan plan_of(const ChunkArgs& a) {
     return p;
 }
 
-template <class T, int kDim>
+template <class T, int kDim, int kUsed>
 hipError_t launch_tiles(const ChunkArgs& a, const ChunkPlan& plan, dim3 grid, hipStream_t stream) {
     if constexpr (sizeof(T) == 2) {
         constexpr int kStage = stage_keys<T>(kDim);
@@ -1403,8 +1425,8 @@ hipError_t launch_tiles(const ChunkArgs& a, const ChunkPlan& plan, dim3 grid, hi
             hipLaunchKernelGGL(kernel, grid, dim3(kThreads), kLds, stream, a, plan);
             return hipGetLastError();
         };
-        if (a.wide && reinterpret_cast<uintptr_t>(a.out) % 8 == 0) return launch(chunk_tile_kernel<T, kDim, true>);
-        return launch(chunk_tile_kernel<T, kDim, false>);
+        if (a.wide && reinterpret_cast<uintptr_t>(a.out) % 8 == 0) return launch(chunk_tile_kernel<T, kDim, kUsed, true>);
+        return launch(chunk_tile_kernel<T, kDim, kUsed, false>);
     } else {
         if constexpr (kDim == 64) {
             if (by_limbs(a)) {
@@ -1427,11 +1449,12 @@ hipError_t launch_chunks(const ChunkArgs& a, hipStream_t stream) {
     if (blocks >= (int64_t{1} << 24)) return hipErrorInvalidValue;  // a grid has below 2^32 threads
     const dim3 grid(static_cast<uint32_t>(blocks));
     hipError_t launched;
-    switch (padded_dim(a.dim)) {
-        case 64: launched = launch_tiles<T, 64>(a, plan, grid, stream); break;
-        case 128: launched = launch_tiles<T, 128>(a, plan, grid, stream); break;
-        default: launched = launch_tiles<T, 256>(a, plan, grid, stream);
-    }
+    // The 16-bit kernel leaves the last quarter of a row out: 97 us for 103 at 80 dims.
+    constexpr int kNarrower = sizeof(T) == 2 ? 96 : 128;
+    if (a.dim <= 64) launched = launch_tiles<T, 64, 64>(a, plan, grid, stream);
+    else if (a.dim <= kNarrower) launched = launch_tiles<T, 128, kNarrower>(a, plan, grid, stream);
+    else if (a.dim <= 128) launched = launch_tiles<T, 128, 128>(a, plan, grid, stream);
+    else launched = launch_tiles<T, 256, 256>(a, plan, grid, stream);
     if (launched != hipSuccess || plan.whole) return launched;
     int fours_bits = 0;
     while (4 << fours_bits < a.dim) ++fours_bits;
