@@ -116,6 +116,36 @@ __device__ __forceinline__ uint64_t block_scan(uint64_t v, unsigned long long* w
     return v;
 }
 
+// Of several values a thread, each by itself.
+template <int kThreads, int kValues>
+__device__ __forceinline__ void block_scan(const uint64_t (&v)[kValues], unsigned long long* words, uint64_t (&reached)[kValues], uint64_t (&total)[kValues]) {
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+#pragma unroll
+    for (int i = 0; i < kValues; ++i) reached[i] = v[i], total[i] = 0;
+#pragma unroll
+    for (int step = 1; step < 64; step *= 2) {
+#pragma unroll
+        for (int i = 0; i < kValues; ++i) {
+            const uint64_t below = __shfl_up(static_cast<unsigned long long>(reached[i]), step, kWave);
+            if (lane >= step) reached[i] += below;
+        }
+    }
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < kValues; ++i)
+        if (lane == 63) words[i * (kThreads / kWave) + wave] = reached[i];
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < kThreads / kWave; ++w) {
+#pragma unroll
+        for (int i = 0; i < kValues; ++i) {
+            const uint64_t sum = words[i * (kThreads / kWave) + w];
+            if (w < wave) reached[i] += sum;
+            total[i] += sum;
+        }
+    }
+}
+
 // What a row asks for.
 struct RowOptions {
     uint32_t greedy;
@@ -126,20 +156,29 @@ struct RowOptions {
     double rate, top;
 };
 
-__device__ __forceinline__ RowOptions options_of(const SampleArgs& a, int64_t row, int bits, uint64_t best) {
+// As they are given: read while the largest logit is not known yet.
+struct GivenOptions {
+    float temperature, p, least;
+    int64_t k;
+    __device__ __forceinline__ GivenOptions(const SampleArgs& a, int64_t row) {
+        temperature = a.temperature ? a.temperature[row] : 1.0f;
+        k = a.top_k ? a.top_k[row] : 0;
+        p = a.top_p ? a.top_p[row] : 1.0f;
+        least = a.min_p ? a.min_p[row] : 0.0f;
+    }
+};
+
+__device__ __forceinline__ RowOptions options_of(const SampleArgs& a, const GivenOptions& given, int bits, uint64_t best) {
     RowOptions o;
     o.greedy = ~static_cast<uint32_t>(best);
     const float top = value_of(static_cast<uint32_t>(best >> 32));
-    const float temperature = a.temperature ? a.temperature[row] : 1.0f;
-    o.draws = temperature > 0.0f && fabsf(top) < INFINITY;
-    const int64_t k = a.top_k ? a.top_k[row] : 0;
-    o.k = k > 0 && k < a.vocab ? k : a.vocab;
-    const float p = a.top_p ? a.top_p[row] : 1.0f;
-    o.p = p < 1.0f ? (p > 0.0f ? p : 0.0f) : 1.0f;
-    const float least = a.min_p ? a.min_p[row] : 0.0f;
+    o.draws = given.temperature > 0.0f && fabsf(top) < INFINITY;
+    o.k = given.k > 0 && given.k < a.vocab ? given.k : a.vocab;
+    o.p = given.p < 1.0f ? (given.p > 0.0f ? given.p : 0.0f) : 1.0f;
+    const float least = given.least;
     o.least = least > 0.0f ? static_cast<uint64_t>(ceil(ldexp(static_cast<double>(least < 1.0f ? least : 1.0f), bits))) : 0;
     o.top = top;
-    o.rate = 32.0 * 1.44269504088896340736 / static_cast<double>(temperature);
+    o.rate = 32.0 * 1.44269504088896340736 / static_cast<double>(given.temperature);
     return o;
 }
 
@@ -178,31 +217,47 @@ template <class T, int kThreads>
 __device__ void draw_in(const SampleArgs& a, int64_t row, const T* in, bool wide, int64_t from, int64_t to, const Weigher& weigh,
                         uint64_t end, uint64_t least, uint64_t before, uint64_t target, uint64_t all, unsigned long long* words) {
     using U = Unit<T>;
+    constexpr int kAhead = 2;  // units of a thread that are read and summed at once
     uint64_t running = before;
-    for (int64_t base = from; base < to; base += kThreads * U::kWidth) {
-        const int64_t v = base + U::kWidth * static_cast<int>(threadIdx.x);
-        U unit;
-        unit.load(in, v, to, wide);
-        uint64_t w[U::kWidth], sum = 0;
+    for (int64_t base = from; base < to; base += kAhead * kThreads * U::kWidth) {
+        U units[kAhead];
+        uint64_t sums[kAhead], totals[kAhead];
+        auto weight_of = [&](float x, int64_t v) -> uint64_t {
+            const uint64_t w = v < to && rank_of(x, static_cast<uint32_t>(v)) >= end ? weigh(x) : 0;
+            return w < least ? 0 : w;
+        };
+        auto at = [&](int i) { return base + U::kWidth * (i * kThreads + static_cast<int>(threadIdx.x)); };
 #pragma unroll
-        for (int j = 0; j < U::kWidth; ++j) {
-            w[j] = v + j < to && rank_of(unit[j], static_cast<uint32_t>(v + j)) >= end ? weigh(unit[j]) : 0;
-            if (w[j] < least) w[j] = 0;
-            sum += w[j];
-        }
-        uint64_t total;
-        uint64_t reached = running + block_scan<kThreads>(sum, words, &total) - sum;
+        for (int i = 0; i < kAhead; ++i) units[i].load(in, at(i), to, wide);
 #pragma unroll
-        for (int j = 0; j < U::kWidth; ++j) {
-            if (w[j] && reached <= target && reached + w[j] > target) {
-                double f;
-                const int step = weigh.step_of(unit[j], f);
-                a.tokens[row] = v + j;
-                a.probabilities[row] = static_cast<float>(weigh.power(step, f) / static_cast<double>(all));
+        for (int i = 0; i < kAhead; ++i) {
+            sums[i] = 0;
+            if (at(i) < to) {
+#pragma unroll
+                for (int j = 0; j < U::kWidth; ++j) sums[i] += weight_of(units[i][j], at(i) + j);
             }
-            reached += w[j];
         }
-        running += total;
+        uint64_t reached[kAhead];
+        block_scan<kThreads>(sums, words, reached, totals);
+#pragma unroll
+        for (int i = 0; i < kAhead; ++i) {
+            uint64_t sum = running + reached[i] - sums[i];
+            if (sum <= target && sum + sums[i] > target) {
+#pragma unroll
+                for (int j = 0; j < U::kWidth; ++j) {
+                    const float x = units[i][j];
+                    const uint64_t w = weight_of(x, at(i) + j);
+                    if (sum <= target && sum + w > target) {
+                        double f;
+                        const int step = weigh.step_of(x, f);
+                        a.tokens[row] = at(i) + j;
+                        a.probabilities[row] = static_cast<float>(weigh.power(step, f) / static_cast<double>(all));
+                    }
+                    sum += w;
+                }
+            }
+            running += totals[i];
+        }
         if (running > target) return;
     }
 }
@@ -215,7 +270,7 @@ constexpr int kDigitBins = 2048;
 struct DigitShared {
     unsigned long long mass[kDigitBins];
     uint32_t count[kDigitBins];
-    unsigned long long words[kRowThreads / kWave];
+    unsigned long long words[2 * kRowThreads / kWave];
     unsigned long long word, above;
     uint32_t index;
     double roots[32];
@@ -339,6 +394,7 @@ __global__ void __launch_bounds__(kRowThreads) sample_row_kernel(SampleArgs a, i
     const int64_t row = blockIdx.x;
     const T* in = static_cast<const T*>(a.logits) + row * a.logits_stride;
     if (threadIdx.x < 32) s.roots[threadIdx.x] = kRoots[threadIdx.x];
+    const GivenOptions given(a, row);
     uint64_t best = 0;
     for (int64_t v = U::kWidth * static_cast<int>(threadIdx.x); v < a.vocab; v += U::kWidth * kRowThreads) {
         U unit;
@@ -350,7 +406,7 @@ __global__ void __launch_bounds__(kRowThreads) sample_row_kernel(SampleArgs a, i
         }
     }
     best = block_best<kRowThreads>(best, s.words);
-    const RowOptions o = options_of(a, row, bits, best);
+    const RowOptions o = options_of(a, given, bits, best);
     if (!o.draws) {
         if (threadIdx.x == 0) a.tokens[row] = o.greedy, a.probabilities[row] = 1.0f;
         return;
@@ -365,16 +421,30 @@ constexpr int kWaves = kThreads / kWave;
 constexpr int kSteps = 1600;  // of weights that are not 0: 32 (bits + 1), at most 48 bits
 constexpr int kList = 1024;   // tokens in the steps where top-k and top-p end
 constexpr int kMostParts = 64;
+constexpr int kGranules = 2048;
 
 struct SampleSplit {
-    int parts;      // of a row
-    int64_t part;   // tokens
+    int parts;       // of a row
+    int64_t part;    // tokens
+    int units;       // a wave's in a row: a granule, of 64 units' tokens each
+    int granules;    // of a row, at most kGranules
+    int part_granules;
     unsigned long long* best;    // [rows, parts]
-    unsigned long long* mass;    // [rows, parts]
+    unsigned long long* mass;    // [rows, granules]
     unsigned long long* masses;  // [rows, kSteps]
     unsigned long long* list;    // [rows, kList] ranks
+    struct Ends* ends;           // [rows]
     uint32_t* counts;            // [rows, kSteps]
     uint32_t* listed;            // [rows]
+};
+
+// Where the kept tokens of a row end, as far as its histogram tells: steps below `sure` are kept, the end is in the list, that
+// is the steps [sure, last] and `by_count`, in which the k-th token is.  kSteps: none.
+struct Ends {
+    int sure, last, by_count;
+    uint64_t count_before, mass_before;  // of the step by_count
+    uint64_t mass_sure;  // of the steps below `sure`
+    uint64_t mass_all;
 };
 
 // All parts of a row on one XCD (block index modulo 8), whose L2 then holds the row and its histogram.
@@ -383,6 +453,33 @@ __device__ __forceinline__ bool place_of(const SampleArgs& a, const SampleSplit&
     row = static_cast<int64_t>(j / s.parts) * 8 + blockIdx.x % 8;
     part = j % s.parts;
     return row < a.rows;
+}
+
+// A part's tokens, by each wave in granules: `each` has a unit and its first token, `all` the granule's number and the sum
+// of what `each` returned.
+template <class T, class Each, class All>
+__device__ __forceinline__ void walk(const SampleArgs& a, const SampleSplit& s, int64_t row, int part, bool wide, Each each, All all) {
+    using U = Unit<T>;
+    const T* in = static_cast<const T*>(a.logits) + row * a.logits_stride;
+    const int64_t granule = static_cast<int64_t>(s.units) * kWave * U::kWidth;
+    const int64_t from = part * s.part, to = from + s.part < a.vocab ? from + s.part : a.vocab;
+    const int lane = threadIdx.x & 63;
+    int number = part * s.part_granules + (threadIdx.x >> 6);
+    for (int64_t start = from + (threadIdx.x >> 6) * granule; start < to; start += kWaves * granule, number += kWaves) {
+        uint64_t sum = 0;
+        for (int u = 0; u < s.units; ++u) {
+            const int64_t v = start + (u * kWave + lane) * U::kWidth;
+            U unit;
+            unit.load(in, v, to, wide);
+            sum += each(unit, v);
+        }
+        all(number, sum);
+    }
+}
+__device__ __forceinline__ uint64_t wave_sum_of(uint64_t v) {
+#pragma unroll
+    for (int step = 1; step < 64; step *= 2) v += __shfl_xor(static_cast<unsigned long long>(v), step, kWave);
+    return v;
 }
 
 template <class T>
@@ -413,8 +510,9 @@ __global__ void __launch_bounds__(kThreads) sample_best_kernel(SampleArgs a, Sam
 }
 
 __device__ __forceinline__ RowOptions row_options(const SampleArgs& a, const SampleSplit& s, int64_t row, int bits, unsigned long long* words) {
+    const GivenOptions given(a, row);
     uint64_t best = threadIdx.x < static_cast<uint32_t>(s.parts) ? s.best[row * s.parts + threadIdx.x] : 0;  // at most kMostParts
-    return options_of(a, row, bits, block_best<kThreads>(best, words));
+    return options_of(a, given, bits, block_best<kThreads>(best, words));
 }
 
 template <class T>
@@ -439,30 +537,33 @@ __global__ void __launch_bounds__(kThreads) sample_mass_kernel(SampleArgs a, Sam
         __syncthreads();
     }
     const Weigher weigh{roots, o.top, o.rate, bits};
-    const T* in = static_cast<const T*>(a.logits) + row * a.logits_stride;
-    const int64_t from = part * s.part, to = from + s.part < a.vocab ? from + s.part : a.vocab;
-    uint64_t sum = 0;
-    for (int64_t v = from + U::kWidth * static_cast<int>(threadIdx.x); v < to; v += U::kWidth * kThreads) {
-        U unit;
-        unit.load(in, v, to, wide);
+    if (!filtered) {
+        __syncthreads();
+        walk<T>(a, s, row, part, wide, [&](const U& unit, int64_t) {
+            uint64_t sum = 0;
+#pragma unroll
+            for (int j = 0; j < U::kWidth; ++j) {
+                const uint64_t w = weigh(unit[j]);
+                sum += w < o.least ? 0 : w;
+            }
+            return sum;
+        }, [&](int granule, uint64_t sum) {
+            sum = wave_sum_of(sum);
+            if ((threadIdx.x & 63) == 0) s.mass[row * s.granules + granule] = sum;
+        });
+        return;
+    }
+    walk<T>(a, s, row, part, wide, [&](const U& unit, int64_t) -> uint64_t {
 #pragma unroll
         for (int j = 0; j < U::kWidth; ++j) {
             double f;
             const int step = weigh.step_of(unit[j], f);
             if (step >= kSteps) continue;
             if (by_count) atomicAdd(counts + step, 1u);
-            if (by_count && !by_mass) continue;
-            const uint64_t w = weigh.weight(step, f);
-            if (by_mass) atomicAdd(masses + step, static_cast<unsigned long long>(w));
-            else sum += w < o.least ? 0 : w;
+            if (by_mass) atomicAdd(masses + step, static_cast<unsigned long long>(weigh.weight(step, f)));
         }
-    }
-    if (!filtered) {
-        uint64_t all;
-        block_scan<kThreads>(sum, words, &all);
-        if (threadIdx.x == 0) s.mass[row * s.parts + part] = all;
-        return;
-    }
+        return 0;
+    }, [](int, uint64_t) {});
     __syncthreads();
     for (int b = threadIdx.x; b < kSteps; b += kThreads) {
         if (counts[b]) atomicAdd(s.counts + row * kSteps + b, counts[b]);
@@ -470,45 +571,49 @@ __global__ void __launch_bounds__(kThreads) sample_mass_kernel(SampleArgs a, Sam
     }
 }
 
-// Where the kept tokens of a row end, as far as its histogram tells: steps below `sure` are kept, the end is in the list, that
-// is the steps [sure, last] and `by_count`, in which the k-th token is.  kSteps: none.
-struct Ends {
-    int sure, last, by_count;
-    uint64_t count_before, mass_before;  // of the step by_count
-    uint64_t mass_sure;  // of the steps below `sure`
-    uint64_t mass_all;
-};
-
 struct EndsShared {
-    unsigned long long words[kWaves];
+    unsigned long long words[2 * kWaves];
     int step;
-    unsigned long long count, mass;
+    unsigned long long count, mass, own_mass;
 };
 
-__device__ Ends ends_of(const SampleSplit& s, int64_t row, const RowOptions& o, int64_t vocab, EndsShared& shared) {
-    constexpr int kEach = (kSteps + kThreads - 1) / kThreads;
-    const int b0 = kEach * threadIdx.x;
-    uint64_t mass[kEach], masses = 0, count[kEach], counts = 0;
+// A thread's steps of the row's histogram.
+constexpr int kStepsEach = (kSteps + kThreads - 1) / kThreads;
+struct ThreadSteps {
+    uint64_t mass[kStepsEach];
+    uint32_t count[kStepsEach];
+    __device__ __forceinline__ ThreadSteps(const SampleSplit& s, int64_t row) {
 #pragma unroll
-    for (int j = 0; j < kEach; ++j) {
-        const bool real = b0 + j < kSteps;
-        mass[j] = real ? s.masses[row * kSteps + b0 + j] : 0;
-        count[j] = real && o.k < vocab ? s.counts[row * kSteps + b0 + j] : 0;
-        masses += mass[j];
-        counts += count[j];
+        for (int j = 0; j < kStepsEach; ++j) {
+            const int b = kStepsEach * static_cast<int>(threadIdx.x) + j;
+            mass[j] = b < kSteps ? s.masses[row * kSteps + b] : 0;
+            count[j] = b < kSteps ? s.counts[row * kSteps + b] : 0;
+        }
     }
-    uint64_t all_mass, all_count = 0, count_before = 0;
-    const uint64_t mass_before = block_scan<kThreads>(masses, shared.words, &all_mass) - masses;
-    if (o.k < vocab) count_before = block_scan<kThreads>(counts, shared.words, &all_count) - counts;
+};
+
+__device__ Ends ends_of(const ThreadSteps& steps, const RowOptions& o, int64_t vocab, EndsShared& shared) {
+    const int b0 = kStepsEach * threadIdx.x;
+    const uint64_t(&mass)[kStepsEach] = steps.mass;
+    uint64_t count[kStepsEach], sums[2] = {0, 0}, before[2], all[2];
+#pragma unroll
+    for (int j = 0; j < kStepsEach; ++j) {
+        count[j] = steps.count[j];
+        sums[0] += mass[j];
+        sums[1] += count[j];
+    }
+    block_scan<kThreads>(sums, shared.words, before, all);
+    const uint64_t all_mass = all[0], all_count = all[1], mass_before = before[0] - sums[0], count_before = before[1] - sums[1];
     // The first step at which the sum reaches the limit.
-    auto reach = [&](uint64_t limit, uint64_t before, const uint64_t (&added)[kEach]) {
+    auto reach = [&](uint64_t limit, uint64_t before, const uint64_t (&added)[kStepsEach]) {
         __syncthreads();
         if (threadIdx.x == 0) shared.step = kSteps;
         __syncthreads();
         uint64_t mass_at = mass_before, at = before;
 #pragma unroll
-        for (int j = 0; j < kEach; ++j) {
-            if (at < limit && at + added[j] >= limit) shared.step = b0 + j, shared.count = at, shared.mass = mass_at;
+        for (int j = 0; j < kStepsEach; ++j) {
+            if (at < limit && at + added[j] >= limit)
+                shared.step = b0 + j, shared.count = at, shared.mass = mass_at, shared.own_mass = mass[j];
             at += added[j];
             mass_at += mass[j];
         }
@@ -523,7 +628,7 @@ __device__ Ends ends_of(const SampleSplit& s, int64_t row, const RowOptions& o, 
         e.mass_before = e.mass_sure = shared.mass;
         e.sure = e.last = e.by_count;
         low = e.mass_before;
-        high = e.by_count < kSteps ? e.mass_before + s.masses[row * kSteps + e.by_count] : all_mass;
+        high = e.by_count < kSteps ? e.mass_before + shared.own_mass : all_mass;
     }
     if (o.p < 1.0f) {
         e.last = reach(mass_limit(o.p, high), mass_before, mass);
@@ -544,20 +649,24 @@ __global__ void __launch_bounds__(kThreads) sample_list_kernel(SampleArgs a, Sam
     int part;
     if (!place_of(a, s, row, part)) return;
     if (threadIdx.x < 32) roots[threadIdx.x] = kRoots[threadIdx.x];
+    const ThreadSteps steps(s, row);
     const RowOptions o = row_options(a, s, row, bits, shared.words);
     if (!o.draws || (o.k >= a.vocab && o.p >= 1.0f)) return;
-    const Ends e = ends_of(s, row, o, a.vocab, shared);
+    const Ends e = ends_of(steps, o, a.vocab, shared);
+    if (threadIdx.x == 0 && part == 0) s.ends[row] = e;
     if (threadIdx.x == 0) count = 0;
     __syncthreads();
     const Weigher weigh{roots, o.top, o.rate, bits};
-    const T* in = static_cast<const T*>(a.logits) + row * a.logits_stride;
-    const int64_t from = part * s.part, to = from + s.part < a.vocab ? from + s.part : a.vocab;
-    uint64_t sum = 0;
-    for (int64_t v = from + U::kWidth * static_cast<int>(threadIdx.x); v < to; v += U::kWidth * kThreads) {
-        U unit;
-        unit.load(in, v, to, wide);
+    // Most logits are far below the ends.  Their step to three roundings of 2^-24, or an earlier one where the rate is beyond
+    // float32's, is off by less than 2^-10 of a step: what lies a whole step behind the last is left out by it.
+    const int last = e.by_count < kSteps && e.by_count > e.last ? e.by_count : e.last;
+    const float top = static_cast<float>(o.top), rate = o.rate < 0x1p127 ? static_cast<float>(o.rate) : 0x1p127f;
+    const float far = -static_cast<float>(last + 1);
+    walk<T>(a, s, row, part, wide, [&](const U& unit, int64_t v) {
+        uint64_t sum = 0;
 #pragma unroll
         for (int j = 0; j < U::kWidth; ++j) {
+            if ((unit[j] - top) * rate < far) continue;
             double f;
             const int step = weigh.step_of(unit[j], f);
             if (step >= kSteps) continue;
@@ -569,21 +678,21 @@ __global__ void __launch_bounds__(kThreads) sample_list_kernel(SampleArgs a, Sam
                 if (at < kList) found[at] = rank_of(unit[j], static_cast<uint32_t>(v + j));
             }
         }
-    }
-    uint64_t all;
-    block_scan<kThreads>(sum, shared.words, &all);
-    if (threadIdx.x == 0) {
-        s.mass[row * s.parts + part] = all;
-        first = count ? atomicAdd(s.listed + row, count) : 0;
-    }
+        return sum;
+    }, [&](int granule, uint64_t sum) {
+        sum = wave_sum_of(sum);
+        if ((threadIdx.x & 63) == 0) s.mass[row * s.granules + granule] = sum;
+    });
+    __syncthreads();
+    if (threadIdx.x == 0) first = count ? atomicAdd(s.listed + row, count) : 0;
     __syncthreads();
     for (uint32_t i = threadIdx.x; i < count && i < kList; i += kThreads)
         if (first + i < kList) s.list[row * kList + first + i] = found[i];
 }
 
 struct DrawShared {
-    unsigned long long list[kList], sorted[kList];
-    unsigned long long part_mass[kMostParts];
+    unsigned long long sorted[kList];
+    unsigned long long mass[kGranules];
     unsigned long long end, before;
     int index;
 };
@@ -603,8 +712,13 @@ __global__ void __launch_bounds__(kThreads) sample_draw_kernel(SampleArgs a, Sam
     const Weigher weigh{roots, o.top, o.rate, bits};
     const T* in = static_cast<const T*>(a.logits) + row * a.logits_stride;
     DrawShared& d = u.draw;
-    const bool mine = threadIdx.x < static_cast<uint32_t>(s.parts);
-    if (threadIdx.x < kMostParts) d.part_mass[threadIdx.x] = mine ? s.mass[row * s.parts + threadIdx.x] : 0;
+    const int64_t granule = static_cast<int64_t>(s.units) * kWave * Unit<T>::kWidth;
+    constexpr int kGranulesEach = kGranules / kThreads;
+#pragma unroll
+    for (int i = 0; i < kGranulesEach; ++i) {
+        const int g = i * kThreads + static_cast<int>(threadIdx.x);
+        d.mass[g] = g < s.granules ? s.mass[row * s.granules + g] : 0;
+    }
     uint64_t end = 0;
     if (o.k < a.vocab || o.p < 1.0f) {
         const uint32_t listed = s.listed[row];
@@ -615,17 +729,23 @@ __global__ void __launch_bounds__(kThreads) sample_draw_kernel(SampleArgs a, Sam
             sample_row<T, kThreads>(a, row, o, bits, wide, u.digits);
             return;
         }
-        const Ends e = ends_of(s, row, o, a.vocab, shared);
-        // In their order: every token counts those before it.
-        for (uint32_t i = threadIdx.x; i < listed; i += kThreads) d.list[i] = s.list[row * kList + i];
+        const Ends e = s.ends[row];
+        // In their order, by a bitonic network; a rank is never 0, which fills the list up to a power of two.
+        uint32_t places = 2;
+        while (places < listed) places *= 2;
+        for (uint32_t i = threadIdx.x; i < places; i += kThreads) d.sorted[i] = i < listed ? s.list[row * kList + i] : 0;
         if (threadIdx.x == 0) d.end = ~0ull;
         __syncthreads();
-        for (uint32_t i = threadIdx.x; i < listed; i += kThreads) {
-            uint32_t before = 0;
-            for (uint32_t j = 0; j < listed; ++j) before += d.list[j] > d.list[i];
-            d.sorted[before] = d.list[i];
+        for (uint32_t run = 2; run <= places; run *= 2) {
+            for (uint32_t apart = run / 2; apart > 0; apart /= 2) {
+                const uint32_t i = 2 * threadIdx.x - (threadIdx.x & (apart - 1));  // one pair a thread
+                if (i < places) {
+                    const uint64_t x = d.sorted[i], y = d.sorted[i + apart];
+                    if ((x < y) == ((i & run) == 0)) d.sorted[i] = y, d.sorted[i + apart] = x;
+                }
+                __syncthreads();
+            }
         }
-        __syncthreads();
         constexpr int kEach = kList / kThreads;
         const uint32_t i0 = kEach * threadIdx.x;
         uint64_t w[kEach], sum = 0, counted = 0, below = 0;
@@ -658,47 +778,58 @@ __global__ void __launch_bounds__(kThreads) sample_draw_kernel(SampleArgs a, Sam
         uint64_t reached = e.mass_sure + block_scan<kThreads>(sum, shared.words, &total) - sum;
 #pragma unroll
         for (int j = 0; j < kEach; ++j) {
-            if (i0 + j < listed && reached < limit && (!of_count[j] || i0 + j < first_of_count + kept_of_count)) {
-                atomicMin(&d.end, d.sorted[i0 + j]);
+            const bool kept = i0 + j < listed && reached < limit && (!of_count[j] || i0 + j < first_of_count + kept_of_count);
+            if (kept) {
                 const uint32_t index = ~static_cast<uint32_t>(d.sorted[i0 + j]);
-                if (w[j] >= o.least) atomicAdd(d.part_mass + index / s.part, static_cast<unsigned long long>(w[j]));
+                if (w[j] >= o.least) atomicAdd(d.mass + index / static_cast<uint32_t>(granule), static_cast<unsigned long long>(w[j]));
             }
+            const uint64_t lanes = __ballot(kept);
+            if (lanes && (threadIdx.x & 63) == 63 - static_cast<uint32_t>(__builtin_clzll(lanes))) atomicMin(&d.end, d.sorted[i0 + j]);  // the wave's last
             reached += w[j];
         }
         __syncthreads();
         if (listed) end = d.end;
     }
     __syncthreads();
-    uint64_t all;
-    const uint64_t mass = threadIdx.x < kMostParts ? d.part_mass[threadIdx.x] : 0;
-    const uint64_t reached = block_scan<kThreads>(mass, shared.words, &all);
+    uint64_t all, mass[kGranulesEach], masses = 0;
+#pragma unroll
+    for (int i = 0; i < kGranulesEach; ++i) masses += mass[i] = d.mass[kGranulesEach * threadIdx.x + i];
+    uint64_t before = block_scan<kThreads>(masses, shared.words, &all) - masses;
     const uint64_t target = drawn_mass(a.uniforms[row], all);
-    if (mass && reached > target && reached - mass <= target) d.index = threadIdx.x, d.before = reached - mass;
+#pragma unroll
+    for (int i = 0; i < kGranulesEach; ++i) {
+        if (mass[i] && before <= target && before + mass[i] > target) d.index = kGranulesEach * threadIdx.x + i, d.before = before;
+        before += mass[i];
+    }
     __syncthreads();
-    const int64_t from = d.index * s.part, to = from + s.part < a.vocab ? from + s.part : a.vocab;
+    const int64_t from = d.index * granule, to = from + granule < a.vocab ? from + granule : a.vocab;
     draw_in<T, kThreads>(a, row, in, wide, from, to, weigh, end, o.least, d.before, target, all, shared.words);
 }
 
 // Rows up to this many tokens are one workgroup's.
 constexpr int64_t kShortRow = 8192;
-// Tokens that all threads of a workgroup read at once in 16-bit types: parts are multiples of it.
-constexpr int64_t kPartStep = 4096;
-
-// About four workgroups a CU.
-SampleSplit split_of(int64_t rows, int64_t vocab, void* workspace, size_t* bytes) {
+// About four workgroups a CU, and parts of whole granules for every wave.
+SampleSplit split_of(int64_t rows, int64_t vocab, int size, void* workspace, size_t* bytes) {
     SampleSplit s{};
+    const int64_t unit = kWave * 16 / size;  // tokens that a wave reads at once
+    s.units = 1;
+    while ((vocab + s.units * unit - 1) / (s.units * unit) > kGranules) s.units *= 2;
+    const int64_t granule = s.units * unit, step = kWaves * granule;
     int64_t parts = (1024 + rows - 1) / rows;
     if (parts > kMostParts) parts = kMostParts;
-    s.part = ((vocab + parts - 1) / parts + kPartStep - 1) / kPartStep * kPartStep;
+    s.part = ((vocab + parts - 1) / parts + step - 1) / step * step;
     s.parts = static_cast<int>((vocab + s.part - 1) / s.part);
+    s.part_granules = static_cast<int>(s.part / granule);
+    s.granules = static_cast<int>((vocab + granule - 1) / granule);
     auto* at = static_cast<unsigned long long*>(workspace);
     s.best = at;
     s.mass = s.best + rows * s.parts;
-    s.masses = s.mass + rows * s.parts;
+    s.masses = s.mass + rows * s.granules;
     s.list = s.masses + rows * kSteps;
-    s.counts = reinterpret_cast<uint32_t*>(s.list + rows * kList);
+    s.ends = reinterpret_cast<Ends*>(s.list + rows * kList);
+    s.counts = reinterpret_cast<uint32_t*>(s.ends + rows);
     s.listed = s.counts + rows * kSteps;
-    *bytes = static_cast<size_t>(rows) * (16 * s.parts + 8 * kSteps + 8 * kList + 4 * kSteps) + static_cast<size_t>(rows + rows % 2) * 4;
+    *bytes = static_cast<size_t>(rows) * (8 * s.parts + 8 * s.granules + 8 * kSteps + 8 * kList + sizeof(Ends) + 4 * kSteps) + static_cast<size_t>(rows + rows % 2) * 4;
     return s;
 }
 
@@ -713,7 +844,7 @@ hipError_t launch_sample(const SampleArgs& a, hipStream_t stream) {
         return hipGetLastError();
     }
     size_t bytes = 0;
-    const SampleSplit s = split_of(a.rows, a.vocab, a.workspace, &bytes);
+    const SampleSplit s = split_of(a.rows, a.vocab, sizeof(T), a.workspace, &bytes);
     const dim3 grid((rows + 7) / 8 * 8 * static_cast<uint32_t>(s.parts));
     hipLaunchKernelGGL(HIP_KERNEL_NAME(sample_best_kernel<T>), grid, dim3(kThreads), 0, stream, a, s, wide);
     hipLaunchKernelGGL(HIP_KERNEL_NAME(sample_mass_kernel<T>), grid, dim3(kThreads), 0, stream, a, s, bits, wide);
@@ -727,7 +858,7 @@ hipError_t launch_sample(const SampleArgs& a, hipStream_t stream) {
 size_t sample_workspace_bytes(int64_t rows, int64_t vocab) {
     if (vocab <= kShortRow) return 0;
     size_t bytes = 0;
-    split_of(rows, vocab, nullptr, &bytes);
+    split_of(rows, vocab, 4, nullptr, &bytes);  // float32 has the most granules
     return bytes;
 }
 
