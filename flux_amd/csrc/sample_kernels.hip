@@ -657,16 +657,17 @@ __global__ void __launch_bounds__(kThreads) sample_list_kernel(SampleArgs a, Sam
     if (threadIdx.x == 0) count = 0;
     __syncthreads();
     const Weigher weigh{roots, o.top, o.rate, bits};
-    // Most logits are far below the ends.  Their step to three roundings of 2^-24, or an earlier one where the rate is beyond
-    // float32's, is off by less than 2^-10 of a step: what lies a whole step behind the last is left out by it.
+    // Most logits are far below the ends.  Their step to three roundings of 2^-24, of halves whose difference does not overflow, or
+    // an earlier one where the rate is beyond float32's, is off by less than 2^-10 of a step: what lies a whole step behind the
+    // last is left out by it.
     const int last = e.by_count < kSteps && e.by_count > e.last ? e.by_count : e.last;
-    const float top = static_cast<float>(o.top), rate = o.rate < 0x1p127 ? static_cast<float>(o.rate) : 0x1p127f;
+    const float top = 0.5f * static_cast<float>(o.top), rate = 2.0f * (o.rate < 0x1p126 ? static_cast<float>(o.rate) : 0x1p126f);
     const float far = -static_cast<float>(last + 1);
     walk<T>(a, s, row, part, wide, [&](const U& unit, int64_t v) {
         uint64_t sum = 0;
 #pragma unroll
         for (int j = 0; j < U::kWidth; ++j) {
-            if ((unit[j] - top) * rate < far) continue;
+            if ((0.5f * unit[j] - top) * rate < far) continue;
             double f;
             const int step = weigh.step_of(unit[j], f);
             if (step >= kSteps) continue;
@@ -836,7 +837,7 @@ SampleSplit split_of(int64_t rows, int64_t vocab, int size, void* workspace, siz
 template <class T>
 hipError_t launch_sample(const SampleArgs& a, hipStream_t stream) {
     int bits = 51;
-    while (bits > 0 && (a.vocab << bits) > (int64_t{1} << 62)) --bits;
+    while (a.vocab > (int64_t{1} << (62 - bits))) --bits;  // not the vocabulary shifted, which does not fit
     const bool wide = reinterpret_cast<uintptr_t>(a.logits) % 16 == 0 && a.logits_stride * sizeof(T) % 16 == 0;
     const auto rows = static_cast<uint32_t>(a.rows);
     if (a.vocab <= kShortRow) {

@@ -355,6 +355,91 @@ def test_chunk_loses_no_key(gpu_device, dtype, heads, kv_heads, dim, window, sin
         assert bool(((lost - expected[1, 0]).abs() > bound[1, 0]).any())
 
 
+# float32 chunks of many rows are multiplied in three limbs of 16 bits: 141 tokens of 16 heads are such.
+
+MANY = [(70, 60), (2, 3000), (60, 700), (9, 0)]
+
+
+def _many_rows(seed, dim=64, scale=None):
+    return _chunk_case(seed, torch.float32, 16, 1, dim, 16, MANY, scale=scale)
+
+
+@pytest.mark.parametrize("dim", [64, 40, 33, 2])
+@pytest.mark.parametrize("window,sinks", [(0, 0), (900, 20), (1, 0)])
+def test_chunk_of_many_rows(gpu_device, dim, window, sinks):
+    case = _many_rows(71, dim)
+    _check_chunk(case, gpu_device, window=window, sinks=sinks)
+    moved = _to(case, gpu_device)
+    for name in ("key_pages", "value_pages"):  # rows that start at no 16 bytes
+        store = torch.full((*moved[name].shape[:3], dim + 3), math.nan, device=gpu_device)
+        store[..., 1 : dim + 1] = moved[name]
+        moved[name] = store[..., 1 : dim + 1]
+    moved["query"] = moved["query"].transpose(0, 2).contiguous().transpose(0, 2)
+    _check_chunk(case, gpu_device, ops.paged_chunk_attention_native(**moved, window=window, sinks=sinks), window=window, sinks=sinks)
+
+
+@pytest.mark.parametrize("name,factor", [("value_pages", 2.0 ** 21), ("value_pages", 2.0 ** -70), ("value_pages", 2.0 ** -110),
+                                         ("query", 2.0 ** 64), ("query", 2.0 ** -60), ("key_pages", 2.0 ** 70),
+                                         ("key_pages", 2.0 ** -90)])
+def test_chunk_of_many_rows_and_magnitudes(gpu_device, name, factor):
+    """What the limbs do not hold is computed otherwise; every second request has ordinary numbers."""
+    case = _many_rows(73)
+    if name == "query":
+        case["query"][:70] *= factor
+    else:
+        case[name][case["page_table"][0, :9].long()] *= factor
+    if factor > 1 and name != "value_pages":  # the scores stay as they were
+        case["scale"] /= factor
+    expected = steps.chunk_attention(**case)
+    actual = ops.paged_chunk_attention_native(**_to(case, gpu_device))
+    for rows, pages in ((slice(0, 70), case["page_table"][0, :9]), (slice(70, 141), case["page_table"][1:].flatten())):
+        pages = pages[pages >= 0].long()
+        own = {**case, "query": case["query"][rows], "key_pages": case["key_pages"][pages], "value_pages": case["value_pages"][pages]}
+        _close(actual[rows], expected[rows], _bound(own, expected[rows]))
+
+
+@pytest.mark.parametrize("scale", [-0.125, 1e-38, 1e38, -3e38, 1e-45])
+def test_chunk_of_many_rows_and_scales(gpu_device, scale):
+    case = _many_rows(79, scale=scale)
+    if abs(scale) > 1:
+        case["query"].zero_()[..., 0] = 1
+        case["key_pages"][..., 1:] = 0
+        case["key_pages"][..., 0] = case["key_pages"][..., 0].sign()
+    expected = steps.chunk_attention(**case)
+    actual = ops.paged_chunk_attention_native(**_to(case, gpu_device))
+    _close(actual, expected, _bound({**case, "scale": scale if abs(scale) < 1 else 0.0}, expected))
+
+
+def test_chunk_of_many_rows_infinities_and_nan(gpu_device):
+    case = _many_rows(83)
+    table = case["page_table"]
+    case["value_pages"][table[0, 4], 0, 10] = math.nan   # key 74, which the tokens 14 and on of the first request see
+    case["value_pages"][table[1, 50], 0, 3, 0] = math.inf
+    case["key_pages"][table[2, 2], 0, 5] = math.nan
+    expected = steps.chunk_attention(**case)
+    actual = ops.paged_chunk_attention_native(**_to(case, gpu_device)).cpu().double()
+    assert torch.equal(actual.isnan(), expected.isnan()) and torch.equal(actual == math.inf, expected == math.inf)
+    finite = expected.isfinite()
+    assert bool(finite[:14].all()) and not bool(finite[14:70].any()) and not bool(finite[72:132].any()) and bool(finite[132:].all())
+    clean = {**case, "key_pages": case["key_pages"].nan_to_num(posinf=0), "value_pages": case["value_pages"].nan_to_num(posinf=0)}
+    assert float(((actual - expected).abs() - _bound(clean, expected.nan_to_num(posinf=0)))[finite].max()) <= 0
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_chunk_pools_beyond_four_gigabytes(gpu_device, dtype):
+    """Pages whose rows lie behind 2^32 bytes (2^31 elements): rows are written there and attended over."""
+    case = _chunk_case(89, dtype, 16, 1, 64, 16, [(70, 60), (2, 3000), (80, 100)])
+    pages, here = (2 ** 31) // 1024 + 4, case["key_pages"].shape[0]
+    order = torch.cat((torch.arange(2), torch.arange(pages - here + 2, pages)))
+    pools = [torch.empty(pages, 1, 16, 64, device=gpu_device, dtype=dtype) for _ in range(2)]
+    rows = (order[:, None] * 16 + torch.arange(16)).flatten().to(gpu_device)
+    key, value = (case[n].transpose(1, 2).reshape(-1, 1, 64).to(gpu_device) for n in ("key_pages", "value_pages"))
+    ops.paged_cache_write_rows_native(key, value, *pools, rows)
+    table = case["page_table"]
+    far = {**case, "key_pages": pools[0], "value_pages": pools[1], "page_table": torch.where(table >= 0, order[table.long().clamp(min=0)], -1).int()}
+    _check_chunk(case, gpu_device, ops.paged_chunk_attention_native(**_to(far, gpu_device)))
+
+
 def test_chunk_no_tokens_or_requests(gpu_device):
     case = _to(_chunk_case(3, torch.bfloat16, 4, 2, 64, 16, [(3, 5)]), gpu_device)
     nothing = torch.zeros(1, dtype=torch.int64, device=gpu_device)
@@ -512,6 +597,92 @@ def test_sample_strides(gpu_device):
     assert actual.tolist() == steps.sample(one, **options)[0]
 
 
+# Rows that several workgroups take.
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_sample_long_rows_of_ties(gpu_device, dtype):
+    """More equal logits at the end of what is kept than a list holds, and fewer."""
+    g = torch.Generator().manual_seed(19)
+    vocab = 20011
+    logits = torch.randint(0, 4, (8, vocab), generator=g).to(dtype)
+    logits[2] = 0.25  # all equal
+    logits[3, ::2], logits[3, 1::2] = -0.0, 0.0
+    logits[4:6] = torch.randint(0, 200, (2, vocab), generator=g).to(dtype) / 64
+    u = torch.rand(8, generator=g)
+    _check_sample(logits, gpu_device, **_options(g, 8, share=0.8))
+    _check_sample(logits, gpu_device, uniforms=u, top_k=torch.tensor([1, 4000, 9000, 20010, 1030, 5, 2 ** 40, 1024]))
+    _check_sample(logits, gpu_device, uniforms=1 - u / 1000, top_p=torch.tensor([0.1, 0.9, 0.5, 1e-9, 0.2, 0.99, 0.3, 0.7]))
+    _check_sample(logits, gpu_device, uniforms=u, top_k=torch.tensor([3000, 300, 9000, 7, 130, 5000, 9, 20000]),
+                  top_p=torch.tensor([0.6, 0.9, 0.5, 0.1, 0.2, 0.99, 0.3, 0.7]), min_p=torch.tensor([0.2, 0, 1, 0, 0.5, 0, 0, 0]))
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_sample_long_rows_infinities_and_nan(gpu_device, dtype):
+    inf, nan = math.inf, math.nan
+    g = torch.Generator().manual_seed(23)
+    vocab = 9001
+    logits = (2 * torch.randn(9, vocab, generator=g)).to(dtype)
+    logits[0, ::2] = -inf
+    logits[1, :9000] = -inf
+    logits[2] = -inf
+    logits[3, 8500], logits[3, 8600] = inf, inf
+    logits[4, 40], logits[4, 41] = nan, inf
+    logits[5] = torch.finfo(dtype).min
+    logits[5, 7:9] = -inf
+    logits[6] = torch.finfo(dtype).min
+    logits[6, 8999] = torch.finfo(dtype).max
+    logits[7, 1:] = -inf
+    options = _options(g, 9)
+    tokens = _check_sample(logits, gpu_device, **options)
+    assert tokens[1:5].tolist() == [9000, 0, 8500, 40] and tokens[6:8].tolist() == [8999, 0]
+    _check_sample(logits, gpu_device, uniforms=options["uniforms"], temperature=torch.full((9,), inf))
+    _check_sample(logits, gpu_device, uniforms=options["uniforms"], top_k=options["top_k"],
+                  temperature=torch.tensor([0.0, 1e-30, 1e-45, -1.0, nan, 1e30, 3e38, 0.01, 1e-38]))
+
+
+def test_sample_long_rows_strides(gpu_device):
+    g = torch.Generator().manual_seed(29)
+    logits = 3 * torch.randn(4, 20011, generator=g)
+    options = _options(g, 4, share=0.9)
+    for dtype in TYPES:
+        expected = _check_sample(logits.to(dtype), gpu_device, **options)
+        for left in (1, 2, 8):
+            store = torch.full((4, 20033), math.nan, device=gpu_device, dtype=dtype)
+            store[:, left : left + 20011] = logits.to(dtype)
+            assert torch.equal(ops.logits_sample_native(store[:, left : left + 20011], **_to(options, gpu_device))[0], expected)
+        # Rows 2^31 elements apart.
+        store = torch.empty(3 * 2 ** 31 + 20011, device=gpu_device, dtype=dtype) if dtype != torch.float32 else None
+        if store is not None:
+            rows = store.as_strided((4, 20011), (2 ** 31, 1))
+            rows.copy_(logits.to(dtype))
+            assert torch.equal(ops.logits_sample_native(rows, **_to(options, gpu_device))[0], expected)
+
+
+@pytest.mark.parametrize("dtype,vocab", [(torch.float32, 600001), (torch.bfloat16, 1100003)])
+def test_sample_large_vocabularies(gpu_device, dtype, vocab):
+    g = torch.Generator().manual_seed(vocab)
+    logits = (2 * torch.randn(1, vocab, generator=g)).to(dtype)
+    u = torch.rand(1, generator=g)
+    _check_sample(logits, gpu_device, uniforms=u)
+    _check_sample(logits, gpu_device, uniforms=u, top_k=torch.tensor([50]), top_p=torch.tensor([0.7]), min_p=torch.tensor([0.01]))
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_sample_the_largest_vocabulary(gpu_device, dtype):
+    """Sixteen million tokens, a few of which are possible, the first and the last among them."""
+    vocab = 1 << 24
+    places = torch.tensor([0, 1, 511, 512, 70000, 8388607, 8388608, vocab - 2, vocab - 1])
+    few = torch.tensor([[1.0, 0.5, 2.0, 0.0, 1.0, 1.5, -1.0, 0.25, 1.0]])
+    row = torch.full((1, vocab), -math.inf, device=gpu_device, dtype=dtype)
+    row[0, places.to(gpu_device)] = few[0].to(gpu_device).to(dtype)
+    for u in (0.0, 0.1, 0.3, 0.5, 0.7, 0.8, 0.9, 0.95, 1 - 2.0 ** -24):
+        for options in ({}, {"top_k": torch.tensor([4])}, {"top_p": torch.tensor([0.9]), "top_k": torch.tensor([8])},
+                        {"min_p": torch.tensor([0.3])}):
+            options = {"uniforms": torch.tensor([u]), **options}
+            token, _ = ops.logits_sample_native(row, **_to(options, gpu_device))
+            assert int(token) == int(places[steps.sample(few, **options)[0][0]])
+
+
 # --------------------------------------------------------------------------- together
 
 class _Server:
@@ -635,3 +806,26 @@ def test_steps_on_another_stream(gpu_device):
         actual = ops.paged_chunk_attention_native(**moved), *ops.logits_sample_native(later, u)
     torch.cuda.current_stream().wait_stream(stream)
     assert all(torch.equal(a, e) for a, e in zip(actual, expected))
+
+
+def test_two_streams_at_once(gpu_device):
+    """Calls whose tiles are cut and joined, and rows of several workgroups, side by side on two streams."""
+    cases = [_to(_chunk_case(91 + i, dtype, 4, 2, 64, 16, [(40, 5000), (1, 9000), (300 * i, 20)]), gpu_device)
+             for i, dtype in enumerate((torch.bfloat16, torch.float32))]
+    logits = [3 * torch.randn(4, 30000 + 7 * i, device=gpu_device) for i in range(2)]
+    u = torch.rand(4, device=gpu_device)
+    k = torch.tensor([0, 5, 100, 3000], device=gpu_device)
+
+    def call(i):
+        return ops.paged_chunk_attention_native(**cases[i]), *ops.logits_sample_native(logits[i], u, top_k=k)
+
+    expected = [call(i) for i in range(2)]
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    torch.cuda.synchronize()
+    got = [[], []]
+    for _ in range(8):
+        for i in range(2):
+            with torch.cuda.stream(streams[i]):
+                got[i].append(call(i))
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, e) for i in range(2) for one in got[i] for a, e in zip(one, expected[i]))
