@@ -571,6 +571,8 @@ __device__ __forceinline__ void register_rows(const ChunkArgs& a, const ChunkPla
     }
 }
 
+// Other float32 work: bound by latency where it is little (16 tokens over 900 keys: 13 us, of which the plan, the table and the first
+// keys are dependent reads), by the float32 matrix instruction where it is much.
 template <int kDim, Rows kRowsRead>
 __global__ void __launch_bounds__(kThreads, kDim <= 64 ? 3 : (kDim <= 128 ? 2 : 1)) chunk_register_kernel(ChunkArgs a, ChunkPlan plan) {
     constexpr int kRows = rows_of_tile<float>(kDim);
@@ -593,8 +595,14 @@ __global__ void __launch_bounds__(kThreads, kDim <= 64 ? 3 : (kDim <= 128 ? 2 : 
 // keys 8 (r / 4) + 4 h + r % 4 of row n, which rounded in pairs are the right operand of O^T = V^T P; V's left operand, one dim
 // of four keys, comes by reads that transpose 4 x 16 blocks.  A row's 16-byte pieces lie permuted, so that these reads meet
 // different banks: piece c of row r is at c ^ swizzle(r).  Where a stage's rows lie is looked up two stages ahead.  Weights are
-// rounded once to the values' type for the product and summed unrounded; the running maximum moves only when a tile exceeds it
-// by 2^kLazy.
+// rounded once to the values' type for the product and summed unrounded (half a step of a mean's largest value, as the result's own
+// rounding; two terms would double that product); the running maximum moves only when a tile exceeds it by 2^kLazy.
+//
+// Bound by matrix and vector instructions that overlap in part: 4096 tokens behind 28672 (32 / 8 heads of 128, bfloat16) take
+// 2230 us, 930 TFLOP/s; the matrix units are busy for 40% of a SIMD's cycles, the vector ones for 46%, and no bank conflicts.  Keys
+// and values through registers took 3780 us against 2500; a priority for one of a SIMD's two waves changes nothing, and a loop unrolled over
+// the stages' parity spills.  Single tokens fill few of the 128 rows, and HBM bounds them: 32 of them over 4000 keys 98 us,
+// 3.2 TB/s.
 template <int kDim>
 __device__ __forceinline__ int swizzle(int r) {
     if constexpr (kDim == 64) return (r >> 1 & 1) << 2 | (r >> 2 & 3);  // rows of half the banks
@@ -971,9 +979,13 @@ __global__ void __launch_bounds__(kThreads, kDim <= 128 ? 2 : 1) chunk_tile_kern
 // float32 chunks of heads up to 64: products of three bf16 limbs, six of the nine (prefill_limb.h states what they carry), whose rate
 // is 16 / 6 times that of the float32 instruction, closer to 64 bits than that one's sums.  A workgroup's four waves take 32 rows each.
 // The threads fetch a stage's rows while the stage before is worked on, and split them into limbs on the way to LDS, where
-// each limb's rows lie as a 16-bit type's do below.  Scores are in powers of two: the query is multiplied by scale * log2(e).
-// Where limbs do not do (an infinity, a NaN, magnitudes of kLimbMaxScore or kLimbMaxValue on, scores of kFar on, sums so small that
+// each limb's rows lie as a 16-bit type's do above.  Scores are in powers of two: the query is multiplied by scale * log2(e).
+// Where limbs do not do (an infinity, a NaN, magnitudes beyond kLimbMostScore or kLimbMostValue, scores of kFar on, sums so small that
 // bits are lacking) the tile is computed again by register_rows.
+//
+// Bound as the 16-bit kernel is: 4 chunks of prompts (up to 1024 tokens over 7168 keys, 9 / 3 heads of 64) take 221 us,
+// 132 TFLOP/s of float32 products; the matrix units are busy for 37% of the cycles, the vector ones for 41%, most of them splitting
+// rows and weights.  Eight waves 333 us against 287 at that step; sums of their own for the small products 287 against 247 (they spill).
 constexpr float kLimbMostScore = 0x1p60f;  // of a scaled query and of a key: no sum of 64 products overflows
 constexpr float kLimbMostValue = 0x1p19f;
 constexpr float kLimbLeastSum = 0x1p-82f;  // of a row, per 64 keys: bits below 2^-134 of each factor are under 2^-26 of it

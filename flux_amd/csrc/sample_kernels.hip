@@ -14,6 +14,12 @@
 // and a list of the tokens in these; the end's place in that list, the workgroup's part in which the number lies, and the
 // token in it.  Short rows, and rows whose list is too long (thousands of equal logits at the end), are one workgroup's,
 // which finds the end digit by digit of the logits' bits.
+//
+// 128 rows of 128000 bfloat16 logits with all filters: 73 us, of which the largest logit takes 10.5, masses and histogram 24 (the
+// histogram's atomics in LDS), the list 25 (the kept tokens' exponentials in 64 bits; dependent reads before them), the draw 17.
+// Sums by granules of 512 tokens instead of by workgroup took the draw from 27 to 17, the list's early test and the ends
+// read once 91 to 87 in all; loops over a unit's tokens that are not unrolled 95.  One row of 49152 is latency: four
+// launches of 3, 5, 7 and 9 us.
 #include "serving.h"
 
 namespace flux {
