@@ -15,11 +15,11 @@
 // token in it.  Short rows, and rows whose list is too long (thousands of equal logits at the end), are one workgroup's,
 // which finds the end digit by digit of the logits' bits.
 //
-// 128 rows of 128000 bfloat16 logits with all filters: 73 us, of which the largest logit takes 10.5, masses and histogram 24 (the
-// histogram's atomics in LDS), the list 25 (the kept tokens' exponentials in 64 bits; dependent reads before them), the draw 17.
-// Sums by granules of 512 tokens instead of by workgroup took the draw from 27 to 17, the list's early test and the ends
-// read once 91 to 87 in all; loops over a unit's tokens that are not unrolled 95.  One row of 49152 is latency: four
-// launches of 3, 5, 7 and 9 us.
+// 128 rows of 128000 bfloat16 logits with all filters: 73 us, of which the largest logit takes 10.5, masses and histogram 24
+// (exponentials in 64 bits), the list 23 (those of the kept tokens again), the draw 17.  Sums by granules of 512 tokens instead
+// of by workgroup took the draw from 27 to 17, the list's early test and the ends read once 91 to 87 in all, gathering the kept
+// tokens the list from 25 to 23.  Units read ahead and a histogram without its atomics change nothing: instructions bound
+// it.  One row of 49152 is latency: four launches of 3, 5, 7 and 9 us.
 #include "serving.h"
 
 namespace flux {
@@ -294,6 +294,7 @@ __device__ uint64_t find_end(const T* row, int64_t vocab, bool wide, const Weigh
         const int fixed = digit == 0 ? 32 : (digit == 1 ? 21 : 10);
         __syncthreads();
         for (int b = threadIdx.x; b < kDigitBins; b += kThreads) s.mass[b] = 0, s.count[b] = 0;
+        if (threadIdx.x == 0) s.index = 0;  // a bin, also when the logits change during the call
         __syncthreads();
         for (int64_t v = U::kWidth * static_cast<int>(threadIdx.x); v < vocab; v += U::kWidth * kThreads) {
             U unit;
@@ -649,7 +650,7 @@ __global__ void __launch_bounds__(kThreads) sample_list_kernel(SampleArgs a, Sam
     using U = Unit<T>;
     __shared__ EndsShared shared;
     __shared__ double roots[32];
-    __shared__ unsigned long long found[kList];
+    __shared__ unsigned long long found[kList], gathered[kWaves][kWave * U::kWidth];
     __shared__ uint32_t count, first;
     int64_t row;
     int part;
@@ -669,22 +670,33 @@ __global__ void __launch_bounds__(kThreads) sample_list_kernel(SampleArgs a, Sam
     const int last = e.by_count < kSteps && e.by_count > e.last ? e.by_count : e.last;
     const float top = 0.5f * static_cast<float>(o.top), rate = 2.0f * (o.rate < 0x1p126 ? static_cast<float>(o.rate) : 0x1p126f);
     const float far = -static_cast<float>(last + 1);
+    // The others of a wave's unit are gathered, so that a few of them do not take all lanes through the exponential.
+    unsigned long long* near = gathered[threadIdx.x >> 6];
+    const int lane = threadIdx.x & 63;
     walk<T>(a, s, row, part, wide, [&](const U& unit, int64_t v) {
-        uint64_t sum = 0;
+        int held = 0;
 #pragma unroll
         for (int j = 0; j < U::kWidth; ++j) {
-            if ((0.5f * unit[j] - top) * rate < far) continue;
+            const bool is_near = !((0.5f * unit[j] - top) * rate < far);
+            const uint64_t lanes = __ballot(is_near);
+            if (is_near) near[held + __popcll(lanes & ((uint64_t{1} << lane) - 1))] = rank_of(unit[j], static_cast<uint32_t>(v + j));
+            held += __popcll(lanes);
+        }
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        uint64_t sum = 0;
+        for (int i = lane; i < held; i += kWave) {
+            const uint64_t rank = near[i];
             double f;
-            const int step = weigh.step_of(unit[j], f);
-            if (step >= kSteps) continue;
+            const int step = weigh.step_of(value_of(static_cast<uint32_t>(rank >> 32)), f);
             if (step < e.sure) {
                 const uint64_t w = weigh.weight(step, f);
                 sum += w < o.least ? 0 : w;
-            } else if (step <= e.last || step == e.by_count) {
+            } else if (step < kSteps && (step <= e.last || step == e.by_count)) {
                 const uint32_t at = atomicAdd(&count, 1u);
-                if (at < kList) found[at] = rank_of(unit[j], static_cast<uint32_t>(v + j));
+                if (at < kList) found[at] = rank;
             }
         }
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
         return sum;
     }, [&](int granule, uint64_t sum) {
         sum = wave_sum_of(sum);
@@ -803,6 +815,8 @@ __global__ void __launch_bounds__(kThreads) sample_draw_kernel(SampleArgs a, Sam
     for (int i = 0; i < kGranulesEach; ++i) masses += mass[i] = d.mass[kGranulesEach * threadIdx.x + i];
     uint64_t before = block_scan<kThreads>(masses, shared.words, &all) - masses;
     const uint64_t target = drawn_mass(a.uniforms[row], all);
+    if (threadIdx.x == 0) d.index = 0, d.before = 0;  // a granule of the row, also when the logits change during the call
+    __syncthreads();
 #pragma unroll
     for (int i = 0; i < kGranulesEach; ++i) {
         if (mass[i] && before <= target && before + mass[i] > target) d.index = kGranulesEach * threadIdx.x + i, d.before = before;
