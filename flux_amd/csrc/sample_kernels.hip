@@ -49,39 +49,51 @@ __constant__ double kRoots[32] = {
     0x1.306fe0a31b715p-1, 0x1.29e9df51fdee1p-1, 0x1.2387a6e756238p-1, 0x1.1d4873168b9aap-1,
     0x1.172b83c7d517bp-1, 0x1.11301d0125b51p-1, 0x1.0b5586cf9890fp-1, 0x1.059b0d3158574p-1};
 
-// 2^bits exp((x - top) / t), rounded.  In steps of 1/32 below the largest logit, -(x - top) / t log2(e) = (step - f) / 32 with
-// |f| <= 1/2: 2^(-step / 32) from a table of 32 (one for each bank pair of the LDS: no conflicts) and 2^(f / 32) by its
-// Taylor series, whose first term left out, (ln 2 / 64)^6 / 6!, is 2^-48.7.
+// The first 32 threads': 2^(bits + j / 32) in LDS.
+__device__ __forceinline__ void fill_roots(double* roots, int bits) {
+    const int j = threadIdx.x;
+    if (j < 32) roots[j] = ldexp(kRoots[(32 - j) & 31], j ? bits + 1 : bits);
+}
+
+// 2^bits exp((x - top) / t), rounded.  In steps of 1/32 below the largest logit, (x - top) / t log2(e) = (n + f) / 32 with
+// |f| <= 1/2: 2^(n / 32) from a table of 32 (one for each bank pair of the LDS: no conflicts) and 2^(f / 32) by its
+// Taylor series, whose first term left out, (ln 2 / 64)^6 / 6!, is 2^-48.7.  Rounding to integers is an addition that leaves no
+// bits below them: 1.5 2^52 for n, 2^52 for the weight.
 struct Weigher {
     const double* roots;  // in LDS
     double top, rate;     // rate: 32 log2(e) / t
-    int bits;
+    int none;             // step of what weighs nothing: 2^(-1 - 1/32), which is rounded to 0
 
-    // The step, and f; a step beyond those that weigh anything, also for NaN (an infinite temperature's -inf).
+    __device__ __forceinline__ Weigher(const double* table, double largest, double by, int bits)
+        : roots(table), top(largest), rate(by), none(32 * (bits + 1) + 1) {}
+    // -n, and f.  `none` for all beyond it, and for NaN (-inf at an infinite temperature).
     __device__ __forceinline__ int step_of(float x, double& f) const {
-        const double y = (static_cast<double>(x) - top) * rate;
-        if (!(y >= -32.0 * (bits + 1))) return 1 << 20;
-        const double n = __builtin_rint(y);
-        f = y - n;
-        return -static_cast<int>(n);
+        const double y = __builtin_fmax((static_cast<double>(x) - top) * rate, static_cast<double>(-none));
+        const double n = y + 0x1.8p52;
+        f = y - (n - 0x1.8p52);
+        return -static_cast<int>(__double_as_longlong(n));
     }
-    __device__ __forceinline__ double power(int step, double f) const {
+    __device__ __forceinline__ double series(double f) const {
         double p = 0x1.5d87fe78a6731p-35;
         p = fma(p, f, 0x1.3b2ab6fba4e77p-27);
         p = fma(p, f, 0x1.c6b08d704a0c0p-20);
         p = fma(p, f, 0x1.ebfbdff82c58fp-13);
         p = fma(p, f, 0x1.62e42fefa39efp-6);
-        p = fma(p, f, 1.0);
-        return __builtin_amdgcn_ldexp(p * roots[step & 31], bits - (step >> 5));
+        return fma(p, f, 1.0);
     }
-    // An integer below 2^52 by the addition of 2^52.
+    __device__ __forceinline__ double root(int step) const {  // n / 32's whole part goes to the exponent
+        const int n = -step;
+        const int64_t whole = static_cast<int64_t>(n >> 5) << 52;
+        return __longlong_as_double(__double_as_longlong(roots[n & 31]) + whole);
+    }
+    __device__ __forceinline__ double power(int step, double f) const { return series(f) * root(step); }
     __device__ __forceinline__ uint64_t weight(int step, double f) const {
-        return __double_as_longlong(power(step, f) + 0x1p52) - __double_as_longlong(0x1p52);
+        return __double_as_longlong(fma(series(f), root(step), 0x1p52)) - __double_as_longlong(0x1p52);
     }
     __device__ __forceinline__ uint64_t operator()(float x) const {
         double f;
         const int step = step_of(x, f);
-        return step < 1 << 20 ? weight(step, f) : 0;
+        return weight(step, f);
     }
 };
 
@@ -364,7 +376,7 @@ template <class T, int kThreads>
 __device__ void sample_row(const SampleArgs& a, int64_t row, const RowOptions& o, int bits, bool wide, DigitShared& s) {
     using U = Unit<T>;
     const T* in = static_cast<const T*>(a.logits) + row * a.logits_stride;
-    const Weigher weigh{s.roots, o.top, o.rate, bits};
+    const Weigher weigh(s.roots, o.top, o.rate, bits);
     uint64_t end = 0, mass = 0;
     if (o.k < a.vocab) end = find_end<true, T, kThreads>(in, a.vocab, wide, weigh, o.k, s, &mass);
     if (mass == 0) {
@@ -400,7 +412,7 @@ __global__ void __launch_bounds__(kRowThreads) sample_row_kernel(SampleArgs a, i
     __shared__ DigitShared s;
     const int64_t row = blockIdx.x;
     const T* in = static_cast<const T*>(a.logits) + row * a.logits_stride;
-    if (threadIdx.x < 32) s.roots[threadIdx.x] = kRoots[threadIdx.x];
+    fill_roots(s.roots, bits);
     const GivenOptions given(a, row);
     uint64_t best = 0;
     for (int64_t v = U::kWidth * static_cast<int>(threadIdx.x); v < a.vocab; v += U::kWidth * kRowThreads) {
@@ -425,7 +437,7 @@ __global__ void __launch_bounds__(kRowThreads) sample_row_kernel(SampleArgs a, i
 // Several workgroups a row.
 constexpr int kThreads = 512;
 constexpr int kWaves = kThreads / kWave;
-constexpr int kSteps = 1600;  // of weights that are not 0: 32 (bits + 1), at most 48 bits
+constexpr int kSteps = 1600;  // more than those of weights that are not 0, 32 (bits + 1): rows of this kind have at most 48 bits
 constexpr int kList = 1024;   // tokens in the steps where top-k and top-p end
 constexpr int kMostParts = 64;
 constexpr int kGranules = 2048;
@@ -532,7 +544,7 @@ __global__ void __launch_bounds__(kThreads) sample_mass_kernel(SampleArgs a, Sam
     int64_t row;
     int part;
     if (!place_of(a, s, row, part)) return;
-    if (threadIdx.x < 32) roots[threadIdx.x] = kRoots[threadIdx.x];
+    fill_roots(roots, bits);
     const RowOptions o = row_options(a, s, row, bits, words);
     if (!o.draws) {
         if (part == 0 && threadIdx.x == 0) a.tokens[row] = o.greedy, a.probabilities[row] = 1.0f;
@@ -543,7 +555,7 @@ __global__ void __launch_bounds__(kThreads) sample_mass_kernel(SampleArgs a, Sam
         for (int b = threadIdx.x; b < kSteps; b += kThreads) masses[b] = 0, counts[b] = 0;
         __syncthreads();
     }
-    const Weigher weigh{roots, o.top, o.rate, bits};
+    const Weigher weigh(roots, o.top, o.rate, bits);
     if (!filtered) {
         __syncthreads();
         walk<T>(a, s, row, part, wide, [&](const U& unit, int64_t) {
@@ -565,7 +577,7 @@ __global__ void __launch_bounds__(kThreads) sample_mass_kernel(SampleArgs a, Sam
         for (int j = 0; j < U::kWidth; ++j) {
             double f;
             const int step = weigh.step_of(unit[j], f);
-            if (step >= kSteps) continue;
+            if (step >= weigh.none) continue;
             if (by_count) atomicAdd(counts + step, 1u);
             if (by_mass) atomicAdd(masses + step, static_cast<unsigned long long>(weigh.weight(step, f)));
         }
@@ -655,7 +667,7 @@ __global__ void __launch_bounds__(kThreads) sample_list_kernel(SampleArgs a, Sam
     int64_t row;
     int part;
     if (!place_of(a, s, row, part)) return;
-    if (threadIdx.x < 32) roots[threadIdx.x] = kRoots[threadIdx.x];
+    fill_roots(roots, bits);
     const ThreadSteps steps(s, row);
     const RowOptions o = row_options(a, s, row, bits, shared.words);
     if (!o.draws || (o.k >= a.vocab && o.p >= 1.0f)) return;
@@ -663,7 +675,7 @@ __global__ void __launch_bounds__(kThreads) sample_list_kernel(SampleArgs a, Sam
     if (threadIdx.x == 0 && part == 0) s.ends[row] = e;
     if (threadIdx.x == 0) count = 0;
     __syncthreads();
-    const Weigher weigh{roots, o.top, o.rate, bits};
+    const Weigher weigh(roots, o.top, o.rate, bits);
     // Most logits are far below the ends.  Their step to three roundings of 2^-24, of halves whose difference does not overflow, or
     // an earlier one where the rate is beyond float32's, is off by less than 2^-10 of a step: what lies a whole step behind the
     // last is left out by it.
@@ -691,7 +703,7 @@ __global__ void __launch_bounds__(kThreads) sample_list_kernel(SampleArgs a, Sam
             if (step < e.sure) {
                 const uint64_t w = weigh.weight(step, f);
                 sum += w < o.least ? 0 : w;
-            } else if (step < kSteps && (step <= e.last || step == e.by_count)) {
+            } else if (step < weigh.none && (step <= e.last || step == e.by_count)) {
                 const uint32_t at = atomicAdd(&count, 1u);
                 if (at < kList) found[at] = rank;
             }
@@ -725,10 +737,10 @@ __global__ void __launch_bounds__(kThreads) sample_draw_kernel(SampleArgs a, Sam
     __shared__ EndsShared shared;
     __shared__ double roots[32];
     const int64_t row = blockIdx.x;
-    if (threadIdx.x < 32) roots[threadIdx.x] = kRoots[threadIdx.x];
+    fill_roots(roots, bits);
     const RowOptions o = row_options(a, s, row, bits, shared.words);
     if (!o.draws) return;
-    const Weigher weigh{roots, o.top, o.rate, bits};
+    const Weigher weigh(roots, o.top, o.rate, bits);
     const T* in = static_cast<const T*>(a.logits) + row * a.logits_stride;
     DrawShared& d = u.draw;
     const int64_t granule = static_cast<int64_t>(s.units) * kWave * Unit<T>::kWidth;
@@ -743,7 +755,7 @@ __global__ void __launch_bounds__(kThreads) sample_draw_kernel(SampleArgs a, Sam
         const uint32_t listed = s.listed[row];
         if (listed > kList) {
             __syncthreads();
-            if (threadIdx.x < 32) u.digits.roots[threadIdx.x] = kRoots[threadIdx.x];
+            fill_roots(u.digits.roots, bits);
             __syncthreads();
             sample_row<T, kThreads>(a, row, o, bits, wide, u.digits);
             return;
