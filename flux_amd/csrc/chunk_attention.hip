@@ -212,6 +212,11 @@ __device__ Part part_of(const ChunkArgs& a, const ChunkPlan& plan, int place, bo
             }
             units_to += units_before, slots_to += slots_before, splits_to += splits_before;
             units_before += units_here, slots_before += slots_here, splits_before += splits_here;
+            // Only offsets that decrease come this far; a round adds 2^30 and some at most, and no part from there on is anybody's.
+            constexpr int kMost = 1 << 29;
+            units_before = units_before < kMost ? units_before : kMost;
+            slots_before = slots_before < kMost ? slots_before : kMost;
+            splits_before = splits_before < kMost ? splits_before : kMost;
             if (one_round) all_units = units_before, all_splits = splits_before;
             if (round == 0) continue;
             const int strip = (all_units + kStrips - 1) / kStrips;
@@ -1339,6 +1344,10 @@ __global__ void __launch_bounds__(kThreads) chunk_join_kernel(ChunkArgs a, Chunk
     if (static_cast<int>(blockIdx.x) >= header[0]) return;
     const int* d = header + kDescription * (1 + blockIdx.x);
     const int begin = d[0], row0 = d[1], rows = d[2], slot = d[3], parts = d[4];
+    // With offsets that decrease some tile's first part may be no workgroup's, and its description anything.
+    if (begin < 0 || row0 < 0 || rows < 0 || rows > plan.slot_rows || parts < 2 || slot < 0 ||
+        static_cast<int64_t>(slot) + parts > plan.slots || static_cast<int64_t>(row0) + rows > (a.tokens - begin) * a.group)
+        return;
     const int kv_head = blockIdx.y, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const int64_t stride = static_cast<int64_t>(plan.slot_rows) * plan.width;
     const int each = (rows + gridDim.z - 1) / gridDim.z, from = blockIdx.z * each, to = from + each < rows ? from + each : rows;

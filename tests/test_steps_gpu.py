@@ -255,6 +255,37 @@ def test_chunk_strides_and_alignment(gpu_device, dtype):
 
 
 @pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("heads,kv_heads,dim,page_size", [(200, 1, 16, 1), (130, 2, 72, 1000), (257, 1, 64, 17), (64, 64, 8, 3)])
+def test_chunk_wide_groups_and_odd_pages(gpu_device, dtype, heads, kv_heads, dim, page_size):
+    """Groups beyond a tile's rows, many KV heads, pages of one row and pages beyond every length."""
+    case = _chunk_case(97, dtype, heads, kv_heads, dim, page_size, [(3, 50), (1, 700), (0, 5), (20, 0)], spare_rows=2)
+    _check_chunk(case, gpu_device)
+    _check_chunk(case, gpu_device, window=33, sinks=2)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("window", [0, 40, 1 << 24])
+def test_chunk_tables_of_the_largest_width(gpu_device, dtype, window):
+    case = _chunk_case(101, dtype, 4, 2, 64, 16, [(3, 50), (1, 700), (80, 100)])
+    device = _to(case, gpu_device)
+    wide = torch.full((3, (1 << 24) // 16), -1, dtype=torch.int32, device=gpu_device)
+    wide[:, : case["page_table"].shape[1]] = device["page_table"]
+    out = ops.paged_chunk_attention_native(**{**device, "page_table": wide}, window=window, sinks=window)
+    _check_chunk(case, gpu_device, out, window=window, sinks=window)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_chunk_offsets_that_decrease(gpu_device, dtype):
+    """Not allowed, and within bounds all the same."""
+    case = _chunk_case(103, dtype, 4, 2, 64, 16, [(10, 3000), (40, 600), (30, 100)])
+    device = _to(case, gpu_device)
+    for offsets in ([0, 50, 10, 80], [80, 0, 80, 0], [-5, 2 ** 62, -(2 ** 62), 80], [70, 60, 50, 40]):
+        device["offsets"] = torch.tensor(offsets, device=gpu_device)
+        assert ops.paged_chunk_attention_native(**device).shape == case["query"].shape
+    torch.cuda.synchronize()
+
+
+@pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("dim", [64, 80, 128])
 def test_chunk_infinities_and_nan(gpu_device, dtype, dim):
     """They reach the tokens that see them, and no others; scores of -inf weigh nothing."""
