@@ -96,13 +96,13 @@ struct KeyStages {
     __device__ __forceinline__ int base(int t) const { return (t < sink_stages ? t : first_stage + t - sink_stages) * kStage; }
 };
 
-// Positions of the rows [from, from + rows) that are a key's; first > last when there is none.
+// Positions of the rows [from, from + rows) that are a key's; 0 and -1 when there is none.
 __device__ __forceinline__ void positions_of(const ChunkArgs& a, const Sequence& s, int from, int rows, int& first, int& last) {
     const int all = s.count * a.group, to = from + rows < all ? from + rows - 1 : all - 1;
     const int p = s.start + static_cast<int>(divide(from, a.group_of)), q = s.start + static_cast<int>(divide(to < 0 ? 0 : to, a.group_of));
     first = p < 0 ? 0 : p;
     last = q >= s.n ? s.n - 1 : q;
-    if (from > to) last = first - 1;
+    if (from > to || first > last) first = 0, last = -1;
 }
 
 // Stages of a request's longest tile, at most.
