@@ -161,7 +161,7 @@ __device__ __forceinline__ void clear_other_rows(const ChunkArgs& a, int before,
 
 // Parts lie in kStrips strips, from which the workgroups take one each in turn: what runs at the same time is then of all
 // requests, chunks that matrix instructions bound next to single tokens that memory does.  A step of both in bfloat16 (2
-// chunks of some 1000 tokens, 48 single tokens, 15000 keys and fewer) took 765, 762, 788 and 729 us with 1, 4, 16 and 64.
+// chunks of some 1000 tokens, 48 single tokens, 15000 keys and fewer) took 765, 762, 788 and 729 us with 1, 4, 16 and 64, and at a later step 729, 668 and 730 with 16, 64 and 256.
 constexpr int kStrips = 64;
 
 template <class T, int kRows, int kStage>
@@ -606,8 +606,8 @@ __global__ void __launch_bounds__(kThreads, kDim <= 64 ? 3 : (kDim <= 128 ? 2 : 
 // Bound by matrix and vector instructions that overlap in part: 4096 tokens behind 28672 (32 / 8 heads of 128, bfloat16) take
 // 2230 us, 930 TFLOP/s; the matrix units are busy for 40% of a SIMD's cycles, the vector ones for 46%, and no bank conflicts.  Keys
 // and values through registers took 3780 us against 2500; a priority for one of a SIMD's two waves changes nothing, and a loop unrolled over
-// the stages' parity spills.  Single tokens fill few of the 128 rows, and HBM bounds them: 32 of them over 4000 keys 98 us,
-// 3.2 TB/s.
+// the stages' parity spills.  Single tokens fill few of the 128 rows, and HBM bounds them: 32 of them over 4000 keys 95 us,
+// 3.3 TB/s.
 template <int kDim>
 __device__ __forceinline__ int swizzle(int r) {
     if constexpr (kDim == 64) return (r >> 1 & 1) << 2 | (r >> 2 & 3);  // rows of half the banks
@@ -988,8 +988,8 @@ __global__ void __launch_bounds__(kThreads, kDim <= 128 ? 2 : 1) chunk_tile_kern
 // Where limbs do not do (an infinity, a NaN, magnitudes beyond kLimbMostScore or kLimbMostValue, scores of kFar on, sums so small that
 // bits are lacking) the tile is computed again by register_rows.
 //
-// Bound as the 16-bit kernel is: 4 chunks of prompts (up to 1024 tokens over 7168 keys, 9 / 3 heads of 64) take 221 us,
-// 132 TFLOP/s of float32 products; the matrix units are busy for 37% of the cycles, the vector ones for 41%, most of them splitting
+// Bound as the 16-bit kernel is: 4 chunks of prompts (up to 1024 tokens over 7168 keys, 9 / 3 heads of 64) take 216 us,
+// 135 TFLOP/s of float32 products; the matrix units are busy for 37% of the cycles, the vector ones for 41%, most of them splitting
 // rows and weights.  Eight waves 333 us against 287 at that step; sums of their own for the small products 287 against 247 (they spill).
 constexpr float kLimbMostScore = 0x1p60f;  // of a scaled query and of a key: no sum of 64 products overflows
 constexpr float kLimbMostValue = 0x1p19f;
@@ -1389,10 +1389,12 @@ __global__ void __launch_bounds__(kThreads) chunk_join_kernel(ChunkArgs a, Chunk
 
 constexpr int64_t kJoinBlocks = 1024;  // about, many of which find no cut tile (4096: 89 us for 88 of a call, 16384: 93)
 
-// Parts that a step's work is cut into: two rounds of two workgroups on each of 256 CUs, so that a CU whose parts end early
-// takes others.  The step of chunks and single tokens took 860, 809, 787 and 778 us with 512, 768, 1024 and 1536, where more
-// parts write and join more sums: 16 chunks in a window of 2048 keys took 102 us with 1024 and 104 with 2048.
-constexpr int kTarget = 1024;
+// Parts that a step's work is cut into: 16-bit two rounds of two workgroups on each of 256 CUs, so that a CU whose parts end early
+// takes others; more parts write and join more sums.  With 512, 768, 1024, 1280 and 1536 the step of chunks and single tokens took 796, 720,
+// 668, 687 and 645 us, the 16 chunks in a window 121, 82, 88, 89 and 90.  float32, whose single tokens' workgroups are three a
+// CU: 32 of them over 4000 keys 44 us with 768 and 52 with 1024, prompts 226 and 235.
+template <class T>
+constexpr int parts_of_step() { return sizeof(T) == 2 ? 1024 : 768; }
 
 // Whether float32 takes the limb kernel: its tiles have 128 rows, which single tokens leave empty, and few of them leave CUs
 // idle.  Limbs and float32 products: 4 x 512 tokens over 512 keys each 161 and 238 us, 2048 tokens over 8192 253 and 443;
@@ -1412,7 +1414,7 @@ ChunkPlan plan_of(const ChunkArgs& a) {
     const int64_t rows = a.tokens * a.group;
     p.tiles = rows / p.rows + a.requests;
     if (p.tiles > rows) p.tiles = rows;
-    p.target = (kTarget + a.kv_heads - 1) / a.kv_heads;
+    p.target = (parts_of_step<T>() + a.kv_heads - 1) / a.kv_heads;
     int64_t stages = (a.keys + stage - 1) / stage;
     if (a.window > 0) {
         const int64_t windowed = (static_cast<int64_t>(a.sinks) + stage - 1) / stage + (static_cast<int64_t>(a.window) + p.rows / a.group + 1) / stage + 2;
