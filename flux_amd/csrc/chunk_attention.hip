@@ -563,7 +563,7 @@ __device__ __forceinline__ void register_rows(const ChunkArgs& a, const ChunkPla
                 });
             } else {
                 float* o = part_row(a, plan, kv_head, part.slot, r - tile_row0);
-                M::template each_dim<kDim>(g, a.dim, [&](int k, int j, int d) { o[d] = out[c][k][j]; });
+                M::template each_dim<kDim>(g, a.dim, [&](int k, int j, int d) { o[d] = mine[c].position < 0 ? 0.0f : out[c][k][j]; });
                 const float highest = mine[c].position < 0 ? -INFINITY : top[c];
                 if (g == 0) put_statistics(o + plan.width - 4, highest * kLog2e, mine[c].position < 0 ? 0.0f : weight[c], highest);
             }
@@ -966,7 +966,8 @@ __global__ void __launch_bounds__(kThreads, kDim <= 128 ? 2 : 1) chunk_tile_kern
 #pragma unroll
                 for (int j = 0; j < 16; j += 4) {
                     const int d = 32 * i + 2 * j + 4 * half;
-                    if (d < a.dim) *reinterpret_cast<f32x4*>(o + d) = f32x4{out[i][j], out[i][j + 1], out[i][j + 2], out[i][j + 3]};
+                    if (d < a.dim)
+                        *reinterpret_cast<f32x4*>(o + d) = mine.position < 0 ? f32x4{0, 0, 0, 0} : f32x4{out[i][j], out[i][j + 1], out[i][j + 2], out[i][j + 3]};
                 }
             const float highest = mine.position < 0 ? -INFINITY : top;
             if (half == 0)
@@ -1291,10 +1292,11 @@ __global__ void __launch_bounds__(kThreads, 2) chunk_limb_kernel(ChunkArgs a, Ch
 constexpr int kFewParts = 8;
 constexpr int kJoinParts = 1024;  // whose shares are kept
 
+// Nothing is left out where a share is 0: a part's sums may be NaN or infinite, and 0 times these is NaN as in a tile that is not cut.
 __device__ __forceinline__ float share_of(const float* statistics, float top, float natural) {
     const bool near = fabsf(top) < kFar && fabsf(statistics[0]) < kFar;
     const float share = fast_exp2(near ? statistics[0] - top : (statistics[2] - natural) * kLog2e);
-    return statistics[1] != 0.0f ? share : 0.0f;  // else it saw nothing, or its sums are zeros
+    return statistics[2] == -INFINITY ? 0.0f : share;  // it saw nothing, or no score above -inf that is a number
 }
 
 template <class T>
@@ -1328,10 +1330,10 @@ __device__ __forceinline__ void join_few(const ChunkArgs& a, const ChunkPlan& pl
 #pragma unroll
         for (int p = 0; p < kMost; ++p) {
             const float own[3] = {statistics[p][0], statistics[p][1], statistics[p][2]};
-            const float share = p < parts ? share_of(own, top, natural) : 0.0f;
-            weight += share != 0.0f ? own[1] * share : 0.0f;
+            const float share = share_of(own, top, natural);
+            weight += p < parts ? own[1] * share : 0.0f;
 #pragma unroll
-            for (int l = 0; l < 4; ++l) sum[l] += share != 0.0f ? sums[p][l] * share : 0.0f;
+            for (int l = 0; l < 4; ++l) sum[l] += p < parts ? sums[p][l] * share : 0.0f;
         }
         store_joined<T>(a, begin, row0 + r, kv_head, four, weight, sum);
     }
@@ -1366,7 +1368,7 @@ __global__ void __launch_bounds__(kThreads) chunk_join_kernel(ChunkArgs a, Chunk
         float weight = 0.0f;
         for (int p = lane; p < parts; p += kWave) {
             const float share = share_of(of + p * stride, top, natural);
-            weight += share != 0.0f ? of[p * stride + 1] * share : 0.0f;
+            weight += of[p * stride + 1] * share;
             if (p < kJoinParts) shares[wave][p] = share;
         }
         weight = wave_sum(weight);
@@ -1377,7 +1379,7 @@ __global__ void __launch_bounds__(kThreads) chunk_join_kernel(ChunkArgs a, Chunk
                 const f32x4 part_sum = *reinterpret_cast<const f32x4*>(o + p * stride + 4 * four);
                 const float share = p < kJoinParts ? shares[wave][p] : share_of(of + p * stride, top, natural);
 #pragma unroll
-                for (int l = 0; l < 4; ++l) sum[l] += share != 0.0f ? part_sum[l] * share : 0.0f;
+                for (int l = 0; l < 4; ++l) sum[l] += part_sum[l] * share;
             }
         }
         for (int step = 1 << fours_bits; step < kWave; step *= 2)

@@ -1,0 +1,73 @@
+"""Mixed steps where parts of a tile, or numbers next to a limit, could go another way than the whole (``oracle/steps.py``)."""
+
+from __future__ import annotations
+
+import math
+
+import pytest
+import torch
+
+from flux_amd import ops
+from oracle import steps
+from tests.test_steps_gpu import TYPES, _bound, _chunk_case, _close, _to
+
+pytestmark = pytest.mark.gpu
+
+# Heads, KV heads, head dimension, tokens of the one request, keys before them: tiles in two parts and more (at most 4, 8, and
+# beyond), float32 on its own instruction and, from 2048 rows on, in limbs.
+CUT = [(4, 2, 64, 1, 700), (4, 2, 64, 3, 1100), (4, 2, 128, 1, 600), (4, 2, 128, 20, 1500), (4, 1, 80, 1, 4400), (2, 1, 256, 5, 900),
+       (32, 1, 64, 70, 400), (32, 1, 40, 70, 3000), (1, 1, 64, 1, 20000)]
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("heads,kv_heads,dim,tokens,before", CUT)
+def test_nan_that_fills_a_part_reaches_the_row(gpu_device, dtype, heads, kv_heads, dim, tokens, before):
+    """Three quarters of the keys are NaN, so that whole parts have no other score: every row that sees one is NaN."""
+    case = _chunk_case(dim + before, dtype, heads, kv_heads, dim, 16, [(tokens, before)])
+    pages = case["page_table"][0, : before * 3 // 4 // 16].long()
+    case["key_pages"][pages] = math.nan
+    expected = steps.chunk_attention(**case)
+    assert bool(expected.isnan().all())
+    assert bool(ops.paged_chunk_attention_native(**_to(case, gpu_device)).isnan().all())
+    # The token's own key alone.
+    case = _chunk_case(dim + before, dtype, heads, kv_heads, dim, 16, [(1, before // 64 * 64)])
+    case["key_pages"][case["page_table"][0, before // 64 * 4].long(), :, 0] = math.nan
+    assert bool(ops.paged_chunk_attention_native(**_to(case, gpu_device)).isnan().all())
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("heads,kv_heads,dim,tokens,before", CUT)
+@pytest.mark.parametrize("score", [-300.0, -math.inf])
+def test_nan_and_infinite_values_behind_no_weight_reach_the_row(gpu_device, dtype, heads, kv_heads, dim, tokens, before, score):
+    """0 times NaN or infinity is NaN, also where a whole part's weights are 0 next to another's: scores 300 below, and -inf."""
+    case = _chunk_case(dim + before + 1, dtype, heads, kv_heads, dim, 16, [(tokens, before)], scale=0.125)
+    case["query"][..., 0] = 1
+    table = case["page_table"][0].long()
+    pages = table[: before * 3 // 4 // 16]
+    case["key_pages"][table, :, :, 0] = 0
+    case["key_pages"][pages, :, :, 0] = 8 * score
+    clean = {**case, "value_pages": case["value_pages"].clone(), "key_pages": case["key_pages"].nan_to_num(neginf=-2400)}
+    for bad in (math.nan, math.inf):
+        case["value_pages"][pages[3], :, 5, dim // 2] = bad
+        actual = ops.paged_chunk_attention_native(**_to(case, gpu_device)).cpu()
+        assert not bool(actual[..., dim // 2].isfinite().any())
+    expected = steps.chunk_attention(**clean)
+    kept = [d for d in range(dim) if d != dim // 2]
+    close = {**clean, "key_pages": case["key_pages"].clamp(min=-64).nan_to_num()}  # the far ones' scores are no term
+    _close(actual[..., kept], expected[..., kept], _bound(close, expected)[..., kept])
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("heads,kv_heads,dim,tokens,before", CUT)
+def test_rows_that_see_nothing_stay_zero_next_to_nan(gpu_device, dtype, heads, kv_heads, dim, tokens, before):
+    """In cut tiles: a token before the first key, and a request whose pages are all gone (NaN stands for what is not its own)."""
+    case = _chunk_case(dim + before + 2, dtype, heads, kv_heads, dim, 16, [(tokens, before)])
+    case["key_pages"][case["page_table"][0, :2].long()] = math.nan
+    case["value_pages"][case["page_table"][0, :2].long()] = math.nan
+    positions = torch.tensor([-1])
+    expected = steps.chunk_attention(**case, positions=positions)
+    actual = ops.paged_chunk_attention_native(**_to(case, gpu_device), positions=positions.to(gpu_device)).cpu()
+    assert not bool(actual[0].any()) and torch.equal(actual.isnan(), expected.isnan())
+    gone = {**case, "key_pages": torch.full_like(case["key_pages"], math.nan), "value_pages": torch.full_like(case["key_pages"], math.nan),
+            "page_table": torch.full_like(case["page_table"], -1)}
+    assert not bool(ops.paged_chunk_attention_native(**_to(gone, gpu_device)).any())
