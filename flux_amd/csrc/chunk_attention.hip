@@ -283,10 +283,10 @@ __device__ __forceinline__ Row row_of(const ChunkArgs& a, const Sequence& s, int
     return row;
 }
 
-// Weights are 2^(s log2(e) - top) by one fused product, top = m log2(e) rounded: what that moves is common to
-// all weights of a row and cancels, unless top is so large that it moves them out of float32's range.  From kFar on the
-// difference s - m is taken first.
-constexpr float kFar = 4194304.0f;
+// Weights are 2^(s log2(e) - top) by one fused product, top = m log2(e) rounded: what that moves is common to all weights that
+// refer to one maximum.  Where sums are rescaled or joined it is not, and below kFar it is then 2^-16 of a weight at most (with
+// kShift in the sum).  From kFar on the difference s - m is taken first.
+constexpr float kFar = 256.0f;
 // Of a weight relative to one of another maximum.
 __device__ __forceinline__ float exponent_of(float maximum, float other) {
     const float scaled = other * kLog2e;
@@ -986,7 +986,7 @@ __global__ void __launch_bounds__(kThreads, kDim <= 128 ? 2 : 1) chunk_tile_kern
 // is 16 / 6 times that of the float32 instruction, closer to 64 bits than that one's sums.  A workgroup's four waves take 32 rows each.
 // The threads fetch a stage's rows while the stage before is worked on, and split them into limbs on the way to LDS, where
 // each limb's rows lie as a 16-bit type's do above.  Scores are in powers of two: the query is multiplied by scale * log2(e).
-// Where limbs do not do (an infinity, a NaN, magnitudes beyond kLimbMostScore or kLimbMostValue, scores of kFar on, sums so small that
+// Where limbs do not do (an infinity, a NaN, magnitudes beyond kLimbMostScore or kLimbMostValue, scores of kLimbFar on, sums so small that
 // bits are lacking) the tile is computed again by register_rows.
 //
 // Bound as the 16-bit kernel is: 4 chunks of prompts (up to 1024 tokens over 7168 keys, 9 / 3 heads of 64) take 216 us,
@@ -994,6 +994,7 @@ __global__ void __launch_bounds__(kThreads, kDim <= 128 ? 2 : 1) chunk_tile_kern
 // rows and weights.  Eight waves 333 us against 287 at that step; sums of their own for the small products 287 against 247 (they spill).
 constexpr float kLimbMostScore = 0x1p60f;  // of a scaled query and of a key: no sum of 64 products overflows
 constexpr float kLimbMostValue = 0x1p19f;
+constexpr float kLimbFar = 1024.0f;  // of a score, whose rounding then moves a weight by 2^-14 of itself at most
 constexpr float kLimbLeastSum = 0x1p-82f;  // of a row, per 64 keys: bits below 2^-134 of each factor are under 2^-26 of it
 
 __device__ __forceinline__ bool beyond(const f32x4& a, const f32x4& b, float most) {
@@ -1252,7 +1253,7 @@ __global__ void __launch_bounds__(kThreads, 2) chunk_limb_kernel(ChunkArgs a, Ch
             least = min(least, magnitude_key(out[b][j]));
         }
     unsure |= least < magnitude_key(kLimbLeastSum * static_cast<float>(to - from + 1));
-    unsure |= mine.position >= 0 && top != -INFINITY && !(fabsf(top) < kFar);
+    unsure |= mine.position >= 0 && top != -INFINITY && !(fabsf(top) < kLimbFar);
     if (__syncthreads_or(unsure)) {
         for (int row = row0; row < row0 + kRows && row < all_rows; row += rows_of_tile<float>(kDim)) {
             register_rows<kDim, kWide ? kWideRows : kNarrow>(a, plan, s, part, kv_head, row0, row, stages, from, to, reinterpret_cast<float*>(planes));

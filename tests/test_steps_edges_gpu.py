@@ -71,3 +71,23 @@ def test_rows_that_see_nothing_stay_zero_next_to_nan(gpu_device, dtype, heads, k
     gone = {**case, "key_pages": torch.full_like(case["key_pages"], math.nan), "value_pages": torch.full_like(case["key_pages"], math.nan),
             "page_table": torch.full_like(case["page_table"], -1)}
     assert not bool(ops.paged_chunk_attention_native(**_to(gone, gpu_device)).any())
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("heads,kv_heads,dim,tokens,before", CUT)
+@pytest.mark.parametrize("size", [11.0, 2.0 ** 8, 2.0 ** 9, 2.0 ** 10, 2.0 ** 12])
+def test_scores_that_are_exact_count_exactly(gpu_device, dtype, heads, kv_heads, dim, tokens, before, size):
+    """Scores of 121, 2^16 to 2^24 and a few, exact in float32, that rise along the keys: the maximum moves, and what was summed
+    before has to keep its weight."""
+    case = _chunk_case(dim + before + 3, dtype, heads, kv_heads, dim, 16, [(tokens, before)], scale=1.0)
+    case["query"].zero_()[..., 0] = size
+    case["query"][..., 1] = 1
+    key, n = case["key_pages"], tokens + before
+    key.nan_to_num_().zero_()
+    key[..., 0] = size
+    rise = (torch.arange(n) * 64 // n).to(dtype)  # by one, 64 times
+    at = torch.arange(n)
+    key[case["page_table"][0, at // 16].long(), :, at % 16, 1] = (rise if size < 2.0 ** 12 else rise // 2 * 2)[:, None]
+    expected = steps.chunk_attention(**case)
+    actual = ops.paged_chunk_attention_native(**_to(case, gpu_device))
+    _close(actual, expected, _bound({**case, "scale": 0.0}, expected))
