@@ -293,8 +293,19 @@ __device__ __forceinline__ float exponent_of(float maximum, float other) {
     return fabsf(scaled) < kFar ? maximum * kLog2e - scaled : (maximum - other) * kLog2e;
 }
 
+// What a score <q, k> is multiplied by: before the maximum is looked for, and in the argument of 2^x.  16-bit types' leave all of the
+// scale's size to the argument, where it is neither 0 nor next to what float32 holds (chunk_tile_kernel says why).
+template <class T>
+struct ScoreScale {
+    float before, argument;
+    __device__ __forceinline__ ScoreScale(float scale) : before(scale), argument(kLog2e) {
+        const float size = fabsf(scale);
+        if (sizeof(T) == 2 && size >= 1e-30f && size <= 1e30f) before = scale < 0.0f ? -1.0f : 1.0f, argument = size * kLog2e;
+    }
+};
+
 // What the join needs to know of a part's row: the maximum that its weights refer to, in powers of two, its sum of weights, and the
-// maximum of the scores.
+// maximum of the scores, as ScoreScale leaves them before the argument: the difference of two of them does not overflow.
 __device__ __forceinline__ void put_statistics(float* to, float top, float weight, float natural) {
     to[0] = top;
     to[1] = weight;
@@ -314,6 +325,7 @@ __device__ void exact_row(const ChunkArgs& a, const ChunkPlan& plan, const Seque
     const T* keys = static_cast<const T*>(a.key) + kv_head * a.key_strides[1];
     const T* values = static_cast<const T*>(a.value) + kv_head * a.value_strides[1];
     const int32_t* table = a.table + (s.slot < 0 ? 0 : s.slot) * a.table_stride;
+    const ScoreScale<T> scale(a.scale);
     float top = -INFINITY, weight = 0.0f, sum[kServingMaxDim / kWave];
 #pragma unroll
     for (int c = 0; c < kServingMaxDim / kWave; ++c) sum[c] = 0.0f;
@@ -333,13 +345,13 @@ __device__ void exact_row(const ChunkArgs& a, const ChunkPlan& plan, const Seque
             score = 0.0f;
             for (int d = 0; d < a.dim; ++d)
                 score = fmaf(static_cast<float>(query[d * a.query_strides[2]]), static_cast<float>(key[d]), score);
-            score *= a.scale;
+            score *= scale.before;
         }
         const float now = fmaxf(top, wave_max(score));
-        const float reference = now == -INFINITY ? 0.0f : now, scaled = reference * kLog2e;
+        const float reference = now == -INFINITY ? 0.0f : now, scaled = reference * scale.argument;
         const bool near = fabsf(scaled) < kFar;
-        auto difference = [&](float x) { return near ? fmaf(x, kLog2e, -scaled) : (x - reference) * kLog2e; };
-        const float shrink = top == -INFINITY ? 0.0f : fast_exp2(near ? top * kLog2e - scaled : (top - reference) * kLog2e);
+        auto difference = [&](float x) { return near ? fmaf(x, scale.argument, -scaled) : (x - reference) * scale.argument; };
+        const float shrink = top == -INFINITY ? 0.0f : fast_exp2(difference(top));
         top = now;
         const float p = seen ? fast_exp2(difference(score) + shift) : 0.0f;
         weight = weight * shrink + wave_sum(p);
@@ -369,7 +381,7 @@ __device__ void exact_row(const ChunkArgs& a, const ChunkPlan& plan, const Seque
         if (partial) partial[d] = sum[c];
         else out[d] = static_cast<T>(weight == 0.0f ? 0.0f : sum[c] / weight);
     }
-    if (partial && lane == 0) put_statistics(partial + plan.width - 4, top * kLog2e, weight, top);
+    if (partial && lane == 0) put_statistics(partial + plan.width - 4, top * scale.argument, weight, top);
 }
 
 // ---------------------------------------------------------------------------
@@ -971,7 +983,7 @@ __global__ void __launch_bounds__(kThreads, kDim <= 128 ? 2 : 1) chunk_tile_kern
                 }
             const float highest = mine.position < 0 ? -INFINITY : top;
             if (half == 0)
-                put_statistics(o + plan.width - 4, highest * factor, mine.position < 0 ? 0.0f : weight, ordinary ? highest * size : highest);
+                put_statistics(o + plan.width - 4, highest * factor, mine.position < 0 ? 0.0f : weight, highest);
         }
     }
     while (again) {
@@ -1294,9 +1306,9 @@ constexpr int kFewParts = 8;
 constexpr int kJoinParts = 1024;  // whose shares are kept
 
 // Nothing is left out where a share is 0: a part's sums may be NaN or infinite, and 0 times these is NaN as in a tile that is not cut.
-__device__ __forceinline__ float share_of(const float* statistics, float top, float natural) {
+__device__ __forceinline__ float share_of(const float* statistics, float top, float natural, float argument) {
     const bool near = fabsf(top) < kFar && fabsf(statistics[0]) < kFar;
-    const float share = fast_exp2(near ? statistics[0] - top : (statistics[2] - natural) * kLog2e);
+    const float share = fast_exp2(near ? statistics[0] - top : (statistics[2] - natural) * argument);
     return statistics[2] == -INFINITY ? 0.0f : share;  // it saw nothing, or no score above -inf that is a number
 }
 
@@ -1314,6 +1326,7 @@ template <class T, int kMost>
 __device__ __forceinline__ void join_few(const ChunkArgs& a, const ChunkPlan& plan, int begin, int row0, int slot, int parts, int from, int to) {
     const int kv_head = blockIdx.y, fours = (a.dim + 3) / 4;
     const int64_t stride = static_cast<int64_t>(plan.slot_rows) * plan.width;
+    const ScoreScale<T> scale(a.scale);
     for (int item = threadIdx.x; item < (to - from) * fours; item += kThreads) {
         const int r = from + item / fours, four = item % fours;
         const float* o = part_row(a, plan, kv_head, slot, r);
@@ -1331,7 +1344,7 @@ __device__ __forceinline__ void join_few(const ChunkArgs& a, const ChunkPlan& pl
 #pragma unroll
         for (int p = 0; p < kMost; ++p) {
             const float own[3] = {statistics[p][0], statistics[p][1], statistics[p][2]};
-            const float share = share_of(own, top, natural);
+            const float share = share_of(own, top, natural, scale.argument);
             weight += p < parts ? own[1] * share : 0.0f;
 #pragma unroll
             for (int l = 0; l < 4; ++l) sum[l] += p < parts ? sums[p][l] * share : 0.0f;
@@ -1357,6 +1370,7 @@ __global__ void __launch_bounds__(kThreads) chunk_join_kernel(ChunkArgs a, Chunk
     if (parts <= 2) return join_few<T, 2>(a, plan, begin, row0, slot, parts, from, to);
     if (parts <= 4) return join_few<T, 4>(a, plan, begin, row0, slot, parts, from, to);
     if (parts <= kFewParts) return join_few<T, kFewParts>(a, plan, begin, row0, slot, parts, from, to);
+    const ScoreScale<T> scale(a.scale);
     const int four = lane & ((1 << fours_bits) - 1), turn = lane >> fours_bits, turns = kWave >> fours_bits;
     for (int r = from + wave; r < to; r += kWaves) {
         const float* o = part_row(a, plan, kv_head, slot, r);
@@ -1368,7 +1382,7 @@ __global__ void __launch_bounds__(kThreads) chunk_join_kernel(ChunkArgs a, Chunk
         natural = wave_max(natural);
         float weight = 0.0f;
         for (int p = lane; p < parts; p += kWave) {
-            const float share = share_of(of + p * stride, top, natural);
+            const float share = share_of(of + p * stride, top, natural, scale.argument);
             weight += of[p * stride + 1] * share;
             if (p < kJoinParts) shares[wave][p] = share;
         }
@@ -1378,7 +1392,7 @@ __global__ void __launch_bounds__(kThreads) chunk_join_kernel(ChunkArgs a, Chunk
 #pragma unroll 8
             for (int p = turn; p < parts; p += turns) {
                 const f32x4 part_sum = *reinterpret_cast<const f32x4*>(o + p * stride + 4 * four);
-                const float share = p < kJoinParts ? shares[wave][p] : share_of(of + p * stride, top, natural);
+                const float share = p < kJoinParts ? shares[wave][p] : share_of(of + p * stride, top, natural, scale.argument);
 #pragma unroll
                 for (int l = 0; l < 4; ++l) sum[l] += part_sum[l] * share;
             }

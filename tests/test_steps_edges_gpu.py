@@ -91,3 +91,19 @@ def test_scores_that_are_exact_count_exactly(gpu_device, dtype, heads, kv_heads,
     expected = steps.chunk_attention(**case)
     actual = ops.paged_chunk_attention_native(**_to(case, gpu_device))
     _close(actual, expected, _bound({**case, "scale": 0.0}, expected))
+
+
+@pytest.mark.parametrize("dtype", TYPES[1:])
+@pytest.mark.parametrize("heads,kv_heads,dim,tokens,before", CUT)
+def test_scaled_scores_beyond_float32_in_cut_tiles(gpu_device, dtype, heads, kv_heads, dim, tokens, before):
+    """16-bit scores are multiplied by the scale in the exponent's argument, after the maximum is taken off: three keys of 2^30
+    among 2^29, times 1e30, share the row whether or not they lie in one part."""
+    case = _chunk_case(dim + before + 4, dtype, heads, kv_heads, dim, 16, [(tokens, before)], scale=1e30)
+    case["query"].zero_()[..., 0] = 2.0 ** 15
+    key, table = case["key_pages"], case["page_table"][0].long()
+    key.nan_to_num_().zero_()[..., 0] = 2.0 ** 14
+    for j in (before // 8, before // 2, before - 1):
+        key[table[j // 16], :, j % 16, 0] = 2.0 ** 15
+    expected = steps.chunk_attention(**case)
+    actual = ops.paged_chunk_attention_native(**_to(case, gpu_device))
+    _close(actual, expected, _bound({**case, "scale": 0.0}, expected))
