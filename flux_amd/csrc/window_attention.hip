@@ -346,7 +346,10 @@ __global__ void __launch_bounds__(kThreads, kDim <= 64 ? 4 : (kDim <= 128 ? 2 : 
 // at most half a step of that type relative to themselves, which moves a weighted mean of the values by at most half a step
 // of the largest of them, as the result's own rounding does.  They are summed unrounded in float32.  (Two terms a weight, as
 // in paged_attention.hip, would double the matrix instructions of the product, here where they bound the kernel.)
+// The maximum in powers of two is rounded, which is common to all weights and cancels.  From 2^24 on it is no longer (float16's
+// 2^11 is lost in part next to it, and then its rounding takes all weights out of float32's range): such rows are computed again.
 constexpr int64_t kStagedStride = 1 << 22;
+constexpr float kMostTop = 0x1p24f;
 
 // Rows of one stage.  With kWide 16 bytes at a byte offset through a buffer that ends with the last row (kStagedStride
 // keeps offsets in 31 bits); else eight elements, of the last row where there is none.
@@ -561,7 +564,8 @@ window_tile_kernel(AttentionArgs a, int row_tiles, int tiles_total) {
     for (int i = 0; i < kBlocks; ++i)
 #pragma unroll
         for (int j = 0; j < 16; ++j) worst += fabsf(out[i][j]);  // keeps NaN, infinity
-    const uint64_t odd = __ballot(mine.position >= 0 && !(worst < INFINITY));
+    const bool far = top > -INFINITY && !(fabsf(top) < kMostTop);
+    const uint64_t odd = __ballot(mine.position >= 0 && (far || !(worst < INFINITY)));
     uint32_t again = static_cast<uint32_t>(odd | odd >> 32);
     if (real && !(again >> n32 & 1)) {
         T* o = static_cast<T*>(a.out) + ((rows.b * a.query_heads + head) * a.queries + query_index) * a.dim;

@@ -1201,3 +1201,25 @@ def test_offsets_beyond_32_bits(gpu_device):
         q = case["query"][:, :, :queries]
         expected = ops.window_attention_native(**{**case, "query": q}, window=90, sinks=5)
         assert torch.equal(ops.window_attention_native(q, **spread, scale=case["scale"], window=90, sinks=5), expected)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("dim", [64, 128, 256])
+@pytest.mark.parametrize("size,dims", [(11.0, 1), (2.0 ** 8, 1), (2.0 ** 10, 1), (2.0 ** 12, 1), (3 * 2.0 ** 13, 1), (2.0 ** 15, 1),
+                                       (2.0 ** 15, 4), (2.0 ** 15, 6), (2.0 ** 15, 7), (2.0 ** 15, 11), (2.0 ** 15, 16)])
+def test_window_large_scores_that_are_exact_count_exactly(gpu_device, dtype, dim, size, dims):
+    """Scores of 121 to 2^34 that rise along the keys by the smallest steps float32 holds there (1 at least), so that the maximum
+    moves and what was summed before keeps its weight; and such that are all equal, of which none is lost."""
+    n, base = 700, dims * size * size
+    step = max(1.0, 2.0 ** (math.floor(math.log2(base)) - 23))
+    case = {**_window_case(67, dtype, 1, 2, 1, dim, 40, n), "scale": 1.0}
+    for name in ("query", "key"):
+        case[name].zero_()[..., :dims] = size
+    case["query"][..., 20] = 1
+    case["key"][0, 0, :, 20] = ((torch.arange(n) * 16 // n) * step).to(dtype)
+    for window, sinks, equal in ((0, 0, False), (300, 5, False), (300, 5, True)):
+        if equal:
+            case["key"][..., 20] = 0
+        expected = ref.window_attention(**case, window=window, sinks=sinks)
+        bound = ref.attention_bound(case["query"], case["key"], case["value"], 0.0, n, dtype, expected, True)
+        _close(ops.window_attention_native(**_to(case, gpu_device), window=window, sinks=sinks), expected, bound)
