@@ -7,6 +7,8 @@
 // planned in 7.5), the copies by HBM (40 pages of 30 layers, 59 MB moved, in 11.8 us).
 #include "serving.h"
 
+#include <type_traits>
+
 namespace flux {
 namespace {
 
@@ -532,14 +534,49 @@ __global__ void __launch_bounds__(256) page_compact_kernel(PagePool p, PageBooks
 // looked up once; every thread requests kAhead units before it writes any.
 constexpr int kWriteTokens = 16;
 
-// The rows of `tokens` tokens, from `sources` (keys, values) to their places: bytes from the pool's start, -1: nowhere.
-template <class Unit>
-__device__ __forceinline__ void move_rows(const PagePool& p, const int64_t (&place)[2][kWriteTokens], int tokens,
-                                          const char* key, const char* value, int64_t key_head, int64_t key_token,
-                                          int64_t value_head, int64_t value_token) {
+// Two forms of the arguments: a padded batch whose places are looked up, and packed tokens whose rows of the pool are given (row
+// r is row r % page of page r / page).  16384 packed tokens of 8 heads of 128 in 16 bits take 24 us, 5.7 TB/s read and written (partly
+// out of the memory-side cache); 16 tokens 4.6.  Both forms in one kernel, because a loop that two of them call takes 81 registers
+// instead of 67, five waves instead of seven (16 prompts to 1000 tokens 9.7 us against 8.6).
+template <class Unit, class Args>
+__global__ void __launch_bounds__(256) page_write_kernel(PagePool p, Args a) {
     constexpr int kBytes = sizeof(Unit);
+    constexpr bool kPacked = std::is_same_v<Args, PageRowsArgs>;
+    constexpr int kHead = 1, kToken = kPacked ? 0 : 2;  // strides
+    __shared__ int64_t place[2][kWriteTokens];  // bytes from the pool's start, -1: no page
+    const int64_t t0 = static_cast<int64_t>(blockIdx.x) * kWriteTokens;
+    int64_t i = 0, count = a.tokens, page = -1, row = 0;
+    if constexpr (!kPacked) {
+        i = blockIdx.y;
+        const int64_t slot = a.slot_list[i], start = a.positions[i];
+        if (slot < 0 || slot >= a.slots || start < 0) return;
+        if (a.counts) count = a.counts[i];
+        if (count > a.tokens) count = a.tokens;
+        const int64_t capacity = a.columns * p.page;
+        if (start >= capacity) return;
+        if (count > capacity - start) count = capacity - start;
+        if (t0 >= count) return;
+        if (static_cast<int>(threadIdx.x) < kWriteTokens && t0 + static_cast<int>(threadIdx.x) < count) {
+            const uint32_t position = static_cast<uint32_t>(start + t0 + threadIdx.x), rows = static_cast<uint32_t>(p.page);
+            page = a.table[slot * a.table_stride + position / rows];
+            row = position % rows;
+        }
+    } else if (static_cast<int>(threadIdx.x) < kWriteTokens && t0 + static_cast<int>(threadIdx.x) < count) {
+        const int64_t of = a.rows[t0 + threadIdx.x];
+        page = of < 0 ? -1 : of / p.page;
+        row = of - page * p.page;
+    }
+    const int tokens = static_cast<int>(count - t0 < kWriteTokens ? count - t0 : kWriteTokens);
+    if (static_cast<int>(threadIdx.x) < tokens) {
+        const bool held = page >= 0 && page < p.pages;
+        place[0][threadIdx.x] = held ? (page * p.key_strides[1] + row * p.key_strides[3]) * p.element : -1;
+        place[1][threadIdx.x] = held ? (page * p.value_strides[1] + row * p.value_strides[3]) * p.element : -1;
+    }
+    __syncthreads();
     const uint32_t width = p.row_units.divisor, heads = p.of_heads.divisor;
     const int side = static_cast<int>(tokens * heads * width);
+    const char* sources[2] = {a.key + ((kPacked ? 0 : i * a.key_strides[0]) + t0 * a.key_strides[kToken]) * p.element,
+                              a.value + ((kPacked ? 0 : i * a.value_strides[0]) + t0 * a.value_strides[kToken]) * p.element};
     constexpr int kEach = 2 * kAhead;
     for (int first = threadIdx.x; first < 2 * side; first += kEach * 256) {
         Unit held[kEach];
@@ -554,58 +591,14 @@ __device__ __forceinline__ void move_rows(const PagePool& p, const int64_t (&pla
             const int64_t where = place[s][t];
             if (where < 0) continue;
             to[j] = (s ? p.value : p.key) + where + head * (s ? p.value_strides : p.key_strides)[2] * p.element + u * kBytes;
-            held[j] = *reinterpret_cast<const Unit*>((s ? value : key) + (head * (s ? value_head : key_head) +
-                                                                          t * (s ? value_token : key_token)) * p.element + u * kBytes);
+            held[j] = *reinterpret_cast<const Unit*>((s ? sources[1] : sources[0]) +
+                                                     (head * (s ? a.value_strides : a.key_strides)[kHead] +
+                                                      t * (s ? a.value_strides : a.key_strides)[kToken]) * p.element + u * kBytes);
         }
 #pragma unroll
         for (int j = 0; j < kEach; ++j)
             if (to[j]) store_unit(to[j], held[j]);
     }
-}
-
-template <class Unit>
-__global__ void __launch_bounds__(256) page_write_kernel(PagePool p, PageWriteArgs a) {
-    __shared__ int64_t place[2][kWriteTokens];
-    const int64_t i = blockIdx.y;
-    const int64_t slot = a.slot_list[i], start = a.positions[i];
-    if (slot < 0 || slot >= a.slots || start < 0) return;
-    int64_t count = a.counts ? a.counts[i] : a.tokens;
-    if (count > a.tokens) count = a.tokens;
-    const int64_t capacity = a.columns * p.page;
-    if (start >= capacity) return;
-    if (count > capacity - start) count = capacity - start;
-    const int64_t t0 = static_cast<int64_t>(blockIdx.x) * kWriteTokens;
-    if (t0 >= count) return;
-    const int tokens = static_cast<int>(count - t0 < kWriteTokens ? count - t0 : kWriteTokens);
-    if (static_cast<int>(threadIdx.x) < tokens) {
-        const uint32_t position = static_cast<uint32_t>(start + t0 + threadIdx.x), rows = static_cast<uint32_t>(p.page);
-        const int64_t page = a.table[slot * a.table_stride + position / rows], row = position % rows;
-        const bool held = page >= 0 && page < p.pages;
-        place[0][threadIdx.x] = held ? (page * p.key_strides[1] + row * p.key_strides[3]) * p.element : -1;
-        place[1][threadIdx.x] = held ? (page * p.value_strides[1] + row * p.value_strides[3]) * p.element : -1;
-    }
-    __syncthreads();
-    move_rows<Unit>(p, place, tokens, a.key + (i * a.key_strides[0] + t0 * a.key_strides[2]) * p.element,
-                    a.value + (i * a.value_strides[0] + t0 * a.value_strides[2]) * p.element, a.key_strides[1],
-                    a.key_strides[2], a.value_strides[1], a.value_strides[2]);
-}
-
-// The same for packed tokens whose rows of the pool are given (row r is row r % page of page r / page).  16384 tokens of 8
-// heads of 128 in 16 bits take 24 us, 5.7 TB/s read and written (partly out of the memory-side cache); 16 tokens 4.6.
-template <class Unit>
-__global__ void __launch_bounds__(256) page_write_rows_kernel(PagePool p, PageRowsArgs a) {
-    __shared__ int64_t place[2][kWriteTokens];
-    const int64_t t0 = static_cast<int64_t>(blockIdx.x) * kWriteTokens;
-    const int tokens = static_cast<int>(a.tokens - t0 < kWriteTokens ? a.tokens - t0 : kWriteTokens);
-    if (static_cast<int>(threadIdx.x) < tokens) {
-        const int64_t of = a.rows[t0 + threadIdx.x], page = of / p.page, row = of - page * p.page;
-        const bool held = of >= 0 && page < p.pages;
-        place[0][threadIdx.x] = held ? (page * p.key_strides[1] + row * p.key_strides[3]) * p.element : -1;
-        place[1][threadIdx.x] = held ? (page * p.value_strides[1] + row * p.value_strides[3]) * p.element : -1;
-    }
-    __syncthreads();
-    move_rows<Unit>(p, place, tokens, a.key + t0 * a.key_strides[0] * p.element, a.value + t0 * a.value_strides[0] * p.element,
-                    a.key_strides[1], a.key_strides[0], a.value_strides[1], a.value_strides[0]);
 }
 
 // ---------------------------------------------------------------------------
@@ -773,7 +766,7 @@ hipError_t launch_page_write(const PagePool& plain, const PageWriteArgs& args, h
 hipError_t launch_page_write_rows(const PagePool& plain, const PageRowsArgs& args, hipStream_t stream) {
     const dim3 grid(static_cast<uint32_t>((args.tokens + kWriteTokens - 1) / kWriteTokens));
     const PagePool pool = with_units(plain, rows_of(plain, 16) && rows_of(args, plain.element, 16));
-    FLUX_BY_UNIT(pool, page_write_rows_kernel, grid, args);
+    FLUX_BY_UNIT(pool, page_write_kernel, grid, args);
 }
 
 #undef FLUX_BY_UNIT
