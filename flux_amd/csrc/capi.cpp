@@ -1245,9 +1245,12 @@ int flux_logits_process(int dtype, const void* logits, int64_t logits_stride, vo
 
 }  // extern "C"
 
+static bool sample_shape(int64_t rows, int64_t vocab) {
+    return rows > 0 && rows <= (1 << 20) && vocab > 0 && vocab <= (1 << 24) && rows <= (int64_t{1} << 32) / (vocab + 1023);
+}
+
 int flux_logits_sample_workspace_bytes(int64_t rows, int64_t vocab, int64_t* bytes) {
-    if (!bytes || rows <= 0 || rows > (1 << 20) || vocab <= 0 || vocab > (1 << 24))
-        return invalid("flux_logits_sample_workspace_bytes: invalid argument");
+    if (!bytes || !sample_shape(rows, vocab)) return invalid("flux_logits_sample_workspace_bytes: invalid argument");
     *bytes = static_cast<int64_t>(flux::sample_workspace_bytes(rows, vocab));
     return FLUX_OK;
 }
@@ -1257,9 +1260,7 @@ int flux_logits_sample(int dtype, const void* logits, int64_t logits_stride, con
                        int64_t rows, int64_t vocab, void* workspace, int64_t workspace_bytes, hipStream_t stream) {
     if (!logits || !uniforms || !tokens || !probabilities) return invalid("flux_logits_sample: null argument");
     if (!known_type(dtype)) return invalid("flux_logits_sample: unknown dtype");
-    if (rows <= 0 || rows > (1 << 20) || vocab <= 0 || vocab > (1 << 24) || logits_stride < 0 ||
-        rows > (int64_t{1} << 32) / (vocab + 1023))
-        return invalid("flux_logits_sample: invalid shape");
+    if (!sample_shape(rows, vocab) || logits_stride < 0) return invalid("flux_logits_sample: invalid shape");
     const auto needed = static_cast<int64_t>(flux::sample_workspace_bytes(rows, vocab));
     if (needed > 0 && (!workspace || workspace_bytes < needed))
         return invalid("flux_logits_sample: workspace missing or too small (flux_logits_sample_workspace_bytes)");

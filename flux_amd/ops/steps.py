@@ -207,8 +207,10 @@ def _chunk_cuda(query, key_pages, value_pages, page_table, lengths, offsets, sca
 
 def _validate_sample(logits, uniforms, temperature=None, top_k=None, top_p=None, min_p=None) -> None:
     shape, device = logits.shape, logits.device
-    if not (len(shape) == 2 and shape[0] > 0 and 0 < shape[1] <= _MAX_VOCAB):
-        _check(False, "flux::logits_sample: logits must be [rows, vocab], non-empty, vocab at most 16777216")
+    if not (len(shape) == 2 and 0 < shape[1] <= _MAX_VOCAB):
+        _check(False, "flux::logits_sample: logits must be [rows, vocab], vocab non-empty and at most 16777216")
+    if not (shape[0] <= 1 << 20 and shape[0] * (shape[1] + 1023) <= 1 << 32):
+        _check(False, "flux::logits_sample: more than 1048576 rows, or rows * (vocab + 1023) beyond 4294967296")
     if not (logits.dtype in _TYPES):
         _check(False, "flux::logits_sample: logits must have dtype float32, float16 or bfloat16")
     if not (logits.stride(1) == 1 or shape[1] == 1):
@@ -232,6 +234,8 @@ def _sample_cuda(logits, uniforms, temperature=None, top_k=None, top_p=None, min
     rows, vocab = logits.shape
     tokens = logits.new_empty(rows, dtype=torch.int64)
     probabilities = logits.new_empty(rows, dtype=torch.float32)
+    if rows == 0:
+        return tokens, probabilities
     needed = _size_from("flux_logits_sample_workspace_bytes", rows, vocab)
     workspace = tokens.new_empty(needed // 8) if needed else None
     _launch("flux_logits_sample", logits.device, _TYPES[logits.dtype], logits.data_ptr(), logits.stride(0),
@@ -348,7 +352,8 @@ def logits_sample_native(logits: torch.Tensor, uniforms: torch.Tensor, temperatu
     All options are vectors with an entry per row.  After division by ``temperature`` (0: greedy) the ``top_k`` largest
     logits are kept (0: all), of those the largest while the mass before them is below ``top_p``, of those the ones
     at least ``min_p`` times as probable as the largest; equal logits are kept from the lowest index on.  The token is the
-    first, by index, at which the kept mass exceeds ``uniforms`` times all of it; its probability is its share.
+    first, by index, at which the kept mass exceeds ``uniforms`` times all of it; its probability is its share.  No rows (a step
+    in which no prompt ends) give empty results.
     """
     _ready("logits sample")
     return _OPS.logits_sample(logits, uniforms, temperature, top_k, top_p, min_p)

@@ -216,3 +216,26 @@ def test_c_entries_refuse_before_any_launch():
         assert message in _native.last_error(), change
     assert lib.flux_logits_sample_workspace_bytes(2, 128000, ctypes.byref(size)) == 0
     assert lib.flux_logits_sample_workspace_bytes(0, 100, ctypes.byref(size)) == bad
+
+
+def _sample_meta(rows, vocab):
+    return {"logits": torch.empty(rows, vocab), "uniforms": torch.empty(rows)}
+
+
+@pytest.mark.parametrize("rows,vocab", [((1 << 20) + 1, 8), (1 << 20, 1 << 13), (1 << 9, 1 << 24)])
+def test_sampling_beyond_the_c_entries_limits_is_refused_by_every_layer(rows, vocab):
+    with FakeTensorMode(), pytest.raises(RuntimeError, match="more than 1048576 rows"):
+        torch.ops.flux.logits_sample(**_sample_meta(rows, vocab))
+    logits = torch.zeros(vocab).expand(rows, vocab)
+    with pytest.raises(RuntimeError, match="more than 1048576 rows"):
+        torch.ops.flux.logits_sample(logits, torch.zeros(rows))
+    size = ctypes.c_int64()
+    assert _native.load().flux_logits_sample_workspace_bytes(rows, vocab, ctypes.byref(size)) == _native.FLUX_ERROR_INVALID_VALUE
+
+
+def test_sampling_no_rows_is_a_valid_call():
+    with FakeTensorMode():
+        tokens, probabilities = torch.ops.flux.logits_sample(**_sample_meta(0, 100))
+    assert tokens.shape == probabilities.shape == (0,) and tokens.dtype == i64 and probabilities.dtype == f32
+    with pytest.raises(RuntimeError, match="no CPU kernel"):
+        torch.ops.flux.logits_sample(torch.zeros(0, 100), torch.zeros(0))

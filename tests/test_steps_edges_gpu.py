@@ -107,3 +107,11 @@ def test_scaled_scores_beyond_float32_in_cut_tiles(gpu_device, dtype, heads, kv_
     expected = steps.chunk_attention(**case)
     actual = ops.paged_chunk_attention_native(**_to(case, gpu_device))
     _close(actual, expected, _bound({**case, "scale": 0.0}, expected))
+
+
+@pytest.mark.parametrize("vocab", [100, 128000])
+def test_sampling_no_rows_gives_nothing(gpu_device, vocab):
+    options = {name: torch.empty(0, device=gpu_device) for name in ("temperature", "top_p", "min_p")}
+    tokens, probabilities = ops.logits_sample_native(torch.empty(0, vocab, device=gpu_device), torch.empty(0, device=gpu_device),
+                                                     top_k=torch.empty(0, dtype=torch.int64, device=gpu_device), **options)
+    assert tokens.shape == probabilities.shape == (0,) and tokens.dtype == torch.int64 and probabilities.dtype == torch.float32
