@@ -922,6 +922,8 @@ const char* chunk_arguments(flux::ChunkArgs& args, int dtype, float scale, int64
     args.sinks = static_cast<int>(sinks);
     args.pages = pages;
     args.page = flux::make_divider(static_cast<uint32_t>(page_size));
+    if (flux::chunk_attention_workgroups(args, static_cast<flux::Type>(dtype)) >= (int64_t{1} << 24))  // a grid has below 2^32 threads
+        return "the rows' tiles are 2^24 or more over all KV heads";
     return nullptr;
 }
 

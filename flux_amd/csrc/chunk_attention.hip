@@ -1482,12 +1482,13 @@ hipError_t launch_tiles(const ChunkArgs& a, const ChunkPlan& plan, dim3 grid, hi
     }
 }
 
+// Every strip ends with a whole turn of kStrips.
+int64_t workgroups_of(const ChunkArgs& a, const ChunkPlan& plan) { return (plan.units + kStrips - 1) * a.kv_heads; }
+
 template <class T>
 hipError_t launch_chunks(const ChunkArgs& a, hipStream_t stream) {
     const ChunkPlan plan = plan_of<T>(a);
-    const int64_t blocks = (plan.units + kStrips - 1) * a.kv_heads;
-    if (blocks >= (int64_t{1} << 24)) return hipErrorInvalidValue;  // a grid has below 2^32 threads
-    const dim3 grid(static_cast<uint32_t>(blocks));
+    const dim3 grid(static_cast<uint32_t>(workgroups_of(a, plan)));
     hipError_t launched;
     // The 16-bit kernel leaves the last quarter of a row out: 97 us for 103 at 80 dims.
     constexpr int kNarrower = sizeof(T) == 2 ? 96 : 128;
@@ -1511,6 +1512,10 @@ hipError_t launch_chunks(const ChunkArgs& a, hipStream_t stream) {
 size_t chunk_attention_workspace_floats(const ChunkArgs& a, Type type) {
     const ChunkPlan p = type == Type::kFloat32 ? plan_of<float>(a) : plan_of<__bf16>(a);
     return p.whole ? 0 : static_cast<size_t>(parts_offset(p) + a.kv_heads * p.slots * p.slot_rows * p.width);
+}
+
+int64_t chunk_attention_workgroups(const ChunkArgs& a, Type type) {
+    return workgroups_of(a, type == Type::kFloat32 ? plan_of<float>(a) : plan_of<__bf16>(a));
 }
 
 hipError_t launch_chunk_attention(const ChunkArgs& args, Type type, hipStream_t stream) {

@@ -119,6 +119,8 @@ struct ChunkArgs {
 };
 
 size_t chunk_attention_workspace_floats(const ChunkArgs& args, Type type);
+// Workgroups of the main launch, 256 threads each.
+int64_t chunk_attention_workgroups(const ChunkArgs& args, Type type);
 hipError_t launch_chunk_attention(const ChunkArgs& args, Type type, hipStream_t stream);
 
 // ---- cache pages ----

@@ -94,6 +94,10 @@ def _validate_rows(key, value, key_pages, value_pages, rows) -> None:
         _check(False, "flux::paged_cache_write_rows: key and value must have unit stride along the head dimension")
     if not (shape[0] <= _MAX_KEYS):
         _check(False, "flux::paged_cache_write_rows: more than 16777216 tokens")
+    if not (pages[0] <= 1 << 28 and pages[2] <= _MAX_KEYS and max(pages[1], pages[3]) <= 1 << 20 and pages[1] * pages[3] <= 1 << 24 and
+            pages[1] * pages[2] * pages[3] <= 1 << 28):
+        _check(False, "flux::paged_cache_write_rows: more than 268435456 pages or elements a page, 16777216 rows a page or elements "
+                      "a token, or 1048576 heads or dims")
     _check_list(rows, torch.int64, device,
                 "flux::paged_cache_write_rows: rows must be a contiguous int64 vector on the cache's device",
                 shape[0], "flux::paged_cache_write_rows: rows must have one entry per token")
@@ -126,6 +130,14 @@ def _rows_cuda(key, value, key_pages, value_pages, rows):
 # ---------------------------------------------------------------------------
 # paged_chunk_attention
 
+def _workgroups(shape, kv_heads, dtype, requests) -> int:
+    """At most, of a call: its tiles, each request's last one partly filled, and what they are cut into."""
+    rows = shape[0] * (shape[1] // kv_heads)
+    whole = dtype is not torch.float32 or shape[2] <= 64 and rows >= max(64 * requests, 2048)
+    tiles = min(rows, rows // (128 if whole else 32 if shape[2] <= 128 else 16) + requests)
+    return (tiles + 1024 // kv_heads + 64) * kv_heads
+
+
 def _validate_chunk(query, key_pages, value_pages, page_table, lengths, offsets, scale, window=0, sinks=0, slots=None,
                     positions=None) -> None:
     shape, pages, table, dtype, device = query.shape, key_pages.shape, page_table.shape, query.dtype, query.device
@@ -143,6 +155,8 @@ def _validate_chunk(query, key_pages, value_pages, page_table, lengths, offsets,
         _check(False, "flux::paged_chunk_attention: query heads must be divisible by KV heads")
     if not (shape[0] <= _MAX_KEYS and shape[0] * (shape[1] // pages[1]) <= 1 << 27):
         _check(False, "flux::paged_chunk_attention: more than 16777216 tokens or 134217728 rows of a KV head")
+    if not (shape[1] <= 65535 and pages[0] <= 1 << 28):
+        _check(False, "flux::paged_chunk_attention: more than 65535 query heads or 268435456 pages")
     if not (len(table) == 2 and page_table.dtype is torch.int32 and 0 not in table):
         _check(False, "flux::paged_chunk_attention: page_table must be int32 [slots, columns]")
     if not (page_table.stride(1) == 1 or table[1] == 1):
@@ -157,6 +171,10 @@ def _validate_chunk(query, key_pages, value_pages, page_table, lengths, offsets,
     requests = offsets.shape[0] - 1
     if not (0 <= requests <= _MAX_REQUESTS):
         _check(False, "flux::paged_chunk_attention: offsets must have one entry more than the requests, at most 65535")
+    # The bound of the smallest tiles first: hardly any call is beyond it.
+    if (shape[0] * shape[1] + 16 * ((requests + 64) * pages[1] + 1024) >= 1 << 28 and
+            _workgroups(shape, pages[1], dtype, requests) >= 1 << 24):
+        _check(False, "flux::paged_chunk_attention: the rows' tiles are 16777216 or more over all KV heads")
     if slots is None:
         _check(table[0] >= requests,
                "flux::paged_chunk_attention: without slots page_table must have one row per request")

@@ -484,7 +484,10 @@ int flux_paged_decode_attention(int dtype, const void* query, const void* key_pa
  * (NULL: lengths[r] less its tokens), the others behind it; a token at p sees the keys j <= p, j < lengths[r] with
  * j > p - window or j < sinks (window 0: all).  Keys on a page outside [0, pages) are left out and never read.  A token
  * that sees nothing, nothing whose score is above -inf, with p outside [0, lengths[r]), or of no request gives zeros.
- * Strides: query's token, head, dim; pages' page, head, row.  output contiguous. */
+ * Strides: query's token, head, dim; pages' page, head, row.  output contiguous.  At most 2^24 tokens, 65535 requests and query
+ * heads, 2^27 rows of a KV head (tokens times its query heads), 2^28 pages; the rows' tiles (128 rows, float32's 32 or 16) and
+ * about 1024 parts are below 2^24 over all KV heads.  The workspace's size depends on shapes alone, because lengths are on the device:
+ * to 1024 KV heads at most 138 MB at 128 dims and 273 MB at 256 in 16 bits (2048 parts of 128 rows), 54 MB in float32. */
 int flux_paged_chunk_attention_workspace_bytes(int dtype, int64_t tokens, int64_t requests, int64_t query_heads, int64_t kv_heads,
                                                int64_t head_dim, int64_t page_size, int64_t columns, int64_t window,
                                                int64_t sinks, int64_t* bytes);

@@ -239,3 +239,66 @@ def test_sampling_no_rows_is_a_valid_call():
     assert tokens.shape == probabilities.shape == (0,) and tokens.dtype == i64 and probabilities.dtype == f32
     with pytest.raises(RuntimeError, match="no CPU kernel"):
         torch.ops.flux.logits_sample(torch.zeros(0, 100), torch.zeros(0))
+
+
+def _fake_chunk(tokens, heads, kv_heads, dim, requests=1, pages=5, dtype=torch.bfloat16):
+    return {"query": torch.empty(tokens, heads, dim, dtype=dtype), "key_pages": torch.empty(pages, kv_heads, 4, dim, dtype=dtype),
+            "value_pages": torch.empty(pages, kv_heads, 4, dim, dtype=dtype), "page_table": torch.empty(requests, 3, dtype=i32),
+            "lengths": torch.empty(requests, dtype=i64), "offsets": torch.empty(requests + 1, dtype=i64), "scale": 0.25}
+
+
+def _refused_by_c(dtype, tokens, heads, kv_heads, dim, requests=1, columns=4000):
+    size = ctypes.c_int64()
+    return _native.load().flux_paged_chunk_attention_workspace_bytes(dtype, tokens, requests, heads, kv_heads, dim, 4, columns, 0, 0,
+                                                                     ctypes.byref(size)) != 0
+
+
+@pytest.mark.parametrize("sizes,message", [((1, 65536, 65536, 16), "more than 65535 query heads"),
+                                           ((1, 65535, 65535, 16), None),
+                                           ((1 << 24, 128, 128, 128), "tiles are 16777216 or more"),
+                                           ((1 << 23, 128, 128, 128), None)])
+def test_chunk_sizes_beyond_the_c_entries_limits_are_refused_by_every_layer(sizes, message):
+    with FakeTensorMode():
+        if message:
+            with pytest.raises(RuntimeError, match=message):
+                torch.ops.flux.paged_chunk_attention(**_fake_chunk(*sizes))
+        else:
+            assert torch.ops.flux.paged_chunk_attention(**_fake_chunk(*sizes)).shape == (sizes[0], sizes[1], sizes[3])
+        with pytest.raises(RuntimeError, match="268435456 pages"):
+            torch.ops.flux.paged_chunk_attention(**_fake_chunk(1, 1, 1, 16, pages=(1 << 28) + 1))
+    assert _refused_by_c(2, *sizes) == (message is not None)
+    lib, three = _native.load(), (ctypes.c_int64 * 3)(64, 16, 1)
+    some = ctypes.c_void_p(16)  # never dereferenced
+    if message and "tiles" in message:
+        assert lib.flux_paged_chunk_attention(2, some, some, some, some, some, some, None, None, some, some, 1 << 40, 1.0, sizes[0], 1,
+                                              *sizes[1:], 4, 4, 2, 400, 400, 0, 0, three, three, three, None) == _native.FLUX_ERROR_INVALID_VALUE
+        assert "tiles" in _native.last_error()
+
+
+@pytest.mark.parametrize("dtype", [0, 1, 2])
+def test_what_the_c_entry_refuses_for_its_tiles_is_refused_before(dtype):
+    of = {0: f32, 1: torch.float16, 2: torch.bfloat16}[dtype]
+    refused = 0
+    for heads, kv_heads in ((1, 1), (7, 7), (128, 128), (128, 16), (1000, 1000), (8192, 8192), (65535, 65535)):
+        for dim in (16, 64, 65, 128, 129):
+            for requests in (1, 3000, 65535):
+                for tokens in (1, 3, 255, 2048, 65535, 1 << 20, 1 << 21, 1 << 22, 1 << 23, (1 << 24) - 1):
+                    if tokens * (heads // kv_heads) > 1 << 27 or not _refused_by_c(dtype, tokens, heads, kv_heads, dim, requests):
+                        continue
+                    refused += 1
+                    assert steps._workgroups((tokens, heads, dim), kv_heads, of, requests) >= 1 << 24
+                    assert tokens * heads + 16 * ((requests + 64) * kv_heads + 1024) >= 1 << 28
+    assert refused > 20
+
+
+@pytest.mark.parametrize("shape", [((1 << 28) + 1, 1, 1, 1), (1, 1, (1 << 24) + 1, 1), (1, (1 << 20) + 1, 1, 1), (1, 1, 1, (1 << 20) + 1),
+                                   (1, 1 << 13, 1, (1 << 11) + 1), (1, 1 << 10, 1 << 10, 257)])
+def test_row_writes_beyond_the_c_entries_limits_are_refused_by_every_layer(shape):
+    with FakeTensorMode(), pytest.raises(RuntimeError, match="more than 268435456 pages or elements a page"):
+        torch.ops.flux.paged_cache_write_rows(torch.empty(2, shape[1], shape[3]), torch.empty(2, shape[1], shape[3]), torch.empty(shape),
+                                              torch.empty(shape), torch.empty(2, dtype=i64))
+    pool = _native.PagePool(key=1 << 32, value=1 << 60, layers=1, pages=shape[0], heads=shape[1], page_size=shape[2], head_dim=shape[3], dtype=0)
+    pool.key_strides[:] = pool.value_strides[:] = (0, shape[1] * shape[2] * shape[3], shape[2] * shape[3], shape[3])
+    two, some = (ctypes.c_int64 * 2)(shape[1] * shape[3], shape[3]), ctypes.c_void_p(16)
+    assert _native.load().flux_page_write_rows(ctypes.byref(pool), some, some, two, two, 2, some, None) == _native.FLUX_ERROR_INVALID_VALUE
+    assert "shape" in _native.last_error()
