@@ -1264,8 +1264,8 @@ int flux_logits_sample(int dtype, const void* logits, int64_t logits_stride, con
     if (!known_type(dtype)) return invalid("flux_logits_sample: unknown dtype");
     if (!sample_shape(rows, vocab) || logits_stride < 0) return invalid("flux_logits_sample: invalid shape");
     const auto needed = static_cast<int64_t>(flux::sample_workspace_bytes(rows, vocab));
-    if (needed > 0 && (!workspace || workspace_bytes < needed))
-        return invalid("flux_logits_sample: workspace missing or too small (flux_logits_sample_workspace_bytes)");
+    if (needed > 0 && (!workspace || !aligned16(workspace) || workspace_bytes < needed))  // 64-bit atomics
+        return invalid("flux_logits_sample: workspace missing, too small (flux_logits_sample_workspace_bytes) or not 16-byte aligned");
     flux::SampleArgs args{};
     args.logits = logits;
     args.logits_stride = logits_stride;

@@ -623,7 +623,7 @@ int flux_logits_process(int dtype, const void* logits, int64_t logits_stride, vo
  * first of any weight, u >= 1: the last); probabilities[row]: its share of them.  A row whose temperature is not above 0 or whose
  * largest logit is not finite gives the lowest index of the largest logit (NaN above all numbers) and 1.  Vectors [rows];
  * NULL: temperature 1, no filter.  At most 2^20 rows, 2^24 tokens each, rows * (vocab + 1023) at most 2^32.  Weights are held in integers of 2^-b, b = min(51, 62 - ceil(log2 vocab)): results
- * do not depend on scheduling. */
+ * do not depend on scheduling.  The workspace is aligned to 16 bytes. */
 int flux_logits_sample_workspace_bytes(int64_t rows, int64_t vocab, int64_t* bytes);
 int flux_logits_sample(int dtype, const void* logits, int64_t logits_stride, const float* uniforms, const float* temperature,
                        const int64_t* top_k, const float* top_p, const float* min_p, int64_t* tokens, float* probabilities,

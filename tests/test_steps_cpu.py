@@ -302,3 +302,13 @@ def test_row_writes_beyond_the_c_entries_limits_are_refused_by_every_layer(shape
     two, some = (ctypes.c_int64 * 2)(shape[1] * shape[3], shape[3]), ctypes.c_void_p(16)
     assert _native.load().flux_page_write_rows(ctypes.byref(pool), some, some, two, two, 2, some, None) == _native.FLUX_ERROR_INVALID_VALUE
     assert "shape" in _native.last_error()
+
+
+def test_sampling_refuses_a_workspace_that_its_atomics_cannot_use():
+    lib, size, some = _native.load(), ctypes.c_int64(), ctypes.c_void_p(16)  # never dereferenced
+    assert lib.flux_logits_sample_workspace_bytes(2, 128000, ctypes.byref(size)) == 0 and size.value > 0
+    for workspace, given in ((None, size.value), (ctypes.c_void_p(64), size.value - 1), (ctypes.c_void_p(68), size.value),
+                             (ctypes.c_void_p(72), size.value)):
+        assert lib.flux_logits_sample(0, some, 128000, some, None, None, None, None, some, some, 2, 128000, workspace, given,
+                                      None) == _native.FLUX_ERROR_INVALID_VALUE
+        assert "16-byte aligned" in _native.last_error()
