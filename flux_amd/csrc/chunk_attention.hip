@@ -1386,6 +1386,7 @@ __global__ void __launch_bounds__(kThreads) chunk_join_kernel(ChunkArgs a, Chunk
             weight += of[p * stride + 1] * share;
             if (p < kJoinParts) shares[wave][p] = share;
         }
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");  // other lanes of the wave read them
         weight = wave_sum(weight);
         f32x4 sum = {0, 0, 0, 0};
         if (4 * four < a.dim) {
@@ -1400,6 +1401,7 @@ __global__ void __launch_bounds__(kThreads) chunk_join_kernel(ChunkArgs a, Chunk
         for (int step = 1 << fours_bits; step < kWave; step *= 2)
 #pragma unroll
             for (int l = 0; l < 4; ++l) sum[l] += __shfl_xor(sum[l], step, kWave);
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");  // the next row's shares take their places
         if (turn == 0) store_joined<T>(a, begin, row0 + r, kv_head, four, weight, sum);
     }
 }
