@@ -642,10 +642,17 @@ __device__ __forceinline__ u32x2 read_transposed(const char* at) {
 }
 
 // out *= shrink where `moves`.  In assembly, with its branch inside: behind a branch of the compiler's the sums' registers are
-// moved in the other arm, 64 moves a tile.  The waits cover the matrix instructions that wrote the sums and read them next.
+// moved in the other arm, 64 moves a tile.  The compiler does not count what an assembly block needs, so it waits itself: a matrix
+// instruction's result is there 11 states later (what the compiler leaves before its own reads of one), here 32; the next one may
+// read a product after 2, here 8.
+//
+// Not for more than 128 dims, whose sums, scores and keys leave it no registers: with it the kernel keeps 280 to 290 bytes a lane in
+// memory, without it 170 to 180.  One such build gave wrong float16 results: the compiler had saved registers (a row's number, token
+// and head) where a branch had lanes off, so that rows were written to other places.  The sums were right.
+// tests/test_assembly_cpu.py looks for such saves in every kernel.
 template <int kBlocks>
 __device__ __forceinline__ void scale_if(bool moves, float shrink, f32x16 (&out)[kBlocks]) {
-    if constexpr (kBlocks > 4) {  // these are in accumulation registers, which no vector instruction takes
+    if constexpr (kBlocks > 4) {
         if (moves) {
 #pragma unroll
             for (int b = 0; b < kBlocks; ++b) out[b] *= shrink;
