@@ -330,7 +330,8 @@ def paged_step_layout_native(page_table: torch.Tensor, slots: torch.Tensor, posi
 
     Request i has ``counts[i]`` (default one) tokens from ``positions[i]`` on of ``slots[i]``, as ``paged_cache_reserve``
     gave them; refused ones (position -1) have none.  ``tokens`` is the step's fixed size: entries behind the last token
-    are -1, and tokens that do not fit are left out.  A token beyond the table's columns or on no page has the row -1.
+    are -1, and tokens that do not fit are left out (``paged_chunk_attention`` then needs ``positions``: a request that was
+    cut no longer ends with its sequence's last token).  A token beyond the table's columns or on no page has the row -1.
     """
     _ready("paged step")
     return _OPS.paged_step_layout(page_table, slots, positions, counts, page_size, tokens)
@@ -356,6 +357,9 @@ def paged_chunk_attention_native(query: torch.Tensor, key_pages: torch.Tensor, v
     and ``lengths``; its first token is at ``positions[i]`` (default: its tokens are the sequence's last).  A token sees the
     keys up to its own, with ``window`` > 0 the last ``window`` of them and the first ``sinks``.  Keys on an entry outside
     the pool are left out; tokens that see nothing, or of no request, give zeros.  ``offsets`` must not decrease.
+    16-bit weights are rounded once to the type for their product with the values, as in ``window_attention`` and also
+    for a single token, whose weights ``paged_decode_attention`` holds in two terms.  A call takes a workspace of up to
+    138 MB at 128 dims (273 MB at 256, float32 54 MB), because the host does not know the lengths.
     """
     _ready("paged step")
     return _OPS.paged_chunk_attention(query, key_pages, value_pages, page_table, lengths, offsets, scale, window, sinks,

@@ -483,7 +483,9 @@ int flux_paged_decode_attention(int dtype, const void* query, const void* key_pa
  * row r = slots[i] (i when slots is NULL) of page_table and lengths, as above.  Its first token is at positions[i]
  * (NULL: lengths[r] less its tokens), the others behind it; a token at p sees the keys j <= p, j < lengths[r] with
  * j > p - window or j < sinks (window 0: all).  Keys on a page outside [0, pages) are left out and never read.  A token
- * that sees nothing, nothing whose score is above -inf, with p outside [0, lengths[r]), or of no request gives zeros.
+ * that sees nothing, nothing whose score is above -inf, with p outside [0, lengths[r]), or of no request gives zeros.  As in
+ * flux_window_attention 16-bit weights are rounded once to the type for their product with the values, also a single token's
+ * (flux_paged_decode_attention holds them in two terms); statistics and sums are float32.
  * Strides: query's token, head, dim; pages' page, head, row.  output contiguous.  At most 2^24 tokens, 65535 requests and query
  * heads, 2^27 rows of a KV head (tokens times its query heads), 2^28 pages; the rows' tiles (128 rows, float32's 32 or 16) and
  * about 1024 parts are below 2^24 over all KV heads.  The workspace's size depends on shapes alone, because lengths are on the device:
@@ -622,8 +624,9 @@ int flux_logits_process(int dtype, const void* logits, int64_t logits_stride, vo
  * tokens[row]: the first one kept, by index, at which the kept weights reached exceed u times all of them (u <= 0 or NaN: the
  * first of any weight, u >= 1: the last); probabilities[row]: its share of them.  A row whose temperature is not above 0 or whose
  * largest logit is not finite gives the lowest index of the largest logit (NaN above all numbers) and 1.  Vectors [rows];
- * NULL: temperature 1, no filter.  At most 2^20 rows, 2^24 tokens each, rows * (vocab + 1023) at most 2^32.  Weights are held in integers of 2^-b, b = min(51, 62 - ceil(log2 vocab)): results
- * do not depend on scheduling.  The workspace is aligned to 16 bytes. */
+ * NULL: temperature 1, no filter.  At most 2^20 rows, 2^24 tokens each, rows * (vocab + 1023) at most 2^32.  Weights are held in
+ * integers of 2^-b, b = min(51, 62 - ceil(log2 vocab)): results do not depend on scheduling, and borders between tokens move by at
+ * most vocab 2^-(b + 1) of the mass.  The workspace is aligned to 16 bytes. */
 int flux_logits_sample_workspace_bytes(int64_t rows, int64_t vocab, int64_t* bytes);
 int flux_logits_sample(int dtype, const void* logits, int64_t logits_stride, const float* uniforms, const float* temperature,
                        const int64_t* top_k, const float* top_p, const float* min_p, int64_t* tokens, float* probabilities,

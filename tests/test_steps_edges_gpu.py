@@ -9,7 +9,7 @@ import torch
 
 from flux_amd import ops
 from oracle import steps
-from tests.test_steps_gpu import TYPES, _bound, _chunk_case, _close, _to
+from tests.test_steps_gpu import TYPES, _bound, _check_chunk, _check_sample, _chunk_case, _close, _to
 
 pytestmark = pytest.mark.gpu
 
@@ -115,3 +115,26 @@ def test_sampling_no_rows_gives_nothing(gpu_device, vocab):
     tokens, probabilities = ops.logits_sample_native(torch.empty(0, vocab, device=gpu_device), torch.empty(0, device=gpu_device),
                                                      top_k=torch.empty(0, dtype=torch.int64, device=gpu_device), **options)
     assert tokens.shape == probabilities.shape == (0,) and tokens.dtype == torch.int64 and probabilities.dtype == torch.float32
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("top_p,top_k", [(0.9, 0), (0.97, 90000), (1.0, 60000)])
+def test_sampling_flat_rows(gpu_device, dtype, top_p, top_k):
+    """More than 1024 tokens lie where the filters end, few of them equal: rows that one workgroup takes."""
+    g = torch.Generator().manual_seed(31)
+    logits = torch.randn(3, 152000, generator=g).to(dtype)
+    options = {"uniforms": torch.rand(3, generator=g), "temperature": torch.tensor([1.0, 2.0, 0.9]), "top_p": torch.full((3,), top_p),
+               "top_k": torch.tensor([top_k, top_k, 0]), "min_p": torch.tensor([0.0, 0.0, 1e-3])}
+    _check_sample(logits, gpu_device, **options)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_a_layout_that_cuts_a_request_needs_its_positions(gpu_device, dtype):
+    case = _chunk_case(41, dtype, 4, 2, 64, 16, [(5, 30), (40, 500), (3, 3)])
+    slots, positions, counts = torch.arange(3), torch.tensor([30, 500, 3]), torch.tensor([5, 40, 3])
+    offsets, *_ = ops.paged_step_layout_native(case["page_table"].to(gpu_device), *(t.to(gpu_device) for t in (slots, positions, counts)), 16, 33)
+    assert offsets.tolist() == [0, 5, 33, 33]
+    cut = {**case, "query": case["query"][:33].contiguous(), "offsets": offsets.cpu()}
+    _check_chunk(cut, gpu_device, positions=positions)
+    whole = steps.chunk_attention(**case)[:33]
+    assert torch.equal(steps.chunk_attention(**cut, positions=positions), whole)
