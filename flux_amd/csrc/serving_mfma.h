@@ -290,8 +290,6 @@ struct Wide<__bf16> {
     static __device__ __forceinline__ uint32_t round(float a, float b) {
         return __builtin_bit_cast(uint32_t, __builtin_convertvector((f32x2{a, b}), Pair));
     }
-    static __device__ __forceinline__ float low(uint32_t pair) { return __uint_as_float(pair << 16); }
-    static __device__ __forceinline__ float high(uint32_t pair) { return __uint_as_float(pair & 0xffff0000u); }
     static __device__ __forceinline__ f32x16 multiply(u32x4 a, u32x4 b, f32x16 c) {
         return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c,
                                                        0, 0, 0);
@@ -307,8 +305,6 @@ struct Wide<_Float16> {
     static __device__ __forceinline__ uint32_t round(float a, float b) {
         return __builtin_bit_cast(uint32_t, __builtin_convertvector((f32x2{a, b}), Pair));
     }
-    static __device__ __forceinline__ float low(uint32_t pair) { return static_cast<float>(__builtin_bit_cast(Pair, pair)[0]); }
-    static __device__ __forceinline__ float high(uint32_t pair) { return static_cast<float>(__builtin_bit_cast(Pair, pair)[1]); }
     static __device__ __forceinline__ f32x16 multiply(u32x4 a, u32x4 b, f32x16 c) {
         return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0,
                                                       0, 0);
