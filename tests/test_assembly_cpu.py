@@ -2,8 +2,9 @@
 
 Where a branch takes some lanes, its end is a label and the restoring of the lanes (``s_or_b64 exec, exec, ..``).  The compiler
 may put a register that it has to save to memory between the two: then only the branch's lanes are saved, and the others read
-back what lay there.  Found in a kernel for heads of 256 in float16, whose rows all took their first lane's place: of the sums and
-addresses that it held 284 bytes a lane were in memory.  No source asks for such a save, so that only the result can be looked at.
+back what lay there.  Two builds had it, both with more to hold than registers (284 bytes a lane in memory in one): a row's number
+and place were saved, and results were written to other rows.  No source asks for such a save, so that only the result can be
+looked at.
 """
 
 from __future__ import annotations
