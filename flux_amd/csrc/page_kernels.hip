@@ -536,7 +536,7 @@ constexpr int kWriteTokens = 16;
 
 // Two forms of the arguments: a padded batch whose places are looked up, and packed tokens whose rows of the pool are given (row
 // r is row r % page of page r / page).  16384 packed tokens of 8 heads of 128 in 16 bits take 24 us, 5.7 TB/s read and written (partly
-// out of the memory-side cache); 16 tokens 4.6.  Both forms in one kernel, because a loop that two of them call takes 81 registers
+// out of the memory-side cache); 16 tokens 3.9.  Both forms in one kernel, because a loop that two of them call takes 81 registers
 // instead of 67, five waves instead of seven (16 prompts to 1000 tokens 9.7 us against 8.6).
 template <class Unit, class Args>
 __global__ void __launch_bounds__(256) page_write_kernel(PagePool p, Args a) {
